@@ -6,8 +6,8 @@ A case is a dict of plain values; ``kind`` names the public entry point it goes 
   128. Serving cases hold a weight that was quantised once, training cases a bf16 or fp32 weight that is
   quantised in the call, and return the gradients too.
 * ``experts``  ``scattermoe.mlp.GLUMLP.quantize_fp8()``: the SwiGLU experts' products in e4m3 on given routing.
-* ``grouped``  ``scattermoe.parallel_experts.parallel_linear(..., fp8=True)``: one grouped product with routing
-  weights, forward and backward.
+* ``grouped``  ``scattermoe.parallel_experts.parallel_linear(..., fp8=True)``: one grouped product, forward and
+  backward, as an expert MLP's first: tokens' rows gathered, output rows sorted by expert.
 * ``norm``     ``zmoe.functional.norm_residual``: the norm after a block, its gate, the scaled residual and the next
   block's norm.
 
@@ -175,8 +175,8 @@ def _inputs(case, seed):
     if kind == "grouped":
         K, N, E = case["K"], case["N"], case["E"]
         t = {"x": _activations(normal, T, K), "W": normal(E, N, K, std=K ** -0.5, dtype=_BF16),
-             "dout": normal(T, N, dtype=_BF16)}
-        t["idx"], t["p"] = _routing(case, g)
+             "dout": normal(T * case["k"], N, dtype=_BF16)}
+        t["idx"], _ = _routing(case, g)
         return t
     d = case["d"]
     stream = _F32 if case["stream"] == "f32" else _BF16
@@ -224,7 +224,7 @@ def prepare(case, seed):
             t["W1"] = _dequantized_blocks(t["W1"].view(2 * E, f, d)).view(E, 2 * f, d)
             t["W2"] = _dequantized_blocks(t["W2"])
     if case.get("train", case["kind"] == "grouped") and own:
-        for n in ("x", "W", "p", "r", "y", "w1", "w2", "gate", "scale"):
+        for n in ("x", "W", "r", "y", "w1", "w2", "gate", "scale"):
             if n in t:
                 t[n].requires_grad_(True)
     s.update(t)
@@ -255,12 +255,11 @@ def _run_own(s):
     if kind == "grouped":
         from scattermoe.parallel_experts import flatten_sort_count, parallel_linear
 
-        for n in ("x", "W", "p"):
-            s[n].grad = None
+        s["x"].grad = s["W"].grad = None
         se, ss, off = flatten_sort_count(s["idx"], case["E"])
-        out = parallel_linear(s["x"], s["W"].permute(0, 2, 1), case["k"], se, ss, off, gates=s["p"], fp8=True)
+        out = parallel_linear(s["x"], s["W"].permute(0, 2, 1), case["k"], se, ss, off, grouped_out=True, fp8=True)
         out.backward(s["dout"])
-        return {"out": out.detach(), "d x": s["x"].grad, "d W": s["W"].grad, "d p": s["p"].grad}
+        return {"out": out.detach(), "d x": s["x"].grad, "d W": s["W"].grad}
     from zmoe.functional import norm_residual
 
     leaves = [n for n in ("r", "y", "w1", "w2", "gate", "scale") if n in s]
@@ -333,10 +332,9 @@ def _run_plain(s):
     if kind in ("experts", "grouped"):
         T, k = s["idx"].shape
         x = _quantized_rows(s["x"])
-        p = s["p"].reshape(-1)
         slots = _by_expert(s["idx"], case["E"])
     if kind == "experts":
-        f = case["f"]
+        f, p = case["f"], s["p"].reshape(-1)
         Y = torch.empty(T * k, case["d"], device=x.device)
         for e, sl in enumerate(slots):
             if sl.numel():
@@ -346,19 +344,19 @@ def _run_plain(s):
         return {"out": (Y * p.unsqueeze(1)).view(T, k, -1).sum(1).to(_BF16)}
     if kind == "grouped":
         W = _dequantized_blocks(s["W"])
-        G = s["dout"].to(_F32).repeat_interleave(k, 0) * p.unsqueeze(1)
-        Gq = _quantized_rows(G)
-        Y, dX = torch.empty_like(G), torch.empty(T * k, case["K"], device=x.device)
+        dout = s["dout"].to(_F32)
+        dq, xf = _quantized_rows(s["dout"]), s["x"].to(_F32)
+        out, dX = torch.empty_like(dout), torch.empty(T * k, case["K"], device=x.device)
         dW = torch.zeros_like(W)
-        xf = s["x"].to(_F32)
+        at = 0
         for e, sl in enumerate(slots):
             if sl.numel():
-                Y[sl] = x[sl // k] @ W[e].T
-                dX[sl] = Gq[sl] @ W[e]
-                dW[e] = G[sl].T @ xf[sl // k]
-        dp = (Y.view(T, k, -1) * s["dout"].to(_F32).unsqueeze(1)).sum(-1)
-        return {"out": (Y * p.unsqueeze(1)).view(T, k, -1).sum(1).to(_BF16),
-                "d x": dX.view(T, k, -1).sum(1).to(_BF16), "d W": dW.to(_BF16), "d p": dp}
+                rows = slice(at, at + sl.numel())
+                out[rows] = x[sl // k] @ W[e].T
+                dX[sl] = dq[rows] @ W[e]
+                dW[e] = dout[rows].T @ xf[sl // k]
+                at += sl.numel()
+        return {"out": out.to(_BF16), "d x": dX.view(T, k, -1).sum(1).to(_BF16), "d W": dW.to(_BF16)}
     return _norm_plain(s)
 
 
@@ -420,7 +418,7 @@ def work(case):
         return {"bytes": int(touched * 3 * d * f + 4 * T * d + 12 * R), "flops": 6 * R * d * f}
     if kind == "grouped":
         K, N, E, R = case["K"], case["N"], case["E"], T * case["k"]
-        return {"bytes": 4 * T * K + 4 * E * K * N + 4 * T * N + 16 * R, "flops": 6 * R * K * N}
+        return {"bytes": 4 * T * K + 4 * E * K * N + 4 * R * N + 16 * R, "flops": 6 * R * K * N}
     d = case["d"]
     st = 4 if case["stream"] == "f32" else 2
     full = 2 if case["gate"] == "full" else 0
@@ -493,9 +491,8 @@ def exact(case, seed):
         return _norm64(case, t)
     T, k = t["idx"].shape
     x = _rows64(t["x"])
-    p = t["p"].to(_F64)
     if kind == "experts":
-        f = case["f"]
+        f, p = case["f"], t["p"].to(_F64)
         out = torch.zeros(T, case["d"], dtype=_F64, device=x.device)
         for e in range(case["E"]):
             rows, j = (t["idx"] == e).nonzero(as_tuple=True)
@@ -505,22 +502,20 @@ def exact(case, seed):
                 out.index_add_(0, rows, (_rows64(torch.sigmoid(gt) * gt * up) @ _weight64(t["W2"][e]).T)
                                * p[rows, j, None])
         return {"out": out}
-    out = torch.zeros(T, case["N"], dtype=_F64, device=x.device)
     dx = torch.zeros(T, case["K"], dtype=_F64, device=x.device)
     dW = torch.zeros(t["W"].shape, dtype=_F64, device=x.device)
-    dp = torch.zeros(T, k, dtype=_F64, device=x.device)
-    dout = t["dout"].to(_F64)
+    dout, dq = t["dout"].to(_F64), _rows64(t["dout"])
+    out, at = torch.zeros_like(dout), 0
     for e in range(case["E"]):
-        rows, j = (t["idx"] == e).nonzero(as_tuple=True)
+        rows = (t["idx"] == e).nonzero(as_tuple=True)[0]  # in token order, as the sort leaves them
+        end = at + rows.numel()
         if rows.numel():
-            W, g = _weight64(t["W"][e]), p[rows, j, None]
-            Y = x[rows] @ W.T
-            out.index_add_(0, rows, g * Y)
-            dp[rows, j] = (Y * dout[rows]).sum(-1)
-            # (the product of two 32-bit values, as it is quantised: rounded to 32 bits)
-            dx.index_add_(0, rows, _rows64((g * dout[rows]).to(_F32)) @ W)
-            dW[e] = (g * dout[rows]).T @ t["x"][rows].to(_F64)
-    return {"out": out, "d x": dx, "d W": dW, "d p": dp}
+            W = _weight64(t["W"][e])
+            out[at:end] = x[rows] @ W.T
+            dx.index_add_(0, rows, dq[at:end] @ W)
+            dW[e] = dout[at:end].T @ t["x"][rows].to(_F64)
+        at = end
+    return {"out": out, "d x": dx, "d W": dW}
 
 
 def _norm64(case, t):
