@@ -1,0 +1,758 @@
+// Products in 8-bit floating point (OCP e4m3) with a power-of-two scale for each block of 128, dense
+// and grouped by expert, the quantisers in front of them and the SwiGLU between two of them.
+//
+// A block of values v (1 x 128 along an activation row, 128 x 128 of a weight; the last one of a row or
+// column is shorter) is held as q s with a = max |v| over its finite values,
+//   s = 2^c, c the least whole number >= -127 with a <= 448 s,   q = e4m3(v / s), nearest even,
+// 448 being e4m3's largest value; inf and NaN become e4m3's NaN. s is stored as the E8M0 byte c + 127.
+// v / s is exact in f32 (short of f32's own underflow, where e4m3 has 0 anyway), so a block has one
+// quantised form. gfx950's scaled MFMA (v_mfma_scale_f32_16x16x128_f8f6f4) takes E8M0 bytes as an
+// operand: both scales of a product are applied inside the matrix unit, at no cost in vector
+// instructions, and sums run on through the whole depth in its f32 accumulators. (An arbitrary f32
+// scale would cost a vector FMA for every output and 128 of depth.)
+#include <type_traits>
+#include <utility>
+
+#include "zmoe_tiles.h"
+
+namespace zmoe {
+namespace {
+
+constexpr int kBlk = 128;  // values of one scale along the depth, and bytes of an LDS row
+constexpr uint32_t kNaN8 = 0x7f;
+
+typedef int v8i32_t __attribute__((ext_vector_type(8)));
+
+__host__ __device__ inline int64_t blocks_of(int64_t n) { return (n + kBlk - 1) / kBlk; }
+// Bytes of one row of scales: a whole number of dwords.
+__host__ __device__ inline int64_t scale_pitch(int64_t K) { return (blocks_of(K) + 3) / 4 * 4; }
+
+// E8M0 byte of the least power of two s >= 2^-127 with a <= 448 s (448 = 1.75 * 2^8), a finite, >= 0.
+__device__ __forceinline__ int scale_code(float a) {
+  const int bits = __float_as_int(a);
+  const int c = (bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+  return c > 0 ? c : 0;
+}
+// 2^-c of that byte (code <= 247: the exponent field stays normal).
+__device__ __forceinline__ float scale_inverse(int code) { return __int_as_float((254 - code) << 23); }
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
+__device__ __forceinline__ float finite_abs(float v) { return finite(v) ? fabsf(v) : 0.f; }
+
+// Four values, already divided by their scale, to e4m3 bytes. Non-finite ones become NaN (the
+// conversion itself would depend on the wave's overflow mode).
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  return (uint32_t)w;
+}
+__device__ __forceinline__ uint32_t quantize4(const float (&v)[4], float inv) {
+  uint32_t w = pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (!finite(v[u])) w = (w & ~(0xffu << (8 * u))) | (kNaN8 << (8 * u));
+  return w;
+}
+
+// Largest of v over 16 consecutive lanes, in every one of them.
+__device__ __forceinline__ float max16(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0xB1>{}));   // lane ^ 1
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x4E>{}));   // lane ^ 2
+  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x141>{}));  // 7 - lane within 8
+  return fmaxf(v, dpp(v, std::integral_constant<int, 0x140>{}));  // 15 - lane within 16
+}
+
+// Eight elements from column c of a row (zeros past K): 16-byte loads where the row allows them.
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int64_t K, bool vec, float (&v)[8]) {
+  constexpr int VN = 16 / sizeof(T);
+  if (vec && c + 8 <= K) {
+#pragma unroll
+    for (int q = 0; q < 8 / VN; ++q) unpack_chunk(*reinterpret_cast<const uint4*>(row + c + q * VN), &v[q * VN], T{});
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = c + u < K ? to_f32(row[c + u]) : 0.f;
+  }
+}
+
+// ------------------------------------------------------------------ activations
+// Sixteen lanes hold one block of 128 of a row, eight values each: one load of 16 (bf16) or 32 bytes,
+// the largest magnitude by four lane exchanges, 8 bytes written by each lane. Bound by HBM (2 or 4
+// bytes read, 1 written). Optionally row i is X[rows[i] / row_div] times row_scale[rows[i]] (the grouped,
+// routing-weighted rows of an output gradient, never written anywhere in 16 bits).
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ X, int64_t ldx, int64_t x_rows,
+                                                            const int64_t* __restrict__ rows, int row_div,
+                                                            const float* __restrict__ row_scale, uint32_t total,
+                                                            int64_t K, int nb, int vec, uint8_t* __restrict__ Q,
+                                                            uint8_t* __restrict__ S, int64_t pitch) {
+  const uint32_t g = blockIdx.x * 16 + threadIdx.x / 16;  // (row, block)
+  if (g >= total) return;  // whole groups of 16 lanes
+  const uint32_t i = g / (uint32_t)nb, b = g % (uint32_t)nb;
+  const int lane = threadIdx.x & 15;
+  int64_t src = i;
+  float sc = 1.f;
+  if (rows != nullptr) {
+    const int64_t slot = rows[i];
+    src = slot < 0 ? -1 : slot / row_div;
+    if (src >= x_rows) src = -1;
+    if (src < 0) sc = 0.f;  // an index out of range: a row of zeros
+    else if (row_scale != nullptr) sc = row_scale[slot];
+  } else if (row_scale != nullptr) {
+    sc = row_scale[i];
+  }
+  const int64_t c = (int64_t)b * kBlk + lane * 8;
+  float v[8];
+  load8(X + (src < 0 ? 0 : src) * ldx, c, src < 0 ? 0 : K, vec != 0, v);
+  float a = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    if (row_scale != nullptr) v[u] *= sc;
+    a = fmaxf(a, finite_abs(v[u]));
+  }
+  const int code = scale_code(max16(a));
+  const float inv = scale_inverse(code);
+  const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+  *reinterpret_cast<uint2*>(Q + (int64_t)i * nb * kBlk + c) = make_uint2(quantize4(lo, inv), quantize4(hi, inv));
+  if (lane == 0) S[(int64_t)i * pitch + b] = (uint8_t)code;
+}
+
+// ------------------------------------------------------------------ weights
+// One workgroup per 128 x 128 block: eight rows a thread, the block's largest magnitude through LDS.
+// With Qt the block is also written transposed (through LDS): W^T's blocks are W's, so one scale
+// serves both, and the input gradient's product reads rows of W^T with the depth contiguous.
+template <typename T, bool TRANS>
+__global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restrict__ W, int64_t se, int64_t sn,
+                                                              int64_t N, int64_t K, int vec, uint8_t* __restrict__ Q,
+                                                              uint8_t* __restrict__ S, uint8_t* __restrict__ Qt,
+                                                              uint8_t* __restrict__ St) {
+  __shared__ float red[4];
+  constexpr int TP = kBlk + 16;  // pitch of the transposed block, rows still 16-byte aligned
+  __shared__ __align__(16) uint8_t tile[TRANS ? kBlk * TP : 16];
+  const int64_t kb = blockIdx.x, nb = blockIdx.y, e = blockIdx.z;
+  const int t = threadIdx.x, row0 = t >> 4, col = (t & 15) * 8;
+  float v[8][8];
+  float a = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t n = nb * kBlk + row0 + 16 * j;
+    load8(W + e * se + (n < N ? n : 0) * sn, kb * kBlk + col, n < N ? K : 0, vec != 0, v[j]);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) a = fmaxf(a, finite_abs(v[j][u]));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+  if ((t & 63) == 0) red[t >> 6] = a;
+  __syncthreads();
+  const int code = scale_code(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  const float inv = scale_inverse(code);
+  const int64_t nbs = blocks_of(N), kbs = blocks_of(K);
+  if (t == 0) {
+    S[(e * nbs + nb) * scale_pitch(K) + kb] = (uint8_t)code;
+    if (TRANS) St[(e * kbs + kb) * scale_pitch(N) + nb] = (uint8_t)code;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t n = nb * kBlk + row0 + 16 * j;
+    const float lo[4] = {v[j][0], v[j][1], v[j][2], v[j][3]}, hi[4] = {v[j][4], v[j][5], v[j][6], v[j][7]};
+    const uint2 w = make_uint2(quantize4(lo, inv), quantize4(hi, inv));
+    if (n < N) *reinterpret_cast<uint2*>(Q + ((e * N + n) * kbs + kb) * kBlk + col) = w;
+    if constexpr (TRANS) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) tile[(col + u) * TP + row0 + 16 * j] = (uint8_t)((u < 4 ? w.x : w.y) >> (8 * (u & 3)));
+    }
+  }
+  if constexpr (TRANS) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int kr = (t >> 3) + 32 * q, ch = (t & 7) * 16;
+      const int64_t k = kb * kBlk + kr;
+      if (k < K)
+        *reinterpret_cast<uint4*>(Qt + ((e * K + k) * nbs + nb) * kBlk + ch) =
+            *reinterpret_cast<const uint4*>(tile + kr * TP + ch);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ products
+// C[i, :] = A(i, :) B_e^T for the sorted rows i of expert e (or all rows of one weight), A rows and
+// B rows of K / 128 blocks, one 128-byte line each. A stage is one block of the depth: BM + BN lines in
+// LDS (the geometry of 64 bf16 elements), one 16 x 16 x 128 MFMA per 16 x 16 outputs. The weight rows
+// are the MFMA's first operand, so a lane ends up with 4 consecutive output columns of one row.
+enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2 };
+
+struct Fp8Params {
+  const uint8_t* a;
+  const uint8_t* as;
+  int64_t lda, a_pitch;    // bytes between rows of A and of its scales
+  const int64_t* a_rows;   // A row of sorted row i = a_rows[i] / a_div (null: i)
+  int a_div;
+  int64_t a_bytes;         // bytes of A
+  const uint8_t* b;
+  const uint8_t* bs;
+  int64_t b_estride, bs_estride, bs_pitch;
+  uint32_t b_bytes;        // bytes of one expert's weights
+  void* c;
+  int64_t ldc;             // elements (GLU: bytes of a row of Aq)
+  const int64_t* c_rows;   // output row of sorted row i = c_rows[i] (null: i)
+  uint8_t* cs;             // GLU: the activations' scales
+  int64_t cs_pitch;
+  int vec_c;               // rows of C take 16-byte stores
+  const int64_t* offsets;  // inclusive expert ends [E] (null: one weight, ns_m rows)
+  int nk, N, E, n_tiles, n_major;
+  int half;                // GLU: pairs f
+  int ns_m;                // rows of a dense launch (0: grouped)
+  static constexpr int ns_sym = 0;
+};
+
+template <int BM, int BN, int NW>
+struct Grid8 {
+  static constexpr int GN = BN / 64, GM = NW / GN;
+  static constexpr int WM = BM / GM, MF = WM / 16, NF = 4;
+  static_assert(GM * GN == NW && WM % 16 == 0, "waves of 64 columns");
+};
+
+constexpr int kScaleStages = 64;  // stages whose scales are in LDS at once
+
+template <int BM, int BN, int NW, int NS>
+struct Lds8 {
+  static constexpr int kStage = (BM + BN) * kBlk;
+  static constexpr int kPitch = 64 * 2 + 16;  // staged output rows, bf16
+  static constexpr int stages = NS * kStage;
+  static constexpr int glu = BM * kBlk + 4 * BM * 4;  // quantised tile, row maxima of four waves
+  static constexpr int staging = NW * 32 * kPitch;
+  static constexpr int ops = stages > glu ? (stages > staging ? stages : staging) : (glu > staging ? glu : staging);
+  static constexpr int a_scales = ops;
+  static constexpr int b_scales = a_scales + kScaleStages * BM;
+  static constexpr int src = b_scales + kScaleStages * 2;
+  static constexpr int dst = src + BM * 4;
+  static constexpr int total = dst + BM * 4;
+  static constexpr int decode = (kGemmMaxE + 4 + 16) * 4;
+  static_assert(total <= 163840 && decode <= ops, "LDS of one CU");
+};
+
+template <int OFF>
+__device__ __forceinline__ v4i32_t ds_read128(uint32_t addr) {
+  v4i32_t v;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(OFF));
+  return v;
+}
+// MF scale bytes of this lane's rows (one per 16-row fragment), from `addr`
+template <int MF>
+struct AScale {
+  uint32_t w[(MF + 3) / 4];
+  __device__ __forceinline__ void read(uint32_t addr) {
+    if constexpr (MF == 8) {
+      v2i32_t v;
+      asm volatile("ds_read_b64 %0, %1" : "=v"(v) : "v"(addr));
+      w[0] = (uint32_t)v[0];
+      w[1] = (uint32_t)v[1];
+    } else if constexpr (MF == 4) {
+      asm volatile("ds_read_b32 %0, %1" : "=v"(w[0]) : "v"(addr));
+    } else if constexpr (MF == 2) {
+      asm volatile("ds_read_u16 %0, %1" : "=v"(w[0]) : "v"(addr));
+    } else {
+      static_assert(MF == 1, "1, 2, 4 or 8 fragments");
+      asm volatile("ds_read_u8 %0, %1" : "=v"(w[0]) : "v"(addr));
+    }
+  }
+  __device__ __forceinline__ void tie() {
+    asm volatile("" : "+v"(w[0]));
+    if constexpr (MF == 8) asm volatile("" : "+v"(w[1]));
+  }
+};
+
+// 32 bytes of a fragment row: lane (r = lane % 16, g = lane / 16) holds chunks g and g + 4 of row r.
+// Both operands use this order, so which depths the instruction takes them for does not matter.
+struct Frag8 {
+  v4i32_t lo, hi;
+  __device__ __forceinline__ v8i32_t value() const { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+  __device__ __forceinline__ void tie() {
+    asm_tie(lo);
+    asm_tie(hi);
+  }
+};
+
+template <int... I, typename F>
+__device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled(std::make_integer_sequence<int, N>{}, f);
+}
+
+__device__ __forceinline__ int swizzle8(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+// The lines this wave loads of each stage's operand: 8 rows an instruction (1 KB of LDS), lane i the
+// chunk (i % 8) ^ swizzle(row) of row i / 8.
+template <int ROWS, int NW>
+struct Lines8 {
+  static constexpr int NQ = ROWS / (8 * NW);
+  static_assert(NQ >= 1 && NQ * 8 * NW == ROWS, "whole instructions for every wave");
+  uint32_t off[NQ];
+  __device__ __forceinline__ static int row_of(int q) {
+    return 8 * ((int)(threadIdx.x >> 6) * NQ + q) + (int)((threadIdx.x & 63) >> 3);
+  }
+  __device__ __forceinline__ void set(int q, uint32_t row_off) {
+    const int c = (int)(threadIdx.x & 7) ^ swizzle8(row_of(q));
+    off[q] = row_off == kOOB ? kOOB : row_off + 16u * (uint32_t)c;
+  }
+};
+
+template <int BM, int BN, int NW, int NS, int EPI>
+__global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
+  extern __shared__ __align__(128) char smem[];
+  using G = Grid8<BM, BN, NW>;
+  using L = Lds8<BM, BN, NW, NS>;
+  constexpr int MF = G::MF, NF = G::NF;
+  constexpr int NT = NW * 64;
+  static_assert(EPI != F8_GLU || BN == 256, "one block of 128 pairs a tile");
+
+  RowsTile tile;
+  if (!decode_rows_tile<BM, NT>(p, smem, tile)) return;  // uniform per workgroup
+  const int e = __builtin_amdgcn_readfirstlane(tile.e);
+  const int nt = __builtin_amdgcn_readfirstlane(tile.nt);
+  const int rows = tile.rows;
+  const int64_t row0 = tile.row0;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = (int)threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int gm = wave / G::GN, gn = wave % G::GN;
+  lds_char* lds = (lds_char*)(smem);
+
+  // source and output row of each tile row (row numbers < 2^31: the low words of the int64 entries)
+  int* src_table = reinterpret_cast<int*>(smem + L::src);
+  int* dst_table = reinterpret_cast<int*>(smem + L::dst);
+  for (int rl = (int)threadIdx.x; rl < BM; rl += NT) {
+    const int64_t i = row0 + (rl < rows ? rl : 0);
+    src_table[rl] = p.a_rows ? reinterpret_cast<const int*>(p.a_rows)[2 * i] / p.a_div : rl;
+    dst_table[rl] = p.c_rows ? reinterpret_cast<const int*>(p.c_rows)[2 * i] : rl;
+  }
+  __syncthreads();
+
+  // A from its first row (gathered) or from this tile's (contiguous rows: no limit on their number)
+  const char* a_base = reinterpret_cast<const char*>(p.a) + (p.a_rows ? 0 : row0 * p.lda);
+  const int64_t a_left = p.a_bytes - (p.a_rows ? 0 : row0 * p.lda);
+  const uint32_t a_bytes = a_left < 0x7fff0000 ? (uint32_t)a_left : 0x7fff0000u;
+  const uint8_t* as_base = p.as + (p.a_rows ? 0 : row0 * p.a_pitch);
+  const char* b_base = reinterpret_cast<const char*>(p.b) + (int64_t)e * p.b_estride;
+
+  Lines8<BM, NW> la;
+  Lines8<BN, NW> lb;
+  constexpr int NQA = Lines8<BM, NW>::NQ, NQB = Lines8<BN, NW>::NQ, LPS = NQA + NQB;
+#pragma unroll
+  for (int q = 0; q < NQA; ++q) {
+    const int rl = la.row_of(q);
+    la.set(q, rl < rows ? (uint32_t)((int64_t)src_table[rl] * p.lda) : kOOB);
+  }
+#pragma unroll
+  for (int q = 0; q < NQB; ++q) {
+    const int rl = lb.row_of(q);
+    int n;
+    bool ok;
+    if constexpr (EPI == F8_GLU) {  // 64-row pair blocks [up 32 | gate 32] of the tile's 128 pairs
+      const int jj = nt * kBlk + (rl >> 6) * 32 + (rl & 31);
+      ok = jj < p.half;
+      n = (rl & 32) ? p.half + jj : jj;
+    } else {
+      n = nt * BN + rl;
+      ok = n < p.N;
+    }
+    lb.set(q, ok ? (uint32_t)((int64_t)n * ((int64_t)p.nk * kBlk)) : kOOB);
+  }
+  auto issue = [&](int buf, int kt, bool on) {
+    const int64_t k0 = (int64_t)kt * kBlk;
+    const int64_t ra = (int64_t)a_bytes - k0, rb = (int64_t)p.b_bytes - k0;
+    const __amdgpu_buffer_rsrc_t rsa = make_rsrc(a_base + k0, on && ra > 0 ? (uint32_t)ra : 0u);
+    const __amdgpu_buffer_rsrc_t rsb = make_rsrc(b_base + k0, on && rb > 0 ? (uint32_t)rb : 0u);
+    lds_char* st = lds + buf * L::kStage;
+#pragma unroll
+    for (int q = 0; q < NQA; ++q) buf_to_lds(rsa, st + (wave * NQA + q) * 1024, la.off[q]);
+#pragma unroll
+    for (int q = 0; q < NQB; ++q) buf_to_lds(rsb, st + BM * kBlk + (wave * NQB + q) * 1024, lb.off[q]);
+  };
+
+  f32x4_t acc[MF][NF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int n = 0; n < NF; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const uint32_t lds0 = lds_addr(lds);
+  const uint32_t frag_off = (uint32_t)(r16 * kBlk + ((g4 ^ swizzle8(r16)) << 4));
+  const uint32_t a_frag = (uint32_t)(gm * G::WM * kBlk) + frag_off;
+  const uint32_t b_frag = (uint32_t)((BM + gn * 64) * kBlk) + frag_off;
+  const uint32_t as_lane = lds0 + L::a_scales + (uint32_t)((gm * 16 + r16) * MF);
+  const uint32_t bs_lane = lds0 + L::b_scales + (EPI == F8_GLU ? 0u : (uint32_t)(gn / 2));
+  uint8_t* a_scales = reinterpret_cast<uint8_t*>(smem + L::a_scales);
+  uint8_t* b_scales = reinterpret_cast<uint8_t*>(smem + L::b_scales);
+
+  for (int c0 = 0; c0 < p.nk; c0 += kScaleStages) {
+    const int nst = p.nk - c0 < kScaleStages ? p.nk - c0 : kScaleStages;
+    // this tile's scales, [stage][rows in fragment order]: row gm WM + 16 m + r at (gm 16 + r) MF + m
+    const int nd = (nst + 3) / 4;
+    for (int idx = (int)threadIdx.x; idx < BM * nd; idx += NT) {
+      const int rl = idx / nd, d4 = idx - rl * nd;
+      uint32_t w = 0x7f7f7f7fu;
+      if (rl < rows)
+        w = *reinterpret_cast<const uint32_t*>(as_base + (int64_t)src_table[rl] * p.a_pitch + c0 + 4 * d4);
+      const int at = ((rl / G::WM) * 16 + (rl & 15)) * MF + (rl % G::WM) / 16;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a_scales[(4 * d4 + u) * BM + at] = (uint8_t)(w >> (8 * u));
+    }
+    for (int idx = (int)threadIdx.x; idx < 2 * nst; idx += NT) {
+      const int j = idx & 1, st = idx >> 1;
+      const uint8_t* bs = p.bs + (int64_t)e * p.bs_estride;
+      const int64_t nb = EPI == F8_GLU ? (j ? blocks_of(p.half) : 0) + nt : (int64_t)nt * (BN / kBlk) + j;
+      const int64_t last = EPI == F8_GLU ? 2 * blocks_of(p.half) - 1 : blocks_of(p.N) - 1;
+      b_scales[2 * st + j] = bs[(nb < last ? nb : last) * p.bs_pitch + c0 + st];
+    }
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) issue(i, c0 + i, i < nst);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+
+    int cur = 0;
+    for (int st = 0; st < nst; ++st) {
+      __builtin_amdgcn_s_waitcnt(vm_wait((NS - 2) * LPS));  // this wave's loads of stage st are in
+      asm volatile("s_barrier" ::: "memory");               // everyone's are, and the buffer before is read
+      issue(cur == 0 ? NS - 1 : cur - 1, c0 + st + NS - 1, st + NS - 1 < nst);
+      const uint32_t base = lds0 + (uint32_t)(cur * L::kStage);
+      AScale<MF> sa;
+      uint32_t sb;
+      sa.read(as_lane + (uint32_t)(st * BM));
+      if constexpr (EPI == F8_GLU) asm volatile("ds_read_u16 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+      else asm volatile("ds_read_u8 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+      Frag8 fb[NF];
+      unrolled<NF>([&](auto n) {
+        fb[n].lo = ds_read128<n * 2048>(base + b_frag);
+        fb[n].hi = ds_read128<n * 2048>((base + b_frag) ^ 64u);
+      });
+      constexpr int HF = MF < 4 ? MF : 4, STEPS = MF / HF;
+      Frag8 fa[2][HF];
+      auto read_a = [&](auto s) {
+        unrolled<HF>([&](auto m) {
+          fa[s & 1][m].lo = ds_read128<(s * HF + m) * 2048>(base + a_frag);
+          fa[s & 1][m].hi = ds_read128<(s * HF + m) * 2048>((base + a_frag) ^ 64u);
+        });
+      };
+      read_a(std::integral_constant<int, 0>{});
+      unrolled<STEPS>([&](auto s) {
+        if constexpr (s + 1 < STEPS) {
+          read_a(std::integral_constant<int, s + 1>{});
+          asm_wait_lgkm<2 * HF>();  // (in order: at most the next step's reads are out)
+        } else {
+          asm_wait_lgkm<0>();
+        }
+        if constexpr (s == 0) {
+          sa.tie();
+          asm volatile("" : "+v"(sb));
+#pragma unroll
+          for (int n = 0; n < NF; ++n) fb[n].tie();
+        }
+#pragma unroll
+        for (int m = 0; m < HF; ++m) fa[s & 1][m].tie();
+        __builtin_amdgcn_sched_barrier(0);
+        unrolled<HF>([&](auto m) {
+          unrolled<NF>([&](auto n) {
+            constexpr int f = s * HF + m;
+            acc[f][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                fb[n].value(), fa[s & 1][m].value(), acc[f][n], 0, 0, EPI == F8_GLU ? n / 2 : 0, (int)sb, f & 3,
+                (int)sa.w[f / 4]);
+          });
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      cur = cur == NS - 1 ? 0 : cur + 1;
+    }
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));  // loads past the end (zeros) are done before LDS is reused
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+
+  // ---- outputs: acc[m][n][u] is row gm WM + 16 m + r, column gn 64 + 16 n + 4 g + u of the tile
+  if constexpr (EPI == F8_STORE_F32) {
+    float* C = static_cast<float*>(p.c);
+    unrolled<MF>([&](auto m) {
+      const int rl = gm * G::WM + 16 * m + r16;
+      if (rl < rows) {
+        float* out = C + (p.c_rows ? 0 : row0 * p.ldc) + (int64_t)dst_table[rl] * p.ldc;
+#pragma unroll
+        for (int n = 0; n < NF; ++n) {
+          const int col = nt * BN + gn * 64 + 16 * n + 4 * g4;
+          if (p.vec_c && col + 4 <= p.N) {
+            *reinterpret_cast<float4*>(out + col) = make_float4(acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]);
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (col + u < p.N) out[col + u] = acc[m][n][u];
+          }
+        }
+      }
+    });
+  } else if constexpr (EPI == F8_STORE_BF16) {
+    // 32 rows at a time through this wave's own staging area, then whole 128-byte lines
+    char* st = smem + wave * 32 * L::kPitch;
+    uint16_t* C = static_cast<uint16_t*>(p.c) + (p.c_rows ? 0 : row0 * p.ldc);
+    constexpr int MS = MF < 2 ? 1 : 2;
+    const int col0 = nt * BN + gn * 64;
+    unrolled<MF / MS>([&](auto s) {
+#pragma unroll
+      for (int h = 0; h < MS; ++h)
+#pragma unroll
+        for (int n = 0; n < NF; ++n) {
+          const f32x4_t v = acc[s * MS + h][n];
+          *reinterpret_cast<uint2*>(st + (16 * h + r16) * L::kPitch + (16 * n + 4 * g4) * 2) =
+              make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int it = 0; it < 16 * MS / 8; ++it) {
+        const int rr = it * 8 + (lane >> 3), ch = lane & 7;
+        const int rl = gm * G::WM + 16 * MS * s + rr, col = col0 + ch * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(st + rr * L::kPitch + ch * 16);
+        if (rl < rows && col < p.N) {
+          uint16_t* out = C + (int64_t)dst_table[rl] * p.ldc + col;
+          if (p.vec_c && col + 8 <= p.N) {
+            *reinterpret_cast<uint4*>(out) = v;
+          } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              if (col + u < p.N) out[u] = (uint16_t)(w[u / 2] >> (16 * (u & 1)));
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    });
+  } else {
+    // a = silu(gate) up from the f32 sums; a row's 128 pairs of this tile are one block: its largest
+    // magnitude over this wave's 32 pairs (four lanes a row), then over the four waves through LDS
+    float* red = reinterpret_cast<float*>(smem + BM * kBlk);  // [4][BM]
+    unrolled<MF>([&](auto m) {
+      float a = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          acc[m][n][u] *= silu_f(acc[m][2 + n][u]);
+          a = fmaxf(a, finite_abs(acc[m][n][u]));
+        }
+      a = fmaxf(a, __shfl_xor(a, 16, 64));
+      a = fmaxf(a, __shfl_xor(a, 32, 64));
+      if (g4 == 0) red[gn * BM + gm * G::WM + 16 * m + r16] = a;
+    });
+    __syncthreads();
+    unrolled<MF>([&](auto m) {
+      const int rl = gm * G::WM + 16 * m + r16;
+      const int code = scale_code(fmaxf(fmaxf(red[rl], red[BM + rl]), fmaxf(red[2 * BM + rl], red[3 * BM + rl])));
+      const float inv = scale_inverse(code);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float v[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
+        *reinterpret_cast<uint32_t*>(smem + rl * kBlk + gn * 32 + 16 * n + 4 * g4) = quantize4(v, inv);
+      }
+      if (gn == 0 && g4 == 0 && rl < rows) p.cs[(row0 + rl) * p.cs_pitch + nt] = (uint8_t)code;
+    });
+    __syncthreads();
+    uint8_t* C = static_cast<uint8_t*>(p.c) + row0 * p.ldc + (int64_t)nt * kBlk;
+    for (int idx = (int)threadIdx.x; idx < rows * 8; idx += NT)
+      *reinterpret_cast<uint4*>(C + (int64_t)(idx >> 3) * p.ldc + (idx & 7) * 16) =
+          *reinterpret_cast<const uint4*>(smem + (idx >> 3) * kBlk + (idx & 7) * 16);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+template <int BM, int BN, int NW, int NS, int EPI>
+int launch8(Fp8Params p, int64_t R, hipStream_t s) {
+  auto kern = fp8_rows_kernel<BM, BN, NW, NS, EPI>;
+  constexpr int lds = Lds8<BM, BN, NW, NS>::total;
+  int rc = prepare(kern, lds);
+  if (rc) return rc;
+  p.n_tiles = (int)(EPI == F8_GLU ? blocks_of(p.half) : cdiv(p.N, BN));
+  const int64_t mt = cdiv(R, BM) + (p.offsets ? (R < p.E ? R : p.E) : 0);
+  const int64_t total = cdiv(mt * p.n_tiles, (int64_t)kXcds * kSlab) * kXcds * kSlab;  // either tile mapping
+  ZMOE_REQUIRE(mt * p.n_tiles < (int64_t)0x7fffff00, ZMOE_ERR_SHAPE, "fp8 product: too many tiles");
+  hipLaunchKernelGGL(kern, dim3((unsigned)total), dim3(NW * 64), lds, s, p);
+  return check_launch("fp8 rows kernel");
+}
+
+template <int EPI>
+int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
+  const int64_t per = R / p.E;
+  if (per <= 32) return launch8<32, 256, 4, 4, EPI>(p, R, s);
+  if (per <= 96) return launch8<64, 256, 4, 3, EPI>(p, R, s);
+  if (per <= 192) return launch8<128, 256, 8, 3, EPI>(p, R, s);
+  return launch8<256, 256, 8, 2, EPI>(p, R, s);
+}
+
+constexpr int64_t kMaxSpan8 = 0x7fff0000LL;  // bytes that a buffer resource addresses
+constexpr int64_t kMaxRows8 = 0x7fffffffLL;
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int quantize_checks(const char* name, int64_t n, int64_t K, int dtype) {
+  ZMOE_REQUIRE(dtype_ok(dtype), ZMOE_ERR_DTYPE, "%s: dtype %d", name, dtype);
+  ZMOE_REQUIRE(n >= 0 && n < kMaxRows8 && K >= 1 && K < (1 << 30), ZMOE_ERR_SHAPE, "%s: bad sizes (%lld x %lld)", name,
+               (long long)n, (long long)K);
+  return ZMOE_OK;
+}
+
+}  // namespace
+}  // namespace zmoe
+
+using namespace zmoe;
+
+extern "C" int64_t zmoe_fp8_scale_pitch(int64_t K) { return K >= 1 ? scale_pitch(K) : 0; }
+
+extern "C" int zmoe_fp8_quantize_rows(const void* X, int64_t x_stride, int64_t x_rows, const int64_t* rows,
+                                      int row_div, const float* row_scale, int64_t n, int64_t K, int dtype, void* Q,
+                                      void* S, void* stream) {
+  int rc = quantize_checks("fp8_quantize_rows", n, K, dtype);
+  if (rc) return rc;
+  ZMOE_REQUIRE(x_rows >= 0 && x_stride >= K && row_div >= 1, ZMOE_ERR_SHAPE,
+               "fp8_quantize_rows: bad row stride, row count or divisor");
+  ZMOE_REQUIRE(rows || n <= x_rows, ZMOE_ERR_SHAPE, "fp8_quantize_rows: more rows than X has");
+  if (n == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(Q && S && (X || x_rows == 0), ZMOE_ERR_NULL, "fp8_quantize_rows: null pointer");
+  ZMOE_REQUIRE(aligned16(Q) && aligned4(S), ZMOE_ERR_ALIGN, "fp8_quantize_rows: Q on 16, S on 4 bytes");
+  const int64_t nb = blocks_of(K);
+  ZMOE_REQUIRE(n * nb < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "fp8_quantize_rows: too many blocks");
+  const int vec = aligned16(X) && x_stride % (16 / dtype_size(dtype)) == 0;
+  const dim3 grid((unsigned)cdiv(n * nb, 16));
+  hipStream_t s = as_stream(stream);
+  uint8_t *q = static_cast<uint8_t*>(Q), *sc = static_cast<uint8_t*>(S);
+  if (dtype == ZMOE_DTYPE_BF16)
+    hipLaunchKernelGGL(quantize_rows_kernel<uint16_t>, grid, dim3(256), 0, s, static_cast<const uint16_t*>(X), x_stride,
+                       x_rows, rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, vec, q, sc, scale_pitch(K));
+  else
+    hipLaunchKernelGGL(quantize_rows_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(X), x_stride, x_rows,
+                       rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, vec, q, sc, scale_pitch(K));
+  return check_launch("fp8_quantize_rows");
+}
+
+extern "C" int zmoe_fp8_quantize_weight(const void* W, int64_t w_stride_e, int64_t w_stride_n, int64_t E, int64_t N,
+                                        int64_t K, int dtype, void* Q, void* S, void* Qt, void* St, void* stream) {
+  int rc = quantize_checks("fp8_quantize_weight", N, K, dtype);
+  if (rc) return rc;
+  ZMOE_REQUIRE(N >= 1 && E >= 1 && E <= 65535 && w_stride_n >= K && w_stride_e >= 0, ZMOE_ERR_SHAPE,
+               "fp8_quantize_weight: bad sizes or strides");
+  ZMOE_REQUIRE(W && Q && S && (!Qt == !St), ZMOE_ERR_NULL, "fp8_quantize_weight: null pointer");
+  ZMOE_REQUIRE(aligned16(Q) && aligned4(S) && aligned16(Qt) && aligned4(St), ZMOE_ERR_ALIGN,
+               "fp8_quantize_weight: values on 16, scales on 4 bytes");
+  ZMOE_REQUIRE(blocks_of(N) <= 65535, ZMOE_ERR_SHAPE, "fp8_quantize_weight: too many rows");
+  const int v = 16 / dtype_size(dtype);
+  const int vec = aligned16(W) && w_stride_n % v == 0 && w_stride_e % v == 0;
+  const dim3 grid((unsigned)blocks_of(K), (unsigned)blocks_of(N), (unsigned)E);
+  hipStream_t s = as_stream(stream);
+  uint8_t *q = static_cast<uint8_t*>(Q), *sc = static_cast<uint8_t*>(S), *qt = static_cast<uint8_t*>(Qt),
+          *st = static_cast<uint8_t*>(St);
+  auto go = [&](auto t, auto trans) {
+    using T = decltype(t);
+    hipLaunchKernelGGL((quantize_weight_kernel<T, decltype(trans)::value>), grid, dim3(256), 0, s,
+                       static_cast<const T*>(W), w_stride_e, w_stride_n, N, K, vec, q, sc, qt, st);
+  };
+  if (dtype == ZMOE_DTYPE_BF16) {
+    if (Qt) go(uint16_t{}, std::true_type{});
+    else go(uint16_t{}, std::false_type{});
+  } else {
+    if (Qt) go(float{}, std::true_type{});
+    else go(float{}, std::false_type{});
+  }
+  return check_launch("fp8_quantize_weight");
+}
+
+namespace {
+// What both products check of A (rows of K values), its gather and B ([rows_b, K] per expert); fills them in.
+int product_operands(const char* name, const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
+                     int64_t K, int64_t rows_b, int64_t blocks_b, int E, const int64_t* offsets, Fp8Params& p) {
+  ZMOE_REQUIRE(Xq && Xs && Wq && Ws, ZMOE_ERR_NULL, "%s: null pointer", name);
+  ZMOE_REQUIRE(aligned16(Xq) && aligned4(Xs) && aligned16(Wq) && aligned4(Ws), ZMOE_ERR_ALIGN,
+               "%s: values on 16, scales on 4 bytes", name);
+  const int64_t nk = blocks_of(K);
+  p.a = static_cast<const uint8_t*>(Xq);
+  p.as = static_cast<const uint8_t*>(Xs);
+  p.lda = nk * kBlk;
+  p.a_pitch = scale_pitch(K);
+  p.a_bytes = M * p.lda;
+  p.b = static_cast<const uint8_t*>(Wq);
+  p.bs = static_cast<const uint8_t*>(Ws);
+  p.b_estride = rows_b * p.lda;
+  p.bs_pitch = scale_pitch(K);
+  p.bs_estride = blocks_b * p.bs_pitch;
+  ZMOE_REQUIRE(p.b_estride <= kMaxSpan8, ZMOE_ERR_SHAPE, "%s: one expert's weights span more than 2 GiB", name);
+  ZMOE_REQUIRE(!p.a_rows || p.a_bytes <= kMaxSpan8, ZMOE_ERR_SHAPE, "%s: gathered rows span more than 2 GiB", name);
+  ZMOE_REQUIRE(256 * p.lda <= kMaxSpan8, ZMOE_ERR_SHAPE, "%s: K too large", name);
+  p.b_bytes = (uint32_t)p.b_estride;
+  p.nk = (int)nk;
+  p.E = E;
+  p.offsets = offsets;
+  return ZMOE_OK;
+}
+}  // namespace
+
+extern "C" int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
+                                        const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t K,
+                                        int64_t N, int E, int k, int x_grouped, int y_grouped, int out_dtype, void* Y,
+                                        int64_t y_stride, void* stream) {
+  ZMOE_REQUIRE(dtype_ok(out_dtype), ZMOE_ERR_DTYPE, "fp8_scatter2scatter: dtype %d", out_dtype);
+  ZMOE_REQUIRE(M >= 0 && K >= 1 && N >= 1 && K < (1 << 30) && N < (1 << 30) && E >= 1 && E <= kGemmMaxE && k >= 1,
+               ZMOE_ERR_SHAPE, "fp8_scatter2scatter: bad sizes (M=%lld K=%lld N=%lld E=%d k=%d)", (long long)M,
+               (long long)K, (long long)N, E, k);
+  ZMOE_REQUIRE(M < kMaxRows8 && M * (x_grouped ? 1 : k) < kMaxRows8, ZMOE_ERR_SHAPE,
+               "fp8_scatter2scatter: rows must be below 2^31");
+  ZMOE_REQUIRE(expert_offsets || (E == 1 && x_grouped && y_grouped), ZMOE_ERR_NULL,
+               "fp8_scatter2scatter: no expert_offsets only for one weight and rows in order");
+  ZMOE_REQUIRE((x_grouped && y_grouped) || sorted_scattered_idxs, ZMOE_ERR_NULL,
+               "fp8_scatter2scatter: sorted_scattered_idxs required unless x_grouped and y_grouped");
+  ZMOE_REQUIRE(y_stride >= N, ZMOE_ERR_SHAPE, "fp8_scatter2scatter: row stride of Y");
+  const int64_t R = x_grouped ? M : M * k;
+  if (R == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(Y, ZMOE_ERR_NULL, "fp8_scatter2scatter: null pointer");
+  ZMOE_REQUIRE((reinterpret_cast<uintptr_t>(Y) % dtype_size(out_dtype)) == 0, ZMOE_ERR_ALIGN,
+               "fp8_scatter2scatter: Y's alignment");
+  Fp8Params p{};
+  p.a_rows = x_grouped ? nullptr : sorted_scattered_idxs;
+  p.a_div = k;
+  int rc = product_operands("fp8_scatter2scatter", Xq, Xs, M, Wq, Ws, K, N, blocks_of(N), E, expert_offsets, p);
+  if (rc) return rc;
+  p.c = Y;
+  p.ldc = y_stride;
+  p.c_rows = y_grouped ? nullptr : sorted_scattered_idxs;
+  p.vec_c = aligned16(Y) && y_stride % (16 / dtype_size(out_dtype)) == 0;
+  p.N = (int)N;
+  p.n_major = x_grouped ? 1 : 0;
+  p.ns_m = expert_offsets ? 0 : (int)M;
+  return out_dtype == ZMOE_DTYPE_BF16 ? dispatch8<F8_STORE_BF16>(p, R, as_stream(stream))
+                                      : dispatch8<F8_STORE_F32>(p, R, as_stream(stream));
+}
+
+extern "C" int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T, const void* W1q, const void* W1s,
+                                       const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t d,
+                                       int64_t f, int E, int k, void* Aq, void* As, void* stream) {
+  ZMOE_REQUIRE(T >= 0 && d >= 1 && f >= 1 && d < (1 << 30) && f < (1 << 29) && E >= 1 && E <= kGemmMaxE && k >= 1,
+               ZMOE_ERR_SHAPE, "fp8_glu_w1_forward: bad sizes");
+  ZMOE_REQUIRE(T < kMaxRows8 && T * k < kMaxRows8, ZMOE_ERR_SHAPE, "fp8_glu_w1_forward: T*k must be below 2^31");
+  ZMOE_REQUIRE(expert_offsets ? sorted_scattered_idxs != nullptr : (E == 1 && k == 1), ZMOE_ERR_NULL,
+               "fp8_glu_w1_forward: no expert_offsets only for one weight, else sorted_scattered_idxs too");
+  const int64_t R = T * k;
+  if (R == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(Aq && As, ZMOE_ERR_NULL, "fp8_glu_w1_forward: null pointer");
+  ZMOE_REQUIRE(aligned16(Aq) && aligned4(As), ZMOE_ERR_ALIGN, "fp8_glu_w1_forward: values on 16, scales on 4 bytes");
+  Fp8Params p{};
+  p.a_rows = expert_offsets ? sorted_scattered_idxs : nullptr;
+  p.a_div = k;
+  int rc = product_operands("fp8_glu_w1_forward", Xq, Xs, T, W1q, W1s, d, 2 * f, 2 * blocks_of(f), E, expert_offsets, p);
+  if (rc) return rc;
+  p.c = Aq;
+  p.ldc = blocks_of(f) * kBlk;
+  p.cs = static_cast<uint8_t*>(As);
+  p.cs_pitch = scale_pitch(f);
+  p.half = (int)f;
+  p.N = (int)(2 * f);
+  p.n_major = 0;
+  p.ns_m = expert_offsets ? 0 : (int)T;
+  return dispatch8<F8_GLU>(p, R, as_stream(stream));
+}

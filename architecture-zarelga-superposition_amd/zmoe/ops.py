@@ -813,6 +813,131 @@ def rmsnorm_rows_backward(dY: torch.Tensor, X: torch.Tensor, rows: Optional[torc
     return dX, dw.view(weight.shape)
 
 
+# --------------------------------------------------------------------- e4m3 with a scale per block of 128
+# Activation rows: q float8_e4m3fn [n, Kp], s uint8 [n, pitch] (E8M0 bytes, one per block; include/zmoe.h).
+# Weights: q [..., N, Kp], s [..., ceil(N / 128), pitch].
+FP8_BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+
+
+def fp8_width(K: int) -> int:
+    """Bytes of a quantised row of K values."""
+    return -(-K // FP8_BLOCK) * FP8_BLOCK
+
+
+def fp8_scale_pitch(K: int) -> int:
+    """Bytes of its scales (zmoe_fp8_scale_pitch, in Python so that tracing can follow it)."""
+    return -(-K // (4 * FP8_BLOCK)) * 4
+
+
+def fp8_quantize_rows(X: torch.Tensor, rows: Optional[torch.Tensor] = None, row_div: int = 1,
+                      row_scale: Optional[torch.Tensor] = None):
+    """(q, s) of the rows of X [M, K] (any width and row stride); with ``rows`` (int64) row i is
+    X[rows[i] // row_div], with ``row_scale`` (f32) times row_scale[rows[i]]."""
+    dev = _require_cuda(X, rows, row_scale)
+    X = _rows(X)
+    M, K = X.shape
+    r = None if rows is None else _idx64(rows)
+    n = M if r is None else r.numel()
+    if row_scale is not None:
+        row_scale = row_scale.reshape(-1).to(torch.float32).contiguous()
+        if row_scale.numel() != (n if r is None else M * row_div):
+            raise ValueError("fp8_quantize_rows: one scale per row")
+    q = torch.empty((n, fp8_width(K)), dtype=_E4M3, device=dev)
+    s = torch.empty((n, fp8_scale_pitch(K)), dtype=torch.uint8, device=dev)
+    with profiling.region("fp8_quantize_rows", dev):
+        L.call("zmoe_fp8_quantize_rows", _ptr(X), max(X.stride(0), K), M, _ptr(r), row_div, _ptr(row_scale), n, K,
+               _dtype_code(X), _ptr(q), _ptr(s), _stream(dev))
+    return q, s
+
+
+def fp8_quantize_weight(W: torch.Tensor, transposed: bool = False):
+    """(q, s) of W [..., N, K], with ``transposed`` (q, s, qt, st): qt, st of W^T, the same values."""
+    dev = _require_cuda(W)
+    if W.dim() < 2 or W.numel() == 0:
+        raise ValueError(f"fp8_quantize_weight: expected [..., N, K], got {tuple(W.shape)}")
+    lead, (N, K) = W.shape[:-2], W.shape[-2:]
+    W3 = W.reshape(-1, N, K)
+    if W3.stride(2) != 1 or (N > 1 and W3.stride(1) < K):
+        W3 = W3.contiguous()
+    E = W3.shape[0]
+
+    def new(n, k):
+        return (torch.empty((*lead, n, fp8_width(k)), dtype=_E4M3, device=dev),
+                torch.empty((*lead, -(-n // FP8_BLOCK), fp8_scale_pitch(k)), dtype=torch.uint8, device=dev))
+
+    out = (*new(N, K), *new(K, N)) if transposed else (*new(N, K), None, None)
+    with profiling.region("fp8_quantize_weight", dev):
+        L.call("zmoe_fp8_quantize_weight", _ptr(W3), W3.stride(0), max(W3.stride(1), K), E, N, K, _dtype_code(W3),
+               *map(_ptr, out), _stream(dev))
+    return out if transposed else out[:2]
+
+
+def _fp8_operand(q: torch.Tensor, s: torch.Tensor, K: int, what: str):
+    """Checks of a quantised operand's two tensors: (q, s) contiguous."""
+    if (q.dtype != _E4M3 or s.dtype != torch.uint8 or q.dim() != s.dim() or q.shape[-1] != fp8_width(K)
+            or s.shape[-1] != fp8_scale_pitch(K) or q.shape[:-2] != s.shape[:-2]):
+        raise ValueError(f"{what}: not a quantised operand of depth {K}")
+    return _on16(q), s.contiguous()
+
+
+def fp8_scatter2scatter(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, K: int,
+                        sorted_scattered_idxs: Optional[torch.Tensor] = None,
+                        expert_offsets: Optional[torch.Tensor] = None, k: int = 1, x_grouped: bool = True,
+                        y_grouped: bool = True, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``scatter2scatter`` on quantised operands: rows xq, xs times the weights wq [E, N, Kp]. Without
+    ``expert_offsets``: one weight wq [N, Kp], rows in order (a dense product)."""
+    dev = _require_cuda(xq, xs, wq, ws, sorted_scattered_idxs, expert_offsets)
+    xq, xs = _fp8_operand(xq, xs, K, "fp8_scatter2scatter")
+    wq, ws = _fp8_operand(wq, ws, K, "fp8_scatter2scatter")
+    M, N = xq.shape[0], wq.shape[-2]
+    if xs.shape[0] != M or ws.shape[-2] != -(-N // FP8_BLOCK):
+        raise ValueError("fp8_scatter2scatter: values and scales do not match")
+    R = M if x_grouped else M * k
+    if expert_offsets is None:
+        if wq.dim() != 2 or not (x_grouped and y_grouped):
+            raise ValueError("fp8_scatter2scatter: several weights need expert_offsets")
+        E, off, ss = 1, None, None
+    else:
+        E, off = wq.shape[0], _idx64(expert_offsets)
+        ss = None if sorted_scattered_idxs is None else _idx64(sorted_scattered_idxs)
+        if wq.dim() != 3 or off.numel() != E or (ss is None and not (x_grouped and y_grouped)) or (
+                ss is not None and ss.numel() != R):
+            raise ValueError("fp8_scatter2scatter: offsets and indices must match the weights and rows")
+    if out_dtype not in _DT:
+        raise ValueError(f"fp8_scatter2scatter: out_dtype {out_dtype}")
+    out = torch.empty((R, N), dtype=out_dtype, device=dev)
+    with profiling.region("fp8_scatter2scatter", dev):
+        L.call("zmoe_fp8_scatter2scatter", _ptr(xq), _ptr(xs), M, _ptr(wq), _ptr(ws), _ptr(ss), _ptr(off), K, N, E, k,
+               int(x_grouped), int(y_grouped), _DT[out_dtype], _ptr(out), N, _stream(dev))
+    return out
+
+
+def fp8_glu_w1_forward(xq: torch.Tensor, xs: torch.Tensor, w1q: torch.Tensor, w1s: torch.Tensor, d: int,
+                       sorted_scattered_idxs: Optional[torch.Tensor] = None,
+                       expert_offsets: Optional[torch.Tensor] = None, k: int = 1):
+    """(aq, as) [T*k rows in sorted order]: the quantised silu(gate) * up of the rows' products with
+    w1q [2E, f, dp] (the [E, 2f, d] weight's halves, quantised as 2E weights). Without
+    ``expert_offsets``: one expert, rows in order."""
+    dev = _require_cuda(xq, xs, w1q, w1s, sorted_scattered_idxs, expert_offsets)
+    xq, xs = _fp8_operand(xq, xs, d, "fp8_glu_w1_forward")
+    w1q, w1s = _fp8_operand(w1q, w1s, d, "fp8_glu_w1_forward")
+    T, (E2, f) = xq.shape[0], w1q.shape[:2]
+    E = E2 // 2
+    off = None if expert_offsets is None else _idx64(expert_offsets)
+    ss = None if sorted_scattered_idxs is None or off is None else _idx64(sorted_scattered_idxs)
+    if (w1q.dim() != 3 or E2 % 2 or xs.shape[0] != T or w1s.shape[1] != -(-f // FP8_BLOCK)
+            or (off is None and (E != 1 or k != 1)) or (off is not None and off.numel() != E)
+            or (off is not None and (ss is None or ss.numel() != T * k))):
+        raise ValueError("fp8_glu_w1_forward: operand shapes do not match")
+    aq = torch.empty((T * k, fp8_width(f)), dtype=_E4M3, device=dev)
+    as_ = torch.empty((T * k, fp8_scale_pitch(f)), dtype=torch.uint8, device=dev)
+    with profiling.region("fp8_glu_w1_forward", dev):
+        L.call("zmoe_fp8_glu_w1_forward", _ptr(xq), _ptr(xs), T, _ptr(w1q), _ptr(w1s), _ptr(ss), _ptr(off), d, f, E, k,
+               _ptr(aq), _ptr(as_), _stream(dev))
+    return aq, as_
+
+
 NS_COEFFS = (3.4445, -4.7750, 2.0315)  # optimizer/muon.py:16
 
 

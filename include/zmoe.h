@@ -430,6 +430,47 @@ size_t zmoe_newton_schulz5_workspace_bytes(int64_t E, int64_t m, int64_t n);
 int zmoe_newton_schulz5(void* X, int64_t E, int64_t m, int64_t n, int steps, float a, float b, float c,
                         void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Products in 8-bit floating point (OCP e4m3) with a power-of-two scale for each block of 128,
+ * dense and grouped by expert.
+ *   A block of values v (1 x 128 along a row of activations; 128 x 128 of a weight; the last block
+ *   of a row or column is shorter) is held as q s: s = 2^c with c the least whole number >= -127
+ *   for which max |v| <= 448 s (over the finite values), q = v / s rounded to e4m3 (nearest, ties to
+ *   even); inf and NaN become e4m3's NaN. Scales are bytes c + 127 (E8M0).
+ * Layout: K values take Kp = 128 ceil(K / 128) bytes (zeros past K), their scales
+ * zmoe_fp8_scale_pitch(K) bytes (a multiple of 4, one byte a block). Rows lie one after the other. Values start on 16
+ * bytes, scales on 4.
+ * ------------------------------------------------------------------------- */
+int64_t zmoe_fp8_scale_pitch(int64_t K);
+
+/* Q [n, Kp], S [n, pitch] of rows of X [x_rows, K] (F32 or BF16, rows x_stride elements apart): row i is X[i], or
+ * with rows (int64 [n]) X[rows[i] / row_div] (zeros for an index out of range); with row_scale (f32) times
+ * row_scale[rows[i]] (row_scale[i] without rows), the product rounded to f32. */
+int zmoe_fp8_quantize_rows(const void* X, int64_t x_stride, int64_t x_rows, const int64_t* rows, int row_div,
+                           const float* row_scale, int64_t n, int64_t K, int dtype, void* Q, void* S, void* stream);
+
+/* Q [E, N, Kp], S [E, ceil(N / 128), pitch(K)] of weights W [E, N, K] (F32 or BF16; unit stride along K); with Qt and
+ * St (both or neither) also the same values transposed: Qt [E, K, Np], St [E, ceil(K / 128), pitch(N)]. E <= 65535,
+ * N <= 128 * 65535. */
+int zmoe_fp8_quantize_weight(const void* W, int64_t w_stride_e, int64_t w_stride_n, int64_t E, int64_t N, int64_t K,
+                             int dtype, void* Q, void* S, void* Qt, void* St, void* stream);
+
+/* zmoe_scatter2scatter on such operands: Y (BF16 or F32, rows y_stride elements apart) rows = X rows times W_e^T, W_e
+ * [N, K]; sums in f32, one rounding. Without expert_offsets (E = 1, x_grouped and y_grouped): one weight for all M
+ * rows. Any K and N. One expert's weights, and gathered X rows, must span less than 2 GiB - 64 KiB. */
+int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
+                             const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t K,
+                             int64_t N, int E, int k, int x_grouped, int y_grouped, int out_dtype, void* Y,
+                             int64_t y_stride, void* stream);
+
+/* The first product of SwiGLU experts with the activation and its quantisation: for sorted row i
+ *   A[i, j] = silu(g) u, u = X[sorted_scattered_idxs[i] / k] W1_e[j], g = that times W1_e[f + j]  (f32)
+ * and Aq [R, fp], As [R, pitch(f)] its quantised rows. W1q, W1s: the quantised [2E, f, d] view of W1 [E, 2f, d], so
+ * that no block holds rows of both halves. Without expert_offsets: E = k = 1, rows in order. */
+int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T, const void* W1q, const void* W1s,
+                            const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t d, int64_t f,
+                            int E, int k, void* Aq, void* As, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,159 @@
+"""Block-scaled e4m3 on the GPU against the format and the products in float64 (oracle.fp8_oracle).
+
+Tolerances. Quantised values and scales are equal to the oracle's: v / s is exact. A product's terms are exact
+(4-bit mantissas times 4-bit ones). The matrix unit adds them 128 at a time: in each group of 8 consecutive
+depths it cuts every term off at 2^-13 of the power of two below the group's largest (measured: terms of 1.875 x
+1.875 beside one of 2^16 keep bits down to 2^3), so a group loses less than 7 * 2^-13 of its largest term; the 16
+group sums and the running sum are added to 24 bits or more, each cut off by less than 2^-23 of a partial sum, which is
+at most S = sum |terms|. With G = sum over groups of the largest |term|:
+|error| < 7 * 2^-13 G + 17 ceil(K / 128) 2^-23 S, plus half a step of the output, 2^-8 |y| in bf16, 2^-24 |y| in f32.
+"""
+
+import pytest
+import torch
+
+from helpers import gen, random_topk
+from oracle import fp8_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def z():
+    from zmoe import ops
+
+    return ops
+
+
+def same(a, b):
+    """Equal, NaN in the same places."""
+    return torch.equal(torch.nan_to_num(a.double(), nan=12345.0), torch.nan_to_num(b.double(), nan=12345.0))
+
+
+def rows_values(q, s, K):
+    """The values quantised rows stand for, and their exponents."""
+    n, kp = q.shape
+    c = s[:, :kp // 128].to(torch.int64) - 127
+    v = q.to(torch.float32).double().view(n, kp // 128, 128) * O.two(c).unsqueeze(-1)
+    return v.view(n, kp), c
+
+
+def activations(n, K, dtype, seed, dev):
+    g = gen(seed)
+    x = torch.randn(n, K, generator=g) * torch.exp(torch.randn(K, generator=g))
+    return x.to(dtype).to(dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("n,K", [(1, 1), (1, 128), (3, 127), (5, 129), (7, 510), (64, 512), (33, 2048), (0, 256)])
+def test_quantize_rows(n, K, dtype, hip_device):
+    x = activations(n, K, DT[dtype], n * K + 1, hip_device)
+    q, s = z().fp8_quantize_rows(x)
+    v, c = rows_values(q, s, K)
+    ref, cref = O.quantize_rows(x)
+    assert torch.equal(c, cref) and torch.equal(v[:, :K], ref)
+    assert not v[:, K:].any()
+
+
+def test_quantize_rows_at_the_borders(hip_device):
+    """Zeros, the largest value on and next to 448 2^c, ties, f32 denormals and the largest f32, inf and NaN."""
+    base = torch.zeros(12, 256)
+    base[1, 5] = 448.0
+    base[2, 5] = 448.0 + 2.0 ** -14
+    base[3, :128] = torch.linspace(-448, 448, 128)
+    base[4, :128] = (torch.arange(128) + 0.5) / 16 + 1      # ties of several binades
+    base[4, 0] = 448.0
+    base[5, 0], base[5, 1] = 2.0 ** -140, -2.0 ** -149
+    base[6, 0], base[6, 1] = torch.finfo(torch.float32).max, 1.0
+    base[7, 3], base[7, 4], base[7, 5] = float("inf"), 2.5, float("-inf")
+    base[8, 3], base[8, 130] = float("nan"), 7.0
+    base[9] = float("inf")
+    base[10, 0], base[10, 1:40] = 448.0, torch.arange(1, 40) * 2.0 ** -10  # e4m3's own denormals
+    base[11] = -0.0
+    for x in (base, base.to(torch.bfloat16)):
+        x = x.to(hip_device)
+        q, s = z().fp8_quantize_rows(x)
+        v, c = rows_values(q, s, 256)
+        ref, cref = O.quantize_rows(x)
+        assert torch.equal(c, cref) and same(v, ref)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantize_rows_views(dtype, hip_device):
+    """Row strides and starts off 16 bytes, gathered and scaled rows, indices out of range."""
+    big = activations(40, 301, DT[dtype], 5, hip_device)
+    for x in (big[:, 1:258], big[::2, :256], big.t()[:, 3:], big[3:4, 2:]):
+        q, s = z().fp8_quantize_rows(x)
+        ref, cref = O.quantize_rows(x)
+        v, c = rows_values(q, s, x.shape[1])
+        assert torch.equal(c, cref) and torch.equal(v[:, :x.shape[1]], ref)
+    x = big[:, :300]
+    slots = torch.randperm(120, generator=gen(3)).to(hip_device)
+    w = torch.rand(120, generator=gen(4)).to(hip_device)
+    q, s = z().fp8_quantize_rows(x, rows=slots, row_div=3, row_scale=w)
+    ref, cref = O.quantize_rows(x.float()[slots // 3] * w[slots].unsqueeze(1))
+    v, c = rows_values(q, s, 300)
+    assert torch.equal(c, cref) and torch.equal(v[:, :300], ref)
+    bad = torch.tensor([0, -1, 119, 120, -120, 1 << 40], device=hip_device)
+    q, s = z().fp8_quantize_rows(x, rows=bad, row_div=3, row_scale=w)
+    v, _ = rows_values(q, s, 300)
+    assert not v[[1, 3, 4, 5]].any() and v[0].any() and v[2].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("E,N,K", [(1, 1, 1), (2, 128, 128), (3, 130, 257), (1, 510, 1030), (4, 96, 512)])
+def test_quantize_weight(E, N, K, dtype, hip_device):
+    W = (torch.randn(E, N, K, generator=gen(E * N + K)) * 0.05).to(DT[dtype]).to(hip_device)
+    W[0, N // 2, K // 2] = float("nan")
+    q, s, qt, st = z().fp8_quantize_weight(W, transposed=True)
+    ref, cref = O.quantize_weight(W)
+    nb, kb = -(-N // 128), -(-K // 128)
+
+    def values(q, s, rows, cols):
+        c = s[..., :-(-cols // 128)].to(torch.int64) - 127
+        sc = O.two(c).repeat_interleave(128, 1)[:, :rows].repeat_interleave(128, 2)
+        return q.to(torch.float32).double() * sc
+
+    assert torch.equal(s[..., :kb].to(torch.int64) - 127, cref)
+    assert torch.equal(st[..., :nb], s[..., :kb].transpose(1, 2))
+    assert same(values(q, s, N, K)[..., :K], ref) and same(values(qt, st, K, N)[..., :N], ref.transpose(1, 2))
+    assert not values(q, s, N, K)[..., K:].any() and not values(qt, st, K, N)[..., N:].any()
+    q2, s2 = z().fp8_quantize_weight(W)
+    assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2[..., :kb], s[..., :kb])
+
+
+def check(got, ref, S, G, K):
+    assert got.shape == ref.shape and not torch.isnan(got).any()
+    half = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+    b = half * ref.abs() + 7 * 2.0 ** -13 * G + 17 * -(-K // 128) * 2.0 ** -23 * S
+    err = (got.double() - ref).abs()
+    worst = float((err / b.clamp(min=1e-300)).max()) if err.numel() else 0.0
+    print(f"  worst |err| / bound {worst:.3f}", flush=True)
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 1536, 2048), (3, 130, 127), (31, 256, 512), (33, 510, 1030),
+                                   (200, 264, 640), (257, 1000, 384), (600, 770, 8200), (1025, 512, 128)])
+def test_dense_product(M, N, K, out, hip_device):
+    x = activations(M, K, torch.bfloat16, M + K, hip_device)
+    W = (torch.randn(N, K, generator=gen(N)) * 0.1).to(torch.bfloat16).to(hip_device)
+    W *= torch.exp2(torch.randint(-9, 9, (N, 1), generator=gen(1))).to(torch.bfloat16).to(hip_device)
+    xr, wr = O.quantize_rows(x)[0], O.quantize_weight(W)[0]
+    got = z().fp8_scatter2scatter(*z().fp8_quantize_rows(x), *z().fp8_quantize_weight(W), K, out_dtype=DT[out])
+    check(got, *O.product(xr, wr), K)
+
+
+@pytest.mark.parametrize("T,E,k,N,K,skew", [(1, 8, 2, 256, 256, 0.0), (40, 8, 2, 130, 200, 0.0), (300, 16, 4, 512, 512, 1.2),
+                                            (500, 4, 2, 264, 384, 0.5), (1500, 5, 2, 770, 640, 1.5),
+                                            (700, 130, 1, 96, 160, 1.0)])
+@pytest.mark.parametrize("xg,yg", [(False, True), (True, False), (True, True), (False, False)])
+def test_grouped_product(T, E, k, N, K, skew, xg, yg, hip_device):
+    idx = random_topk(T, E, k, T + E, skew).to(hip_device)
+    se, ss, off, inv = z().flatten_sort_count(idx, E)
+    x = activations(T * k if xg else T, K, torch.bfloat16, T, hip_device)
+    W = (torch.randn(E, N, K, generator=gen(N)) * 0.1).to(torch.bfloat16).to(hip_device)
+    ref = O.grouped_product(O.quantize_rows(x)[0], O.quantize_weight(W)[0], ss, off, k, xg, yg)
+    got = z().fp8_scatter2scatter(*z().fp8_quantize_rows(x), *z().fp8_quantize_weight(W), K, ss, off, 1 if xg else k, xg, yg)
+    check(got, *ref, K)
