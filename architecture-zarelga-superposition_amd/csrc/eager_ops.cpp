@@ -601,6 +601,232 @@ Tensors rmsnorm_rows_backward(const Tensor& dY, const Tensor& X, const Opt& rows
   return op.call(dY, X, rows, rstd, weight);
 }
 
+// ------------------------------------------------------------------ e4m3 with a scale per block of 128
+int64_t width8(int64_t K) { return (K + 127) / 128 * 128; }
+int64_t blocks8(int64_t n) { return (n + 127) / 128; }
+int64_t pitch8(int64_t K) { return (K + 511) / 512 * 4; }  // zmoe_fp8_scale_pitch
+
+// rows2 whose rows do not overlap (expanded tensors go to the general form).
+bool apart(const Tensor& t) { return rows2(t, t) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
+
+struct Rows8 {
+  Tensor q, s;
+};
+Rows8 empty8(int64_t n, int64_t K, const Tensor& like) {
+  return {empty({n, width8(K)}, like, at::kFloat8_e4m3fn), empty({n, pitch8(K)}, like, at::kByte)};
+}
+// A quantised weight [..., N, Kp] and its scales, dims of values and scales alike.
+bool weight8(const Tensor& q, const Tensor& s, int64_t K, int64_t dim, const Tensor& like) {
+  return flat(q, like, at::kFloat8_e4m3fn) && flat(s, like, at::kByte) && q.dim() == dim && s.dim() == dim &&
+         q.size(-1) == width8(K) && s.size(-1) == pitch8(K) && s.size(-2) == blocks8(q.size(-2)) &&
+         (dim < 3 || q.size(0) == s.size(0));
+}
+bool rows8(const Tensor& q, const Tensor& s, int64_t K, const Tensor& like) {
+  return flat(q, like, at::kFloat8_e4m3fn) && flat(s, like, at::kByte) && q.dim() == 2 && s.dim() == 2 &&
+         q.size(1) == width8(K) && s.size(1) == pitch8(K) && s.size(0) == q.size(0);
+}
+// X's rows quantised into r; false on an error.
+bool quantize_into(const Tensor& X, const Rows8& r, const Opt& rows, int64_t div, const Opt& scale) {
+  const int64_t K = X.size(1);
+  return zmoe_fp8_quantize_rows(raw(X), std::max(X.stride(0), K), X.size(0), rows ? ids(*rows) : nullptr, (int)div,
+                                scale ? ptr<const float>(*scale) : nullptr, r.q.size(0), K, code(X), raw(r.q),
+                                raw(r.s), stream_of(X)) == ZMOE_OK;
+}
+
+Tensors fp8_quantize_rows(const Tensor& X, const Opt& rows, int64_t div, const Opt& scale) {
+  if (X.is_cuda() && known(X) && apart(X) && X.size(1) > 0 && div > 0 && fits_int(div) &&
+      (!rows || flat(*rows, X, at::kLong))) {
+    const int64_t n = rows ? rows->numel() : X.size(0);
+    if (!scale || (flat(*scale, X, at::kFloat) && scale->numel() == (rows ? X.size(0) * div : n))) {
+      const c10::DeviceGuard guard(X.device());
+      const Rows8 r = empty8(n, X.size(1), X);
+      if (quantize_into(X, r, rows, div, scale)) return {r.q, r.s};
+    }
+  }
+  static const auto op = general<Tensors(const Tensor&, const Opt&, c10::SymInt, const Opt&)>("zmoe::fp8_quantize_rows");
+  return op.call(X, rows, div, scale);
+}
+
+Tensors fp8_quantize_weight(const Tensor& W, bool transposed) {
+  if (W.is_cuda() && known(W) && W.dim() >= 2 && W.numel() > 0 && W.is_contiguous()) {
+    const c10::DeviceGuard guard(W.device());
+    const int64_t N = W.size(-2), K = W.size(-1), E = W.numel() / (N * K);
+    auto make = [&](int64_t n, int64_t k, Tensors& out) {
+      auto q = W.sizes().slice(0, W.dim() - 2).vec(), s = q;
+      q.insert(q.end(), {n, width8(k)});
+      s.insert(s.end(), {blocks8(n), pitch8(k)});
+      out.push_back(empty(q, W, at::kFloat8_e4m3fn));
+      out.push_back(empty(s, W, at::kByte));
+    };
+    Tensors out;
+    make(N, K, out);
+    if (transposed) make(K, N, out);
+    if (zmoe_fp8_quantize_weight(raw(W), N * K, K, E, N, K, code(W), raw(out[0]), raw(out[1]),
+                                 transposed ? raw(out[2]) : nullptr, transposed ? raw(out[3]) : nullptr,
+                                 stream_of(W)) == ZMOE_OK)
+      return out;
+  }
+  static const auto op = general<Tensors(const Tensor&, bool)>("zmoe::fp8_quantize_weight");
+  return op.call(W, transposed);
+}
+
+Tensor fp8_mm(const Tensor& xq, const Tensor& xs, const Tensor& wq, const Tensor& ws, int64_t K, const Opt& ss,
+              const Opt& off, int64_t k, bool xg, bool yg, bool out_f32) {
+  if (K > 0 && k > 0 && fits_int(k) && xq.is_cuda() && rows8(xq, xs, K, xq) && weight8(wq, ws, K, off ? 3 : 2, xq)) {
+    const int64_t M = xq.size(0), N = wq.size(-2), E = off ? wq.size(0) : 1, R = xg ? M : M * k;
+    if ((off ? index(*off, xq, E) && (ss ? index(*ss, xq, R) : xg && yg) : xg && yg) && fits_int(E)) {
+      const c10::DeviceGuard guard(xq.device());
+      Tensor Y = empty({R, N}, xq, out_f32 ? at::kFloat : at::kBFloat16);
+      if (zmoe_fp8_scatter2scatter(raw(xq), raw(xs), M, raw(wq), raw(ws), off && ss ? ids(*ss) : nullptr,
+                                   off ? ids(*off) : nullptr, K, N, (int)E, (int)k, xg, yg, code(Y), raw(Y), N,
+                                   stream_of(xq)) == ZMOE_OK)
+        return Y;
+    }
+  }
+  static const auto op = general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, c10::SymInt,
+                                        const Opt&, const Opt&, c10::SymInt, bool, bool, bool)>("zmoe::fp8_mm");
+  return op.call(xq, xs, wq, ws, K, ss, off, k, xg, yg, out_f32);
+}
+
+Tensor fp8_linear(const Tensor& x, const Tensor& wq, const Tensor& ws) {
+  if (x.is_cuda() && known(x) && apart(x) && x.size(1) > 0 && weight8(wq, ws, x.size(1), 2, x)) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), K = x.size(1), N = wq.size(0);
+    const Rows8 r = empty8(M, K, x);
+    Tensor Y = empty({M, N}, x);
+    if (quantize_into(x, r, std::nullopt, 1, std::nullopt) &&
+        zmoe_fp8_scatter2scatter(raw(r.q), raw(r.s), M, raw(wq), raw(ws), nullptr, nullptr, K, N, 1, 1, 1, 1, code(Y),
+                                 raw(Y), N, stream_of(x)) == ZMOE_OK)
+      return Y;
+  }
+  static const auto op = general<Tensor(const Tensor&, const Tensor&, const Tensor&)>("zmoe::fp8_linear");
+  return op.call(x, wq, ws);
+}
+
+Tensor fp8_glu_mlp(const Tensor& x, const Tensor& w1q, const Tensor& w1s, const Tensor& w2q, const Tensor& w2s) {
+  if (x.is_cuda() && known(x) && apart(x) && x.size(1) > 0 && weight8(w1q, w1s, x.size(1), 3, x) &&
+      w1q.size(0) == 2 && w1q.size(1) > 0 && weight8(w2q, w2s, w1q.size(1), 2, x) && w2q.size(0) == x.size(1)) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), d = x.size(1), f = w1q.size(1);
+    const Rows8 r = empty8(M, d, x), a = empty8(M, f, x);
+    Tensor Y = empty({M, d}, x);
+    void* s = stream_of(x);
+    if (quantize_into(x, r, std::nullopt, 1, std::nullopt) &&
+        zmoe_fp8_glu_w1_forward(raw(r.q), raw(r.s), M, raw(w1q), raw(w1s), nullptr, nullptr, d, f, 1, 1, raw(a.q),
+                                raw(a.s), s) == ZMOE_OK &&
+        zmoe_fp8_scatter2scatter(raw(a.q), raw(a.s), M, raw(w2q), raw(w2s), nullptr, nullptr, f, d, 1, 1, 1, 1, code(Y),
+                                 raw(Y), d, s) == ZMOE_OK)
+      return Y;
+  }
+  static const auto op = general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&)>(
+      "zmoe::fp8_glu_mlp");
+  return op.call(x, w1q, w1s, w2q, w2s);
+}
+
+Tensors fp8_glu_experts(const Tensor& x, const Tensor& gates, const Tensor& idx, const Tensor& w1q, const Tensor& w1s,
+                        const Tensor& w2q, const Tensor& w2s, const Opt& residual, const Opt& out_rows,
+                        int64_t out_total) {
+  if (x.is_cuda() && known(x) && apart(x) && x.size(1) > 0 && flat(idx, x, at::kLong) && idx.dim() == 2 &&
+      idx.size(0) == x.size(0) && idx.size(1) > 0 && flat(gates, x, at::kFloat) && gates.numel() == idx.numel() &&
+      weight8(w1q, w1s, x.size(1), 3, x) && w1q.size(0) % 2 == 0 && w1q.size(1) > 0 &&
+      weight8(w2q, w2s, w1q.size(1), 3, x) && w2q.size(0) * 2 == w1q.size(0) && w2q.size(1) == x.size(1) &&
+      fits_int(w2q.size(0)) && fits_int(idx.size(1))) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t T = x.size(0), d = x.size(1), f = w1q.size(1), E = w2q.size(0), k = idx.size(1), R = T * k;
+    const Tensors sorted = flatten_sort_count(idx, E);
+    const Tensor &ss = sorted[1], &off = sorted[2];
+    const Rows8 r = empty8(T, d, x), a = empty8(R, f, x);
+    Tensor Y = empty({R, d}, x);
+    void* s = stream_of(x);
+    if (quantize_into(x, r, std::nullopt, 1, std::nullopt) &&
+        zmoe_fp8_glu_w1_forward(raw(r.q), raw(r.s), T, raw(w1q), raw(w1s), ids(ss), ids(off), d, f, (int)E, (int)k,
+                                raw(a.q), raw(a.s), s) == ZMOE_OK &&
+        zmoe_fp8_scatter2scatter(raw(a.q), raw(a.s), R, raw(w2q), raw(w2s), ids(ss), ids(off), f, d, (int)E, 1, 1, 0,
+                                 code(Y), raw(Y), d, s) == ZMOE_OK)
+      return {combine(Y, gates, k, residual, out_rows, out_total), off};
+  }
+  static const auto op = general<Tensors(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                         const Tensor&, const Tensor&, const Opt&, const Opt&, c10::SymInt)>(
+      "zmoe::fp8_glu_experts");
+  return op.call(x, gates, idx, w1q, w1s, w2q, w2s, residual, out_rows, out_total);
+}
+
+// ------------------------------------------------------------------ the step between two sublayers
+// What norm_residual and its backward take here: rows of known types, weights and gate as their kinds ask.
+bool norm_residual_ok(const Tensor& R, const Tensor& Y, const Opt& w1, const Opt& w2, const Opt& gate, int64_t kind,
+                      const Opt& scale) {
+  if (!(Y.is_cuda() && known(Y) && apart(Y) && on(R, Y) && known(R) && apart(R) && R.sizes() == Y.sizes() &&
+        (w1 || w2)))
+    return false;
+  const int64_t n = Y.size(0), d = Y.size(1);
+  for (const Opt* w : {&w1, &w2})
+    if (*w && !(on(**w, Y) && known(**w) && (*w)->is_contiguous() && (*w)->numel() == d)) return false;
+  if (w1 && w2 && w1->scalar_type() != w2->scalar_type()) return false;
+  if (kind < 0 || kind > 3 || (kind == 0) == gate.has_value()) return false;
+  if (gate && !(on(*gate, Y) && known(*gate) &&
+                (kind == 3 ? apart(*gate) && gate->sizes() == Y.sizes()
+                           : gate->dim() == 1 && gate->is_contiguous() && gate->numel() == (kind == 1 ? d : n))))
+    return false;
+  return !scale || (flat(*scale, Y, at::kFloat) && scale->numel() == 1);
+}
+
+Tensors norm_residual(const Tensor& R, const Tensor& Y, const Opt& w1, const Opt& w2, const Opt& gate, int64_t kind,
+                      const Opt& scale, double scale_value, double eps) {
+  if (norm_residual_ok(R, Y, w1, w2, gate, kind, scale)) {
+    const c10::DeviceGuard guard(Y.device());
+    const int64_t n = Y.size(0), d = Y.size(1);
+    const Tensor none = empty({0}, Y);
+    Tensor out = empty({n, d}, R), X = w2 ? empty({n, d}, Y) : none, rho1 = w1 ? empty({n}, Y, at::kFloat) : none,
+           rho2 = w2 ? empty({n}, Y, at::kFloat) : none;
+    if (zmoe_norm_residual(raw(R), std::max(R.stride(0), d), code(R), raw(Y), std::max(Y.stride(0), d), code(Y), n, d,
+                           w1 ? raw(*w1) : nullptr, w2 ? raw(*w2) : nullptr, code(w1 ? *w1 : *w2),
+                           gate ? raw(*gate) : nullptr, (int)kind, kind == 3 ? std::max(gate->stride(0), d) : 0,
+                           gate ? code(*gate) : ZMOE_DTYPE_F32, scale ? ptr<const float>(*scale) : nullptr,
+                           (float)scale_value, (float)eps, raw(out), w2 ? raw(X) : nullptr,
+                           w1 ? ptr<float>(rho1) : nullptr, w2 ? ptr<float>(rho2) : nullptr, stream_of(Y)) == ZMOE_OK)
+      return {out, X, rho1, rho2};
+  }
+  static const auto op = general<Tensors(const Tensor&, const Tensor&, const Opt&, const Opt&, const Opt&, c10::SymInt,
+                                         const Opt&, double, double)>("zmoe::norm_residual");
+  return op.call(R, Y, w1, w2, gate, kind, scale, scale_value, eps);
+}
+
+Tensors norm_residual_backward(const Opt& dR_out, const Opt& dX, const Tensor& R, const Tensor& Y, const Opt& w1,
+                               const Opt& w2, const Opt& gate, int64_t kind, const Opt& scale, double scale_value,
+                               const Opt& rho1, const Opt& rho2) {
+  if (norm_residual_ok(R, Y, w1, w2, gate, kind, scale)) {
+    const int64_t n = Y.size(0), d = Y.size(1);
+    auto rstd = [&](const Opt& w, const Opt& r) {
+      return !w || (r && flat(*r, Y, at::kFloat) && r->numel() == n);
+    };
+    if ((!dR_out || (flat(*dR_out, Y, R.scalar_type()) && dR_out->sizes() == Y.sizes())) &&
+        (!dX || (w2 && flat(*dX, Y, Y.scalar_type()) && dX->sizes() == Y.sizes())) && rstd(w1, rho1) &&
+        rstd(w2, rho2)) {
+      const c10::DeviceGuard guard(Y.device());
+      const Tensor none = empty({0}, Y);
+      Tensor dR = empty({n, d}, R), dY = empty({n, d}, Y), dw1 = w1 ? empty(w1->sizes(), *w1) : none,
+             dw2 = w2 ? empty(w2->sizes(), *w2) : none, dg = gate ? empty(gate->sizes(), *gate) : none,
+             ds = scale ? empty(scale->sizes(), *scale) : none;
+      const size_t bytes = zmoe_norm_residual_backward_workspace_bytes(n, d);
+      Tensor ws = workspace(bytes, Y);
+      if (zmoe_norm_residual_backward(
+              dR_out ? raw(*dR_out) : nullptr, dX ? raw(*dX) : nullptr, raw(R), std::max(R.stride(0), d), code(R),
+              raw(Y), std::max(Y.stride(0), d), code(Y), n, d, w1 ? raw(*w1) : nullptr, w2 ? raw(*w2) : nullptr,
+              code(w1 ? *w1 : *w2), gate ? raw(*gate) : nullptr, (int)kind,
+              kind == 3 ? std::max(gate->stride(0), d) : 0, gate ? code(*gate) : ZMOE_DTYPE_F32,
+              scale ? ptr<const float>(*scale) : nullptr, (float)scale_value, w1 ? ptr<const float>(*rho1) : nullptr,
+              w2 ? ptr<const float>(*rho2) : nullptr, raw(dR), raw(dY), w1 ? raw(dw1) : nullptr,
+              w2 ? raw(dw2) : nullptr, gate ? raw(dg) : nullptr, scale ? ptr<float>(ds) : nullptr, raw(ws), bytes,
+              stream_of(Y)) == ZMOE_OK)
+        return {dR, dY, dw1, dw2, dg, ds};
+    }
+  }
+  static const auto op =
+      general<Tensors(const Opt&, const Opt&, const Tensor&, const Tensor&, const Opt&, const Opt&, const Opt&,
+                      c10::SymInt, const Opt&, double, const Opt&, const Opt&)>("zmoe::norm_residual_backward");
+  return op.call(dR_out, dX, R, Y, w1, w2, gate, kind, scale, scale_value, rho1, rho2);
+}
+
 // ------------------------------------------------------------------ mutating building blocks
 void rowwise_sum_product(const Tensor& out, const Tensor& A, const Tensor& B) {
   if (A.is_cuda() && known(A) && A.dim() == 3 && A.is_contiguous() && on(B, A) && known(B) && B.dim() == 2 &&
@@ -707,6 +933,22 @@ TORCH_LIBRARY(zmoe_eager, m) {
   ZMOE_EAGER(rmsnorm_rows, "(Tensor X, Tensor weight, float eps, Tensor? rows) -> Tensor[]");
   ZMOE_EAGER(rmsnorm_rows_backward,
              "(Tensor dY, Tensor X, Tensor? rows, Tensor rstd, Tensor weight) -> Tensor[]");
+  ZMOE_EAGER(fp8_quantize_rows, "(Tensor X, Tensor? rows, int row_div, Tensor? row_scale) -> Tensor[]");
+  ZMOE_EAGER(fp8_quantize_weight, "(Tensor W, bool transposed) -> Tensor[]");
+  ZMOE_EAGER(fp8_mm,
+             "(Tensor xq, Tensor xs, Tensor wq, Tensor ws, int K, Tensor? sorted_scattered_idxs, "
+             "Tensor? expert_offsets, int k, bool x_grouped, bool y_grouped, bool out_f32) -> Tensor");
+  ZMOE_EAGER(fp8_linear, "(Tensor x, Tensor wq, Tensor ws) -> Tensor");
+  ZMOE_EAGER(fp8_glu_mlp, "(Tensor x, Tensor w1q, Tensor w1s, Tensor w2q, Tensor w2s) -> Tensor");
+  ZMOE_EAGER(fp8_glu_experts,
+             "(Tensor x, Tensor gates, Tensor expert_idxs, Tensor w1q, Tensor w1s, Tensor w2q, Tensor w2s, "
+             "Tensor? residual, Tensor? out_rows, int out_total) -> Tensor[]");
+  ZMOE_EAGER(norm_residual,
+             "(Tensor R, Tensor Y, Tensor? w_post, Tensor? w_next, Tensor? gate, int gate_kind, Tensor? scale, "
+             "float scale_value, float eps) -> Tensor[]");
+  ZMOE_EAGER(norm_residual_backward,
+             "(Tensor? dR_out, Tensor? dX, Tensor R, Tensor Y, Tensor? w_post, Tensor? w_next, Tensor? gate, "
+             "int gate_kind, Tensor? scale, float scale_value, Tensor? rstd_post, Tensor? rstd_next) -> Tensor[]");
   ZMOE_EAGER(rowwise_sum_product, "(Tensor(a!) output, Tensor A, Tensor B) -> ()");
   ZMOE_EAGER(group,
              "(Tensor A, int K, int N, Tensor(a!) Y, Tensor? coeff, bool has_coeff, int fan_out, "

@@ -605,7 +605,12 @@ int quantize_checks(const char* name, int64_t n, int64_t K, int dtype) {
 
 using namespace zmoe;
 
-extern "C" int64_t zmoe_fp8_scale_pitch(int64_t K) { return K >= 1 ? scale_pitch(K) : 0; }
+extern "C" int zmoe_fp8_scale_pitch(int64_t K, int64_t* pitch) {
+  ZMOE_REQUIRE(K >= 1 && K < (1 << 30), ZMOE_ERR_SHAPE, "fp8_scale_pitch: K=%lld", (long long)K);
+  ZMOE_REQUIRE(pitch, ZMOE_ERR_NULL, "fp8_scale_pitch: null pointer");
+  *pitch = scale_pitch(K);
+  return ZMOE_OK;
+}
 
 extern "C" int zmoe_fp8_quantize_rows(const void* X, int64_t x_stride, int64_t x_rows, const int64_t* rows,
                                       int row_div, const float* row_scale, int64_t n, int64_t K, int dtype, void* Q,

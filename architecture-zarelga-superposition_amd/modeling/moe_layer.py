@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from scattermoe.mlp import GLUMLP, _records_graph
+from scattermoe.mlp import Fp8Module, GLUMLP, _records_graph
 from zmoe import functional as _zf
 from zmoe import library as _zl
 
@@ -186,6 +186,10 @@ class MoELayer(nn.Module):
         nn.init.normal_(self.routed_experts.experts.weight, mean=0.0, std=std)
         nn.init.normal_(self.routed_experts.output_experts.weight, mean=0.0, std=std)
 
+    def quantize_fp8(self) -> "Fp8MoELayer":
+        """A serving layer with the present expert weights in e4m3 (the gate as it is)."""
+        return Fp8MoELayer(self)
+
     def _fused_weights(self, x):
         """The layer's weights for _FusedMoELayer, or None where the module composition runs.
 
@@ -260,3 +264,34 @@ class MoELayer(nn.Module):
                                   pad=(unpad_indices, bsz * seq_len))
         topk_idx = pad_input(topk_idx.squeeze(0), unpad_indices, bsz, seq_len)
         return out.view(bsz, seq_len, -1), topk_idx
+
+
+class Fp8MoELayer(Fp8Module):
+    """``MoELayer`` for serving: the routed and the shared experts' weights in e4m3 with a power-of-two scale for each
+    128 x 128 block (``Fp8GLUMLP``, ``Fp8ExpertMLP``); the gate, routing and combine as in the layer. Same
+    arguments and results as ``MoELayer.forward``; no gradients."""
+
+    def __init__(self, layer: MoELayer):
+        super().__init__()
+        self.gate = MoEGate(layer.config)
+        self.gate.load_state_dict({n: t.clone() for n, t in layer.gate.state_dict().items()}, assign=True)
+        self.gate.requires_grad_(False)
+        self.shared_experts = layer.shared_experts.quantize_fp8()
+        self.routed_experts = layer.routed_experts.quantize_fp8()
+
+    def forward(self, hidden_states, unpad_indices=None, norm=None):
+        bsz, seq_len, h = hidden_states.shape
+        x = self._serve(hidden_states).reshape(bsz * seq_len, h)
+        with torch.no_grad():
+            if norm is not None:
+                x = _zf.rmsnorm_rows(hidden_states.reshape(bsz * seq_len, h), norm.weight, norm.eps,
+                                     rows=unpad_indices).to(x.dtype)
+            elif unpad_indices is not None:
+                x = index_first_axis(x, unpad_indices)
+            topk_idx, topk_weight = self.gate(x.unsqueeze(0).to(self.gate.weight.dtype))
+            pad = None if unpad_indices is None else (unpad_indices, bsz * seq_len)
+            out = self.routed_experts(x, topk_weight.squeeze(0), topk_idx.squeeze(0),
+                                      residual=self.shared_experts(x), pad=pad).view(bsz, seq_len, h)
+            if unpad_indices is None:
+                return out, topk_idx.view(bsz, seq_len, -1)
+            return out, pad_input(topk_idx.squeeze(0), unpad_indices, bsz, seq_len)

@@ -92,15 +92,15 @@ class GLUExpertsFunction(torch.autograd.Function):
 
 
 class MLP(nn.Module):
-    """Reference scattermoe/mlp.py:6-49 (non-GLU expert MLP)."""
+    """Reference scattermoe/mlp.py:6-49 (non-GLU expert MLP). ``fp8``: ``ParallelExperts``'."""
 
-    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, activation=None):
+    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, activation=None, fp8=False):
         super(MLP, self).__init__()
         self.num_experts = num_experts
         self.input_size = input_size
         self.hidden_size = hidden_size
-        self.experts = ParallelExperts(num_experts, input_size, hidden_size, bias=bias)
-        self.output_experts = ParallelExperts(num_experts, hidden_size, input_size, bias=bias)
+        self.experts = ParallelExperts(num_experts, input_size, hidden_size, bias=bias, fp8=fp8)
+        self.output_experts = ParallelExperts(num_experts, hidden_size, input_size, bias=bias, fp8=fp8)
         self.top_k = min(top_k, self.num_experts)
         self.activation = activation
 
@@ -122,24 +122,32 @@ class MLP(nn.Module):
 
 
 class GLUMLP(nn.Module):
-    """Reference scattermoe/mlp.py:51-95 (SwiGLU expert MLP)."""
+    """Reference scattermoe/mlp.py:51-95 (SwiGLU expert MLP). ``fp8``: trained with ``ParallelExperts``' 8-bit
+    products (the module composition); ``quantize_fp8`` makes a serving module of any of them."""
 
-    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, activation=nn.SiLU(), fused=True):
+    def __init__(self, input_size, hidden_size, num_experts, top_k, bias=False, activation=nn.SiLU(), fused=True,
+                 fp8=False):
         super(GLUMLP, self).__init__()
         self.num_experts = num_experts
         self.input_size = input_size
         self.hidden_size = hidden_size
-        self.experts = ParallelExperts(num_experts, input_size, 2 * hidden_size, bias=bias)
-        self.output_experts = ParallelExperts(num_experts, hidden_size, input_size, bias=bias)
+        self.experts = ParallelExperts(num_experts, input_size, 2 * hidden_size, bias=bias, fp8=fp8)
+        self.output_experts = ParallelExperts(num_experts, hidden_size, input_size, bias=bias, fp8=fp8)
         self.top_k = min(top_k, self.num_experts)
         self.activation = activation
         # The fused kernels implement SiLU-gated units without expert biases.
-        self.fused = fused and not bias and isinstance(activation, nn.SiLU)
+        self.fused = fused and not bias and not fp8 and isinstance(activation, nn.SiLU)
         # expert_offsets of the last forward's sort (device tensor; not module state)
         self.last_expert_offsets = None
 
     def extra_repr(self):
         return "k={}".format(self.top_k)
+
+    def quantize_fp8(self) -> "Fp8GLUMLP":
+        """A serving module with these experts' weights in e4m3 (the present values; no copy of them is kept)."""
+        if self.experts.bias is not None or not isinstance(self.activation, nn.SiLU):
+            raise ValueError("quantize_fp8: SiLU-gated experts without biases only")
+        return Fp8GLUMLP(self.experts.weight, self.output_experts.weight, self.top_k)
 
     def forward(self, x: torch.Tensor, expert_p: torch.Tensor, expert_idxs: torch.Tensor, residual=None, pad=None):
         """mlp.py:74-95. Two arguments beyond the reference signature (their defaults keep its
@@ -171,3 +179,68 @@ class GLUMLP(nn.Module):
             y = torch.zeros((int(total), y.size(-1)), dtype=y.dtype, device=y.device).index_copy(
                 0, rows, y.reshape(-1, y.size(-1)))
         return y
+
+
+def glu_weights_fp8(W1: torch.Tensor, W2: torch.Tensor):
+    """(w1q, w1s, w2q, w2s) of SwiGLU weights W1 [E, 2f, d] = [up; gate] and W2 [E, d, f]: W1's halves are
+    quantised as 2E weights [f, d], so that no 128 x 128 block holds rows of both."""
+    with torch.no_grad():
+        E, two_f, d = W1.shape
+        w1q, w1s = _zl.fp8_quantize_weight(W1.detach().reshape(2 * E, two_f // 2, d), False)
+        w2q, w2s = _zl.fp8_quantize_weight(W2.detach(), False)
+    return w1q, w1s, w2q, w2s
+
+
+class Fp8Module(nn.Module):
+    """Base of the serving modules: quantised weights as uint8 buffers, which module-wide dtype casts leave alone."""
+
+    def _hold(self, **tensors):
+        for name, t in tensors.items():
+            self.register_buffer(name, t.view(torch.uint8))
+
+    def _weights(self, *names):
+        """(values, scales) of each name."""
+        out = []
+        for n in names:
+            out += [getattr(self, n + "_values").view(torch.float8_e4m3fn), getattr(self, n + "_scales")]
+        return out
+
+    def _serve(self, x: torch.Tensor) -> torch.Tensor:
+        """x in the compute dtype; refused where its gradient would be asked for."""
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError(f"{type(self).__name__} serves only: it has no gradients (run it under torch.no_grad())")
+        return x.to(_compute_dtype(x))
+
+
+class Fp8GLUMLP(Fp8Module):
+    """``GLUMLP`` for serving, its weights in e4m3 with a power-of-two scale for each 128 x 128 block (``zmoe.fp8``).
+
+    The rows are quantised once per call; the first product's epilogue forms silu(gate) * up from its float32 sums and
+    quantises it, so the activations are never written in 16 bits. Same arguments and result as
+    ``GLUMLP.forward``; no gradients. Weights: ``W1`` [E, 2f, d], ``W2`` [E, d, f] on the device."""
+
+    def __init__(self, W1: torch.Tensor, W2: torch.Tensor, top_k: int):
+        super().__init__()
+        E, two_f, d = W1.shape
+        if W2.shape != (E, d, two_f // 2) or two_f % 2:
+            raise ValueError(f"Fp8GLUMLP: W1 [E, 2f, d] and W2 [E, d, f], got {tuple(W1.shape)} and {tuple(W2.shape)}")
+        self.num_experts, self.input_size, self.hidden_size, self.top_k = E, d, two_f // 2, top_k
+        w1q, w1s, w2q, w2s = glu_weights_fp8(W1, W2)
+        self._hold(w1_values=w1q, w1_scales=w1s, w2_values=w2q, w2_scales=w2s)
+        self.last_expert_offsets = None  # as GLUMLP's
+
+    def extra_repr(self):
+        return f"experts={self.num_experts}, d={self.input_size}, f={self.hidden_size}, k={self.top_k}"
+
+    def forward(self, x: torch.Tensor, expert_p: torch.Tensor, expert_idxs: torch.Tensor, residual=None, pad=None):
+        x_shape = x.size()
+        x = self._serve(x).reshape(-1, x_shape[-1])
+        if x.shape[1] != self.input_size:
+            raise ValueError(f"Fp8GLUMLP: rows of {self.input_size}, got {x.shape[1]}")
+        with torch.no_grad():
+            res = None if residual is None else residual.reshape(-1, x_shape[-1]).to(x.dtype)
+            rows, total = (None, 0) if pad is None else (pad[0], int(pad[1]))
+            y, self.last_expert_offsets = _zl.fp8_glu_experts(x, expert_p.reshape(x.shape[0], -1).float(),
+                                                              expert_idxs.reshape(x.shape[0], -1),
+                                                              *self._weights("w1", "w2"), res, rows, total)
+        return y if pad is not None else y.view(*x_shape[:-1], y.size(-1))

@@ -106,18 +106,83 @@ class ParallelLinear(torch.autograd.Function):
         return (d_input, d_weights, None, None, None, None, d_biases, d_gates, None, None)
 
 
+class Fp8ParallelLinear(torch.autograd.Function):
+    """``ParallelLinear`` with its products in e4m3 (``zmoe.fp8``): Y = Q(x) Q(W_e) for every sorted row; the input
+    grad is the product of the quantised grouped output grad (gate-weighted in float32, quantised unrounded) with
+    the same weights transposed; the weight and gate grads are ``ParallelLinear``'s, from the unquantised operands
+    and from Y. (x, expert_weights [E, K, N], k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates,
+    grouped_in, grouped_out, dx); ``dx``: an input grad will be asked for."""
+
+    @staticmethod
+    def forward(ctx, x, expert_weights, k: int, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates,
+                grouped_in: bool, grouped_out: bool, dx: bool):
+        K, f32 = x.size(1), x.dtype == torch.float32
+        wq, ws, *qt = _zl.fp8_quantize_weight(expert_weights.permute(0, 2, 1), dx)
+        xq, xs = _zl.fp8_quantize_rows(x, None, 1, None)
+        output = _zl.fp8_mm(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, grouped_in, grouped_out, f32)
+        expanded = None
+        if gates is not None:
+            expanded = output.view(gates.size(0), gates.size(1), output.size(-1))
+            output = _zl.combine(output, gates.float(), gates.size(1), None, None, 0)
+        ctx.save_for_backward(x, sorted_scattered_idxs, expert_offsets, gates, expanded, *qt)
+        ctx.k, ctx.grouped_in, ctx.grouped_out = k, grouped_in, grouped_out
+        ctx.w_dtype = expert_weights.dtype
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        x, ss, off, gates, expanded, *qt = ctx.saved_tensors
+        need_x, need_w, need_g = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[6]
+        k, f32 = ctx.k, x.dtype == torch.float32
+        grad_out = grad_out.to(x.dtype).contiguous()
+        d_gates = flat = None
+        fan = 1
+        if gates is not None:
+            if need_g:
+                d_gates = kernels.ops.rowwise_sum_product(expanded, grad_out, dtype=torch.float32).to(gates.dtype)
+            flat, fan = gates.float().flatten(), gates.size(1)
+        d_input = d_weights = None
+        if need_x:
+            gather = None if ctx.grouped_out else ss
+            gq, gs = _zl.fp8_quantize_rows(grad_out, gather, fan, flat)
+            d_input = _zl.fp8_mm(gq, gs, *qt, grad_out.size(1), ss, off, 1, True, ctx.grouped_in, f32)
+            if k > 1:
+                d_input = _zl.sum_k(d_input, k, None)
+        if need_w:
+            grouped = grad_out if ctx.grouped_out else kernels.ops.group(grad_out, ss, fan_out=fan, coeff=flat)
+            DWt = _zl.group_bwd_w(grouped, x, off, off.numel(), None if ctx.grouped_in else ss, k,
+                                  ctx.w_dtype == torch.float32 and not f32)
+            d_weights = DWt.to(ctx.w_dtype).permute(0, 2, 1)
+        return d_input, d_weights, None, None, None, None, d_gates, None, None, None
+
+
 def parallel_linear(inputs, expert_weights, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets,
-                    expert_biases=None, gates=None, grouped_in=False, grouped_out=False):
-    """Reference parallel_experts.py:137-147."""
+                    expert_biases=None, gates=None, grouped_in=False, grouped_out=False, fp8=False):
+    """Reference parallel_experts.py:137-147. ``fp8``: the products in e4m3 with a scale per block of 128
+    (``Fp8ParallelLinear``), the weights bfloat16 or float32, without biases."""
+    if fp8:
+        if expert_biases is not None:
+            raise ValueError("parallel_linear: fp8 products take no biases")
+        if gates is not None and grouped_out:
+            raise ValueError("parallel_linear: gates combine rows in slot order, not grouped ones")
+        if sorted_scattered_idxs.size(0) != inputs.size(0) * k:
+            raise ValueError("parallel_linear: one sorted index per input row and slot")
+        dx = torch.is_grad_enabled() and inputs.requires_grad
+        return Fp8ParallelLinear.apply(inputs, expert_weights, k, sorted_expert_idxs, sorted_scattered_idxs,
+                                       expert_offsets, gates, grouped_in, grouped_out, dx)
     return ParallelLinear.apply(inputs, expert_weights, k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets,
                                 expert_biases, gates, grouped_in, grouped_out)
 
 
 class ParallelExperts(nn.Module):
-    """Reference parallel_experts.py:149-183: weight [E, out, in], optional bias [E, out]."""
+    """Reference parallel_experts.py:149-183: weight [E, out, in], optional bias [E, out]. ``fp8``: products in
+    e4m3 with a scale per block of 128, the parameters unchanged (no bias)."""
 
-    def __init__(self, num_experts, input_size, output_size, bias=False) -> None:
+    def __init__(self, num_experts, input_size, output_size, bias=False, fp8=False) -> None:
         super().__init__()
+        if fp8 and bias:
+            raise ValueError("ParallelExperts: fp8 products take no biases")
+        self.fp8 = fp8
         self.weight = nn.Parameter(torch.empty(num_experts, output_size, input_size))
         if bias:
             self.bias = nn.Parameter(torch.empty(num_experts, output_size))
@@ -145,6 +210,10 @@ class ParallelExperts(nn.Module):
                 grouped_in=False, grouped_out=False):
         dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled() else inputs.dtype
         inputs = inputs.to(dtype)
+        if self.fp8:  # quantised straight from the parameter, whatever its type
+            return parallel_linear(inputs, self.weight.permute(0, 2, 1), k, sorted_expert_idxs, sorted_scattered_idxs,
+                                   expert_offsets, gates=gates, grouped_in=grouped_in, grouped_out=grouped_out,
+                                   fp8=True)
         bias = None if self.bias is None else self.bias.to(dtype)
         return parallel_linear(inputs, self.compute_weight(dtype).permute(0, 2, 1), k, sorted_expert_idxs,
                                sorted_scattered_idxs, expert_offsets, expert_biases=bias, gates=gates,

@@ -80,11 +80,16 @@ SIGNATURES = {
     "zmoe_rmsnorm_rows": (I32, [P, I64, I64, P, I64, I64, P, I32, F32, I32, P, P, P]),
     "zmoe_rmsnorm_rows_backward_workspace_bytes": (SZ, [I64, I64, I32]),
     "zmoe_rmsnorm_rows_backward": (I32, [P, P, I64, I64, P, I64, I64, P, P, I32, I32, P, I64, P, P, SZ, P]),
-    "zmoe_fp8_scale_pitch": (I64, [I64]),
+    "zmoe_fp8_scale_pitch": (I32, [I64, P]),
     "zmoe_fp8_quantize_rows": (I32, [P, I64, I64, P, I32, P, I64, I64, I32, P, P, P]),
     "zmoe_fp8_quantize_weight": (I32, [P, I64, I64, I64, I64, I64, I32, P, P, P, P, P]),
     "zmoe_fp8_scatter2scatter": (I32, [P, P, I64, P, P, P, P, I64, I64, I32, I32, I32, I32, I32, P, I64, P]),
     "zmoe_fp8_glu_w1_forward": (I32, [P, P, I64, P, P, P, P, I64, I64, I32, I32, P, P, P]),
+    "zmoe_norm_residual": (I32, [P, I64, I32, P, I64, I32, I64, I64, P, P, I32, P, I32, I64, I32, P, F32, F32, P, P, P,
+                                 P, P]),
+    "zmoe_norm_residual_backward_workspace_bytes": (SZ, [I64, I64]),
+    "zmoe_norm_residual_backward": (I32, [P, P, P, I64, I32, P, I64, I32, I64, I64, P, P, I32, P, I32, I64, I32, P, F32,
+                                          P, P, P, P, P, P, P, P, P, SZ, P]),
     "zmoe_newton_schulz5_workspace_bytes": (SZ, [I64, I64, I64]),
     "zmoe_newton_schulz5": (I32, [P, I64, I64, I64, I32, F32, F32, F32, P, SZ, P]),
 }

@@ -15,12 +15,14 @@ torch ops, as the reference does.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 import torch.nn.functional as F
 
 from . import library as zl
+from . import ops as _z
+from .fp8 import Fp8Weight
 
 
 def _fused(x, *ws) -> bool:
@@ -116,3 +118,133 @@ def rmsnorm_rows(hidden: torch.Tensor, weight: torch.Tensor, eps: float,
     flat = hidden.reshape(-1, d)
     y = _RMSNormRows.apply(flat, weight, float(eps), rows)
     return y.view(hidden.shape) if rows is None else y
+
+
+def _compute_dtype(x: torch.Tensor) -> torch.dtype:
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+
+
+def _needs_graph(*ts: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _Fp8Linear(torch.autograd.Function):
+    """Q(x) Q(W)^T for x [M, K], W [N, K]; the quantisers pass gradients through: dx = Q(dy) Q(W) (dy's
+    blocks run along N), dW = dy^T x from the unquantised operands."""
+
+    @staticmethod
+    def forward(ctx, x, W, dx: bool):
+        q = zl.fp8_quantize_weight(W, dx)
+        ctx.save_for_backward(x, *q[2:])
+        ctx.w_dtype, ctx.N = W.dtype, W.shape[0]
+        return zl.fp8_linear(x, q[0], q[1])
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, *qt = ctx.saved_tensors
+        dx = dW = None
+        if ctx.needs_input_grad[0]:
+            dx = zl.fp8_linear(dy, *qt)
+        if ctx.needs_input_grad[1]:
+            f32 = ctx.w_dtype == torch.float32 and x.dtype != torch.float32  # fp32 master weights
+            dW = zl.dense_wgrad(dy, x, f32).to(ctx.w_dtype)
+        return dx, dW, None
+
+
+class _Fp8LinearServed(torch.autograd.Function):
+    """The same with a weight that was quantised before and takes no gradient."""
+
+    @staticmethod
+    def forward(ctx, x, q, s, qt, st):
+        ctx.save_for_backward(qt, st)
+        return zl.fp8_linear(x, q, s)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return zl.fp8_linear(dy, *ctx.saved_tensors), None, None, None, None
+
+
+def fp8_linear(x: torch.Tensor, W: Union[torch.Tensor, Fp8Weight]) -> torch.Tensor:
+    """F.linear(x, W) in e4m3 with a power-of-two scale for each block of 128 (``zmoe.fp8``), x [..., K].
+
+    ``W``: a bfloat16 or float32 weight [N, K], quantised in the call, with gradients (of x by a product of the
+    quantised output grad, of W from the unquantised operands; float32 weights get float32 grads); or an
+    ``Fp8Weight``, quantised once (``fp8.quantize_weight``), which has a gradient for x only where it was made
+    with ``transposed=True``. The result has x's dtype (under autocast, autocast's)."""
+    x = x.to(_compute_dtype(x))
+    served = isinstance(W, Fp8Weight)
+    if len(W.shape) != 2 or x.dim() < 1 or x.shape[-1] != W.shape[1]:
+        raise ValueError(f"fp8_linear: x [..., K] and W [N, K], got {tuple(x.shape)} and {tuple(W.shape)}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if served:
+        if not _needs_graph(x):
+            with torch.no_grad():
+                y = zl.fp8_linear(x2, W.q, W.s)
+        elif W.qt is None:
+            raise RuntimeError("fp8_linear: the gradient of x needs a weight quantised with transposed=True")
+        else:
+            y = _Fp8LinearServed.apply(x2, W.q, W.s, W.qt, W.st)
+    else:
+        y = _Fp8Linear.apply(x2, W, _needs_graph(x))
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], W.shape[0])
+
+
+class _NormResidual(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, r, y, w_post, w_next, gate, kind: int, scale, scale_value: float, eps: float):
+        r_out, x, rho1, rho2 = zl.norm_residual(r, y, w_post, w_next, gate, kind, scale, scale_value, eps)
+        ctx.save_for_backward(r, y, w_post, w_next, gate, scale, rho1 if w_post is not None else None,
+                              rho2 if w_next is not None else None)
+        ctx.kind, ctx.scale_value = kind, scale_value
+        ctx.set_materialize_grads(False)
+        return r_out, x if w_next is not None else None
+
+    @staticmethod
+    def backward(ctx, dr_out, dx):
+        if dr_out is None and dx is None:
+            return (None,) * 9
+        r, y, w_post, w_next, gate, scale, rho1, rho2 = ctx.saved_tensors
+        cont = lambda g: None if g is None else g.contiguous()  # noqa: E731
+        dr, dy, dw1, dw2, dg, ds = zl.norm_residual_backward(cont(dr_out), cont(dx), r, y, w_post, w_next, gate,
+                                                             ctx.kind, scale, ctx.scale_value, rho1, rho2)
+        part = lambda t, g: None if t is None else g  # noqa: E731
+        return dr, dy, part(w_post, dw1), part(w_next, dw2), part(gate, dg), None, part(scale, ds), None, None
+
+
+def norm_residual(residual: torch.Tensor, y: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                  next_weight: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                  residual_scale: Union[None, float, torch.Tensor] = None, eps: float = 1e-6):
+    """The step from one sublayer to the next in one pass, for a residual stream and a sublayer's output y [..., d]:
+
+      r = residual_scale * residual + gate * norm(y; weight),   x = norm(r; next_weight)
+
+    with zero-centred RMSNorms (gain 1 + weight), either of which may be left out (not both). Returns (r, x), x
+    None without ``next_weight``; r in the residual's dtype, x in y's (bfloat16 or float32 each), both rounded once from
+    float32. ``gate``: [d] (a gain for each channel), [..., 1] (for each token), y's shape, or anything that
+    broadcasts to it. ``residual_scale``: a number, or a tensor of one element, which gets a gradient."""
+    if residual.shape != y.shape or y.dim() < 1:
+        raise ValueError(f"norm_residual: residual and y must have one shape, got {tuple(residual.shape)} and "
+                         f"{tuple(y.shape)}")
+    if weight is None and next_weight is None:
+        raise ValueError("norm_residual: neither weight nor next_weight given")
+    d = y.shape[-1]
+    if weight is not None and next_weight is not None and weight.dtype != next_weight.dtype:
+        weight, next_weight = weight.float(), next_weight.float()
+    kind = _z.GATE_NONE
+    if gate is not None:
+        if gate.shape == (d,):
+            kind = _z.GATE_CHANNEL
+        elif gate.shape == (*y.shape[:-1], 1) and d > 1:
+            kind, gate = _z.GATE_ROW, gate.reshape(-1)
+        else:
+            kind, gate = _z.GATE_FULL, gate.expand(y.shape).reshape(-1, d)
+    scale, value = None, 1.0
+    if isinstance(residual_scale, torch.Tensor):
+        if residual_scale.numel() != 1:
+            raise ValueError("norm_residual: residual_scale is one number")
+        scale = residual_scale.float()
+    elif residual_scale is not None:
+        value = float(residual_scale)
+    r, x = _NormResidual.apply(residual.reshape(-1, d), y.reshape(-1, d), weight, next_weight, gate, kind, scale, value,
+                               float(eps))
+    return r.view(residual.shape), None if x is None else x.view(y.shape)

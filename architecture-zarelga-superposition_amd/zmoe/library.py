@@ -436,3 +436,128 @@ def rmsnorm_rows_backward(dY: torch.Tensor, X: torch.Tensor, rows: Optional[torc
 @rmsnorm_rows_backward.register_fake
 def _(dY, X, rows, rstd, weight):
     return [_empty(X.shape, X), _empty(weight.shape, weight)]
+
+
+# ------------------------------------------------------------------ e4m3 with a scale per block of 128
+_E4M3 = torch.float8_e4m3fn
+
+
+def _fp8_rows(n, K, like):
+    return [_empty((n, _z.fp8_width(K)), like, _E4M3), _empty((n, _z.fp8_scale_pitch(K)), like, torch.uint8)]
+
+
+@layer_op("fp8_quantize_rows")
+def fp8_quantize_rows(X: torch.Tensor, rows: Optional[torch.Tensor], row_div: int,
+                      row_scale: Optional[torch.Tensor]) -> List[torch.Tensor]:
+    """[q, s] of X's rows (or of X[rows // row_div] * row_scale[rows])."""
+    return list(_z.fp8_quantize_rows(X, rows, row_div, row_scale))
+
+
+@fp8_quantize_rows.register_fake
+def _(X, rows, row_div, row_scale):
+    return _fp8_rows(X.shape[0] if rows is None else rows.numel(), X.shape[1], X)
+
+
+@layer_op("fp8_quantize_weight")
+def fp8_quantize_weight(W: torch.Tensor, transposed: bool) -> List[torch.Tensor]:
+    """[q, s] of W [..., N, K], with ``transposed`` [q, s, qt, st]."""
+    return list(_z.fp8_quantize_weight(W, transposed))
+
+
+@fp8_quantize_weight.register_fake
+def _(W, transposed):
+    lead, (N, K) = W.shape[:-2], W.shape[-2:]
+    new = lambda n, k: [_empty((*lead, n, _z.fp8_width(k)), W, _E4M3),  # noqa: E731
+                        _empty((*lead, -(-n // _z.FP8_BLOCK), _z.fp8_scale_pitch(k)), W, torch.uint8)]
+    return new(N, K) + (new(K, N) if transposed else [])
+
+
+@layer_op("fp8_mm")
+def fp8_mm(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, K: int,
+           sorted_scattered_idxs: Optional[torch.Tensor], expert_offsets: Optional[torch.Tensor], k: int,
+           x_grouped: bool, y_grouped: bool, out_f32: bool) -> torch.Tensor:
+    """Product of quantised rows and weights, grouped by expert or (no offsets) dense."""
+    return _z.fp8_scatter2scatter(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped, y_grouped,
+                                  torch.float32 if out_f32 else torch.bfloat16)
+
+
+@fp8_mm.register_fake
+def _(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped, y_grouped, out_f32):
+    R = xq.shape[0] if x_grouped else xq.shape[0] * k
+    return _empty((R, wq.shape[-2]), xq, _F32 if out_f32 else torch.bfloat16)
+
+
+@layer_op("fp8_linear")
+def fp8_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor) -> torch.Tensor:
+    """x [M, K] quantised, times a quantised weight [N, Kp]: [M, N] of x's dtype."""
+    return _z.fp8_linear(x, wq, ws)
+
+
+@fp8_linear.register_fake
+def _(x, wq, ws):
+    return _empty((x.shape[0], wq.shape[0]), x)
+
+
+@layer_op("fp8_glu_mlp")
+def fp8_glu_mlp(x: torch.Tensor, w1q: torch.Tensor, w1s: torch.Tensor, w2q: torch.Tensor,
+                w2s: torch.Tensor) -> torch.Tensor:
+    """One dense SwiGLU expert on quantised weights: [M, d]."""
+    return _z.fp8_glu_mlp(x, w1q, w1s, w2q, w2s)
+
+
+@fp8_glu_mlp.register_fake
+def _(x, w1q, w1s, w2q, w2s):
+    return _empty(x.shape, x)
+
+
+@layer_op("fp8_glu_experts")
+def fp8_glu_experts(x: torch.Tensor, gates: torch.Tensor, expert_idxs: torch.Tensor, w1q: torch.Tensor,
+                    w1s: torch.Tensor, w2q: torch.Tensor, w2s: torch.Tensor, residual: Optional[torch.Tensor],
+                    out_rows: Optional[torch.Tensor], out_total: int) -> List[torch.Tensor]:
+    """[out, expert_offsets] of SwiGLU experts on quantised weights; ``residual`` and ``out_rows`` as combine's."""
+    return list(_z.fp8_glu_experts(x, gates, expert_idxs, w1q, w1s, w2q, w2s, residual, out_rows,
+                                   out_total if out_rows is not None else None))
+
+
+@fp8_glu_experts.register_fake
+def _(x, gates, expert_idxs, w1q, w1s, w2q, w2s, residual, out_rows, out_total):
+    rows = out_total if out_rows is not None else x.shape[0]
+    return [_empty((rows, x.shape[1]), x), _empty((w2q.shape[0],), x, _I64)]
+
+
+# ------------------------------------------------------------------ the step between two sublayers
+def _or_none(t: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
+    return _empty((0,), like) if t is None else t  # (an op returns no None)
+
+
+@layer_op("norm_residual")
+def norm_residual(R: torch.Tensor, Y: torch.Tensor, w_post: Optional[torch.Tensor], w_next: Optional[torch.Tensor],
+                  gate: Optional[torch.Tensor], gate_kind: int, scale: Optional[torch.Tensor], scale_value: float,
+                  eps: float) -> List[torch.Tensor]:
+    """[R_out, X, rstd_post, rstd_next] of ``zmoe.ops.norm_residual``, empty where there is none."""
+    return [_or_none(t, Y) for t in _z.norm_residual(R, Y, w_post, w_next, gate, gate_kind, scale, scale_value, eps)]
+
+
+@norm_residual.register_fake
+def _(R, Y, w_post, w_next, gate, gate_kind, scale, scale_value, eps):
+    none, n = _empty((0,), Y), Y.shape[0]
+    return [_empty(R.shape, R), none if w_next is None else _empty(Y.shape, Y),
+            none.clone() if w_post is None else _empty((n,), Y, _F32),
+            none.clone() if w_next is None else _empty((n,), Y, _F32)]
+
+
+@layer_op("norm_residual_backward")
+def norm_residual_backward(dR_out: Optional[torch.Tensor], dX: Optional[torch.Tensor], R: torch.Tensor,
+                           Y: torch.Tensor, w_post: Optional[torch.Tensor], w_next: Optional[torch.Tensor],
+                           gate: Optional[torch.Tensor], gate_kind: int, scale: Optional[torch.Tensor],
+                           scale_value: float, rstd_post: Optional[torch.Tensor],
+                           rstd_next: Optional[torch.Tensor]) -> List[torch.Tensor]:
+    """[dR, dY, dw_post, dw_next, dgate, dscale], empty where there is none."""
+    return [_or_none(t, Y) for t in _z.norm_residual_backward(dR_out, dX, R, Y, w_post, w_next, gate, gate_kind, scale,
+                                                              scale_value, rstd_post, rstd_next)]
+
+
+@norm_residual_backward.register_fake
+def _(dR_out, dX, R, Y, w_post, w_next, gate, gate_kind, scale, scale_value, rstd_post, rstd_next):
+    like = lambda t: _empty((0,), Y) if t is None else _empty(t.shape, t)  # noqa: E731
+    return [_empty(R.shape, R), _empty(Y.shape, Y), like(w_post), like(w_next), like(gate), like(scale)]

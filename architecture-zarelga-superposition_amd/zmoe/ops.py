@@ -55,6 +55,20 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 else t.contiguous()
 
 
+def _rows_apart(t: torch.Tensor) -> torch.Tensor:
+    """``_rows`` whose rows do not overlap (an expanded tensor is copied)."""
+    t = _rows(t)
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """``_rows``, contiguous from a 16-byte boundary where its rows do not all start on one."""
+    t = _rows(t)
+    if t.data_ptr() % 16 or t.stride(0) * t.element_size() % 16:
+        return t.contiguous() if not t.is_contiguous() else t.clone() if t.data_ptr() % 16 else t
+    return t
+
+
 def _on16(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous from a 16-byte boundary (a copy where it is not: a view into a flat buffer)."""
     t = t.contiguous()
@@ -405,12 +419,15 @@ def dense_wgrad(DY: torch.Tensor, X: torch.Tensor, splits: Optional[int] = None,
     """DW [N, K] = DY[M, N]^T X[M, K]: the weight grad of an nn.Linear (F.linear backward);
     ``out_dtype`` float32 with bf16 operands writes the fp32 sum unrounded."""
     dev = _require_cuda(DY, X)
-    DY = _rows(DY)
-    X = _rows(X)
+    DY = _rows16(DY)
+    X = _rows16(X)
     if DY.dtype != X.dtype or DY.shape[0] != X.shape[0]:
         raise ValueError("dense_wgrad: DY and X must share dtype and row count")
     M, N = DY.shape
     K = X.shape[1]
+    if not (_aligned(N, DY.dtype) and _aligned(K, DY.dtype)):  # unaligned widths: padded copies
+        DWp = dense_wgrad(_pad_cols(DY, _up(N, DY.dtype)), _pad_cols(X, _up(K, X.dtype)), splits, out_dtype=out_dtype)
+        return copy_pad(DWp, N, K, out) if out is None or _plain_out(out, DWp, (N, K)) else out.copy_(DWp[:N, :K])
     if splits is None:
         splits = dense_wgrad_splits(M, N, K)
     od = _wgrad_out_dtype(DY, out_dtype, "dense_wgrad")
@@ -835,7 +852,7 @@ def fp8_quantize_rows(X: torch.Tensor, rows: Optional[torch.Tensor] = None, row_
     """(q, s) of the rows of X [M, K] (any width and row stride); with ``rows`` (int64) row i is
     X[rows[i] // row_div], with ``row_scale`` (f32) times row_scale[rows[i]]."""
     dev = _require_cuda(X, rows, row_scale)
-    X = _rows(X)
+    X = _rows_apart(X)
     M, K = X.shape
     r = None if rows is None else _idx64(rows)
     n = M if r is None else r.numel()
@@ -936,6 +953,111 @@ def fp8_glu_w1_forward(xq: torch.Tensor, xs: torch.Tensor, w1q: torch.Tensor, w1
         L.call("zmoe_fp8_glu_w1_forward", _ptr(xq), _ptr(xs), T, _ptr(w1q), _ptr(w1s), _ptr(ss), _ptr(off), d, f, E, k,
                _ptr(aq), _ptr(as_), _stream(dev))
     return aq, as_
+
+
+GATE_NONE, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3
+
+
+def _norm_residual_operands(R, Y, w_post, w_next, gate, gate_kind, scale, what):
+    dev = _require_cuda(R, Y, w_post, w_next, gate, scale)
+    R, Y = _rows_apart(R), _rows_apart(Y)
+    n, d = Y.shape
+    ws = [None if w is None else w.reshape(-1).contiguous() for w in (w_post, w_next)]
+    if R.shape != (n, d) or any(w is not None and w.numel() != d for w in ws):
+        raise ValueError(f"{what}: residual and rows must be [n, d], the weights [d]")
+    if ws[0] is not None and ws[1] is not None and ws[0].dtype != ws[1].dtype:
+        raise ValueError(f"{what}: the weights' dtypes differ")
+    want = {GATE_NONE: None, GATE_CHANNEL: (d,), GATE_ROW: (n,), GATE_FULL: (n, d)}[gate_kind]
+    if (gate is None) != (want is None) or (gate is not None and tuple(gate.shape) != want):
+        raise ValueError(f"{what}: the gate does not have the shape of its kind")
+    if gate is not None:
+        gate = _rows_apart(gate) if gate_kind == GATE_FULL else gate.contiguous()
+    if scale is not None and (scale.numel() != 1 or scale.dtype != torch.float32):
+        raise ValueError(f"{what}: the residual scale is one float32")
+    w = ws[0] if ws[0] is not None else ws[1]
+    if w is None:
+        raise ValueError(f"{what}: neither norm's weight given")
+    # (a tensor of one row or none may have any row stride)
+    stride = lambda t: max(t.stride(0), d)  # noqa: E731
+    args = (_ptr(R), stride(R), _dtype_code(R), _ptr(Y), stride(Y), _dtype_code(Y), n, d, _ptr(ws[0]), _ptr(ws[1]),
+            _dtype_code(w), _ptr(gate), gate_kind, stride(gate) if gate_kind == GATE_FULL else 0,
+            _dtype_code(gate) if gate is not None else L.DTYPE_F32, _ptr(scale))
+    return dev, (R, Y, ws, gate), args
+
+
+def norm_residual(R: torch.Tensor, Y: torch.Tensor, w_post: Optional[torch.Tensor], w_next: Optional[torch.Tensor],
+                  gate: Optional[torch.Tensor], gate_kind: int, scale: Optional[torch.Tensor], scale_value: float,
+                  eps: float):
+    """scale R + gate norm_post(Y) and its norm_next, over rows [n, d] (zmoe_norm_residual): (R_out, X or None,
+    rstd_post or None, rstd_next or None). ``scale``: a float32 tensor of one element, or None: ``scale_value``."""
+    dev, keep, args = _norm_residual_operands(R, Y, w_post, w_next, gate, gate_kind, scale, "norm_residual")
+    n, d = Y.shape
+    new = lambda on, *a: torch.empty(*a, device=dev) if on is not None else None  # noqa: E731
+    R_out = torch.empty((n, d), dtype=R.dtype, device=dev)
+    X = None if w_next is None else torch.empty((n, d), dtype=Y.dtype, device=dev)
+    rho1, rho2 = new(w_post, n), new(w_next, n)
+    with profiling.region("norm_residual", dev):
+        L.call("zmoe_norm_residual", *args, float(scale_value), float(eps), _ptr(R_out), _ptr(X), _ptr(rho1),
+               _ptr(rho2), _stream(dev))
+    del keep
+    return R_out, X, rho1, rho2
+
+
+def norm_residual_backward(dR_out: Optional[torch.Tensor], dX: Optional[torch.Tensor], R: torch.Tensor,
+                           Y: torch.Tensor, w_post: Optional[torch.Tensor], w_next: Optional[torch.Tensor],
+                           gate: Optional[torch.Tensor], gate_kind: int, scale: Optional[torch.Tensor],
+                           scale_value: float, rstd_post: Optional[torch.Tensor], rstd_next: Optional[torch.Tensor]):
+    """Backward of ``norm_residual``: (dR, dY, dw_post, dw_next, dgate, dscale), None for what was not given."""
+    dev, keep, args = _norm_residual_operands(R, Y, w_post, w_next, gate, gate_kind, scale, "norm_residual_backward")
+    _require_cuda(R, dR_out, dX, rstd_post, rstd_next)
+    n, d = Y.shape
+    for g, like in ((dR_out, R), (dX, Y)):
+        if g is not None and g.shape != (n, d):
+            raise ValueError("norm_residual_backward: the output grads must be [n, d]")
+    dR_out = None if dR_out is None else dR_out.to(R.dtype).contiguous()
+    dX = None if dX is None else dX.to(Y.dtype).contiguous()
+    for w, r in ((w_post, rstd_post), (w_next, rstd_next)):
+        if w is not None and (r is None or r.numel() != n or r.dtype != torch.float32 or not r.is_contiguous()):
+            raise ValueError("norm_residual_backward: rstd must be [n] float32")
+    dR, dY = (torch.empty((n, d), dtype=t.dtype, device=dev) for t in (R, Y))
+    dw1, dw2 = (None if w is None else torch.empty(d, dtype=w.dtype, device=dev) for w in (w_post, w_next))
+    dgate = None if gate is None else torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    dscale = None if scale is None else torch.empty(1, dtype=torch.float32, device=dev)
+    nbytes = L.load().zmoe_norm_residual_backward_workspace_bytes(n, d)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    with profiling.region("norm_residual_backward", dev):
+        L.call("zmoe_norm_residual_backward", _ptr(dR_out), _ptr(dX), *args, float(scale_value), _ptr(rstd_post),
+               _ptr(rstd_next), _ptr(dR), _ptr(dY), _ptr(dw1), _ptr(dw2), _ptr(dgate), _ptr(dscale), _ptr(ws),
+               ws.numel(), _stream(dev))
+    del keep
+    return (dR, dY, None if dw1 is None else dw1.view(w_post.shape), None if dw2 is None else dw2.view(w_next.shape),
+            dgate, None if dscale is None else dscale.view(scale.shape))
+
+
+# Whole fp8 paths in one call each (the host's share of a small batch's time is one op's).
+def fp8_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor) -> torch.Tensor:
+    """x [M, K] times a quantised weight wq [N, Kp]: [M, N] of x's dtype; x's rows are quantised first."""
+    return fp8_scatter2scatter(*fp8_quantize_rows(x), wq, ws, x.shape[1], out_dtype=x.dtype)
+
+
+def fp8_glu_mlp(x: torch.Tensor, w1q: torch.Tensor, w1s: torch.Tensor, w2q: torch.Tensor,
+                w2s: torch.Tensor) -> torch.Tensor:
+    """One dense SwiGLU expert: x [M, d], w1q [2, f, dp] (up, gate), w2q [d, fp] -> [M, d] of x's dtype."""
+    aq, as_ = fp8_glu_w1_forward(*fp8_quantize_rows(x), w1q, w1s, x.shape[1])
+    return fp8_scatter2scatter(aq, as_, w2q, w2s, w1q.shape[1], out_dtype=x.dtype)
+
+
+def fp8_glu_experts(x: torch.Tensor, gates: torch.Tensor, expert_idxs: torch.Tensor, w1q: torch.Tensor,
+                    w1s: torch.Tensor, w2q: torch.Tensor, w2s: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                    out_rows: Optional[torch.Tensor] = None, out_total: Optional[int] = None):
+    """SwiGLU experts on given routing (gates and ids [T, k]): (out as ``combine``'s, expert_offsets)."""
+    E, (T, k) = w2q.shape[0], expert_idxs.shape
+    if x.dim() != 2 or x.shape[0] != T or gates.numel() != T * k:
+        raise ValueError("fp8_glu_experts: x [T, d] with gates and expert ids [T, k]")
+    se, ss, off, _ = flatten_sort_count(expert_idxs, E)
+    aq, as_ = fp8_glu_w1_forward(*fp8_quantize_rows(x), w1q, w1s, x.shape[1], ss, off, k)
+    Y = fp8_scatter2scatter(aq, as_, w2q, w2s, w1q.shape[1], ss, off, 1, True, False, x.dtype)
+    return combine(Y, gates, k, residual, out_rows, out_total), off
 
 
 NS_COEFFS = (3.4445, -4.7750, 2.0315)  # optimizer/muon.py:16

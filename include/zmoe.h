@@ -438,10 +438,10 @@ int zmoe_newton_schulz5(void* X, int64_t E, int64_t m, int64_t n, int steps, flo
  *   for which max |v| <= 448 s (over the finite values), q = v / s rounded to e4m3 (nearest, ties to
  *   even); inf and NaN become e4m3's NaN. Scales are bytes c + 127 (E8M0).
  * Layout: K values take Kp = 128 ceil(K / 128) bytes (zeros past K), their scales
- * zmoe_fp8_scale_pitch(K) bytes (a multiple of 4, one byte a block). Rows lie one after the other. Values start on 16
+ * 4 ceil(K / 512) bytes (one byte a block; zmoe_fp8_scale_pitch). Rows lie one after the other. Values start on 16
  * bytes, scales on 4.
  * ------------------------------------------------------------------------- */
-int64_t zmoe_fp8_scale_pitch(int64_t K);
+int zmoe_fp8_scale_pitch(int64_t K, int64_t* pitch);
 
 /* Q [n, Kp], S [n, pitch] of rows of X [x_rows, K] (F32 or BF16, rows x_stride elements apart): row i is X[i], or
  * with rows (int64 [n]) X[rows[i] / row_div] (zeros for an index out of range); with row_scale (f32) times
@@ -470,6 +470,31 @@ int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const vo
 int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T, const void* W1q, const void* W1s,
                             const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t d, int64_t f,
                             int E, int k, void* Aq, void* As, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The step between two sublayers: the norm after the first, its gate, the scaled residual and the
+ * norm in front of the second (both norms zero-centred as zmoe_rmsnorm_rows), over rows of d <= 32768:
+ *   u = Y rsqrt(mean(Y^2) + eps) (1 + w_post)   (u = Y without w_post)
+ *   R_out = scale R + gate u,   X = R_out rsqrt(mean(R_out^2) + eps) (1 + w_next)   (no X without w_next)
+ * in f32, one rounding each (X from the unrounded R_out). R, R_out: r_dtype; Y, X: y_dtype; w_post and w_next: w_dtype,
+ * at least one of them. gate_kind: 0 none, 1 [d], 2 [n], 3 [n, d] (rows gate_stride elements apart). scale: *scale_ptr
+ * (f32 on the device) or, where that is NULL, the value `scale`. rstd_post, rstd_next [n] f32 (may be NULL): what the
+ * backward takes. Outputs and gradients lie packed.
+ * ------------------------------------------------------------------------- */
+int zmoe_norm_residual(const void* R, int64_t r_stride, int r_dtype, const void* Y, int64_t y_stride, int y_dtype,
+                       int64_t n, int64_t d, const void* w_post, const void* w_next, int w_dtype, const void* gate,
+                       int gate_kind, int64_t gate_stride, int gate_dtype, const float* scale_ptr, float scale,
+                       float eps, void* R_out, void* X, float* rstd_post, float* rstd_next, void* stream);
+
+/* Its gradient from dR_out and dX (either may be NULL: zeros). dR, dY are written; dw_post, dw_next (w_dtype), dgate
+ * (the gate's shape and type) and dscale (f32) where given; sums over rows in a fixed order. */
+size_t zmoe_norm_residual_backward_workspace_bytes(int64_t n, int64_t d);
+int zmoe_norm_residual_backward(const void* dR_out, const void* dX, const void* R, int64_t r_stride, int r_dtype,
+                                const void* Y, int64_t y_stride, int y_dtype, int64_t n, int64_t d, const void* w_post,
+                                const void* w_next, int w_dtype, const void* gate, int gate_kind, int64_t gate_stride,
+                                int gate_dtype, const float* scale_ptr, float scale, const float* rstd_post,
+                                const float* rstd_next, void* dR, void* dY, void* dw_post, void* dw_next, void* dgate,
+                                float* dscale, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
