@@ -53,6 +53,8 @@ bool flat(const Tensor& t, const Tensor& like, at::ScalarType dt) {
 bool rows2(const Tensor& t, const Tensor& like) {
   return on(t, like) && t.scalar_type() == like.scalar_type() && t.dim() == 2 && t.stride(1) == 1;
 }
+// rows2 whose rows do not overlap (expanded tensors go to the general form).
+bool apart(const Tensor& t) { return rows2(t, t) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
 bool index(const Tensor& t, const Tensor& like, int64_t n) { return flat(t, like, at::kLong) && t.numel() == n; }
 
 Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType dt) {
@@ -317,7 +319,7 @@ Tensor glu_w2_backward_dh(const Tensor& dY, const Tensor& W2, const Tensor& H, c
 // dW [E, N, K] (and the bias grad [E, N] when given); false where the general form has to run.
 bool wgrad_into(const Tensor& DY, const Tensor& X, const Tensor& off, int64_t E, const Opt& gather, int64_t div,
                 const Tensor& dW, const Opt& db) {
-  if (!(DY.is_cuda() && known(DY) && rows2(DY, DY) && rows2(X, DY) && index(off, DY, E) && fits_int(E) &&
+  if (!(DY.is_cuda() && known(DY) && apart(DY) && rows2(X, DY) && apart(X) && index(off, DY, E) && fits_int(E) &&
         fits_int(div) && (gather ? index(*gather, DY, DY.size(0)) : X.size(0) == DY.size(0))))
     return false;
   const int64_t N = DY.size(1), K = X.size(1), Np = up(N, DY), Kp = up(K, X);
@@ -378,9 +380,17 @@ Tensor group_bwd_w_gather_dy(const Tensor& DY, const Tensor& gather, int64_t div
 }
 
 Tensor dense_wgrad(const Tensor& DY, const Tensor& X, bool out_f32) {
-  if (DY.is_cuda() && known(DY) && rows2(DY, DY) && rows2(X, DY) && X.size(0) == DY.size(0)) {
+  if (DY.is_cuda() && known(DY) && apart(DY) && rows2(X, DY) && apart(X) && X.size(0) == DY.size(0)) {
     const c10::DeviceGuard guard(DY.device());
     const int64_t M = DY.size(0), N = DY.size(1), K = X.size(1);
+    if (const int64_t Np = up(N, DY), Kp = up(K, X); Np != N || Kp != K) {
+      const Tensor DYp = padded(DY, M, Np), Xp = padded(X, M, Kp);
+      if (DYp.defined() && Xp.defined()) {
+        const Tensor full = dense_wgrad(DYp, Xp, out_f32);
+        Tensor dW = empty({N, K}, full);
+        if (copy_pad_into(full, dW)) return dW;
+      }
+    }
     int splits = 0;
     if (zmoe_dense_wgrad_splits(M, N, K, 256, &splits) == ZMOE_OK) {
       Tensor dW = empty({N, K}, DY, wgrad_dtype(DY, out_f32));
@@ -605,9 +615,6 @@ Tensors rmsnorm_rows_backward(const Tensor& dY, const Tensor& X, const Opt& rows
 int64_t width8(int64_t K) { return (K + 127) / 128 * 128; }
 int64_t blocks8(int64_t n) { return (n + 127) / 128; }
 int64_t pitch8(int64_t K) { return (K + 511) / 512 * 4; }  // zmoe_fp8_scale_pitch
-
-// rows2 whose rows do not overlap (expanded tensors go to the general form).
-bool apart(const Tensor& t) { return rows2(t, t) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
 
 struct Rows8 {
   Tensor q, s;
@@ -845,7 +852,7 @@ void rowwise_sum_product(const Tensor& out, const Tensor& A, const Tensor& B) {
 bool group_into(const Tensor& A, const Tensor& Y, const Opt& coeff, bool has_coeff, int64_t fan_out,
                 const Tensor& idx) {
   const bool use = has_coeff && coeff;
-  if (A.is_cuda() && known(A) && rows2(A, A) && fan_out > 0 && fits_int(fan_out) &&
+  if (A.is_cuda() && known(A) && apart(A) && fan_out > 0 && fits_int(fan_out) &&
       index(idx, A, A.size(0) * fan_out) && rows2(Y, A) && Y.size(0) == idx.numel() && Y.size(1) == A.size(1) &&
       (!use || (on(*coeff, A) && known(*coeff) && coeff->is_contiguous() && coeff->numel() == idx.numel()))) {
     const c10::DeviceGuard guard(A.device());

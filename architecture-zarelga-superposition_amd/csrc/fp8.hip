@@ -710,11 +710,11 @@ extern "C" int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t 
                "fp8_scatter2scatter: rows must be below 2^31");
   ZMOE_REQUIRE(expert_offsets || (E == 1 && x_grouped && y_grouped), ZMOE_ERR_NULL,
                "fp8_scatter2scatter: no expert_offsets only for one weight and rows in order");
-  ZMOE_REQUIRE((x_grouped && y_grouped) || sorted_scattered_idxs, ZMOE_ERR_NULL,
-               "fp8_scatter2scatter: sorted_scattered_idxs required unless x_grouped and y_grouped");
   ZMOE_REQUIRE(y_stride >= N, ZMOE_ERR_SHAPE, "fp8_scatter2scatter: row stride of Y");
   const int64_t R = x_grouped ? M : M * k;
   if (R == 0) return ZMOE_OK;
+  ZMOE_REQUIRE((x_grouped && y_grouped) || sorted_scattered_idxs, ZMOE_ERR_NULL,
+               "fp8_scatter2scatter: sorted_scattered_idxs required unless x_grouped and y_grouped");
   ZMOE_REQUIRE(Y, ZMOE_ERR_NULL, "fp8_scatter2scatter: null pointer");
   ZMOE_REQUIRE((reinterpret_cast<uintptr_t>(Y) % dtype_size(out_dtype)) == 0, ZMOE_ERR_ALIGN,
                "fp8_scatter2scatter: Y's alignment");
@@ -740,10 +740,10 @@ extern "C" int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T
   ZMOE_REQUIRE(T >= 0 && d >= 1 && f >= 1 && d < (1 << 30) && f < (1 << 29) && E >= 1 && E <= kGemmMaxE && k >= 1,
                ZMOE_ERR_SHAPE, "fp8_glu_w1_forward: bad sizes");
   ZMOE_REQUIRE(T < kMaxRows8 && T * k < kMaxRows8, ZMOE_ERR_SHAPE, "fp8_glu_w1_forward: T*k must be below 2^31");
-  ZMOE_REQUIRE(expert_offsets ? sorted_scattered_idxs != nullptr : (E == 1 && k == 1), ZMOE_ERR_NULL,
-               "fp8_glu_w1_forward: no expert_offsets only for one weight, else sorted_scattered_idxs too");
   const int64_t R = T * k;
   if (R == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(expert_offsets ? sorted_scattered_idxs != nullptr : (E == 1 && k == 1), ZMOE_ERR_NULL,
+               "fp8_glu_w1_forward: no expert_offsets only for one weight, else sorted_scattered_idxs too");
   ZMOE_REQUIRE(Aq && As, ZMOE_ERR_NULL, "fp8_glu_w1_forward: null pointer");
   ZMOE_REQUIRE(aligned16(Aq) && aligned4(As), ZMOE_ERR_ALIGN, "fp8_glu_w1_forward: values on 16, scales on 4 bytes");
   Fp8Params p{};

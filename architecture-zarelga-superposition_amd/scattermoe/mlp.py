@@ -240,7 +240,8 @@ class Fp8GLUMLP(Fp8Module):
         with torch.no_grad():
             res = None if residual is None else residual.reshape(-1, x_shape[-1]).to(x.dtype)
             rows, total = (None, 0) if pad is None else (pad[0], int(pad[1]))
-            y, self.last_expert_offsets = _zl.fp8_glu_experts(x, expert_p.reshape(x.shape[0], -1).float(),
-                                                              expert_idxs.reshape(x.shape[0], -1),
+            k = expert_idxs.shape[-1]
+            y, self.last_expert_offsets = _zl.fp8_glu_experts(x, expert_p.reshape(-1, k).float(),
+                                                              expert_idxs.reshape(-1, k).long(),
                                                               *self._weights("w1", "w2"), res, rows, total)
         return y if pad is not None else y.view(*x_shape[:-1], y.size(-1))

@@ -10,6 +10,7 @@ import torch
 import torch.nn as nn
 
 from zmoe import library as _zl
+from zmoe.functional import rows_on_16
 from zmoe import ops as _z
 
 from . import kernels
@@ -134,7 +135,7 @@ class Fp8ParallelLinear(torch.autograd.Function):
         x, ss, off, gates, expanded, *qt = ctx.saved_tensors
         need_x, need_w, need_g = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[6]
         k, f32 = ctx.k, x.dtype == torch.float32
-        grad_out = grad_out.to(x.dtype).contiguous()
+        grad_out = rows_on_16(grad_out.to(x.dtype).contiguous())
         d_gates = flat = None
         fan = 1
         if gates is not None:
@@ -150,7 +151,7 @@ class Fp8ParallelLinear(torch.autograd.Function):
                 d_input = _zl.sum_k(d_input, k, None)
         if need_w:
             grouped = grad_out if ctx.grouped_out else kernels.ops.group(grad_out, ss, fan_out=fan, coeff=flat)
-            DWt = _zl.group_bwd_w(grouped, x, off, off.numel(), None if ctx.grouped_in else ss, k,
+            DWt = _zl.group_bwd_w(grouped, rows_on_16(x), off, off.numel(), None if ctx.grouped_in else ss, k,
                                   ctx.w_dtype == torch.float32 and not f32)
             d_weights = DWt.to(ctx.w_dtype).permute(0, 2, 1)
         return d_input, d_weights, None, None, None, None, d_gates, None, None, None

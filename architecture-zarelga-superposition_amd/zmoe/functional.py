@@ -128,6 +128,19 @@ def _needs_graph(*ts: Optional[torch.Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
+def rows_on_16(t: torch.Tensor) -> torch.Tensor:
+    """Rows [n, c] as the weight-grad kernels take them: unit column stride, no two rows overlapping and, where c is
+    a whole number of 16-byte chunks, every row on 16 bytes (other widths go through padded copies); else a copy.
+    (A tracer knows no storage offsets: there the rows are only made contiguous.)"""
+    if torch.compiler.is_compiling():
+        return t.contiguous()
+    size = t.element_size()
+    ok = t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+    if ok and (t.shape[1] * size) % 16 == 0:
+        ok = (t.storage_offset() * size) % 16 == 0 and (t.stride(0) * size) % 16 == 0
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
 class _Fp8Linear(torch.autograd.Function):
     """Q(x) Q(W)^T for x [M, K], W [N, K]; the quantisers pass gradients through: dx = Q(dy) Q(W) (dy's
     blocks run along N), dW = dy^T x from the unquantised operands."""
@@ -147,7 +160,7 @@ class _Fp8Linear(torch.autograd.Function):
             dx = zl.fp8_linear(dy, *qt)
         if ctx.needs_input_grad[1]:
             f32 = ctx.w_dtype == torch.float32 and x.dtype != torch.float32  # fp32 master weights
-            dW = zl.dense_wgrad(dy, x, f32).to(ctx.w_dtype)
+            dW = zl.dense_wgrad(rows_on_16(dy), rows_on_16(x), f32).to(ctx.w_dtype)
         return dx, dW, None
 
 

@@ -61,14 +61,6 @@ def _rows_apart(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """``_rows``, contiguous from a 16-byte boundary where its rows do not all start on one."""
-    t = _rows(t)
-    if t.data_ptr() % 16 or t.stride(0) * t.element_size() % 16:
-        return t.contiguous() if not t.is_contiguous() else t.clone() if t.data_ptr() % 16 else t
-    return t
-
-
 def _on16(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous from a 16-byte boundary (a copy where it is not: a view into a flat buffer)."""
     t = t.contiguous()
@@ -254,7 +246,7 @@ def group(A: torch.Tensor, sorted_idxs: torch.Tensor, coeff: Optional[torch.Tens
           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """scattermoe/kernels/ops.py:449-458: Y[n] = A[idx[n] // fan_out] * coeff[idx[n]]."""
     dev = _require_cuda(A, sorted_idxs, coeff, out)
-    A = _rows(A)
+    A = _rows_apart(A)
     if not _aligned(A.shape[1], A.dtype):  # unaligned width: through a padded copy
         Kp = _up(A.shape[1], A.dtype)
         return _unpad_into(group(_pad_cols(A, Kp), sorted_idxs, coeff, fan_out), A.shape[1], out)
@@ -342,8 +334,8 @@ def group_bwd_w(DY: torch.Tensor, X: torch.Tensor, expert_offsets: torch.Tensor,
     float32 with bf16 operands: DWt unrounded from the fp32 accumulators (no bias grad).
     """
     dev = _require_cuda(DY, X, expert_offsets, x_gather)
-    DY = _rows(DY)
-    X = _rows(X)
+    DY = _rows_apart(DY)
+    X = _rows_apart(X)
     if DY.dtype != X.dtype:
         raise ValueError("group_bwd_w: DY and X dtypes differ")
     M, N = DY.shape
@@ -419,8 +411,8 @@ def dense_wgrad(DY: torch.Tensor, X: torch.Tensor, splits: Optional[int] = None,
     """DW [N, K] = DY[M, N]^T X[M, K]: the weight grad of an nn.Linear (F.linear backward);
     ``out_dtype`` float32 with bf16 operands writes the fp32 sum unrounded."""
     dev = _require_cuda(DY, X)
-    DY = _rows16(DY)
-    X = _rows16(X)
+    DY = _rows_apart(DY)
+    X = _rows_apart(X)
     if DY.dtype != X.dtype or DY.shape[0] != X.shape[0]:
         raise ValueError("dense_wgrad: DY and X must share dtype and row count")
     M, N = DY.shape
