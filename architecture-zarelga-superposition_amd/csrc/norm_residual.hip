@@ -13,12 +13,11 @@
 // Both passes are bound by HBM. A row belongs to the fewest waves that hold it at eight elements a
 // thread (one wave up to d = 512, four at 2048, sixteen at 8192; above, more elements a thread): few
 // registers, so several workgroups share a CU and one's loads fill the other's row sums and barriers.
-// The backward walks rows with a fixed grid and loads its next row before it reduces the current one;
-// the sums over rows stay in registers until the end, then go through per-block partials added in a
-// fixed order (the same result on every run).
+// The backward walks rows with a fixed grid; the sums over rows go through per-block partials added in
+// a fixed order (the same result on every run).
 #include <type_traits>
 
-#include "zmoe_internal.h"
+#include "zmoe_tiles.h"
 
 namespace zmoe {
 namespace {
@@ -30,42 +29,53 @@ constexpr int kMaxPartials = 512;
 
 enum Gate { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_FULL = 3 };
 
-// A parameter or gate tensor of either type (its type is uniform in a launch: one scalar branch).
+// A parameter, gate or gate grad of either type (uniform in a launch: one scalar branch).
 struct Vec {
   const void* p;
-  int bf16, vec;
+  int bf16;
 };
 struct Out {
   void* p;
-  int bf16, vec;
+  int bf16;
 };
 
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* __restrict__ row, int64_t c, int64_t d, bool vec, float (&v)[kVN]) {
+// Chunk c .. c + 7 of a row of d elements (zeros past it). VEC: d is a multiple of 8 and every row starts on
+// 16 bytes, so a chunk is whole or absent; else element by element.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_chunk(const T* __restrict__ row, int64_t c, int64_t d, float (&v)[kVN]) {
   constexpr int VC = 16 / sizeof(T);
-  if (vec && c + kVN <= d) {
+  if constexpr (VEC) {
+    if (c < d) {
 #pragma unroll
-    for (int q = 0; q < kVN / VC; ++q) unpack_chunk(*reinterpret_cast<const uint4*>(row + c + q * VC), &v[q * VC], T{});
+      for (int q = 0; q < kVN / VC; ++q)
+        unpack_chunk(*reinterpret_cast<const uint4*>(row + c + q * VC), &v[q * VC], T{});
+    } else {
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) v[u] = 0.f;
+    }
   } else {
 #pragma unroll
     for (int u = 0; u < kVN; ++u) v[u] = c + u < d ? to_f32(row[c + u]) : 0.f;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* __restrict__ row, int64_t c, int64_t d, bool vec, const float (&v)[kVN]) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_chunk(T* __restrict__ row, int64_t c, int64_t d, const float (&v)[kVN]) {
   constexpr int VC = 16 / sizeof(T);
-  if (vec && c + kVN <= d) {
+  if constexpr (VEC) {
+    if (c < d) {
 #pragma unroll
-    for (int q = 0; q < kVN / VC; ++q) *reinterpret_cast<uint4*>(row + c + q * VC) = pack_chunk(&v[q * VC], T{});
+      for (int q = 0; q < kVN / VC; ++q) *reinterpret_cast<uint4*>(row + c + q * VC) = pack_chunk(&v[q * VC], T{});
+    }
   } else {
 #pragma unroll
     for (int u = 0; u < kVN; ++u)
       if (c + u < d) row[c + u] = from_f32<T>(v[u]);
   }
 }
+template <bool VEC>
 __device__ __forceinline__ void load_vec(const Vec& w, int64_t at, int64_t c, int64_t d, float (&v)[kVN]) {
-  if (w.bf16) load_chunk(static_cast<const uint16_t*>(w.p) + at, c, d, w.vec != 0, v);
-  else load_chunk(static_cast<const float*>(w.p) + at, c, d, w.vec != 0, v);
+  if (w.bf16) load_chunk<VEC>(static_cast<const uint16_t*>(w.p) + at, c, d, v);
+  else load_chunk<VEC>(static_cast<const float*>(w.p) + at, c, d, v);
 }
 __device__ __forceinline__ float load_one(const Vec& w, int64_t i) {
   return w.bf16 ? to_f32(static_cast<const uint16_t*>(w.p)[i]) : static_cast<const float*>(w.p)[i];
@@ -78,10 +88,21 @@ __device__ __forceinline__ void store_one(const Out& o, int64_t i, float v) {
 // Sums of v[0 .. N - 1] over the threads of a row, W waves, in every one of them. With W > 1 every
 // thread of the block calls it; consecutive calls alternate `slot` (one barrier a call: a slot's
 // values are read before the call after the next one writes it).
+__device__ __forceinline__ float lanes_sum(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  v += dpp(v, std::integral_constant<int, 0xB1>{});   // lane ^ 1
+  v += dpp(v, std::integral_constant<int, 0x4E>{});   // lane ^ 2
+  v += dpp(v, std::integral_constant<int, 0x141>{});  // 7 - lane within 8
+  v += dpp(v, std::integral_constant<int, 0x140>{});  // 15 - lane within 16
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
 template <int W, int N, int WPB>
 __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[WPB][2], int slot) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum(v[i]);
   if constexpr (W > 1) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) {
@@ -103,7 +124,6 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[WPB][2], in
 struct NormArgs {
   const void *r, *y;
   int64_t ldr, ldy, n, d;
-  int vec;  // r, y, outputs and grads take 16-byte accesses
   Vec w1, w2, gate;
   int gate_kind;
   int64_t ldg;
@@ -118,16 +138,19 @@ struct NormArgs {
   float* partial; // [3][P][d] sums for w1, w2 and a channel gate, then [P] for alpha
 };
 
-template <int W>
+// TH: the fewest threads of a block.
+template <int W, int TH = 256>
 struct Map {
   static constexpr int TPR = 64 * W;
-  static constexpr int THREADS = TPR < 256 ? 256 : TPR;
+  static constexpr int THREADS = TPR < TH ? TH : TPR;
   static constexpr int WPB = THREADS / 64, RPB = THREADS / TPR;
 };
+template <int W>
+using FwdMap = Map<W, 256>;
 
-template <typename R, typename Y, int W, int NQ>
-__global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_kernel(NormArgs a) {
-  using M = Map<W>;
+template <typename R, typename Y, int W, int NQ, bool VEC>
+__global__ __launch_bounds__(FwdMap<W>::THREADS) void norm_residual_kernel(NormArgs a) {
+  using M = FwdMap<W>;
   __shared__ float red[2][M::WPB][2];
   const int64_t i = (int64_t)blockIdx.x * M::RPB + threadIdx.x / M::TPR;
   const bool live = i < a.n;  // (every thread stays for the barriers)
@@ -140,10 +163,10 @@ __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_kernel(NormArgs
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     const int64_t c = (int64_t)(lt + q * M::TPR) * kVN, dd = live ? a.d : 0;
-    load_chunk(static_cast<const Y*>(a.y) + row * a.ldy, c, dd, a.vec != 0, y[q]);
-    load_chunk(static_cast<const R*>(a.r) + row * a.ldr, c, dd, a.vec != 0, h[q]);
-    if (a.gate_kind == GATE_FULL) load_vec(a.gate, row * a.ldg, c, dd, g[q]);
-    else if (a.gate_kind == GATE_CHANNEL) load_vec(a.gate, 0, c, a.d, g[q]);
+    load_chunk<VEC>(static_cast<const Y*>(a.y) + row * a.ldy, c, dd, y[q]);
+    load_chunk<VEC>(static_cast<const R*>(a.r) + row * a.ldr, c, dd, h[q]);
+    if (a.gate_kind == GATE_FULL) load_vec<VEC>(a.gate, row * a.ldg, c, dd, g[q]);
+    else if (a.gate_kind == GATE_CHANNEL) load_vec<VEC>(a.gate, 0, c, a.d, g[q]);
 #pragma unroll
     for (int u = 0; u < kVN; ++u) s[0] = fmaf(y[q][u], y[q][u], s[0]);
   }
@@ -159,7 +182,7 @@ __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_kernel(NormArgs
   for (int q = 0; q < NQ; ++q) {
     const int64_t c = (int64_t)(lt + q * M::TPR) * kVN;
     float w[kVN];
-    if (a.w1.p) load_vec(a.w1, 0, c, a.d, w);
+    if (a.w1.p) load_vec<VEC>(a.w1, 0, c, a.d, w);
 #pragma unroll
     for (int u = 0; u < kVN; ++u) {
       float v = y[q][u];
@@ -169,7 +192,7 @@ __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_kernel(NormArgs
       h[q][u] = fmaf(alpha, h[q][u], v);
       s[0] = fmaf(h[q][u], h[q][u], s[0]);
     }
-    if (live) store_chunk(static_cast<R*>(a.r_out) + i * a.d, c, a.d, a.vec != 0, h[q]);
+    if (live) store_chunk<VEC>(static_cast<R*>(a.r_out) + i * a.d, c, a.d, h[q]);
   }
   if (!a.x) return;  // uniform
   row_sums<W, 1, M::WPB>(s, red, 1);
@@ -180,122 +203,244 @@ __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_kernel(NormArgs
   for (int q = 0; q < NQ; ++q) {
     const int64_t c = (int64_t)(lt + q * M::TPR) * kVN;
     float w[kVN];
-    load_vec(a.w2, 0, c, a.d, w);
+    load_vec<VEC>(a.w2, 0, c, a.d, w);
 #pragma unroll
     for (int u = 0; u < kVN; ++u) h[q][u] = h[q][u] * rho2 * (1.f + w[u]);
-    store_chunk(static_cast<Y*>(a.x) + i * a.d, c, a.d, a.vec != 0, h[q]);
+    store_chunk<VEC>(static_cast<Y*>(a.x) + i * a.d, c, a.d, h[q]);
   }
 }
 
-// One row's operands in the backward.
-template <typename R, typename Y, int NQ>
-struct Row {
-  float r[NQ][kVN], y[NQ][kVN], gr[NQ][kVN], gx[NQ][kVN];
-  float rho1, rho2;
-  template <int TPR>
-  __device__ __forceinline__ void load(const NormArgs& a, int64_t i, int lt) {
-    const bool live = i < a.n;
-    const int64_t row = live ? i : 0, dd = live ? a.d : 0;
-    rho1 = live && a.w1.p ? a.rho1[row] : 1.f;
-    rho2 = live && a.w2.p ? a.rho2[row] : 0.f;
+// This block's part of the residual scale's grad.
+template <int WPB>
+__device__ __forceinline__ void block_alpha(const NormArgs& a, float v, float (*red)[WPB][2]) {
+  if (!a.alpha_ptr) return;
+  __syncthreads();
+  v = wave_sum(v);
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6][0] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float all = 0.f;
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int64_t c = (int64_t)(lt + q * TPR) * kVN;
-      load_chunk(static_cast<const Y*>(a.y) + row * a.ldy, c, dd, a.vec != 0, y[q]);
-      load_chunk(static_cast<const R*>(a.r) + row * a.ldr, c, dd, a.vec != 0, r[q]);
-      load_chunk(static_cast<const R*>(a.gr) + row * a.d, c, a.gr ? dd : 0, a.vec != 0, gr[q]);
-      load_chunk(static_cast<const Y*>(a.gx) + row * a.d, c, a.gx ? dd : 0, a.vec != 0, gx[q]);
+    for (int q = 0; q < WPB; ++q) all += red[0][q][0];
+    a.partial[3 * (int64_t)gridDim.x * a.d + blockIdx.x] = all;
+  }
+}
+
+// A chunk as it was loaded: 16 (bf16) or 32 bytes.
+template <typename T, bool VEC>
+struct Chunk {
+  uint4 w[kVN * sizeof(T) / 16];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int64_t c, int64_t d) {
+    constexpr int VC = 16 / sizeof(T);
+    if constexpr (VEC) {
+#pragma unroll
+      for (int q = 0; q < kVN / VC; ++q)
+        w[q] = c < d ? *reinterpret_cast<const uint4*>(row + c + q * VC) : make_uint4(0, 0, 0, 0);
+    } else {
+      float v[kVN];
+      load_chunk<false>(row, c, d, v);
+#pragma unroll
+      for (int q = 0; q < kVN / VC; ++q) w[q] = pack_chunk(&v[q * VC], T{});
     }
+  }
+  // What is formed from the chunk before this is formed again after it, not kept in registers.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (uint4& q : w) asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w));
+  }
+  __device__ __forceinline__ void get(float (&v)[kVN]) const {
+    constexpr int VC = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < kVN / VC; ++q) unpack_chunk(w[q], &v[q * VC], T{});
   }
 };
 
-template <typename R, typename Y, int W, int NQ>
+// A chunk of a full gate of either type, as it was loaded.
+template <bool VEC>
+struct GateChunk {
+  Chunk<uint16_t, VEC> h;
+  Chunk<float, VEC> f;
+  int bf16;
+  __device__ __forceinline__ void load(const Vec& g, int64_t at, int64_t c, int64_t d) {
+    bf16 = g.bf16;
+    if (bf16) h.load(static_cast<const uint16_t*>(g.p) + at, c, d);
+    else f.load(static_cast<const float*>(g.p) + at, c, d);
+  }
+  __device__ __forceinline__ void forget() {
+    if (bf16) h.forget();
+    else f.forget();
+  }
+  __device__ __forceinline__ void get(float (&v)[kVN]) const {
+    if (bf16) h.get(v);
+    else f.get(v);
+  }
+};
+
+// One row's operands in the backward: this thread's chunk of each.
+template <typename R, typename Y, bool VEC>
+struct Row {
+  Chunk<R, VEC> r, gr;
+  Chunk<Y, VEC> y, gx;
+  float rho1, rho2, g_row;
+  __device__ __forceinline__ void load(const NormArgs& a, int64_t i, int64_t c) {
+    const bool live = i < a.n;
+    const int64_t row = live ? i : 0, dd = live ? a.d : 0;
+    rho1 = live && a.w1.p ? a.rho1[row] : 1.f;  // (no norm of y: u = y)
+    rho2 = live && a.w2.p ? a.rho2[row] : 0.f;  // (no next norm: nothing through x)
+    g_row = live && a.gate_kind == GATE_ROW ? load_one(a.gate, row) : 1.f;
+    y.load(static_cast<const Y*>(a.y) + row * a.ldy, c, dd);
+    r.load(static_cast<const R*>(a.r) + row * a.ldr, c, dd);
+    gr.load(static_cast<const R*>(a.gr) + row * a.d, c, a.gr ? dd : 0);
+    gx.load(static_cast<const Y*>(a.gx) + row * a.d, c, a.gx ? dd : 0);
+  }
+};
+
+// 1 + w (1 without a weight) of a chunk.
+template <bool VEC>
+__device__ __forceinline__ void load_gain(const Vec& w, int64_t c, int64_t d, float (&v)[kVN]) {
+  if (w.p) load_vec<VEC>(w, 0, c, d, v);
+#pragma unroll
+  for (int u = 0; u < kVN; ++u) v[u] = w.p ? 1.f + v[u] : 1.f;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_gate(const Out& o, int64_t at, int64_t c, int64_t d, const float (&v)[kVN]) {
+  if (o.bf16) store_chunk<VEC>(static_cast<uint16_t*>(o.p) + at, c, d, v);
+  else store_chunk<VEC>(static_cast<float*>(o.p) + at, c, d, v);
+}
+
+// One chunk a thread (d <= 8192). Up to eight waves a row the three sums over rows live in registers; sixteen waves
+// have 128 registers a thread and one workgroup a CU, so there the sums are in LDS (each thread its own
+// columns: 24 bytes an element of the row against 18 to 12 from HBM at a tenth of LDS's rate) and the
+// next row's operands are loaded before this one is worked on.
+template <typename R, typename Y, int W, bool VEC, bool FULL>
 __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_backward_kernel(NormArgs a) {
   using M = Map<W>;
+  constexpr bool LDS_SUMS = W == kMaxWaves, PREFETCH = false;
   __shared__ float red[2][M::WPB][2];
-  extern __shared__ float fold[];  // [RPB][d] (several rows a block)
+  extern __shared__ __align__(16) float fold[];  // [RPB][d] (several rows a block), or the sums [3][8 TPR]
   const int lt = threadIdx.x % M::TPR, sub = threadIdx.x / M::TPR;
+  const int64_t c = (int64_t)lt * kVN;
   const float alpha = a.alpha_ptr ? *a.alpha_ptr : a.alpha;
   const float inv_d = 1.0f / (float)a.d;
-  float w1[NQ][kVN], w2[NQ][kVN], gc[NQ][kVN], acc1[NQ][kVN], acc2[NQ][kVN], accg[NQ][kVN];
+  float w1[kVN], w2[kVN], gc[kVN], acc1[kVN], acc2[kVN], accg[kVN];
   float acc_alpha = 0.f;
 #pragma unroll
-  for (int q = 0; q < NQ; ++q) {
-    const int64_t c = (int64_t)(lt + q * M::TPR) * kVN;
-#pragma unroll
-    for (int u = 0; u < kVN; ++u) w1[q][u] = w2[q][u] = acc1[q][u] = acc2[q][u] = accg[q][u] = 0.f;
-    if (a.w1.p) load_vec(a.w1, 0, c, a.d, w1[q]);
-    if (a.w2.p) load_vec(a.w2, 0, c, a.d, w2[q]);
-    if (a.gate_kind == GATE_CHANNEL) load_vec(a.gate, 0, c, a.d, gc[q]);
+  for (int u = 0; u < kVN; ++u) {
+    acc1[u] = acc2[u] = accg[u] = 0.f;
+    gc[u] = 1.f;
   }
+  auto params = [&] {
+    load_gain<VEC>(a.w1, c, a.d, w1);
+    load_gain<VEC>(a.w2, c, a.d, w2);
+    if (a.gate_kind == GATE_CHANNEL) load_vec<VEC>(a.gate, 0, c, a.d, gc);
+  };
+  float4* sums = reinterpret_cast<float4*>(fold) + lt;  // this thread's: vector k, half h at (2 k + h) TPR
+  if constexpr (LDS_SUMS) {
+#pragma unroll
+    for (int k = 0; k < 6; ++k) sums[k * M::TPR] = make_float4(0.f, 0.f, 0.f, 0.f);
+  } else {
+    params();
+  }
+  // v added to this thread's part of sum k in LDS
+  auto add = [&](int k, float (&v)[kVN]) {
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      float4 o = sums[(2 * k + hh) * M::TPR];
+      o.x += v[4 * hh];
+      o.y += v[4 * hh + 1];
+      o.z += v[4 * hh + 2];
+      o.w += v[4 * hh + 3];
+      sums[(2 * k + hh) * M::TPR] = o;
+    }
+#pragma unroll
+    for (int u = 0; u < kVN; ++u) v[u] = 0.f;
+  };
   const int64_t first = (int64_t)blockIdx.x * M::RPB, step = (int64_t)gridDim.x * M::RPB;
-  Row<R, Y, NQ> cur, nxt;
-  constexpr bool PREFETCH = NQ == 1;  // (more chunks a thread: no registers for the next row)
-  cur.template load<M::TPR>(a, first + sub, lt);
+  Row<R, Y, VEC> cur, nxt;
+  GateChunk<VEC> gate;  // FULL: this row's gate
+  if constexpr (PREFETCH) cur.load(a, first + sub, c);
   for (int64_t base = first; base < a.n; base += step) {  // uniform in the block
     const int64_t i = base + sub;
     const bool live = i < a.n;
-    if constexpr (PREFETCH) nxt.template load<M::TPR>(a, i + step, lt);
-    const float g_row = a.gate_kind == GATE_ROW && live ? load_one(a.gate, i) : 1.f;
-    float g[NQ][kVN], uu[NQ][kVN], h[NQ][kVN];
-    float s[1] = {0.f};
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int64_t c = (int64_t)(lt + q * M::TPR) * kVN;
-      if (a.gate_kind == GATE_FULL) load_vec(a.gate, (live ? i : 0) * a.ldg, c, live ? a.d : 0, g[q]);
+    if constexpr (PREFETCH) nxt.load(a, i + step, c);
+    else cur.load(a, i, c);
+    if constexpr (LDS_SUMS) params();
+    if constexpr (FULL) gate.load(a.gate, (live ? i : 0) * a.ldg, c, live ? a.d : 0);
+    const float rho1 = cur.rho1, rho2 = cur.rho2, g_row = FULL ? 1.f : cur.g_row;
+    // y rho1, u and r' of this chunk
+    auto values = [&](float (&yh)[kVN], float (&uu)[kVN], float (&r)[kVN], float (&h)[kVN]) {
+      cur.y.get(yh);
+      cur.r.get(r);
+      if constexpr (FULL) gate.get(gc);
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
-        if (a.gate_kind == GATE_CHANNEL) g[q][u] = gc[q][u];
-        else if (a.gate_kind != GATE_FULL) g[q][u] = g_row;
-        uu[q][u] = a.w1.p ? cur.y[q][u] * cur.rho1 * (1.f + w1[q][u]) : cur.y[q][u];
-        h[q][u] = fmaf(alpha, cur.r[q][u], g[q][u] * uu[q][u]);
-        s[0] = fmaf(cur.gx[q][u] * (1.f + w2[q][u]), h[q][u], s[0]);
-        acc2[q][u] = fmaf(cur.gx[q][u] * cur.rho2, h[q][u], acc2[q][u]);
+        yh[u] *= rho1;
+        uu[u] = yh[u] * w1[u];
+        h[u] = fmaf(gc[u] * g_row, uu[u], alpha * r[u]);
       }
+    };
+    float s[1] = {0.f};
+    {
+      float yh[kVN], uu[kVN], r[kVN], h[kVN], gx[kVN];
+      values(yh, uu, r, h);
+      cur.gx.get(gx);
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) {
+        acc2[u] = fmaf(gx[u], rho2 * h[u], acc2[u]);
+        s[0] = fmaf(gx[u] * w2[u], h[u], s[0]);
+      }
+      if (LDS_SUMS && a.w2.p) add(1, acc2);
     }
     float coef2 = 0.f;
     if (a.gx) {
       row_sums<W, 1, M::WPB>(s, red, 0);
-      coef2 = cur.rho2 * cur.rho2 * cur.rho2 * s[0] * inv_d;
+      coef2 = rho2 * rho2 * rho2 * s[0] * inv_d;
     }
-    float s2[2] = {0.f, 0.f};  // du (1 + w1) y, t u
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int64_t c = (int64_t)(lt + q * M::TPR) * kVN;
-      float out[kVN];
+    cur.y.forget();
+    cur.r.forget();
+    cur.gx.forget();
+    if constexpr (FULL) gate.forget();
+    if constexpr (LDS_SUMS) params();
+    float s2[2] = {0.f, 0.f};  // du (1 + w1) y rho1, t u
+    float h[kVN];              // du (1 + w1) after this
+    {
+      float yh[kVN], uu[kVN], r[kVN], gx[kVN], t[kVN];
+      values(yh, uu, r, h);
+      cur.gx.get(gx);
+      cur.gr.get(t);
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
-        const float t = cur.gr[q][u] + cur.rho2 * (1.f + w2[q][u]) * cur.gx[q][u] - h[q][u] * coef2;
-        out[u] = alpha * t;
-        acc_alpha = fmaf(t, cur.r[q][u], acc_alpha);
-        const float du = g[q][u] * t, tu = t * uu[q][u];
-        s2[0] = fmaf(du * (1.f + w1[q][u]), cur.y[q][u], s2[0]);
-        s2[1] += tu;
-        accg[q][u] += tu;
-        acc1[q][u] = fmaf(du * cur.rho1, cur.y[q][u], acc1[q][u]);
-        h[q][u] = du;  // (r' is not needed any more)
-        uu[q][u] = tu;
+        t[u] = fmaf(-coef2, h[u], fmaf(rho2, gx[u] * w2[u], t[u]));
+        acc_alpha = fmaf(t[u], r[u], acc_alpha);
+        uu[u] *= t[u];
+        s2[1] += uu[u];
+        accg[u] += uu[u];
+        h[u] = gc[u] * g_row * t[u];
+        acc1[u] = fmaf(h[u], yh[u], acc1[u]);
+        h[u] *= w1[u];
+        s2[0] = fmaf(h[u], yh[u], s2[0]);
+        t[u] *= alpha;
       }
-      if (live) store_chunk(static_cast<R*>(a.dr) + i * a.d, c, a.d, a.vec != 0, out);
-      if (live && a.gate_kind == GATE_FULL && a.dgate.p) {
-        if (a.dgate.bf16) store_chunk(static_cast<uint16_t*>(a.dgate.p) + i * a.d, c, a.d, a.dgate.vec != 0, uu[q]);
-        else store_chunk(static_cast<float*>(a.dgate.p) + i * a.d, c, a.d, a.dgate.vec != 0, uu[q]);
+      if (live) {
+        store_chunk<VEC>(static_cast<R*>(a.dr) + i * a.d, c, a.d, t);
+        if (FULL && a.dgate.p) store_gate<VEC>(a.dgate, i * a.d, c, a.d, uu);
       }
+      if (LDS_SUMS && a.w1.p) add(0, acc1);
+      if (LDS_SUMS && a.gate_kind == GATE_CHANNEL) add(2, accg);
     }
     if (a.w1.p || a.gate_kind == GATE_ROW) row_sums<W, 2, M::WPB>(s2, red, 1);
+    cur.y.forget();
     if (live && a.gate_kind == GATE_ROW && a.dgate.p && lt == 0) store_one(a.dgate, i, s2[1]);
-    const float coef1 = cur.rho1 * cur.rho1 * cur.rho1 * s2[0] * inv_d;
+    const float coef1 = a.w1.p ? rho1 * s2[0] * inv_d : 0.f;  // (rho1^3 y s = rho1 (y rho1) (s rho1))
+    if (live) {
+      float yh[kVN];
+      cur.y.get(yh);
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      const int64_t c = (int64_t)(lt + q * M::TPR) * kVN;
-      if (a.w1.p) {
-#pragma unroll
-        for (int u = 0; u < kVN; ++u) h[q][u] = cur.rho1 * (1.f + w1[q][u]) * h[q][u] - cur.y[q][u] * coef1;
-      }
-      if (live) store_chunk(static_cast<Y*>(a.dy) + i * a.d, c, a.d, a.vec != 0, h[q]);
+      for (int u = 0; u < kVN; ++u) h[u] = fmaf(-coef1, yh[u] * rho1, rho1 * h[u]);
+      store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, c, a.d, h);
     }
     if constexpr (PREFETCH) cur = nxt;
-    else cur.template load<M::TPR>(a, i + step, lt);
     if constexpr (W > 1) {
       // a row with only one of the two sums reuses its slot in the next one
       if (!(a.gx && (a.w1.p || a.gate_kind == GATE_ROW))) __syncthreads();
@@ -303,47 +448,137 @@ __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_backward_kernel
   }
   // this block's partials; several rows a block: their sums added in order through LDS
   const int64_t P = gridDim.x;
-  auto write = [&](float (&acc)[NQ][kVN], int which) {
+  auto write = [&](float (&acc)[kVN], int which) {
     float* dst = a.partial + ((int64_t)which * P + blockIdx.x) * a.d;
+    if constexpr (LDS_SUMS) {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const float4 o = sums[(2 * which + hh) * M::TPR];
+        acc[4 * hh] = o.x;
+        acc[4 * hh + 1] = o.y;
+        acc[4 * hh + 2] = o.z;
+        acc[4 * hh + 3] = o.w;
+      }
+    }
     if constexpr (M::RPB == 1) {
 #pragma unroll
-      for (int q = 0; q < NQ; ++q)
-#pragma unroll
-        for (int u = 0; u < kVN; ++u) {
-          const int64_t c = (int64_t)(lt + q * M::TPR) * kVN + u;
-          if (c < a.d) dst[c] = acc[q][u];
-        }
+      for (int u = 0; u < kVN; ++u)
+        if (c + u < a.d) dst[c + u] = acc[u];
     } else {
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < kVN; ++u) {
-        const int64_t c = (int64_t)lt * kVN + u;
-        if (c < a.d) fold[(int64_t)sub * a.d + c] = acc[0][u];
-      }
+      for (int u = 0; u < kVN; ++u)
+        if (c + u < a.d) fold[(int64_t)sub * a.d + c + u] = acc[u];
       __syncthreads();
-      for (int64_t c = threadIdx.x; c < a.d; c += M::THREADS) {
-        float t = 0.f;
+      for (int64_t k = threadIdx.x; k < a.d; k += M::THREADS) {
+        float tt = 0.f;
 #pragma unroll
-        for (int q = 0; q < M::RPB; ++q) t += fold[(int64_t)q * a.d + c];
-        dst[c] = t;
+        for (int q = 0; q < M::RPB; ++q) tt += fold[(int64_t)q * a.d + k];
+        dst[k] = tt;
       }
     }
   };
   if (a.w1.p) write(acc1, 0);
   if (a.w2.p) write(acc2, 1);
   if (a.gate_kind == GATE_CHANNEL) write(accg, 2);
-  if (a.alpha_ptr) {
-    __syncthreads();
-    const float t = wave_sum(acc_alpha);
-    if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6][0] = t;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      float all = 0.f;
+  block_alpha<M::WPB>(a, acc_alpha, red);
+}
+
+// Wider rows (d > 8192), sixteen waves a row and several chunks a thread: a chunk's operands are read again
+// (from L2) for each of the three phases instead of being held, and the sums over rows are kept in this block's
+// own partials in memory. Right for any width; about half the rate of the form above.
+template <typename R, typename Y, bool VEC>
+__global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide_backward_kernel(NormArgs a) {
+  using M = Map<kMaxWaves>;
+  __shared__ float red[2][M::WPB][2];
+  const int64_t c0 = (int64_t)threadIdx.x * kVN, cstep = (int64_t)M::TPR * kVN, P = gridDim.x;
+  const float alpha = a.alpha_ptr ? *a.alpha_ptr : a.alpha;
+  const float inv_d = 1.0f / (float)a.d;
+  float acc_alpha = 0.f;
+  float* part[3] = {a.w1.p ? a.partial + (int64_t)blockIdx.x * a.d : nullptr,
+                    a.w2.p ? a.partial + (P + blockIdx.x) * a.d : nullptr,
+                    a.gate_kind == GATE_CHANNEL ? a.partial + (2 * P + blockIdx.x) * a.d : nullptr};
+  bool fresh = true;  // this block's first row: its partials are written, not added to
+  auto add = [&](float* p, int64_t c, const float (&v)[kVN]) {
+    if (!p) return;
 #pragma unroll
-      for (int q = 0; q < M::WPB; ++q) all += red[0][q][0];
-      a.partial[3 * P * a.d + blockIdx.x] = all;
+    for (int u = 0; u < kVN; ++u)
+      if (c + u < a.d) p[c + u] = fresh ? v[u] : p[c + u] + v[u];
+  };
+  for (int64_t i = blockIdx.x; i < a.n; i += P) {  // (a grid of at most n blocks: each has a row)
+    float rho1 = 1.f, rho2 = 0.f;
+    // y rho1, u, r' and r of a chunk, and its gains
+    float y[kVN], uu[kVN], h[kVN], r[kVN], gx[kVN], w1[kVN], w2[kVN], g[kVN], t[kVN];
+    Row<R, Y, VEC> row;
+    auto chunk = [&](int64_t c) {
+      row.load(a, i, c);
+      rho1 = row.rho1;
+      rho2 = row.rho2;
+      row.y.get(y);
+      row.r.get(r);
+      row.gx.get(gx);
+      row.gr.get(t);
+      load_gain<VEC>(a.w1, c, a.d, w1);
+      load_gain<VEC>(a.w2, c, a.d, w2);
+      if (a.gate_kind == GATE_CHANNEL) load_vec<VEC>(a.gate, 0, c, a.d, g);
+      else if (a.gate_kind == GATE_FULL) load_vec<VEC>(a.gate, i * a.ldg, c, a.d, g);
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) {
+        if (a.gate_kind == GATE_NONE || a.gate_kind == GATE_ROW) g[u] = row.g_row;
+        y[u] *= rho1;
+        uu[u] = y[u] * w1[u];
+        h[u] = fmaf(g[u], uu[u], alpha * r[u]);
+      }
+    };
+    float s[1] = {0.f};
+    for (int64_t c = c0; c < a.d; c += cstep) {
+      chunk(c);
+      float v[kVN];
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) {
+        v[u] = gx[u] * (rho2 * h[u]);
+        s[0] = fmaf(gx[u] * w2[u], h[u], s[0]);
+      }
+      add(part[1], c, v);
     }
+    row_sums<kMaxWaves, 1, M::WPB>(s, red, 0);
+    const float coef2 = a.gx ? rho2 * rho2 * rho2 * s[0] * inv_d : 0.f;
+    auto grad = [&](int64_t c) {  // t, the whole grad of r'
+      chunk(c);
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) t[u] = fmaf(-coef2, h[u], fmaf(rho2, gx[u] * w2[u], t[u]));
+    };
+    float s2[2] = {0.f, 0.f};
+    for (int64_t c = c0; c < a.d; c += cstep) {
+      grad(c);
+      float v[kVN];
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) {
+        acc_alpha = fmaf(t[u], r[u], acc_alpha);
+        uu[u] *= t[u];
+        s2[1] += uu[u];
+        h[u] = g[u] * t[u];
+        v[u] = h[u] * y[u];
+        s2[0] = fmaf(h[u] * w1[u], y[u], s2[0]);
+        t[u] *= alpha;
+      }
+      add(part[0], c, v);
+      add(part[2], c, uu);
+      store_chunk<VEC>(static_cast<R*>(a.dr) + i * a.d, c, a.d, t);
+      if (a.gate_kind == GATE_FULL && a.dgate.p) store_gate<VEC>(a.dgate, i * a.d, c, a.d, uu);
+    }
+    row_sums<kMaxWaves, 2, M::WPB>(s2, red, 1);
+    if (a.gate_kind == GATE_ROW && a.dgate.p && threadIdx.x == 0) store_one(a.dgate, i, s2[1]);
+    const float coef1 = a.w1.p ? rho1 * s2[0] * inv_d : 0.f;
+    for (int64_t c = c0; c < a.d; c += cstep) {
+      grad(c);
+#pragma unroll
+      for (int u = 0; u < kVN; ++u) h[u] = fmaf(-coef1, y[u], rho1 * w1[u] * (g[u] * t[u]));
+      store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, c, a.d, h);
+    }
+    fresh = false;
   }
+  block_alpha<M::WPB>(a, acc_alpha, red);
 }
 
 // dw[c] = the sum of P partials in a fixed order, rounded once: 64 columns a block, wave v takes
@@ -403,13 +638,11 @@ int row_chunks(int64_t d) {
   return nq;
 }
 constexpr int64_t kMaxD = (int64_t)kMaxWaves * 64 * kVN * kMaxNQ;
-int rows_per_block(int64_t d) {
-  const int w = row_waves(d);
-  return w < 4 ? 4 / w : 1;
-}
+// Blocks of the backward: two of eight waves a CU, or one of sixteen.
 int partials(int64_t n, int64_t d) {
-  const int64_t want = cdiv(n > 0 ? n : 1, rows_per_block(d));
-  return (int)(want < kMaxPartials ? want : kMaxPartials);
+  const int w = row_waves(d);
+  const int64_t want = cdiv(n > 0 ? n : 1, w < 8 ? 8 / w : 1), most = w == kMaxWaves ? kMaxPartials / 2 : kMaxPartials;
+  return (int)(want < most ? want : most);
 }
 
 // f(waves, chunks) with compile-time constants.
@@ -438,6 +671,12 @@ void with_types(int r_dtype, int y_dtype, F f) {
 }
 
 bool vec_ok(const void* p, int64_t ld, int dtype) { return aligned16(p) && ld % (16 / dtype_size(dtype)) == 0; }
+// What both passes read has 16-byte rows of whole chunks.
+bool operands_vec(const NormArgs& a, int r_dtype, int y_dtype, int gate_dtype) {
+  return a.d % kVN == 0 && vec_ok(a.r, a.ldr, r_dtype) && vec_ok(a.y, a.ldy, y_dtype) && aligned16(a.w1.p) &&
+         aligned16(a.w2.p) &&
+         (a.gate_kind == GATE_FULL ? vec_ok(a.gate.p, a.ldg, gate_dtype) : a.gate_kind == GATE_ROW || aligned16(a.gate.p));
+}
 
 int common_checks(const char* name, int64_t n, int64_t d, int r_dtype, int y_dtype, int p_dtype, int gate_kind,
                   int gate_dtype, int64_t ldr, int64_t ldy, int64_t ldg, const void* w1, const void* gate,
@@ -464,9 +703,9 @@ NormArgs fill(const void* r, int64_t ldr, int r_dtype, const void* y, int64_t ld
   a.n = n;
   a.d = d;
   const int pb = p_dtype == ZMOE_DTYPE_BF16, gb = gate_dtype == ZMOE_DTYPE_BF16;
-  a.w1 = Vec{w1, pb, aligned16(w1)};
-  a.w2 = Vec{w2, pb, aligned16(w2)};
-  a.gate = Vec{gate, gb, gate_kind == GATE_FULL ? vec_ok(gate, ldg, gate_dtype) : aligned16(gate)};
+  a.w1 = Vec{w1, pb};
+  a.w2 = Vec{w2, pb};
+  a.gate = Vec{gate, gb};
   a.gate_kind = gate_kind;
   a.ldg = ldg;
   a.alpha_ptr = alpha_ptr;
@@ -492,8 +731,7 @@ extern "C" int zmoe_norm_residual(const void* R, int64_t r_stride, int r_dtype, 
   NormArgs a = fill(R, r_stride, r_dtype, Y, y_stride, y_dtype, n, d, w_post, w_next, w_dtype, gate, gate_kind,
                     gate_stride, gate_dtype, scale_ptr, scale);
   a.eps = eps;
-  a.vec = vec_ok(R, r_stride, r_dtype) && vec_ok(Y, y_stride, y_dtype) && vec_ok(R_out, d, r_dtype) &&
-          vec_ok(X, d, y_dtype);
+  const bool vec = operands_vec(a, r_dtype, y_dtype, gate_dtype) && aligned16(R_out) && aligned16(X);
   a.r_out = R_out;
   a.x = X;
   a.rho1 = rstd_post;
@@ -501,9 +739,11 @@ extern "C" int zmoe_norm_residual(const void* R, int64_t r_stride, int r_dtype, 
   hipStream_t s = as_stream(stream);
   with_types(r_dtype, y_dtype, [&](auto rt, auto yt) {
     with_map(d, [&](auto w, auto nq) {
-      using M = Map<decltype(w)::value>;
-      hipLaunchKernelGGL((norm_residual_kernel<decltype(rt), decltype(yt), decltype(w)::value, decltype(nq)::value>),
-                         dim3((unsigned)cdiv(n, M::RPB)), dim3(M::THREADS), 0, s, a);
+      using M = FwdMap<decltype(w)::value>;
+      constexpr int W = decltype(w)::value, NQ = decltype(nq)::value;
+      auto kern = vec ? norm_residual_kernel<decltype(rt), decltype(yt), W, NQ, true>
+                      : norm_residual_kernel<decltype(rt), decltype(yt), W, NQ, false>;
+      hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(n, M::RPB)), dim3(M::THREADS), 0, s, a);
     });
   });
   return check_launch("norm_residual");
@@ -536,28 +776,47 @@ extern "C" int zmoe_norm_residual_backward(const void* dR_out, const void* dX, c
   ZMOE_REQUIRE(aligned16(workspace), ZMOE_ERR_ALIGN, "norm_residual_backward: workspace on 16 bytes");
   NormArgs a = fill(R, r_stride, r_dtype, Y, y_stride, y_dtype, n, d, w_post, w_next, w_dtype, gate, gate_kind,
                     gate_stride, gate_dtype, scale_ptr, scale);
-  a.vec = vec_ok(R, r_stride, r_dtype) && vec_ok(Y, y_stride, y_dtype) && vec_ok(dR, d, r_dtype) &&
-          vec_ok(dY, d, y_dtype) && vec_ok(dR_out, d, r_dtype) && vec_ok(dX, d, y_dtype);
+  const bool vec = operands_vec(a, r_dtype, y_dtype, gate_dtype) && aligned16(dR) && aligned16(dY) &&
+                   aligned16(dR_out) && aligned16(dX) && (gate_kind != GATE_FULL || aligned16(dgate));
   a.rho1 = const_cast<float*>(rstd_post);
   a.rho2 = const_cast<float*>(rstd_next);
   a.gr = dR_out;
   a.gx = dX;
   a.dr = dR;
   a.dy = dY;
-  a.dgate = Out{gate_kind == GATE_ROW || gate_kind == GATE_FULL ? dgate : nullptr, gate_dtype == ZMOE_DTYPE_BF16,
-                vec_ok(dgate, d, gate_dtype)};
+  a.dgate = Out{gate_kind == GATE_ROW || gate_kind == GATE_FULL ? dgate : nullptr, gate_dtype == ZMOE_DTYPE_BF16};
   a.partial = static_cast<float*>(workspace);
   const int P = partials(n, d);
+  bool prepared = true;
   hipStream_t s = as_stream(stream);
   with_types(r_dtype, y_dtype, [&](auto rt, auto yt) {
+    if (d > (int64_t)kMaxWaves * 64 * kVN) {
+      auto kern = vec ? norm_residual_wide_backward_kernel<decltype(rt), decltype(yt), true>
+                      : norm_residual_wide_backward_kernel<decltype(rt), decltype(yt), false>;
+      hipLaunchKernelGGL(kern, dim3((unsigned)P), dim3(Map<kMaxWaves>::THREADS), 0, s, a);
+      return;
+    }
     with_map(d, [&](auto w, auto nq) {
-      using M = Map<decltype(w)::value>;
-      const size_t lds = M::RPB > 1 ? (size_t)M::RPB * (size_t)d * sizeof(float) : 0;  // at most 8 KB
-      hipLaunchKernelGGL(
-          (norm_residual_backward_kernel<decltype(rt), decltype(yt), decltype(w)::value, decltype(nq)::value>),
-          dim3((unsigned)P), dim3(M::THREADS), lds, s, a);
+      constexpr int W = decltype(w)::value;
+      if constexpr (decltype(nq)::value == 1) {
+        using M = Map<W>;
+        using RT = decltype(rt);
+        using YT = decltype(yt);
+        auto kern = gate_kind == GATE_FULL ? (vec ? norm_residual_backward_kernel<RT, YT, W, true, true>
+                                                  : norm_residual_backward_kernel<RT, YT, W, false, true>)
+                                           : (vec ? norm_residual_backward_kernel<RT, YT, W, true, false>
+                                                  : norm_residual_backward_kernel<RT, YT, W, false, false>);
+        const size_t lds = W == kMaxWaves ? (size_t)M::TPR * 6 * sizeof(float4)  // 96 KB
+                                          : (M::RPB > 1 ? (size_t)M::RPB * (size_t)d * sizeof(float) : 0);  // <= 16 KB
+        if (W == kMaxWaves && prepare(kern, (int)lds) != ZMOE_OK) {
+          prepared = false;
+          return;
+        }
+        hipLaunchKernelGGL(kern, dim3((unsigned)P), dim3(M::THREADS), lds, s, a);
+      }
     });
   });
+  if (!prepared) return ZMOE_ERR_HIP;
   rc = check_launch("norm_residual_backward");
   if (rc) return rc;
   Reduce red{};
@@ -565,9 +824,9 @@ extern "C" int zmoe_norm_residual_backward(const void* dR_out, const void* dX, c
   red.P = P;
   red.d = d;
   const int pb = w_dtype == ZMOE_DTYPE_BF16;
-  red.out[0] = Out{w_post ? dw_post : nullptr, pb, 0};
-  red.out[1] = Out{w_next ? dw_next : nullptr, pb, 0};
-  red.out[2] = Out{gate_kind == GATE_CHANNEL ? dgate : nullptr, gate_dtype == ZMOE_DTYPE_BF16, 0};
+  red.out[0] = Out{w_post ? dw_post : nullptr, pb};
+  red.out[1] = Out{w_next ? dw_next : nullptr, pb};
+  red.out[2] = Out{gate_kind == GATE_CHANNEL ? dgate : nullptr, gate_dtype == ZMOE_DTYPE_BF16};
   red.dalpha = dscale;
   if (red.out[0].p || red.out[1].p || red.out[2].p || dscale) {
     hipLaunchKernelGGL(norm_residual_reduce_kernel, dim3((unsigned)cdiv(d, 64), 4), dim3(64 * kRedWaves), 0, s, red);
