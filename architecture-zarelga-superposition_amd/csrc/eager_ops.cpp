@@ -695,6 +695,53 @@ Tensor fp8_mm(const Tensor& xq, const Tensor& xs, const Tensor& wq, const Tensor
   return op.call(xq, xs, wq, ws, K, ss, off, k, xg, yg, out_f32);
 }
 
+// f16 rows [R, N] with a scale per 64 columns, for combine_half.
+Rows8 empty_half(int64_t R, int64_t N, const Tensor& like) {
+  const int64_t nb = (N + 63) / 64;
+  return {empty({R, nb * 64}, like, at::kHalf), empty({R, nb}, like, at::kByte)};
+}
+
+Tensors fp8_mm_half(const Tensor& xq, const Tensor& xs, const Tensor& wq, const Tensor& ws, int64_t K, const Opt& ss,
+                    const Opt& off, int64_t k, bool xg, bool yg) {
+  if (K > 0 && k > 0 && fits_int(k) && xq.is_cuda() && rows8(xq, xs, K, xq) && weight8(wq, ws, K, off ? 3 : 2, xq)) {
+    const int64_t M = xq.size(0), N = wq.size(-2), E = off ? wq.size(0) : 1, R = xg ? M : M * k;
+    if ((off ? index(*off, xq, E) && (ss ? index(*ss, xq, R) : xg && yg) : xg && yg) && fits_int(E)) {
+      const c10::DeviceGuard guard(xq.device());
+      const Rows8 Y = empty_half(R, N, xq);
+      if (zmoe_fp8_scatter2scatter_half(raw(xq), raw(xs), M, raw(wq), raw(ws), off && ss ? ids(*ss) : nullptr,
+                                        off ? ids(*off) : nullptr, K, N, (int)E, (int)k, xg, yg, raw(Y.q), raw(Y.s),
+                                        stream_of(xq)) == ZMOE_OK)
+        return {Y.q, Y.s};
+    }
+  }
+  static const auto op = general<Tensors(const Tensor&, const Tensor&, const Tensor&, const Tensor&, c10::SymInt,
+                                         const Opt&, const Opt&, c10::SymInt, bool, bool)>("zmoe::fp8_mm_half");
+  return op.call(xq, xs, wq, ws, K, ss, off, k, xg, yg);
+}
+
+Tensor combine_half(const Tensor& Y, const Tensor& Ys, const Opt& gates, int64_t k, int64_t N, const Opt& addend,
+                    const Opt& out_rows, int64_t out_total) {
+  const int64_t nb = (N + 63) / 64;
+  if (Y.is_cuda() && flat(Y, Y, at::kHalf) && Y.dim() == 2 && N > 0 && Y.size(1) == nb * 64 && flat(Ys, Y, at::kByte) &&
+      Ys.dim() == 2 && Ys.size(0) == Y.size(0) && Ys.size(1) == nb && k > 0 && fits_int(k) && Y.size(0) % k == 0) {
+    const int64_t T = Y.size(0) / k;
+    if ((!gates || (flat(*gates, Y, at::kFloat) && gates->numel() == T * k)) &&
+        (!addend || (flat(*addend, Y, at::kBFloat16) && addend->numel() == T * N)) &&
+        (!out_rows || (index(*out_rows, Y, T) && out_total >= 0))) {
+      const c10::DeviceGuard guard(Y.device());
+      const auto opts = Y.options().dtype(at::kBFloat16);
+      Tensor out = out_rows ? at::zeros({out_total, N}, opts) : at::empty({T, N}, opts);
+      if (zmoe_combine_half(raw(Y), raw(Ys), gates ? ptr<const float>(*gates) : nullptr, addend ? raw(*addend) : nullptr,
+                            T, (int)k, N, ZMOE_DTYPE_BF16, out_rows ? ids(*out_rows) : nullptr, out.size(0), raw(out),
+                            stream_of(Y)) == ZMOE_OK)
+        return out;
+    }
+  }
+  static const auto op = general<Tensor(const Tensor&, const Tensor&, const Opt&, c10::SymInt, c10::SymInt, const Opt&,
+                                        const Opt&, c10::SymInt)>("zmoe::combine_half");
+  return op.call(Y, Ys, gates, k, N, addend, out_rows, out_total);
+}
+
 Tensor fp8_linear(const Tensor& x, const Tensor& wq, const Tensor& ws) {
   if (x.is_cuda() && known(x) && apart(x) && x.size(1) > 0 && weight8(wq, ws, x.size(1), 2, x)) {
     const c10::DeviceGuard guard(x.device());
@@ -743,11 +790,18 @@ Tensors fp8_glu_experts(const Tensor& x, const Tensor& gates, const Tensor& idx,
     const Tensors sorted = flatten_sort_count(idx, E);
     const Tensor &ss = sorted[1], &off = sorted[2];
     const Rows8 r = empty8(T, d, x), a = empty8(R, f, x);
-    Tensor Y = empty({R, d}, x);
     void* s = stream_of(x);
-    if (quantize_into(x, r, std::nullopt, 1, std::nullopt) &&
-        zmoe_fp8_glu_w1_forward(raw(r.q), raw(r.s), T, raw(w1q), raw(w1s), ids(ss), ids(off), d, f, (int)E, (int)k,
-                                raw(a.q), raw(a.s), s) == ZMOE_OK &&
+    const bool first = quantize_into(x, r, std::nullopt, 1, std::nullopt) &&
+                       zmoe_fp8_glu_w1_forward(raw(r.q), raw(r.s), T, raw(w1q), raw(w1s), ids(ss), ids(off), d, f,
+                                               (int)E, (int)k, raw(a.q), raw(a.s), s) == ZMOE_OK;
+    if (first && x.scalar_type() == at::kBFloat16) {
+      const Rows8 Y = empty_half(R, d, x);
+      if (zmoe_fp8_scatter2scatter_half(raw(a.q), raw(a.s), R, raw(w2q), raw(w2s), ids(ss), ids(off), f, d, (int)E, 1, 1,
+                                        0, raw(Y.q), raw(Y.s), s) == ZMOE_OK)
+        return {combine_half(Y.q, Y.s, gates, k, d, residual, out_rows, out_total), off};
+    }
+    Tensor Y = empty({R, d}, x);
+    if (first &&
         zmoe_fp8_scatter2scatter(raw(a.q), raw(a.s), R, raw(w2q), raw(w2s), ids(ss), ids(off), f, d, (int)E, 1, 1, 0,
                                  code(Y), raw(Y), d, s) == ZMOE_OK)
       return {combine(Y, gates, k, residual, out_rows, out_total), off};
@@ -945,6 +999,12 @@ TORCH_LIBRARY(zmoe_eager, m) {
   ZMOE_EAGER(fp8_mm,
              "(Tensor xq, Tensor xs, Tensor wq, Tensor ws, int K, Tensor? sorted_scattered_idxs, "
              "Tensor? expert_offsets, int k, bool x_grouped, bool y_grouped, bool out_f32) -> Tensor");
+  ZMOE_EAGER(fp8_mm_half,
+             "(Tensor xq, Tensor xs, Tensor wq, Tensor ws, int K, Tensor? sorted_scattered_idxs, "
+             "Tensor? expert_offsets, int k, bool x_grouped, bool y_grouped) -> Tensor[]");
+  ZMOE_EAGER(combine_half,
+             "(Tensor Y, Tensor Ys, Tensor? gates, int k, int N, Tensor? addend, Tensor? out_rows, int out_total) "
+             "-> Tensor");
   ZMOE_EAGER(fp8_linear, "(Tensor x, Tensor wq, Tensor ws) -> Tensor");
   ZMOE_EAGER(fp8_glu_mlp, "(Tensor x, Tensor w1q, Tensor w1s, Tensor w2q, Tensor w2s) -> Tensor");
   ZMOE_EAGER(fp8_glu_experts,

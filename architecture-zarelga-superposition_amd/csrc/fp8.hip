@@ -21,6 +21,8 @@ namespace {
 constexpr int kBlk = 128;  // values of one scale along the depth, and bytes of an LDS row
 constexpr uint32_t kNaN8 = 0x7f;
 
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef int v8i32_t __attribute__((ext_vector_type(8)));
 
 __host__ __device__ inline int64_t blocks_of(int64_t n) { return (n + kBlk - 1) / kBlk; }
@@ -32,6 +34,11 @@ __device__ __forceinline__ int scale_code(float a) {
   const int bits = __float_as_int(a);
   const int c = (bits >> 23) - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
   return c > 0 ? c : 0;
+}
+// Byte of the power of two that puts a into [2^14, 2^15) (the least is 2^-126).
+__device__ __forceinline__ int half_code(float a) {
+  const int c = (__float_as_int(a) >> 23) - 14;
+  return c > 1 ? c : 1;
 }
 // 2^-c of that byte (code <= 247: the exponent field stays normal).
 __device__ __forceinline__ float scale_inverse(int code) { return __int_as_float((254 - code) << 23); }
@@ -183,7 +190,10 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
 // B rows of K / 128 blocks, one 128-byte line each. A stage is one block of the depth: BM + BN lines in
 // LDS (the geometry of 64 bf16 elements), one 16 x 16 x 128 MFMA per 16 x 16 outputs. The weight rows
 // are the MFMA's first operand, so a lane ends up with 4 consecutive output columns of one row.
-enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2 };
+// F8_HALF: rows that a sum over a token's k slots reads next, as f16 with a power-of-two scale for each 64 columns:
+// 16 bits like bf16, but within 2^-12 of each value (bf16: 2^-9), so that the sum has its own rounding only.
+enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2, F8_HALF = 3 };
+constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 
 struct Fp8Params {
   const uint8_t* a;
@@ -199,7 +209,7 @@ struct Fp8Params {
   void* c;
   int64_t ldc;             // elements (GLU: bytes of a row of Aq)
   const int64_t* c_rows;   // output row of sorted row i = c_rows[i] (null: i)
-  uint8_t* cs;             // GLU: the activations' scales
+  uint8_t* cs;             // GLU: the activations' scales; HALF: the rows'
   int64_t cs_pitch;
   int vec_c;               // rows of C take 16-byte stores
   const int64_t* offsets;  // inclusive expert ends [E] (null: one weight, ns_m rows)
@@ -527,6 +537,49 @@ __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
       }
       __builtin_amdgcn_wave_barrier();
     });
+  } else if constexpr (EPI == F8_HALF) {
+    // a row's 64 columns of this wave are in four lanes: the power of two that puts the largest into
+    // [2^14, 2^15) (f16 ends at 65504; values down to 2^-28 of the largest keep all 11 bits), then as the bf16 store
+    char* st = smem + wave * 32 * L::kPitch;
+    uint16_t* C = static_cast<uint16_t*>(p.c);
+    constexpr int MS = MF < 2 ? 1 : 2;
+    const int cb = nt * (BN / kHalfCols) + gn;
+    unrolled<MF / MS>([&](auto s) {
+#pragma unroll
+      for (int h = 0; h < MS; ++h) {
+        constexpr int m0 = s * MS;
+        float a = 0.f;
+#pragma unroll
+        for (int n = 0; n < NF; ++n)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) a = fmaxf(a, finite_abs(acc[m0 + h][n][u]));
+        a = fmaxf(a, __shfl_xor(a, 16, 64));
+        a = fmaxf(a, __shfl_xor(a, 32, 64));
+        const int code = half_code(a);
+        const float inv = scale_inverse(code);
+        const int rl = gm * G::WM + 16 * (m0 + h) + r16;
+#pragma unroll
+        for (int n = 0; n < NF; ++n) {
+          const f32x4_t v = acc[m0 + h][n];
+          f16x4_t w;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[u] = (_Float16)(v[u] * inv);
+          *reinterpret_cast<uint2*>(st + (16 * h + r16) * L::kPitch + (16 * n + 4 * g4) * 2) = __builtin_bit_cast(uint2, w);
+        }
+        if (g4 == 0 && rl < rows && cb < p.cs_pitch)
+          p.cs[((p.c_rows ? 0 : row0) + dst_table[rl]) * p.cs_pitch + cb] = (uint8_t)code;
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int it = 0; it < 16 * MS / 8; ++it) {
+        const int rr = it * 8 + (lane >> 3), ch = lane & 7;
+        const int rl = gm * G::WM + 16 * MS * s + rr;
+        const uint4 v = *reinterpret_cast<const uint4*>(st + rr * L::kPitch + ch * 16);
+        if (rl < rows && cb < p.cs_pitch)
+          *reinterpret_cast<uint4*>(C + ((p.c_rows ? 0 : row0) + dst_table[rl]) * p.ldc + cb * kHalfCols + ch * 8) = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+    });
   } else {
     // a = silu(gate) up from the f32 sums; a row's 128 pairs of this tile are one block: its largest
     // magnitude over this wave's 32 pairs (four lanes a row), then over the four waves through LDS
@@ -561,6 +614,64 @@ __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
     for (int idx = (int)threadIdx.x; idx < rows * 8; idx += NT)
       *reinterpret_cast<uint4*>(C + (int64_t)(idx >> 3) * p.ldc + (idx & 7) * 16) =
           *reinterpret_cast<const uint4*>(smem + (idx >> 3) * kBlk + (idx & 7) * 16);
+  }
+}
+
+// ------------------------------------------------------------------ sums over slots
+// out[t] = add[t] + sum_j g[t, j] Y[t k + j] of F8_HALF rows (g null: 1), one rounding. A thread has eight columns;
+// the k rows' loads (compiled for k up to 8) are all issued before the first is used. Bound by HBM.
+template <typename T, int KF>
+__global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __restrict__ Y, const uint8_t* __restrict__ S,
+                                                           int64_t ldy, int64_t pitch, const float* __restrict__ g,
+                                                           const T* __restrict__ add, int64_t T_, int k_rt, int64_t N,
+                                                           T* __restrict__ out, const int64_t* __restrict__ out_rows,
+                                                           int64_t out_total, int vec, uint32_t chunks) {
+  const int k = KF > 0 ? KF : k_rt;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t t = idx / chunks;
+  if (t >= T_) return;
+  const int64_t c = (idx - t * chunks) * 8;
+  const int64_t orow = out_rows ? out_rows[t] : t;
+  if (orow < 0 || orow >= out_total) return;
+  float acc[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) acc[u] = 0.f;
+  auto one = [&](const uint4& y, int code, float w) {
+    const f16x8_t h = __builtin_bit_cast(f16x8_t, y);
+    const float sc = __int_as_float(code << 23);  // (code >= 1: a normal number)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[u] = fmaf(w, (float)h[u] * sc, acc[u]);
+  };
+  const uint16_t* y0 = Y + t * k * ldy + c;
+  const uint8_t* s0 = S + t * k * pitch + c / kHalfCols;
+  if constexpr (KF > 0) {
+    uint4 y[KF];
+    int code[KF];
+#pragma unroll
+    for (int j = 0; j < KF; ++j) {
+      y[j] = *reinterpret_cast<const uint4*>(y0 + j * ldy);
+      code[j] = s0[j * pitch];
+    }
+#pragma unroll
+    for (int j = 0; j < KF; ++j) one(y[j], code[j], g ? g[t * KF + j] : 1.f);
+  } else {
+    for (int j = 0; j < k; ++j) one(*reinterpret_cast<const uint4*>(y0 + j * ldy), s0[j * pitch], g ? g[t * k + j] : 1.f);
+  }
+  if (add) {
+    float v[8];
+    load8(add + t * N, c, N, vec != 0, v);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[u] += v[u];
+  }
+  T* o = out + orow * N + c;
+  if (vec && c + 8 <= N) {
+    constexpr int VN = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < 8 / VN; ++q) *reinterpret_cast<uint4*>(o + q * VN) = pack_chunk(&acc[q * VN], T{});
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (c + u < N) o[u] = from_f32<T>(acc[u]);
   }
 }
 
@@ -698,40 +809,94 @@ int product_operands(const char* name, const void* Xq, const void* Xs, int64_t M
 }
 }  // namespace
 
+namespace {
+// Both forms of the product; half: Y in f16 with scales Ys, else out_dtype.
+int scatter2scatter8(const char* name, const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
+                     const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t K, int64_t N, int E,
+                     int k, int x_grouped, int y_grouped, int out_dtype, bool half, void* Y, void* Ys, int64_t y_stride,
+                     void* stream) {
+  ZMOE_REQUIRE(half || dtype_ok(out_dtype), ZMOE_ERR_DTYPE, "%s: dtype %d", name, out_dtype);
+  ZMOE_REQUIRE(M >= 0 && K >= 1 && N >= 1 && K < (1 << 30) && N < (1 << 30) && E >= 1 && E <= kGemmMaxE && k >= 1,
+               ZMOE_ERR_SHAPE, "%s: bad sizes (M=%lld K=%lld N=%lld E=%d k=%d)", name, (long long)M, (long long)K,
+               (long long)N, E, k);
+  ZMOE_REQUIRE(M < kMaxRows8 && M * (x_grouped ? 1 : k) < kMaxRows8, ZMOE_ERR_SHAPE, "%s: rows must be below 2^31", name);
+  ZMOE_REQUIRE(expert_offsets || (E == 1 && x_grouped && y_grouped), ZMOE_ERR_NULL,
+               "%s: no expert_offsets only for one weight and rows in order", name);
+  ZMOE_REQUIRE(half || y_stride >= N, ZMOE_ERR_SHAPE, "%s: row stride of Y", name);
+  const int64_t R = x_grouped ? M : M * k;
+  if (R == 0) return ZMOE_OK;
+  ZMOE_REQUIRE((x_grouped && y_grouped) || sorted_scattered_idxs, ZMOE_ERR_NULL,
+               "%s: sorted_scattered_idxs required unless x_grouped and y_grouped", name);
+  ZMOE_REQUIRE(Y && (!half || Ys), ZMOE_ERR_NULL, "%s: null pointer", name);
+  ZMOE_REQUIRE(half ? aligned16(Y) : (reinterpret_cast<uintptr_t>(Y) % dtype_size(out_dtype)) == 0, ZMOE_ERR_ALIGN,
+               "%s: Y's alignment", name);
+  Fp8Params p{};
+  p.a_rows = x_grouped ? nullptr : sorted_scattered_idxs;
+  p.a_div = k;
+  int rc = product_operands(name, Xq, Xs, M, Wq, Ws, K, N, blocks_of(N), E, expert_offsets, p);
+  if (rc) return rc;
+  p.c = Y;
+  p.c_rows = y_grouped ? nullptr : sorted_scattered_idxs;
+  p.N = (int)N;
+  p.n_major = x_grouped ? 1 : 0;
+  p.ns_m = expert_offsets ? 0 : (int)M;
+  hipStream_t s = as_stream(stream);
+  if (half) {
+    p.cs = static_cast<uint8_t*>(Ys);
+    p.cs_pitch = cdiv(N, kHalfCols);
+    p.ldc = p.cs_pitch * kHalfCols;
+    return dispatch8<F8_HALF>(p, R, s);
+  }
+  p.ldc = y_stride;
+  p.vec_c = aligned16(Y) && y_stride % (16 / dtype_size(out_dtype)) == 0;
+  return out_dtype == ZMOE_DTYPE_BF16 ? dispatch8<F8_STORE_BF16>(p, R, s) : dispatch8<F8_STORE_F32>(p, R, s);
+}
+}  // namespace
+
 extern "C" int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
                                         const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t K,
                                         int64_t N, int E, int k, int x_grouped, int y_grouped, int out_dtype, void* Y,
                                         int64_t y_stride, void* stream) {
-  ZMOE_REQUIRE(dtype_ok(out_dtype), ZMOE_ERR_DTYPE, "fp8_scatter2scatter: dtype %d", out_dtype);
-  ZMOE_REQUIRE(M >= 0 && K >= 1 && N >= 1 && K < (1 << 30) && N < (1 << 30) && E >= 1 && E <= kGemmMaxE && k >= 1,
-               ZMOE_ERR_SHAPE, "fp8_scatter2scatter: bad sizes (M=%lld K=%lld N=%lld E=%d k=%d)", (long long)M,
-               (long long)K, (long long)N, E, k);
-  ZMOE_REQUIRE(M < kMaxRows8 && M * (x_grouped ? 1 : k) < kMaxRows8, ZMOE_ERR_SHAPE,
-               "fp8_scatter2scatter: rows must be below 2^31");
-  ZMOE_REQUIRE(expert_offsets || (E == 1 && x_grouped && y_grouped), ZMOE_ERR_NULL,
-               "fp8_scatter2scatter: no expert_offsets only for one weight and rows in order");
-  ZMOE_REQUIRE(y_stride >= N, ZMOE_ERR_SHAPE, "fp8_scatter2scatter: row stride of Y");
-  const int64_t R = x_grouped ? M : M * k;
-  if (R == 0) return ZMOE_OK;
-  ZMOE_REQUIRE((x_grouped && y_grouped) || sorted_scattered_idxs, ZMOE_ERR_NULL,
-               "fp8_scatter2scatter: sorted_scattered_idxs required unless x_grouped and y_grouped");
-  ZMOE_REQUIRE(Y, ZMOE_ERR_NULL, "fp8_scatter2scatter: null pointer");
-  ZMOE_REQUIRE((reinterpret_cast<uintptr_t>(Y) % dtype_size(out_dtype)) == 0, ZMOE_ERR_ALIGN,
-               "fp8_scatter2scatter: Y's alignment");
-  Fp8Params p{};
-  p.a_rows = x_grouped ? nullptr : sorted_scattered_idxs;
-  p.a_div = k;
-  int rc = product_operands("fp8_scatter2scatter", Xq, Xs, M, Wq, Ws, K, N, blocks_of(N), E, expert_offsets, p);
-  if (rc) return rc;
-  p.c = Y;
-  p.ldc = y_stride;
-  p.c_rows = y_grouped ? nullptr : sorted_scattered_idxs;
-  p.vec_c = aligned16(Y) && y_stride % (16 / dtype_size(out_dtype)) == 0;
-  p.N = (int)N;
-  p.n_major = x_grouped ? 1 : 0;
-  p.ns_m = expert_offsets ? 0 : (int)M;
-  return out_dtype == ZMOE_DTYPE_BF16 ? dispatch8<F8_STORE_BF16>(p, R, as_stream(stream))
-                                      : dispatch8<F8_STORE_F32>(p, R, as_stream(stream));
+  return scatter2scatter8("fp8_scatter2scatter", Xq, Xs, M, Wq, Ws, sorted_scattered_idxs, expert_offsets, K, N, E, k,
+                          x_grouped, y_grouped, out_dtype, false, Y, nullptr, y_stride, stream);
+}
+
+extern "C" int zmoe_fp8_scatter2scatter_half(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
+                                             const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets,
+                                             int64_t K, int64_t N, int E, int k, int x_grouped, int y_grouped, void* Y,
+                                             void* Ys, void* stream) {
+  return scatter2scatter8("fp8_scatter2scatter_half", Xq, Xs, M, Wq, Ws, sorted_scattered_idxs, expert_offsets, K, N, E,
+                          k, x_grouped, y_grouped, 0, true, Y, Ys, 0, stream);
+}
+
+extern "C" int zmoe_combine_half(const void* Y, const void* Ys, const float* gates, const void* addend, int64_t T, int k,
+                                 int64_t N, int dtype, const int64_t* out_rows, int64_t out_total, void* out,
+                                 void* stream) {
+  ZMOE_REQUIRE(dtype_ok(dtype), ZMOE_ERR_DTYPE, "combine_half: dtype %d", dtype);
+  ZMOE_REQUIRE(T >= 0 && T < kMaxRows8 && k >= 1 && T * k < kMaxRows8 && N >= 1 && N < (1 << 30) && out_total >= 0,
+               ZMOE_ERR_SHAPE, "combine_half: bad sizes");
+  if (T == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(Y && Ys && out, ZMOE_ERR_NULL, "combine_half: null pointer");
+  ZMOE_REQUIRE(aligned16(Y), ZMOE_ERR_ALIGN, "combine_half: Y on 16 bytes");
+  const int64_t chunks = cdiv(N, 8), pitch = cdiv(N, kHalfCols), blocks = cdiv(T * chunks, 256);
+  ZMOE_REQUIRE(blocks < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "combine_half: too many elements");
+  const int vec = aligned16(out) && aligned16(addend) && N % (16 / dtype_size(dtype)) == 0;
+  auto go = [&](auto tt, auto kf) {
+    using TT = decltype(tt);
+    hipLaunchKernelGGL((combine_half_kernel<TT, decltype(kf)::value>), dim3((unsigned)blocks), dim3(256), 0,
+                       as_stream(stream), static_cast<const uint16_t*>(Y), static_cast<const uint8_t*>(Ys),
+                       pitch * kHalfCols, pitch, gates, static_cast<const TT*>(addend), T, k, N, static_cast<TT*>(out),
+                       out_rows, out_rows ? out_total : T, vec, (uint32_t)chunks);
+  };
+  auto by_k = [&](auto tt) {
+    if (k == 8) go(tt, std::integral_constant<int, 8>{});
+    else if (k == 4) go(tt, std::integral_constant<int, 4>{});
+    else if (k == 2) go(tt, std::integral_constant<int, 2>{});
+    else go(tt, std::integral_constant<int, 0>{});
+  };
+  if (dtype == ZMOE_DTYPE_BF16) by_k(uint16_t{});
+  else by_k(float{});
+  return check_launch("combine_half");
 }
 
 extern "C" int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T, const void* W1q, const void* W1s,

@@ -146,9 +146,13 @@ class Fp8ParallelLinear(torch.autograd.Function):
         if need_x:
             gather = None if ctx.grouped_out else ss
             gq, gs = _zl.fp8_quantize_rows(grad_out, gather, fan, flat)
-            d_input = _zl.fp8_mm(gq, gs, *qt, grad_out.size(1), ss, off, 1, True, ctx.grouped_in, f32)
-            if k > 1:
-                d_input = _zl.sum_k(d_input, k, None)
+            args = (gq, gs, *qt, grad_out.size(1), ss, off, 1, True, ctx.grouped_in)
+            if k > 1 and not f32:  # summed over the slots before the grad is rounded to 16 bits
+                d_input = _zl.combine_half(*_zl.fp8_mm_half(*args), None, k, x.size(1), None, None, 0)
+            else:
+                d_input = _zl.fp8_mm(*args, f32)
+                if k > 1:
+                    d_input = _zl.sum_k(d_input, k, None)
         if need_w:
             grouped = grad_out if ctx.grouped_out else kernels.ops.group(grad_out, ss, fan_out=fan, coeff=flat)
             DWt = _zl.group_bwd_w(grouped, rows_on_16(x), off, off.numel(), None if ctx.grouped_in else ss, k,

@@ -487,6 +487,33 @@ def _(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped, y_
     return _empty((R, wq.shape[-2]), xq, _F32 if out_f32 else torch.bfloat16)
 
 
+@layer_op("fp8_mm_half")
+def fp8_mm_half(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, K: int,
+                sorted_scattered_idxs: Optional[torch.Tensor], expert_offsets: Optional[torch.Tensor], k: int,
+                x_grouped: bool, y_grouped: bool) -> List[torch.Tensor]:
+    """``fp8_mm`` into f16 rows with a scale per 64 columns, for ``combine_half``: [Y, Ys]."""
+    return list(_z.fp8_scatter2scatter_half(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped,
+                                            y_grouped))
+
+
+@fp8_mm_half.register_fake
+def _(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped, y_grouped):
+    ys, ss = _z.half_shapes(xq.shape[0] if x_grouped else xq.shape[0] * k, wq.shape[-2])
+    return [_empty(ys, xq, torch.float16), _empty(ss, xq, torch.uint8)]
+
+
+@layer_op("combine_half")
+def combine_half(Y: torch.Tensor, Ys: torch.Tensor, gates: Optional[torch.Tensor], k: int, N: int,
+                 addend: Optional[torch.Tensor], out_rows: Optional[torch.Tensor], out_total: int) -> torch.Tensor:
+    """``combine`` of ``fp8_mm_half``'s rows, bf16."""
+    return _z.combine_half(Y, Ys, gates, k, N, addend, out_rows, out_total if out_rows is not None else None)
+
+
+@combine_half.register_fake
+def _(Y, Ys, gates, k, N, addend, out_rows, out_total):
+    return _empty((Y.shape[0] // k if out_rows is None else out_total, N), Y, torch.bfloat16)
+
+
 @layer_op("fp8_linear")
 def fp8_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor) -> torch.Tensor:
     """x [M, K] quantised, times a quantised weight [N, Kp]: [M, N] of x's dtype."""

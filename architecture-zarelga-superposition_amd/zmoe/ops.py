@@ -890,35 +890,88 @@ def _fp8_operand(q: torch.Tensor, s: torch.Tensor, K: int, what: str):
     return _on16(q), s.contiguous()
 
 
-def fp8_scatter2scatter(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, K: int,
-                        sorted_scattered_idxs: Optional[torch.Tensor] = None,
-                        expert_offsets: Optional[torch.Tensor] = None, k: int = 1, x_grouped: bool = True,
-                        y_grouped: bool = True, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``scatter2scatter`` on quantised operands: rows xq, xs times the weights wq [E, N, Kp]. Without
-    ``expert_offsets``: one weight wq [N, Kp], rows in order (a dense product)."""
+def _fp8_product(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped, y_grouped, what):
+    """Checks of both forms of the product: (device, operands kept alive, R, N, leading C arguments)."""
     dev = _require_cuda(xq, xs, wq, ws, sorted_scattered_idxs, expert_offsets)
-    xq, xs = _fp8_operand(xq, xs, K, "fp8_scatter2scatter")
-    wq, ws = _fp8_operand(wq, ws, K, "fp8_scatter2scatter")
+    xq, xs = _fp8_operand(xq, xs, K, what)
+    wq, ws = _fp8_operand(wq, ws, K, what)
     M, N = xq.shape[0], wq.shape[-2]
-    if xs.shape[0] != M or ws.shape[-2] != -(-N // FP8_BLOCK):
-        raise ValueError("fp8_scatter2scatter: values and scales do not match")
+    if xq.dim() != 2 or xs.shape[0] != M or ws.shape[-2] != -(-N // FP8_BLOCK):
+        raise ValueError(f"{what}: values and scales do not match")
     R = M if x_grouped else M * k
     if expert_offsets is None:
         if wq.dim() != 2 or not (x_grouped and y_grouped):
-            raise ValueError("fp8_scatter2scatter: several weights need expert_offsets")
+            raise ValueError(f"{what}: several weights need expert_offsets")
         E, off, ss = 1, None, None
     else:
         E, off = wq.shape[0], _idx64(expert_offsets)
         ss = None if sorted_scattered_idxs is None else _idx64(sorted_scattered_idxs)
         if wq.dim() != 3 or off.numel() != E or (ss is None and not (x_grouped and y_grouped)) or (
                 ss is not None and ss.numel() != R):
-            raise ValueError("fp8_scatter2scatter: offsets and indices must match the weights and rows")
+            raise ValueError(f"{what}: offsets and indices must match the weights and rows")
+    return dev, (xq, xs, wq, ws, ss, off), R, N, (_ptr(xq), _ptr(xs), M, _ptr(wq), _ptr(ws), _ptr(ss), _ptr(off), K, N,
+                                                  E, k, int(x_grouped), int(y_grouped))
+
+
+def fp8_scatter2scatter(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, K: int,
+                        sorted_scattered_idxs: Optional[torch.Tensor] = None,
+                        expert_offsets: Optional[torch.Tensor] = None, k: int = 1, x_grouped: bool = True,
+                        y_grouped: bool = True, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``scatter2scatter`` on quantised operands: rows xq, xs times the weights wq [E, N, Kp]. Without
+    ``expert_offsets``: one weight wq [N, Kp], rows in order (a dense product)."""
     if out_dtype not in _DT:
         raise ValueError(f"fp8_scatter2scatter: out_dtype {out_dtype}")
+    dev, keep, R, N, args = _fp8_product(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped,
+                                         y_grouped, "fp8_scatter2scatter")
     out = torch.empty((R, N), dtype=out_dtype, device=dev)
     with profiling.region("fp8_scatter2scatter", dev):
-        L.call("zmoe_fp8_scatter2scatter", _ptr(xq), _ptr(xs), M, _ptr(wq), _ptr(ws), _ptr(ss), _ptr(off), K, N, E, k,
-               int(x_grouped), int(y_grouped), _DT[out_dtype], _ptr(out), N, _stream(dev))
+        L.call("zmoe_fp8_scatter2scatter", *args, _DT[out_dtype], _ptr(out), N, _stream(dev))
+    del keep
+    return out
+
+
+def half_shapes(R: int, N: int):
+    """Shapes of f16 rows for ``combine_half`` and of their scales."""
+    nb = -(-N // 64)
+    return (R, 64 * nb), (R, nb)
+
+
+def fp8_scatter2scatter_half(xq: torch.Tensor, xs: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, K: int,
+                             sorted_scattered_idxs: Optional[torch.Tensor] = None,
+                             expert_offsets: Optional[torch.Tensor] = None, k: int = 1, x_grouped: bool = True,
+                             y_grouped: bool = True):
+    """The same into f16 rows with a power-of-two scale for each 64 columns, which ``combine_half`` sums: (Y, Ys)."""
+    dev, keep, R, N, args = _fp8_product(xq, xs, wq, ws, K, sorted_scattered_idxs, expert_offsets, k, x_grouped,
+                                         y_grouped, "fp8_scatter2scatter_half")
+    ys, ss = half_shapes(R, N)
+    out, sc = torch.empty(ys, dtype=torch.float16, device=dev), torch.empty(ss, dtype=torch.uint8, device=dev)
+    with profiling.region("fp8_scatter2scatter", dev):
+        L.call("zmoe_fp8_scatter2scatter_half", *args, _ptr(out), _ptr(sc), _stream(dev))
+    del keep
+    return out, sc
+
+
+def combine_half(Y: torch.Tensor, Ys: torch.Tensor, gates: Optional[torch.Tensor], k: int, N: int,
+                 addend: Optional[torch.Tensor] = None, out_rows: Optional[torch.Tensor] = None,
+                 out_total: Optional[int] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``combine`` of ``fp8_scatter2scatter_half``'s rows [T*k, 64 ceil(N / 64)]: [T, N] (or [out_total, N])."""
+    dev = _require_cuda(Y, Ys, gates, addend, out_rows)
+    R = Y.shape[0]
+    if (Y.dtype != torch.float16 or Ys.dtype != torch.uint8 or (tuple(Y.shape), tuple(Ys.shape)) != half_shapes(R, N)
+            or R % k or out_dtype not in _DT):
+        raise ValueError("combine_half: rows, scales or out_dtype do not match")
+    T = R // k
+    g = None if gates is None else gates.reshape(T, k).to(torch.float32).contiguous()
+    a = None if addend is None else addend.reshape(T, N).to(out_dtype).contiguous()
+    rows = None if out_rows is None else _idx64(out_rows)
+    if rows is not None and rows.numel() != T:
+        raise ValueError("combine_half: out_rows must hold one row per token")
+    shape = (T, N) if rows is None else (int(out_total), N)
+    out = (torch.empty if rows is None else torch.zeros)(shape, dtype=out_dtype, device=dev)
+    Y, Ys = _on16(Y), Ys.contiguous()
+    with profiling.region("combine", dev):
+        L.call("zmoe_combine_half", _ptr(Y), _ptr(Ys), _ptr(g), _ptr(a), T, k, N, _DT[out_dtype], _ptr(rows), shape[0],
+               _ptr(out), _stream(dev))
     return out
 
 
@@ -1048,7 +1101,11 @@ def fp8_glu_experts(x: torch.Tensor, gates: torch.Tensor, expert_idxs: torch.Ten
         raise ValueError("fp8_glu_experts: x [T, d] with gates and expert ids [T, k]")
     se, ss, off, _ = flatten_sort_count(expert_idxs, E)
     aq, as_ = fp8_glu_w1_forward(*fp8_quantize_rows(x), w1q, w1s, x.shape[1], ss, off, k)
-    Y = fp8_scatter2scatter(aq, as_, w2q, w2s, w1q.shape[1], ss, off, 1, True, False, x.dtype)
+    f = w1q.shape[1]
+    if x.dtype == torch.bfloat16:
+        Y, Ys = fp8_scatter2scatter_half(aq, as_, w2q, w2s, f, ss, off, 1, True, False)
+        return combine_half(Y, Ys, gates, k, x.shape[1], residual, out_rows, out_total), off
+    Y = fp8_scatter2scatter(aq, as_, w2q, w2s, f, ss, off, 1, True, False, x.dtype)
     return combine(Y, gates, k, residual, out_rows, out_total), off
 
 

@@ -463,6 +463,18 @@ int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const vo
                              int64_t N, int E, int k, int x_grouped, int y_grouped, int out_dtype, void* Y,
                              int64_t y_stride, void* stream);
 
+/* The same into rows that a sum over each token's slots reads next: Y f16 [R, Nh], Nh = 64 ceil(N / 64), each 64 columns
+ * of a row divided by a power of two 2^c, Ys [R, Nh / 64] bytes c + 127, which puts the largest into [2^14, 2^15).
+ * zmoe_combine_half: out[t] = addend[t] + sum_j gates[t, j] Y[t k + j] (dtype of out [T, N] and the addend; gates f32, NULL:
+ * 1; addend may be NULL), summed in f32 and rounded once; with out_rows into row out_rows[t] of [out_total, N], whose
+ * other rows are left untouched (a row outside is not written). */
+int zmoe_fp8_scatter2scatter_half(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
+                                  const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t K,
+                                  int64_t N, int E, int k, int x_grouped, int y_grouped, void* Y, void* Ys,
+                                  void* stream);
+int zmoe_combine_half(const void* Y, const void* Ys, const float* gates, const void* addend, int64_t T, int k, int64_t N,
+                      int dtype, const int64_t* out_rows, int64_t out_total, void* out, void* stream);
+
 /* The first product of SwiGLU experts with the activation and its quantisation: for sorted row i
  *   A[i, j] = silu(g) u, u = X[sorted_scattered_idxs[i] / k] W1_e[j], g = that times W1_e[f + j]  (f32)
  * and Aq [R, fp], As [R, pitch(f)] its quantised rows. W1q, W1s: the quantised [2E, f, d] view of W1 [E, 2f, d], so

@@ -195,9 +195,13 @@ def test_parallel_linear_gathered(T, K, N, E, k, skew, wt, hip_device):
     wr = O.quantize_weight(W.detach())[0]
     check(y.detach(), *O.grouped_product(O.quantize_rows(x.detach())[0], wr, ss, off, k, False, True), K)
     v, S, G = O.grouped_product(O.quantize_rows(dy)[0], wr.transpose(1, 2), ss, off, 1, True, False)
-    # each slot's row is rounded to bf16 before the k of a token are summed and rounded again
+    # a slot's row is held to 2^-12 of each value (2^-11 half steps of f16, or 2^-25 beside one of 2^14) and the k of a
+    # token are added before the one rounding to bf16
     fold = lambda t: t.view(T, k, K).sum(1)  # noqa: E731
-    b = 2.0 ** -8 * (fold(v).abs() + fold(v.abs())) * 1.01 + fold(7 * 2.0 ** -13 * G + 17 * -(-N // 128) * 2.0 ** -23 * S) * 1.01
+    top = torch.nn.functional.pad(v.abs(), (0, -K % 64)).view(T * k, -1, 64).amax(-1, keepdim=True).expand(-1, -1, 64)
+    top = top.reshape(T * k, -1)[:, :K]
+    b = 2.0 ** -8 * fold(v).abs() + 1.01 * fold(2.0 ** -11 * v.abs() + 2.0 ** -38 * top + 7 * 2.0 ** -13 * G
+                                               + 17 * -(-N // 128) * 2.0 ** -23 * S)
     assert ((x.grad.double() - fold(v)).abs() <= b).all()
     assert W.grad.dtype == W.dtype and W.grad.shape == W.shape
     beg = 0
@@ -260,6 +264,69 @@ def test_expert_mlps_train(hip_device):
             assert u.dtype == v.dtype and float((u.double() - v.double()).norm() / v.double().norm()) < 0.25
 
 
+# ------------------------------------------------------------------ f16 rows and their sums
+def row_top(v):
+    """The largest magnitude of each 64 columns, in each of them."""
+    K = v.shape[1]
+    t = torch.nn.functional.pad(v.abs(), (0, -K % 64)).view(v.shape[0], -1, 64).amax(-1, keepdim=True).expand(-1, -1, 64)
+    return t.reshape(v.shape[0], -1)[:, :K]
+
+
+def half_check(Y, Ys, val, S, G, K):
+    """f16 rows over their scales: 2^-11 of a value (half a step, and the product's own error), or half a
+    step of f16's denormals, 2^-25 where the largest of the 64 is 2^14: 2^-39 of it."""
+    N = val.shape[1]
+    got = (Y.double() * O.two(Ys.to(torch.int64) - 127).repeat_interleave(64, 1))[:, :N]
+    bound = 2.0 ** -11 * val.abs() + 2.0 ** -38 * row_top(val) + 1.01 * (7 * 2.0 ** -13 * G + 17 * -(-K // 128) * 2.0 ** -23 * S)
+    assert ((got - val).abs() <= bound).all()
+    assert not Y[:, N:].any()
+
+
+@pytest.mark.parametrize("T,k,N,K", [(1, 1, 1, 64), (5, 2, 130, 200), (33, 3, 64, 256), (300, 8, 264, 128), (70, 4, 511, 130)])
+def test_half_rows_and_their_sums(T, k, N, K, hip_device):
+    from zmoe import ops
+
+    E = 9
+    idx = random_topk(T, E, k, T).to(hip_device)
+    _, ss, off, _ = ops.flatten_sort_count(idx, E)
+    x = activations(T * k, K, BF, 1, hip_device) * torch.exp2(torch.arange(T * k) % 40 - 20.).to(hip_device).unsqueeze(1).to(BF)
+    W = weight((E, N, K), 2, BF, hip_device)
+    Y, Ys = ops.fp8_scatter2scatter_half(*ops.fp8_quantize_rows(x), *ops.fp8_quantize_weight(W), K, ss, off, 1, True, False)
+    half_check(Y, Ys, *O.grouped_product(O.quantize_rows(x)[0], O.quantize_weight(W)[0], ss, off, 1, True, False), K)
+    rows = (Y.double() * O.two(Ys.to(torch.int64) - 127).repeat_interleave(64, 1))[:, :N].view(T, k, N)
+    g = torch.randn(T, k, generator=gen(3)).to(hip_device)
+    for dt in (BF, torch.float32):
+        add = torch.randn(T, N, generator=gen(4)).to(dt).to(hip_device)
+        at = torch.randperm(T + 3, generator=gen(5))[:T].to(hip_device)
+        for gates, addend, out_rows in ((None, None, None), (g, None, None), (g, add, None), (g, add, at)):
+            out = ops.combine_half(Y, Ys, gates, k, N, addend, out_rows, T + 3, out_dtype=dt)
+            w = torch.ones_like(g) if gates is None else gates
+            a = torch.zeros_like(add) if addend is None else addend
+            ref = (w.double().unsqueeze(-1) * rows).sum(1) + a.double()
+            mag = (w.double().abs().unsqueeze(-1) * rows.abs()).sum(1) + a.double().abs()
+            got = out if out_rows is None else out[at]
+            half = 2.0 ** -8 if dt == BF else 2.0 ** -24
+            assert ((got.double() - ref).abs() <= half * ref.abs() + (k + 2) * 2.0 ** -24 * mag).all()
+            if out_rows is not None:
+                assert not out[[i for i in range(T + 3) if i not in at.tolist()]].any()
+
+
+def test_half_rows_not_finite(hip_device):
+    """inf and NaN reach their own rows only, and the largest finite sums do not overflow."""
+    from zmoe import ops
+
+    x = torch.ones(6, 128, dtype=torch.float32, device=hip_device)
+    x[1, 5], x[2, 7], x[3] = float("inf"), float("nan"), 3e37
+    W = torch.ones(70, 128, device=hip_device)
+    Y, Ys = ops.fp8_scatter2scatter_half(*ops.fp8_quantize_rows(x), *ops.fp8_quantize_weight(W), 128)
+    out = ops.combine_half(Y, Ys, None, 1, 70, out_dtype=torch.float32)
+    assert torch.isnan(out[1]).all() and torch.isnan(out[2]).all()
+    assert (out[0] == 128).all() and (out[5] == 128).all()
+    ref = O.quantize_rows(x[3:4])[0].sum()  # beyond f32: infinite; below: itself
+    big = float(ref) if float(ref) < 3.4e38 else float("inf")
+    assert (out[3] == big).all() or abs(float(out[3, 0]) / big - 1) < 1e-3
+
+
 # ------------------------------------------------------------------ serving modules
 @pytest.mark.parametrize("T,d,f,E,k", [(1, 128, 64, 8, 2), (37, 200, 100, 8, 3), (600, 256, 160, 4, 2), (0, 64, 64, 4, 2)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -283,12 +350,24 @@ def test_served_experts(T, d, f, E, k, dtype, hip_device):
         _, ss, off, _ = ops.flatten_sort_count(idx, E)
         aq, as_ = ops.fp8_glu_w1_forward(*ops.fp8_quantize_rows(x), *ops.fp8_quantize_weight(W1.view(2 * E, f, d)), d, ss, off, k)
         w2 = ops.fp8_quantize_weight(W2)
-        Y = ops.fp8_scatter2scatter(aq, as_, *w2, f, ss, off, 1, True, False, DT[dtype])
-        assert torch.equal(out, ops.combine(Y, p, k)) and torch.equal(s.last_expert_offsets, off)
-        check(Y, *O.grouped_product(rows_values(aq, as_, f), O.quantize_weight(W2)[0], ss, off, 1, True, False), f)
-        assert torch.equal(s(x, p, idx, residual=res), ops.combine(Y, p, k, res))
+        val, S, G = O.grouped_product(rows_values(aq, as_, f), O.quantize_weight(W2)[0], ss, off, 1, True, False)
+        if dtype == "f32":
+            Y = ops.fp8_scatter2scatter(aq, as_, *w2, f, ss, off, 1, True, False, DT[dtype])
+            check(Y, val, S, G, f)
+            total = lambda *a, **kw: ops.combine(Y, p, k, *a, **kw)  # noqa: E731
+        else:
+            Y, Ys = ops.fp8_scatter2scatter_half(aq, as_, *w2, f, ss, off, 1, True, False)
+            total = lambda *a, **kw: ops.combine_half(Y, Ys, p, k, d, *a, **kw)  # noqa: E731
+            half_check(Y, Ys, val, S, G, f)
+        assert torch.equal(out, total()) and torch.equal(s.last_expert_offsets, off)
+        pe = p.double().unsqueeze(-1)
+        ref, err = ((pe * v.view(T, k, d)).sum(1) for v in (val, 2.0 ** -11 * val.abs() + 7 * 2.0 ** -13 * G
+                                                            + (17 * -(-f // 128) * 2.0 ** -23 + 2.0 ** -22) * S + 2.0 ** -38 * row_top(val)))
+        half = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -24
+        assert ((out.double() - ref).abs() <= half * ref.abs() + 1.01 * err).all()
+        assert torch.equal(s(x, p, idx, residual=res), total(res))
         rows = torch.randperm(T + 5, generator=gen(5))[:T].to(hip_device)
-        assert torch.equal(s(x, p, idx, pad=(rows, T + 5)), ops.combine(Y, p, k, out_rows=rows, out_total=T + 5))
+        assert torch.equal(s(x, p, idx, pad=(rows, T + 5)), total(out_rows=rows, out_total=T + 5))
         # near the 16-bit experts: two quantised products, 2^-4 of each operand at most
         assert float((out.float() - m(x, p, idx).float()).norm()) < 0.25 * float(out.float().norm())
         again = s.to(torch.float16)  # a module-wide cast leaves the weights alone
