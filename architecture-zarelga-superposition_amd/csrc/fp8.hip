@@ -314,6 +314,151 @@ struct Lines8 {
   }
 };
 
+// The K loop of 256 x 256 tiles on eight waves, 128 x 64 outputs each: two buffers, every instruction placed. A stage
+// is four steps of 32 of the wave's rows (two fragments against the four of B, 8 MFMAs, 256 cycles of the matrix
+// unit). A step reads the next one's two A fragments while its MFMAs run; the fourth, after the one barrier of a stage
+// (this wave's loads of the next stage are in, everyone is done reading this one), reads the next stage's first A
+// fragments, its scales and, each as soon as its last MFMA is issued, its B fragments into the registers that
+// become free. The loads of the stage after the next go out four in that step and four in the next one, one every
+// other MFMA: issued together they hold a wave for ~70 cycles each, with its partner on the SIMD in the same phase.
+// Waits count the LDS reads outstanding (they return in order). acc[m][n] as in the ring loop. GLU: B fragments 2 and 3
+// take the second scale.
+template <bool GLU, int BM, int STAGE, int LPS, typename Dma>
+__device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
+                                           uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma) {
+  static_assert(LPS == 8, "eight loads a stage");
+  Frag8 fa[2][2], fb[4];
+  AScale<8> sa, sa_next;
+  uint32_t sb, sb_next;
+  // LDS reads: half h of A fragment m, of B fragment n, the scales of stage st
+  auto read_a = [&](uint32_t base, auto f, auto m, auto h) {
+    const uint32_t at = (base + a_frag) ^ (h ? 64u : 0u);
+    if constexpr (h == 0) fa[f][m & 1].lo = ds_read128<m * 2048>(at);
+    else fa[f][m & 1].hi = ds_read128<m * 2048>(at);
+  };
+  auto read_b = [&](uint32_t base, auto n) {
+    fb[n].lo = ds_read128<n * 2048>(base + b_frag);
+    fb[n].hi = ds_read128<n * 2048>((base + b_frag) ^ 64u);
+  };
+  auto read_scales = [&](int st) {
+    sa_next.read(as_lane + (uint32_t)(st * BM));
+    if constexpr (GLU) asm volatile("ds_read_u16 %0, %1" : "=v"(sb_next) : "v"(bs_lane + 2u * (uint32_t)st));
+    else asm volatile("ds_read_u8 %0, %1" : "=v"(sb_next) : "v"(bs_lane + 2u * (uint32_t)st));
+  };
+  auto mma = [&](auto m, auto n) {
+    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[n].value(), fa[(m >> 1) & 1][m & 1].value(), acc[m][n],
+                                                                0, 0, GLU ? n / 2 : 0, (int)sb, m & 3, (int)sa.w[m / 4]);
+  };
+  auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+  using std::integral_constant;
+  const integral_constant<int, 0> c0_{};
+  const integral_constant<int, 1> c1_{};
+#pragma unroll
+  for (int q = 0; q < LPS; ++q) dma(q, 0, c0, true);
+#pragma unroll
+  for (int q = 0; q < LPS / 2; ++q) dma(q, 1, c0 + 1, nst > 1);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the scales are in LDS)
+  __builtin_amdgcn_s_waitcnt(vm_wait(LPS / 2));
+  asm volatile("s_barrier" ::: "memory");
+  read_scales(0);
+  read_a(lds0, c0_, c0_, c0_);
+  read_a(lds0, c0_, c0_, c1_);
+  read_a(lds0, c0_, c1_, c0_);
+  read_a(lds0, c0_, c1_, c1_);
+  unrolled<4>([&](auto n) { read_b(lds0, n); });
+  // step 0 of stage st: B fragment n is in once at most the reads after its own are out; the second half of the
+  // next stage's loads; at its end the A fragments of step 1 are in
+  auto step0 = [&](int st) {
+    const int buf = st & 1;
+    const uint32_t base = lds0 + (uint32_t)(buf * STAGE);
+    __builtin_amdgcn_s_setprio(1);
+    unrolled<4>([&](auto n) {
+      // allowed: the later B fragments' reads, and the A reads issued so far in this step
+      asm_wait_lgkm<2 * (3 - n) + (n == 0 ? 0 : n == 1 ? 2 : 4)>();
+      if constexpr (n == 0) {
+        sa_next.tie();
+        asm volatile("" : "+v"(sb_next));
+        sa = sa_next;
+        sb = sb_next;
+        fa[0][0].tie();
+        fa[0][1].tie();
+      }
+      fb[n].tie();
+      fence();
+      mma(c0_, n);
+      dma(LPS / 2 + n, buf ^ 1, c0 + st + 1, st + 1 < nst);
+      fence();
+      mma(c1_, n);
+      if constexpr (n < 2) {
+        read_a(base, c1_, integral_constant<int, 2 + n>{}, c0_);
+        read_a(base, c1_, integral_constant<int, 2 + n>{}, c1_);
+      }
+      fence();
+    });
+    __builtin_amdgcn_s_setprio(0);
+    asm_wait_lgkm<0>();
+    fa[1][0].tie();
+    fa[1][1].tie();
+  };
+  // steps 1 and 2
+  auto steps12 = [&](int st) {
+    const uint32_t base = lds0 + (uint32_t)((st & 1) * STAGE);
+    unrolled<2>([&](auto t) {
+      constexpr int m0 = 2 + 2 * t;  // this step's fragments; the next step's: m0 + 2
+      fence();
+      unrolled<4>([&](auto n) {
+        mma(integral_constant<int, m0>{}, n);
+        if constexpr (n < 2) read_a(base, integral_constant<int, t>{}, integral_constant<int, m0 + 2 + n>{}, c0_);
+        fence();
+        mma(integral_constant<int, m0 + 1>{}, n);
+        if constexpr (n < 2) read_a(base, integral_constant<int, t>{}, integral_constant<int, m0 + 2 + n>{}, c1_);
+        fence();
+      });
+      asm_wait_lgkm<0>();
+      fa[t][0].tie();
+      fa[t][1].tie();
+    });
+  };
+  // step 3 of a stage with one after it
+  auto step3 = [&](int st) {
+    const int buf = st & 1;
+    const uint32_t next = lds0 + (uint32_t)((buf ^ 1) * STAGE);
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));
+    asm volatile("s_barrier" ::: "memory");
+    fence();
+    __builtin_amdgcn_s_setprio(1);
+    read_scales(st + 1);
+    unrolled<4>([&](auto n) {
+      mma(integral_constant<int, 6>{}, n);
+      dma(n, buf, c0 + st + 2, st + 2 < nst);
+      fence();
+      mma(integral_constant<int, 7>{}, n);
+      if constexpr (n == 0) {
+        read_a(next, c0_, c0_, c0_);
+        read_a(next, c0_, c0_, c1_);
+        read_a(next, c0_, c1_, c0_);
+        read_a(next, c0_, c1_, c1_);
+      }
+      read_b(next, n);
+      fence();
+    });
+  };
+  // The loop closes where no LDS read is out: a register copy that the compiler puts on its back edge must not
+  // meet one whose data is still coming.
+  step0(0);
+  for (int st = 0; st + 1 < nst; ++st) {
+    steps12(st);
+    step3(st);
+    step0(st + 1);
+  }
+  steps12(nst - 1);
+  unrolled<4>([&](auto n) {
+    mma(integral_constant<int, 6>{}, n);
+    mma(integral_constant<int, 7>{}, n);
+  });
+  __builtin_amdgcn_s_setprio(0);
+}
+
 template <int BM, int BN, int NW, int NS, int EPI>
 __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
   extern __shared__ __align__(128) char smem[];
@@ -321,6 +466,7 @@ __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
   using L = Lds8<BM, BN, NW, NS>;
   constexpr int MF = G::MF, NF = G::NF;
   constexpr int NT = NW * 64;
+  constexpr bool PIPE = BM == 256 && BN == 256 && NW == 8 && NS == 2;
   static_assert(EPI != F8_GLU || BN == 256, "one block of 128 pairs a tile");
 
   RowsTile tile;
@@ -374,16 +520,17 @@ __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
     }
     lb.set(q, ok ? (uint32_t)((int64_t)n * ((int64_t)p.nk * kBlk)) : kOOB);
   }
-  auto issue = [&](int buf, int kt, bool on) {
-    const int64_t k0 = (int64_t)kt * kBlk;
-    const int64_t ra = (int64_t)a_bytes - k0, rb = (int64_t)p.b_bytes - k0;
-    const __amdgpu_buffer_rsrc_t rsa = make_rsrc(a_base + k0, on && ra > 0 ? (uint32_t)ra : 0u);
-    const __amdgpu_buffer_rsrc_t rsb = make_rsrc(b_base + k0, on && rb > 0 ? (uint32_t)rb : 0u);
+  // load q of this wave's LPS of stage kt into buffer buf (zeros when !on)
+  auto dma = [&](int q, int buf, int kt, bool on) {
+    const int64_t k0 = (int64_t)kt * kBlk, room = (q < NQA ? (int64_t)a_bytes : (int64_t)p.b_bytes) - k0;
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc((q < NQA ? a_base : b_base) + k0, on && room > 0 ? (uint32_t)room : 0u);
     lds_char* st = lds + buf * L::kStage;
+    if (q < NQA) buf_to_lds(rs, st + (wave * NQA + q) * 1024, la.off[q < NQA ? q : 0]);
+    else buf_to_lds(rs, st + BM * kBlk + (wave * NQB + q - NQA) * 1024, lb.off[q < NQA ? 0 : q - NQA]);
+  };
+  auto issue = [&](int buf, int kt, bool on) {
 #pragma unroll
-    for (int q = 0; q < NQA; ++q) buf_to_lds(rsa, st + (wave * NQA + q) * 1024, la.off[q]);
-#pragma unroll
-    for (int q = 0; q < NQB; ++q) buf_to_lds(rsb, st + BM * kBlk + (wave * NQB + q) * 1024, lb.off[q]);
+    for (int q = 0; q < LPS; ++q) dma(q, buf, kt, on);
   };
 
   f32x4_t acc[MF][NF];
@@ -421,62 +568,66 @@ __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
       const int64_t last = EPI == F8_GLU ? 2 * blocks_of(p.half) - 1 : blocks_of(p.N) - 1;
       b_scales[2 * st + j] = bs[(nb < last ? nb : last) * p.bs_pitch + c0 + st];
     }
+    if constexpr (PIPE) {
+      piped_loop<EPI == F8_GLU, BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma);
+    } else {
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) issue(i, c0 + i, i < nst);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int i = 0; i < NS - 1; ++i) issue(i, c0 + i, i < nst);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 
-    int cur = 0;
-    for (int st = 0; st < nst; ++st) {
-      __builtin_amdgcn_s_waitcnt(vm_wait((NS - 2) * LPS));  // this wave's loads of stage st are in
-      asm volatile("s_barrier" ::: "memory");               // everyone's are, and the buffer before is read
-      issue(cur == 0 ? NS - 1 : cur - 1, c0 + st + NS - 1, st + NS - 1 < nst);
-      const uint32_t base = lds0 + (uint32_t)(cur * L::kStage);
-      AScale<MF> sa;
-      uint32_t sb;
-      sa.read(as_lane + (uint32_t)(st * BM));
-      if constexpr (EPI == F8_GLU) asm volatile("ds_read_u16 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
-      else asm volatile("ds_read_u8 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
-      Frag8 fb[NF];
-      unrolled<NF>([&](auto n) {
-        fb[n].lo = ds_read128<n * 2048>(base + b_frag);
-        fb[n].hi = ds_read128<n * 2048>((base + b_frag) ^ 64u);
-      });
-      constexpr int HF = MF < 4 ? MF : 4, STEPS = MF / HF;
-      Frag8 fa[2][HF];
-      auto read_a = [&](auto s) {
-        unrolled<HF>([&](auto m) {
-          fa[s & 1][m].lo = ds_read128<(s * HF + m) * 2048>(base + a_frag);
-          fa[s & 1][m].hi = ds_read128<(s * HF + m) * 2048>((base + a_frag) ^ 64u);
+      int cur = 0;
+      for (int st = 0; st < nst; ++st) {
+        __builtin_amdgcn_s_waitcnt(vm_wait((NS - 2) * LPS));  // this wave's loads of stage st are in
+        asm volatile("s_barrier" ::: "memory");               // everyone's are, and the buffer before is read
+        issue(cur == 0 ? NS - 1 : cur - 1, c0 + st + NS - 1, st + NS - 1 < nst);
+        const uint32_t base = lds0 + (uint32_t)(cur * L::kStage);
+        AScale<MF> sa;
+        uint32_t sb;
+        sa.read(as_lane + (uint32_t)(st * BM));
+        if constexpr (EPI == F8_GLU) asm volatile("ds_read_u16 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+        else asm volatile("ds_read_u8 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+        Frag8 fb[NF];
+        unrolled<NF>([&](auto n) {
+          fb[n].lo = ds_read128<n * 2048>(base + b_frag);
+          fb[n].hi = ds_read128<n * 2048>((base + b_frag) ^ 64u);
         });
-      };
-      read_a(std::integral_constant<int, 0>{});
-      unrolled<STEPS>([&](auto s) {
-        if constexpr (s + 1 < STEPS) {
-          read_a(std::integral_constant<int, s + 1>{});
-          asm_wait_lgkm<2 * HF>();  // (in order: at most the next step's reads are out)
-        } else {
-          asm_wait_lgkm<0>();
-        }
-        if constexpr (s == 0) {
-          sa.tie();
-          asm volatile("" : "+v"(sb));
-#pragma unroll
-          for (int n = 0; n < NF; ++n) fb[n].tie();
-        }
-#pragma unroll
-        for (int m = 0; m < HF; ++m) fa[s & 1][m].tie();
-        __builtin_amdgcn_sched_barrier(0);
-        unrolled<HF>([&](auto m) {
-          unrolled<NF>([&](auto n) {
-            constexpr int f = s * HF + m;
-            acc[f][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                fb[n].value(), fa[s & 1][m].value(), acc[f][n], 0, 0, EPI == F8_GLU ? n / 2 : 0, (int)sb, f & 3,
-                (int)sa.w[f / 4]);
+        constexpr int HF = MF < 4 ? MF : 4, STEPS = MF / HF;
+        Frag8 fa[2][HF];
+        auto read_a = [&](auto s) {
+          unrolled<HF>([&](auto m) {
+            fa[s & 1][m].lo = ds_read128<(s * HF + m) * 2048>(base + a_frag);
+            fa[s & 1][m].hi = ds_read128<(s * HF + m) * 2048>((base + a_frag) ^ 64u);
           });
+        };
+        read_a(std::integral_constant<int, 0>{});
+        unrolled<STEPS>([&](auto s) {
+          if constexpr (s + 1 < STEPS) {
+            read_a(std::integral_constant<int, s + 1>{});
+            asm_wait_lgkm<2 * HF>();  // (in order: at most the next step's reads are out)
+          } else {
+            asm_wait_lgkm<0>();
+          }
+          if constexpr (s == 0) {
+            sa.tie();
+            asm volatile("" : "+v"(sb));
+#pragma unroll
+            for (int n = 0; n < NF; ++n) fb[n].tie();
+          }
+#pragma unroll
+          for (int m = 0; m < HF; ++m) fa[s & 1][m].tie();
+          __builtin_amdgcn_sched_barrier(0);
+          unrolled<HF>([&](auto m) {
+            unrolled<NF>([&](auto n) {
+              constexpr int f = s * HF + m;
+              acc[f][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                  fb[n].value(), fa[s & 1][m].value(), acc[f][n], 0, 0, EPI == F8_GLU ? n / 2 : 0, (int)sb, f & 3,
+                  (int)sa.w[f / 4]);
+            });
+          });
+          __builtin_amdgcn_sched_barrier(0);
         });
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      cur = cur == NS - 1 ? 0 : cur + 1;
+        cur = cur == NS - 1 ? 0 : cur + 1;
+      }
     }
     __builtin_amdgcn_s_waitcnt(vm_wait(0));  // loads past the end (zeros) are done before LDS is reused
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
