@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
 // LDS (the geometry of 64 bf16 elements), one 16 x 16 x 128 MFMA per 16 x 16 outputs. The weight rows
 // are the MFMA's first operand, so a lane ends up with 4 consecutive output columns of one row.
 // F8_HALF: rows that a sum over a token's k slots reads next, as f16 with a power-of-two scale for each 64 columns:
-// 16 bits like bf16, but within 2^-12 of each value (bf16: 2^-9), so that the sum has its own rounding only.
+// 16 bits like bf16, but within 2^-11 of each value (bf16: 2^-8), so that the sum has its own rounding only.
 enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2, F8_HALF = 3 };
 constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 
@@ -459,8 +459,70 @@ __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint3
   __builtin_amdgcn_s_setprio(0);
 }
 
+// The K loop of 128 x 256 tiles on four waves, two workgroups a CU (128 x 64 outputs a wave): one LDS buffer, the
+// stage's fragments in registers.
+template <bool GLU, int BM, int LPS, typename Dma>
+__device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
+                                            uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma) {
+  static_assert(LPS == 12, "twelve loads a stage");
+  Frag8 fa[8], fb[4];
+  AScale<8> sa;
+  uint32_t sb;
+  auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+  auto read_a = [&](auto m) {
+    fa[m].lo = ds_read128<m * 2048>(lds0 + a_frag);
+    fa[m].hi = ds_read128<m * 2048>((lds0 + a_frag) ^ 64u);
+  };
+  using std::integral_constant;
+#pragma unroll
+  for (int q = 0; q < LPS; ++q) dma(q, 0, c0, true);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int st = 0; st < nst; ++st) {
+    __builtin_amdgcn_s_waitcnt(vm_wait(0));
+    asm volatile("s_barrier" ::: "memory");
+    fence();
+    sa.read(as_lane + (uint32_t)(st * BM));
+    if constexpr (GLU) asm volatile("ds_read_u16 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+    else asm volatile("ds_read_u8 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+    unrolled<4>([&](auto n) {
+      fb[n].lo = ds_read128<n * 2048>(lds0 + b_frag);
+      fb[n].hi = ds_read128<n * 2048>((lds0 + b_frag) ^ 64u);
+    });
+    read_a(integral_constant<int, 0>{});
+    read_a(integral_constant<int, 1>{});
+    unrolled<8>([&](auto m) {
+      // (reads return in order) allowed: A fragments after m that are out
+      if constexpr (m < 4) asm_wait_lgkm<(m == 0 ? 2 : m == 1 ? 4 : m == 2 ? 6 : 8)>();
+      if constexpr (m == 0) {
+        sa.tie();
+        asm volatile("" : "+v"(sb));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) fb[n].tie();
+      }
+      if constexpr (m < 4) fa[m].tie();
+      if constexpr (m < 3) {
+        read_a(integral_constant<int, 2 * m + 2>{});
+        read_a(integral_constant<int, 2 * m + 3>{});
+      }
+      fence();
+      unrolled<4>([&](auto n) {
+        acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[n].value(), fa[m].value(), acc[m][n], 0, 0,
+                                                                    GLU ? n / 2 : 0, (int)sb, m & 3, (int)sa.w[m / 4]);
+        if constexpr (m >= 4 && n < 3) dma((m - 4) * 3 + n, 0, c0 + st + 1, st + 1 < nst);
+        fence();
+      });
+      if constexpr (m == 3) {  // everything is in registers: the buffer is the next stage's
+        asm_wait_lgkm<0>();
+#pragma unroll
+        for (int q = 4; q < 8; ++q) fa[q].tie();
+        asm volatile("s_barrier" ::: "memory");
+      }
+    });
+  }
+}
+
 template <int BM, int BN, int NW, int NS, int EPI>
-__global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
+__global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp8Params p) {
   extern __shared__ __align__(128) char smem[];
   using G = Grid8<BM, BN, NW>;
   using L = Lds8<BM, BN, NW, NS>;
@@ -568,7 +630,9 @@ __global__ __launch_bounds__(NW * 64, 1) void fp8_rows_kernel(Fp8Params p) {
       const int64_t last = EPI == F8_GLU ? 2 * blocks_of(p.half) - 1 : blocks_of(p.N) - 1;
       b_scales[2 * st + j] = bs[(nb < last ? nb : last) * p.bs_pitch + c0 + st];
     }
-    if constexpr (PIPE) {
+    if constexpr (NS == 1) {
+      single_loop<EPI == F8_GLU, BM, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma);
+    } else if constexpr (PIPE) {
       piped_loop<EPI == F8_GLU, BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma);
     } else {
 #pragma unroll
@@ -826,6 +890,85 @@ __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __res
   }
 }
 
+// ------------------------------------------------------------------ a few rows against one weight
+// At most 32 rows read the weight once and hardly compute: a workgroup takes 16 columns, its eight waves share out
+// the depth, and each wave loads its part of the weight straight into the matrix instruction's registers, up to four
+// blocks of 128 ahead, with no LDS and no barrier before the one sum over the waves (in their order).
+// One row, 2048 -> 1536: 4.1 us, 4096 -> 4096: 4.7, 16384 -> 4096: 13 (5.2 TB/s, the copy rate); 32 rows 5.3, 10.1
+// and 30.8. Tiles of 32 x 128 that walk the whole depth: 8.9, 14.4, 48 for one row, 9.1, 14.7, 49 for 32. At 64 rows
+// the two are level (8.0 and 9.1, 16.0 and 15.1, 52 and 49), as every workgroup reads all rows here.
+constexpr int kFewWaves = 8;
+constexpr int kCus = 256;
+
+template <int MF, int U, int EPI>
+__global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
+  __shared__ float part[kFewWaves][16][20];
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lane = (int)threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int col0 = (int)blockIdx.x * 16, rows = p.ns_m;
+  const int each = (p.nk + kFewWaves - 1) / kFewWaves, k0 = wave * each;
+  const int cnt = p.nk - k0 < each ? p.nk - k0 : each;  // (may be below 1)
+
+  // rows and columns past the end repeat the last one: their outputs are not stored
+  const int n = col0 + r16 < p.N ? col0 + r16 : p.N - 1;
+  const uint8_t *a[MF], *as[MF], *b = p.b + (int64_t)n * p.lda + (int64_t)k0 * kBlk + 16 * g4;
+  const uint8_t* bs = p.bs + (int64_t)(col0 / kBlk) * p.bs_pitch + k0;
+#pragma unroll
+  for (int m = 0; m < MF; ++m) {
+    const int r = 16 * m + r16 < rows ? 16 * m + r16 : rows - 1;
+    a[m] = p.a + (int64_t)r * p.lda + (int64_t)k0 * kBlk + 16 * g4;
+    as[m] = p.as + (int64_t)r * p.a_pitch + k0;
+  }
+  f32x4_t acc[MF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto load = [](const uint8_t* q) { return *reinterpret_cast<const v4i32_t*>(q); };
+  for (int i = 0; i < cnt; i += U) {
+    Frag8 fb[U], fa[U][MF];
+    int sb[U], sa[U][MF];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int kb = i + u < cnt ? i + u : cnt - 1;
+      sb[u] = bs[kb];
+      fb[u].lo = load(b + (int64_t)kb * kBlk);
+      fb[u].hi = load(b + (int64_t)kb * kBlk + 64);
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
+        fa[u][m].lo = load(a[m] + (int64_t)kb * kBlk);
+        fa[u][m].hi = load(a[m] + (int64_t)kb * kBlk + 64);
+        sa[u][m] = as[m][kb];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads first
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < cnt) {
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+          acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[u].value(), fa[u][m].value(), acc[m], 0, 0, 0,
+                                                                   sb[u], 0, sa[u][m]);
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < MF; ++m) {
+    if (m) __syncthreads();
+    *reinterpret_cast<f32x4_t*>(&part[wave][r16][4 * g4]) = acc[m];
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      const int r = (int)threadIdx.x >> 4, c = (int)threadIdx.x & 15;
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) v += part[w][r][c];
+      if (16 * m + r < rows && col0 + c < p.N) {
+        const int64_t at = (int64_t)(16 * m + r) * p.ldc + col0 + c;
+        if constexpr (EPI == F8_STORE_F32) static_cast<float*>(p.c)[at] = v;
+        else static_cast<uint16_t*>(p.c)[at] = bf16_bits(v);
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------ host side
 template <int BM, int BN, int NW, int NS, int EPI>
 int launch8(Fp8Params p, int64_t R, hipStream_t s) {
@@ -841,13 +984,47 @@ int launch8(Fp8Params p, int64_t R, hipStream_t s) {
   return check_launch("fp8 rows kernel");
 }
 
+template <int MF, int U, int EPI>
+int launch_few(const Fp8Params& p, hipStream_t s) {
+  auto kern = fp8_few_kernel<MF, U, EPI>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(p.N, 16)), dim3(kFewWaves * 64), 0, s, p);
+  return check_launch("fp8 few rows kernel");
+}
+
+// The tile. Wider ones read the operands less often (a 128-deep step of 256 x 256 is 64 KB for 16.8 MFLOP, of 64 x 128
+// 24 KB for 2.1), narrower ones leave less of a short expert's last tile empty and put more workgroups on the 256 CUs.
+//  - Experts of a few rows: what counts is the weight's stream. 128 experts of 2048 -> 2 x 768 and back, 16 rows each:
+//    GLU 84.6 us with 32 rows a tile, 89.7 with 128; back 44.2 with 64 x 128, 45.6 with 128 x 256. 32 rows each: 107.6
+//    against 90.9, and 47 against 47.
+//  - A launch that fits on the CUs at once takes the narrowest tile with which it still does. 4096 -> 4096: 1000 rows
+//    27.6 us (64 x 128), 31.4 (128 x 128), 45 (128 x 256); 2048 rows 47.8, 39.2, 47.6; 128 rows 15.4 (32 x 128), 19.1.
+//    GLU, 4096 -> 2 x 4096: 500 rows 52 (32), 36 (64), 42 (128); 1000 rows 98, 68, 46; 128 x 256 on four waves 51.
+//  - Else 128 x 256 on four waves, two workgroups a CU: one's prologue and epilogue run under the other's loop. Long
+//    loops over long experts want 256 x 256 (outputs/loop step): 8192 x 7168 -> 4096 198 us against 226, 16384 x 2048
+//    -> 2048 64 against 66; but 65536 x 1536 -> 2048 over 64 experts 297 against 293, and, where rows are skewed over
+//    the experts (16384 of them, 2048 -> 7168, 64 experts), 436 against 370. GLU has a longer epilogue: 262144 rows,
+//    2048 -> 2 x 768, 128 experts 924 against 883; 8000 rows 4096 -> 2 x 4096 223 against 229.
 template <int EPI>
 int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
   const int64_t per = R / p.E;
-  if (per <= 32) return launch8<32, 256, 4, 4, EPI>(p, R, s);
-  if (per <= 96) return launch8<64, 256, 4, 3, EPI>(p, R, s);
-  if (per <= 192) return launch8<128, 256, 8, 3, EPI>(p, R, s);
-  return launch8<256, 256, 8, 2, EPI>(p, R, s);
+  const int n = EPI == F8_GLU ? 2 * p.half : p.N;
+  const auto fits = [&](int bm, int bn) { return (cdiv(R, bm) + (p.offsets ? p.E : 0)) * cdiv(n, bn) <= kCus; };
+  const bool few = p.offsets && per <= 24, longest = per >= 1024 && p.nk >= (EPI == F8_GLU ? 32 : 16);
+  if constexpr (EPI == F8_GLU) {
+    if (few || fits(32, 256)) return launch8<32, 256, 4, 4, EPI>(p, R, s);
+    if (fits(64, 256)) return launch8<64, 256, 4, 3, EPI>(p, R, s);
+    if (fits(128, 256)) return launch8<128, 256, 8, 3, EPI>(p, R, s);
+  } else {
+    if constexpr (EPI != F8_HALF) {
+      if (!p.offsets && R <= 16) return launch_few<1, 4, EPI>(p, s);
+      if (!p.offsets && R <= 32) return launch_few<2, 2, EPI>(p, s);
+    }
+    if (!few && fits(32, 128)) return launch8<32, 128, 4, 4, EPI>(p, R, s);
+    if (few || fits(64, 128)) return launch8<64, 128, 4, 3, EPI>(p, R, s);
+    if (fits(128, 128)) return launch8<128, 128, 4, 2, EPI>(p, R, s);
+  }
+  if (longest) return launch8<256, 256, 8, 2, EPI>(p, R, s);
+  return launch8<128, 256, 4, 1, EPI>(p, R, s);
 }
 
 constexpr int64_t kMaxSpan8 = 0x7fff0000LL;  // bytes that a buffer resource addresses

@@ -123,9 +123,9 @@ def test_quantize_weight(E, N, K, dtype, hip_device):
     assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2[..., :kb], s[..., :kb])
 
 
-def check(got, ref, S, G, K):
+def check(got, ref, S, G, K, half=None):
     assert got.shape == ref.shape and not torch.isnan(got).any()
-    half = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+    half = half or (2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24)
     b = half * ref.abs() + 7 * 2.0 ** -13 * G + 17 * -(-K // 128) * 2.0 ** -23 * S
     err = (got.double() - ref).abs()
     worst = float((err / b.clamp(min=1e-300)).max()) if err.numel() else 0.0
@@ -157,3 +157,60 @@ def test_grouped_product(T, E, k, N, K, skew, xg, yg, hip_device):
     ref = O.grouped_product(O.quantize_rows(x)[0], O.quantize_weight(W)[0], ss, off, k, xg, yg)
     got = z().fp8_scatter2scatter(*z().fp8_quantize_rows(x), *z().fp8_quantize_weight(W), K, ss, off, 1 if xg else k, xg, yg)
     check(got, *ref, K)
+
+
+def some(n, count, seed):
+    """The first and last of n and some others, in order."""
+    if n <= count:
+        return torch.arange(n)
+    mid = torch.randperm(n - 2, generator=gen(seed))[:count - 2] + 1
+    return torch.cat([torch.tensor([0, n - 1]), mid]).sort().values
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(8, 4100, 1160), (16, 33, 8300), (17, 1030, 640), (32, 1500, 130), (40, 300, 8400),
+                                   (500, 2000, 300), (1000, 1500, 640), (900, 4000, 512), (1100, 5100, 200),
+                                   (4200, 2304, 384), (900, 9000, 8330), (4200, 2050, 2100), (2100, 4100, 8330)])
+def test_dense_product_tiles(M, N, K, out, hip_device):
+    """Sizes for every tile (few rows, launches that fit on the CUs at once, long ones), sampled rows and columns."""
+    from zmoe import _lib as L
+
+    x = activations(M, K, torch.bfloat16, M + K, hip_device)
+    W = (torch.randn(N, K, generator=gen(N)) * 0.1).to(torch.bfloat16).to(hip_device)
+    Y = torch.full((M + 1, N + 3), 7.0, dtype=DT[out], device=hip_device)  # a stride of its own, a row behind
+    (xq, xs), (wq, ws) = z().fp8_quantize_rows(x), z().fp8_quantize_weight(W)
+    L.call("zmoe_fp8_scatter2scatter", xq.data_ptr(), xs.data_ptr(), M, wq.data_ptr(), ws.data_ptr(), None, None, K, N, 1,
+           1, 1, 1, {"f32": L.DTYPE_F32, "bf16": L.DTYPE_BF16}[out], Y.data_ptr(), N + 3,
+           torch.cuda.current_stream().cuda_stream)
+    assert bool((Y[M] == 7.0).all()) and bool((Y[:, N:] == 7.0).all())
+    ri, ci = some(M, 32, 1).to(hip_device), some(N, 96, 2).to(hip_device)
+    got = Y[:M, :N][ri][:, ci]
+    ref = O.product(O.quantize_rows(x)[0][ri], O.quantize_weight(W)[0][ci])
+    check(got, *ref, K)
+
+
+@pytest.mark.parametrize("T,E,k,N,K", [(700, 40, 1, 1500, 384), (60, 2, 2, 500, 200), (2000, 4, 2, 500, 300),
+                                       (2600, 16, 2, 1100, 300), (4300, 4, 1, 770, 2050), (6000, 3, 1, 2304, 2100),
+                                       (300, 64, 4, 600, 130)])
+@pytest.mark.parametrize("half", [False, True])
+def test_grouped_product_tiles(T, E, k, N, K, half, hip_device):
+    """The same by expert, bf16 rows and f16 ones with their scales (half a step is 2^-11 |y|, and at most 2^-39 of the
+    largest of 64 columns: below the bound's S term, whose columns here differ by far less than 2^20)."""
+    idx = random_topk(T, E, k, T + E, 0.0).to(hip_device)
+    _, ss, off, _ = z().flatten_sort_count(idx, E)
+    x = activations(T, K, torch.bfloat16, T, hip_device)
+    W = (torch.randn(E, N, K, generator=gen(N)) * 0.1).to(torch.bfloat16).to(hip_device)
+    q, w = z().fp8_quantize_rows(x), z().fp8_quantize_weight(W)
+    ri, ci = some(T * k, 32, 1).to(hip_device), some(N, 96, 2).to(hip_device)
+    slots = ss[ri]
+    experts = idx.flatten()[slots]
+    xr, wr = O.quantize_rows(x)[0][slots // k], O.quantize_weight(W)[0]
+    parts = [O.product(xr[i:i + 1], wr[int(e)][ci]) for i, e in enumerate(experts)]
+    ref = [torch.cat([p[j] for p in parts]) for j in range(len(parts[0]))]
+    if half:
+        y, s = z().fp8_scatter2scatter_half(*q, *w, K, ss, off, k, False, False)
+        cols = torch.arange(y.shape[1], device=hip_device)
+        v = y.double() * torch.exp2(s.double()[:, cols // 64] - 127)  # (2^c exact in float64)
+        check(v[slots][:, ci], *ref, K, half=2.0 ** -11)
+    else:
+        check(z().fp8_scatter2scatter(*q, *w, K, ss, off, k, False, False)[slots][:, ci], *ref, K)

@@ -9,7 +9,7 @@ import torch.nn as nn
 
 from helpers import gen, random_topk
 from oracle import fp8_oracle as O
-from test_gpu_fp8 import activations, check
+from test_gpu_fp8 import activations, check, some
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +86,28 @@ def test_swiglu_grouped(T, d, f, E, k, skew, hip_device):
         if end > beg:
             swiglu_check(aq[beg:end], as_[beg:end], f, xr[ss[beg:end] // k], wr[2 * e], wr[2 * e + 1], d)
         beg = end
+
+
+@pytest.mark.parametrize("T,d,f,E,k", [(600, 300, 1700, 1, 1), (1100, 256, 2000, 1, 1), (1500, 200, 3000, 1, 1),
+                                       (1500, 4100, 3000, 1, 1), (1000, 8300, 4300, 1, 1), (2000, 300, 520, 16, 2),
+                                       (6000, 260, 520, 16, 2), (5000, 4100, 1200, 3, 1)])
+def test_swiglu_tiles(T, d, f, E, k, hip_device):
+    """Sizes for every tile, sampled rows."""
+    from zmoe import ops
+
+    x, W1 = activations(T, d, BF, T, hip_device), weight((2 * E, f, d), f, BF, hip_device)
+    idx = random_topk(T, E, k, T, 0.0).to(hip_device) if E > 1 else torch.zeros(T, 1, dtype=torch.int64, device=hip_device)
+    w1q, w1s = zl().fp8_quantize_weight(W1, False)
+    _, ss, off, _ = ops.flatten_sort_count(idx, E)
+    route = (ss, off, k) if E > 1 else ()
+    aq, as_ = ops.fp8_glu_w1_forward(*ops.fp8_quantize_rows(x), w1q, w1s, d, *route)
+    wr, xr = O.quantize_weight(W1)[0], O.quantize_rows(x)[0]
+    ri = some(T * k, 24, 3).to(hip_device)
+    slots = ss[ri] if E > 1 else ri
+    experts = idx.flatten()[slots]
+    for e in experts.unique().tolist():
+        at = ri[experts == e]
+        swiglu_check(aq[at], as_[at], f, xr[slots[experts == e] // k], wr[2 * e], wr[2 * e + 1], d)
 
 
 # ------------------------------------------------------------------ fp8_linear
