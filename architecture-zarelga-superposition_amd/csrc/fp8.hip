@@ -234,15 +234,14 @@ struct Lds8 {
   static constexpr int kPitch = 64 * 2 + 16;  // staged output rows, bf16
   static constexpr int stages = NS * kStage;
   static constexpr int glu = BM * kBlk + 4 * BM * 4;  // quantised tile, row maxima of four waves
-  static constexpr int staging = NW * 32 * kPitch;
+  static constexpr int kRows = Grid8<BM, BN, NW>::WM < 64 ? Grid8<BM, BN, NW>::WM : 64;  // rows a wave stages at once
+  static constexpr int staging = NW * kRows * kPitch;
   static constexpr int ops = stages > glu ? (stages > staging ? stages : staging) : (glu > staging ? glu : staging);
   static constexpr int a_scales = ops;
   static constexpr int b_scales = a_scales + kScaleStages * BM;
-  static constexpr int src = b_scales + kScaleStages * 2;
-  static constexpr int dst = src + BM * 4;
+  static constexpr int dst = b_scales + kScaleStages * 2;
   static constexpr int total = dst + BM * 4;
-  static constexpr int decode = (kGemmMaxE + 4 + 16) * 4;
-  static_assert(total <= 163840 && decode <= ops, "LDS of one CU");
+  static_assert(total <= 163840, "LDS of one CU");
 };
 
 template <int OFF>
@@ -298,6 +297,84 @@ __device__ __forceinline__ void unrolled(F f) {
 
 __device__ __forceinline__ int swizzle8(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
+constexpr uint32_t kInfBits = 0x7f800000u;  // magnitudes from here on: inf, NaN
+// Largest magnitude of v and m, as bits (two instructions for two values, and inf and NaN show).
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const f32x4_t& v) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) m = max(m, __float_as_uint(v[u]) & 0x7fffffffu);
+  return m;
+}
+// Largest over the four lanes that hold one row (lane % 16).
+__device__ __forceinline__ uint32_t max_rows4(uint32_t v) {
+  auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max((uint32_t)a[0], (uint32_t)a[1]);
+  a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max((uint32_t)a[0], (uint32_t)a[1]);
+}
+
+// decode_rows_tile, each wave for itself: no LDS and no barrier in the chain of loads that a tile begins with.
+template <int BM, typename P>
+__device__ __forceinline__ bool decode_rows_wave(const P& p, RowsTile& t) {
+  if (p.ns_m > 0) {
+    const int nm = (p.ns_m + BM - 1) / BM, logical = xcd_logical_tile(nm * p.n_tiles);
+    if (logical < 0) return false;
+    expert_tile_order(logical, p.n_tiles, nm, t.nt, t.mt);
+    t.e = 0;
+    t.row0 = (int64_t)t.mt * BM;
+    t.rows = min(BM, p.ns_m - t.mt * BM);
+    return true;
+  }
+  // a lane counts the row tiles of its ept consecutive experts (rows are below 2^31: the ends' low words)
+  const int lane = (int)threadIdx.x & 63, ept = (p.E + 63) / 64, e0 = lane * ept;
+  const int* ends = reinterpret_cast<const int*>(p.offsets);
+  auto end_of = [&](int e) { return e >= 0 ? ends[2 * (e < p.E ? e : p.E - 1)] : 0; };
+  int local = 0, singles = 0;
+  for (int q0 = 0; q0 < ept; q0 += 4) {
+    int end[5];
+#pragma unroll
+    for (int q = 0; q < 5; ++q) end[q] = end_of(e0 + q0 + q - 1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = q0 + q < ept && end[q + 1] > end[q] ? (end[q + 1] - end[q] + BM - 1) / BM : 0;
+      local += n;
+      singles += __builtin_popcountll(__builtin_amdgcn_ballot_w64(n == 1));
+    }
+  }
+  int run = local;  // inclusive sums over the lanes
+  auto add = [&](auto ctrl, auto rows) {
+    run += __builtin_amdgcn_update_dpp(0, run, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // the row before's last lane, the lower half's
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  const int total = __builtin_amdgcn_readlane(run, 63) * p.n_tiles;
+  const int logical = 4 * singles > p.E ? slab_logical_tile(total) : xcd_logical_tile(total);  // (as there)
+  if (logical < 0) return false;
+  const uint64_t later = __builtin_amdgcn_ballot_w64(run * p.n_tiles > logical);
+  const int owner = __builtin_ctzll(later);  // (logical < total: some lane's sum is past it)
+  int rest = logical - (__builtin_amdgcn_readlane(run, owner) - __builtin_amdgcn_readlane(local, owner)) * p.n_tiles;
+  int e = owner * ept, beg = end_of(e - 1), end = end_of(e);
+  auto tiles_of = [&] { return end > beg ? (end - beg + BM - 1) / BM : 0; };
+  while (rest >= tiles_of() * p.n_tiles) {  // (ends at the lane's last expert at the latest)
+    rest -= tiles_of() * p.n_tiles;
+    beg = end;
+    end = end_of(++e);
+  }
+  int inner, outer;
+  const int nm = tiles_of();
+  expert_tile_order(rest, p.n_major ? nm : p.n_tiles, p.n_major ? p.n_tiles : nm, inner, outer);
+  t.e = e;
+  t.nt = p.n_major ? outer : inner;
+  t.mt = p.n_major ? inner : outer;
+  t.row0 = (int64_t)beg + (int64_t)t.mt * BM;
+  t.rows = min(BM, end - (int)t.row0);
+  return true;
+}
+
 // The lines this wave loads of each stage's operand: 8 rows an instruction (1 KB of LDS), lane i the
 // chunk (i % 8) ^ swizzle(row) of row i / 8.
 template <int ROWS, int NW>
@@ -323,9 +400,9 @@ struct Lines8 {
 // other MFMA: issued together they hold a wave for ~70 cycles each, with its partner on the SIMD in the same phase.
 // Waits count the LDS reads outstanding (they return in order). acc[m][n] as in the ring loop. GLU: B fragments 2 and 3
 // take the second scale.
-template <bool GLU, int BM, int STAGE, int LPS, typename Dma>
+template <bool GLU, int BM, int STAGE, int LPS, typename Dma, typename Fill>
 __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
-                                           uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma) {
+                                           uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma, Fill fill) {
   static_assert(LPS == 8, "eight loads a stage");
   Frag8 fa[2][2], fb[4];
   AScale<8> sa, sa_next;
@@ -354,9 +431,8 @@ __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint3
   const integral_constant<int, 0> c0_{};
   const integral_constant<int, 1> c1_{};
 #pragma unroll
-  for (int q = 0; q < LPS; ++q) dma(q, 0, c0, true);
-#pragma unroll
   for (int q = 0; q < LPS / 2; ++q) dma(q, 1, c0 + 1, nst > 1);
+  fill();
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the scales are in LDS)
   __builtin_amdgcn_s_waitcnt(vm_wait(LPS / 2));
   asm volatile("s_barrier" ::: "memory");
@@ -461,9 +537,9 @@ __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint3
 
 // The K loop of 128 x 256 tiles on four waves, two workgroups a CU (128 x 64 outputs a wave): one LDS buffer, the
 // stage's fragments in registers.
-template <bool GLU, int BM, int LPS, typename Dma>
+template <bool GLU, int BM, int LPS, typename Dma, typename Fill>
 __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
-                                            uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma) {
+                                            uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma, Fill fill) {
   static_assert(LPS == 12, "twelve loads a stage");
   Frag8 fa[8], fb[4];
   AScale<8> sa;
@@ -474,8 +550,7 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
     fa[m].hi = ds_read128<m * 2048>((lds0 + a_frag) ^ 64u);
   };
   using std::integral_constant;
-#pragma unroll
-  for (int q = 0; q < LPS; ++q) dma(q, 0, c0, true);
+  fill();
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   for (int st = 0; st < nst; ++st) {
     __builtin_amdgcn_s_waitcnt(vm_wait(0));
@@ -532,25 +607,28 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
   static_assert(EPI != F8_GLU || BN == 256, "one block of 128 pairs a tile");
 
   RowsTile tile;
-  if (!decode_rows_tile<BM, NT>(p, smem, tile)) return;  // uniform per workgroup
-  const int e = __builtin_amdgcn_readfirstlane(tile.e);
-  const int nt = __builtin_amdgcn_readfirstlane(tile.nt);
-  const int rows = tile.rows;
+  if (!decode_rows_wave<BM>(p, tile)) return;  // uniform per workgroup
+  const int e = tile.e, nt = tile.nt, rows = tile.rows;
   const int64_t row0 = tile.row0;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = (int)threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
   const int gm = wave / G::GN, gn = wave % G::GN;
   lds_char* lds = (lds_char*)(smem);
+  const uint32_t lds0 = lds_addr(lds);
 
-  // source and output row of each tile row (row numbers < 2^31: the low words of the int64 entries)
-  int* src_table = reinterpret_cast<int*>(smem + L::src);
+  // Before the loop a tile waits for memory three times in a row (the expert ends, its rows' numbers, their lines and
+  // scales), so nothing else stands between: each lane reads the numbers of the rows that it loads itself, the
+  // weight's lines go out before they are in, the scales before A's lines, and the scales' LDS writes come last.
+  // Row numbers are below 2^31: the low words of the int64 entries.
+  auto row_no = [&](const int64_t* list, int rl) {  // (rows past the tile's: its first)
+    rl = rl < rows ? rl : 0;
+    return list ? reinterpret_cast<const int*>(list)[2 * (row0 + rl)] : rl;
+  };
+  auto a_row = [&](int rl) {
+    const int r = row_no(p.a_rows, rl);
+    return p.a_rows ? (int)((uint32_t)r / (uint32_t)p.a_div) : r;
+  };
   int* dst_table = reinterpret_cast<int*>(smem + L::dst);
-  for (int rl = (int)threadIdx.x; rl < BM; rl += NT) {
-    const int64_t i = row0 + (rl < rows ? rl : 0);
-    src_table[rl] = p.a_rows ? reinterpret_cast<const int*>(p.a_rows)[2 * i] / p.a_div : rl;
-    dst_table[rl] = p.c_rows ? reinterpret_cast<const int*>(p.c_rows)[2 * i] : rl;
-  }
-  __syncthreads();
 
   // A from its first row (gathered) or from this tile's (contiguous rows: no limit on their number)
   const char* a_base = reinterpret_cast<const char*>(p.a) + (p.a_rows ? 0 : row0 * p.lda);
@@ -562,11 +640,6 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
   Lines8<BM, NW> la;
   Lines8<BN, NW> lb;
   constexpr int NQA = Lines8<BM, NW>::NQ, NQB = Lines8<BN, NW>::NQ, LPS = NQA + NQB;
-#pragma unroll
-  for (int q = 0; q < NQA; ++q) {
-    const int rl = la.row_of(q);
-    la.set(q, rl < rows ? (uint32_t)((int64_t)src_table[rl] * p.lda) : kOOB);
-  }
 #pragma unroll
   for (int q = 0; q < NQB; ++q) {
     const int rl = lb.row_of(q);
@@ -594,6 +667,15 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
 #pragma unroll
     for (int q = 0; q < LPS; ++q) dma(q, buf, kt, on);
   };
+#pragma unroll
+  for (int q = NQA; q < LPS; ++q) dma(q, 0, 0, true);
+#pragma unroll
+  for (int q = 0; q < NQA; ++q) {
+    const int rl = la.row_of(q);
+    la.set(q, rl < rows ? (uint32_t)((int64_t)a_row(rl) * p.lda) : kOOB);
+  }
+  constexpr int TPR = NT / BM, SW = kScaleStages / 4 / TPR;  // threads of a row, words of scales a thread takes at most
+  const int scales_row = a_row((int)threadIdx.x % BM);
 
   f32x4_t acc[MF][NF];
 #pragma unroll
@@ -601,42 +683,63 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
 #pragma unroll
     for (int n = 0; n < NF; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  const uint32_t lds0 = lds_addr(lds);
   const uint32_t frag_off = (uint32_t)(r16 * kBlk + ((g4 ^ swizzle8(r16)) << 4));
   const uint32_t a_frag = (uint32_t)(gm * G::WM * kBlk) + frag_off;
   const uint32_t b_frag = (uint32_t)((BM + gn * 64) * kBlk) + frag_off;
   const uint32_t as_lane = lds0 + L::a_scales + (uint32_t)((gm * 16 + r16) * MF);
   const uint32_t bs_lane = lds0 + L::b_scales + (EPI == F8_GLU ? 0u : (uint32_t)(gn / 2));
-  uint8_t* a_scales = reinterpret_cast<uint8_t*>(smem + L::a_scales);
-  uint8_t* b_scales = reinterpret_cast<uint8_t*>(smem + L::b_scales);
-
   for (int c0 = 0; c0 < p.nk; c0 += kScaleStages) {
     const int nst = p.nk - c0 < kScaleStages ? p.nk - c0 : kScaleStages;
-    // this tile's scales, [stage][rows in fragment order]: row gm WM + 16 m + r at (gm 16 + r) MF + m
     const int nd = (nst + 3) / 4;
-    for (int idx = (int)threadIdx.x; idx < BM * nd; idx += NT) {
-      const int rl = idx / nd, d4 = idx - rl * nd;
-      uint32_t w = 0x7f7f7f7fu;
-      if (rl < rows)
-        w = *reinterpret_cast<const uint32_t*>(as_base + (int64_t)src_table[rl] * p.a_pitch + c0 + 4 * d4);
-      const int at = ((rl / G::WM) * 16 + (rl & 15)) * MF + (rl % G::WM) / 16;
+    int tid = (int)threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (nothing that follows from it is worth a register throughout the loop)
+    const int srow = tid % BM, spart = tid / BM;
+    uint32_t sw[SW], bsw = 0;
+    int dst_row = 0;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) a_scales[(4 * d4 + u) * BM + at] = (uint8_t)(w >> (8 * u));
-    }
-    for (int idx = (int)threadIdx.x; idx < 2 * nst; idx += NT) {
-      const int j = idx & 1, st = idx >> 1;
-      const uint8_t* bs = p.bs + (int64_t)e * p.bs_estride;
-      const int64_t nb = EPI == F8_GLU ? (j ? blocks_of(p.half) : 0) + nt : (int64_t)nt * (BN / kBlk) + j;
+    for (int j = 0; j < SW; ++j)
+      if (spart + TPR * j < nd)
+        sw[j] = *reinterpret_cast<const uint32_t*>(as_base + (int64_t)scales_row * p.a_pitch + c0 + 4 * (spart + TPR * j));
+    if (tid < 2 * nst) {
+      const int64_t nb = EPI == F8_GLU ? (tid & 1 ? blocks_of(p.half) : 0) + nt : (int64_t)nt * (BN / kBlk) + (tid & 1);
       const int64_t last = EPI == F8_GLU ? 2 * blocks_of(p.half) - 1 : blocks_of(p.N) - 1;
-      b_scales[2 * st + j] = bs[(nb < last ? nb : last) * p.bs_pitch + c0 + st];
+      bsw = p.bs[(int64_t)e * p.bs_estride + (nb < last ? nb : last) * p.bs_pitch + c0 + (tid >> 1)];
     }
+    if (c0 == 0) dst_row = row_no(p.c_rows, srow);
+    if (c0 > 0) {
+#pragma unroll
+      for (int q = NQA; q < LPS; ++q) dma(q, 0, c0, true);
+    }
+#pragma unroll
+    for (int q = 0; q < NQA; ++q) dma(q, 0, c0, true);
+    // scales are kept as [stage][rows in fragment order]: row gm WM + 16 m + r at (gm 16 + r) MF + m
+    // (asm: the compiler would have an LDS write wait for every load to LDS)
+    auto fill = [&] {
+      const uint32_t at = lds0 + L::a_scales + (uint32_t)(((srow / G::WM) * 16 + (srow & 15)) * MF + (srow % G::WM) / 16) +
+                          (uint32_t)(spart * 4 * BM);
+      unrolled<SW>([&](auto j) {
+        if (spart + TPR * j < nd) {
+          const uint32_t to = at, w = sw[j];
+          unrolled<4>([&](auto u) {
+            const uint32_t to_ = to, v = w >> (8 * u);
+            asm volatile("ds_write_b8 %0, %1 offset:%2" ::"v"(to_), "v"(v), "n"((TPR * decltype(j)::value * 4 + u) * BM)
+                         : "memory");
+          });
+        }
+      });
+      if (tid < 2 * nst)
+        asm volatile("ds_write_b8 %0, %1" ::"v"(lds0 + L::b_scales + (uint32_t)tid), "v"(bsw) : "memory");
+      if (c0 == 0 && tid < BM)
+        asm volatile("ds_write_b32 %0, %1" ::"v"(lds0 + L::dst + 4u * (uint32_t)tid), "v"(dst_row) : "memory");
+    };
     if constexpr (NS == 1) {
-      single_loop<EPI == F8_GLU, BM, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma);
+      single_loop<EPI == F8_GLU, BM, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
     } else if constexpr (PIPE) {
-      piped_loop<EPI == F8_GLU, BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma);
+      piped_loop<EPI == F8_GLU, BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
     } else {
 #pragma unroll
-      for (int i = 0; i < NS - 1; ++i) issue(i, c0 + i, i < nst);
+      for (int i = 1; i < NS - 1; ++i) issue(i, c0 + i, i < nst);
+      fill();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 
       int cur = 0;
@@ -718,10 +821,10 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
       }
     });
   } else if constexpr (EPI == F8_STORE_BF16) {
-    // 32 rows at a time through this wave's own staging area, then whole 128-byte lines
-    char* st = smem + wave * 32 * L::kPitch;
+    // up to 64 rows at a time through this wave's own staging area, then whole 128-byte lines
+    char* st = smem + wave * L::kRows * L::kPitch;
     uint16_t* C = static_cast<uint16_t*>(p.c) + (p.c_rows ? 0 : row0 * p.ldc);
-    constexpr int MS = MF < 2 ? 1 : 2;
+    constexpr int MS = L::kRows / 16;
     const int col0 = nt * BN + gn * 64;
     unrolled<MF / MS>([&](auto s) {
 #pragma unroll
@@ -755,22 +858,34 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
   } else if constexpr (EPI == F8_HALF) {
     // a row's 64 columns of this wave are in four lanes: the power of two that puts the largest into
     // [2^14, 2^15) (f16 ends at 65504; values down to 2^-28 of the largest keep all 11 bits), then as the bf16 store
-    char* st = smem + wave * 32 * L::kPitch;
+    char* st = smem + wave * L::kRows * L::kPitch;
     uint16_t* C = static_cast<uint16_t*>(p.c);
-    constexpr int MS = MF < 2 ? 1 : 2;
+    constexpr int MS = L::kRows / 16;
     const int cb = nt * (BN / kHalfCols) + gn;
-    unrolled<MF / MS>([&](auto s) {
+    uint32_t top[MF], all = 0;
 #pragma unroll
-      for (int h = 0; h < MS; ++h) {
-        constexpr int m0 = s * MS;
+    for (int m = 0; m < MF; ++m) {
+      top[m] = 0;
+#pragma unroll
+      for (int n = 0; n < NF; ++n) top[m] = max_bits(top[m], acc[m][n]);
+      all = top[m] > all ? top[m] : all;
+    }
+    if (__builtin_amdgcn_ballot_w64(all >= kInfBits)) {  // rare: the largest finite values
+#pragma unroll
+      for (int m = 0; m < MF; ++m) {
         float a = 0.f;
 #pragma unroll
         for (int n = 0; n < NF; ++n)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) a = fmaxf(a, finite_abs(acc[m0 + h][n][u]));
-        a = fmaxf(a, __shfl_xor(a, 16, 64));
-        a = fmaxf(a, __shfl_xor(a, 32, 64));
-        const int code = half_code(a);
+          for (int u = 0; u < 4; ++u) a = fmaxf(a, finite_abs(acc[m][n][u]));
+        top[m] = __float_as_uint(a);
+      }
+    }
+    unrolled<MF / MS>([&](auto s) {
+#pragma unroll
+      for (int h = 0; h < MS; ++h) {
+        constexpr int m0 = s * MS;
+        const int code = half_code(__uint_as_float(max_rows4(top[m0 + h])));
         const float inv = scale_inverse(code);
         const int rl = gm * G::WM + 16 * (m0 + h) + r16;
 #pragma unroll
@@ -798,29 +913,43 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
   } else {
     // a = silu(gate) up from the f32 sums; a row's 128 pairs of this tile are one block: its largest
     // magnitude over this wave's 32 pairs (four lanes a row), then over the four waves through LDS
-    float* red = reinterpret_cast<float*>(smem + BM * kBlk);  // [4][BM]
+    uint32_t* red = reinterpret_cast<uint32_t*>(smem + BM * kBlk);  // [BM][4]
+    uint32_t top[MF], all = 0;
     unrolled<MF>([&](auto m) {
-      float a = 0.f;
+      top[m] = 0;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < 2; ++n) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          acc[m][n][u] *= silu_f(acc[m][2 + n][u]);
-          a = fmaxf(a, finite_abs(acc[m][n][u]));
-        }
-      a = fmaxf(a, __shfl_xor(a, 16, 64));
-      a = fmaxf(a, __shfl_xor(a, 32, 64));
-      if (g4 == 0) red[gn * BM + gm * G::WM + 16 * m + r16] = a;
+        for (int u = 0; u < 4; ++u) acc[m][n][u] *= silu_f(acc[m][2 + n][u]);
+        top[m] = max_bits(top[m], acc[m][n]);
+      }
+      all = top[m] > all ? top[m] : all;
+    });
+    const bool odd = __builtin_amdgcn_ballot_w64(all >= kInfBits) != 0;  // this wave holds values that are not finite
+    unrolled<MF>([&](auto m) {
+      if (odd) {
+        float a = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) a = fmaxf(a, finite_abs(acc[m][n][u]));
+        top[m] = __float_as_uint(a);
+      }
+      const uint32_t a = max_rows4(top[m]);
+      if (g4 == 0) red[(gm * G::WM + 16 * m + r16) * 4 + gn] = a;
     });
     __syncthreads();
     unrolled<MF>([&](auto m) {
       const int rl = gm * G::WM + 16 * m + r16;
-      const int code = scale_code(fmaxf(fmaxf(red[rl], red[BM + rl]), fmaxf(red[2 * BM + rl], red[3 * BM + rl])));
+      const uint4 r = *reinterpret_cast<const uint4*>(red + rl * 4);
+      const uint32_t a = max(max(r.x, r.y), max(r.z, r.w));
+      const int code = scale_code(__uint_as_float(a));
       const float inv = scale_inverse(code);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const float v[4] = {acc[m][n][0], acc[m][n][1], acc[m][n][2], acc[m][n][3]};
-        *reinterpret_cast<uint32_t*>(smem + rl * kBlk + gn * 32 + 16 * n + 4 * g4) = quantize4(v, inv);
+        *reinterpret_cast<uint32_t*>(smem + rl * kBlk + gn * 32 + 16 * n + 4 * g4) =
+            odd ? quantize4(v, inv) : pack_e4m3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
       }
       if (gn == 0 && g4 == 0 && rl < rows) p.cs[(row0 + rl) * p.cs_pitch + nt] = (uint8_t)code;
     });
