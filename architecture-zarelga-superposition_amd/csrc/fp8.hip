@@ -535,21 +535,16 @@ __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint3
   __builtin_amdgcn_s_setprio(0);
 }
 
-// The K loop of 128 x 256 tiles on four waves, two workgroups a CU (128 x 64 outputs a wave): one LDS buffer, the
-// stage's fragments in registers.
+// The K loop of 128 x 256 tiles on four waves, two workgroups a CU (128 x 64 outputs a wave). One LDS buffer: a stage's
+// fragments go to registers at once, and the next stage's loads go out, one behind each MFMA, when every wave has
+// its own (spread over the last MFMAs instead, with the A fragments read between the first ones: 1-2% slower).
 template <bool GLU, int BM, int LPS, typename Dma, typename Fill>
 __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
                                             uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma, Fill fill) {
-  static_assert(LPS == 12, "twelve loads a stage");
   Frag8 fa[8], fb[4];
   AScale<8> sa;
   uint32_t sb;
   auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
-  auto read_a = [&](auto m) {
-    fa[m].lo = ds_read128<m * 2048>(lds0 + a_frag);
-    fa[m].hi = ds_read128<m * 2048>((lds0 + a_frag) ^ 64u);
-  };
-  using std::integral_constant;
   fill();
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   for (int st = 0; st < nst; ++st) {
@@ -563,35 +558,26 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
       fb[n].lo = ds_read128<n * 2048>(lds0 + b_frag);
       fb[n].hi = ds_read128<n * 2048>((lds0 + b_frag) ^ 64u);
     });
-    read_a(integral_constant<int, 0>{});
-    read_a(integral_constant<int, 1>{});
     unrolled<8>([&](auto m) {
-      // (reads return in order) allowed: A fragments after m that are out
-      if constexpr (m < 4) asm_wait_lgkm<(m == 0 ? 2 : m == 1 ? 4 : m == 2 ? 6 : 8)>();
-      if constexpr (m == 0) {
-        sa.tie();
-        asm volatile("" : "+v"(sb));
+      fa[m].lo = ds_read128<m * 2048>(lds0 + a_frag);
+      fa[m].hi = ds_read128<m * 2048>((lds0 + a_frag) ^ 64u);
+    });
+    asm_wait_lgkm<0>();
+    sa.tie();
+    asm volatile("" : "+v"(sb));
 #pragma unroll
-        for (int n = 0; n < 4; ++n) fb[n].tie();
-      }
-      if constexpr (m < 4) fa[m].tie();
-      if constexpr (m < 3) {
-        read_a(integral_constant<int, 2 * m + 2>{});
-        read_a(integral_constant<int, 2 * m + 3>{});
-      }
-      fence();
+    for (int n = 0; n < 4; ++n) fb[n].tie();
+#pragma unroll
+    for (int m = 0; m < 8; ++m) fa[m].tie();
+    asm volatile("s_barrier" ::: "memory");
+    fence();
+    unrolled<8>([&](auto m) {
       unrolled<4>([&](auto n) {
         acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[n].value(), fa[m].value(), acc[m][n], 0, 0,
                                                                     GLU ? n / 2 : 0, (int)sb, m & 3, (int)sa.w[m / 4]);
-        if constexpr (m >= 4 && n < 3) dma((m - 4) * 3 + n, 0, c0 + st + 1, st + 1 < nst);
+        if constexpr (m * 4 + n < LPS) dma(m * 4 + n, 0, c0 + st + 1, st + 1 < nst);
         fence();
       });
-      if constexpr (m == 3) {  // everything is in registers: the buffer is the next stage's
-        asm_wait_lgkm<0>();
-#pragma unroll
-        for (int q = 4; q < 8; ++q) fa[q].tie();
-        asm volatile("s_barrier" ::: "memory");
-      }
     });
   }
 }
@@ -963,7 +949,9 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
 
 // ------------------------------------------------------------------ sums over slots
 // out[t] = add[t] + sum_j g[t, j] Y[t k + j] of F8_HALF rows (g null: 1), one rounding. A thread has eight columns;
-// the k rows' loads (compiled for k up to 8) are all issued before the first is used. Bound by HBM.
+// the k rows' loads (compiled for k up to 8) are all issued before the first is used. Bound by HBM: 32768 x 8 rows of
+// 2048 in 230 us (5.2 TB/s). (Rows left in the products' order and read through the inverse permutation: the product
+// 702 -> 670 us, the sum 243, but 60 -> 65 and 277 -> 270 for 16384 x 4: not worth a second form.)
 template <typename T, int KF>
 __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __restrict__ Y, const uint8_t* __restrict__ S,
                                                            int64_t ldy, int64_t pitch, const float* __restrict__ g,
@@ -1128,17 +1116,17 @@ int launch_few(const Fp8Params& p, hipStream_t s) {
 //  - A launch that fits on the CUs at once takes the narrowest tile with which it still does. 4096 -> 4096: 1000 rows
 //    27.6 us (64 x 128), 31.4 (128 x 128), 45 (128 x 256); 2048 rows 47.8, 39.2, 47.6; 128 rows 15.4 (32 x 128), 19.1.
 //    GLU, 4096 -> 2 x 4096: 500 rows 52 (32), 36 (64), 42 (128); 1000 rows 98, 68, 46; 128 x 256 on four waves 51.
-//  - Else 128 x 256 on four waves, two workgroups a CU: one's prologue and epilogue run under the other's loop. Long
-//    loops over long experts want 256 x 256 (outputs/loop step): 8192 x 7168 -> 4096 198 us against 226, 16384 x 2048
-//    -> 2048 64 against 66; but 65536 x 1536 -> 2048 over 64 experts 297 against 293, and, where rows are skewed over
-//    the experts (16384 of them, 2048 -> 7168, 64 experts), 436 against 370. GLU has a longer epilogue: 262144 rows,
-//    2048 -> 2 x 768, 128 experts 924 against 883; 8000 rows 4096 -> 2 x 4096 223 against 229.
+//  - Else 128 x 256 on four waves, two workgroups a CU (one's prologue and epilogue run under the other's loop), or
+//    256 x 256 for experts of six or more such tiles, whose last one, half empty on average, then costs less than a
+//    tenth. 8192 x 7168 -> 4096: 189 and 175 us; 262144 rows over 128 experts, 2048 -> 2 x 768 (GLU): 815 and 797;
+//    65536 rows over 128 experts: 244 and 263, over 64, 1536 -> 2048: 274 and 281; 16384 rows skewed over 64 experts,
+//    7168 -> 2 x 2048 (GLU): 605 and 668, back 356 and 404.
 template <int EPI>
 int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
   const int64_t per = R / p.E;
   const int n = EPI == F8_GLU ? 2 * p.half : p.N;
   const auto fits = [&](int bm, int bn) { return (cdiv(R, bm) + (p.offsets ? p.E : 0)) * cdiv(n, bn) <= kCus; };
-  const bool few = p.offsets && per <= 24, longest = per >= 1024 && p.nk >= (EPI == F8_GLU ? 32 : 16);
+  const bool few = p.offsets && per <= 24;
   if constexpr (EPI == F8_GLU) {
     if (few || fits(32, 256)) return launch8<32, 256, 4, 4, EPI>(p, R, s);
     if (fits(64, 256)) return launch8<64, 256, 4, 3, EPI>(p, R, s);
@@ -1152,7 +1140,7 @@ int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
     if (few || fits(64, 128)) return launch8<64, 128, 4, 3, EPI>(p, R, s);
     if (fits(128, 128)) return launch8<128, 128, 4, 2, EPI>(p, R, s);
   }
-  if (longest) return launch8<256, 256, 8, 2, EPI>(p, R, s);
+  if (per >= 1536) return launch8<256, 256, 8, 2, EPI>(p, R, s);
   return launch8<128, 256, 4, 1, EPI>(p, R, s);
 }
 
