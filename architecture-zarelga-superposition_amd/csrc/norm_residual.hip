@@ -11,7 +11,7 @@
 // r' is formed again in the backward from r and y, which it has to read anyway, so nothing but the two
 // rstds is kept and no rounding of a stored r' gets into the grads.
 // Both passes are bound by HBM. A row belongs to the fewest waves that hold it at eight elements a
-// thread (one wave up to d = 512, four at 2048, sixteen at 8192; above, more elements a thread): few
+// thread (one wave up to d = 512, four at 2048, sixteen at 8192 in the forward; above, more elements a thread): few
 // registers, so several workgroups share a CU and one's loads fill the other's row sums and barriers.
 // The backward walks rows with a fixed grid; the sums over rows go through per-block partials added in
 // a fixed order (the same result on every run).
@@ -25,7 +25,6 @@ namespace {
 constexpr int kVN = 8;        // elements of a thread's chunk
 constexpr int kMaxWaves = 16; // waves of one row
 constexpr int kMaxNQ = 4;
-constexpr int kMaxPartials = 512;
 
 enum Gate { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_FULL = 3 };
 
@@ -276,22 +275,27 @@ struct GateChunk {
   }
 };
 
-// One row's operands in the backward: this thread's chunk of each.
-template <typename R, typename Y, bool VEC>
+// One row's operands in the backward: this thread's chunks of each.
+template <typename R, typename Y, int NQ, bool VEC>
 struct Row {
-  Chunk<R, VEC> r, gr;
-  Chunk<Y, VEC> y, gx;
+  Chunk<R, VEC> r[NQ], gr[NQ];
+  Chunk<Y, VEC> y[NQ], gx[NQ];
   float rho1, rho2, g_row;
-  __device__ __forceinline__ void load(const NormArgs& a, int64_t i, int64_t c) {
+  template <typename Col>
+  __device__ __forceinline__ void load(const NormArgs& a, int64_t i, Col col) {
     const bool live = i < a.n;
     const int64_t row = live ? i : 0, dd = live ? a.d : 0;
     rho1 = live && a.w1.p ? a.rho1[row] : 1.f;  // (no norm of y: u = y)
     rho2 = live && a.w2.p ? a.rho2[row] : 0.f;  // (no next norm: nothing through x)
     g_row = live && a.gate_kind == GATE_ROW ? load_one(a.gate, row) : 1.f;
-    y.load(static_cast<const Y*>(a.y) + row * a.ldy, c, dd);
-    r.load(static_cast<const R*>(a.r) + row * a.ldr, c, dd);
-    gr.load(static_cast<const R*>(a.gr) + row * a.d, c, a.gr ? dd : 0);
-    gx.load(static_cast<const Y*>(a.gx) + row * a.d, c, a.gx ? dd : 0);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int64_t c = col(q);
+      y[q].load(static_cast<const Y*>(a.y) + row * a.ldy, c, dd);
+      r[q].load(static_cast<const R*>(a.r) + row * a.ldr, c, dd);
+      gr[q].load(static_cast<const R*>(a.gr) + row * a.d, c, a.gr ? dd : 0);
+      gx[q].load(static_cast<const Y*>(a.gx) + row * a.d, c, a.gx ? dd : 0);
+    }
   }
 };
 
@@ -309,138 +313,141 @@ __device__ __forceinline__ void store_gate(const Out& o, int64_t at, int64_t c, 
   else store_chunk<VEC>(static_cast<float*>(o.p) + at, c, d, v);
 }
 
-// One chunk a thread (d <= 8192). Up to eight waves a row the three sums over rows live in registers; sixteen waves
-// have 128 registers a thread and one workgroup a CU, so there the sums are in LDS (each thread its own
-// columns: 24 bytes an element of the row against 18 to 12 from HBM at a tenth of LDS's rate) and the
-// next row's operands are loaded before this one is worked on.
-template <typename R, typename Y, int W, bool VEC, bool FULL>
-__global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_backward_kernel(NormArgs a) {
+// Up to eight waves a row with one chunk a thread (d <= 4096): a row's operands, the parameters and the sums over rows
+// stay in registers, some 160 a thread. Wider rows (to 8192) have two chunks a thread and the sums in LDS, each thread its
+// own columns (24 bytes an element of the row, 12 to 18 from HBM at a tenth of LDS's rate). 4096 rows, f32 stream,
+// bf16 y: 34 us at d = 2048 (4.4 TB/s), 66 at 4096, 126 at 7168 (4.2; sixteen waves of one chunk, with a quarter of the
+// registers a thread and the parameters read again for every row, took 166).
+template <typename R, typename Y, int W, int NQ, bool VEC, bool FULL>
+__global__ __launch_bounds__(Map<W>::THREADS, 2) void norm_residual_backward_kernel(NormArgs a) {
   using M = Map<W>;
-  constexpr bool LDS_SUMS = W == kMaxWaves, PREFETCH = false;
   __shared__ float red[2][M::WPB][2];
-  extern __shared__ __align__(16) float fold[];  // [RPB][d] (several rows a block), or the sums [3][8 TPR]
+  constexpr bool LDS_SUMS = NQ > 1;
+  extern __shared__ __align__(16) float fold[];  // [RPB][d] (several rows a block), or the sums [3][NQ][2][TPR]
   const int lt = threadIdx.x % M::TPR, sub = threadIdx.x / M::TPR;
-  const int64_t c = (int64_t)lt * kVN;
+  auto col = [&](int q) { return (int64_t)(lt + q * M::TPR) * kVN; };
   const float alpha = a.alpha_ptr ? *a.alpha_ptr : a.alpha;
   const float inv_d = 1.0f / (float)a.d;
-  float w1[kVN], w2[kVN], gc[kVN], acc1[kVN], acc2[kVN], accg[kVN];
+  float w1[NQ][kVN], w2[NQ][kVN], gc[NQ][kVN], acc1[NQ][kVN], acc2[NQ][kVN], accg[NQ][kVN];
   float acc_alpha = 0.f;
-#pragma unroll
-  for (int u = 0; u < kVN; ++u) {
-    acc1[u] = acc2[u] = accg[u] = 0.f;
-    gc[u] = 1.f;
-  }
-  auto params = [&] {
-    load_gain<VEC>(a.w1, c, a.d, w1);
-    load_gain<VEC>(a.w2, c, a.d, w2);
-    if (a.gate_kind == GATE_CHANNEL) load_vec<VEC>(a.gate, 0, c, a.d, gc);
-  };
-  float4* sums = reinterpret_cast<float4*>(fold) + lt;  // this thread's: vector k, half h at (2 k + h) TPR
-  if constexpr (LDS_SUMS) {
-#pragma unroll
-    for (int k = 0; k < 6; ++k) sums[k * M::TPR] = make_float4(0.f, 0.f, 0.f, 0.f);
-  } else {
-    params();
-  }
-  // v added to this thread's part of sum k in LDS
-  auto add = [&](int k, float (&v)[kVN]) {
+  float4* sums = reinterpret_cast<float4*>(fold) + lt;
+  // v added to this thread's part of sum k in LDS, and cleared
+  auto add = [&](int k, int q, float (&v)[kVN]) {
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
-      float4 o = sums[(2 * k + hh) * M::TPR];
-      o.x += v[4 * hh];
-      o.y += v[4 * hh + 1];
-      o.z += v[4 * hh + 2];
-      o.w += v[4 * hh + 3];
-      sums[(2 * k + hh) * M::TPR] = o;
+      float4& at = sums[((k * NQ + q) * 2 + hh) * M::TPR];
+      const float4 o = at;
+      at = make_float4(o.x + v[4 * hh], o.y + v[4 * hh + 1], o.z + v[4 * hh + 2], o.w + v[4 * hh + 3]);
     }
 #pragma unroll
     for (int u = 0; u < kVN; ++u) v[u] = 0.f;
   };
+  if constexpr (LDS_SUMS) {
+#pragma unroll
+    for (int k = 0; k < 6 * NQ; ++k) sums[k * M::TPR] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+    for (int u = 0; u < kVN; ++u) {
+      acc1[q][u] = acc2[q][u] = accg[q][u] = 0.f;
+      gc[q][u] = 1.f;
+    }
+    load_gain<VEC>(a.w1, col(q), a.d, w1[q]);
+    load_gain<VEC>(a.w2, col(q), a.d, w2[q]);
+    if (a.gate_kind == GATE_CHANNEL) load_vec<VEC>(a.gate, 0, col(q), a.d, gc[q]);
+  }
   const int64_t first = (int64_t)blockIdx.x * M::RPB, step = (int64_t)gridDim.x * M::RPB;
-  Row<R, Y, VEC> cur, nxt;
-  GateChunk<VEC> gate;  // FULL: this row's gate
-  if constexpr (PREFETCH) cur.load(a, first + sub, c);
+  Row<R, Y, NQ, VEC> cur;
+  GateChunk<VEC> gate[NQ];  // FULL: this row's gate
   for (int64_t base = first; base < a.n; base += step) {  // uniform in the block
     const int64_t i = base + sub;
     const bool live = i < a.n;
-    if constexpr (PREFETCH) nxt.load(a, i + step, c);
-    else cur.load(a, i, c);
-    if constexpr (LDS_SUMS) params();
-    if constexpr (FULL) gate.load(a.gate, (live ? i : 0) * a.ldg, c, live ? a.d : 0);
+    cur.load(a, i, col);
+    if constexpr (FULL) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) gate[q].load(a.gate, (live ? i : 0) * a.ldg, col(q), live ? a.d : 0);
+    }
     const float rho1 = cur.rho1, rho2 = cur.rho2, g_row = FULL ? 1.f : cur.g_row;
-    // y rho1, u and r' of this chunk
-    auto values = [&](float (&yh)[kVN], float (&uu)[kVN], float (&r)[kVN], float (&h)[kVN]) {
-      cur.y.get(yh);
-      cur.r.get(r);
-      if constexpr (FULL) gate.get(gc);
+    // y rho1, u and r' of a chunk
+    auto values = [&](int q, float (&yh)[kVN], float (&uu)[kVN], float (&r)[kVN], float (&h)[kVN]) {
+      cur.y[q].get(yh);
+      cur.r[q].get(r);
+      if constexpr (FULL) gate[q].get(gc[q]);
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
         yh[u] *= rho1;
-        uu[u] = yh[u] * w1[u];
-        h[u] = fmaf(gc[u] * g_row, uu[u], alpha * r[u]);
+        uu[u] = yh[u] * w1[q][u];
+        h[u] = fmaf(gc[q][u] * g_row, uu[u], alpha * r[u]);
       }
     };
     float s[1] = {0.f};
-    {
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
       float yh[kVN], uu[kVN], r[kVN], h[kVN], gx[kVN];
-      values(yh, uu, r, h);
-      cur.gx.get(gx);
+      values(q, yh, uu, r, h);
+      cur.gx[q].get(gx);
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
-        acc2[u] = fmaf(gx[u], rho2 * h[u], acc2[u]);
-        s[0] = fmaf(gx[u] * w2[u], h[u], s[0]);
+        acc2[q][u] = fmaf(gx[u], rho2 * h[u], acc2[q][u]);
+        s[0] = fmaf(gx[u] * w2[q][u], h[u], s[0]);
       }
-      if (LDS_SUMS && a.w2.p) add(1, acc2);
+      if (LDS_SUMS && a.w2.p) add(1, q, acc2[q]);
+      if constexpr (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // (one chunk's values at a time)
     }
     float coef2 = 0.f;
     if (a.gx) {
       row_sums<W, 1, M::WPB>(s, red, 0);
       coef2 = rho2 * rho2 * rho2 * s[0] * inv_d;
     }
-    cur.y.forget();
-    cur.r.forget();
-    cur.gx.forget();
-    if constexpr (FULL) gate.forget();
-    if constexpr (LDS_SUMS) params();
     float s2[2] = {0.f, 0.f};  // du (1 + w1) y rho1, t u
-    float h[kVN];              // du (1 + w1) after this
-    {
+    float h[NQ][kVN];          // du (1 + w1) after this
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      cur.y[q].forget();
+      cur.r[q].forget();
+      cur.gx[q].forget();
+      if constexpr (FULL) gate[q].forget();
       float yh[kVN], uu[kVN], r[kVN], gx[kVN], t[kVN];
-      values(yh, uu, r, h);
-      cur.gx.get(gx);
-      cur.gr.get(t);
+      values(q, yh, uu, r, h[q]);
+      cur.gx[q].get(gx);
+      cur.gr[q].get(t);
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
-        t[u] = fmaf(-coef2, h[u], fmaf(rho2, gx[u] * w2[u], t[u]));
+        t[u] = fmaf(-coef2, h[q][u], fmaf(rho2, gx[u] * w2[q][u], t[u]));
         acc_alpha = fmaf(t[u], r[u], acc_alpha);
         uu[u] *= t[u];
         s2[1] += uu[u];
-        accg[u] += uu[u];
-        h[u] = gc[u] * g_row * t[u];
-        acc1[u] = fmaf(h[u], yh[u], acc1[u]);
-        h[u] *= w1[u];
-        s2[0] = fmaf(h[u], yh[u], s2[0]);
+        accg[q][u] += uu[u];
+        h[q][u] = gc[q][u] * g_row * t[u];
+        acc1[q][u] = fmaf(h[q][u], yh[u], acc1[q][u]);
+        h[q][u] *= w1[q][u];
+        s2[0] = fmaf(h[q][u], yh[u], s2[0]);
         t[u] *= alpha;
       }
       if (live) {
-        store_chunk<VEC>(static_cast<R*>(a.dr) + i * a.d, c, a.d, t);
-        if (FULL && a.dgate.p) store_gate<VEC>(a.dgate, i * a.d, c, a.d, uu);
+        store_chunk<VEC>(static_cast<R*>(a.dr) + i * a.d, col(q), a.d, t);
+        if (FULL && a.dgate.p) store_gate<VEC>(a.dgate, i * a.d, col(q), a.d, uu);
       }
-      if (LDS_SUMS && a.w1.p) add(0, acc1);
-      if (LDS_SUMS && a.gate_kind == GATE_CHANNEL) add(2, accg);
+      if (LDS_SUMS && a.w1.p) add(0, q, acc1[q]);
+      if (LDS_SUMS && a.gate_kind == GATE_CHANNEL) add(2, q, accg[q]);
+      if constexpr (NQ > 1) __builtin_amdgcn_sched_barrier(0);
     }
     if (a.w1.p || a.gate_kind == GATE_ROW) row_sums<W, 2, M::WPB>(s2, red, 1);
-    cur.y.forget();
     if (live && a.gate_kind == GATE_ROW && a.dgate.p && lt == 0) store_one(a.dgate, i, s2[1]);
     const float coef1 = a.w1.p ? rho1 * s2[0] * inv_d : 0.f;  // (rho1^3 y s = rho1 (y rho1) (s rho1))
-    if (live) {
-      float yh[kVN];
-      cur.y.get(yh);
 #pragma unroll
-      for (int u = 0; u < kVN; ++u) h[u] = fmaf(-coef1, yh[u] * rho1, rho1 * h[u]);
-      store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, c, a.d, h);
+    for (int q = 0; q < NQ; ++q) {
+      cur.y[q].forget();
+      if (live) {
+        float yh[kVN];
+        cur.y[q].get(yh);
+#pragma unroll
+        for (int u = 0; u < kVN; ++u) h[q][u] = fmaf(-coef1, yh[u] * rho1, rho1 * h[q][u]);
+        store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, col(q), a.d, h[q]);
+      }
+      if constexpr (NQ > 1) __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (PREFETCH) cur = nxt;
     if constexpr (W > 1) {
       // a row with only one of the two sums reuses its slot in the next one
       if (!(a.gx && (a.w1.p || a.gate_kind == GATE_ROW))) __syncthreads();
@@ -448,27 +455,29 @@ __global__ __launch_bounds__(Map<W>::THREADS) void norm_residual_backward_kernel
   }
   // this block's partials; several rows a block: their sums added in order through LDS
   const int64_t P = gridDim.x;
-  auto write = [&](float (&acc)[kVN], int which) {
+  auto write = [&](float (&acc)[NQ][kVN], int which) {
     float* dst = a.partial + ((int64_t)which * P + blockIdx.x) * a.d;
     if constexpr (LDS_SUMS) {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const float4 o = sums[(2 * which + hh) * M::TPR];
-        acc[4 * hh] = o.x;
-        acc[4 * hh + 1] = o.y;
-        acc[4 * hh + 2] = o.z;
-        acc[4 * hh + 3] = o.w;
-      }
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const float4 o = sums[((which * NQ + q) * 2 + hh) * M::TPR];
+          acc[q][4 * hh] = o.x;
+          acc[q][4 * hh + 1] = o.y;
+          acc[q][4 * hh + 2] = o.z;
+          acc[q][4 * hh + 3] = o.w;
+        }
     }
     if constexpr (M::RPB == 1) {
 #pragma unroll
-      for (int u = 0; u < kVN; ++u)
-        if (c + u < a.d) dst[c + u] = acc[u];
+      for (int q = 0; q < NQ; ++q) store_chunk<VEC>(dst, col(q), a.d, acc[q]);
     } else {
+      static_assert(NQ == 1 || M::RPB == 1, "rows that share a block have one chunk a thread");
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < kVN; ++u)
-        if (c + u < a.d) fold[(int64_t)sub * a.d + c + u] = acc[u];
+        if (col(0) + u < a.d) fold[(int64_t)sub * a.d + col(0) + u] = acc[0][u];
       __syncthreads();
       for (int64_t k = threadIdx.x; k < a.d; k += M::THREADS) {
         float tt = 0.f;
@@ -509,15 +518,15 @@ __global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide
     float rho1 = 1.f, rho2 = 0.f;
     // y rho1, u, r' and r of a chunk, and its gains
     float y[kVN], uu[kVN], h[kVN], r[kVN], gx[kVN], w1[kVN], w2[kVN], g[kVN], t[kVN];
-    Row<R, Y, VEC> row;
+    Row<R, Y, 1, VEC> row;
     auto chunk = [&](int64_t c) {
-      row.load(a, i, c);
+      row.load(a, i, [&](int) { return c; });
       rho1 = row.rho1;
       rho2 = row.rho2;
-      row.y.get(y);
-      row.r.get(r);
-      row.gx.get(gx);
-      row.gr.get(t);
+      row.y[0].get(y);
+      row.r[0].get(r);
+      row.gx[0].get(gx);
+      row.gr[0].get(t);
       load_gain<VEC>(a.w1, c, a.d, w1);
       load_gain<VEC>(a.w2, c, a.d, w2);
       if (a.gate_kind == GATE_CHANNEL) load_vec<VEC>(a.gate, 0, c, a.d, g);
@@ -638,10 +647,17 @@ int row_chunks(int64_t d) {
   return nq;
 }
 constexpr int64_t kMaxD = (int64_t)kMaxWaves * 64 * kVN * kMaxNQ;
-// Blocks of the backward: two of eight waves a CU, or one of sixteen.
-int partials(int64_t n, int64_t d) {
+// Waves of a row in the backward, and its blocks. More of them hide more of each row's waits (up to three of four
+// waves fit on a CU, one of eight), fewer leave less to the sum of their partials: 16384 rows of 2048 (f32 stream) 126 us
+// with 768, 134 with 512, 220 with 256; 4096 rows 42, 40, 48; 1024 rows 28, 24, 22; 4096 rows of 4096 87 with 512, 76
+// with 256.
+int back_waves(int64_t d) {
   const int w = row_waves(d);
-  const int64_t want = cdiv(n > 0 ? n : 1, w < 8 ? 8 / w : 1), most = w == kMaxWaves ? kMaxPartials / 2 : kMaxPartials;
+  return w == kMaxWaves && d <= (int64_t)kMaxWaves * 64 * kVN ? kMaxWaves / 2 : w;
+}
+int partials(int64_t n, int64_t d) {
+  const int w = back_waves(d);
+  const int64_t want = cdiv(n > 0 ? n : 1, w < 4 ? 4 / w : 1), most = w >= 8 || want <= 1024 ? 256 : want <= 4096 ? 512 : 768;
   return (int)(want < most ? want : most);
 }
 
@@ -797,18 +813,19 @@ extern "C" int zmoe_norm_residual_backward(const void* dR_out, const void* dX, c
       return;
     }
     with_map(d, [&](auto w, auto nq) {
-      constexpr int W = decltype(w)::value;
       if constexpr (decltype(nq)::value == 1) {
+        // sixteen waves of one chunk become eight of two
+        constexpr int NQ = decltype(w)::value == kMaxWaves ? 2 : 1, W = decltype(w)::value / NQ;
         using M = Map<W>;
         using RT = decltype(rt);
         using YT = decltype(yt);
-        auto kern = gate_kind == GATE_FULL ? (vec ? norm_residual_backward_kernel<RT, YT, W, true, true>
-                                                  : norm_residual_backward_kernel<RT, YT, W, false, true>)
-                                           : (vec ? norm_residual_backward_kernel<RT, YT, W, true, false>
-                                                  : norm_residual_backward_kernel<RT, YT, W, false, false>);
-        const size_t lds = W == kMaxWaves ? (size_t)M::TPR * 6 * sizeof(float4)  // 96 KB
-                                          : (M::RPB > 1 ? (size_t)M::RPB * (size_t)d * sizeof(float) : 0);  // <= 16 KB
-        if (W == kMaxWaves && prepare(kern, (int)lds) != ZMOE_OK) {
+        auto kern = gate_kind == GATE_FULL ? (vec ? norm_residual_backward_kernel<RT, YT, W, NQ, true, true>
+                                                  : norm_residual_backward_kernel<RT, YT, W, NQ, false, true>)
+                                           : (vec ? norm_residual_backward_kernel<RT, YT, W, NQ, true, false>
+                                                  : norm_residual_backward_kernel<RT, YT, W, NQ, false, false>);
+        const size_t lds = NQ > 1 ? (size_t)M::TPR * 6 * NQ * sizeof(float4)  // 96 KB
+                                  : (M::RPB > 1 ? (size_t)M::RPB * (size_t)d * sizeof(float) : 0);  // <= 8 KB
+        if (NQ > 1 && prepare(kern, (int)lds) != ZMOE_OK) {
           prepared = false;
           return;
         }

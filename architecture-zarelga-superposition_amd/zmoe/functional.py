@@ -258,6 +258,8 @@ def norm_residual(residual: torch.Tensor, y: torch.Tensor, weight: Optional[torc
         scale = residual_scale.float()
     elif residual_scale is not None:
         value = float(residual_scale)
+    if y.dim() == 2:
+        return _NormResidual.apply(residual, y, weight, next_weight, gate, kind, scale, value, float(eps))
     r, x = _NormResidual.apply(residual.reshape(-1, d), y.reshape(-1, d), weight, next_weight, gate, kind, scale, value,
                                float(eps))
     return r.view(residual.shape), None if x is None else x.view(y.shape)
