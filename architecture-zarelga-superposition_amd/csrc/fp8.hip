@@ -43,6 +43,7 @@ __device__ __forceinline__ int half_code(float a) {
 // 2^-c of that byte (code <= 247: the exponent field stays normal).
 __device__ __forceinline__ float scale_inverse(int code) { return __int_as_float((254 - code) << 23); }
 
+constexpr uint32_t kInfBits = 0x7f800000u;  // magnitudes from here on: inf, NaN
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 __device__ __forceinline__ float finite_abs(float v) { return finite(v) ? fabsf(v) : 0.f; }
 
@@ -72,13 +73,33 @@ __device__ __forceinline__ float max16(float v) {
   return fmaxf(v, dpp(v, std::integral_constant<int, 0x140>{}));  // 15 - lane within 16
 }
 
-// Eight elements from column c of a row (zeros past K): 16-byte loads where the row allows them.
+// How rows can be loaded: in 16-byte chunks, in 4-byte pairs (16-bit elements), one by one.
+enum Width { W_ONE = 0, W_PAIR = 1, W_CHUNK = 2 };
+int row_width(const void* p, int64_t stride, int size) {
+  if (aligned16(p) && stride % (16 / size) == 0) return W_CHUNK;
+  return size == 2 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0 && stride % 2 == 0 ? W_PAIR : W_ONE;
+}
+
+// Eight elements from column c of a row, zeros past K.
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int64_t K, bool vec, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int64_t K, int width, float (&v)[8]) {
   constexpr int VN = 16 / sizeof(T);
-  if (vec && c + 8 <= K) {
+  if (width == W_CHUNK && c + 8 <= K) {
 #pragma unroll
     for (int q = 0; q < 8 / VN; ++q) unpack_chunk(*reinterpret_cast<const uint4*>(row + c + q * VN), &v[q * VN], T{});
+  } else if (sizeof(T) == 2 && width != W_ONE) {
+    uint32_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t at = c + 2 * q;
+      w[q] = at + 1 < K ? *reinterpret_cast<const uint32_t*>(row + at)
+                        : (at < K ? (uint32_t)row[at] : 0u);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      v[2 * q] = __uint_as_float(w[q] << 16);
+      v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+    }
   } else {
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = c + u < K ? to_f32(row[c + u]) : 0.f;
@@ -94,7 +115,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ X, int64_t ldx, int64_t x_rows,
                                                             const int64_t* __restrict__ rows, int row_div,
                                                             const float* __restrict__ row_scale, uint32_t total,
-                                                            int64_t K, int nb, int vec, uint8_t* __restrict__ Q,
+                                                            int64_t K, int nb, int width, uint8_t* __restrict__ Q,
                                                             uint8_t* __restrict__ S, int64_t pitch) {
   const uint32_t g = blockIdx.x * 16 + threadIdx.x / 16;  // (row, block)
   if (g >= total) return;  // whole groups of 16 lanes
@@ -113,7 +134,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   }
   const int64_t c = (int64_t)b * kBlk + lane * 8;
   float v[8];
-  load8(X + (src < 0 ? 0 : src) * ldx, c, src < 0 ? 0 : K, vec != 0, v);
+  load8(X + (src < 0 ? 0 : src) * ldx, c, src < 0 ? 0 : K, width, v);
   float a = 0.f;
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
@@ -128,51 +149,82 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 }
 
 // ------------------------------------------------------------------ weights
-// One workgroup per 128 x 128 block: eight rows a thread, the block's largest magnitude through LDS.
-// With Qt the block is also written transposed (through LDS): W^T's blocks are W's, so one scale
-// serves both, and the input gradient's product reads rows of W^T with the depth contiguous.
+// One workgroup per 128 x 128 block: eight rows of eight columns a thread, the block's largest magnitude through LDS.
+// With Qt the block is also written transposed (8 x 8 bytes in registers, the rest through LDS): W^T's blocks are W's,
+// so one scale serves both, and the input gradient's product reads rows of W^T with the depth contiguous. Bound by HBM:
+// 64 x 1536 x 2048 bf16 with both forms in 160 us (5.0 TB/s), f32 in 229 (5.3), 16 x 1030 x 510 in 16.
 template <typename T, bool TRANS>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restrict__ W, int64_t se, int64_t sn,
-                                                              int64_t N, int64_t K, int vec, uint8_t* __restrict__ Q,
+                                                              int64_t N, int64_t K, int width, uint8_t* __restrict__ Q,
                                                               uint8_t* __restrict__ S, uint8_t* __restrict__ Qt,
                                                               uint8_t* __restrict__ St) {
-  __shared__ float red[4];
+  __shared__ uint32_t red[4];
   constexpr int TP = kBlk + 16;  // pitch of the transposed block, rows still 16-byte aligned
   __shared__ __align__(16) uint8_t tile[TRANS ? kBlk * TP : 16];
   const int64_t kb = blockIdx.x, nb = blockIdx.y, e = blockIdx.z;
-  const int t = threadIdx.x, row0 = t >> 4, col = (t & 15) * 8;
+  const int t = threadIdx.x, row0 = (t >> 4) * 8, col = (t & 15) * 8;
   float v[8][8];
-  float a = 0.f;
+  uint32_t a = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int64_t n = nb * kBlk + row0 + 16 * j;
-    load8(W + e * se + (n < N ? n : 0) * sn, kb * kBlk + col, n < N ? K : 0, vec != 0, v[j]);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) a = fmaxf(a, finite_abs(v[j][u]));
+    const int64_t n = nb * kBlk + row0 + j;
+    load8(W + e * se + (n < N ? n : 0) * sn, kb * kBlk + col, n < N ? K : 0, width, v[j]);
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) a = max(a, __float_as_uint(v[j][u]) & 0x7fffffffu);
+  const bool odd = __builtin_amdgcn_ballot_w64(a >= kInfBits) != 0;  // this wave holds values that are not finite
+  if (odd) {
+    float f = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) f = fmaxf(f, finite_abs(v[j][u]));
+    a = __float_as_uint(f);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
   if ((t & 63) == 0) red[t >> 6] = a;
   __syncthreads();
-  const int code = scale_code(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  const int code = scale_code(__uint_as_float(max(max(red[0], red[1]), max(red[2], red[3]))));
   const float inv = scale_inverse(code);
   const int64_t nbs = blocks_of(N), kbs = blocks_of(K);
   if (t == 0) {
     S[(e * nbs + nb) * scale_pitch(K) + kb] = (uint8_t)code;
     if (TRANS) St[(e * kbs + kb) * scale_pitch(N) + nb] = (uint8_t)code;
   }
+  uint2 w[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int64_t n = nb * kBlk + row0 + 16 * j;
+    const int64_t n = nb * kBlk + row0 + j;
     const float lo[4] = {v[j][0], v[j][1], v[j][2], v[j][3]}, hi[4] = {v[j][4], v[j][5], v[j][6], v[j][7]};
-    const uint2 w = make_uint2(quantize4(lo, inv), quantize4(hi, inv));
-    if (n < N) *reinterpret_cast<uint2*>(Q + ((e * N + n) * kbs + kb) * kBlk + col) = w;
-    if constexpr (TRANS) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) tile[(col + u) * TP + row0 + 16 * j] = (uint8_t)((u < 4 ? w.x : w.y) >> (8 * (u & 3)));
-    }
+    if (odd) w[j] = make_uint2(quantize4(lo, inv), quantize4(hi, inv));
+    else w[j] = make_uint2(pack_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv),
+                           pack_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv));
+    if (n < N) *reinterpret_cast<uint2*>(Q + ((e * N + n) * kbs + kb) * kBlk + col) = w[j];
   }
   if constexpr (TRANS) {
+    // columns 4 c .. 4 c + 3 of rows 4 r .. 4 r + 3: byte pairs of two rows, then of two pairs
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint32_t out[4][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        uint32_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = c ? w[4 * r + j].y : w[4 * r + j].x;
+        const uint32_t p01 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), q01 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+        const uint32_t p23 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), q23 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+        out[0][r] = __builtin_amdgcn_perm(p23, p01, 0x05040100u);
+        out[1][r] = __builtin_amdgcn_perm(p23, p01, 0x07060302u);
+        out[2][r] = __builtin_amdgcn_perm(q23, q01, 0x05040100u);
+        out[3][r] = __builtin_amdgcn_perm(q23, q01, 0x07060302u);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<uint2*>(tile + (col + 4 * c + u) * TP + row0) = make_uint2(out[u][0], out[u][1]);
+    }
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -297,7 +349,6 @@ __device__ __forceinline__ void unrolled(F f) {
 
 __device__ __forceinline__ int swizzle8(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
-constexpr uint32_t kInfBits = 0x7f800000u;  // magnitudes from here on: inf, NaN
 // Largest magnitude of v and m, as bits (two instructions for two values, and inf and NaN show).
 __device__ __forceinline__ uint32_t max_bits(uint32_t m, const f32x4_t& v) {
 #pragma unroll
@@ -991,7 +1042,7 @@ __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __res
   }
   if (add) {
     float v[8];
-    load8(add + t * N, c, N, vec != 0, v);
+    load8(add + t * N, c, N, vec ? W_CHUNK : W_ONE, v);
 #pragma unroll
     for (int u = 0; u < 8; ++u) acc[u] += v[u];
   }
@@ -1181,16 +1232,16 @@ extern "C" int zmoe_fp8_quantize_rows(const void* X, int64_t x_stride, int64_t x
   ZMOE_REQUIRE(aligned16(Q) && aligned4(S), ZMOE_ERR_ALIGN, "fp8_quantize_rows: Q on 16, S on 4 bytes");
   const int64_t nb = blocks_of(K);
   ZMOE_REQUIRE(n * nb < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "fp8_quantize_rows: too many blocks");
-  const int vec = aligned16(X) && x_stride % (16 / dtype_size(dtype)) == 0;
+  const int width = row_width(X, x_stride, dtype_size(dtype));
   const dim3 grid((unsigned)cdiv(n * nb, 16));
   hipStream_t s = as_stream(stream);
   uint8_t *q = static_cast<uint8_t*>(Q), *sc = static_cast<uint8_t*>(S);
   if (dtype == ZMOE_DTYPE_BF16)
     hipLaunchKernelGGL(quantize_rows_kernel<uint16_t>, grid, dim3(256), 0, s, static_cast<const uint16_t*>(X), x_stride,
-                       x_rows, rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, vec, q, sc, scale_pitch(K));
+                       x_rows, rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, width, q, sc, scale_pitch(K));
   else
     hipLaunchKernelGGL(quantize_rows_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(X), x_stride, x_rows,
-                       rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, vec, q, sc, scale_pitch(K));
+                       rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, width, q, sc, scale_pitch(K));
   return check_launch("fp8_quantize_rows");
 }
 
@@ -1204,8 +1255,8 @@ extern "C" int zmoe_fp8_quantize_weight(const void* W, int64_t w_stride_e, int64
   ZMOE_REQUIRE(aligned16(Q) && aligned4(S) && aligned16(Qt) && aligned4(St), ZMOE_ERR_ALIGN,
                "fp8_quantize_weight: values on 16, scales on 4 bytes");
   ZMOE_REQUIRE(blocks_of(N) <= 65535, ZMOE_ERR_SHAPE, "fp8_quantize_weight: too many rows");
-  const int v = 16 / dtype_size(dtype);
-  const int vec = aligned16(W) && w_stride_n % v == 0 && w_stride_e % v == 0;
+  const int size = dtype_size(dtype), wn = row_width(W, w_stride_n, size), we = row_width(W, w_stride_e, size);
+  const int width = wn < we ? wn : we;
   const dim3 grid((unsigned)blocks_of(K), (unsigned)blocks_of(N), (unsigned)E);
   hipStream_t s = as_stream(stream);
   uint8_t *q = static_cast<uint8_t*>(Q), *sc = static_cast<uint8_t*>(S), *qt = static_cast<uint8_t*>(Qt),
@@ -1213,7 +1264,7 @@ extern "C" int zmoe_fp8_quantize_weight(const void* W, int64_t w_stride_e, int64
   auto go = [&](auto t, auto trans) {
     using T = decltype(t);
     hipLaunchKernelGGL((quantize_weight_kernel<T, decltype(trans)::value>), grid, dim3(256), 0, s,
-                       static_cast<const T*>(W), w_stride_e, w_stride_n, N, K, vec, q, sc, qt, st);
+                       static_cast<const T*>(W), w_stride_e, w_stride_n, N, K, width, q, sc, qt, st);
   };
   if (dtype == ZMOE_DTYPE_BF16) {
     if (Qt) go(uint16_t{}, std::true_type{});
