@@ -245,6 +245,13 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
 // F8_HALF: rows that a sum over a token's k slots reads next, as f16 with a power-of-two scale for each 64 columns:
 // 16 bits like bf16, but within 2^-11 of each value (bf16: 2^-8), so that the sum has its own rounding only.
 enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2, F8_HALF = 3 };
+// The SwiGLU's sums are rounded to e4m3 next, where an error of a few 2^-13 (a scaled MFMA's, of its largest terms) turns
+// one value in some thousand to its neighbour, 2^-3 away: little in the mean over many rows (0.0023 from the exact
+// result where bf16's own rounding is 0.0017), but up to 0.018 for a single row of a narrow expert. Tiles of 32 rows,
+// whose launches are bound by the weights' stream, therefore take their terms to bf16 (exact) and add in f32: 0.0017,
+// and 18.4 -> 19.7 us for one row in each of 32 experts of 2048 -> 2 x 768.
+constexpr int kExactRows = 32;
+constexpr int64_t kExactValues = 1 << 19;  // activations of a launch up to which the mean does not cover it
 constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 
 struct Fp8Params {
@@ -338,6 +345,18 @@ struct Frag8 {
   }
 };
 
+// Eight e4m3 values times the power of two of E8M0 byte `code`, in bf16: exact (but for values below 2^-126).
+typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8v_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ bf16x8v_t to_bf16x8(int lo, int hi, uint32_t code) {
+  const float s = __uint_as_float(code << 23);
+  const bf16x2v_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, s, false),
+                  b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, s, true),
+                  c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, s, false),
+                  d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, s, true);
+  return bf16x8v_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 template <int... I, typename F>
 __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) {
   (f(std::integral_constant<int, I>{}), ...);
@@ -345,6 +364,24 @@ __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F f) 
 template <int N, typename F>
 __device__ __forceinline__ void unrolled(F f) {
   unrolled(std::make_integer_sequence<int, N>{}, f);
+}
+
+// One stage of the wave's MF x 4 fragments with their sums at f32's precision: bf16 MFMAs of 32 depths.
+template <int MF>
+__device__ __forceinline__ void mma_exact(f32x4_t (&acc)[MF][4], const Frag8 (&fa)[MF], const Frag8 (&fb)[4],
+                                          const AScale<MF>& sa, uint32_t sb) {
+  unrolled<4>([&](auto h) {
+    auto part = [&](const Frag8& f, uint32_t code) {
+      const v4i32_t& v = h < 2 ? f.lo : f.hi;
+      return to_bf16x8(v[2 * (h & 1)], v[2 * (h & 1) + 1], code);
+    };
+    bf16x8v_t a[MF];
+    unrolled<MF>([&](auto m) { a[m] = part(fa[m], (sa.w[m / 4] >> (8 * (m & 3))) & 0xffu); });
+    unrolled<4>([&](auto n) {
+      const bf16x8v_t b = part(fb[n], (sb >> (8 * (n / 2))) & 0xffu);
+      unrolled<MF>([&](auto m) { acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a[m], acc[m][n], 0, 0, 0); });
+    });
+  });
 }
 
 __device__ __forceinline__ int swizzle8(int row) { return (row & 7) ^ ((row >> 3) & 1); }
@@ -586,14 +623,15 @@ __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint3
   __builtin_amdgcn_s_setprio(0);
 }
 
-// The K loop of 128 x 256 tiles on four waves, two workgroups a CU (128 x 64 outputs a wave). One LDS buffer: a stage's
-// fragments go to registers at once, and the next stage's loads go out, one behind each MFMA, when every wave has
-// its own (spread over the last MFMAs instead, with the A fragments read between the first ones: 1-2% slower).
-template <bool GLU, int BM, int LPS, typename Dma, typename Fill>
+// The K loop of tiles that share a CU: 128 x 256 on four waves (128 x 64 outputs a wave, two workgroups a CU), 64 x 256
+// and 128 x 128 (64 x 64, three). One LDS buffer: a stage's fragments go to registers at once, and the next stage's
+// loads go out, one behind each MFMA, when every wave has its own (spread over the last MFMAs instead, with the A
+// fragments read between the first ones: 1-2% slower). What a wave waits for is covered by the other workgroups.
+template <bool GLU, int BM, int LPS, int MF, typename Dma, typename Fill>
 __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
-                                            uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[8][4], Dma dma, Fill fill) {
-  Frag8 fa[8], fb[4];
-  AScale<8> sa;
+                                            uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[MF][4], Dma dma, Fill fill) {
+  Frag8 fa[MF], fb[4];
+  AScale<MF> sa;
   uint32_t sb;
   auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
   fill();
@@ -609,7 +647,7 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
       fb[n].lo = ds_read128<n * 2048>(lds0 + b_frag);
       fb[n].hi = ds_read128<n * 2048>((lds0 + b_frag) ^ 64u);
     });
-    unrolled<8>([&](auto m) {
+    unrolled<MF>([&](auto m) {
       fa[m].lo = ds_read128<m * 2048>(lds0 + a_frag);
       fa[m].hi = ds_read128<m * 2048>((lds0 + a_frag) ^ 64u);
     });
@@ -619,10 +657,10 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
 #pragma unroll
     for (int n = 0; n < 4; ++n) fb[n].tie();
 #pragma unroll
-    for (int m = 0; m < 8; ++m) fa[m].tie();
+    for (int m = 0; m < MF; ++m) fa[m].tie();
     asm volatile("s_barrier" ::: "memory");
     fence();
-    unrolled<8>([&](auto m) {
+    unrolled<MF>([&](auto m) {
       unrolled<4>([&](auto n) {
         acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[n].value(), fa[m].value(), acc[m][n], 0, 0,
                                                                     GLU ? n / 2 : 0, (int)sb, m & 3, (int)sa.w[m / 4]);
@@ -634,7 +672,7 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
 }
 
 template <int BM, int BN, int NW, int NS, int EPI>
-__global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp8Params p) {
+__global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2)) void fp8_rows_kernel(Fp8Params p) {
   extern __shared__ __align__(128) char smem[];
   using G = Grid8<BM, BN, NW>;
   using L = Lds8<BM, BN, NW, NS>;
@@ -770,7 +808,7 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
         asm volatile("ds_write_b32 %0, %1" ::"v"(lds0 + L::dst + 4u * (uint32_t)tid), "v"(dst_row) : "memory");
     };
     if constexpr (NS == 1) {
-      single_loop<EPI == F8_GLU, BM, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
+      single_loop<EPI == F8_GLU, BM, LPS, MF>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
     } else if constexpr (PIPE) {
       piped_loop<EPI == F8_GLU, BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
     } else {
@@ -820,7 +858,9 @@ __global__ __launch_bounds__(NW * 64, (NS == 1 ? 2 : 1)) void fp8_rows_kernel(Fp
 #pragma unroll
           for (int m = 0; m < HF; ++m) fa[s & 1][m].tie();
           __builtin_amdgcn_sched_barrier(0);
-          unrolled<HF>([&](auto m) {
+          if constexpr (EPI == F8_GLU && BM == kExactRows) {
+            mma_exact<MF>(acc, fa[0], fb, sa, sb);
+          } else unrolled<HF>([&](auto m) {
             unrolled<NF>([&](auto n) {
               constexpr int f = s * HF + m;
               acc[f][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
@@ -1138,6 +1178,12 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
 }
 
 // ------------------------------------------------------------------ host side
+// Row tiles of a launch, at most: an expert has at least one row in each, and at most one that is not full.
+int64_t row_tiles(const Fp8Params& p, int64_t R, int bm) {
+  const int64_t most = cdiv(R, bm) + (p.offsets ? (R < p.E ? R : p.E) : 0);
+  return most < R ? most : R;
+}
+
 template <int BM, int BN, int NW, int NS, int EPI>
 int launch8(Fp8Params p, int64_t R, hipStream_t s) {
   auto kern = fp8_rows_kernel<BM, BN, NW, NS, EPI>;
@@ -1145,7 +1191,7 @@ int launch8(Fp8Params p, int64_t R, hipStream_t s) {
   int rc = prepare(kern, lds);
   if (rc) return rc;
   p.n_tiles = (int)(EPI == F8_GLU ? blocks_of(p.half) : cdiv(p.N, BN));
-  const int64_t mt = cdiv(R, BM) + (p.offsets ? (R < p.E ? R : p.E) : 0);
+  const int64_t mt = row_tiles(p, R, BM);
   const int64_t total = cdiv(mt * p.n_tiles, (int64_t)kXcds * kSlab) * kXcds * kSlab;  // either tile mapping
   ZMOE_REQUIRE(mt * p.n_tiles < (int64_t)0x7fffff00, ZMOE_ERR_SHAPE, "fp8 product: too many tiles");
   hipLaunchKernelGGL(kern, dim3((unsigned)total), dim3(NW * 64), lds, s, p);
@@ -1161,35 +1207,37 @@ int launch_few(const Fp8Params& p, hipStream_t s) {
 
 // The tile. Wider ones read the operands less often (a 128-deep step of 256 x 256 is 64 KB for 16.8 MFLOP, of 64 x 128
 // 24 KB for 2.1), narrower ones leave less of a short expert's last tile empty and put more workgroups on the 256 CUs.
-//  - Experts of a few rows: what counts is the weight's stream. 128 experts of 2048 -> 2 x 768 and back, 16 rows each:
-//    GLU 84.6 us with 32 rows a tile, 89.7 with 128; back 44.2 with 64 x 128, 45.6 with 128 x 256. 32 rows each: 107.6
-//    against 90.9, and 47 against 47.
-//  - A launch that fits on the CUs at once takes the narrowest tile with which it still does. 4096 -> 4096: 1000 rows
-//    27.6 us (64 x 128), 31.4 (128 x 128), 45 (128 x 256); 2048 rows 47.8, 39.2, 47.6; 128 rows 15.4 (32 x 128), 19.1.
-//    GLU, 4096 -> 2 x 4096: 500 rows 52 (32), 36 (64), 42 (128); 1000 rows 98, 68, 46; 128 x 256 on four waves 51.
-//  - Else 128 x 256 on four waves, two workgroups a CU (one's prologue and epilogue run under the other's loop), or
-//    256 x 256 for experts of six or more such tiles, whose last one, half empty on average, then costs less than a
-//    tenth. 8192 x 7168 -> 4096: 189 and 175 us; 262144 rows over 128 experts, 2048 -> 2 x 768 (GLU): 815 and 797;
-//    65536 rows over 128 experts: 244 and 263, over 64, 1536 -> 2048: 274 and 281; 16384 rows skewed over 64 experts,
-//    7168 -> 2 x 2048 (GLU): 605 and 668, back 356 and 404.
+// Measured in us, bf16 or f16 rows out unless GLU:
+//  - A launch whose workgroups are on the CUs all at once takes the narrowest tile with which they are, its stages loaded
+//    well ahead. 4096 -> 4096: 128 rows 15.5 (32 x 128), 19.0 (64 x 128); 1000 rows 25.8 (64 x 128), 33.3 (128 x 128);
+//    2048 rows 50 (64 x 128), 39 (128 x 128), 47 (128 x 256). GLU, 2048 -> 2 x 768: 1000 rows 13.9 (32 x 256), 16.4
+//    (64 x 256); 4000 rows 40, 22.5, 26.7 (128 x 256). One row for each of 32 experts: GLU 18.4 (32) and 22.9 (64), back
+//    11.3 (64 x 128) and 13.7 (64 x 256).
+//  - Experts of some tens of rows stream their weights: 64 x 256, three workgroups a CU. 128 experts of 2048 -> 2 x 768
+//    (GLU) and back: 4 rows each 73 (76.6 with 32 x 256, 87 with 128 x 256) and 34.4 (38.6 with 64 x 128, 39.6); 32 each 79
+//    (98, 94) and 37.3 (41.5, 42.3); 64 each 88 and 92.6, back 44.3 and 44.5; 126 each 109 and 119, back 70 and 66.
+//  - Else 128 x 256, two workgroups a CU (one's prologue and epilogue run under the other's loop), or 256 x 256 for experts
+//    of six or more such tiles, whose last one, half empty on average, then costs less than a tenth. 8192 x 7168 -> 4096:
+//    189 and 175; 262144 rows over 128 experts, 2048 -> 2 x 768 (GLU): 815 and 797; 65536 rows over 128 experts: 244
+//    and 263, over 64, 1536 -> 2048: 274 and 281; 16384 rows skewed over 64 experts, 7168 -> 2 x 2048 (GLU): 605 and
+//    668, back 356 and 404.
 template <int EPI>
 int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
   const int64_t per = R / p.E;
   const int n = EPI == F8_GLU ? 2 * p.half : p.N;
-  const auto fits = [&](int bm, int bn) { return (cdiv(R, bm) + (p.offsets ? p.E : 0)) * cdiv(n, bn) <= kCus; };
-  const bool few = p.offsets && per <= 24;
+  const auto fits = [&](int bm, int bn, int per_cu) { return row_tiles(p, R, bm) * cdiv(n, bn) <= per_cu * kCus; };
   if constexpr (EPI == F8_GLU) {
-    if (few || fits(32, 256)) return launch8<32, 256, 4, 4, EPI>(p, R, s);
-    if (fits(64, 256)) return launch8<64, 256, 4, 3, EPI>(p, R, s);
-    if (fits(128, 256)) return launch8<128, 256, 8, 3, EPI>(p, R, s);
+    if (fits(32, 256, 1) || R * p.half <= kExactValues) return launch8<kExactRows, 256, 4, 4, EPI>(p, R, s);
+    if (per <= 128 || fits(64, 256, 3)) return launch8<64, 256, 4, 1, EPI>(p, R, s);
   } else {
     if constexpr (EPI != F8_HALF) {
       if (!p.offsets && R <= 16) return launch_few<1, 4, EPI>(p, s);
       if (!p.offsets && R <= 32) return launch_few<2, 2, EPI>(p, s);
     }
-    if (!few && fits(32, 128)) return launch8<32, 128, 4, 4, EPI>(p, R, s);
-    if (few || fits(64, 128)) return launch8<64, 128, 4, 3, EPI>(p, R, s);
-    if (fits(128, 128)) return launch8<128, 128, 4, 2, EPI>(p, R, s);
+    if (fits(32, 128, 1)) return launch8<32, 128, 4, 4, EPI>(p, R, s);
+    if (fits(64, 128, 2)) return launch8<64, 128, 4, 3, EPI>(p, R, s);
+    if (p.offsets && per <= 64) return launch8<64, 256, 4, 1, EPI>(p, R, s);
+    if (fits(128, 128, 3)) return launch8<128, 128, 4, 1, EPI>(p, R, s);
   }
   if (per >= 1536) return launch8<256, 256, 8, 2, EPI>(p, R, s);
   return launch8<128, 256, 4, 1, EPI>(p, R, s);

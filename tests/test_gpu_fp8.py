@@ -170,7 +170,8 @@ def some(n, count, seed):
 @pytest.mark.parametrize("out", ["bf16", "f32"])
 @pytest.mark.parametrize("M,N,K", [(8, 4100, 1160), (16, 33, 8300), (17, 1030, 640), (32, 1500, 130), (40, 300, 8400),
                                    (500, 2000, 300), (1000, 1500, 640), (900, 4000, 512), (1100, 5100, 200),
-                                   (4200, 2304, 384), (900, 9000, 8330), (4200, 2050, 2100), (2100, 4100, 8330)])
+                                   (4200, 2304, 384), (900, 9000, 8330), (1400, 9100, 300), (1400, 9100, 8330),
+                                   (4200, 2050, 2100), (2100, 4100, 8330)])
 def test_dense_product_tiles(M, N, K, out, hip_device):
     """Sizes for every tile (few rows, launches that fit on the CUs at once, long ones), sampled rows and columns."""
     from zmoe import _lib as L
@@ -191,10 +192,10 @@ def test_dense_product_tiles(M, N, K, out, hip_device):
 
 @pytest.mark.parametrize("T,E,k,N,K", [(700, 40, 1, 1500, 384), (60, 2, 2, 500, 200), (2000, 4, 2, 500, 300),
                                        (2600, 16, 2, 1100, 300), (4300, 4, 1, 770, 2050), (6000, 3, 1, 2304, 2100),
-                                       (300, 64, 4, 600, 130)])
-@pytest.mark.parametrize("half", [False, True])
-def test_grouped_product_tiles(T, E, k, N, K, half, hip_device):
-    """The same by expert, bf16 rows and f16 ones with their scales (half a step is 2^-11 |y|, and at most 2^-39 of the
+                                       (300, 64, 4, 600, 130), (9000, 8, 1, 1300, 300), (90, 40, 2, 1500, 8330)])
+@pytest.mark.parametrize("out", ["bf16", "f32", "half"])
+def test_grouped_product_tiles(T, E, k, N, K, out, hip_device):
+    """The same by expert, bf16 and f32 rows and f16 ones with their scales (half a step is 2^-11 |y|, and at most 2^-39 of the
     largest of 64 columns: below the bound's S term, whose columns here differ by far less than 2^20)."""
     idx = random_topk(T, E, k, T + E, 0.0).to(hip_device)
     _, ss, off, _ = z().flatten_sort_count(idx, E)
@@ -207,10 +208,10 @@ def test_grouped_product_tiles(T, E, k, N, K, half, hip_device):
     xr, wr = O.quantize_rows(x)[0][slots // k], O.quantize_weight(W)[0]
     parts = [O.product(xr[i:i + 1], wr[int(e)][ci]) for i, e in enumerate(experts)]
     ref = [torch.cat([p[j] for p in parts]) for j in range(len(parts[0]))]
-    if half:
+    if out == "half":
         y, s = z().fp8_scatter2scatter_half(*q, *w, K, ss, off, k, False, False)
         cols = torch.arange(y.shape[1], device=hip_device)
         v = y.double() * torch.exp2(s.double()[:, cols // 64] - 127)  # (2^c exact in float64)
         check(v[slots][:, ci], *ref, K, half=2.0 ** -11)
     else:
-        check(z().fp8_scatter2scatter(*q, *w, K, ss, off, k, False, False)[slots][:, ci], *ref, K)
+        check(z().fp8_scatter2scatter(*q, *w, K, ss, off, k, False, False, DT[out])[slots][:, ci], *ref, K)

@@ -89,8 +89,9 @@ def test_swiglu_grouped(T, d, f, E, k, skew, hip_device):
 
 
 @pytest.mark.parametrize("T,d,f,E,k", [(600, 300, 1700, 1, 1), (1100, 256, 2000, 1, 1), (1500, 200, 3000, 1, 1),
-                                       (1500, 4100, 3000, 1, 1), (1000, 8300, 4300, 1, 1), (2000, 300, 520, 16, 2),
-                                       (6000, 260, 520, 16, 2), (5000, 4100, 1200, 3, 1)])
+                                       (1500, 4100, 3000, 1, 1), (1000, 8300, 4300, 1, 1), (1500, 200, 4300, 1, 1),
+                                       (1500, 8300, 4300, 1, 1), (2000, 300, 520, 16, 2), (6000, 260, 520, 16, 2),
+                                       (5000, 4100, 1200, 3, 1)])
 def test_swiglu_tiles(T, d, f, E, k, hip_device):
     """Sizes for every tile, sampled rows."""
     from zmoe import ops
