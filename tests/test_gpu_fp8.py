@@ -215,3 +215,34 @@ def test_grouped_product_tiles(T, E, k, N, K, out, hip_device):
         check(v[slots][:, ci], *ref, K, half=2.0 ** -11)
     else:
         check(z().fp8_scatter2scatter(*q, *w, K, ss, off, k, False, False, DT[out])[slots][:, ci], *ref, K)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantize_weight_views_and_values_not_finite(dtype, hip_device):
+    """Rows that start on 16, 4 and 2 (or 4) bytes give the same bytes; inf and NaN become NaN beside the finite values."""
+    E, N, K = 2, 140, 262
+    base = (torch.randn(E, N, 300, generator=gen(3)) * 0.05).to(DT[dtype]).to(hip_device)
+    base[0, 3, 20], base[1, 139, 140], base[1, 0, 130] = float("inf"), float("-inf"), float("nan")
+    for at in (0, 2, 1):
+        view = base[:, :, at:at + K]
+        ref = z().fp8_quantize_weight(view.contiguous(), transposed=True)
+        for a, b in zip(z().fp8_quantize_weight(view, transposed=True)[::2], ref[::2]):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        q = ref[0].float()[..., :K]
+        assert torch.equal(torch.isnan(q), ~torch.isfinite(view.float()))
+        assert torch.equal(torch.isnan(ref[2].float()[..., :N]), ~torch.isfinite(view.float()).transpose(1, 2))
+
+
+def test_dense_rows_past_two_gib(hip_device):
+    """Rows in order have no limit on their span (gathered ones have); the last ones are right too."""
+    M, N, K = 1100000, 40, 2048
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=hip_device).normal_(generator=torch.Generator(hip_device).manual_seed(1))
+    w = z().fp8_quantize_weight((torch.randn(N, K, generator=gen(2)) * 0.05).to(hip_device))
+    xq, xs = z().fp8_quantize_rows(x)
+    y = z().fp8_scatter2scatter(xq, xs, *w, K)
+    for rows in (slice(0, 40), slice(M // 2, M // 2 + 40), slice(M - 40, M)):
+        a, wr = O.quantize_rows(x[rows])[0], rows_values(w[0], w[1].repeat_interleave(128, 0)[:N], K)[0]
+        check(y[rows], *O.product(a, wr), K)
+    ss, off = torch.arange(M, device=hip_device), torch.tensor([M], device=hip_device)
+    with pytest.raises(Exception, match="2 GiB"):
+        z().fp8_scatter2scatter(xq, xs, w[0][None], w[1][None], K, ss, off, 1, False, True)

@@ -334,6 +334,72 @@ def test_half_rows_and_their_sums(T, k, N, K, hip_device):
                 assert not out[[i for i in range(T + 3) if i not in at.tolist()]].any()
 
 
+@pytest.mark.parametrize("T", [1, 2, 5])
+def test_few_rows_of_narrow_experts_are_exact_before_the_rounding(T, hip_device):
+    """The activations of a small launch are rounded to e4m3 from f32 sums, so that none lands on a neighbour (2^-3 away,
+    0.018 of the result in single rows) and the result's error is its own rounding to bf16: at most 2^-8 of each value,
+    uniform below half a step, so of a norm hardly over 2^-8 / sqrt(3 * 1.5 / ln 2) = 0.0015; the bound is half of 2^-8."""
+    d, f, E, k = 512, 160, 32, 2
+    for seed in range(20):
+        x, W1 = activations(T, d, BF, seed, hip_device), weight((2 * E, f, d), seed + 1, BF, hip_device, d ** -0.5)
+        W2 = weight((E, d, f), seed + 2, BF, hip_device, f ** -0.5)
+        idx = random_topk(T, E, k, seed).to(hip_device)
+        p = torch.softmax(torch.randn(T, k, generator=gen(seed)), -1).to(hip_device)
+        out, _ = zl().fp8_glu_experts(x, p, idx, *zl().fp8_quantize_weight(W1, False), *zl().fp8_quantize_weight(W2, False),
+                                      None, None, 0)
+        xr, w1, w2 = O.quantize_rows(x)[0], O.quantize_weight(W1)[0], O.quantize_weight(W2)[0]
+        ref = torch.zeros(T, d, dtype=torch.float64, device=hip_device)
+        for t in range(T):
+            for j in range(k):
+                e = int(idx[t, j])
+                u, g = xr[t] @ w1[2 * e].T, xr[t] @ w1[2 * e + 1].T
+                a = O.quantize_rows((g * torch.sigmoid(g) * u).unsqueeze(0))[0]
+                ref[t] += p[t, j].double() * (a @ w2[e].T)[0]
+        assert float((out.double() - ref).norm() / ref.norm()) <= 2.0 ** -9
+
+
+def test_experts_not_finite_and_twice_the_same(hip_device):
+    """A row with a NaN and one with an inf spoil themselves alone; a token may name one expert twice."""
+    from zmoe import ops
+
+    T, d, f, E, k = 9, 256, 130, 4, 2
+    x, idx = activations(T, d, BF, 1, hip_device), random_topk(T, E, k, 3).to(hip_device)
+    idx[4, 1] = idx[4, 0]
+    p = torch.rand(T, k, generator=gen(2)).to(hip_device)
+    w = [*ops.fp8_quantize_weight(weight((2 * E, f, d), 3, BF, hip_device)), *ops.fp8_quantize_weight(weight((E, d, f), 4, BF, hip_device))]
+    out, off = ops.fp8_glu_experts(x, p, idx, *w)
+    bad = x.clone()
+    bad[2, 7], bad[6, 200] = float("nan"), float("inf")
+    got, _ = ops.fp8_glu_experts(bad, p, idx, *w)
+    spoilt = torch.tensor([t in (2, 6) for t in range(T)], device=hip_device)
+    assert torch.isnan(got[spoilt]).all() and torch.equal(got[~spoilt], out[~spoilt])
+    one = torch.stack([p[4].sum(), torch.zeros((), device=hip_device)]).view(1, 2)
+    alone, _ = ops.fp8_glu_experts(x[4:5], one, idx[4:5], *w)
+    assert float((alone - out[4:5]).float().norm()) <= 2.0 ** -7 * float(alone.float().norm())
+
+
+def test_on_another_stream(hip_device):
+    """Work queued on a side stream, while the default one is busy with other calls of the same ops."""
+    from zmoe import ops
+
+    T, d, f, E, k = 300, 512, 160, 8, 2
+    x, idx = activations(T, d, BF, 1, hip_device), random_topk(T, E, k, 3).to(hip_device)
+    p = torch.rand(T, k, generator=gen(2)).to(hip_device)
+    w = [*ops.fp8_quantize_weight(weight((2 * E, f, d), 3, BF, hip_device)), *ops.fp8_quantize_weight(weight((E, d, f), 4, BF, hip_device))]
+    run = lambda: (ops.fp8_glu_experts(x, p, idx, *w)[0], ops.fp8_linear(x, w[0][0], w[1][0]))  # noqa: E731
+    ref = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        theirs = [run() for _ in range(5)]
+    ours = [run() for _ in range(5)]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for pair in theirs + ours:
+        for a, b in zip(pair, ref):
+            assert torch.equal(a, b)
+
+
 def test_half_rows_not_finite(hip_device):
     """inf and NaN reach their own rows only, and the largest finite sums do not overflow."""
     from zmoe import ops
