@@ -742,12 +742,22 @@ Tensor combine_half(const Tensor& Y, const Tensor& Ys, const Opt& gates, int64_t
   return op.call(Y, Ys, gates, k, N, addend, out_rows, out_total);
 }
 
+// Rows that zmoe_fp8_linear_few takes as they are, of a product for which it is faster (FP8_FEW_WEIGHTS in ops.py).
+bool few8(const Tensor& x, int64_t stride, int64_t N) {
+  return x.size(0) <= 16 && x.size(1) % 8 == 0 && N * x.size(1) <= (1 << 24) && stride % (16 / x.element_size()) == 0 &&
+         reinterpret_cast<uintptr_t>(raw(x)) % 16 == 0;
+}
+
 Tensor fp8_linear(const Tensor& x, const Tensor& wq, const Tensor& ws) {
   if (x.is_cuda() && known(x) && apart(x) && x.size(1) > 0 && weight8(wq, ws, x.size(1), 2, x)) {
     const c10::DeviceGuard guard(x.device());
     const int64_t M = x.size(0), K = x.size(1), N = wq.size(0);
-    const Rows8 r = empty8(M, K, x);
+    const int64_t stride = std::max(x.stride(0), K);
     Tensor Y = empty({M, N}, x);
+    if (few8(x, stride, N) && zmoe_fp8_linear_few(raw(x), stride, M, raw(wq), raw(ws), K, N, code(x), raw(Y), N,
+                                               stream_of(x)) == ZMOE_OK)
+      return Y;
+    const Rows8 r = empty8(M, K, x);
     if (quantize_into(x, r, std::nullopt, 1, std::nullopt) &&
         zmoe_fp8_scatter2scatter(raw(r.q), raw(r.s), M, raw(wq), raw(ws), nullptr, nullptr, K, N, 1, 1, 1, 1, code(Y),
                                  raw(Y), N, stream_of(x)) == ZMOE_OK)

@@ -257,7 +257,7 @@ constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 struct Fp8Params {
   const uint8_t* a;
   const uint8_t* as;
-  int64_t lda, a_pitch;    // bytes between rows of A and of its scales
+  int64_t lda, a_pitch;    // bytes between rows of A and of its scales (few unquantised rows: K, elements between them)
   const int64_t* a_rows;   // A row of sorted row i = a_rows[i] / a_div (null: i)
   int a_div;
   int64_t a_bytes;         // bytes of A
@@ -1108,8 +1108,53 @@ __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __res
 constexpr int kFewWaves = 8;
 constexpr int kCus = 256;
 
-template <int MF, int U, int EPI>
+// What a lane of a fragment holds of a block of a row before it is quantised: values 16 g .. 16 g + 15 and 64 more on.
+template <typename T>
+struct Raw8 {
+  static constexpr int VN = 16 / sizeof(T);
+  uint4 w[32 / VN];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int64_t c, int64_t K) {  // K in whole eights
+#pragma unroll
+    for (int q = 0; q < 32 / VN; ++q) {
+      const int64_t at = c + (q * VN & 15) + (q * VN & 16) * 4;
+      w[q] = at < K ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  // The block's scale (its four lanes are this row's) and the lane's part of it: quantize_rows_kernel's bytes.
+  __device__ __forceinline__ int quantize(Frag8& f) const {
+    float v[32];
+#pragma unroll
+    for (int q = 0; q < 32 / VN; ++q) unpack_chunk(w[q], &v[q * VN], T{});
+    uint32_t a = 0;
+#pragma unroll
+    for (int u = 0; u < 32; ++u) a = max(a, __float_as_uint(v[u]) & 0x7fffffffu);
+    const bool odd = __builtin_amdgcn_ballot_w64(a >= kInfBits) != 0;
+    if (odd) {
+      float m = 0.f;
+#pragma unroll
+      for (int u = 0; u < 32; ++u) m = fmaxf(m, finite_abs(v[u]));
+      a = __float_as_uint(m);
+    }
+    const int code = scale_code(__uint_as_float(max_rows4(a)));
+    const float inv = scale_inverse(code);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float x[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      const int b = (int)(odd ? quantize4(x, inv) : pack_e4m3(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv));
+      if (q < 4) f.lo[q] = b;
+      else f.hi[q - 4] = b;
+    }
+    return code;
+  }
+};
+
+// X: uint8_t for quantised rows, or the type of rows (at most 16 of them) that each wave quantises for itself as it goes,
+// in registers: its lanes hold whole blocks. (One bf16 row 2048 -> 1536: 5.4 us, 6.3 with a launch of the quantiser;
+// 16 rows 4096 -> 4096 9.4 and 9.8; one row 16384 -> 4096 24.8 and 16.3, as every workgroup quantises the rows again.)
+template <int MF, int U, int EPI, typename X>
 __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
+  constexpr bool RAW = !std::is_same<X, uint8_t>::value;
+  static_assert(!RAW || MF == 1, "16 rows");
   __shared__ float part[kFewWaves][16][20];
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lane = (int)threadIdx.x & 63, r16 = lane & 15, g4 = lane >> 4;
@@ -1119,8 +1164,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
 
   // rows and columns past the end repeat the last one: their outputs are not stored
   const int n = col0 + r16 < p.N ? col0 + r16 : p.N - 1;
-  const uint8_t *a[MF], *as[MF], *b = p.b + (int64_t)n * p.lda + (int64_t)k0 * kBlk + 16 * g4;
+  const uint8_t *a[MF], *as[MF], *b = p.b + ((int64_t)n * p.nk + k0) * kBlk + 16 * g4;
   const uint8_t* bs = p.bs + (int64_t)(col0 / kBlk) * p.bs_pitch + k0;
+  const X* x = reinterpret_cast<const X*>(p.a) + (r16 < rows ? r16 : rows - 1) * p.a_pitch;  // RAW: K is lda
 #pragma unroll
   for (int m = 0; m < MF; ++m) {
     const int r = 16 * m + r16 < rows ? 16 * m + r16 : rows - 1;
@@ -1135,23 +1181,29 @@ __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
   for (int i = 0; i < cnt; i += U) {
     Frag8 fb[U], fa[U][MF];
     int sb[U], sa[U][MF];
+    Raw8<std::conditional_t<RAW, X, float>> raw[RAW ? U : 1];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int kb = i + u < cnt ? i + u : cnt - 1;
       sb[u] = bs[kb];
       fb[u].lo = load(b + (int64_t)kb * kBlk);
       fb[u].hi = load(b + (int64_t)kb * kBlk + 64);
+      if constexpr (RAW) {
+        raw[u].load(x, (int64_t)(k0 + kb) * kBlk + 16 * g4, p.lda);
+      } else {
 #pragma unroll
-      for (int m = 0; m < MF; ++m) {
-        fa[u][m].lo = load(a[m] + (int64_t)kb * kBlk);
-        fa[u][m].hi = load(a[m] + (int64_t)kb * kBlk + 64);
-        sa[u][m] = as[m][kb];
+        for (int m = 0; m < MF; ++m) {
+          fa[u][m].lo = load(a[m] + (int64_t)kb * kBlk);
+          fa[u][m].hi = load(a[m] + (int64_t)kb * kBlk + 64);
+          sa[u][m] = as[m][kb];
+        }
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // all loads first
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i + u < cnt) {
+        if constexpr (RAW) sa[u][0] = raw[u].quantize(fa[u][0]);
 #pragma unroll
         for (int m = 0; m < MF; ++m)
           acc[m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[u].value(), fa[u][m].value(), acc[m], 0, 0, 0,
@@ -1198,9 +1250,9 @@ int launch8(Fp8Params p, int64_t R, hipStream_t s) {
   return check_launch("fp8 rows kernel");
 }
 
-template <int MF, int U, int EPI>
+template <int MF, int U, int EPI, typename X = uint8_t>
 int launch_few(const Fp8Params& p, hipStream_t s) {
-  auto kern = fp8_few_kernel<MF, U, EPI>;
+  auto kern = fp8_few_kernel<MF, U, EPI, X>;
   hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(p.N, 16)), dim3(kFewWaves * 64), 0, s, p);
   return check_launch("fp8 few rows kernel");
 }
@@ -1403,6 +1455,33 @@ extern "C" int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t 
                                         int64_t y_stride, void* stream) {
   return scatter2scatter8("fp8_scatter2scatter", Xq, Xs, M, Wq, Ws, sorted_scattered_idxs, expert_offsets, K, N, E, k,
                           x_grouped, y_grouped, out_dtype, false, Y, nullptr, y_stride, stream);
+}
+
+extern "C" int zmoe_fp8_linear_few(const void* X, int64_t x_stride, int64_t M, const void* Wq, const void* Ws, int64_t K,
+                                   int64_t N, int dtype, void* Y, int64_t y_stride, void* stream) {
+  int rc = quantize_checks("fp8_linear_few", M, K, dtype);
+  if (rc) return rc;
+  ZMOE_REQUIRE(M <= 16 && K % 8 == 0 && N >= 1 && N < (1 << 30) && x_stride >= K && x_stride % (16 / dtype_size(dtype)) == 0 &&
+                   y_stride >= N,
+               ZMOE_ERR_SHAPE, "fp8_linear_few: at most 16 rows in whole 16-byte chunks (M=%lld K=%lld N=%lld)", (long long)M,
+               (long long)K, (long long)N);
+  if (M == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(X && Y, ZMOE_ERR_NULL, "fp8_linear_few: null pointer");
+  ZMOE_REQUIRE(aligned16(X) && (reinterpret_cast<uintptr_t>(Y) % dtype_size(dtype)) == 0, ZMOE_ERR_ALIGN,
+               "fp8_linear_few: X on 16 bytes, Y on its elements");
+  Fp8Params p{};
+  rc = product_operands("fp8_linear_few", X, Ws, M, Wq, Ws, K, N, blocks_of(N), 1, nullptr, p);
+  if (rc) return rc;
+  p.as = nullptr;
+  p.lda = K;
+  p.a_pitch = x_stride;
+  p.c = Y;
+  p.ldc = y_stride;
+  p.N = (int)N;
+  p.ns_m = (int)M;
+  hipStream_t s = as_stream(stream);
+  return dtype == ZMOE_DTYPE_BF16 ? launch_few<1, 4, F8_STORE_BF16, uint16_t>(p, s)
+                                  : launch_few<1, 2, F8_STORE_F32, float>(p, s);
 }
 
 extern "C" int zmoe_fp8_scatter2scatter_half(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,

@@ -84,6 +84,7 @@ SIGNATURES = {
     "zmoe_fp8_quantize_rows": (I32, [P, I64, I64, P, I32, P, I64, I64, I32, P, P, P]),
     "zmoe_fp8_quantize_weight": (I32, [P, I64, I64, I64, I64, I64, I32, P, P, P, P, P]),
     "zmoe_fp8_scatter2scatter": (I32, [P, P, I64, P, P, P, P, I64, I64, I32, I32, I32, I32, I32, P, I64, P]),
+    "zmoe_fp8_linear_few": (I32, [P, I64, I64, P, P, I64, I64, I32, P, I64, P]),
     "zmoe_fp8_scatter2scatter_half": (I32, [P, P, I64, P, P, P, P, I64, I64, I32, I32, I32, I32, P, P, P]),
     "zmoe_combine_half": (I32, [P, P, P, P, I64, I32, I64, I32, P, I64, P, P]),
     "zmoe_fp8_glu_w1_forward": (I32, [P, P, I64, P, P, P, P, I64, I64, I32, I32, P, P, P]),

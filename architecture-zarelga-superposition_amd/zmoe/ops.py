@@ -1079,9 +1079,28 @@ def norm_residual_backward(dR_out: Optional[torch.Tensor], dX: Optional[torch.Te
             dgate, None if dscale is None else dscale.view(scale.shape))
 
 
+# Elements of a weight up to which a few rows are quantised in the product's launch: every workgroup quantises its part of
+# them again. One bf16 row, 2048 -> 1536: 5.4 us, in two launches 6.3 (and 14.4 of host time against 8.9); 16 rows
+# 4096 -> 4096 9.4 and 9.8; one row 16384 -> 4096 24.8 and 16.3.
+FP8_FEW_WEIGHTS = 1 << 24
+
+
 # Whole fp8 paths in one call each (the host's share of a small batch's time is one op's).
 def fp8_linear(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor) -> torch.Tensor:
-    """x [M, K] times a quantised weight wq [N, Kp]: [M, N] of x's dtype; x's rows are quantised first."""
+    """x [M, K] times a quantised weight wq [N, Kp]: [M, N] of x's dtype; x's rows are quantised first (a few of them in
+    the product's own launch)."""
+    if (x.dim() == wq.dim() == 2 and x.dtype in _DT and x.shape[0] <= 16 and x.shape[1] % 8 == 0
+            and wq.shape[0] * x.shape[1] <= FP8_FEW_WEIGHTS):
+        dev = _require_cuda(x, wq, ws)
+        r, K = _rows_apart(x), x.shape[1]
+        wq, ws = _fp8_operand(wq, ws, K, "fp8_linear")
+        stride = max(r.stride(0), K)
+        if ws.shape[0] == -(-wq.shape[0] // FP8_BLOCK) and r.data_ptr() % 16 == 0 and stride * r.element_size() % 16 == 0:
+            out = torch.empty((r.shape[0], wq.shape[0]), dtype=x.dtype, device=dev)
+            with profiling.region("fp8_scatter2scatter", dev):
+                L.call("zmoe_fp8_linear_few", _ptr(r), stride, r.shape[0], _ptr(wq), _ptr(ws), K, wq.shape[0],
+                       _DT[x.dtype], _ptr(out), wq.shape[0], _stream(dev))
+            return out
     return fp8_scatter2scatter(*fp8_quantize_rows(x), wq, ws, x.shape[1], out_dtype=x.dtype)
 
 

@@ -463,6 +463,12 @@ int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const vo
                              int64_t N, int E, int k, int x_grouped, int y_grouped, int out_dtype, void* Y,
                              int64_t y_stride, void* stream);
 
+/* The dense product of at most 16 rows X [M, K] (F32 or BF16 on 16 bytes, rows x_stride elements apart, K and x_stride in
+ * whole 16-byte chunks and K in whole eights), quantised in the same launch: zmoe_fp8_quantize_rows and the product
+ * above, bit for bit, Y of X's type. */
+int zmoe_fp8_linear_few(const void* X, int64_t x_stride, int64_t M, const void* Wq, const void* Ws, int64_t K, int64_t N,
+                        int dtype, void* Y, int64_t y_stride, void* stream);
+
 /* The same into rows that a sum over each token's slots reads next: Y f16 [R, Nh], Nh = 64 ceil(N / 64), each 64 columns
  * of a row divided by a power of two 2^c, Ys [R, Nh / 64] bytes c + 127, which puts the largest into [2^14, 2^15).
  * zmoe_combine_half: out[t] = addend[t] + sum_j gates[t, j] Y[t k + j] (dtype of out [T, N] and the addend; gates f32, NULL:

@@ -92,6 +92,18 @@ def test_product_refusals(half):
     assert call(name, *empty) == OK
 
 
+def test_few_rows_refusals():
+    # X, x_stride, M, Wq, Ws, K, N, dtype, Y, y_stride, stream
+    good = (P, 256, 16, P, P, 256, 64, BF16, P, 64, None)
+    refused("zmoe_fp8_linear_few", good, [
+        (DTYPE, {7: 5}), (SHAPE, {2: 17}), (SHAPE, {2: -1}), (SHAPE, {5: 0}), (SHAPE, {5: 252}), (SHAPE, {1: 248}), (SHAPE, {1: 260}),
+        (SHAPE, {7: F32, 1: 258}), (SHAPE, {6: 0}), (SHAPE, {9: 63}), (NULL, {0: None}), (NULL, {3: None}), (NULL, {4: None}),
+        (NULL, {8: None}), (ALIGN, {0: P + 8}), (ALIGN, {3: P + 8}), (ALIGN, {4: P + 2}), (ALIGN, {8: P + 1}),
+        (SHAPE, {6: 1 << 23, 9: 1 << 23}),
+    ])
+    assert call("zmoe_fp8_linear_few", None, 256, 0, None, None, 256, 64, BF16, None, 64, None) == OK
+
+
 def test_glu_refusals():
     # Xq, Xs, T, W1q, W1s, idxs, offsets, d, f, E, k, Aq, As, stream
     good = (P, P, 16, P, P, P, P, 256, 64, 4, 2, P, P, None)

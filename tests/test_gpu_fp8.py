@@ -233,6 +233,26 @@ def test_quantize_weight_views_and_values_not_finite(dtype, hip_device):
         assert torch.equal(torch.isnan(ref[2].float()[..., :N]), ~torch.isfinite(view.float()).transpose(1, 2))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 8), (1, 1536, 2048), (3, 130, 136), (16, 40, 4104), (16, 1000, 1000), (5, 70, 16392),
+                                   (9, 33, 512)])
+def test_few_rows_quantised_in_the_product(M, N, K, dtype, hip_device):
+    """The same, bit for bit, as quantising first: also rows with a stride, values that are not finite, zero blocks."""
+    base = activations(M, K + 24, torch.float32, M + K, hip_device).to(DT[dtype])
+    x = base[:, 8:8 + K]
+    x[M // 2, K // 2], x[M - 1, :8] = float("nan"), 0.0
+    if M > 2:
+        x[1, K - 1], x[0] = float("-inf"), 0.0
+    wq, ws = z().fp8_quantize_weight((torch.randn(N, K, generator=gen(N)) * 0.1).to(DT[dtype]).to(hip_device))
+    got = z().fp8_linear(x, wq, ws)
+    q, s = z().fp8_quantize_rows(x)
+    assert same(got, z().fp8_scatter2scatter(q, s, wq, ws, K, out_dtype=DT[dtype]))
+    ok = torch.isfinite(x.float()).all(1)
+    assert torch.isnan(got[~ok]).all() and not torch.isnan(got[ok]).any()
+    odd = base[:, 7:7 + K]  # off 16 bytes: quantised first
+    assert same(z().fp8_linear(odd, wq, ws), z().fp8_linear(odd.clone(), wq, ws))
+
+
 def test_dense_rows_past_two_gib(hip_device):
     """Rows in order have no limit on their span (gathered ones have); the last ones are right too."""
     M, N, K = 1100000, 40, 2048
