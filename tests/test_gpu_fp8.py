@@ -217,6 +217,28 @@ def test_grouped_product_tiles(T, E, k, N, K, out, hip_device):
         check(z().fp8_scatter2scatter(*q, *w, K, ss, off, k, False, False, DT[out])[slots][:, ci], *ref, K)
 
 
+@pytest.mark.parametrize("E,T,empty", [(1, 300, 0.0), (2, 1, 0.0), (63, 40, 0.5), (64, 200, 0.9), (65, 3000, 0.0), (257, 700, 0.3),
+                                       (1000, 5000, 0.98), (1024, 9000, 0.0), (1024, 2, 0.0)])
+def test_every_expert_count(E, T, empty, hip_device):
+    """Tiles are found among up to 1024 experts, many of them without a row (also the first and the last)."""
+    N, K = 40, 130
+    g = gen(E + T)
+    some_e = (torch.rand(E, generator=g) >= empty).nonzero().flatten()
+    if empty and len(some_e) > 2:
+        some_e = some_e[(some_e != 0) & (some_e != E - 1)]
+    idx = some_e[torch.randint(len(some_e), (T, 1), generator=g)].to(hip_device)
+    idx[T // 2:] = idx[T // 2].clone()  # half the rows to one of them
+    _, ss, off, _ = z().flatten_sort_count(idx, E)
+    x = activations(T, K, torch.bfloat16, T, hip_device)
+    W = (torch.randn(E, N, K, generator=g) * 0.1).to(torch.bfloat16).to(hip_device)
+    q, w = z().fp8_quantize_rows(x), z().fp8_quantize_weight(W)
+    got = z().fp8_scatter2scatter(*q, *w, K, ss, off, 1, False, False, torch.float32)
+    xr, wr = O.quantize_rows(x)[0], O.quantize_weight(W)[0]
+    for e in idx.unique().tolist()[:40] + [int(idx[-1])]:
+        rows = (idx[:, 0] == e).nonzero().flatten()
+        check(got[rows], *O.product(xr[rows], wr[e]), K)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_quantize_weight_views_and_values_not_finite(dtype, hip_device):
     """Rows that start on 16, 4 and 2 (or 4) bytes give the same bytes; inf and NaN become NaN beside the finite values."""
