@@ -63,14 +63,14 @@ __device__ __forceinline__ uint32_t quantize4(const float (&v)[4], float inv) {
 }
 
 // Largest of v over 16 consecutive lanes, in every one of them.
-__device__ __forceinline__ float max16(float v) {
-  auto dpp = [](float x, auto ctrl) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  auto dpp = [](uint32_t x, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true);
   };
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0xB1>{}));   // lane ^ 1
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x4E>{}));   // lane ^ 2
-  v = fmaxf(v, dpp(v, std::integral_constant<int, 0x141>{}));  // 7 - lane within 8
-  return fmaxf(v, dpp(v, std::integral_constant<int, 0x140>{}));  // 15 - lane within 16
+  v = max(v, dpp(v, std::integral_constant<int, 0xB1>{}));   // lane ^ 1
+  v = max(v, dpp(v, std::integral_constant<int, 0x4E>{}));   // lane ^ 2
+  v = max(v, dpp(v, std::integral_constant<int, 0x141>{}));  // 7 - lane within 8
+  return max(v, dpp(v, std::integral_constant<int, 0x140>{}));  // 15 - lane within 16
 }
 
 // How rows can be loaded: in 16-byte chunks, in 4-byte pairs (16-bit elements), one by one.
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
                                                             uint8_t* __restrict__ S, int64_t pitch) {
   const uint32_t g = blockIdx.x * 16 + threadIdx.x / 16;  // (row, block)
   if (g >= total) return;  // whole groups of 16 lanes
-  const uint32_t i = g / (uint32_t)nb, b = g % (uint32_t)nb;
+  const uint32_t i = g / (uint32_t)nb, b = g - i * (uint32_t)nb;
   const int lane = threadIdx.x & 15;
   int64_t src = i;
   float sc = 1.f;
@@ -135,16 +135,28 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
   const int64_t c = (int64_t)b * kBlk + lane * 8;
   float v[8];
   load8(X + (src < 0 ? 0 : src) * ldx, c, src < 0 ? 0 : K, width, v);
-  float a = 0.f;
+  if (row_scale != nullptr) {
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    if (row_scale != nullptr) v[u] *= sc;
-    a = fmaxf(a, finite_abs(v[u]));
+    for (int u = 0; u < 8; ++u) v[u] *= sc;
   }
-  const int code = scale_code(max16(a));
+  uint32_t a = 0;  // largest magnitude, as bits: inf and NaN show
+#pragma unroll
+  for (int u = 0; u < 8; ++u) a = max(a, __float_as_uint(v[u]) & 0x7fffffffu);
+  const bool odd = __builtin_amdgcn_ballot_w64(a >= kInfBits) != 0;
+  if (odd) {
+    float m = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m = fmaxf(m, finite_abs(v[u]));
+    a = __float_as_uint(m);
+  }
+  const int code = scale_code(__uint_as_float(max16(a)));
   const float inv = scale_inverse(code);
   const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
-  *reinterpret_cast<uint2*>(Q + (int64_t)i * nb * kBlk + c) = make_uint2(quantize4(lo, inv), quantize4(hi, inv));
+  uint2 w;
+  if (odd) w = make_uint2(quantize4(lo, inv), quantize4(hi, inv));
+  else w = make_uint2(pack_e4m3(lo[0] * inv, lo[1] * inv, lo[2] * inv, lo[3] * inv),
+                      pack_e4m3(hi[0] * inv, hi[1] * inv, hi[2] * inv, hi[3] * inv));
+  *reinterpret_cast<uint2*>(Q + (int64_t)g * kBlk + lane * 8) = w;
   if (lane == 0) S[(int64_t)i * pitch + b] = (uint8_t)code;
 }
 
