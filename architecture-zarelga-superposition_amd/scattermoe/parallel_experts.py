@@ -33,7 +33,8 @@ def flatten_sort_count(expert_idxs: torch.Tensor, num_experts: int):
     Returns (sorted_expert_idxs, sorted_scattered_idxs, expert_offsets); equal
     experts keep flat-slot order, offsets are inclusive ends.
     """
-    se, ss, off, _ = _zl.flatten_sort_count(expert_idxs, num_experts)
+    with torch.no_grad():  # (whole numbers: nothing to record, and the op's native form runs)
+        se, ss, off, _ = _zl.flatten_sort_count(expert_idxs, num_experts)
     return se, ss, off
 
 
