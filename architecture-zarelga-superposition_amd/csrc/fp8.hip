@@ -256,14 +256,14 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
 // are the MFMA's first operand, so a lane ends up with 4 consecutive output columns of one row.
 // F8_HALF: rows that a sum over a token's k slots reads next, as f16 with a power-of-two scale for each 64 columns:
 // 16 bits like bf16, but within 2^-11 of each value (bf16: 2^-8), so that the sum has its own rounding only.
-enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2, F8_HALF = 3 };
-// The SwiGLU's sums are rounded to e4m3 next, where an error of a few 2^-13 (a scaled MFMA's, of its largest terms) turns
-// one value in some thousand to its neighbour, 2^-3 away: little in the mean over many rows (0.0023 from the exact
-// result where bf16's own rounding is 0.0017), but up to 0.018 for a single row of a narrow expert. Tiles of 32 rows,
-// whose launches are bound by the weights' stream, therefore take their terms to bf16 (exact) and add in f32: 0.0017,
-// and 18.4 -> 19.7 us for one row in each of 32 experts of 2048 -> 2 x 768.
-constexpr int kExactRows = 32;
-constexpr int64_t kExactValues = 1 << 19;  // activations of a launch up to which the mean does not cover it
+enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2, F8_HALF = 3, F8_GLU_EXACT = 4 };
+constexpr bool is_glu(int epi) { return epi == F8_GLU || epi == F8_GLU_EXACT; }
+// F8_GLU_EXACT: the SwiGLU's sums are rounded to e4m3 next, where an error of a few 2^-13 (a scaled MFMA's, of its largest
+// terms) turns one value in some thousand to its neighbour, 2^-3 away: little in the mean over many rows (0.0023 from
+// the exact result where bf16's own rounding is 0.0017), but up to 0.018 for a single row of a narrow expert. Launches of
+// few activations, which the weights' stream bounds, therefore take their terms to bf16 (exact) and add in f32: 0.0017. One
+// row in each of 32 experts of 2048 -> 2 x 768: 18.4 -> 20 us; 128 such experts of 4 rows 72 -> 80, of 21 rows 75 -> 84.
+constexpr int64_t kExactValues = 1 << 21;  // activations of a launch up to which the mean does not cover it
 constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 
 struct Fp8Params {
@@ -378,10 +378,11 @@ __device__ __forceinline__ void unrolled(F f) {
   unrolled(std::make_integer_sequence<int, N>{}, f);
 }
 
-// One stage of the wave's MF x 4 fragments with their sums at f32's precision: bf16 MFMAs of 32 depths.
-template <int MF>
+// One stage of the wave's MF x 4 fragments with their sums at f32's precision: bf16 MFMAs of 32 depths. between(i) is
+// called 16 times, between the MFMAs.
+template <int MF, typename Between>
 __device__ __forceinline__ void mma_exact(f32x4_t (&acc)[MF][4], const Frag8 (&fa)[MF], const Frag8 (&fb)[4],
-                                          const AScale<MF>& sa, uint32_t sb) {
+                                          const AScale<MF>& sa, uint32_t sb, Between between) {
   unrolled<4>([&](auto h) {
     auto part = [&](const Frag8& f, uint32_t code) {
       const v4i32_t& v = h < 2 ? f.lo : f.hi;
@@ -392,6 +393,7 @@ __device__ __forceinline__ void mma_exact(f32x4_t (&acc)[MF][4], const Frag8 (&f
     unrolled<4>([&](auto n) {
       const bf16x8v_t b = part(fb[n], (sb >> (8 * (n / 2))) & 0xffu);
       unrolled<MF>([&](auto m) { acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a[m], acc[m][n], 0, 0, 0); });
+      between(std::integral_constant<int, h * 4 + n>{});
     });
   });
 }
@@ -639,9 +641,10 @@ __device__ __forceinline__ void piped_loop(int nst, int c0, uint32_t lds0, uint3
 // and 128 x 128 (64 x 64, three). One LDS buffer: a stage's fragments go to registers at once, and the next stage's
 // loads go out, one behind each MFMA, when every wave has its own (spread over the last MFMAs instead, with the A
 // fragments read between the first ones: 1-2% slower). What a wave waits for is covered by the other workgroups.
-template <bool GLU, int BM, int LPS, int MF, typename Dma, typename Fill>
+template <int EPI, int BM, int LPS, int MF, typename Dma, typename Fill>
 __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint32_t a_frag, uint32_t b_frag,
                                             uint32_t as_lane, uint32_t bs_lane, f32x4_t (&acc)[MF][4], Dma dma, Fill fill) {
+  constexpr bool GLU = is_glu(EPI);
   Frag8 fa[MF], fb[4];
   AScale<MF> sa;
   uint32_t sb;
@@ -672,7 +675,12 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
     for (int m = 0; m < MF; ++m) fa[m].tie();
     asm volatile("s_barrier" ::: "memory");
     fence();
-    unrolled<MF>([&](auto m) {
+    if constexpr (EPI == F8_GLU_EXACT) {
+      mma_exact<MF>(acc, fa, fb, sa, sb, [&](auto i) {
+        if constexpr (i < LPS) dma(i, 0, c0 + st + 1, st + 1 < nst);
+        fence();
+      });
+    } else unrolled<MF>([&](auto m) {
       unrolled<4>([&](auto n) {
         acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[n].value(), fa[m].value(), acc[m][n], 0, 0,
                                                                     GLU ? n / 2 : 0, (int)sb, m & 3, (int)sa.w[m / 4]);
@@ -684,14 +692,15 @@ __device__ __forceinline__ void single_loop(int nst, int c0, uint32_t lds0, uint
 }
 
 template <int BM, int BN, int NW, int NS, int EPI>
-__global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2)) void fp8_rows_kernel(Fp8Params p) {
+__global__ __launch_bounds__(NW * 64, NS > 1 ? 1 : (BM * BN <= 128 * 128 && EPI != F8_GLU_EXACT ? 3 : 2))
+void fp8_rows_kernel(Fp8Params p) {
   extern __shared__ __align__(128) char smem[];
   using G = Grid8<BM, BN, NW>;
   using L = Lds8<BM, BN, NW, NS>;
   constexpr int MF = G::MF, NF = G::NF;
   constexpr int NT = NW * 64;
   constexpr bool PIPE = BM == 256 && BN == 256 && NW == 8 && NS == 2;
-  static_assert(EPI != F8_GLU || BN == 256, "one block of 128 pairs a tile");
+  static_assert(!is_glu(EPI) || BN == 256, "one block of 128 pairs a tile");
 
   RowsTile tile;
   if (!decode_rows_wave<BM>(p, tile)) return;  // uniform per workgroup
@@ -732,7 +741,7 @@ __global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2
     const int rl = lb.row_of(q);
     int n;
     bool ok;
-    if constexpr (EPI == F8_GLU) {  // 64-row pair blocks [up 32 | gate 32] of the tile's 128 pairs
+    if constexpr (is_glu(EPI)) {  // 64-row pair blocks [up 32 | gate 32] of the tile's 128 pairs
       const int jj = nt * kBlk + (rl >> 6) * 32 + (rl & 31);
       ok = jj < p.half;
       n = (rl & 32) ? p.half + jj : jj;
@@ -774,7 +783,7 @@ __global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2
   const uint32_t a_frag = (uint32_t)(gm * G::WM * kBlk) + frag_off;
   const uint32_t b_frag = (uint32_t)((BM + gn * 64) * kBlk) + frag_off;
   const uint32_t as_lane = lds0 + L::a_scales + (uint32_t)((gm * 16 + r16) * MF);
-  const uint32_t bs_lane = lds0 + L::b_scales + (EPI == F8_GLU ? 0u : (uint32_t)(gn / 2));
+  const uint32_t bs_lane = lds0 + L::b_scales + (is_glu(EPI) ? 0u : (uint32_t)(gn / 2));
   for (int c0 = 0; c0 < p.nk; c0 += kScaleStages) {
     const int nst = p.nk - c0 < kScaleStages ? p.nk - c0 : kScaleStages;
     const int nd = (nst + 3) / 4;
@@ -788,8 +797,8 @@ __global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2
       if (spart + TPR * j < nd)
         sw[j] = *reinterpret_cast<const uint32_t*>(as_base + (int64_t)scales_row * p.a_pitch + c0 + 4 * (spart + TPR * j));
     if (tid < 2 * nst) {
-      const int64_t nb = EPI == F8_GLU ? (tid & 1 ? blocks_of(p.half) : 0) + nt : (int64_t)nt * (BN / kBlk) + (tid & 1);
-      const int64_t last = EPI == F8_GLU ? 2 * blocks_of(p.half) - 1 : blocks_of(p.N) - 1;
+      const int64_t nb = is_glu(EPI) ? (tid & 1 ? blocks_of(p.half) : 0) + nt : (int64_t)nt * (BN / kBlk) + (tid & 1);
+      const int64_t last = is_glu(EPI) ? 2 * blocks_of(p.half) - 1 : blocks_of(p.N) - 1;
       bsw = p.bs[(int64_t)e * p.bs_estride + (nb < last ? nb : last) * p.bs_pitch + c0 + (tid >> 1)];
     }
     if (c0 == 0) dst_row = row_no(p.c_rows, srow);
@@ -820,9 +829,9 @@ __global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2
         asm volatile("ds_write_b32 %0, %1" ::"v"(lds0 + L::dst + 4u * (uint32_t)tid), "v"(dst_row) : "memory");
     };
     if constexpr (NS == 1) {
-      single_loop<EPI == F8_GLU, BM, LPS, MF>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
+      single_loop<EPI, BM, LPS, MF>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
     } else if constexpr (PIPE) {
-      piped_loop<EPI == F8_GLU, BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
+      piped_loop<is_glu(EPI), BM, L::kStage, LPS>(nst, c0, lds0, a_frag, b_frag, as_lane, bs_lane, acc, dma, fill);
     } else {
 #pragma unroll
       for (int i = 1; i < NS - 1; ++i) issue(i, c0 + i, i < nst);
@@ -838,7 +847,7 @@ __global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2
         AScale<MF> sa;
         uint32_t sb;
         sa.read(as_lane + (uint32_t)(st * BM));
-        if constexpr (EPI == F8_GLU) asm volatile("ds_read_u16 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
+        if constexpr (is_glu(EPI)) asm volatile("ds_read_u16 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
         else asm volatile("ds_read_u8 %0, %1" : "=v"(sb) : "v"(bs_lane + 2u * (uint32_t)st));
         Frag8 fb[NF];
         unrolled<NF>([&](auto n) {
@@ -870,13 +879,13 @@ __global__ __launch_bounds__(NW * 64, (NS > 1 ? 1 : BM * BN <= 128 * 128 ? 3 : 2
 #pragma unroll
           for (int m = 0; m < HF; ++m) fa[s & 1][m].tie();
           __builtin_amdgcn_sched_barrier(0);
-          if constexpr (EPI == F8_GLU && BM == kExactRows) {
-            mma_exact<MF>(acc, fa[0], fb, sa, sb);
+          if constexpr (EPI == F8_GLU_EXACT) {
+            mma_exact<MF>(acc, fa[0], fb, sa, sb, [](auto) {});
           } else unrolled<HF>([&](auto m) {
             unrolled<NF>([&](auto n) {
               constexpr int f = s * HF + m;
               acc[f][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                  fb[n].value(), fa[s & 1][m].value(), acc[f][n], 0, 0, EPI == F8_GLU ? n / 2 : 0, (int)sb, f & 3,
+                  fb[n].value(), fa[s & 1][m].value(), acc[f][n], 0, 0, is_glu(EPI) ? n / 2 : 0, (int)sb, f & 3,
                   (int)sa.w[f / 4]);
             });
           });
@@ -1254,7 +1263,7 @@ int launch8(Fp8Params p, int64_t R, hipStream_t s) {
   constexpr int lds = Lds8<BM, BN, NW, NS>::total;
   int rc = prepare(kern, lds);
   if (rc) return rc;
-  p.n_tiles = (int)(EPI == F8_GLU ? blocks_of(p.half) : cdiv(p.N, BN));
+  p.n_tiles = (int)(is_glu(EPI) ? blocks_of(p.half) : cdiv(p.N, BN));
   const int64_t mt = row_tiles(p, R, BM);
   const int64_t total = cdiv(mt * p.n_tiles, (int64_t)kXcds * kSlab) * kXcds * kSlab;  // either tile mapping
   ZMOE_REQUIRE(mt * p.n_tiles < (int64_t)0x7fffff00, ZMOE_ERR_SHAPE, "fp8 product: too many tiles");
@@ -1280,6 +1289,8 @@ int launch_few(const Fp8Params& p, hipStream_t s) {
 //  - Experts of some tens of rows stream their weights: 64 x 256, three workgroups a CU. 128 experts of 2048 -> 2 x 768
 //    (GLU) and back: 4 rows each 73 (76.6 with 32 x 256, 87 with 128 x 256) and 34.4 (38.6 with 64 x 128, 39.6); 32 each 79
 //    (98, 94) and 37.3 (41.5, 42.3); 64 each 88 and 92.6, back 44.3 and 44.5; 126 each 109 and 119, back 70 and 66.
+//    Of exact sums (two workgroups a CU): 4 rows each 79.5 with 32 x 256 and 82.3 with 64 x 256, 12 each 83 and 88.6,
+//    21 each 95 and 84.
 //  - Else 128 x 256, two workgroups a CU (one's prologue and epilogue run under the other's loop), or 256 x 256 for experts
 //    of six or more such tiles, whose last one, half empty on average, then costs less than a tenth. 8192 x 7168 -> 4096:
 //    189 and 175; 262144 rows over 128 experts, 2048 -> 2 x 768 (GLU): 815 and 797; 65536 rows over 128 experts: 244
@@ -1288,10 +1299,12 @@ int launch_few(const Fp8Params& p, hipStream_t s) {
 template <int EPI>
 int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
   const int64_t per = R / p.E;
-  const int n = EPI == F8_GLU ? 2 * p.half : p.N;
+  const int n = is_glu(EPI) ? 2 * p.half : p.N;
   const auto fits = [&](int bm, int bn, int per_cu) { return row_tiles(p, R, bm) * cdiv(n, bn) <= per_cu * kCus; };
-  if constexpr (EPI == F8_GLU) {
-    if (fits(32, 256, 1) || R * p.half <= kExactValues) return launch8<kExactRows, 256, 4, 4, EPI>(p, R, s);
+  if constexpr (is_glu(EPI)) {
+    const bool exact = R * p.half <= kExactValues;
+    if (fits(32, 256, 1) || (exact && per <= 16)) return launch8<32, 256, 4, 4, F8_GLU_EXACT>(p, R, s);
+    if (exact) return launch8<64, 256, 4, 1, F8_GLU_EXACT>(p, R, s);
     if (per <= 128 || fits(64, 256, 3)) return launch8<64, 256, 4, 1, EPI>(p, R, s);
   } else {
     if constexpr (EPI != F8_HALF) {

@@ -90,6 +90,7 @@ def test_swiglu_grouped(T, d, f, E, k, skew, hip_device):
 
 @pytest.mark.parametrize("T,d,f,E,k", [(600, 300, 1700, 1, 1), (1100, 256, 2000, 1, 1), (1500, 200, 3000, 1, 1),
                                        (1500, 4100, 3000, 1, 1), (1000, 8300, 4300, 1, 1), (1500, 200, 4300, 1, 1),
+                                       (700, 8300, 1700, 1, 1), (500, 260, 1300, 16, 4),
                                        (1500, 8300, 4300, 1, 1), (2000, 300, 520, 16, 2), (6000, 260, 520, 16, 2),
                                        (5000, 4100, 1200, 3, 1)])
 def test_swiglu_tiles(T, d, f, E, k, hip_device):
@@ -356,6 +357,30 @@ def test_few_rows_of_narrow_experts_are_exact_before_the_rounding(T, hip_device)
                 a = O.quantize_rows((g * torch.sigmoid(g) * u).unsqueeze(0))[0]
                 ref[t] += p[t, j].double() * (a @ w2[e].T)[0]
         assert float((out.double() - ref).norm() / ref.norm()) <= 2.0 ** -9
+
+
+@pytest.mark.parametrize("T,d,f,E,k", [(1500, 512, 160, 32, 2), (300, 1000, 512, 16, 4), (1300, 512, 1500, 1, 1)])
+def test_exact_sums_do_not_depend_on_the_tile(T, d, f, E, k, hip_device):
+    """Rows of a launch on 64-row tiles are those of launches of their own on 32-row ones, bit for bit."""
+    from zmoe import ops
+
+    x, W1 = activations(T, d, BF, T, hip_device), weight((2 * E, f, d), 1, BF, hip_device)
+    idx = random_topk(T, E, k, 1).to(hip_device) if E > 1 else torch.zeros(T, 1, dtype=torch.int64, device=hip_device)
+    w = ops.fp8_quantize_weight(W1)
+
+    def run(rows):
+        _, ss, off, _ = ops.flatten_sort_count(idx[rows], E)
+        aq, as_ = ops.fp8_glu_w1_forward(*ops.fp8_quantize_rows(x[rows]), *w, d, ss, off, k)
+        out = torch.empty_like(aq.view(torch.uint8)), torch.empty_like(as_[:, :-(-f // 128)])
+        out[0][ss], out[1][ss] = aq.view(torch.uint8), as_[:, :-(-f // 128)]
+        return out
+
+    q, s = run(torch.arange(T, device=hip_device))
+    for rows in (some(T, 7, 1), some(T, 30, 2)):
+        rows = rows.to(hip_device)
+        slots = (rows.unsqueeze(1) * k + torch.arange(k, device=hip_device)).flatten()
+        a, b = run(rows)
+        assert torch.equal(a, q[slots]) and torch.equal(b, s[slots])
 
 
 def test_experts_not_finite_and_twice_the_same(hip_device):
