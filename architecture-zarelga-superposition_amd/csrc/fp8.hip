@@ -109,7 +109,7 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int6
 // ------------------------------------------------------------------ activations
 // Sixteen lanes hold one block of 128 of a row, eight values each: one load of 16 (bf16) or 32 bytes,
 // the largest magnitude by four lane exchanges, 8 bytes written by each lane. Bound by HBM (2 or 4
-// bytes read, 1 written). Optionally row i is X[rows[i] / row_div] times row_scale[rows[i]] (the grouped,
+// bytes read, 1 written): 8192 x 7168 bf16 in 33 us (5.3 TB/s); two or four blocks a thread are 6-20% slower. Optionally row i is X[rows[i] / row_div] times row_scale[rows[i]] (the grouped,
 // routing-weighted rows of an output gradient, never written anywhere in 16 bits).
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ X, int64_t ldx, int64_t x_rows,
