@@ -109,8 +109,9 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c, int6
 // ------------------------------------------------------------------ activations
 // Sixteen lanes hold one block of 128 of a row, eight values each: one load of 16 (bf16) or 32 bytes,
 // the largest magnitude by four lane exchanges, 8 bytes written by each lane. Bound by HBM (2 or 4
-// bytes read, 1 written): 8192 x 7168 bf16 in 33 us (5.3 TB/s); two or four blocks a thread are 6-20% slower. Optionally row i is X[rows[i] / row_div] times row_scale[rows[i]] (the grouped,
-// routing-weighted rows of an output gradient, never written anywhere in 16 bits).
+// bytes read, 1 written): 8192 x 7168 bf16 in 33 us (5.3 TB/s); two or four blocks a thread are 6-20% slower.
+// Optionally row i is X[rows[i] / row_div] times row_scale[rows[i]] (the grouped, routing-weighted rows of an
+// output gradient, never written anywhere in 16 bits).
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ X, int64_t ldx, int64_t x_rows,
                                                             const int64_t* __restrict__ rows, int row_div,
@@ -226,8 +227,10 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
         uint32_t x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = c ? w[4 * r + j].y : w[4 * r + j].x;
-        const uint32_t p01 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), q01 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
-        const uint32_t p23 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u), q23 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+        const uint32_t p01 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u);
+        const uint32_t q01 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u);
+        const uint32_t p23 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+        const uint32_t q23 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
         out[0][r] = __builtin_amdgcn_perm(p23, p01, 0x05040100u);
         out[1][r] = __builtin_amdgcn_perm(p23, p01, 0x07060302u);
         out[2][r] = __builtin_amdgcn_perm(q23, q01, 0x05040100u);
@@ -1486,10 +1489,10 @@ extern "C" int zmoe_fp8_linear_few(const void* X, int64_t x_stride, int64_t M, c
                                    int64_t N, int dtype, void* Y, int64_t y_stride, void* stream) {
   int rc = quantize_checks("fp8_linear_few", M, K, dtype);
   if (rc) return rc;
-  ZMOE_REQUIRE(M <= 16 && K % 8 == 0 && N >= 1 && N < (1 << 30) && x_stride >= K && x_stride % (16 / dtype_size(dtype)) == 0 &&
-                   y_stride >= N,
-               ZMOE_ERR_SHAPE, "fp8_linear_few: at most 16 rows in whole 16-byte chunks (M=%lld K=%lld N=%lld)", (long long)M,
-               (long long)K, (long long)N);
+  ZMOE_REQUIRE(M <= 16 && K % 8 == 0 && N >= 1 && N < (1 << 30) && x_stride >= K &&
+                   x_stride % (16 / dtype_size(dtype)) == 0 && y_stride >= N,
+               ZMOE_ERR_SHAPE, "fp8_linear_few: at most 16 rows in whole 16-byte chunks (M=%lld K=%lld N=%lld)",
+               (long long)M, (long long)K, (long long)N);
   if (M == 0) return ZMOE_OK;
   ZMOE_REQUIRE(X && Y, ZMOE_ERR_NULL, "fp8_linear_few: null pointer");
   ZMOE_REQUIRE(aligned16(X) && (reinterpret_cast<uintptr_t>(Y) % dtype_size(dtype)) == 0, ZMOE_ERR_ALIGN,
