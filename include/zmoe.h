@@ -484,7 +484,9 @@ int zmoe_combine_half(const void* Y, const void* Ys, const float* gates, const v
 /* The first product of SwiGLU experts with the activation and its quantisation: for sorted row i
  *   A[i, j] = silu(g) u, u = X[sorted_scattered_idxs[i] / k] W1_e[j], g = that times W1_e[f + j]  (f32)
  * and Aq [R, fp], As [R, pitch(f)] its quantised rows. W1q, W1s: the quantised [2E, f, d] view of W1 [E, 2f, d], so
- * that no block holds rows of both halves. Without expert_offsets: E = k = 1, rows in order. */
+ * that no block holds rows of both halves. Without expert_offsets: E = k = 1, rows in order. Up to T k f = 2^21 the
+ * products' terms are added at f32's precision, so that the rounding of A to e4m3 is its only one that shows; past
+ * that the scaled matrix instruction adds them (terms cut at 2^-13 of the largest of 8 neighbouring depths). */
 int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T, const void* W1q, const void* W1s,
                             const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t d, int64_t f,
                             int E, int k, void* Aq, void* As, void* stream);
