@@ -514,7 +514,7 @@ __global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide
     for (int u = 0; u < kVN; ++u)
       if (c + u < a.d) p[c + u] = fresh ? v[u] : p[c + u] + v[u];
   };
-  for (int64_t i = blockIdx.x; i < a.n; i += P) {  // (a grid of at most n blocks: each has a row)
+  for (int64_t i = blockIdx.x; i < a.n; i += P) {  // (each block has a row, but for the one of a launch without rows)
     float rho1 = 1.f, rho2 = 0.f;
     // y rho1, u, r' and r of a chunk, and its gains
     float y[kVN], uu[kVN], h[kVN], r[kVN], gx[kVN], w1[kVN], w2[kVN], g[kVN], t[kVN];
@@ -586,6 +586,13 @@ __global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide
       store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, c, a.d, h);
     }
     fresh = false;
+  }
+  if (fresh) {  // no rows: sums of nothing
+    const float zero[kVN] = {};
+    for (int64_t c = c0; c < a.d; c += cstep) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) add(part[k], c, zero);
+    }
   }
   block_alpha<M::WPB>(a, acc_alpha, red);
 }

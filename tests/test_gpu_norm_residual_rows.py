@@ -1,0 +1,30 @@
+"""norm_residual where rows are none, by the bounds of test_gpu_norm_residual."""
+
+import pytest
+import torch
+
+from test_gpu_norm_residual import make, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d", [64, 2048, 4100, 8200, 16384])
+def test_no_rows_give_zero_gradients(d, hip_device):
+    """From a workspace full of NaN: what the sums over rows start from is the kernel's to write."""
+    from zmoe import _lib as L
+
+    lib, dev = L.load(), hip_device
+    nbytes = lib.zmoe_norm_residual_backward_workspace_bytes(0, d)
+    ws = torch.full((nbytes // 4,), float("nan"), device=dev)
+    w1, w2, gate = (torch.ones(d, device=dev) for _ in range(3))
+    scale = torch.ones(1, device=dev)
+    dw1, dw2, dg, ds = (torch.full_like(t, float("nan")) for t in (w1, w2, gate, scale))
+    p = lambda t: t.data_ptr()  # noqa: E731
+    L.call("zmoe_norm_residual_backward", None, None, None, d, L.DTYPE_F32, None, d, L.DTYPE_F32, 0, d, p(w1), p(w2),
+           L.DTYPE_F32, p(gate), 1, 0, L.DTYPE_F32, p(scale), 1.0, None, None, None, None, p(dw1), p(dw2), p(dg), p(ds),
+           p(ws), nbytes, torch.cuda.current_stream().cuda_stream)
+    for g in (dw1, dw2, dg, ds):
+        assert (g == 0).all()
+    t = make(0, d, "bf16", "bf16", "channel", True, True, True, dev)
+    r, x, g = run(t)
+    assert r.shape == x.shape == (0, d) and all((g[n] == 0).all() for n in ("w_post", "w_next", "gate", "scale"))
