@@ -736,6 +736,22 @@ NormArgs fill(const void* r, int64_t ldr, int r_dtype, const void* y, int64_t ld
   return a;
 }
 
+// The forward's operands of n rows from row `first`; bytes of an element of R and Y.
+NormArgs rows_from(NormArgs a, int64_t first, int64_t n, size_t r_size, size_t y_size) {
+  auto on = [](const void* p, int64_t bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; };
+  auto to = [](void* p, int64_t bytes) { return p ? static_cast<char*>(p) + bytes : nullptr; };
+  a.n = n;
+  a.r = on(a.r, first * a.ldr * (int64_t)r_size);
+  a.y = on(a.y, first * a.ldy * (int64_t)y_size);
+  if (a.gate_kind == GATE_ROW || a.gate_kind == GATE_FULL)
+    a.gate.p = on(a.gate.p, first * (a.gate_kind == GATE_ROW ? 1 : a.ldg) * (a.gate.bf16 ? 2 : 4));
+  a.r_out = to(a.r_out, first * a.d * (int64_t)r_size);
+  a.x = to(a.x, first * a.d * (int64_t)y_size);
+  if (a.rho1) a.rho1 += first;
+  if (a.rho2) a.rho2 += first;
+  return a;
+}
+
 }  // namespace
 }  // namespace zmoe
 
@@ -766,7 +782,11 @@ extern "C" int zmoe_norm_residual(const void* R, int64_t r_stride, int r_dtype, 
       constexpr int W = decltype(w)::value, NQ = decltype(nq)::value;
       auto kern = vec ? norm_residual_kernel<decltype(rt), decltype(yt), W, NQ, true>
                       : norm_residual_kernel<decltype(rt), decltype(yt), W, NQ, false>;
-      hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(n, M::RPB)), dim3(M::THREADS), 0, s, a);
+      constexpr int64_t step = kMaxLaunchThreads / M::THREADS * M::RPB;  // rows of a launch
+      for (int64_t first = 0; first < n; first += step) {
+        const NormArgs part = rows_from(a, first, n - first < step ? n - first : step, sizeof(rt), sizeof(yt));
+        hipLaunchKernelGGL(kern, dim3((unsigned)cdiv(part.n, M::RPB)), dim3(M::THREADS), 0, s, part);
+      }
     });
   });
   return check_launch("norm_residual");

@@ -130,6 +130,9 @@ inline bool dtype_ok(int dt) { return dt == ZMOE_DTYPE_BF16 || dt == ZMOE_DTYPE_
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t align_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+// Threads of a launch along x, at most: their number is taken modulo 2^32, with no error (2^26 + 12 rows of 64 threads
+// each ran as 12).
+constexpr int64_t kMaxLaunchThreads = 0xffffffffLL;
 
 }  // namespace zmoe
 

@@ -28,3 +28,21 @@ def test_no_rows_give_zero_gradients(d, hip_device):
     t = make(0, d, "bf16", "bf16", "channel", True, True, True, dev)
     r, x, g = run(t)
     assert r.shape == x.shape == (0, d) and all((g[n] == 0).all() for n in ("w_post", "w_next", "gate", "scale"))
+
+
+@pytest.mark.parametrize("gate", ["row", "full"])
+def test_rows_past_one_launch(gate, hip_device):
+    """2^26 rows and some of 64 threads each are 2^32 threads: the rows of a call on all of them are those of calls on
+    parts."""
+    from zmoe import ops
+
+    n, d = (1 << 26) + 300, 4
+    g = torch.Generator(device=hip_device).manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=hip_device, dtype=torch.bfloat16)  # noqa: E731
+    r, y, w = rnd(n, d), rnd(n, d), rnd(d)
+    kind = ops.GATE_ROW if gate == "row" else ops.GATE_FULL
+    gt = rnd(n) if gate == "row" else rnd(n, d)
+    whole = ops.norm_residual(r, y, w, w, gt, kind, None, 0.5, 1e-6)
+    for lo, hi in ((0, n // 2), (n // 2, n)):
+        part = ops.norm_residual(r[lo:hi], y[lo:hi], w, w, gt[lo:hi], kind, None, 0.5, 1e-6)
+        assert all(torch.equal(a[lo:hi], b) for a, b in zip(whole, part))
