@@ -1361,15 +1361,22 @@ extern "C" int zmoe_fp8_quantize_rows(const void* X, int64_t x_stride, int64_t x
   const int64_t nb = blocks_of(K);
   ZMOE_REQUIRE(n * nb < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "fp8_quantize_rows: too many blocks");
   const int width = row_width(X, x_stride, dtype_size(dtype));
-  const dim3 grid((unsigned)cdiv(n * nb, 16));
   hipStream_t s = as_stream(stream);
-  uint8_t *q = static_cast<uint8_t*>(Q), *sc = static_cast<uint8_t*>(S);
-  if (dtype == ZMOE_DTYPE_BF16)
-    hipLaunchKernelGGL(quantize_rows_kernel<uint16_t>, grid, dim3(256), 0, s, static_cast<const uint16_t*>(X), x_stride,
-                       x_rows, rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, width, q, sc, scale_pitch(K));
-  else
-    hipLaunchKernelGGL(quantize_rows_kernel<float>, grid, dim3(256), 0, s, static_cast<const float*>(X), x_stride, x_rows,
-                       rows, row_div, row_scale, (uint32_t)(n * nb), K, (int)nb, width, q, sc, scale_pitch(K));
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    const int64_t step = kMaxLaunchThreads / 256 * 16 / nb;  // rows of a launch
+    for (int64_t i = 0; i < n; i += step) {
+      const int64_t m = n - i < step ? n - i : step;
+      // rows in order: X and the scales from row i; listed ones: the list
+      hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)cdiv(m * nb, 16)), dim3(256), 0, s,
+                         static_cast<const T*>(X) + (rows ? 0 : i * x_stride), x_stride, rows ? x_rows : x_rows - i,
+                         rows ? rows + i : nullptr, row_div, row_scale && !rows ? row_scale + i : row_scale,
+                         (uint32_t)(m * nb), K, (int)nb, width, static_cast<uint8_t*>(Q) + i * nb * kBlk,
+                         static_cast<uint8_t*>(S) + i * scale_pitch(K), scale_pitch(K));
+    }
+  };
+  if (dtype == ZMOE_DTYPE_BF16) go(uint16_t{});
+  else go(float{});
   return check_launch("fp8_quantize_rows");
 }
 
