@@ -381,22 +381,22 @@ __global__ __launch_bounds__(Map<W>::THREADS, 2) void norm_residual_backward_ker
         h[u] = fmaf(gc[q][u] * g_row, uu[u], alpha * r[u]);
       }
     };
-    float s[1] = {0.f};
-#pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      float yh[kVN], uu[kVN], r[kVN], h[kVN], gx[kVN];
-      values(q, yh, uu, r, h);
-      cur.gx[q].get(gx);
-#pragma unroll
-      for (int u = 0; u < kVN; ++u) {
-        acc2[q][u] = fmaf(gx[u], rho2 * h[u], acc2[q][u]);
-        s[0] = fmaf(gx[u] * w2[q][u], h[u], s[0]);
-      }
-      if (LDS_SUMS && a.w2.p) add(1, q, acc2[q]);
-      if constexpr (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // (one chunk's values at a time)
-    }
     float coef2 = 0.f;
-    if (a.gx) {
+    if (a.gx) {  // (else r' takes no part in its own grad: 0 times an r' that is not finite is left out too)
+      float s[1] = {0.f};
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        float yh[kVN], uu[kVN], r[kVN], h[kVN], gx[kVN];
+        values(q, yh, uu, r, h);
+        cur.gx[q].get(gx);
+#pragma unroll
+        for (int u = 0; u < kVN; ++u) {
+          acc2[q][u] = fmaf(gx[u], rho2 * h[u], acc2[q][u]);
+          s[0] = fmaf(gx[u] * w2[q][u], h[u], s[0]);
+        }
+        if (LDS_SUMS) add(1, q, acc2[q]);
+        if constexpr (NQ > 1) __builtin_amdgcn_sched_barrier(0);  // (one chunk's values at a time)
+      }
       row_sums<W, 1, M::WPB>(s, red, 0);
       coef2 = rho2 * rho2 * rho2 * s[0] * inv_d;
     }
@@ -412,9 +412,12 @@ __global__ __launch_bounds__(Map<W>::THREADS, 2) void norm_residual_backward_ker
       values(q, yh, uu, r, h[q]);
       cur.gx[q].get(gx);
       cur.gr[q].get(t);
+      if (a.gx) {
+#pragma unroll
+        for (int u = 0; u < kVN; ++u) t[u] = fmaf(-coef2, h[q][u], fmaf(rho2, gx[u] * w2[q][u], t[u]));
+      }
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
-        t[u] = fmaf(-coef2, h[q][u], fmaf(rho2, gx[u] * w2[q][u], t[u]));
         acc_alpha = fmaf(t[u], r[u], acc_alpha);
         uu[u] *= t[u];
         s2[1] += uu[u];
@@ -442,8 +445,10 @@ __global__ __launch_bounds__(Map<W>::THREADS, 2) void norm_residual_backward_ker
       if (live) {
         float yh[kVN];
         cur.y[q].get(yh);
+        if (a.w1.p) {  // (else dy = du)
 #pragma unroll
-        for (int u = 0; u < kVN; ++u) h[q][u] = fmaf(-coef1, yh[u] * rho1, rho1 * h[q][u]);
+          for (int u = 0; u < kVN; ++u) h[q][u] = fmaf(-coef1, yh[u] * rho1, rho1 * h[q][u]);
+        }
         store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, col(q), a.d, h[q]);
       }
       if constexpr (NQ > 1) __builtin_amdgcn_sched_barrier(0);
@@ -545,7 +550,7 @@ __global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide
       float v[kVN];
 #pragma unroll
       for (int u = 0; u < kVN; ++u) {
-        v[u] = gx[u] * (rho2 * h[u]);
+        v[u] = a.gx ? gx[u] * (rho2 * h[u]) : 0.f;  // (no dx: 0, also where r' is not finite)
         s[0] = fmaf(gx[u] * w2[u], h[u], s[0]);
       }
       add(part[1], c, v);
@@ -554,6 +559,7 @@ __global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide
     const float coef2 = a.gx ? rho2 * rho2 * rho2 * s[0] * inv_d : 0.f;
     auto grad = [&](int64_t c) {  // t, the whole grad of r'
       chunk(c);
+      if (!a.gx) return;
 #pragma unroll
       for (int u = 0; u < kVN; ++u) t[u] = fmaf(-coef2, h[u], fmaf(rho2, gx[u] * w2[u], t[u]));
     };
@@ -582,7 +588,10 @@ __global__ __launch_bounds__(Map<kMaxWaves>::THREADS, 4) void norm_residual_wide
     for (int64_t c = c0; c < a.d; c += cstep) {
       grad(c);
 #pragma unroll
-      for (int u = 0; u < kVN; ++u) h[u] = fmaf(-coef1, y[u], rho1 * w1[u] * (g[u] * t[u]));
+      for (int u = 0; u < kVN; ++u) {
+        h[u] = rho1 * w1[u] * (g[u] * t[u]);
+        if (a.w1.p) h[u] = fmaf(-coef1, y[u], h[u]);
+      }
       store_chunk<VEC>(static_cast<Y*>(a.dy) + i * a.d, c, a.d, h);
     }
     fresh = false;

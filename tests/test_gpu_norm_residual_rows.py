@@ -1,9 +1,10 @@
-"""norm_residual where rows are none, by the bounds of test_gpu_norm_residual."""
+"""norm_residual where rows are none, too many for one launch or not finite, by the bounds of test_gpu_norm_residual."""
 
 import pytest
 import torch
 
-from test_gpu_norm_residual import make, run
+from oracle import norm_residual_oracle as O
+from test_gpu_norm_residual import EPS, close, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,34 @@ def test_rows_past_one_launch(gate, hip_device):
     for lo, hi in ((0, n // 2), (n // 2, n)):
         part = ops.norm_residual(r[lo:hi], y[lo:hi], w, w, gt[lo:hi], kind, None, 0.5, 1e-6)
         assert all(torch.equal(a[lo:hi], b) for a, b in zip(whole, part))
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "row", "full"])
+@pytest.mark.parametrize("d", [96, 2048, 7168, 8200])
+def test_residual_not_finite_and_no_grad_through_x(d, gate, hip_device):
+    """Without a next norm, or with x unused, r' takes no part in its own gradient: what is finite by the formula stays
+    finite where the residual is not."""
+    for nxt in (False, True):
+        t = make(5, d, "f32", "bf16", gate, True, nxt, False, hip_device)
+        t["r"][1, 3], t["r"][2, 5], t["r"][3, 7] = float("inf"), -float("inf"), float("nan")
+        _, _, g = run(t, use_dx=False)
+        val, mag = O.backward(t["r"], t["y"], t["w_post"], None, t["gate"], 1.0, EPS, t["dr"], None)
+        for name in ("r", "y", "w_post", "gate"):
+            if name in g:
+                rows = name == "w_post" or (name == "gate" and gate == "channel")
+                close("d " + name, g[name], val[name].reshape(g[name].shape), mag[name].reshape(g[name].shape),
+                      512 + (5 if rows else 0))
+        assert not nxt or (g["w_next"] == 0).all()
+
+
+@pytest.mark.parametrize("d", [96, 2048, 7168, 8200])
+def test_rows_not_finite_without_their_norm(d, hip_device):
+    """The same of y where it has no norm: dy = gate dr'."""
+    for gate in ("none", "channel", "row", "full"):
+        t = make(5, d, "f32", "bf16", gate, False, True, False, hip_device)
+        t["y"][1, 3], t["y"][2, 5] = float("inf"), float("nan")
+        _, _, g = run(t, use_dx=False)
+        val, mag = O.backward(t["r"], t["y"], None, None, t["gate"], 1.0, EPS, t["dr"], None)
+        for name in ("r", "y"):
+            close("d " + name, g[name], val[name], mag[name], 512)
+        assert (g["w_next"] == 0).all()
