@@ -250,6 +250,8 @@ def norm_residual(residual: torch.Tensor, y: torch.Tensor, weight: Optional[torc
         elif gate.shape == (*y.shape[:-1], 1) and d > 1:
             kind, gate = _z.GATE_ROW, gate.reshape(-1)
         else:
+            if gate.shape != y.shape and _needs_graph(gate):
+                gate = gate.float()  # its grad is rounded once, after the sum over what it broadcasts over
             kind, gate = _z.GATE_FULL, gate.expand(y.shape).reshape(-1, d)
     scale, value = None, 1.0
     if isinstance(residual_scale, torch.Tensor):

@@ -1,8 +1,10 @@
-"""norm_residual where rows are none, too many for one launch or not finite, by the bounds of test_gpu_norm_residual."""
+"""norm_residual where rows are none, too many for one launch or not finite, and a gate that broadcasts over them, by the
+bounds of test_gpu_norm_residual."""
 
 import pytest
 import torch
 
+from helpers import gen
 from oracle import norm_residual_oracle as O
 from test_gpu_norm_residual import EPS, close, make, run
 
@@ -78,3 +80,19 @@ def test_rows_not_finite_without_their_norm(d, hip_device):
         for name in ("r", "y"):
             close("d " + name, g[name], val[name], mag[name], 512)
         assert (g["w_next"] == 0).all()
+
+
+def test_gradient_of_a_gate_that_broadcasts(hip_device):
+    """One gate a sequence, bf16: its gradient is rounded once, after the sum over the rows."""
+    from zmoe.functional import norm_residual
+
+    B, S, d = 3, 50, 264
+    t = make(B * S, d, "bf16", "bf16", "none", True, True, False, hip_device)
+    gate = torch.randn(B, 1, d, generator=gen(9)).to(torch.bfloat16).to(hip_device).requires_grad_(True)
+    r, x = norm_residual(t["r"].view(B, S, d), t["y"].view(B, S, d), t["w_post"], t["w_next"], gate, None, EPS)
+    torch.autograd.backward([r, x], [t["dr"].view(B, S, d), t["dx"].view(B, S, d)])
+    full = gate.detach().expand(B, S, d).reshape(-1, d)
+    val, mag = O.backward(t["r"], t["y"], t["w_post"], t["w_next"], full, 1.0, EPS, t["dr"], t["dx"])
+    fold = lambda v: v.view(B, S, d).sum(1, keepdim=True)  # noqa: E731
+    assert gate.grad.dtype == gate.dtype
+    close("d gate", gate.grad, fold(val["gate"]), fold(mag["gate"]), 512 + S)
