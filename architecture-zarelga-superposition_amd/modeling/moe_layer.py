@@ -281,7 +281,7 @@ class Fp8MoELayer(Fp8Module):
 
     def forward(self, hidden_states, unpad_indices=None, norm=None):
         bsz, seq_len, h = hidden_states.shape
-        x = self._serve(hidden_states).reshape(bsz * seq_len, h)
+        x = self._serve(hidden_states, self.gate.weight, None if norm is None else norm.weight).reshape(bsz * seq_len, h)
         with torch.no_grad():
             if norm is not None:
                 x = _zf.rmsnorm_rows(hidden_states.reshape(bsz * seq_len, h), norm.weight, norm.eps,

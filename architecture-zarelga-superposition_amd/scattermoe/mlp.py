@@ -16,6 +16,8 @@ ParallelLinear). ``fused=False`` runs that composition through ParallelExperts.
 
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 from torch import nn
 
@@ -205,9 +207,9 @@ class Fp8Module(nn.Module):
             out += [getattr(self, n + "_values").view(torch.float8_e4m3fn), getattr(self, n + "_scales")]
         return out
 
-    def _serve(self, x: torch.Tensor) -> torch.Tensor:
-        """x in the compute dtype; refused where its gradient would be asked for."""
-        if torch.is_grad_enabled() and x.requires_grad:
+    def _serve(self, x: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.Tensor:
+        """x in the compute dtype; refused where its gradient, or that of another operand, would be asked for."""
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, *others)):
             raise RuntimeError(f"{type(self).__name__} serves only: it has no gradients (run it under torch.no_grad())")
         return x.to(_compute_dtype(x))
 
@@ -234,7 +236,7 @@ class Fp8GLUMLP(Fp8Module):
 
     def forward(self, x: torch.Tensor, expert_p: torch.Tensor, expert_idxs: torch.Tensor, residual=None, pad=None):
         x_shape = x.size()
-        x = self._serve(x).reshape(-1, x_shape[-1])
+        x = self._serve(x, expert_p, residual).reshape(-1, x_shape[-1])
         if x.shape[1] != self.input_size:
             raise ValueError(f"Fp8GLUMLP: rows of {self.input_size}, got {x.shape[1]}")
         with torch.no_grad():
