@@ -1537,7 +1537,7 @@ extern "C" int zmoe_combine_half(const void* Y, const void* Ys, const float* gat
   ZMOE_REQUIRE(Y && Ys && out, ZMOE_ERR_NULL, "combine_half: null pointer");
   ZMOE_REQUIRE(aligned16(Y), ZMOE_ERR_ALIGN, "combine_half: Y on 16 bytes");
   const int64_t chunks = cdiv(N, 8), pitch = cdiv(N, kHalfCols), blocks = cdiv(T * chunks, 256);
-  ZMOE_REQUIRE(blocks < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "combine_half: too many elements");
+  ZMOE_REQUIRE(launch_fits(blocks, 256), ZMOE_ERR_SHAPE, "combine_half: too many elements");
   const int vec = aligned16(out) && aligned16(addend) && N % (16 / dtype_size(dtype)) == 0;
   auto go = [&](auto tt, auto kf) {
     using TT = decltype(tt);

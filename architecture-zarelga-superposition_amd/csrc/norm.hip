@@ -276,6 +276,8 @@ template <typename T, typename TW>
 int launch_norm_fwd(const void* X, int64_t ldx, int64_t x_rows, const int64_t* rows, int64_t n, int64_t d,
                     const void* w, float eps, void* Y, float* rstd, hipStream_t s) {
   const NormMap m = norm_map(d / (16 / (int64_t)sizeof(T)));
+  ZMOE_REQUIRE(launch_fits(cdiv(n, m.rpb()), kNormThreads), ZMOE_ERR_SHAPE,
+               "rmsnorm_rows: too many rows for one launch (%lld)", (long long)n);
   with_norm_map(m, [&](auto wpr, auto nq) {
     hipLaunchKernelGGL((rmsnorm_rows_kernel<T, TW, wpr(), nq()>), dim3((unsigned)cdiv(n, m.rpb())),
                        dim3(kNormThreads), 0, s, static_cast<const T*>(X), ldx, x_rows, rows, n, d,

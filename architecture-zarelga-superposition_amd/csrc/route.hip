@@ -462,6 +462,7 @@ extern "C" int zmoe_route_topk_backward(const float* d_weight, const float* topk
                (long long)ld_d_logits, E);
   if (T == 0) return ZMOE_OK;
   ZMOE_REQUIRE(d_weight && topk_prob && topk_idx && d_logits, ZMOE_ERR_NULL, "route_topk_backward: null pointer");
+  ZMOE_REQUIRE(launch_fits(cdiv(T, 4), 256), ZMOE_ERR_SHAPE, "route_topk_backward: too many tokens for one launch");
   const dim3 grid((unsigned)cdiv(T, 4)), block(256);
   if (d_logits_dtype == ZMOE_DTYPE_BF16)
     hipLaunchKernelGGL(route_topk_backward_kernel<uint16_t>, grid, block, 0, as_stream(stream), d_weight,

@@ -468,6 +468,7 @@ extern "C" int zmoe_group(const void* A, int64_t lda, int64_t K, int dtype, cons
                (long long)K, vec_of(dtype));
   const int64_t nch = K / vec_of(dtype);
   const RowMap m = row_map(nch);
+  ZMOE_REQUIRE(launch_fits(cdiv(N, m.rpb), kRowThreads), ZMOE_ERR_SHAPE, "group: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(N, m.rpb)), block(kRowThreads);
   hipStream_t s = as_stream(stream);
 #define ZMOE_GROUP_LAUNCH(T, CT)                                                                                  \
@@ -496,6 +497,7 @@ int combine_impl(const void* Y, const float* gates, const void* addend, int64_t 
                    rows_aligned(dtype, addend, d),
                ZMOE_ERR_ALIGN, "combine: d must be a multiple of %d, pointers 16-byte aligned", vec_of(dtype));
   const RowMap m = row_map(d / vec_of(dtype));
+  ZMOE_REQUIRE(launch_fits(cdiv(T, m.rpb), kRowThreads), ZMOE_ERR_SHAPE, "combine: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(T, m.rpb)), block(kRowThreads);
   auto launch = [&](auto kf, auto tt) {
     using TT = decltype(tt);
@@ -529,6 +531,7 @@ int combine_backward_impl(const void* Y, const void* grad_out, const int64_t* gr
                ZMOE_ERR_ALIGN, "combine_backward: d must be a multiple of %d, pointers 16-byte aligned",
                vec_of(dtype));
   const RowMap m = row_map(d / vec_of(dtype));
+  ZMOE_REQUIRE(launch_fits(cdiv(T, m.rpb), kRowThreads), ZMOE_ERR_SHAPE, "combine_backward: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(T, m.rpb)), block(kRowThreads);
   auto launch = [&](auto km, auto tt) {
     using TT = decltype(tt);
@@ -596,6 +599,7 @@ extern "C" int zmoe_sum_k(const void* Xe, int64_t T, int k, int64_t d, int dtype
                    rows_aligned(dtype, add0, d) && rows_aligned(dtype, add1, d),
                ZMOE_ERR_ALIGN, "sum_k: d must be a multiple of %d, pointers 16-byte aligned", vec_of(dtype));
   const RowMap m = row_map(d / vec_of(dtype));
+  ZMOE_REQUIRE(launch_fits(cdiv(T, m.rpb), kRowThreads), ZMOE_ERR_SHAPE, "sum_k: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(T, m.rpb)), block(kRowThreads);
   auto launch = [&](auto kf, auto tt, auto to) {
     using TT = decltype(tt);
@@ -622,7 +626,7 @@ extern "C" int zmoe_cast_f32_bf16(const float* src, int64_t n, void* dst, void* 
   ZMOE_REQUIRE(src && dst, ZMOE_ERR_NULL, "cast_f32_bf16: null pointer");
   ZMOE_REQUIRE(aligned16(src) && aligned16(dst), ZMOE_ERR_ALIGN, "cast_f32_bf16: pointers must be 16-byte aligned");
   const int64_t blocks = cdiv(n / 8 > 0 ? n / 8 : 1, 256);
-  ZMOE_REQUIRE(blocks < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "cast_f32_bf16: n too large");
+  ZMOE_REQUIRE(launch_fits(blocks, 256), ZMOE_ERR_SHAPE, "cast_f32_bf16: n too large");
   hipLaunchKernelGGL(cast_f32_bf16_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), src, n,
                      (uint16_t*)dst);
   return check_launch("cast_f32_bf16");
@@ -649,7 +653,7 @@ extern "C" int zmoe_cast_f32_bf16_segments(const float* const* src, const int64_
     const int64_t chunks = n[i] / 8 > 0 ? n[i] / 8 : 1;
     ZMOE_REQUIRE(chunks < ((int64_t)1 << 39), ZMOE_ERR_SHAPE, "cast_f32_bf16_segments: n too large");
     blocks += cdiv(chunks, 256);
-    ZMOE_REQUIRE(blocks < (int64_t)0x7fffffff, ZMOE_ERR_SHAPE, "cast_f32_bf16_segments: n too large");
+    ZMOE_REQUIRE(launch_fits(blocks, 256), ZMOE_ERR_SHAPE, "cast_f32_bf16_segments: n too large");
     ++used;
   }
   if (used == 0) return ZMOE_OK;
@@ -690,6 +694,8 @@ extern "C" int zmoe_rowwise_sum_product(const void* A, int a_dtype, const void* 
   ZMOE_REQUIRE(T >= 0 && F >= 0 && H >= 0, ZMOE_ERR_SHAPE, "rowwise_sum_product: bad sizes");
   if (T == 0 || F == 0) return ZMOE_OK;
   ZMOE_REQUIRE(A && B && out, ZMOE_ERR_NULL, "rowwise_sum_product: null pointer");
+  ZMOE_REQUIRE(T <= kMaxLaunchThreads / F && launch_fits(cdiv(T * F, kRowThreads / 64), kRowThreads), ZMOE_ERR_SHAPE,
+               "rowwise_sum_product: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(T * F, kRowThreads / 64)), block(kRowThreads);
   hipStream_t s = as_stream(stream);
 #define ZMOE_RW(TA, TB, TO) \
@@ -714,6 +720,7 @@ extern "C" int zmoe_swiglu(const void* H, int64_t R, int64_t f, int dtype, void*
   ZMOE_REQUIRE(f % vec_of(dtype) == 0 && aligned16(H) && aligned16(A), ZMOE_ERR_ALIGN,
                "swiglu: f must be a multiple of %d", vec_of(dtype));
   const int64_t n = R * (f / vec_of(dtype));
+  ZMOE_REQUIRE(launch_fits(cdiv(n, kRowThreads), kRowThreads), ZMOE_ERR_SHAPE, "swiglu: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(n, kRowThreads)), block(kRowThreads);
   if (dtype == ZMOE_DTYPE_BF16)
     hipLaunchKernelGGL(swiglu_kernel<uint16_t>, grid, block, 0, as_stream(stream), (const uint16_t*)H, R, f,
@@ -733,6 +740,8 @@ extern "C" int zmoe_swiglu_backward_gates(const void* dA, const void* H, int64_t
                "swiglu_backward_gates: null pointer");
   ZMOE_REQUIRE(f % vec_of(dtype) == 0 && aligned16(H) && aligned16(dA) && aligned16(dH), ZMOE_ERR_ALIGN,
                "swiglu_backward_gates: f must be a multiple of %d", vec_of(dtype));
+  ZMOE_REQUIRE(launch_fits(cdiv(R, kRowThreads / 64), kRowThreads), ZMOE_ERR_SHAPE,
+               "swiglu_backward_gates: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(R, kRowThreads / 64)), block(kRowThreads);
   if (dtype == ZMOE_DTYPE_BF16)
     hipLaunchKernelGGL(swiglu_backward_gates_kernel<uint16_t>, grid, block, 0, as_stream(stream),
@@ -753,6 +762,8 @@ extern "C" int zmoe_swiglu_backward(const void* dA, const void* H, int64_t R, in
                    aligned16(dH),
                ZMOE_ERR_ALIGN, "swiglu_backward: f and the dH row stride must be multiples of %d", vec_of(dtype));
   const int64_t n = R * (f / vec_of(dtype));
+  ZMOE_REQUIRE(launch_fits(cdiv(n, kRowThreads), kRowThreads), ZMOE_ERR_SHAPE,
+               "swiglu_backward: too many rows for one launch");
   const dim3 grid((unsigned)cdiv(n, kRowThreads)), block(kRowThreads);
   if (dtype == ZMOE_DTYPE_BF16)
     hipLaunchKernelGGL(swiglu_backward_kernel<uint16_t>, grid, block, 0, as_stream(stream), (const uint16_t*)dA,

@@ -133,6 +133,7 @@ inline int64_t align_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 // Threads of a launch along x, at most: their number is taken modulo 2^32, with no error (2^26 + 12 rows of 64 threads
 // each ran as 12).
 constexpr int64_t kMaxLaunchThreads = 0xffffffffLL;
+inline bool launch_fits(int64_t blocks, int threads) { return blocks <= kMaxLaunchThreads / threads; }
 
 }  // namespace zmoe
 
