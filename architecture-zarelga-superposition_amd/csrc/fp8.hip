@@ -262,11 +262,14 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
 enum Fp8Epi { F8_STORE_BF16 = 0, F8_STORE_F32 = 1, F8_GLU = 2, F8_HALF = 3, F8_GLU_EXACT = 4 };
 constexpr bool is_glu(int epi) { return epi == F8_GLU || epi == F8_GLU_EXACT; }
 // F8_GLU_EXACT: the SwiGLU's sums are rounded to e4m3 next, where an error of a few 2^-13 (a scaled MFMA's, of its largest
-// terms) turns one value in some thousand to its neighbour, 2^-3 away: little in the mean over many rows (0.0023 from
-// the exact result where bf16's own rounding is 0.0017), but up to 0.018 for a single row of a narrow expert. Launches of
-// few activations, which the weights' stream bounds, therefore take their terms to bf16 (exact) and add in f32: 0.0017. One
-// row in each of 32 experts of 2048 -> 2 x 768: 18.4 -> 20 us; 128 such experts of 4 rows 72 -> 80, of 21 rows 75 -> 84.
-constexpr int64_t kExactValues = 1 << 21;  // activations of a launch up to which the mean does not cover it
+// terms) turns one value in some thousand to its neighbour, up to 2^-3 away: 0.0023 of the result's norm over many rows,
+// where bf16's own rounding is 0.0017, and up to 0.018 of a single row of a narrow expert, whatever the launch's size. Terms
+// taken to bf16 (exact) and added in f32 do not: 0.0017. They run at bf16's matrix rate, so that what they cost is the
+// only reason against them, and that grows with the launch. One row in each of 32 experts of 2048 -> 2 x 768: 18.4 -> 20 us;
+// 128 such experts of 4 rows 72 -> 80, of 21 rows 75 -> 84, of 32 rows 79 -> 94, of 128 rows 110 -> 149, of 2048 rows
+// 799 -> 1529; 16384 rows skewed over 64 experts of 7168 -> 2 x 2048 619 -> 1009. Rows are independent: a larger
+// batch called in parts of up to kExactValues has exact sums too.
+constexpr int64_t kExactValues = 1 << 21;  // activations of a launch up to which it adds in f32
 constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 
 struct Fp8Params {
@@ -1298,7 +1301,10 @@ int launch_few(const Fp8Params& p, hipStream_t s) {
 //    of six or more such tiles, whose last one, half empty on average, then costs less than a tenth. 8192 x 7168 -> 4096:
 //    189 and 175; 262144 rows over 128 experts, 2048 -> 2 x 768 (GLU): 815 and 797; 65536 rows over 128 experts: 244
 //    and 263, over 64, 1536 -> 2048: 274 and 281; 16384 rows skewed over 64 experts, 7168 -> 2 x 2048 (GLU): 605 and
-//    668, back 356 and 404.
+//    668, back 356 and 404. The depth moves this little: 2048 rows for each of 64 experts, f16 rows out, 768 -> 2048: 371
+//    and 364, 1536 -> 2048: 544 and 533, 2048 -> 1536: 504 and 487, 7168 -> 1536: 1413 and 1341.
+// Rows per expert are R / E: the host does not know which experts have rows, so skewed routing runs on tiles that are
+// narrower than its large experts would take.
 template <int EPI>
 int dispatch8(const Fp8Params& p, int64_t R, hipStream_t s) {
   const int64_t per = R / p.E;

@@ -5,8 +5,10 @@ power of two, at least 2^-127, for which the block's largest finite magnitude is
 value), q = v / s rounded to e4m3; inf and NaN become NaN. Both scales of a product are applied inside the
 matrix unit; sums are made in its float32 accumulators and rounded once. The unit cuts the terms of 8 neighbouring
 depths off at 2^-13 of the largest of them before it adds them: about 2e-5 of a product's norm for
-normally distributed operands, far below a bfloat16 output's rounding. (Between an expert's two products, where the
-result is rounded to e4m3, launches of up to 2^21 activations add at float32's precision.)
+normally distributed operands, far below a bfloat16 output's rounding. Between an expert's two products the result is
+rounded to e4m3, where this turns one activation in some thousand to its neighbour, up to 2^-3 away. Calls of up to 2^21
+activations (rows times slots times expert width) add in float32 there, which larger ones would pay with up to twice
+the first product's time; a larger batch called in such parts is added in float32 too.
 
 ``quantize_weight`` makes the weight that ``zmoe.functional.fp8_linear`` serves with;
 ``GLUMLP.quantize_fp8``, ``ExpertMLP.quantize_fp8`` and ``MoELayer.quantize_fp8`` make serving modules of
