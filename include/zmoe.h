@@ -458,8 +458,8 @@ int zmoe_fp8_quantize_weight(const void* W, int64_t w_stride_e, int64_t w_stride
 /* zmoe_scatter2scatter on such operands: Y (BF16 or F32, rows y_stride elements apart) rows = X rows times W_e^T, W_e
  * [N, K]; f32 accumulators, one rounding. The scaled matrix instruction cuts the terms of 8 neighbouring depths off at 2^-13
  * of the largest of them: a sum is within 7 2^-13 G + 17 ceil(K / 128) 2^-23 S of the exact one, G the sum over groups of
- * 8 depths of the largest |term|, S that of all |terms|. Without expert_offsets (E = 1, x_grouped and y_grouped): one weight for all M
- * rows. Any K and N. One expert's weights, and gathered X rows, must span less than 2 GiB - 64 KiB. */
+ * 8 depths of the largest |term|, S that of all |terms|. Without expert_offsets (E = 1, x_grouped and y_grouped): one weight
+ * for all M rows. Any K and N. One expert's weights, and gathered X rows, must span less than 2 GiB - 64 KiB. */
 int zmoe_fp8_scatter2scatter(const void* Xq, const void* Xs, int64_t M, const void* Wq, const void* Ws,
                              const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t K,
                              int64_t N, int E, int k, int x_grouped, int y_grouped, int out_dtype, void* Y,
@@ -487,12 +487,13 @@ int zmoe_combine_half(const void* Y, const void* Ys, const float* gates, const v
  *   A[i, j] = silu(g) u, u = X[sorted_scattered_idxs[i] / k] W1_e[j], g = that times W1_e[f + j]  (f32)
  * and Aq [R, fp], As [R, pitch(f)] its quantised rows. W1q, W1s: the quantised [2E, f, d] view of W1 [E, 2f, d], so
  * that no block holds rows of both halves. Without expert_offsets: E = k = 1, rows in order.
- * In every row, an activation held is the e4m3 rounding of a value within D of A, so A's own rounding or, where A is
- * within D of the border between two, its neighbour (at most 2^-3 of it away): D = |silu(g)| eu + 1.1 (|u| + eu) eg + 2^-18 |A|,
- * eu and eg the bounds of the two sums. Up to T k f = 2^21 in a call terms are added in f32, and these are
- * 17 ceil(d / 128) 2^-23 S; past that the scaled matrix instruction adds them, by the bound of zmoe_fp8_scatter2scatter (one
- * activation in some thousand is a neighbour; rows of 160 to 768 activations were off by up to 0.018 of their result, by
- * 0.0015 over many). Rows are independent: calls on parts of up to 2^21 have sums in f32 for any number of rows. */
+ * In every row, an activation held is the e4m3 rounding, at a scale for magnitudes within D of its block's, of a value
+ * within D of A, so A's own rounding or, where A is within D of the border between two, its neighbour:
+ * D = |silu(g)| eu + 1.1 (|u| + eu) eg + 2^-18 |A|, eu and eg the bounds of the two sums. Up to T k f = 2^21 in a call
+ * terms are added in f32, and these are 17 ceil(d / 128) 2^-23 S; past that the scaled matrix instruction adds them, by the
+ * bound of zmoe_fp8_scatter2scatter (one activation in some thousand is a neighbour; single rows of narrow experts were off
+ * by up to 0.018 of their result, rows together by 0.0015). Rows are independent: calls on parts of up to 2^21 have
+ * sums in f32 for any number of rows. */
 int zmoe_fp8_glu_w1_forward(const void* Xq, const void* Xs, int64_t T, const void* W1q, const void* W1s,
                             const int64_t* sorted_scattered_idxs, const int64_t* expert_offsets, int64_t d, int64_t f,
                             int E, int k, void* Aq, void* As, void* stream);

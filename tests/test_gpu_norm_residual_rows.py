@@ -1,12 +1,12 @@
-"""norm_residual where rows are none, too many for one launch or not finite, and a gate that broadcasts over them, by the
-bounds of test_gpu_norm_residual."""
+"""norm_residual where rows are none, many, too many for one launch or not finite, and a gate that broadcasts over them, by
+the bounds of test_gpu_norm_residual."""
 
 import pytest
 import torch
 
 from helpers import gen
 from oracle import norm_residual_oracle as O
-from test_gpu_norm_residual import EPS, close, make, run
+from test_gpu_norm_residual import EPS, check, close, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -96,3 +96,14 @@ def test_gradient_of_a_gate_that_broadcasts(hip_device):
     fold = lambda v: v.view(B, S, d).sum(1, keepdim=True)  # noqa: E731
     assert gate.grad.dtype == gate.dtype
     close("d gate", gate.grad, fold(val["gate"]), fold(mag["gate"]), 512 + S)
+
+
+@pytest.mark.parametrize("n,d", [(2600, 200), (2100, 1024), (1030, 2048), (600, 4096), (520, 7168), (600, 8200), (520, 16384)])
+@pytest.mark.parametrize("gate,post,nxt,use_dr,use_dx", [
+    ("none", True, True, True, True), ("row", True, True, True, True), ("full", True, True, True, True),
+    ("channel", True, False, True, True), ("row", False, True, True, True), ("full", False, True, True, True),
+    ("none", False, True, True, True), ("none", True, True, True, False), ("channel", False, True, True, False),
+    ("row", True, True, False, True)])
+def test_blocks_of_many_rows(n, d, gate, post, nxt, use_dr, use_dx, hip_device):
+    """More rows than the backward has blocks, in every form of a row's sums: one of the two, both, neither."""
+    check(make(n, d, "bf16" if n % 200 else "f32", "bf16", gate, post, nxt, gate != "none", hip_device), use_dr, use_dx)
