@@ -58,4 +58,4 @@ class MoEGate(nn.Module):
         hidden_states = hidden_states.view(-1, h)
         gate_output = _zf.linear(hidden_states, self.weight)                     # moe_gate.py:26
         topk_idx, topk_weight = RouteTopK.apply(gate_output, self.expert_biases, self.top_k)  # :27-34
-        return topk_idx.view(bsz, seq_len, -1), topk_weight.view(bsz, seq_len, -1)
+        return topk_idx.view(bsz, seq_len, self.top_k), topk_weight.view(bsz, seq_len, self.top_k)

@@ -240,7 +240,7 @@ class MoELayer(nn.Module):
             out, topk_idx, offsets = _FusedMoELayer.apply(*ins, _records_graph(ins))
             self.routed_experts.last_expert_offsets = offsets
             if unpad_indices is None:
-                return out.view(bsz, seq_len, h), topk_idx.view(bsz, seq_len, -1)
+                return out.view(bsz, seq_len, h), topk_idx.view(bsz, seq_len, self.gate.top_k)
             return out.view(bsz, seq_len, h), pad_input(topk_idx, unpad_indices, bsz, seq_len)
         if normed is not None:
             x = normed if unpad_indices is None else normed.unsqueeze(0)
@@ -293,5 +293,5 @@ class Fp8MoELayer(Fp8Module):
             out = self.routed_experts(x, topk_weight.squeeze(0), topk_idx.squeeze(0),
                                       residual=self.shared_experts(x), pad=pad).view(bsz, seq_len, h)
             if unpad_indices is None:
-                return out, topk_idx.view(bsz, seq_len, -1)
+                return out, topk_idx.view(bsz, seq_len, self.gate.top_k)
             return out, pad_input(topk_idx.squeeze(0), unpad_indices, bsz, seq_len)
