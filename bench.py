@@ -55,15 +55,15 @@ GEMM_OPS = ("glu_w1_forward", "scatter2scatter", "glu_w2_backward_dh", "group_bw
 # they were measured on (TRAFFIC_C3_GEMM_SHA256, the sha256 of TRAFFIC_C3_SOURCES read
 # one after the other): when those differ, the line reports traffic null and says why.
 TRAFFIC_C3_PROFILE = "profiles/grouped_gemm_c3_hbm_bytes.md"
-TRAFFIC_C3_SOURCES = ("gemm.hip", "zmoe_internal.h")  # what the grouped GEMM kernels compile from
-TRAFFIC_C3_GEMM_SHA256 = "6a8781b83020dd4922df24bfad290a25517cb04d3b21e522fbf2cec7394d72d7"
+TRAFFIC_C3_SOURCES = ("gemm.hip", "zmoe_internal.h", "zmoe_tiles.h")  # what the grouped GEMM kernels compile from
+TRAFFIC_C3_GEMM_SHA256 = "35ada6ba7260b075082785dd80df57c87f935258a42051b03f2f1e1a56b2362d"
 TRAFFIC_C3 = {
-    "glu_w1_forward#0": 6090792544,
-    "scatter2scatter#0": 2875663040,
-    "glu_w2_backward_dh#0": 2496369301,
-    "scatter2scatter#1": 5726834901,
-    "group_bwd_w#0": 2166642133,
-    "group_bwd_w#1": 3670652715,
+    "glu_w1_forward#0": 6050033888,
+    "scatter2scatter#0": 2883434368,
+    "glu_w2_backward_dh#0": 2484112683,
+    "scatter2scatter#1": 5836111552,
+    "group_bwd_w#0": 2171156608,
+    "group_bwd_w#1": 3656640960,
 }
 ROW_OPS = ("route_topk", "flatten_sort_count", "combine", "combine_backward", "combine_backward_scale",
            "swiglu_backward_gates", "sum_k")
