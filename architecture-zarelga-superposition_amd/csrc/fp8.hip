@@ -1068,7 +1068,7 @@ void fp8_rows_kernel(Fp8Params p) {
 // ------------------------------------------------------------------ sums over slots
 // out[t] = add[t] + sum_j g[t, j] Y[t k + j] of F8_HALF rows (g null: 1), one rounding. A thread has eight columns;
 // the k rows' loads (compiled for k up to 8) are all issued before the first is used. Bound by HBM: 32768 x 8 rows of
-// 2048 in 230 us (5.2 TB/s). (Rows left in the products' order and read through the inverse permutation: the product
+// 2048 in 230 us (5.2 TB/s), 261 right behind the product that wrote them. (Rows left in the products' order and read through the inverse permutation: the product
 // 702 -> 670 us, the sum 243, but 60 -> 65 and 277 -> 270 for 16384 x 4: not worth a second form.)
 template <typename T, int KF>
 __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __restrict__ Y, const uint8_t* __restrict__ S,
@@ -1129,7 +1129,7 @@ __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __res
 // At most 32 rows read the weight once and hardly compute: a workgroup takes 16 columns, its eight waves share out
 // the depth, and each wave loads its part of the weight straight into the matrix instruction's registers, up to four
 // blocks of 128 ahead, with no LDS and no barrier before the one sum over the waves (in their order).
-// One row, 2048 -> 1536: 4.1 us, 4096 -> 4096: 4.7, 16384 -> 4096: 13 (5.2 TB/s, the copy rate); 32 rows 5.3, 10.1
+// One row, 2048 -> 1536: 4.3 us, 4096 -> 4096: 5.0, 16384 -> 4096: 13.5 (5.0 TB/s, the copy rate); 32 rows 5.5, 9.6
 // and 30.8. Tiles of 32 x 128 that walk the whole depth: 8.9, 14.4, 48 for one row, 9.1, 14.7, 49 for 32. At 64 rows
 // the two are level (8.0 and 9.1, 16.0 and 15.1, 52 and 49), as every workgroup reads all rows here.
 constexpr int kFewWaves = 8;
@@ -1176,8 +1176,8 @@ struct Raw8 {
 };
 
 // X: uint8_t for quantised rows, or the type of rows (at most 16 of them) that each wave quantises for itself as it goes,
-// in registers: its lanes hold whole blocks. (One bf16 row 2048 -> 1536: 5.4 us, 6.3 with a launch of the quantiser;
-// 16 rows 4096 -> 4096 9.4 and 9.8; one row 16384 -> 4096 24.8 and 16.3, as every workgroup quantises the rows again.)
+// in registers: its lanes hold whole blocks. (One bf16 row 2048 -> 1536: 5.6 us, 6.4 with a launch of the quantiser;
+// 16 rows 4096 -> 4096 9.8 and 9.7, in one call less; one row 16384 -> 4096 24.8 and 16.3, as every workgroup quantises the rows again.)
 template <int MF, int U, int EPI, typename X>
 __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
   constexpr bool RAW = !std::is_same<X, uint8_t>::value;

@@ -1080,8 +1080,8 @@ def norm_residual_backward(dR_out: Optional[torch.Tensor], dX: Optional[torch.Te
 
 
 # Elements of a weight up to which a few rows are quantised in the product's launch: every workgroup quantises its part of
-# them again. One bf16 row, 2048 -> 1536: 5.4 us, in two launches 6.3 (and 14.4 of host time against 8.9); 16 rows
-# 4096 -> 4096 9.4 and 9.8; one row 16384 -> 4096 24.8 and 16.3.
+# them again. One bf16 row, 2048 -> 1536: 5.6 us, in two launches 6.4 (and 14.4 of host time against 8.9); 16 rows
+# 4096 -> 4096 9.8 and 9.7; one row 16384 -> 4096 24.8 and 16.3.
 FP8_FEW_WEIGHTS = 1 << 24
 
 
