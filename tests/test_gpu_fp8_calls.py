@@ -147,3 +147,85 @@ def test_backward_twice_and_recomputed(hip_device):
         again.backward(dout)
         for a, b, v in zip(first, second, leaves):
             assert torch.equal(a, b) and torch.equal(a, v.grad)
+
+
+def test_training_step_captured(hip_device):
+    """SwiGLU experts trained in e4m3, forward and backward in a graph: replays on new inputs and routing, with eager steps
+    between, bit for bit."""
+    from scattermoe.mlp import GLUMLP
+
+    T, d, f, E, k = 50, 136, 100, 6, 2
+    m = GLUMLP(d, f, E, k, fp8=True).to(hip_device).to(BF)
+    names = [n for n, _ in m.named_parameters()]
+    weights = {n: p.detach().clone() for n, p in m.named_parameters()}
+
+    def inputs(seed):
+        return [activations(T, d, BF, seed, hip_device), torch.rand(T, k, generator=gen(seed)).to(hip_device),
+                random_topk(T, E, k, seed).to(hip_device), activations(T, d, BF, seed + 1, hip_device)]
+
+    def step(x, p, idx, dout):
+        leaves = [x.detach().requires_grad_(True), p.detach().requires_grad_(True)]
+        own = {n: w.detach().requires_grad_(True) for n, w in weights.items()}
+        out = torch.func.functional_call(m, own, (leaves[0], leaves[1], idx))
+        return [out.detach(), *torch.autograd.grad(out, leaves + [own[n] for n in names], dout)]
+
+    held = inputs(1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held)
+    for seed in (3, 5, 7):
+        new = inputs(seed)
+        for a, b in zip(held, new):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, step(*new)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("what", ["norm", "experts", "served", "layer"])
+def test_compiled_as_eager(what, hip_device):
+    """Training of norm_residual and of SwiGLU experts in e4m3, and the served modules, compiled in one graph."""
+    from modeling.model_config import ModelConfig
+    from modeling.moe_layer import MoELayer
+    from scattermoe.mlp import GLUMLP
+    from zmoe.functional import norm_residual
+
+    T, d, f, E, k = 24, 128, 64, 8, 2
+    idx, p = random_topk(T, E, k, 1).to(hip_device), torch.rand(T, k, generator=gen(2)).to(hip_device)
+    x = activations(T, d, BF, 3, hip_device)
+    torch._dynamo.reset()
+    if what in ("norm", "experts"):
+        m = GLUMLP(d, f, E, k, fp8=True).to(hip_device).to(BF)
+        w1, w2, g = (weight((d,), i, BF, hip_device).requires_grad_(True) for i in (5, 6, 7))
+        scale = torch.full((1,), 0.9, device=hip_device, requires_grad=True)
+
+        def fn(x, p):
+            if what == "experts":
+                return m(x, p, idx)
+            r, n = norm_residual(x, x * 0.5, w1, w2, g, scale)
+            return r + n
+
+        dout, outs = activations(T, d, BF, 4, hip_device), []
+        for call in (fn, torch.compile(fn, fullgraph=True, backend="aot_eager")):
+            xi, pi = x.clone().requires_grad_(True), p.clone().requires_grad_(True)
+            leaves = [xi, pi, *m.parameters()] if what == "experts" else [xi, w1, w2, g, scale]
+            out = call(xi, pi)
+            outs.append([out.detach(), *torch.autograd.grad(out, leaves, dout)])
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+        return
+    if what == "served":
+        s = GLUMLP(d, f, E, k).to(hip_device).to(BF).quantize_fp8()
+        call = lambda x: s(x, p, idx, residual=x)  # noqa: E731
+    else:
+        layer = MoELayer(ModelConfig(hidden_size=d, intermediate_size=f, n_experts=9, n_shared_experts=1, n_experts_per_token=k))
+        s = layer.to(hip_device).bfloat16().quantize_fp8()
+        s.gate.expert_biases = s.gate.expert_biases.float()
+        call = lambda x: s(x.view(2, T // 2, d))[0]  # noqa: E731
+    with torch.no_grad():
+        assert torch.equal(torch.compile(call, fullgraph=True, backend="aot_eager")(x), call(x))
