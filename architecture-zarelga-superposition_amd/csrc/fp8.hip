@@ -268,7 +268,7 @@ constexpr bool is_glu(int epi) { return epi == F8_GLU || epi == F8_GLU_EXACT; }
 // only reason against them, and that grows with the launch. One row in each of 32 experts of 2048 -> 2 x 768: 18.4 -> 20 us;
 // 128 such experts of 4 rows 72 -> 80, of 21 rows 75 -> 84, of 32 rows 79 -> 94, of 128 rows 110 -> 149, of 2048 rows
 // 799 -> 1529; 16384 rows skewed over 64 experts of 7168 -> 2 x 2048 619 -> 1009. Rows are independent: a larger
-// batch called in parts of up to kExactValues has exact sums too.
+// batch called in parts of up to kExactValues has sums in f32 too.
 constexpr int64_t kExactValues = 1 << 21;  // activations of a launch up to which it adds in f32
 constexpr int kHalfCols = 64;  // columns of one scale: a wave's
 
@@ -1068,8 +1068,9 @@ void fp8_rows_kernel(Fp8Params p) {
 // ------------------------------------------------------------------ sums over slots
 // out[t] = add[t] + sum_j g[t, j] Y[t k + j] of F8_HALF rows (g null: 1), one rounding. A thread has eight columns;
 // the k rows' loads (compiled for k up to 8) are all issued before the first is used. Bound by HBM: 32768 x 8 rows of
-// 2048 in 230 us (5.2 TB/s), 261 right behind the product that wrote them. (Rows left in the products' order and read through the inverse permutation: the product
-// 702 -> 670 us, the sum 243, but 60 -> 65 and 277 -> 270 for 16384 x 4: not worth a second form.)
+// 2048 in 230 us (5.2 TB/s), 261 right behind the product that wrote them. (Rows left in the products' order and read
+// through the inverse permutation: the product 702 -> 670 us, the sum 243, but 60 -> 65 and 277 -> 270 for 16384 x 4:
+// not worth a second form.)
 template <typename T, int KF>
 __global__ __launch_bounds__(256) void combine_half_kernel(const uint16_t* __restrict__ Y, const uint8_t* __restrict__ S,
                                                            int64_t ldy, int64_t pitch, const float* __restrict__ g,
@@ -1177,7 +1178,8 @@ struct Raw8 {
 
 // X: uint8_t for quantised rows, or the type of rows (at most 16 of them) that each wave quantises for itself as it goes,
 // in registers: its lanes hold whole blocks. (One bf16 row 2048 -> 1536: 5.6 us, 6.4 with a launch of the quantiser;
-// 16 rows 4096 -> 4096 9.8 and 9.7, in one call less; one row 16384 -> 4096 24.8 and 16.3, as every workgroup quantises the rows again.)
+// 16 rows 4096 -> 4096 9.8 and 9.7, in one call less; one row 16384 -> 4096 24.8 and 16.3, as every workgroup quantises the
+// rows again.)
 template <int MF, int U, int EPI, typename X>
 __global__ __launch_bounds__(kFewWaves * 64) void fp8_few_kernel(Fp8Params p) {
   constexpr bool RAW = !std::is_same<X, uint8_t>::value;

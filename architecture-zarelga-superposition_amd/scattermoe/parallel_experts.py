@@ -113,8 +113,8 @@ class Fp8ParallelLinear(torch.autograd.Function):
     grad is the product of the quantised grouped output grad (gate-weighted in float32, quantised unrounded) with
     the same weights transposed; the weight and gate grads are ``ParallelLinear``'s, from the unquantised operands
     and from Y. With gates, Y is held in x's dtype (the gates' grad reads it), so slots are rounded before their
-    weighted sum, as there. (x, expert_weights [E, K, N], k, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates,
-    grouped_in, grouped_out, dx); ``dx``: an input grad will be asked for."""
+    weighted sum, as there. (x, expert_weights [E, K, N], k, sorted_expert_idxs, sorted_scattered_idxs,
+    expert_offsets, gates, grouped_in, grouped_out, dx); ``dx``: an input grad will be asked for."""
 
     @staticmethod
     def forward(ctx, x, expert_weights, k: int, sorted_expert_idxs, sorted_scattered_idxs, expert_offsets, gates,
