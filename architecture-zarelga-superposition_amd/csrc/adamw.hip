@@ -1,0 +1,530 @@
+// An AdamW step over many tensors at once (zmoe_adamw), with moments in 32 or in 8 bits, and the grads' global norm with
+// the factor that clips it (zmoe_sum_squares, zmoe_clip_factor).
+//   g' = clip g,  m' = b1 m + (1 - b1) g',  v' = b2 v + (1 - b2) g'^2
+//   p' = p - lr wd p - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+// in f32, p' rounded once to its type. t is each tensor's own count on the device, so a captured step counts on.
+//
+// 8 bits: a block of 256 consecutive elements keeps its largest magnitude A in f32 and for each element the code q of
+//   m = sign q^2 A / 127^2 (signed),   v = q^4 A / 255^4 (unsigned)
+// rounded to f32: codes are spaced evenly in sqrt(|m|) and v^(1/4), so that a moment 10^-4 of the block's largest still has
+// one (16 bits of range under a root, as large as the step of an element with the largest moments; evenly spaced codes would
+// take all below 1 / 254 to 0). A code is the nearest in the root's domain, half-way ones up: that is the comparison of
+// (2q - 1)^2 A with 4 127^2 |m| (and of fourth powers), which double holds exactly (v: to 2^-53), so the same codes come
+// from any evaluation that is right to a few bits. v' > 0 never becomes 0: its root stands under the step. The scale is
+// the magnitude itself, not a power of two, for a moment that decays by 0.1% a step has to be able to. The moments are
+// formed in double and rounded to f32 before the step and the codes are taken from them; a moment that is not
+// finite makes its block's scale so, and all of the block's moments NaN.
+//
+// Everything is one pass over memory: 28 bytes an element (f32, 32 bits), 16 (f32, 8 bits), 22 and 10 (bf16). Tensors'
+// pointers travel in the launches' arguments, so nothing is copied to the device and a graph keeps them.
+#include <type_traits>
+
+#include "zmoe_internal.h"
+
+namespace zmoe {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kBlock = 256;   // elements with one scale
+constexpr int kBlocks = 16;   // of them in a workgroup's chunk: four a wave
+constexpr int kChunk = kBlock * kBlocks;
+constexpr int kTensors = 48;  // in a launch's arguments (under 4 KB)
+constexpr int kNormChunk = 16384;
+constexpr int kNormTensors = 128;
+
+struct Table {
+  zmoe_adamw_tensor t[kTensors];
+  int32_t start[kTensors + 1];  // first chunk of each tensor in this launch
+  uint64_t vec;                 // bit i: tensor i's arrays lie on whole vectors
+  int count;
+};
+
+struct Hyper {
+  double b1, b2;
+  float b1f, b2f, c1f, c2f, eps;  // c = 1 - b
+};
+
+// The tensor that a launch's chunk belongs to.
+__device__ __forceinline__ int owner_of(const int32_t* start, int count, int chunk) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (start[mid] <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// ------------------------------------------------------------------ the step count and what follows from it
+struct StepTable {
+  float* step[kNormTensors];
+  int count;
+};
+
+// coef[i] = {lr / (1 - b1^t), 1 / sqrt(1 - b2^t), lr wd, clip} with t counted on.
+__global__ void adamw_prepare_kernel(const StepTable s, const float* lr_ptr, double lr, double b1, double b2, double wd,
+                                     const float* clip, float4* coef) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= s.count) return;
+  const float t = *s.step[i] + 1.f;
+  *s.step[i] = t;
+  const double rate = lr_ptr ? (double)*lr_ptr : lr;
+  coef[i] = make_float4((float)(rate / (1.0 - pow(b1, (double)t))), (float)(1.0 / sqrt(1.0 - pow(b2, (double)t))),
+                        (float)(rate * wd), clip ? *clip : 1.f);
+}
+
+// ------------------------------------------------------------------ codes
+constexpr int kTop2 = 127, kTop4 = 255;
+constexpr double kDiv2 = 127.0 * 127.0, kDiv4 = 255.0 * 255.0 * 255.0 * 255.0;
+
+// A / div rounded once: the product with the reciprocal, mended by what it leaves.
+__device__ __forceinline__ double unit_of(float A, double div, double inv) {
+  const double q = (double)A * inv;
+  return fma(fma(-q, div, (double)A), inv, q);
+}
+__device__ __forceinline__ double unit2(float A) { return unit_of(A, kDiv2, 1.0 / kDiv2); }
+__device__ __forceinline__ double unit4(float A) { return unit_of(A, kDiv4, 1.0 / kDiv4); }
+// x a + y b, each step rounded: with a fused multiply-add the sum differs in its last bit, and with grads of few bits one
+// value in a thousand lies half-way between two f32 numbers, where that decides.
+__device__ __forceinline__ float blend(double x, double a, double y, double b) {
+#pragma clang fp contract(off)
+  const double xa = x * a, yb = y * b;
+  return (float)(xa + yb);
+}
+
+__device__ __forceinline__ float value2(int q, double unit) {  // q signed, unit = A / 127^2
+  const float v = (float)((double)(q * q) * unit);
+  return q < 0 ? -v : v;
+}
+__device__ __forceinline__ float value4(uint32_t q, double unit) {  // unit = A / 255^4
+  const uint32_t q2 = q * q;
+  return (float)((double)(q2 * q2) * unit);
+}
+
+// inv = 1 / A, 0 for A = 0
+__device__ __forceinline__ int code2(float x, double A, double inv) {
+  const double mag = (double)fabsf(x);
+  int q = (int)(sqrtf((float)(mag * inv)) * 127.f + 0.5f);
+  q = min(max(q, 0), kTop2);
+  const double at = mag * (4.0 * 127.0 * 127.0);
+  const int l = 2 * q - 1, h = 2 * q + 1;
+  q += (int)(q < kTop2 && (double)(h * h) * A <= at && A > 0.0) - (int)(q > 0 && (double)(l * l) * A > at);
+  return x < 0.f ? -q : q;
+}
+__device__ __forceinline__ uint32_t code4(float x, double A, double inv) {
+  const double mag = (double)x;
+  int q = (int)(sqrtf(sqrtf((float)(mag * inv))) * 255.f + 0.5f);
+  q = min(max(q, 0), kTop4);
+  const double at = mag * (16.0 * 255.0 * 255.0 * 255.0 * 255.0);
+  const double l = (double)((2 * q - 1) * (2 * q - 1)), h = (double)((2 * q + 1) * (2 * q + 1));
+  q += (int)(q < kTop4 && h * h * A <= at && A > 0.0) - (int)(q > 0 && l * l * A > at);
+  return q == 0 && x > 0.f ? 1u : (uint32_t)q;
+}
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return v;
+}
+
+// ------------------------------------------------------------------ elements
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float (&v)[4]) {
+  if (vec && i + 3 < n) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + i);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(p + i);
+      v[0] = __uint_as_float(x.x << 16), v[1] = __uint_as_float(x.x & 0xffff0000u);
+      v[2] = __uint_as_float(x.y << 16), v[3] = __uint_as_float(x.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = i + u < n ? to_f32(p[i + u]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float (&v)[4]) {
+  if (vec && i + 3 < n) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>(p + i) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u < n) p[i + u] = from_f32<T>(v[u]);
+  }
+}
+// Four codes as the bytes of a dword.
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int64_t n, bool vec) {
+  if (vec && i + 3 < n) return *reinterpret_cast<const uint32_t*>(p + i);
+  uint32_t c = 0;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (i + u < n) c |= (uint32_t)p[i + u] << (8 * u);
+  return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, int64_t i, int64_t n, bool vec, uint32_t c) {
+  if (vec && i + 3 < n) {
+    *reinterpret_cast<uint32_t*>(p + i) = c;
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u < n) p[i + u] = (uint8_t)(c >> (8 * u));
+  }
+}
+
+template <typename T, bool EIGHT>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const Hyper h,
+                                                         const float4* __restrict__ coef) {
+  const int which = owner_of(tab.start, tab.count, blockIdx.x);
+  const zmoe_adamw_tensor& t = tab.t[which];
+  const bool vec = (tab.vec >> which) & 1;
+  const float4 c = coef[which];
+  T* p = (T*)t.param;
+  const T* g = (const T*)t.grad;
+  const int64_t n = t.n, chunk = blockIdx.x - tab.start[which];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll 2
+  for (int u = 0; u < kBlocks / 4; ++u) {
+    const int64_t b = chunk * kBlocks + wave * (kBlocks / 4) + u, i = b * kBlock + lane * 4;
+    if (b * kBlock >= n) break;
+    float w[4], gr[4], m[4], v[4];
+    load4(p, i, n, vec, w);
+    load4(g, i, n, vec, gr);
+    if constexpr (EIGHT) {
+      const uint32_t cm = load_codes((const uint8_t*)t.exp_avg, i, n, vec);
+      const uint32_t cv = load_codes((const uint8_t*)t.exp_avg_sq, i, n, vec);
+      const double um = unit2(t.scale_avg[b]), uv = unit4(t.scale_sq[b]);
+      uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const double gd = (double)gr[e] * (double)c.w;
+        m[e] = blend(h.b1, (double)value2((int)(int8_t)(cm >> (8 * e)), um), 1.0 - h.b1, gd);
+        v[e] = blend(h.b2, (double)value4((cv >> (8 * e)) & 0xffu, uv), 1.0 - h.b2, gd * gd);
+        if (i + e < n) {  // magnitudes order as their bits, NaN above all
+          top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
+          top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
+        }
+      }
+      const float Am = __uint_as_float(wave_max_bits(top_m)), Av = __uint_as_float(wave_max_bits(top_v));
+      const double Amd = (double)Am, Avd = (double)Av;
+      const double im = Am > 0.f ? 1.0 / Amd : 0.0, iv = Av > 0.f ? 1.0 / Avd : 0.0;
+      uint32_t qm = 0, qv = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        qm |= ((uint32_t)code2(m[e], Amd, im) & 0xffu) << (8 * e);
+        qv |= code4(v[e], Avd, iv) << (8 * e);
+      }
+      store_codes((uint8_t*)t.exp_avg, i, n, vec, qm);
+      store_codes((uint8_t*)t.exp_avg_sq, i, n, vec, qv);
+      if (lane == 0) {
+        t.scale_avg[b] = Am;
+        t.scale_sq[b] = Av;
+      }
+    } else {
+      load4((const float*)t.exp_avg, i, n, vec, m);
+      load4((const float*)t.exp_avg_sq, i, n, vec, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float gs = gr[e] * c.w;
+        m[e] = fmaf(h.b1f, m[e], h.c1f * gs);
+        v[e] = fmaf(h.b2f, v[e], h.c2f * (gs * gs));
+      }
+      store4((float*)t.exp_avg, i, n, vec, m);
+      store4((float*)t.exp_avg_sq, i, n, vec, v);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float d = c.x * m[e] / (sqrtf(v[e]) * c.y + h.eps);
+      w[e] = fmaf(-c.z, w[e], w[e]) - d;
+    }
+    store4(p, i, n, vec, w);
+  }
+}
+
+// ------------------------------------------------------------------ moments in f32 again
+struct MomentTable {
+  zmoe_moment t[kTensors];
+  int32_t start[kTensors + 1];
+  uint64_t vec;
+  int count;
+};
+
+__global__ __launch_bounds__(kThreads) void moments_kernel(const MomentTable tab) {
+  const int which = owner_of(tab.start, tab.count, blockIdx.x);
+  const zmoe_moment& t = tab.t[which];
+  const bool vec = (tab.vec >> which) & 1;
+  const int64_t chunk = blockIdx.x - tab.start[which];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int u = 0; u < kBlocks / 4; ++u) {
+    const int64_t b = chunk * kBlocks + wave * (kBlocks / 4) + u, i = b * kBlock + lane * 4;
+    if (b * kBlock >= t.n) break;
+    const uint32_t q = load_codes((const uint8_t*)t.codes, i, t.n, vec);
+    const double unit = t.second ? unit4(t.scale[b]) : unit2(t.scale[b]);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[e] = t.second ? value4((q >> (8 * e)) & 0xffu, unit) : value2((int)(int8_t)(q >> (8 * e)), unit);
+    store4(t.out, i, t.n, vec, v);
+  }
+}
+
+// ------------------------------------------------------------------ the grads' norm
+struct NormTable {
+  const void* g[kNormTensors];
+  int64_t n[kNormTensors];
+  int32_t start[kNormTensors + 1];
+  int count;
+};
+
+// parts[chunk] = sum g^2 over a chunk, in double: a clip that moved by one f32 rounding would turn codes.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sum_squares_kernel(const NormTable tab, double* __restrict__ parts) {
+  __shared__ double red[kThreads / 64];
+  constexpr int VC = 16 / sizeof(T);
+  const int which = owner_of(tab.start, tab.count, blockIdx.x);
+  const T* g = (const T*)tab.g[which];
+  const int64_t a = (int64_t)(blockIdx.x - tab.start[which]) * kNormChunk;
+  const int64_t b = a + kNormChunk < tab.n[which] ? a + kNormChunk : tab.n[which];
+  double sum = 0.0;
+  int64_t i = a;
+  if ((reinterpret_cast<uintptr_t>(g) & 15u) == 0) {  // (a is a whole number of chunks)
+    i = a + (b - a) / VC * VC;
+#pragma unroll 4
+    for (int64_t j = a + threadIdx.x * VC; j < i; j += kThreads * VC) {
+      float v[VC];
+      unpack_chunk(*reinterpret_cast<const uint4*>(g + j), v, T{});
+#pragma unroll
+      for (int u = 0; u < VC; ++u) sum += (double)v[u] * (double)v[u];
+    }
+  }
+  for (i += threadIdx.x; i < b; i += kThreads) sum += (double)to_f32(g[i]) * (double)to_f32(g[i]);
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) parts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__global__ __launch_bounds__(1024) void clip_factor_kernel(const double* __restrict__ parts, int64_t count,
+                                                           float max_norm, float* __restrict__ out) {
+  __shared__ double red[16];
+  double sum = 0.0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < count; i += 1024) sum += parts[i];
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) sum += red[w];
+    const float norm = (float)sqrt(sum), f = max_norm / (norm + 1e-6f);
+    out[0] = norm;
+    out[1] = f > 1.f ? 1.f : f;  // a norm that is NaN stays so
+  }
+}
+
+bool on(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace
+}  // namespace zmoe
+
+using namespace zmoe;
+
+extern "C" size_t zmoe_sum_squares_workspace_bytes(int64_t n) {
+  return n > 0 && n < (1LL << 40) ? (size_t)cdiv(n, kNormChunk) * 8 : 0;
+}
+
+extern "C" int zmoe_sum_squares(const void* const* tensors, const int64_t* n, int count, int dtype, double* parts,
+                                void* stream) {
+  ZMOE_REQUIRE(dtype_ok(dtype), ZMOE_ERR_DTYPE, "sum_squares: dtype %d", dtype);
+  ZMOE_REQUIRE(count >= 0, ZMOE_ERR_SHAPE, "sum_squares: %d tensors", count);
+  ZMOE_REQUIRE(count == 0 || (tensors && n && parts), ZMOE_ERR_NULL, "sum_squares: null pointer");
+  for (int i = 0; i < count; ++i) {
+    ZMOE_REQUIRE(n[i] >= 0 && n[i] < (1LL << 40), ZMOE_ERR_SHAPE, "sum_squares: tensor %d of %lld elements", i,
+                 (long long)n[i]);
+    ZMOE_REQUIRE(n[i] == 0 || tensors[i], ZMOE_ERR_NULL, "sum_squares: null pointer");
+  }
+  NormTable tab;
+  tab.count = 0;
+  tab.start[0] = 0;
+  int64_t done = 0;
+  auto launch = [&]() {
+    if (tab.count == 0) return (int)ZMOE_OK;
+    const unsigned blocks = (unsigned)tab.start[tab.count];
+    if (dtype == ZMOE_DTYPE_BF16)
+      hipLaunchKernelGGL(sum_squares_kernel<uint16_t>, dim3(blocks), dim3(kThreads), 0, as_stream(stream), tab,
+                         parts + done);
+    else
+      hipLaunchKernelGGL(sum_squares_kernel<float>, dim3(blocks), dim3(kThreads), 0, as_stream(stream), tab,
+                         parts + done);
+    done += blocks;
+    tab.count = 0;
+    return check_launch("sum_squares");
+  };
+  // a launch's chunks: fewer threads than a launch holds (one tensor of more is dealt out over several launches)
+  constexpr int64_t kMost = kMaxLaunchThreads / kThreads / 2;
+  const int size = dtype_size(dtype);
+  for (int i = 0; i < count; ++i) {
+    for (int64_t first = 0, all = cdiv(n[i], kNormChunk); first < all;) {
+      const int64_t room = kMost - tab.start[tab.count];
+      if (room <= 0 || tab.count == kNormTensors) {
+        if (const int rc = launch()) return rc;
+        continue;
+      }
+      const int64_t take = all - first < room ? all - first : room, at = first * kNormChunk;
+      tab.g[tab.count] = (const char*)tensors[i] + at * size;
+      tab.n[tab.count] = n[i] - at < take * kNormChunk ? n[i] - at : take * kNormChunk;
+      tab.start[tab.count + 1] = tab.start[tab.count] + (int32_t)take;
+      ++tab.count;
+      first += take;
+    }
+  }
+  return launch();
+}
+
+extern "C" int zmoe_clip_factor(const double* parts, int64_t count, float max_norm, float* norm_and_factor,
+                                void* stream) {
+  ZMOE_REQUIRE(count >= 0, ZMOE_ERR_SHAPE, "clip_factor: %lld parts", (long long)count);
+  ZMOE_REQUIRE(norm_and_factor && (count == 0 || parts), ZMOE_ERR_NULL, "clip_factor: null pointer");
+  hipLaunchKernelGGL(clip_factor_kernel, dim3(1), dim3(1024), 0, as_stream(stream), parts, count, max_norm,
+                     norm_and_factor);
+  return check_launch("clip_factor");
+}
+
+extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype, int state_bits, const float* lr_ptr,
+                          double lr, double beta1, double beta2, double eps, double weight_decay, const float* clip,
+                          float* workspace, size_t workspace_bytes, void* stream) {
+  ZMOE_REQUIRE(dtype_ok(dtype), ZMOE_ERR_DTYPE, "adamw: dtype %d", dtype);
+  ZMOE_REQUIRE(state_bits == 32 || state_bits == 8, ZMOE_ERR_DTYPE, "adamw: moments in 32 or 8 bits (%d)", state_bits);
+  ZMOE_REQUIRE(count >= 0, ZMOE_ERR_SHAPE, "adamw: %d tensors", count);
+  ZMOE_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, ZMOE_ERR_SHAPE, "adamw: betas %g, %g", beta1,
+               beta2);
+  if (count == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(tensors && workspace, ZMOE_ERR_NULL, "adamw: null pointer");
+  ZMOE_REQUIRE(aligned16(workspace), ZMOE_ERR_ALIGN, "adamw: the workspace must be 16-byte aligned");
+  ZMOE_REQUIRE(workspace_bytes >= (size_t)count * 16, ZMOE_ERR_WORKSPACE, "adamw: workspace %zu < %zu bytes",
+               workspace_bytes, (size_t)count * 16);
+  const int size = dtype_size(dtype);
+  for (int i = 0; i < count; ++i) {
+    const zmoe_adamw_tensor& t = tensors[i];
+    ZMOE_REQUIRE(t.n >= 0 && t.n < (1LL << 40), ZMOE_ERR_SHAPE, "adamw: tensor %d of %lld elements", i, (long long)t.n);
+    ZMOE_REQUIRE(t.step, ZMOE_ERR_NULL, "adamw: null pointer");
+    if (t.n == 0) continue;
+    ZMOE_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq && (state_bits == 32 || (t.scale_avg && t.scale_sq)),
+                 ZMOE_ERR_NULL, "adamw: null pointer");
+    ZMOE_REQUIRE(on(t.param, size) && on(t.grad, size) &&
+                     (state_bits == 8 ? on(t.scale_avg, 4) && on(t.scale_sq, 4) : on(t.exp_avg, 4) && on(t.exp_avg_sq, 4)),
+                 ZMOE_ERR_ALIGN, "adamw: tensor %d is not on whole elements", i);
+  }
+  float4* coef = reinterpret_cast<float4*>(workspace);
+  for (int i = 0; i < count; i += kNormTensors) {
+    StepTable s;
+    s.count = count - i < kNormTensors ? count - i : kNormTensors;
+    for (int j = 0; j < s.count; ++j) s.step[j] = tensors[i + j].step;
+    hipLaunchKernelGGL(adamw_prepare_kernel, dim3(kNormTensors / 64), dim3(64), 0, as_stream(stream), s, lr_ptr, lr, beta1,
+                       beta2, weight_decay, clip, coef + i);
+    if (const int rc = check_launch("adamw")) return rc;
+  }
+  const Hyper h{beta1, beta2, (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)eps};
+  Table tab;
+  tab.count = 0;
+  tab.start[0] = 0;
+  tab.vec = 0;
+  int first_of_launch = 0;
+  auto launch = [&](int next) {
+    const bool any = tab.count > 0 && tab.start[tab.count] > 0;
+    if (any) {
+      auto go = [&](auto type, auto eight) {
+        hipLaunchKernelGGL((adamw_kernel<decltype(type), decltype(eight)::value>), dim3((unsigned)tab.start[tab.count]),
+                           dim3(kThreads), 0, as_stream(stream), tab, h, coef + first_of_launch);
+      };
+      if (dtype == ZMOE_DTYPE_BF16) state_bits == 8 ? go(uint16_t{}, std::true_type{}) : go(uint16_t{}, std::false_type{});
+      else state_bits == 8 ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+    }
+    tab.count = 0;
+    tab.vec = 0;
+    first_of_launch = next;
+    return any ? check_launch("adamw") : (int)ZMOE_OK;
+  };
+  constexpr int64_t kMost = kMaxLaunchThreads / kThreads / 2;
+  const unsigned wide = 4 * size, codes = state_bits == 8 ? 4 : 16;
+  for (int i = 0; i < count; ++i) {
+    const zmoe_adamw_tensor& t = tensors[i];
+    const int64_t all = cdiv(t.n, kChunk);
+    for (int64_t first = 0; first < all || (all == 0 && first == 0);) {
+      const int64_t room = kMost - tab.start[tab.count];
+      if (room <= 0 || tab.count == kTensors) {
+        if (const int rc = launch(i)) return rc;
+        continue;
+      }
+      const int64_t take = all - first < room ? all - first : room, at = first * kChunk;
+      zmoe_adamw_tensor& u = tab.t[tab.count];
+      u = t;
+      u.param = (char*)t.param + at * size;
+      u.grad = (const char*)t.grad + at * size;
+      u.exp_avg = (char*)t.exp_avg + at * (state_bits / 8);
+      u.exp_avg_sq = (char*)t.exp_avg_sq + at * (state_bits / 8);
+      if (state_bits == 8) {
+        u.scale_avg = t.scale_avg + first * kBlocks;
+        u.scale_sq = t.scale_sq + first * kBlocks;
+      }
+      u.n = t.n - at < take * kChunk ? t.n - at : take * kChunk;
+      if (on(t.param, wide) && on(t.grad, wide) && on(t.exp_avg, codes) && on(t.exp_avg_sq, codes))
+        tab.vec |= 1ull << tab.count;
+      tab.start[tab.count + 1] = tab.start[tab.count] + (int32_t)take;
+      ++tab.count;
+      first += take;
+      if (all == 0) break;  // no elements: its place in the table keeps coef's order
+      if (first < all)      // the rest of this tensor opens the next launch, and has its coef there
+        if (const int rc = launch(i)) return rc;
+    }
+  }
+  return launch(count);
+}
+
+extern "C" int zmoe_adamw_moments(const zmoe_moment* moments, int count, void* stream) {
+  ZMOE_REQUIRE(count >= 0, ZMOE_ERR_SHAPE, "adamw_moments: %d tensors", count);
+  ZMOE_REQUIRE(count == 0 || moments, ZMOE_ERR_NULL, "adamw_moments: null pointer");
+  for (int i = 0; i < count; ++i) {
+    const zmoe_moment& t = moments[i];
+    ZMOE_REQUIRE(t.n >= 0 && t.n < (1LL << 40), ZMOE_ERR_SHAPE, "adamw_moments: tensor %d of %lld elements", i,
+                 (long long)t.n);
+    ZMOE_REQUIRE(t.n == 0 || (t.codes && t.scale && t.out), ZMOE_ERR_NULL, "adamw_moments: null pointer");
+    ZMOE_REQUIRE(on(t.scale, 4) && on(t.out, 4), ZMOE_ERR_ALIGN, "adamw_moments: tensor %d is not on whole elements", i);
+  }
+  MomentTable tab;
+  tab.count = 0;
+  tab.start[0] = 0;
+  tab.vec = 0;
+  auto launch = [&]() {
+    if (tab.count == 0) return (int)ZMOE_OK;
+    hipLaunchKernelGGL(moments_kernel, dim3((unsigned)tab.start[tab.count]), dim3(kThreads), 0, as_stream(stream), tab);
+    tab.count = 0;
+    tab.vec = 0;
+    return check_launch("adamw_moments");
+  };
+  constexpr int64_t kMost = kMaxLaunchThreads / kThreads / 2;
+  for (int i = 0; i < count; ++i) {
+    const zmoe_moment& t = moments[i];
+    for (int64_t first = 0, all = cdiv(t.n, kChunk); first < all;) {
+      const int64_t room = kMost - tab.start[tab.count];
+      if (room <= 0 || tab.count == kTensors) {
+        if (const int rc = launch()) return rc;
+        continue;
+      }
+      const int64_t take = all - first < room ? all - first : room, at = first * kChunk;
+      zmoe_moment& u = tab.t[tab.count];
+      u = t;
+      u.codes = (const char*)t.codes + at;
+      u.scale = t.scale + first * kBlocks;
+      u.out = t.out + at;
+      u.n = t.n - at < take * kChunk ? t.n - at : take * kChunk;
+      if (on(t.codes, 4) && on(t.out, 16)) tab.vec |= 1ull << tab.count;
+      tab.start[tab.count + 1] = tab.start[tab.count] + (int32_t)take;
+      ++tab.count;
+      first += take;
+    }
+  }
+  return launch();
+}

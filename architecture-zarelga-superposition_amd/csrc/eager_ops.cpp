@@ -146,6 +146,121 @@ Tensor swiglu_route_backward(const Tensor& dAs, const Tensor& Hs, const Tensor& 
   return op.call(dAs, Hs, dg, p, idx, E);
 }
 
+Tensors route(const Tensor& logits, const Opt& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups,
+              int64_t group_scores, bool renorm, double scale) {
+  if (logits.is_cuda() && known(logits) && logits.dim() == 2 && logits.is_contiguous() && k >= 0 && fits_int(k) &&
+      fits_int(logits.size(1)) && fits_int(score) && fits_int(groups) && fits_int(top_groups) &&
+      fits_int(group_scores) && (!bias || (flat(*bias, logits, at::kFloat) && bias->numel() == logits.size(1)))) {
+    const c10::DeviceGuard guard(logits.device());
+    const int64_t T = logits.size(0);
+    Tensor idx = empty({T, k}, logits, at::kLong), w = empty({T, k}, logits, at::kFloat),
+           p = empty({T, k}, logits, at::kFloat);
+    if (zmoe_route(raw(logits), code(logits), T, (int)logits.size(1), (int)k, (int)score,
+                   bias ? ptr<const float>(*bias) : nullptr, (int)groups, (int)top_groups, (int)group_scores, renorm,
+                   (float)scale, ptr<int64_t>(idx), ptr<float>(w), ptr<float>(p), stream_of(logits)) == ZMOE_OK)
+      return {idx, w, p};
+  }
+  static const auto op = general<Tensors(const Tensor&, const Opt&, c10::SymInt, c10::SymInt, c10::SymInt, c10::SymInt,
+                                         c10::SymInt, bool, double)>("zmoe::route");
+  return op.call(logits, bias, k, score, groups, top_groups, group_scores, renorm, scale);
+}
+
+// route's gradient into out [T, E] (rows `ld` elements apart); false where the general form has to run.
+bool route_form_backward_into(const Tensor& dw, const Tensor& p, const Tensor& idx, const Tensor& logits, int64_t score,
+                              bool renorm, double scale, const Opt& add, void* out, int64_t ld) {
+  if (!logits.is_cuda() || !known(logits) || logits.dim() != 2 || !logits.is_contiguous() || idx.dim() != 2 ||
+      idx.size(0) != logits.size(0) || !flat(idx, logits, at::kLong) || !flat(dw, logits, at::kFloat) ||
+      !flat(p, logits, at::kFloat) || dw.sizes() != idx.sizes() || p.sizes() != idx.sizes() ||
+      !fits_int(logits.size(1)) || !fits_int(idx.size(1)) || !fits_int(score) ||
+      (add && !(apart(*add) && rows2(*add, logits) && add->sizes() == logits.sizes())))
+    return false;
+  const int64_t E = logits.size(1);
+  return zmoe_route_backward(ptr<const float>(dw), ptr<const float>(p), ids(idx), idx.size(0), (int)E, (int)idx.size(1),
+                             (int)score, raw(logits), renorm, (float)scale, add ? raw(*add) : nullptr,
+                             add ? std::max(add->stride(0), E) : 0, out, ld, code(logits), stream_of(logits)) == ZMOE_OK;
+}
+
+Tensor route_backward(const Tensor& dw, const Tensor& p, const Tensor& idx, const Tensor& logits, int64_t score,
+                      bool renorm, double scale) {
+  if (logits.is_cuda() && logits.dim() == 2) {
+    const c10::DeviceGuard guard(logits.device());
+    Tensor out = empty(logits.sizes(), logits);
+    if (route_form_backward_into(dw, p, idx, logits, score, renorm, scale, std::nullopt, raw(out), logits.size(1)))
+      return out;
+  }
+  static const auto op = general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, c10::SymInt, bool,
+                                        double)>("zmoe::route_backward");
+  return op.call(dw, p, idx, logits, score, renorm, scale);
+}
+
+Tensor swiglu_route_form_backward(const Tensor& dAs, const Tensor& Hs, const Tensor& dg, const Tensor& p,
+                                  const Tensor& idx, const Tensor& logits, int64_t score, bool renorm, double scale,
+                                  const Opt& add) {
+  if (Hs.is_cuda() && known(Hs) && Hs.dim() == 2 && Hs.is_contiguous() && flat(dAs, Hs, Hs.scalar_type()) &&
+      dAs.numel() * 2 == Hs.numel() && on(logits, Hs) && logits.scalar_type() == Hs.scalar_type() && logits.dim() == 2 &&
+      logits.size(0) == Hs.size(0)) {
+    const c10::DeviceGuard guard(Hs.device());
+    const int64_t T = Hs.size(0), two_f = Hs.size(1), ld = two_f + logits.size(1);
+    Tensor G = empty({T, ld}, Hs);
+    char* tail = static_cast<char*>(raw(G)) + two_f * G.element_size();
+    if (zmoe_swiglu_backward(raw(dAs), raw(Hs), T, two_f / 2, code(Hs), raw(G), ld, stream_of(Hs)) == ZMOE_OK &&
+        route_form_backward_into(dg, p, idx, logits, score, renorm, scale, add, tail, ld))
+      return G;
+  }
+  static const auto op =
+      general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                     c10::SymInt, bool, double, const Opt&)>("zmoe::swiglu_route_form_backward");
+  return op.call(dAs, Hs, dg, p, idx, logits, score, renorm, scale, add);
+}
+
+// Borders of sequences [S + 1], or none.
+bool borders(const Opt& cu, const Tensor& like) {
+  return !cu || (on(*cu, like) && (cu->scalar_type() == at::kInt || cu->scalar_type() == at::kLong) && cu->dim() == 1 &&
+                 cu->is_contiguous() && cu->numel() >= 2);
+}
+
+Tensors router_losses(const Tensor& logits, const Tensor& idx, const Opt& cu, int64_t score) {
+  if (logits.is_cuda() && known(logits) && logits.dim() == 2 && logits.is_contiguous() && idx.dim() == 2 &&
+      flat(idx, logits, at::kLong) && idx.size(0) == logits.size(0) && borders(cu, logits) &&
+      fits_int(logits.size(1)) && fits_int(idx.size(1)) && fits_int(score)) {
+    const c10::DeviceGuard guard(logits.device());
+    const int64_t T = logits.size(0), E = logits.size(1), S = cu ? cu->numel() - 1 : 1;
+    Tensor losses = empty({2}, logits, at::kFloat), grad = empty({S, E}, logits, at::kFloat),
+           inv = empty({1}, logits, at::kFloat);
+    const size_t bytes = zmoe_router_losses_workspace_bytes(T, (int)E, S);
+    Tensor ws = workspace(bytes, logits);
+    if (zmoe_router_losses(raw(logits), code(logits), T, (int)E, ids(idx), (int)idx.size(1), (int)score,
+                           cu ? raw(*cu) : nullptr, cu && cu->scalar_type() == at::kLong, S, ptr<float>(losses),
+                           ptr<float>(grad), ptr<float>(inv), raw(ws), bytes, stream_of(logits)) == ZMOE_OK)
+      return {losses, grad, inv};
+  }
+  static const auto op =
+      general<Tensors(const Tensor&, const Tensor&, const Opt&, c10::SymInt)>("zmoe::router_losses");
+  return op.call(logits, idx, cu, score);
+}
+
+Tensor router_losses_backward(const Opt& d_balance, const Opt& d_z, const Tensor& logits, const Opt& cu, int64_t score,
+                              const Tensor& grad, const Tensor& inv) {
+  auto one = [&](const Opt& g) { return !g || (flat(*g, logits, at::kFloat) && g->numel() == 1); };
+  if (logits.is_cuda() && known(logits) && logits.dim() == 2 && logits.is_contiguous() && borders(cu, logits) &&
+      one(d_balance) && one(d_z) && flat(grad, logits, at::kFloat) && flat(inv, logits, at::kFloat) &&
+      inv.numel() == 1 && fits_int(logits.size(1)) && fits_int(score)) {
+    const int64_t T = logits.size(0), E = logits.size(1), S = cu ? cu->numel() - 1 : 1;
+    if (grad.dim() == 2 && grad.size(0) == S && grad.size(1) == E) {
+      const c10::DeviceGuard guard(logits.device());
+      Tensor out = empty({T, E}, logits);
+      if (zmoe_router_losses_backward(raw(logits), code(logits), T, (int)E, (int)score, cu ? raw(*cu) : nullptr,
+                                      cu && cu->scalar_type() == at::kLong, S, ptr<const float>(grad),
+                                      ptr<const float>(inv), d_balance ? ptr<const float>(*d_balance) : nullptr,
+                                      d_z ? ptr<const float>(*d_z) : nullptr, raw(out), stream_of(logits)) == ZMOE_OK)
+        return out;
+    }
+  }
+  static const auto op = general<Tensor(const Opt&, const Opt&, const Tensor&, const Opt&, c10::SymInt, const Tensor&,
+                                        const Tensor&)>("zmoe::router_losses_backward");
+  return op.call(d_balance, d_z, logits, cu, score, grad, inv);
+}
+
 Tensors flatten_sort_count(const Tensor& e, int64_t E) {
   if (e.is_cuda() && e.scalar_type() == at::kLong && e.is_contiguous() && E >= 0 && fits_int(E)) {
     const c10::DeviceGuard guard(e.device());
@@ -966,6 +1081,19 @@ TORCH_LIBRARY(zmoe_eager, m) {
              "(Tensor dAs, Tensor Hs, Tensor d_gates, Tensor topk_prob, Tensor topk_idx, int num_experts) -> Tensor");
   ZMOE_EAGER(route_topk_backward,
              "(Tensor d_weight, Tensor topk_prob, Tensor topk_idx, int num_experts, Tensor like) -> Tensor");
+  ZMOE_EAGER(route,
+             "(Tensor logits, Tensor? expert_biases, int k, int score, int groups, int top_groups, int group_scores, "
+             "bool renormalize, float scale) -> Tensor[]");
+  ZMOE_EAGER(route_backward,
+             "(Tensor d_weight, Tensor topk_prob, Tensor topk_idx, Tensor logits, int score, bool renormalize, "
+             "float scale) -> Tensor");
+  ZMOE_EAGER(swiglu_route_form_backward,
+             "(Tensor dAs, Tensor Hs, Tensor d_gates, Tensor topk_prob, Tensor topk_idx, Tensor logits, int score, "
+             "bool renormalize, float scale, Tensor? add) -> Tensor");
+  ZMOE_EAGER(router_losses, "(Tensor logits, Tensor topk_idx, Tensor? cu_seqlens, int score) -> Tensor[]");
+  ZMOE_EAGER(router_losses_backward,
+             "(Tensor? d_balance, Tensor? d_z, Tensor logits, Tensor? cu_seqlens, int score, Tensor seq_grad, "
+             "Tensor inv_tokens) -> Tensor");
   ZMOE_EAGER(flatten_sort_count, "(Tensor expert_idxs, int num_experts) -> Tensor[]");
   ZMOE_EAGER(flatten_sort_count_weights, "(Tensor expert_idxs, Tensor weights, int num_experts) -> Tensor[]");
   ZMOE_EAGER(glu_shared_forward,

@@ -10,53 +10,11 @@
 // and each round is a wave-wide max (route_topk_kernel).
 #include <type_traits>
 
-#include "zmoe_internal.h"
+#include "zmoe_route.h"
 
 namespace zmoe {
 
 constexpr int kRouteMaxPerLane = 16;  // E <= 1024
-
-// Sort key of a routing candidate's score; a larger key takes an earlier slot. A monotone
-// image of the biased score: every NaN canonicalised above +inf, -0 folded into +0. Equal
-// scores go to the lower expert. Key 0 marks a taken (or padding) candidate: a real
-// score's key is at least 0x007fffff (that of -inf).
-__device__ __forceinline__ uint32_t score_key(float s) {
-  uint32_t b = __float_as_uint(s);
-  b = s != s ? 0x7fffffffu : b;  // selects, not branches
-  b = s == 0.f ? 0u : b;
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-
-// Logits at or below this value give probability 0: there torch's sigmoid, which forms
-// 1 / (1 + exp(-z)) in fp32, overflows exp(-z) to inf (fp32 exp overflows from
-// 88.72283935546875 up; the true probabilities, below 2.9e-39, would be subnormal).
-constexpr float kSigmoidZeroBelow = -88.72283935546875f;
-
-// Below this |z| the probability comes from p = 0.5 + z/4 - z^3/48 + ...: 0.5 + z/4 is
-// exact in double, and the cubic term cannot move it across an fp32 rounding midpoint
-// unless it lies exactly on one (its distance from a midpoint is a multiple of z's last
-// bit / 4, more than |z|^3/48 here).
-constexpr float kSigmoidSeriesBelow = 0x1p-12f;
-
-// sigmoid correctly rounded to float: for |z| < kSigmoidSeriesBelow, 0.5 + z/4 rounded to
-// nearest with an exact tie going to the side the cubic term puts the true value on (down
-// for z > 0, up for z < 0; many small bf16 logits land on such ties, where a double
-// evaluation's rounding would hang on the last bit of its exp); otherwise
-// 1 / (1 + exp(-z)) in double, rounded once; 0 at or below kSigmoidZeroBelow.
-__device__ __forceinline__ float sigmoid_f64(float z) {
-  if (z <= kSigmoidZeroBelow) return 0.f;
-  if (fabsf(z) < kSigmoidSeriesBelow) {
-    const double s = 0.5 + 0.25 * (double)z;
-    const float f = (float)s;
-    const double fd = (double)f;
-    if (fd != s) {  // f > 0: its other neighbour around s is one bit pattern up or down
-      const float o = __uint_as_float(__float_as_uint(f) + (fd < s ? 1u : 0xffffffffu));
-      if (fabs(s - fd) == fabs((double)o - s)) return z > 0.f ? fminf(f, o) : fmaxf(f, o);
-    }
-    return f;
-  }
-  return (float)(1.0 / (1.0 + exp(-(double)z)));
-}
 
 // bf16(sigmoid_f64(z)) (the probability a bf16 gate stores) from fp32 arithmetic where that
 // is provably the same value: the fp32 estimate is within a few fp32 ulps of the true
@@ -88,21 +46,6 @@ __device__ const uint16_t kSigmoidBf16[65536] = {
 // logits, evaluated for fp32 ones.
 __device__ __forceinline__ float sigmoid_bf16_of(uint16_t zb) { return to_f32(kSigmoidBf16[zb]); }
 __device__ __forceinline__ float sigmoid_bf16_of(float z) { return sigmoid_bf16(z); }
-
-// Wave-wide max of a 32-bit key, the same value in every lane: DPP within rows of 16
-// (xor 1, xor 2, half mirror, mirror: no LDS round trip), then the four row maxima
-// through readlane.
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0xB1, 0xF, 0xF, false));   // quad_perm 1,0,3,2
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xF, 0xF, false));   // quad_perm 2,3,0,1
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x141, 0xF, 0xF, false));  // row_half_mirror
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x140, 0xF, 0xF, false));  // row_mirror
-  const uint32_t r0 = (uint32_t)__builtin_amdgcn_readlane((int)v, 0);
-  const uint32_t r1 = (uint32_t)__builtin_amdgcn_readlane((int)v, 16);
-  const uint32_t r2 = (uint32_t)__builtin_amdgcn_readlane((int)v, 32);
-  const uint32_t r3 = (uint32_t)__builtin_amdgcn_readlane((int)v, 48);
-  return max(max(r0, r1), max(r2, r3));
-}
 
 // Waves stride over tokens (each wave one token at a time, the next row's logits loaded
 // before the current one is ranked); lane l holds experts l + 64 q (q < PL). The score is
@@ -185,33 +128,6 @@ __global__ __launch_bounds__(256) void route_topk_kernel(const LT* __restrict__ 
       if (out_p) out_p[t * k + lane] = my_p;
     }
   }
-}
-
-// Reductions over rows of LPR = 16 or 8 lanes by DPP (xor 1, xor 2, mirror within 8 lanes,
-// mirror within 16); every lane of a row ends with the row's result.
-template <int LPR>
-__device__ __forceinline__ uint32_t row_max_u32(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true));
-  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true));
-  if (LPR == 16) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, true));
-  return v;
-}
-template <int LPR>
-__device__ __forceinline__ uint32_t row_min_u32(uint32_t v) {
-  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0xB1, 0xF, 0xF, false));
-  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x4E, 0xF, 0xF, false));
-  v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x141, 0xF, 0xF, false));
-  if (LPR == 16) v = min(v, (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)v, 0x140, 0xF, 0xF, false));
-  return v;
-}
-template <int LPR>
-__device__ __forceinline__ float row_sum_f32(float v) {
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));
-  v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));
-  if (LPR == 16) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));
-  return v;
 }
 
 // bf16 logits, E % 8 == 0, E <= LPR * VPL, k <= LPR: 64 / LPR tokens per wave, one per

@@ -1,0 +1,400 @@
+// Routing in its other forms (zmoe_route): sigmoid or softmax scores, a bias for the selection, groups of experts of
+// which the best stay, weights renormalised or as they are; and its gradient.
+//   p = sigmoid(z) or softmax(z), rounded once to f32 (a row of -inf alone: p = 0);  s = p + b in f32
+//   a group's score: its highest s, or the sum of its two highest; the top_groups best groups stay
+//   idx = the k best s in them (s desc, expert asc, NaN first);  w = c p_idx / max(sum p_idx, 1e-12), or c p_idx
+// Backward: dp_j = c (dw_j - sum_i dw_i p_i / S) / S (S the clamped sum; clamped or not renormalised: without the
+// sum's part), dz = dp p (1 - p) for a sigmoid, dz_e = p_e (dp_e - sum_j dp_j p_j) for a softmax, where the sum is 0 if
+// the weights are renormalised: then only selected experts have a grad and the logits are not read.
+//
+// Where p + b decides, one f32 rounding of p can decide: p comes from double, whose error (some 2^-52) moves an f32
+// rounding for one value in 2^28. Without a bias the experts' order is their logits' order.
+#include <type_traits>
+
+#include "zmoe_route.h"
+
+namespace zmoe {
+namespace {
+
+constexpr int kMaxSlots = 64;
+constexpr int kWaves = 4;  // of a workgroup
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;  // or null
+  int64_t T;
+  int E, k, groups, top_groups, group_scores, renorm, vec;
+  float scale;
+  int64_t* idx;
+  float* w;
+  float* p;  // or null
+};
+
+// Over the LPR (8, 16 or 64) lanes of a row; every lane gets the result.
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (LPR == 64) return wave_max_u32(v);
+  else return row_max_u32<LPR>(v);
+}
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
+  if constexpr (LPR == 64) return ~wave_max_u32(~v);
+  else return row_min_u32<LPR>(v);
+}
+template <int LPR, typename F>
+__device__ __forceinline__ F lanes_sum(F v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ float lanes_fmax(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// What a wave wrote to LDS is there for its other lanes (a wave's LDS accesses stay in order).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The float whose score_key is key (a NaN, +0 for both zeros).
+__device__ __forceinline__ float key_score(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: E and e0 are whole 16-byte chunks and rows lie on 16.
+template <int VPL, typename LT>
+__device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, int E, bool vec, bool live, float fill,
+                                          float (&v)[VPL]) {
+  constexpr int VC = 16 / sizeof(LT);
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < VPL / VC; ++c) {
+      if (live && e0 + c * VC < E) {
+        unpack_chunk(*reinterpret_cast<const uint4*>(row + e0 + c * VC), &v[c * VC], LT{});
+      } else {
+#pragma unroll
+        for (int u = 0; u < VC; ++u) v[c * VC + u] = fill;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < VPL; ++q) v[q] = live && e0 + q < E ? to_f32(row[e0 + q]) : fill;
+  }
+}
+
+// Rows of LPR lanes, VPL consecutive experts a lane, 64 / LPR tokens a wave at once; waves stride over the tokens.
+template <int LPR, int VPL, bool SOFT, typename LT>
+__global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
+  constexpr int TPW = 64 / LPR, W = LPR * VPL;
+  __shared__ float ps[kWaves][TPW][W];
+  __shared__ uint32_t gk[kWaves][TPW][W];
+  __shared__ uint16_t slots[kWaves][TPW][kMaxSlots];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = lane / LPR, r = lane % LPR, e0 = r * VPL;
+  const int E = a.E, k = a.k, G = a.groups, gsz = E / G;
+  const bool two = a.group_scores == 2 && G > 1;
+  const bool by_p = a.bias != nullptr;
+  float b[VPL];
+#pragma unroll
+  for (int q = 0; q < VPL; ++q) b[q] = by_p && e0 + q < E ? a.bias[e0 + q] : 0.f;
+
+  const int64_t step = (int64_t)gridDim.x * kWaves * TPW;
+  for (int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * TPW; t0 < a.T; t0 += step) {
+    const int64_t t = t0 + row;
+    const bool live = t < a.T;
+    float z[VPL], p[VPL];
+    load_lane<VPL>((const LT*)a.logits + t * E, e0, E, a.vec, live, -INFINITY, z);
+    if constexpr (SOFT) {
+      float m = z[0];
+#pragma unroll
+      for (int q = 1; q < VPL; ++q) m = fmaxf(m, z[q]);
+      m = lanes_fmax<LPR>(m);
+      m = m == -INFINITY ? 0.f : m;  // nothing to choose from: all p are 0
+      double e[VPL], sum = 0.0;
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) {
+        e[q] = exp((double)z[q] - (double)m);
+        sum += e[q];
+      }
+      sum = lanes_sum<LPR>(sum);
+      const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) p[q] = (float)(e[q] * inv);
+    } else {
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) p[q] = sigmoid_f64(z[q]);
+    }
+    uint32_t key[VPL];
+#pragma unroll
+    for (int q = 0; q < VPL; ++q) {
+      key[q] = live && e0 + q < E ? score_key(by_p ? p[q] + b[q] : z[q]) : 0u;
+      ps[wave][row][e0 + q] = p[q];
+    }
+    if (G > 1) {
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) gk[wave][row][e0 + q] = two && !by_p ? score_key(p[q]) : key[q];
+      wave_sync();
+      // lane r scores groups r, r + LPR, ...; the best top_groups of them in rounds
+      uint32_t mine[(64 + LPR - 1) / LPR];
+#pragma unroll
+      for (int i = 0; i < (64 + LPR - 1) / LPR; ++i) {
+        const int g = r + i * LPR;
+        mine[i] = 0;
+        if (g < G && live) {
+          uint32_t k1 = 0, k2 = 0;
+          for (int u = 0; u < gsz; ++u) {
+            const uint32_t v = gk[wave][row][g * gsz + u];
+            k2 = max(k2, min(k1, v));
+            k1 = max(k1, v);
+          }
+          mine[i] = two ? score_key(key_score(k1) + key_score(k2)) : k1;
+        }
+      }
+      uint64_t keep = 0;  // the same in a row's lanes
+      for (int j = 0; j < a.top_groups; ++j) {
+        uint32_t m = mine[0];
+#pragma unroll
+        for (int i = 1; i < (64 + LPR - 1) / LPR; ++i) m = max(m, mine[i]);
+        m = lanes_max<LPR>(m);
+        uint32_t g = 0xffffffffu;
+#pragma unroll
+        for (int i = (64 + LPR - 1) / LPR - 1; i >= 0; --i) g = mine[i] == m ? (uint32_t)(r + i * LPR) : g;
+        g = lanes_min<LPR>(g);
+        keep |= 1ull << (g & 63);
+#pragma unroll
+        for (int i = 0; i < (64 + LPR - 1) / LPR; ++i) mine[i] = (uint32_t)(r + i * LPR) == g ? 0u : mine[i];
+      }
+      int g = e0 / gsz, left = gsz - (e0 - g * gsz);
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) {
+        key[q] = (keep >> (g & 63)) & 1 ? key[q] : 0u;
+        if (--left == 0) {
+          left = gsz;
+          ++g;
+        }
+      }
+    }
+    for (int j = 0; j < k; ++j) {
+      uint32_t m = key[0];
+#pragma unroll
+      for (int q = 1; q < VPL; ++q) m = max(m, key[q]);
+      m = lanes_max<LPR>(m);
+      uint32_t e = 0xffffffffu;  // this lane's lowest expert holding m, then the row's
+#pragma unroll
+      for (int q = VPL - 1; q >= 0; --q) e = key[q] == m ? (uint32_t)(e0 + q) : e;
+      e = lanes_min<LPR>(e);
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) key[q] = (uint32_t)(e0 + q) == e ? 0u : key[q];
+      if (r == 0) slots[wave][row][j] = (uint16_t)e;
+    }
+    wave_sync();
+    float sum = 0.f;
+    for (int j = r; j < k; j += LPR) sum += ps[wave][row][slots[wave][row][j]];
+    sum = lanes_sum<LPR>(sum);
+    const float denom = sum < 1e-12f ? 1e-12f : sum;  // NaN propagates
+    if (live) {
+      for (int j = r; j < k; j += LPR) {
+        const int e = slots[wave][row][j];
+        const float pj = ps[wave][row][e];
+        a.idx[t * k + j] = e;
+        a.w[t * k + j] = a.scale * (a.renorm ? pj / denom : pj);
+        if (a.p) a.p[t * k + j] = pj;
+      }
+    }
+    wave_sync();  // before the next token's values
+  }
+}
+
+struct RouteBackwardArgs {
+  const float* dw;
+  const float* p;
+  const int64_t* idx;
+  const void* logits;  // softmax only
+  const void* add;     // or null: [T, E] of the grad's type, rows ld_add apart
+  int64_t ld_add, T, ld;
+  int E, k, renorm, vec;
+  float scale;
+  void* dz;
+};
+
+template <int LPR, int VPL, bool SOFT, typename LT>
+__global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const RouteBackwardArgs a) {
+#pragma clang fp contract(off)  // (one expert's renormalised weight has a grad of rounding errors alone: 0, not fused ones)
+  constexpr int TPW = 64 / LPR, W = LPR * VPL, VC = 16 / sizeof(LT);
+  __shared__ float ds[kWaves][TPW][W];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = lane / LPR, r = lane % LPR, e0 = r * VPL;
+  const int E = a.E, k = a.k;
+  const int64_t step = (int64_t)gridDim.x * kWaves * TPW;
+  for (int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * TPW; t0 < a.T; t0 += step) {
+    const int64_t t = t0 + row;
+    const bool live = t < a.T;
+    float* mine = &ds[wave][row][0];
+#pragma unroll
+    for (int q = 0; q < VPL; ++q) mine[e0 + q] = 0.f;
+    float add[VPL];
+    if (a.add) load_lane<VPL>((const LT*)a.add + t * a.ld_add, e0, E, a.vec, live, 0.f, add);
+    float S = 0.f, dot = 0.f;  // sum p, sum c dw p
+    if (live)
+      for (int j = r; j < k; j += LPR) {
+        const float pj = a.p[t * k + j];
+        S += pj;
+        dot += a.scale * a.dw[t * k + j] * pj;
+      }
+    S = lanes_sum<LPR>(S);
+    dot = lanes_sum<LPR>(dot);
+    // not scaled: the weights are c p (/ 1e-12), and the softmax's sum of dp p is not 0
+    const bool scaled = a.renorm && !(S <= 1e-12f);
+    const float total = !a.renorm ? 1.f : scaled ? S : 1e-12f;
+    const float mean = scaled ? dot / total : 0.f, inner = scaled ? 0.f : dot / total;
+    wave_sync();
+    if (live)
+      for (int j = r; j < k; j += LPR) {
+        const int64_t e = a.idx[t * k + j];
+        const float pj = a.p[t * k + j], dp = (a.scale * a.dw[t * k + j] - mean) / total;
+        if (e >= 0 && e < E) mine[e] = SOFT ? pj * (dp - inner) : dp * pj * (1.f - pj);
+      }
+    wave_sync();
+    float v[VPL];
+#pragma unroll
+    for (int q = 0; q < VPL; ++q) v[q] = mine[e0 + q];
+    if constexpr (SOFT) {
+      if (!scaled) {  // every logit has a grad: -p_e sum dp p where it is not selected
+        float z[VPL];
+        load_lane<VPL>((const LT*)a.logits + t * E, e0, E, a.vec, live, -INFINITY, z);
+        float m = z[0], sum = 0.f;
+#pragma unroll
+        for (int q = 1; q < VPL; ++q) m = fmaxf(m, z[q]);
+        m = lanes_fmax<LPR>(m);
+        m = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int q = 0; q < VPL; ++q) {
+          z[q] = expf(z[q] - m);
+          sum += z[q];
+        }
+        sum = lanes_sum<LPR>(sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint32_t sel = 0;
+        if (live)
+          for (int j = 0; j < k; ++j) {
+            const int64_t q = a.idx[t * k + j] - e0;
+            if (q >= 0 && q < VPL) sel |= 1u << (int)q;
+          }
+#pragma unroll
+        for (int q = 0; q < VPL; ++q) v[q] = (sel >> q) & 1 ? v[q] : -(z[q] * inv) * inner;
+      }
+    }
+    if (a.add) {
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) v[q] += add[q];
+    }
+    if (live) {
+      LT* out = (LT*)a.dz + t * a.ld;
+      if (a.vec) {
+#pragma unroll
+        for (int c = 0; c < VPL / VC; ++c)
+          if (e0 + c * VC < E) *reinterpret_cast<uint4*>(out + e0 + c * VC) = pack_chunk(&v[c * VC], LT{});
+      } else {
+#pragma unroll
+        for (int q = 0; q < VPL; ++q)
+          if (e0 + q < E) out[e0 + q] = from_f32<LT>(v[q]);
+      }
+    }
+    wave_sync();
+  }
+}
+
+using I8 = std::integral_constant<int, 8>;
+using I16 = std::integral_constant<int, 16>;
+using I64 = std::integral_constant<int, 64>;
+
+// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts.
+template <typename F>
+void by_layout(int E, bool soft, int dtype, F&& f) {
+  auto typed = [&](auto lpr, auto vpl) {
+    auto scored = [&](auto lt) {
+      if (soft) f(lpr, vpl, std::true_type{}, lt);
+      else f(lpr, vpl, std::false_type{}, lt);
+    };
+    if (dtype == ZMOE_DTYPE_BF16) scored(uint16_t{});
+    else scored(float{});
+  };
+  if (E <= 64) typed(I8{}, I8{});
+  else if (E <= 128) typed(I16{}, I8{});
+  else if (E <= 256) typed(I16{}, I16{});
+  else if (E <= 512) typed(I64{}, I8{});
+  else typed(I64{}, I16{});
+}
+
+// Workgroups that hold the tokens, at most eight a CU: their waves loop over the others.
+unsigned grid_of(int64_t T, int lpr) {
+  const int64_t blocks = cdiv(T, (int64_t)kWaves * (64 / lpr));
+  return (unsigned)(blocks < 2048 ? blocks : 2048);
+}
+
+bool rows_on_16(const void* base, int64_t ld, int E, int dtype) {
+  const int size = dtype_size(dtype);
+  return aligned16(base) && (ld * size) % 16 == 0 && (E * size) % 16 == 0;
+}
+
+}  // namespace
+}  // namespace zmoe
+
+using namespace zmoe;
+
+extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E, int k, int score,
+                          const float* expert_biases, int groups, int top_groups, int group_scores, int renormalize,
+                          float scale, int64_t* topk_idx, float* topk_weight, float* topk_prob, void* stream) {
+  ZMOE_REQUIRE(dtype_ok(logits_dtype), ZMOE_ERR_DTYPE, "route: logits dtype %d", logits_dtype);
+  ZMOE_REQUIRE(T >= 0 && E >= 1 && E <= 1024, ZMOE_ERR_SHAPE, "route: need 1 <= E <= 1024 (E=%d)", E);
+  ZMOE_REQUIRE(score == ZMOE_SCORE_SIGMOID || score == ZMOE_SCORE_SOFTMAX, ZMOE_ERR_SHAPE, "route: score %d", score);
+  ZMOE_REQUIRE(groups >= 1 && groups <= 64 && E % groups == 0, ZMOE_ERR_SHAPE,
+               "route: need 1 to 64 groups of equal size (groups=%d, E=%d)", groups, E);
+  ZMOE_REQUIRE(top_groups >= 1 && top_groups <= groups, ZMOE_ERR_SHAPE, "route: need 1 <= top_groups <= groups (%d, %d)",
+               top_groups, groups);
+  ZMOE_REQUIRE(group_scores >= 1 && group_scores <= 2 && (groups == 1 || group_scores <= E / groups), ZMOE_ERR_SHAPE,
+               "route: a group's score is of its 1 or 2 best experts (group_scores=%d, %d in a group)", group_scores,
+               E / groups);
+  ZMOE_REQUIRE(k >= 1 && k <= kMaxSlots && k <= top_groups * (E / groups), ZMOE_ERR_SHAPE,
+               "route: need 1 <= k <= %d and experts to choose from (k=%d, %d)", kMaxSlots, k, top_groups * (E / groups));
+  if (T == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(logits && topk_idx && topk_weight, ZMOE_ERR_NULL, "route: null pointer");
+  const RouteArgs a{logits, expert_biases, T, E, k, groups, top_groups, group_scores, renormalize,
+                    rows_on_16(logits, E, E, logits_dtype), scale, topk_idx, topk_weight, topk_prob};
+  by_layout(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
+    hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
+                       dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
+  });
+  return check_launch("route");
+}
+
+extern "C" int zmoe_route_backward(const float* d_weight, const float* topk_prob, const int64_t* topk_idx, int64_t T,
+                                   int E, int k, int score, const void* logits, int renormalize, float scale,
+                                   const void* add, int64_t ld_add, void* d_logits, int64_t ld_d_logits,
+                                   int d_logits_dtype, void* stream) {
+  ZMOE_REQUIRE(dtype_ok(d_logits_dtype), ZMOE_ERR_DTYPE, "route_backward: dtype %d", d_logits_dtype);
+  ZMOE_REQUIRE(T >= 0 && E >= 1 && E <= 1024 && k >= 1 && k <= E && k <= kMaxSlots, ZMOE_ERR_SHAPE,
+               "route_backward: bad sizes (E=%d, k=%d)", E, k);
+  ZMOE_REQUIRE(score == ZMOE_SCORE_SIGMOID || score == ZMOE_SCORE_SOFTMAX, ZMOE_ERR_SHAPE, "route_backward: score %d",
+               score);
+  ZMOE_REQUIRE(ld_d_logits >= E && (!add || ld_add >= E), ZMOE_ERR_SHAPE, "route_backward: row stride below E=%d", E);
+  if (T == 0) return ZMOE_OK;
+  ZMOE_REQUIRE(d_weight && topk_prob && topk_idx && d_logits && (logits || score == ZMOE_SCORE_SIGMOID), ZMOE_ERR_NULL,
+               "route_backward: null pointer");
+  const bool vec = rows_on_16(d_logits, ld_d_logits, E, d_logits_dtype) &&
+                   (!add || rows_on_16(add, ld_add, E, d_logits_dtype)) &&
+                   (!logits || rows_on_16(logits, E, E, d_logits_dtype));
+  const RouteBackwardArgs a{d_weight, topk_prob, topk_idx, logits, add, ld_add, T, ld_d_logits, E, k, renormalize, vec,
+                            scale, d_logits};
+  by_layout(E, score == ZMOE_SCORE_SOFTMAX, d_logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
+    hipLaunchKernelGGL(
+        (route_backward_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
+        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
+  });
+  return check_launch("route_backward");
+}

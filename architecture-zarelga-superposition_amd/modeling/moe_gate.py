@@ -9,13 +9,19 @@ Contract where the reference leaves order unspecified (topk(sorted=False)):
 slots come in (biased score desc, expert asc) order and NaN ranks first, as in
 torch.topk. Under bf16 logits the probabilities are rounded to bf16 before the
 bias add, as the reference's bf16 sigmoid does under autocast.
+
+A config with other ``router_*`` fields than the reference's form (softmax scores, no bias, groups of experts, weights
+as they are or scaled) routes through ``zmoe.functional.route``, whose probabilities are float32 for any logits.
 """
+
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
 
 from zmoe import functional as _zf
 from zmoe import library as _zl
+from zmoe import ops as _zo
 
 
 class RouteTopK(torch.autograd.Function):
@@ -39,6 +45,26 @@ class RouteTopK(torch.autograd.Function):
         return d_logits, None, None
 
 
+class RouteForm(NamedTuple):
+    """What ``zmoe.functional.route`` takes besides the logits, the bias and k."""
+
+    score: int = 0
+    groups: int = 1
+    top_groups: int = 1
+    group_scores: int = 1
+    renormalize: bool = True
+    scale: float = 1.0
+    bias: bool = True
+
+    @staticmethod
+    def of(config) -> "RouteForm":
+        get = lambda name, default: getattr(config, "router_" + name, default)  # noqa: E731
+        groups = int(get("groups", 1))
+        return RouteForm(_zo.SCORES[get("score", "sigmoid")], groups, int(get("top_groups", 1)),
+                         int(get("group_scores", 2)) if groups > 1 else 1, bool(get("renormalize", True)),
+                         float(get("scale", 1.0)), bool(get("bias", True)))
+
+
 class MoEGate(nn.Module):
     def __init__(self, config):
         super().__init__()
@@ -46,6 +72,8 @@ class MoEGate(nn.Module):
         self.top_k = config.n_experts_per_token
         self.n_routed_experts = config.n_routed_experts
         self.gating_dim = config.hidden_size
+        form = RouteForm.of(config)
+        self.form = None if form == RouteForm() else form  # None: the reference's
         self.weight = nn.Parameter(torch.empty((self.n_routed_experts, self.gating_dim)))
         self.register_buffer("expert_biases", torch.zeros(self.n_routed_experts))
         self.reset_parameters()
@@ -53,9 +81,20 @@ class MoEGate(nn.Module):
     def reset_parameters(self):
         nn.init.normal_(self.weight, mean=0.0, std=self.config.initializer_range)
 
-    def forward(self, hidden_states):
+    @property
+    def score(self) -> str:
+        return "softmax" if self.form is not None and self.form.score else "sigmoid"
+
+    def forward(self, hidden_states, return_logits: bool = False):
+        """(topk_idx, topk_weight), with ``return_logits`` also the logits [T, E] that they come from."""
         bsz, seq_len, h = hidden_states.shape
         hidden_states = hidden_states.view(-1, h)
         gate_output = _zf.linear(hidden_states, self.weight)                     # moe_gate.py:26
-        topk_idx, topk_weight = RouteTopK.apply(gate_output, self.expert_biases, self.top_k)  # :27-34
-        return topk_idx.view(bsz, seq_len, self.top_k), topk_weight.view(bsz, seq_len, self.top_k)
+        f = self.form
+        if f is None:
+            topk_idx, topk_weight = RouteTopK.apply(gate_output, self.expert_biases, self.top_k)  # :27-34
+        else:
+            topk_idx, topk_weight = _zf.route(gate_output, self.top_k, self.expert_biases if f.bias else None, self.score,
+                                              f.groups, f.top_groups, f.group_scores, f.renormalize, f.scale)
+        out = topk_idx.view(bsz, seq_len, self.top_k), topk_weight.view(bsz, seq_len, self.top_k)
+        return (*out, gate_output) if return_logits else out

@@ -33,6 +33,14 @@ def pad_input(x: torch.Tensor, indices: torch.Tensor, batch: int, seqlen: int) -
     return out.view(batch, seqlen, *x.shape[1:])
 
 
+def _routed(logits, expert_biases, k: int, form):
+    """(idx, weight, prob) [T, k] of a bf16 gate."""
+    if form is None:
+        return _zl.route_topk(logits, expert_biases, k, True)
+    return _zl.route(logits, expert_biases if form.bias else None, k, form.score, form.groups, form.top_groups,
+                     form.group_scores, form.renormalize, form.scale)
+
+
 class _FusedMoELayer(torch.autograd.Function):
     """The whole layer in one autograd function (bf16 on the device): gate projection and
     routing, shared expert, routed GLU experts, combine. The routing is computed as in the
@@ -52,8 +60,10 @@ class _FusedMoELayer(torch.autograd.Function):
     adds over [T, d]).
 
     (x [T, d], gate weight, expert_biases, W1, W2, shared gate/up/down weights, k, E,
-    pad_rows, pad_total, backward) -> (out, topk_idx [T, k], expert_offsets [E]); out is [T, d],
-    or with pad_rows (int64 [T]) the padded [pad_total, d] whose row pad_rows[t] is token t's.
+    pad_rows, pad_total, backward, form, with_logits) -> (out, topk_idx [T, k], expert_offsets [E]); out is [T, d],
+    or with pad_rows (int64 [T]) the padded [pad_total, d] whose row pad_rows[t] is token t's. ``form``: the gate's
+    (None: the reference's). ``with_logits``: the router's logits [T, E] as a fourth result, whose grad (the router's
+    losses') joins the routing's in the backward, before its one rounding.
     With backward False (a call that records no graph) the grouped W1 launch writes no
     pre-activations and W3 is formed only where the launches read it; the streaming launches of a
     small batch write theirs either way. Every launch is a ``zmoe::`` custom op, so torch.compile
@@ -69,7 +79,7 @@ class _FusedMoELayer(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, gate_w, expert_biases, W1, W2, Ws_gate, Ws_up, Ws_down, k: int, E: int, pad_rows=None,
-                pad_total: int = 0, backward: bool = True):
+                pad_total: int = 0, backward: bool = True, form=None, with_logits: bool = False):
         bf = torch.bfloat16
         ctx.f32_grads = W1.dtype == torch.float32
         ctx.x_dtype = x.dtype
@@ -97,12 +107,12 @@ class _FusedMoELayer(torch.autograd.Function):
             else:
                 up, gate, router = W3[:fs], W3[fs:2 * fs], W3[2 * fs:]
             logits = F.linear(x, router)                                             # moe_gate.py:26
-            idx, w, p = _zl.route_topk(logits, expert_biases, k, True)
+            idx, w, p = _routed(logits, expert_biases, k, form)
             se, ss, off, inv, w_sorted = _zl.flatten_sort_count_weights(idx, w, E)   # mlp.py:76-77
             H, A_s, Y_s, Hs, As, S = _zl.glu_shared_forward(x, W1, W2, ss, off, k, w_sorted, up, gate, Ws_down)
         else:
             logits = F.linear(x, W3[2 * fs:])                                        # moe_gate.py:26
-            idx, w, p = _zl.route_topk(logits, expert_biases, k, True)
+            idx, w, p = _routed(logits, expert_biases, k, form)
             Hs = F.linear(x, W3[:2 * fs])
             As = _zl.swiglu(Hs)
             S = F.linear(As, Ws_down)                                                # expert_layer.py:23-24
@@ -114,17 +124,20 @@ class _FusedMoELayer(torch.autograd.Function):
             Y_s = _zl.grouped_mm(A_s, W2.permute(0, 2, 1), se, ss, 1, True, False, off,
                                  "scatter2scatter")                                  # = w * Y
         out = _zl.combine(Y_s, None, k, S, pad_rows, pad_total)                      # moe_layer.py:48-56
-        ctx.save_for_backward(x, W1, W2, W3, Ws_down, Hs, As, p, idx, w_sorted, se, ss, off, H, A_s, pad_rows)
-        ctx.k, ctx.E, ctx.fs = k, E, fs
+        ctx.save_for_backward(x, W1, W2, W3, Ws_down, Hs, As, p, idx, w_sorted, se, ss, off, H, A_s, pad_rows,
+                              None if form is None and not with_logits else logits)
+        ctx.k, ctx.E, ctx.fs, ctx.form, ctx.out_rows = k, E, fs, form, out.shape[0]
         ctx.mark_non_differentiable(idx, off)
         ctx.set_materialize_grads(False)  # no zero-filled grads for idx and off (two fill launches)
-        return out, idx, off
+        return (out, idx, off, logits) if with_logits else (out, idx, off)
 
     @staticmethod
-    def backward(ctx, dout, d_idx, d_off):
-        if dout is None:  # out took no part in the loss
-            return (None,) * 13
-        x, W1, W2, W3, Ws_down, Hs, As, p, idx, w_sorted, se, ss, off, H, A_s, pad_rows = ctx.saved_tensors
+    def backward(ctx, dout, d_idx, d_off, d_logits=None):
+        if dout is None and d_logits is None:  # out took no part in the loss
+            return (None,) * 15
+        x, W1, W2, W3, Ws_down, Hs, As, p, idx, w_sorted, se, ss, off, H, A_s, pad_rows, logits = ctx.saved_tensors
+        if dout is None:  # only the router's losses did
+            dout = x.new_zeros(ctx.out_rows, x.shape[1])
         k, E, fs = ctx.k, ctx.E, ctx.fs
         need = ctx.needs_input_grad
         f32 = ctx.f32_grads  # fp32 weight grads from the accumulators (fp32 master weights)
@@ -145,13 +158,17 @@ class _FusedMoELayer(torch.autograd.Function):
         # [d up | d gate | d_logits] side by side, one product for both input grads
         dAs = dS @ Ws_down
         dWs_down = _zl.dense_wgrad(dS, As, f32) if need[7] else None
-        G = _zl.swiglu_route_backward(dAs, Hs, d_gates, p, idx, E)
+        if ctx.form is None and d_logits is None:
+            G = _zl.swiglu_route_backward(dAs, Hs, d_gates, p, idx, E)
+        else:
+            f = (0, True, 1.0) if ctx.form is None else (ctx.form.score, ctx.form.renormalize, ctx.form.scale)
+            G = _zl.swiglu_route_form_backward(dAs, Hs, d_gates, p, idx, logits, *f, d_logits)
         dx_dense = G @ W3                                   # shared expert + gate input grads
         dW3 = _zl.dense_wgrad(G, x, f32) if need[1] or need[5] or need[6] else None
         dx = _zl.sum_k(dXe, k, dx_dense, ctx.x_dtype == torch.float32)  # fp32 input: the fp32 sum
         part = (lambda a, b: None) if dW3 is None else (lambda a, b: dW3[a:b])
         return (dx, part(2 * fs, 2 * fs + E), None, dW1, dW2, part(fs, 2 * fs), part(0, fs), dWs_down,
-                None, None, None, None, None)
+                None, None, None, None, None, None, None)
 
 
 class MoELayer(nn.Module):
@@ -213,8 +230,12 @@ class MoELayer(nn.Module):
               and x.shape[-1] % 8 == 0 and ws[2].shape[2] % 8 == 0)      # and of the d- and f-wide operands
         return ws if ok else None
 
-    def forward(self, hidden_states, unpad_indices=None, norm=None):
+    def forward(self, hidden_states, unpad_indices=None, norm=None, router_losses: bool = False, cu_seqlens=None):
         """(out, topk_idx) as the reference's forward (moe_layer.py:38-59).
+
+        ``router_losses``: (out, topk_idx, (balance, z)) with the losses of ``zmoe.functional.router_losses`` on this call's
+        router, over the sequences ``cu_seqlens`` of the tokens that the layer routes (the unpadded ones where
+        ``unpad_indices`` are given); None: each row of the batch is one, with ``unpad_indices`` all tokens.
 
         ``norm`` (a ZeroCenteredRMSNorm, optional): the layer's input is
         ``norm(hidden_states)``, as the transformer block computes it before calling the
@@ -237,11 +258,14 @@ class MoELayer(nn.Module):
             else:
                 x = flat if unpad_indices is None else index_first_axis(flat, unpad_indices)
             ins = (x, ws[0], self.gate.expert_biases, *ws[1:], self.gate.top_k, self.routed_experts.num_experts, *pad)
-            out, topk_idx, offsets = _FusedMoELayer.apply(*ins, _records_graph(ins))
+            out, topk_idx, offsets, *logits = _FusedMoELayer.apply(*ins, _records_graph(ins), self.gate.form,
+                                                                   router_losses)
             self.routed_experts.last_expert_offsets = offsets
+            losses = ((self._router_losses(logits[0], topk_idx, bsz, seq_len, unpad_indices, cu_seqlens),)
+                      if router_losses else ())
             if unpad_indices is None:
-                return out.view(bsz, seq_len, h), topk_idx.view(bsz, seq_len, self.gate.top_k)
-            return out.view(bsz, seq_len, h), pad_input(topk_idx, unpad_indices, bsz, seq_len)
+                return out.view(bsz, seq_len, h), topk_idx.view(bsz, seq_len, self.gate.top_k), *losses
+            return out.view(bsz, seq_len, h), pad_input(topk_idx, unpad_indices, bsz, seq_len), *losses
         if normed is not None:
             x = normed if unpad_indices is None else normed.unsqueeze(0)
         elif unpad_indices is not None:
@@ -250,7 +274,12 @@ class MoELayer(nn.Module):
         else:
             x = hidden_states
 
-        topk_idx, topk_weight = self.gate(x)
+        losses = ()
+        if router_losses:
+            topk_idx, topk_weight, logits = self.gate(x, return_logits=True)
+            losses = (self._router_losses(logits, topk_idx, bsz, seq_len, unpad_indices, cu_seqlens),)
+        else:
+            topk_idx, topk_weight = self.gate(x)
         shared_output = self.shared_experts(x)
 
         flat_topk_idx = topk_idx.reshape(-1, self.n_experts_per_token)
@@ -259,11 +288,16 @@ class MoELayer(nn.Module):
         # routed experts' combine pass, which also writes the re-padded layout (:55-56)
         # directly when unpad_indices is given
         if unpad_indices is None:
-            return self.routed_experts(x, flat_topk_weight, flat_topk_idx, residual=shared_output), topk_idx
+            return self.routed_experts(x, flat_topk_weight, flat_topk_idx, residual=shared_output), topk_idx, *losses
         out = self.routed_experts(x, flat_topk_weight, flat_topk_idx, residual=shared_output,
                                   pad=(unpad_indices, bsz * seq_len))
         topk_idx = pad_input(topk_idx.squeeze(0), unpad_indices, bsz, seq_len)
-        return out.view(bsz, seq_len, -1), topk_idx
+        return out.view(bsz, seq_len, -1), topk_idx, *losses
+
+    def _router_losses(self, logits, topk_idx, bsz, seq_len, unpad_indices, cu_seqlens):
+        if cu_seqlens is None and unpad_indices is None and bsz > 1 and seq_len > 0:
+            cu_seqlens = torch.arange(0, bsz * seq_len + 1, seq_len, device=logits.device)
+        return _zf.router_losses(logits, topk_idx, self.gate.score, cu_seqlens)
 
 
 class Fp8MoELayer(Fp8Module):

@@ -30,7 +30,21 @@ P = ctypes.c_void_p
 I64 = ctypes.c_int64
 I32 = ctypes.c_int
 F32 = ctypes.c_float
+F64 = ctypes.c_double
 SZ = ctypes.c_size_t
+
+class AdamwTensor(ctypes.Structure):
+    """zmoe_adamw_tensor"""
+
+    _fields_ = [("param", P), ("grad", P), ("exp_avg", P), ("exp_avg_sq", P), ("scale_avg", P), ("scale_sq", P),
+                ("step", P), ("n", I64)]
+
+
+class Moment(ctypes.Structure):
+    """zmoe_moment"""
+
+    _fields_ = [("codes", P), ("scale", P), ("out", P), ("n", I64), ("second", I32)]
+
 
 # name -> (restype, argtypes); mirrors include/zmoe.h
 SIGNATURES = {
@@ -93,6 +107,16 @@ SIGNATURES = {
     "zmoe_norm_residual_backward_workspace_bytes": (SZ, [I64, I64]),
     "zmoe_norm_residual_backward": (I32, [P, P, P, I64, I32, P, I64, I32, I64, I64, P, P, I32, P, I32, I64, I32, P, F32,
                                           P, P, P, P, P, P, P, P, P, SZ, P]),
+    "zmoe_route": (I32, [P, I32, I64, I32, I32, I32, P, I32, I32, I32, I32, F32, P, P, P, P]),
+    "zmoe_route_backward": (I32, [P, P, P, I64, I32, I32, I32, P, I32, F32, P, I64, P, I64, I32, P]),
+    "zmoe_router_losses_workspace_bytes": (SZ, [I64, I32, I64]),
+    "zmoe_router_losses": (I32, [P, I32, I64, I32, P, I32, I32, P, I32, I64, P, P, P, P, SZ, P]),
+    "zmoe_router_losses_backward": (I32, [P, I32, I64, I32, I32, P, I32, I64, P, P, P, P, P, P]),
+    "zmoe_adamw": (I32, [P, I32, I32, I32, P, F64, F64, F64, F64, F64, P, P, SZ, P]),
+    "zmoe_adamw_moments": (I32, [P, I32, P]),
+    "zmoe_sum_squares_workspace_bytes": (SZ, [I64]),
+    "zmoe_sum_squares": (I32, [P, P, I32, I32, P, P]),
+    "zmoe_clip_factor": (I32, [P, I64, F32, P, P]),
     "zmoe_newton_schulz5_workspace_bytes": (SZ, [I64, I64, I64]),
     "zmoe_newton_schulz5": (I32, [P, I64, I64, I64, I32, F32, F32, F32, P, SZ, P]),
 }

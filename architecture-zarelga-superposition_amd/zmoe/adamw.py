@@ -1,0 +1,198 @@
+"""AdamW over many tensors at once, next to the Newton-Schulz step of the matrices (zmoe.muon): the reference trains what
+Muon leaves (gates, norms, embeddings) with an auxiliary Adam (optimizer/muon.py:574-653), inside a captured graph
+(optimizer/hybrid.py:95-117).
+
+``AdamW`` is a ``torch.optim.Optimizer``. A step is one launch over all tensors of a type (forty-eight a launch), a small
+one in front for the step counts, and two more for the grads' norm where it clips. Everything that a step needs is on the
+device, so a step can be captured into a graph and replayed (after one eager step, which makes the state).
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import ops
+
+_STATE_DTYPES = {32: (torch.float32, torch.float32), 8: (torch.int8, torch.uint8)}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill its memory without gaps or overlaps, in any order of its dims."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay, p <- p - lr wd p - lr mhat / (sqrt(vhat) + eps), for float32 and bfloat16
+    parameters on the GPU (float32 arithmetic, one rounding of a bfloat16 parameter).
+
+    ``state_bits`` (also a group's): 32, moments in float32; 8, a byte for each element and a float32 scale for each 256 of
+    them (``zmoe.h``, zmoe_adamw). ``max_grad_norm``: the grads of all groups are multiplied by
+    min(1, max_grad_norm / (norm + 1e-6)), norm their common 2-norm, which ``grad_norm`` holds after a step. ``lr``: a number
+    or a float32 tensor of one element on the device, which a captured step reads anew."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32, max_grad_norm: Optional[float] = None):
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        if self.max_grad_norm is not None and not self.max_grad_norm > 0.0:
+            raise ValueError(f"AdamW: max_grad_norm must be positive, got {max_grad_norm}")
+        self.grad_norm: Optional[torch.Tensor] = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        g = self.param_groups[-1]
+        try:
+            lr, betas = g["lr"], tuple(g["betas"])
+            if isinstance(lr, torch.Tensor):
+                if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
+                    raise ValueError("AdamW: lr must be a number or a float32 tensor of one element")
+            elif not lr >= 0.0:
+                raise ValueError(f"AdamW: lr must not be negative, got {lr}")
+            if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+                raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
+            if not g["eps"] >= 0.0 or not g["weight_decay"] >= 0.0:
+                raise ValueError(f"AdamW: eps and weight_decay must not be negative, got {g['eps']} and {g['weight_decay']}")
+            if g["state_bits"] not in _STATE_DTYPES:
+                raise ValueError(f"AdamW: state_bits must be 32 or 8, got {g['state_bits']}")
+            for p in g["params"]:
+                if p.dtype not in (torch.float32, torch.bfloat16):
+                    raise ValueError(f"AdamW: parameters must be float32 or bfloat16, got {p.dtype}")
+                if not _dense(p):
+                    raise ValueError("AdamW: a parameter's elements must lie in memory without gaps or overlaps "
+                                     f"(shape {tuple(p.shape)}, strides {p.stride()})")
+        except ValueError:
+            self.param_groups.pop()
+            raise
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        for g in self.param_groups:
+            g.setdefault("state_bits", 32)
+
+    def _state_of(self, p: torch.Tensor, bits: int) -> dict:
+        st = self.state[p]
+        if not st:
+            if not p.is_cuda:
+                raise ValueError("zmoe ops need tensors on a HIP device")
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: take a step before capturing one (its state must not be made in the graph)")
+            m, v = _STATE_DTYPES[bits]
+            st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            st["exp_avg"] = torch.zeros_like(p, dtype=m)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=v)
+            if bits == 8:
+                n = -(-p.numel() // ops.ADAMW_BLOCK)
+                st["exp_avg_scale"] = torch.zeros(n, dtype=torch.float32, device=p.device)
+                st["exp_avg_sq_scale"] = torch.zeros(n, dtype=torch.float32, device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work, all_grads = [], []
+        for group in self.param_groups:
+            bits = group["state_bits"]
+            lists: dict = {}  # by device and dtype: (params, grads, m, v, m scales, v scales, steps)
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("AdamW: sparse grads are not supported")
+                if g.dtype != p.dtype:
+                    raise RuntimeError(f"AdamW: a grad of {g.dtype} for a parameter of {p.dtype}")
+                if g.stride() != p.stride():  # the parameter's order in memory
+                    g = torch.empty_like(p).copy_(g)
+                st = self._state_of(p, bits)
+                key = (p.device, p.dtype)
+                to = lists.get(key)
+                if to is None:
+                    to = lists[key] = ([], [], [], [], [], [], [])
+                to[0].append(p)
+                to[1].append(g)
+                to[2].append(st["exp_avg"])
+                to[3].append(st["exp_avg_sq"])
+                if bits == 8:
+                    to[4].append(st["exp_avg_scale"])
+                    to[5].append(st["exp_avg_sq_scale"])
+                to[6].append(st["step"])
+                all_grads.append(g)
+            if lists:
+                work.append((group, lists))
+        clip = None
+        if self.max_grad_norm is not None and all_grads:
+            norm = ops.grad_norm(all_grads, self.max_grad_norm)
+            self.grad_norm, clip = norm[0], norm[1]
+        for group, lists in work:
+            lr = group["lr"]
+            if isinstance(lr, torch.Tensor) and not lr.is_cuda:
+                lr = float(lr)
+            b1, b2 = group["betas"]
+            for to in lists.values():
+                ops.adamw_(*to, group["state_bits"], lr, b1, b2, group["eps"], group["weight_decay"], clip)
+                torch.autograd.graph.increment_version(to[0])
+        return loss
+
+    @torch.no_grad()
+    def moments(self) -> list:
+        """(first, second) moment of every parameter, in the groups' order, as float32 values of its shape: the state itself
+        where it has 32 bits, what the bytes stand for where it has 8, zeros before a first step."""
+        out, codes, scales, second, at = [], [], [], [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                st = self.state.get(p)
+                if not st:
+                    out.append(tuple(torch.zeros_like(p, dtype=torch.float32) for _ in range(2)))
+                elif st["exp_avg"].dtype == torch.float32:
+                    out.append((st["exp_avg"], st["exp_avg_sq"]))
+                else:
+                    at.append(len(out))
+                    out.append(None)
+                    codes += [st["exp_avg"], st["exp_avg_sq"]]
+                    scales += [st["exp_avg_scale"], st["exp_avg_sq_scale"]]
+                    second += [False, True]
+        values = ops.adamw_moments(codes, scales, second) if codes else []
+        for i, k in enumerate(at):
+            out[k] = values[2 * i], values[2 * i + 1]
+        return out
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, with the state's own types kept (torch casts a state to its parameter's); a torch AdamW's state
+        loads too, its moments in float32."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        groups = [(g, p) for g in self.param_groups for p in g["params"]]
+        for i, (g, p) in zip(ids, groups):
+            if i not in saved:
+                continue
+            m, v = _STATE_DTYPES[g["state_bits"]]
+            src, st = saved[i], {}
+            st["step"] = torch.as_tensor(src["step"]).to(dtype=torch.float32, device=p.device, copy=True).reshape(())
+            for name, dtype in (("exp_avg", m), ("exp_avg_sq", v)):
+                t = src[name]
+                if t.shape != p.shape or t.is_floating_point() != (dtype == torch.float32) \
+                        or (dtype != torch.float32 and t.dtype != dtype):
+                    raise ValueError(f"AdamW: {name} of {t.dtype} and shape {tuple(t.shape)} does not fit a parameter of "
+                                     f"shape {tuple(p.shape)} with moments in {g['state_bits']} bits")
+                st[name] = torch.empty_like(p, dtype=dtype)
+                if g["state_bits"] == 8 and not (t.is_contiguous() and p.is_contiguous()) \
+                        and t.stride() != st[name].stride():  # blocks are of elements next to each other in memory
+                    raise ValueError(f"AdamW: 8-bit {name} of strides {t.stride()} for a parameter of strides {p.stride()}")
+                st[name].copy_(t)
+            if g["state_bits"] == 8:
+                for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                    st[name] = src[name].to(dtype=torch.float32, device=p.device, copy=True)
+            self.state[p] = st

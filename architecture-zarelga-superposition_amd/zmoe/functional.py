@@ -265,3 +265,91 @@ def norm_residual(residual: torch.Tensor, y: torch.Tensor, weight: Optional[torc
     r, x = _NormResidual.apply(residual.reshape(-1, d), y.reshape(-1, d), weight, next_weight, gate, kind, scale, value,
                                float(eps))
     return r.view(residual.shape), None if x is None else x.view(y.shape)
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, k: int, score: int, groups: int, top_groups: int, group_scores: int,
+                renormalize: bool, scale: float):
+        idx, w, p = zl.route(logits, bias, k, score, groups, top_groups, group_scores, renormalize, scale)
+        ctx.save_for_backward(p, idx, logits)
+        ctx.form = score, renormalize, scale
+        ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
+        return idx, w
+
+    @staticmethod
+    def backward(ctx, d_idx, d_weight):
+        if d_weight is None:
+            return (None,) * 9
+        p, idx, logits = ctx.saved_tensors
+        return (zl.route_backward(d_weight, p, idx, logits, *ctx.form), *(None,) * 8)
+
+
+def _score(score: str) -> int:
+    if score not in _z.SCORES:
+        raise ValueError(f"score must be one of {sorted(_z.SCORES)}, got {score!r}")
+    return _z.SCORES[score]
+
+
+def route(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, score: str = "sigmoid", groups: int = 1,
+          top_groups: int = 1, group_scores: int = 2, renormalize: bool = True, scale: float = 1.0):
+    """The k experts of each token and their weights, from the router's logits [..., E] (bfloat16 or float32, E <= 1024):
+    (idx int64, weight float32), both [..., k].
+
+    p = sigmoid(logits) or softmax(logits), rounded once to float32; experts rank by p + ``bias`` ([E], float32; it takes
+    part in the selection only), without one by their logits. ``groups`` > 1: experts lie in that many groups of E / groups,
+    of which the ``top_groups`` with the highest score stay, a group's score being the sum of its two best experts'
+    (``group_scores`` 2) or the best one's (1). Slots come best first, equal experts by their number, NaN first. Weights are
+    ``scale`` p / max(sum p, 1e-12) over a token's k, without ``renormalize`` ``scale`` p. Gradients reach the logits through
+    the weights. A row of -inf alone has p = 0."""
+    if logits.dim() < 1:
+        raise ValueError("route: logits must be [..., E]")
+    if bias is not None:
+        if _needs_graph(bias):
+            raise RuntimeError("route: the bias takes no gradient")
+        bias = bias.float()
+    code, scale, E = _score(score), float(scale), logits.shape[-1]
+    group_scores = group_scores if groups > 1 else 1
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, E)
+    args = (flat, bias, int(k), code, int(groups), int(top_groups), int(group_scores), bool(renormalize), scale)
+    if _needs_graph(logits):
+        idx, w = _Route.apply(*args)
+    else:
+        with torch.no_grad():
+            idx, w, _ = zl.route(*args)
+    if logits.dim() == 2:
+        return idx, w
+    return idx.view(*logits.shape[:-1], k), w.view(*logits.shape[:-1], k)
+
+
+class _RouterLosses(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, topk_idx, cu_seqlens, score: int):
+        losses, grad, inv = zl.router_losses(logits, topk_idx, cu_seqlens, score)
+        ctx.save_for_backward(logits, cu_seqlens, grad, inv)
+        ctx.score = score
+        ctx.set_materialize_grads(False)
+        return losses[0], losses[1]
+
+    @staticmethod
+    def backward(ctx, d_balance, d_z):
+        if d_balance is None and d_z is None:
+            return (None,) * 4
+        logits, cu, grad, inv = ctx.saved_tensors
+        return zl.router_losses_backward(d_balance, d_z, logits, cu, ctx.score, grad, inv), None, None, None
+
+
+def router_losses(logits: torch.Tensor, topk_idx: torch.Tensor, score: str = "sigmoid",
+                  cu_seqlens: Optional[torch.Tensor] = None):
+    """The router's balance loss and z loss (float32 numbers on the device), with gradients for the logits.
+
+    ``logits`` [..., E] and the experts chosen from them, ``topk_idx`` [..., k], over T tokens; ``cu_seqlens`` ([S + 1] int32
+    or int64 on the device, not decreasing): sequence s is the tokens cu[s] to cu[s + 1], others take no part; None: one
+    sequence. With f_se = E / (k n_s) times the choices of expert e in sequence s of n_s tokens, and P_se the mean over the
+    sequence of p_e / sum p (p the ``score`` of the logits): balance = mean over sequences with tokens of sum_e f_se P_se,
+    1 for even routing; z = mean over tokens of logsumexp(logits)^2. The choices take no gradient."""
+    E, code = logits.shape[-1], _score(score)
+    flat = logits.reshape(-1, E)
+    idx = topk_idx.reshape(-1, topk_idx.shape[-1])
+    return _RouterLosses.apply(flat, idx, cu_seqlens, code)

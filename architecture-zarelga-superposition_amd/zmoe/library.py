@@ -152,6 +152,75 @@ def _(d_weight, topk_prob, topk_idx, num_experts, like):
     return _empty((topk_idx.shape[0], num_experts), like)
 
 
+@layer_op("route")
+def route(logits: torch.Tensor, expert_biases: Optional[torch.Tensor], k: int, score: int, groups: int, top_groups: int,
+          group_scores: int, renormalize: bool, scale: float) -> List[torch.Tensor]:
+    """Routing in its other forms: [idx int64, weight f32, prob f32], each [T, k]."""
+    return list(_z.route(logits, expert_biases, k, score, groups, top_groups, group_scores, renormalize, scale))
+
+
+@route.register_fake
+def _(logits, expert_biases, k, score, groups, top_groups, group_scores, renormalize, scale):
+    T = logits.shape[0]
+    return [_empty((T, k), logits, _I64), _empty((T, k), logits, _F32), _empty((T, k), logits, _F32)]
+
+
+@layer_op("route_backward")
+def route_backward(d_weight: torch.Tensor, topk_prob: torch.Tensor, topk_idx: torch.Tensor, logits: torch.Tensor,
+                   score: int, renormalize: bool, scale: float) -> torch.Tensor:
+    """d_logits [T, E] in the logits' type."""
+    return _z.route_backward(d_weight, topk_prob, topk_idx, logits.shape[1], logits, score, renormalize, scale,
+                             logits.dtype)
+
+
+@route_backward.register_fake
+def _(d_weight, topk_prob, topk_idx, logits, score, renormalize, scale):
+    return _empty(logits.shape, logits)
+
+
+@layer_op("swiglu_route_form_backward")
+def swiglu_route_form_backward(dAs: torch.Tensor, Hs: torch.Tensor, d_gates: torch.Tensor, topk_prob: torch.Tensor,
+                               topk_idx: torch.Tensor, logits: torch.Tensor, score: int, renormalize: bool, scale: float,
+                               add: Optional[torch.Tensor]) -> torch.Tensor:
+    """``swiglu_route_backward`` for ``route``'s forms; ``add``: what the router's losses give the logits."""
+    (T, two_f), E = Hs.shape, logits.shape[1]
+    G = torch.empty((T, two_f + E), dtype=Hs.dtype, device=Hs.device)
+    _z.swiglu_backward(dAs, Hs, out=G[:, :two_f])
+    _z.route_backward(d_gates, topk_prob, topk_idx, E, logits, score, renormalize, scale, Hs.dtype, add, out=G[:, two_f:])
+    return G
+
+
+@swiglu_route_form_backward.register_fake
+def _(dAs, Hs, d_gates, topk_prob, topk_idx, logits, score, renormalize, scale, add):
+    return _empty((Hs.shape[0], Hs.shape[1] + logits.shape[1]), Hs)
+
+
+@layer_op("router_losses")
+def router_losses(logits: torch.Tensor, topk_idx: torch.Tensor, cu_seqlens: Optional[torch.Tensor],
+                  score: int) -> List[torch.Tensor]:
+    """[losses [2] f32 (balance, z), seq_grad [S, E] f32, inv_tokens [1] f32]."""
+    return list(_z.router_losses(logits, topk_idx, cu_seqlens, score))
+
+
+@router_losses.register_fake
+def _(logits, topk_idx, cu_seqlens, score):
+    S = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    return [_empty((2,), logits, _F32), _empty((S, logits.shape[1]), logits, _F32), _empty((1,), logits, _F32)]
+
+
+@layer_op("router_losses_backward")
+def router_losses_backward(d_balance: Optional[torch.Tensor], d_z: Optional[torch.Tensor], logits: torch.Tensor,
+                           cu_seqlens: Optional[torch.Tensor], score: int, seq_grad: torch.Tensor,
+                           inv_tokens: torch.Tensor) -> torch.Tensor:
+    """d_logits [T, E] in the logits' type."""
+    return _z.router_losses_backward(d_balance, d_z, logits, cu_seqlens, score, seq_grad, inv_tokens)
+
+
+@router_losses_backward.register_fake
+def _(d_balance, d_z, logits, cu_seqlens, score, seq_grad, inv_tokens):
+    return _empty(logits.shape, logits)
+
+
 # ------------------------------------------------------------------ sort
 @layer_op("flatten_sort_count")
 def flatten_sort_count(expert_idxs: torch.Tensor, num_experts: int) -> List[torch.Tensor]:

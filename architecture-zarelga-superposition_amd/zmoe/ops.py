@@ -174,6 +174,114 @@ def route_topk_backward(d_weight: torch.Tensor, topk_prob: torch.Tensor, topk_id
     return out
 
 
+SCORES = {"sigmoid": 0, "softmax": 1}
+
+
+def route(logits: torch.Tensor, expert_biases: Optional[torch.Tensor], k: int, score: int, groups: int, top_groups: int,
+          group_scores: int, renormalize: bool, scale: float):
+    """zmoe_route on logits [T, E] -> (idx, weight, prob) [T, k]; ``score`` 0 sigmoid, 1 softmax."""
+    dev = _require_cuda(logits, expert_biases)
+    if logits.dim() != 2:
+        raise ValueError(f"route: logits must be [T, E], got {tuple(logits.shape)}")
+    logits = logits.contiguous()
+    T, E = logits.shape
+    bias = None
+    if expert_biases is not None:
+        bias = expert_biases.to(torch.float32).contiguous()
+        if bias.numel() != E:
+            raise ValueError(f"route: the bias must have E = {E} entries")
+    dt = _dtype_code(logits)
+    idx = torch.empty((T, max(k, 0)), dtype=torch.int64, device=dev)
+    w, p = (torch.empty((T, max(k, 0)), dtype=torch.float32, device=dev) for _ in range(2))
+    with torch.cuda.device(dev), profiling.region("route", dev):
+        L.call("zmoe_route", _ptr(logits), dt, T, E, k, score, _ptr(bias), groups, top_groups, group_scores,
+               int(renormalize), float(scale), _ptr(idx), _ptr(w), _ptr(p), _stream(dev))
+    return idx, w, p
+
+
+def route_backward(d_weight: torch.Tensor, topk_prob: torch.Tensor, topk_idx: torch.Tensor, num_experts: int,
+                   logits: Optional[torch.Tensor], score: int, renormalize: bool, scale: float, dtype: torch.dtype,
+                   add: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """d_logits [T, E] of ``dtype`` (``add``, of the same, added before its rounding); ``out`` may be a column slice of a
+    wider row-major buffer. ``logits`` (of ``dtype``): softmax scores need them."""
+    dev = _require_cuda(d_weight, topk_prob, topk_idx, logits, add, out)
+    T, k = topk_idx.shape
+    E = num_experts
+    dw, p = d_weight.to(torch.float32).contiguous(), topk_prob.to(torch.float32).contiguous()
+    if dw.shape != (T, k) or p.shape != (T, k) or topk_idx.dtype != torch.int64:
+        raise ValueError("route_backward: d_weight, topk_prob and topk_idx (int64) must be [T, k]")
+    if dtype not in _DT:
+        raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+    for t in (logits, add):
+        if t is not None and (t.shape != (T, E) or t.dtype != dtype):
+            raise ValueError(f"route_backward: logits and add must be [T, E] of {dtype}")
+    logits = None if logits is None else logits.contiguous()
+    add = None if add is None else _rows_apart(add)
+    if out is None:
+        out = torch.empty((T, E), dtype=dtype, device=dev)
+    elif out.shape != (T, E) or out.dtype != dtype or (E > 1 and out.stride(1) != 1):
+        raise ValueError("route_backward: out must be [T, E] of the logits dtype with unit column stride")
+    idx = topk_idx.contiguous()
+    with torch.cuda.device(dev), profiling.region("route_backward", dev):
+        L.call("zmoe_route_backward", _ptr(dw), _ptr(p), _ptr(idx), T, E, k, score, _ptr(logits), int(renormalize),
+               float(scale), _ptr(add), 0 if add is None else max(add.stride(0), E), _ptr(out), max(out.stride(0), E),
+               _DT[dtype], _stream(dev))
+    return out
+
+
+def _cu(cu_seqlens: Optional[torch.Tensor]):
+    """(borders, whether they are int64, their number of sequences)"""
+    if cu_seqlens is None:
+        return None, 0, 1
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise ValueError("router_losses: cu_seqlens must be [S + 1] of int32 or int64, S >= 1")
+    return cu_seqlens.contiguous(), int(cu_seqlens.dtype == torch.int64), cu_seqlens.numel() - 1
+
+
+def router_losses(logits: torch.Tensor, topk_idx: torch.Tensor, cu_seqlens: Optional[torch.Tensor], score: int):
+    """zmoe_router_losses (``cu_seqlens`` None: one sequence of all tokens): (losses [2] f32: balance and z, seq_grad [S, E]
+    f32, inv_tokens [1] f32)."""
+    dev = _require_cuda(logits, topk_idx, cu_seqlens)
+    if logits.dim() != 2 or topk_idx.dim() != 2 or topk_idx.shape[0] != logits.shape[0]:
+        raise ValueError(f"router_losses: logits [T, E] and topk_idx [T, k], got {tuple(logits.shape)} and "
+                         f"{tuple(topk_idx.shape)}")
+    logits = logits.contiguous()
+    cu, wide, S = _cu(cu_seqlens)
+    idx = topk_idx.to(torch.int64).contiguous()
+    T, E = logits.shape
+    dt = _dtype_code(logits)
+    losses, grad, inv = (torch.empty(n, dtype=torch.float32, device=dev) for n in (2, (S, E), 1))
+    nbytes = L.load().zmoe_router_losses_workspace_bytes(T, E, S)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev), profiling.region("router_losses", dev):
+        L.call("zmoe_router_losses", _ptr(logits), dt, T, E, _ptr(idx), idx.shape[1], score, _ptr(cu),
+               wide, S, _ptr(losses), _ptr(grad), _ptr(inv), _ptr(ws), ws.numel(), _stream(dev))
+    return losses, grad, inv
+
+
+def router_losses_backward(d_balance: Optional[torch.Tensor], d_z: Optional[torch.Tensor], logits: torch.Tensor,
+                           cu_seqlens: Optional[torch.Tensor], score: int, seq_grad: torch.Tensor,
+                           inv_tokens: torch.Tensor) -> torch.Tensor:
+    """d_logits [T, E] of the logits' type; the losses' grads are one f32 number each on the device, or None."""
+    dev = _require_cuda(logits, cu_seqlens, seq_grad, inv_tokens, d_balance, d_z)
+    logits = logits.contiguous()
+    cu, wide, S = _cu(cu_seqlens)
+    T, E = logits.shape
+    one = lambda g: None if g is None else g.to(torch.float32).contiguous()  # noqa: E731
+    gb, gz = one(d_balance), one(d_z)
+    if any(g is not None and g.numel() != 1 for g in (gb, gz)):
+        raise ValueError("router_losses_backward: a loss's grad is one number")
+    if seq_grad.shape != (S, E) or seq_grad.dtype != torch.float32 or not seq_grad.is_contiguous() \
+            or inv_tokens.numel() != 1 or inv_tokens.dtype != torch.float32:
+        raise ValueError("router_losses_backward: seq_grad [S, E] and inv_tokens [1] of the forward, f32")
+    dt = _dtype_code(logits)
+    out = torch.empty((T, E), dtype=logits.dtype, device=dev)
+    with torch.cuda.device(dev), profiling.region("router_losses_backward", dev):
+        L.call("zmoe_router_losses_backward", _ptr(logits), dt, T, E, score, _ptr(cu), wide, S,
+               _ptr(seq_grad), _ptr(inv_tokens), _ptr(gb), _ptr(gz), _ptr(out), _stream(dev))
+    return out
+
+
 # --------------------------------------------------------------------- sort
 def bincount(expert_idxs: torch.Tensor, num_experts: int) -> torch.Tensor:
     dev = _require_cuda(expert_idxs)
@@ -1159,3 +1267,87 @@ def newton_schulz5(G: torch.Tensor, steps: int, coeffs=NS_COEFFS) -> torch.Tenso
     if tall:
         X = X.transpose(1, 2)
     return X.reshape(G.shape)
+
+
+# --------------------------------------------------------------------- the optimizer's step
+ADAMW_BLOCK = 256  # elements of an 8-bit moment with one scale
+
+
+def grad_norm(grads, max_norm: float) -> torch.Tensor:
+    """[norm, min(1, max_norm / (norm + 1e-6))] f32 of a list of dense bf16 or f32 tensors' common 2-norm
+    (zmoe_sum_squares, zmoe_clip_factor): squares summed in double, in a fixed order."""
+    dev = _require_cuda(*grads)
+    lib = L.load()
+    parts_of = lambda some: sum(lib.zmoe_sum_squares_workspace_bytes(g.numel()) for g in some) // 8  # noqa: E731
+    parts = torch.empty(max(1, parts_of(grads)), dtype=torch.float64, device=dev)
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    at = 0
+    with torch.cuda.device(dev), profiling.region("grad_norm", dev):
+        for dtype, code in _DT.items():
+            some = [g for g in grads if g.dtype == dtype and g.numel()]
+            if some:
+                n = len(some)
+                L.call("zmoe_sum_squares", (L.P * n)(*[g.data_ptr() for g in some]),
+                       (L.I64 * n)(*[g.numel() for g in some]), n, code, parts.data_ptr() + 8 * at, _stream(dev))
+                at += parts_of(some)
+        L.call("zmoe_clip_factor", _ptr(parts), at, float(max_norm), _ptr(out), _stream(dev))
+    return out
+
+
+def adamw_(params, grads, exp_avgs, exp_avg_sqs, avg_scales, sq_scales, steps, state_bits: int, lr, beta1: float,
+           beta2: float, eps: float, weight_decay: float, clip: Optional[torch.Tensor] = None) -> None:
+    """One AdamW step in place over lists of tensors of one dtype (zmoe_adamw): each tensor, its grad and its moments lie
+    in the same order in memory, without gaps. ``avg_scales``, ``sq_scales``: empty lists with ``state_bits`` 32. ``lr``: a
+    number, or an f32 tensor of one element on the device. ``clip``: such a tensor, which the grads are multiplied by."""
+    n = len(params)
+    if n == 0:
+        return
+    eight = state_bits == 8
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(steps) == n
+            and (not eight or len(avg_scales) == len(sq_scales) == n)):
+        raise ValueError("adamw: lists of different lengths")
+    lr_t = lr if isinstance(lr, torch.Tensor) else None
+    dev = _require_cuda(*params, *grads, *exp_avgs, *exp_avg_sqs, *avg_scales, *sq_scales, *steps, lr_t, clip)
+    dtype = params[0].dtype
+    if dtype not in _DT:
+        raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+    of_m, of_v = (torch.int8, torch.uint8) if eight else (torch.float32, torch.float32)
+    table = (L.AdamwTensor * n)()
+    for i, (p, g, m, v, t) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs, steps)):
+        size = p.numel()
+        if (p.dtype != dtype or g.dtype != dtype or m.dtype != of_m or v.dtype != of_v or t.dtype != torch.float32
+                or g.numel() != size or m.numel() != size or v.numel() != size or t.numel() != 1):
+            raise ValueError(f"adamw: tensor {i}: parameters and grads of one dtype, moments of {of_m} and {of_v} and an "
+                             "f32 step count, of the same size")
+        a, b = (avg_scales[i], sq_scales[i]) if eight else (None, None)
+        if eight and any(s.dtype != torch.float32 or s.numel() != -(-size // ADAMW_BLOCK) or not s.is_contiguous()
+                         for s in (a, b)):
+            raise ValueError(f"adamw: tensor {i}: scales must be f32, one for each {ADAMW_BLOCK} elements")
+        e = table[i]
+        e.param, e.grad, e.exp_avg, e.exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
+        e.scale_avg, e.scale_sq, e.step, e.n = _ptr(a), _ptr(b), t.data_ptr(), size
+    for x in (lr_t, clip):
+        if x is not None and (x.dtype != torch.float32 or x.numel() != 1):
+            raise ValueError("adamw: lr and clip are f32 tensors of one element")
+    ws = torch.empty(4 * n, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev), profiling.region("adamw", dev):
+        L.call("zmoe_adamw", table, n, _DT[dtype], state_bits, _ptr(lr_t), 0.0 if lr_t is not None else float(lr), beta1,
+               beta2, eps, weight_decay, _ptr(clip), _ptr(ws), 16 * n, _stream(dev))
+
+
+def adamw_moments(codes, scales, second) -> list:
+    """8-bit moments in f32 (zmoe_adamw_moments): for each tensor of codes its values, of the same shape and strides;
+    ``second``: whether it is a second moment's."""
+    dev = _require_cuda(*codes, *scales)
+    out = [torch.empty_like(c, dtype=torch.float32) for c in codes]
+    table = (L.Moment * len(codes))()
+    for e, c, s, v, o in zip(table, codes, scales, second, out):
+        if c.dtype != (torch.uint8 if v else torch.int8) or s.dtype != torch.float32 \
+                or s.numel() != -(-c.numel() // ADAMW_BLOCK) or o.stride() != c.stride():
+            raise ValueError("adamw_moments: codes without gaps and an f32 scale for each "
+                             f"{ADAMW_BLOCK} of them")
+        e.codes, e.scale, e.out, e.n, e.second = c.data_ptr(), s.data_ptr(), o.data_ptr(), c.numel(), int(v)
+    if codes:
+        with torch.cuda.device(dev), profiling.region("adamw_moments", dev):
+            L.call("zmoe_adamw_moments", table, len(codes), _stream(dev))
+    return out

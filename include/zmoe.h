@@ -523,6 +523,97 @@ int zmoe_norm_residual_backward(const void* dR_out, const void* dX, const void* 
                                 const float* rstd_next, void* dR, void* dY, void* dw_post, void* dw_next, void* dgate,
                                 float* dscale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Routing in its other forms (the gate of modeling/moe_gate.py:27-34 with what it leaves open):
+ *   p = sigmoid(z) or softmax(z), rounded once to f32 (0 in a row of -inf alone; the sigmoid as in zmoe_route_topk)
+ *   s = p + expert_biases in f32; without biases (NULL) experts rank by their logits
+ *   experts lie in `groups` (1 to 64) groups of E / groups; a group's score is its highest s, or (group_scores 2) the f32
+ *   sum of its two highest (p's without biases); the top_groups best groups stay (equal ones by their number)
+ *   topk_idx: the k (<= 64) best s among their experts, s descending, equal ones by their number, NaN first
+ *   topk_weight = scale p / max(sum p, 1e-12) with `renormalize`, else scale p;  topk_prob = p (may be NULL)
+ * logits [T, E] packed, 1 <= E <= 1024.
+ * ------------------------------------------------------------------------- */
+enum { ZMOE_SCORE_SIGMOID = 0, ZMOE_SCORE_SOFTMAX = 1 };
+
+int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E, int k, int score, const float* expert_biases,
+               int groups, int top_groups, int group_scores, int renormalize, float scale, int64_t* topk_idx,
+               float* topk_weight, float* topk_prob, void* stream);
+
+/* Its gradient by the logits, from d_weight [T, k] f32: d_logits [T, E], rows ld_d_logits >= E apart; `add` (or NULL), of
+ * the same type with rows ld_add apart, is added before the one rounding (the losses' gradient). `logits` (type of
+ * d_logits, packed) are needed for softmax scores. Selection and biases have no gradient. */
+int zmoe_route_backward(const float* d_weight, const float* topk_prob, const int64_t* topk_idx, int64_t T, int E, int k,
+                        int score, const void* logits, int renormalize, float scale, const void* add, int64_t ld_add,
+                        void* d_logits, int64_t ld_d_logits, int d_logits_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The router's losses over S sequences of tokens, cu_seqlens[s] .. cu_seqlens[s + 1] (int32, or int64 with cu_int64; on
+ * the device; not decreasing; values are cut to [0, T]; NULL with S = 1: all T tokens); tokens outside take no part:
+ *   ph = p / sum_e p with p = sigmoid(z) or softmax(z);  n_s tokens, c_se choices of e in s, S' sequences with tokens
+ *   losses[0] = 1/S' sum_s sum_e (E c_se / (k n_s)) (sum_t ph_te / n_s)       balance of each sequence
+ *   losses[1] = 1/N sum_t logsumexp(z_t)^2                                      over all N tokens
+ * (0 without tokens; a token whose p are all 0 adds nothing to the balance, one of -inf alone nothing to either).
+ * topk_idx [T, k]; ids outside [0, E) are not counted. seq_grad [S, E] f32 and inv_tokens [1] f32 are what the backward
+ * takes. Sums in a fixed order.
+ * ------------------------------------------------------------------------- */
+#define ZMOE_ROUTER_LOSSES_MAX_SEQUENCES (1 << 20)
+size_t zmoe_router_losses_workspace_bytes(int64_t T, int E, int64_t S);
+int zmoe_router_losses(const void* logits, int logits_dtype, int64_t T, int E, const int64_t* topk_idx, int k, int score,
+                       const void* cu_seqlens, int cu_int64, int64_t S, float* losses, float* seq_grad, float* inv_tokens,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* d_logits [T, E] packed, of the logits' type, from the losses' grads d_balance and d_z (f32 on the device, either may be
+ * NULL: 0); zeros outside the sequences. The choices have no gradient. */
+int zmoe_router_losses_backward(const void* logits, int logits_dtype, int64_t T, int E, int score, const void* cu_seqlens,
+                                int cu_int64, int64_t S, const float* seq_grad, const float* inv_tokens,
+                                const float* d_balance, const float* d_z, void* d_logits, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * An AdamW step over many tensors (the reference's auxiliary Adam, optimizer/muon.py:574-653, over what Newton-Schulz
+ * leaves), in f32 with one rounding of the parameter:
+ *   g' = clip g;  m' = b1 m + (1 - b1) g';  v' = b2 v + (1 - b2) g'^2
+ *   p' = p - lr wd p - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps),   t = *step + 1, written back
+ * Arrays of n elements each, param and grad of `dtype`. state_bits 32: exp_avg and exp_avg_sq f32. 8: a byte an element
+ * and a scale (f32, a block's largest magnitude A) for each 256 of them, [ceil(n / 256)]:
+ *   m = sign(q) q^2 A / 127^2 (int8), v = q^4 A / 255^4 (uint8), rounded to f32; nearest codes, half-way ones up, v > 0
+ *   at least 1. A moment that is not finite makes its block's moments NaN.
+ * lr: *lr_ptr (device) or, where that is NULL, `lr`. clip: a factor on the device, or NULL. workspace: 16 bytes a tensor.
+ * Tensor descriptions are read before the call returns. A tensor must not be given twice.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scale_avg; /* 8 bits only */
+  float* scale_sq;
+  float* step; /* steps taken, 1 element */
+  int64_t n;
+} zmoe_adamw_tensor;
+
+int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype, int state_bits, const float* lr_ptr, double lr,
+               double beta1, double beta2, double eps, double weight_decay, const float* clip, float* workspace,
+               size_t workspace_bytes, void* stream);
+
+/* 8-bit moments as the f32 values that they stand for. */
+typedef struct {
+  const void* codes;
+  const float* scale;
+  float* out;
+  int64_t n;
+  int second; /* 0: m, 1: v */
+} zmoe_moment;
+
+int zmoe_adamw_moments(const zmoe_moment* moments, int count, void* stream);
+
+/* Sums of squares, in double, of a list's tensors: one part for each started chunk of a tensor, one tensor after the
+ * other; zmoe_sum_squares_workspace_bytes: what the parts of a tensor of n elements take (8 bytes each). */
+size_t zmoe_sum_squares_workspace_bytes(int64_t n);
+int zmoe_sum_squares(const void* const* tensors, const int64_t* n, int count, int dtype, double* parts, void* stream);
+
+/* norm_and_factor[0] = the root of the parts' sum, [1] = min(1, max_norm / (norm + 1e-6)). */
+int zmoe_clip_factor(const double* parts, int64_t count, float max_norm, float* norm_and_factor, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
