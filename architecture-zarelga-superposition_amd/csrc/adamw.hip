@@ -19,7 +19,7 @@
 // pointers travel in the launches' arguments, so nothing is copied to the device and a graph keeps them.
 #include <type_traits>
 
-#include "zmoe_internal.h"
+#include "zmoe_route.h"  // wave_max_u32
 
 namespace zmoe {
 namespace {
@@ -40,8 +40,8 @@ struct Table {
 };
 
 struct Hyper {
-  double b1, b2;
-  float b1f, b2f, c1f, c2f, eps;  // c = 1 - b
+  double b1, b2, c1, c2;  // c = 1 - b
+  float b1f, b2f, c1f, c2f, eps;
 };
 
 // The tensor that a launch's chunk belongs to.
@@ -92,45 +92,89 @@ __device__ __forceinline__ float blend(double x, double a, double y, double b) {
   return (float)(xa + yb);
 }
 
-__device__ __forceinline__ float value2(int q, double unit) {  // q signed, unit = A / 127^2
-  const float v = (float)((double)(q * q) * unit);
-  return q < 0 ? -v : v;
-}
-__device__ __forceinline__ float value4(uint32_t q, double unit) {  // unit = A / 255^4
-  const uint32_t q2 = q * q;
-  return (float)((double)(q2 * q2) * unit);
+// The f32 values of codes: sign q^2 unit, q^4 unit (q^4 as a square in double: exact).
+__device__ __forceinline__ float value2(int q, double unit) { return (float)((double)(q * abs(q)) * unit); }
+__device__ __forceinline__ float value4(uint32_t q, double unit) {
+  const double q2 = (double)(q * q);
+  return (float)(q2 * q2 * unit);
 }
 
-// inv = 1 / A, 0 for A = 0
-__device__ __forceinline__ int code2(float x, double A, double inv) {
-  const double mag = (double)fabsf(x);
-  int q = (int)(sqrtf((float)(mag * inv)) * 127.f + 0.5f);
+// A code's place in the root's domain, + 1/2: the code is its whole part, unless that lies within kNear2 or kNear4 of a
+// border. The estimate has a reciprocal, a product, one or two roots and a product of f32, 2.4 roundings of 2^-23 at most
+// in the root: 127 (255) of those and the last sum's own are 4.0e-5 (8.1e-5).
+constexpr float kNear2 = 0x1p-14f, kNear4 = 0x1p-13f;
+__device__ __forceinline__ float place2(float mag, float inv) {
+  return fmaf(__builtin_amdgcn_sqrtf(mag * inv), (float)kTop2, 0.5f);
+}
+__device__ __forceinline__ float place4(float mag, float inv) {
+  return fmaf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(mag * inv)), (float)kTop4, 0.5f);
+}
+
+// The code itself: an estimate to one code or better, set right by the borders on its two sides.
+__device__ __forceinline__ int exact2(float mag, double A) {
+  const double x = (double)mag;
+  int q = A > 0.0 ? (int)(sqrtf((float)(x / A)) * 127.f + 0.5f) : 0;
   q = min(max(q, 0), kTop2);
-  const double at = mag * (4.0 * 127.0 * 127.0);
+  const double at = x * (4.0 * kDiv2);
   const int l = 2 * q - 1, h = 2 * q + 1;
-  q += (int)(q < kTop2 && (double)(h * h) * A <= at && A > 0.0) - (int)(q > 0 && (double)(l * l) * A > at);
-  return x < 0.f ? -q : q;
+  return q + (int)(q < kTop2 && (double)(h * h) * A <= at && A > 0.0) - (int)(q > 0 && (double)(l * l) * A > at);
 }
-__device__ __forceinline__ uint32_t code4(float x, double A, double inv) {
-  const double mag = (double)x;
-  int q = (int)(sqrtf(sqrtf((float)(mag * inv))) * 255.f + 0.5f);
+__device__ __forceinline__ int exact4(float mag, double A) {
+  const double x = (double)mag;
+  int q = A > 0.0 ? (int)(sqrtf(sqrtf((float)(x / A))) * 255.f + 0.5f) : 0;
   q = min(max(q, 0), kTop4);
-  const double at = mag * (16.0 * 255.0 * 255.0 * 255.0 * 255.0);
+  const double at = x * (16.0 * kDiv4);
   const double l = (double)((2 * q - 1) * (2 * q - 1)), h = (double)((2 * q + 1) * (2 * q + 1));
-  q += (int)(q < kTop4 && h * h * A <= at && A > 0.0) - (int)(q > 0 && l * l * A > at);
-  return q == 0 && x > 0.f ? 1u : (uint32_t)q;
+  return q + (int)(q < kTop4 && h * h * A <= at && A > 0.0) - (int)(q > 0 && l * l * A > at);
 }
 
-__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+// The codes of a lane's four elements of each moment (v > 0 at least 1), the bytes of a dword each. Blocks whose largest
+// magnitude has no f32 reciprocal (or is not finite) take the exact way for all.
+__device__ __forceinline__ void encode(const float (&m)[4], const float (&v)[4], float Am, float Av, uint32_t& qm,
+                                       uint32_t& qv) {
+  const bool plain_m = Am >= 0x1p-100f && Am <= 0x1p100f, plain_v = Av >= 0x1p-100f && Av <= 0x1p100f;
+  const float im = plain_m ? __builtin_amdgcn_rcpf(Am) : 0.f, iv = plain_v ? __builtin_amdgcn_rcpf(Av) : 0.f;
+  int cm[4], cv[4];
+  bool near_m = !plain_m, near_v = !plain_v;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-  return v;
+  for (int e = 0; e < 4; ++e) {
+    const float y = place2(fabsf(m[e]), im), z = place4(v[e], iv);
+    const float fy = __builtin_amdgcn_fractf(y), fz = __builtin_amdgcn_fractf(z);
+    cm[e] = (int)y;
+    cv[e] = (int)z;
+    near_m |= fabsf(fy - 0.5f) > 0.5f - kNear2;
+    near_v |= fabsf(fz - 0.5f) > 0.5f - kNear4;
+  }
+  if (near_m) {  // one lane in two thousand
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cm[e] = exact2(fabsf(m[e]), (double)Am);
+  }
+  if (near_v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) cv[e] = exact4(v[e], (double)Av);
+  }
+  qm = qv = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    cm[e] = min(cm[e], kTop2);
+    cv[e] = min(max(cv[e], v[e] > 0.f ? 1 : 0), kTop4);
+    qm |= ((uint32_t)(m[e] < 0.f ? -cm[e] : cm[e]) & 0xffu) << (8 * e);
+    qv |= (uint32_t)cv[e] << (8 * e);
+  }
+}
+
+// sqrt and a quotient to 1.5 f32 roundings each (v_sqrt_f32 takes no subnormals; denominators here are none).
+__device__ __forceinline__ float root(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v);
+  return small ? r * 0x1p-16f : r;
 }
 
 // ------------------------------------------------------------------ elements
+// Four elements i .. i + 3 of n; vec: all of them there and on a whole vector (the same in a wave).
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float (&v)[4]) {
-  if (vec && i + 3 < n) {
+  if (vec) {
     if constexpr (sizeof(T) == 4) {
       const float4 x = *reinterpret_cast<const float4*>(p + i);
       v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
@@ -146,7 +190,7 @@ __device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec
 }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float (&v)[4]) {
-  if (vec && i + 3 < n) {
+  if (vec) {
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
     else *reinterpret_cast<uint2*>(p + i) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
   } else {
@@ -157,7 +201,7 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, con
 }
 // Four codes as the bytes of a dword.
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int64_t n, bool vec) {
-  if (vec && i + 3 < n) return *reinterpret_cast<const uint32_t*>(p + i);
+  if (vec) return *reinterpret_cast<const uint32_t*>(p + i);
   uint32_t c = 0;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
@@ -165,7 +209,7 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int6
   return c;
 }
 __device__ __forceinline__ void store_codes(uint8_t* p, int64_t i, int64_t n, bool vec, uint32_t c) {
-  if (vec && i + 3 < n) {
+  if (vec) {
     *reinterpret_cast<uint32_t*>(p + i) = c;
   } else {
 #pragma unroll
@@ -179,43 +223,38 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const 
                                                          const float4* __restrict__ coef) {
   const int which = owner_of(tab.start, tab.count, blockIdx.x);
   const zmoe_adamw_tensor& t = tab.t[which];
-  const bool vec = (tab.vec >> which) & 1;
+  const bool wide = (tab.vec >> which) & 1;
   const float4 c = coef[which];
   T* p = (T*)t.param;
   const T* g = (const T*)t.grad;
-  const int64_t n = t.n, chunk = blockIdx.x - tab.start[which];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t n = t.n;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
 #pragma unroll 2
   for (int u = 0; u < kBlocks / 4; ++u) {
-    const int64_t b = chunk * kBlocks + wave * (kBlocks / 4) + u, i = b * kBlock + lane * 4;
+    const int64_t b = first + u, i = b * kBlock + lane * 4;
     if (b * kBlock >= n) break;
+    const bool vec = wide && (b + 1) * kBlock <= n;
     float w[4], gr[4], m[4], v[4];
     load4(p, i, n, vec, w);
     load4(g, i, n, vec, gr);
     if constexpr (EIGHT) {
       const uint32_t cm = load_codes((const uint8_t*)t.exp_avg, i, n, vec);
       const uint32_t cv = load_codes((const uint8_t*)t.exp_avg_sq, i, n, vec);
-      const double um = unit2(t.scale_avg[b]), uv = unit4(t.scale_sq[b]);
+      const double um = unit2(t.scale_avg[b]), uv = unit4(t.scale_sq[b]), clip = (double)c.w;
       uint32_t top_m = 0, top_v = 0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const double gd = (double)gr[e] * (double)c.w;
-        m[e] = blend(h.b1, (double)value2((int)(int8_t)(cm >> (8 * e)), um), 1.0 - h.b1, gd);
-        v[e] = blend(h.b2, (double)value4((cv >> (8 * e)) & 0xffu, uv), 1.0 - h.b2, gd * gd);
-        if (i + e < n) {  // magnitudes order as their bits, NaN above all
-          top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
-          top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
-        }
+        const double gd = (double)gr[e] * clip;
+        m[e] = blend(h.b1, (double)value2((int)(int8_t)(cm >> (8 * e)), um), h.c1, gd);
+        v[e] = blend(h.b2, (double)value4((cv >> (8 * e)) & 0xffu, uv), h.c2, gd * gd);
+        // magnitudes order as their bits, NaN above all (past the end everything is 0)
+        top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
+        top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
       }
-      const float Am = __uint_as_float(wave_max_bits(top_m)), Av = __uint_as_float(wave_max_bits(top_v));
-      const double Amd = (double)Am, Avd = (double)Av;
-      const double im = Am > 0.f ? 1.0 / Amd : 0.0, iv = Av > 0.f ? 1.0 / Avd : 0.0;
-      uint32_t qm = 0, qv = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        qm |= ((uint32_t)code2(m[e], Amd, im) & 0xffu) << (8 * e);
-        qv |= code4(v[e], Avd, iv) << (8 * e);
-      }
+      const float Am = __uint_as_float(wave_max_u32(top_m)), Av = __uint_as_float(wave_max_u32(top_v));
+      uint32_t qm, qv;
+      encode(m, v, Am, Av, qm, qv);
       store_codes((uint8_t*)t.exp_avg, i, n, vec, qm);
       store_codes((uint8_t*)t.exp_avg_sq, i, n, vec, qv);
       if (lane == 0) {
@@ -236,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const 
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float d = c.x * m[e] / (sqrtf(v[e]) * c.y + h.eps);
+      const float d = c.x * m[e] * __builtin_amdgcn_rcpf(fmaf(root(v[e]), c.y, h.eps));
       w[e] = fmaf(-c.z, w[e], w[e]) - d;
     }
     store4(p, i, n, vec, w);
@@ -254,13 +293,14 @@ struct MomentTable {
 __global__ __launch_bounds__(kThreads) void moments_kernel(const MomentTable tab) {
   const int which = owner_of(tab.start, tab.count, blockIdx.x);
   const zmoe_moment& t = tab.t[which];
-  const bool vec = (tab.vec >> which) & 1;
-  const int64_t chunk = blockIdx.x - tab.start[which];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool wide = (tab.vec >> which) & 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
 #pragma unroll
   for (int u = 0; u < kBlocks / 4; ++u) {
-    const int64_t b = chunk * kBlocks + wave * (kBlocks / 4) + u, i = b * kBlock + lane * 4;
+    const int64_t b = first + u, i = b * kBlock + lane * 4;
     if (b * kBlock >= t.n) break;
+    const bool vec = wide && (b + 1) * kBlock <= t.n;
     const uint32_t q = load_codes((const uint8_t*)t.codes, i, t.n, vec);
     const double unit = t.second ? unit4(t.scale[b]) : unit2(t.scale[b]);
     float v[4];
@@ -426,7 +466,7 @@ extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype
                        beta2, weight_decay, clip, coef + i);
     if (const int rc = check_launch("adamw")) return rc;
   }
-  const Hyper h{beta1, beta2, (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)eps};
+  const Hyper h{beta1, beta2, 1.0 - beta1, 1.0 - beta2, (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)eps};
   Table tab;
   tab.count = 0;
   tab.start[0] = 0;
