@@ -19,14 +19,14 @@
 // pointers travel in the launches' arguments, so nothing is copied to the device and a graph keeps them.
 #include <type_traits>
 
-#include "zmoe_route.h"  // wave_max_u32
+#include "zmoe_route.h"  // row_max_u32
 
 namespace zmoe {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;   // elements with one scale
-constexpr int kBlocks = 16;   // of them in a workgroup's chunk: four a wave
+constexpr int kBlocks = 16;   // of them in a workgroup's chunk: four a wave (two pairs in 8 bits)
 constexpr int kChunk = kBlock * kBlocks;
 constexpr int kTensors = 48;  // in a launch's arguments (under 4 KB)
 constexpr int kNormChunk = 16384;
@@ -92,82 +92,107 @@ __device__ __forceinline__ float blend(double x, double a, double y, double b) {
   return (float)(xa + yb);
 }
 
-// The f32 values of codes: sign q^2 unit, q^4 unit (q^4 as a square in double: exact).
-__device__ __forceinline__ float value2(int q, double unit) { return (float)((double)(q * abs(q)) * unit); }
+// The f32 values of codes: sign q^2 unit, q^4 unit.
+__device__ __forceinline__ float value2(int q, double unit) {
+  const double x = (double)q;
+  return (float)(x * fabs(x) * unit);
+}
 __device__ __forceinline__ float value4(uint32_t q, double unit) {
-  const double q2 = (double)(q * q);
-  return (float)(q2 * q2 * unit);
+  const double x = (double)q, x2 = x * x;
+  return (float)(x2 * x2 * unit);
 }
 
-// A code's place in the root's domain, + 1/2: the code is its whole part, unless that lies within kNear2 or kNear4 of a
-// border. The estimate has a reciprocal, a product, one or two roots and a product of f32, 2.4 roundings of 2^-23 at most
-// in the root: 127 (255) of those and the last sum's own are 4.0e-5 (8.1e-5).
+// A code's place in the root's domain: the code is the whole number next to it, unless half-way between two lies within
+// kNear2 or kNear4. The estimate has a reciprocal, a product, one or two roots and a product of f32, 2.4 roundings of 2^-23
+// at most in the root: 127 (255) of those are 3.7e-5 (7.3e-5).
 constexpr float kNear2 = 0x1p-14f, kNear4 = 0x1p-13f;
 __device__ __forceinline__ float place2(float mag, float inv) {
-  return fmaf(__builtin_amdgcn_sqrtf(mag * inv), (float)kTop2, 0.5f);
+  return __builtin_amdgcn_sqrtf(mag * inv) * (float)kTop2;
 }
 __device__ __forceinline__ float place4(float mag, float inv) {
-  return fmaf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(mag * inv)), (float)kTop4, 0.5f);
+  return __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(mag * inv)) * (float)kTop4;
 }
 
-// The code itself: an estimate to one code or better, set right by the borders on its two sides.
-__device__ __forceinline__ int exact2(float mag, double A) {
-  const double x = (double)mag;
-  int q = A > 0.0 ? (int)(sqrtf((float)(x / A)) * 127.f + 0.5f) : 0;
-  q = min(max(q, 0), kTop2);
-  const double at = x * (4.0 * kDiv2);
+// The code itself, from one that is off by one at most: set right by the borders on its two sides.
+__device__ __forceinline__ int settle2(int q, float mag, double A) {
+  const double at = (double)mag * (4.0 * kDiv2);
   const int l = 2 * q - 1, h = 2 * q + 1;
-  return q + (int)(q < kTop2 && (double)(h * h) * A <= at && A > 0.0) - (int)(q > 0 && (double)(l * l) * A > at);
+  return q + (int)(q < kTop2 && at > 0.0 && (double)(h * h) * A <= at) - (int)(q > 0 && (double)(l * l) * A > at);
 }
-__device__ __forceinline__ int exact4(float mag, double A) {
-  const double x = (double)mag;
-  int q = A > 0.0 ? (int)(sqrtf(sqrtf((float)(x / A))) * 255.f + 0.5f) : 0;
-  q = min(max(q, 0), kTop4);
-  const double at = x * (16.0 * kDiv4);
+__device__ __forceinline__ int settle4(int q, float mag, double A) {
+  const double at = (double)mag * (16.0 * kDiv4);
   const double l = (double)((2 * q - 1) * (2 * q - 1)), h = (double)((2 * q + 1) * (2 * q + 1));
-  return q + (int)(q < kTop4 && h * h * A <= at && A > 0.0) - (int)(q > 0 && l * l * A > at);
+  return q + (int)(q < kTop4 && at > 0.0 && h * h * A <= at) - (int)(q > 0 && l * l * A > at);
 }
 
-// The codes of a lane's four elements of each moment (v > 0 at least 1), the bytes of a dword each. Blocks whose largest
-// magnitude has no f32 reciprocal (or is not finite) take the exact way for all.
-__device__ __forceinline__ void encode(const float (&m)[4], const float (&v)[4], float Am, float Av, uint32_t& qm,
-                                       uint32_t& qv) {
-  const bool plain_m = Am >= 0x1p-100f && Am <= 0x1p100f, plain_v = Av >= 0x1p-100f && Av <= 0x1p100f;
-  const float im = plain_m ? __builtin_amdgcn_rcpf(Am) : 0.f, iv = plain_v ? __builtin_amdgcn_rcpf(Av) : 0.f;
-  int cm[4], cv[4];
-  bool near_m = !plain_m, near_v = !plain_v;
+// The codes of a lane's N elements of each moment (v > 0 at least 1), the bytes of dwords. A block whose largest magnitude
+// has no f32 reciprocal takes its estimates from double; one that is not finite has any codes (its scale says it all).
+template <int N>
+__device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], float Am, float Av, uint32_t (&qm)[N / 4],
+                                       uint32_t (&qv)[N / 4]) {
+  const bool odd = (Am > 0.f && Am < 0x1p-100f) || Am > 0x1p100f || (Av > 0.f && Av < 0x1p-100f) || Av > 0x1p100f;
+  const float im = Am > 0.f ? __builtin_amdgcn_rcpf(Am) : 0.f, iv = Av > 0.f ? __builtin_amdgcn_rcpf(Av) : 0.f;
+  float far_m = 0.f, far_v = 0.f;  // from the nearest whole number, at most
+  int cm[N], cv[N];                // magnitudes
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < N; ++e) {
     const float y = place2(fabsf(m[e]), im), z = place4(v[e], iv);
-    const float fy = __builtin_amdgcn_fractf(y), fz = __builtin_amdgcn_fractf(z);
-    cm[e] = (int)y;
-    cv[e] = (int)z;
-    near_m |= fabsf(fy - 0.5f) > 0.5f - kNear2;
-    near_v |= fabsf(fz - 0.5f) > 0.5f - kNear4;
+    const float ry = rintf(y), rz = rintf(z);
+    far_m = fmaxf(far_m, fabsf(y - ry));
+    far_v = fmaxf(far_v, fabsf(z - rz));
+    cm[e] = (int)ry;
+    cv[e] = (int)rz;
   }
-  if (near_m) {  // one lane in two thousand
+  if (odd) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) cm[e] = exact2(fabsf(m[e]), (double)Am);
+    for (int e = 0; e < N; ++e) {
+      cm[e] = Am > 0.f ? (int)rintf(sqrtf((float)(fabs((double)m[e]) / (double)Am)) * (float)kTop2) : 0;
+      cv[e] = Av > 0.f ? (int)rintf(sqrtf(sqrtf((float)((double)v[e] / (double)Av))) * (float)kTop4) : 0;
+    }
+    far_m = far_v = 0.5f;
   }
-  if (near_v) {
+  if (far_m > 0.5f - kNear2) {  // one lane in a thousand
 #pragma unroll
-    for (int e = 0; e < 4; ++e) cv[e] = exact4(v[e], (double)Av);
+    for (int e = 0; e < N; ++e) cm[e] = settle2(cm[e], fabsf(m[e]), (double)Am);
   }
-  qm = qv = 0;
+  if (far_v > 0.5f - kNear4) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    cm[e] = min(cm[e], kTop2);
-    cv[e] = min(max(cv[e], v[e] > 0.f ? 1 : 0), kTop4);
-    qm |= ((uint32_t)(m[e] < 0.f ? -cm[e] : cm[e]) & 0xffu) << (8 * e);
-    qv |= (uint32_t)cv[e] << (8 * e);
+    for (int e = 0; e < N; ++e) cv[e] = settle4(cv[e], v[e], (double)Av);
+  }
+#pragma unroll
+  for (int d = 0; d < N / 4; ++d) {
+    qm[d] = qv[d] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 4 * d + e;
+      const int sign = (int)__float_as_uint(m[i]) >> 31;  // two's complement of a negative moment's code
+      qm[d] |= (uint32_t)(((cm[i] ^ sign) - sign) & 0xff) << (8 * e);
+      qv[d] |= max((uint32_t)cv[i], min(__float_as_uint(v[i]), 1u)) << (8 * e);
+    }
   }
 }
 
-// sqrt and a quotient to 1.5 f32 roundings each (v_sqrt_f32 takes no subnormals; denominators here are none).
+// Max over each half of a wave, in its 32 lanes: within rows of 16 by DPP, then a row and its neighbour exchanged.
+__device__ __forceinline__ uint32_t half_max_u32(uint32_t v) {
+  v = row_max_u32<16>(v);
+  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max((uint32_t)both[0], (uint32_t)both[1]);
+}
+
+// A square root to one rounding of f32. v_sqrt_f32 takes subnormals for 0, which does not count under an eps that is
+// some 2^-40 or more (SCALED false).
+template <bool SCALED>
 __device__ __forceinline__ float root(float v) {
+  if constexpr (!SCALED) return __builtin_amdgcn_sqrtf(v);
   const bool small = v < 0x1p-96f;
   const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p32f : v);
   return small ? r * 0x1p-16f : r;
+}
+
+// The parameter after the step: the quotient by v_rcp_f32, whose argument is a normal number.
+template <bool SCALED>
+__device__ __forceinline__ float stepped(float w, float m, float v, const float4& c, float eps) {
+  return fmaf(-(c.x * m), __builtin_amdgcn_rcpf(fmaf(root<SCALED>(v), c.y, eps)), fmaf(-c.z, w, w));
 }
 
 // ------------------------------------------------------------------ elements
@@ -199,6 +224,50 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, con
       if (i + u < n) p[i + u] = from_f32<T>(v[u]);
   }
 }
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int i, int64_t n, bool vec, float (&v)[8]) {
+  if (vec) {
+    constexpr int VC = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 8 / VC; ++c) unpack_chunk(*reinterpret_cast<const uint4*>(p + i + c * VC), &v[c * VC], T{});
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i + u < n ? to_f32(p[i + u]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int i, int64_t n, bool vec, const float (&v)[8]) {
+  if (vec) {
+    constexpr int VC = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 8 / VC; ++c) *reinterpret_cast<uint4*>(p + i + c * VC) = pack_chunk(&v[c * VC], T{});
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u < n) p[i + u] = from_f32<T>(v[u]);
+  }
+}
+// Eight codes as the bytes of two dwords.
+__device__ __forceinline__ void load_codes8(const uint8_t* p, int i, int64_t n, bool vec, uint32_t (&c)[2]) {
+  if (vec) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p + i);
+    c[0] = x.x, c[1] = x.y;
+  } else {
+    c[0] = c[1] = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u < n) c[u >> 2] |= (uint32_t)p[i + u] << (8 * (u & 3));
+  }
+}
+__device__ __forceinline__ void store_codes8(uint8_t* p, int i, int64_t n, bool vec, const uint32_t (&c)[2]) {
+  if (vec) {
+    *reinterpret_cast<uint2*>(p + i) = make_uint2(c[0], c[1]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i + u < n) p[i + u] = (uint8_t)(c[u >> 2] >> (8 * (u & 3)));
+  }
+}
 // Four codes as the bytes of a dword.
 __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int64_t n, bool vec) {
   if (vec) return *reinterpret_cast<const uint32_t*>(p + i);
@@ -208,77 +277,94 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int6
     if (i + u < n) c |= (uint32_t)p[i + u] << (8 * u);
   return c;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, int64_t i, int64_t n, bool vec, uint32_t c) {
-  if (vec) {
-    *reinterpret_cast<uint32_t*>(p + i) = c;
-  } else {
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + u < n) p[i + u] = (uint8_t)(c >> (8 * u));
-  }
-}
-
-template <typename T, bool EIGHT>
+template <typename T, bool SCALED>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const Hyper h,
                                                          const float4* __restrict__ coef) {
   const int which = owner_of(tab.start, tab.count, blockIdx.x);
   const zmoe_adamw_tensor& t = tab.t[which];
   const bool wide = (tab.vec >> which) & 1;
   const float4 c = coef[which];
-  T* p = (T*)t.param;
-  const T* g = (const T*)t.grad;
   const int64_t n = t.n;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
 #pragma unroll 2
   for (int u = 0; u < kBlocks / 4; ++u) {
-    const int64_t b = first + u, i = b * kBlock + lane * 4;
-    if (b * kBlock >= n) break;
-    const bool vec = wide && (b + 1) * kBlock <= n;
+    const int64_t at = (first + u) * kBlock, left = n - at;
+    if (left <= 0) break;
+    const bool vec = wide && left >= kBlock;
+    const int i = lane * 4;
+    T* p = (T*)t.param + at;
+    float *pm = (float*)t.exp_avg + at, *pv = (float*)t.exp_avg_sq + at;
     float w[4], gr[4], m[4], v[4];
-    load4(p, i, n, vec, w);
-    load4(g, i, n, vec, gr);
-    if constexpr (EIGHT) {
-      const uint32_t cm = load_codes((const uint8_t*)t.exp_avg, i, n, vec);
-      const uint32_t cv = load_codes((const uint8_t*)t.exp_avg_sq, i, n, vec);
-      const double um = unit2(t.scale_avg[b]), uv = unit4(t.scale_sq[b]), clip = (double)c.w;
-      uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const double gd = (double)gr[e] * clip;
-        m[e] = blend(h.b1, (double)value2((int)(int8_t)(cm >> (8 * e)), um), h.c1, gd);
-        v[e] = blend(h.b2, (double)value4((cv >> (8 * e)) & 0xffu, uv), h.c2, gd * gd);
-        // magnitudes order as their bits, NaN above all (past the end everything is 0)
-        top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
-        top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
-      }
-      const float Am = __uint_as_float(wave_max_u32(top_m)), Av = __uint_as_float(wave_max_u32(top_v));
-      uint32_t qm, qv;
-      encode(m, v, Am, Av, qm, qv);
-      store_codes((uint8_t*)t.exp_avg, i, n, vec, qm);
-      store_codes((uint8_t*)t.exp_avg_sq, i, n, vec, qv);
-      if (lane == 0) {
-        t.scale_avg[b] = Am;
-        t.scale_sq[b] = Av;
-      }
-    } else {
-      load4((const float*)t.exp_avg, i, n, vec, m);
-      load4((const float*)t.exp_avg_sq, i, n, vec, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float gs = gr[e] * c.w;
-        m[e] = fmaf(h.b1f, m[e], h.c1f * gs);
-        v[e] = fmaf(h.b2f, v[e], h.c2f * (gs * gs));
-      }
-      store4((float*)t.exp_avg, i, n, vec, m);
-      store4((float*)t.exp_avg_sq, i, n, vec, v);
-    }
+    load4(p, i, left, vec, w);
+    load4((const T*)t.grad + at, i, left, vec, gr);
+    load4(pm, i, left, vec, m);
+    load4(pv, i, left, vec, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float d = c.x * m[e] * __builtin_amdgcn_rcpf(fmaf(root(v[e]), c.y, h.eps));
-      w[e] = fmaf(-c.z, w[e], w[e]) - d;
+      const float gs = gr[e] * c.w;
+      m[e] = fmaf(h.b1f, m[e], h.c1f * gs);
+      v[e] = fmaf(h.b2f, v[e], h.c2f * (gs * gs));
+      w[e] = stepped<SCALED>(w[e], m[e], v[e], c, h.eps);
     }
-    store4(p, i, n, vec, w);
+    store4(pm, i, left, vec, m);
+    store4(pv, i, left, vec, v);
+    store4(p, i, left, vec, w);
+  }
+}
+
+// Moments in 8 bits: a wave has two blocks at once, eight consecutive elements a lane, so that what is done once for a block
+// (the largest magnitudes over its lanes, the scales' quotients) is shared by twice as many. The arithmetic is the bound
+// as much as memory: some 70 instructions an element, 20 of them in double (which runs at f32's rate here).
+template <typename T, bool SCALED>
+__global__ __launch_bounds__(kThreads) void adamw8_kernel(const Table tab, const Hyper h,
+                                                          const float4* __restrict__ coef) {
+  const int which = owner_of(tab.start, tab.count, blockIdx.x);
+  const zmoe_adamw_tensor& t = tab.t[which];
+  const bool wide = (tab.vec >> which) & 1;
+  const float4 c = coef[which];
+  const double clip = (double)c.w;
+  const int64_t n = t.n;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
+  for (int u = 0; u < kBlocks / 4; u += 2) {
+    const int64_t at = (first + u) * kBlock, left = n - at;
+    if (left <= 0) break;
+    const bool vec = wide && left >= 2 * kBlock;
+    const int i = lane * 8, half = lane >> 5;
+    const bool there = left > half * kBlock;  // this half's block has elements
+    T* p = (T*)t.param + at;
+    uint8_t *pm = (uint8_t*)t.exp_avg + at, *pv = (uint8_t*)t.exp_avg_sq + at;
+    float *sm = t.scale_avg + (first + u), *sv = t.scale_sq + (first + u);
+    float w[8], m[8], v[8];
+    uint32_t qm[2], qv[2];
+    load_codes8(pm, i, left, vec, qm);
+    load_codes8(pv, i, left, vec, qv);
+    load8((const T*)t.grad + at, i, left, vec, v);
+    const float am = there ? sm[half] : 0.f, av = there ? sv[half] : 0.f;
+    load8(p, i, left, vec, w);
+    const double um = unit2(am), uv = unit4(av);
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const double gd = (double)v[e] * clip;
+      const uint32_t byte = 8 * (e & 3);
+      m[e] = blend(h.b1, (double)value2((int)(int8_t)(qm[e >> 2] >> byte), um), h.c1, gd);
+      v[e] = blend(h.b2, (double)value4((qv[e >> 2] >> byte) & 0xffu, uv), h.c2, gd * gd);
+      // magnitudes order as their bits, NaN above all (past the end everything is 0)
+      top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
+      top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
+      w[e] = stepped<SCALED>(w[e], m[e], v[e], c, h.eps);
+    }
+    store8(p, i, left, vec, w);
+    const float Am = __uint_as_float(half_max_u32(top_m)), Av = __uint_as_float(half_max_u32(top_v));
+    encode<8>(m, v, Am, Av, qm, qv);
+    store_codes8(pm, i, left, vec, qm);
+    store_codes8(pv, i, left, vec, qv);
+    if ((lane & 31) == 0 && there) {
+      sm[half] = Am;
+      sv[half] = Av;
+    }
   }
 }
 
@@ -475,12 +561,21 @@ extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype
   auto launch = [&](int next) {
     const bool any = tab.count > 0 && tab.start[tab.count] > 0;
     if (any) {
-      auto go = [&](auto type, auto eight) {
-        hipLaunchKernelGGL((adamw_kernel<decltype(type), decltype(eight)::value>), dim3((unsigned)tab.start[tab.count]),
-                           dim3(kThreads), 0, as_stream(stream), tab, h, coef + first_of_launch);
+      const dim3 grid((unsigned)tab.start[tab.count]), block(kThreads);
+      auto go = [&](auto type, auto scaled) {
+        using T = decltype(type);
+        constexpr bool S = decltype(scaled)::value;
+        if (state_bits == 8)
+          hipLaunchKernelGGL((adamw8_kernel<T, S>), grid, block, 0, as_stream(stream), tab, h, coef + first_of_launch);
+        else
+          hipLaunchKernelGGL((adamw_kernel<T, S>), grid, block, 0, as_stream(stream), tab, h, coef + first_of_launch);
       };
-      if (dtype == ZMOE_DTYPE_BF16) state_bits == 8 ? go(uint16_t{}, std::true_type{}) : go(uint16_t{}, std::false_type{});
-      else state_bits == 8 ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+      auto typed = [&](auto type) {
+        if (eps >= 0x1p-40) go(type, std::false_type{});
+        else go(type, std::true_type{});
+      };
+      if (dtype == ZMOE_DTYPE_BF16) typed(uint16_t{});
+      else typed(float{});
     }
     tab.count = 0;
     tab.vec = 0;
@@ -488,7 +583,7 @@ extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype
     return any ? check_launch("adamw") : (int)ZMOE_OK;
   };
   constexpr int64_t kMost = kMaxLaunchThreads / kThreads / 2;
-  const unsigned wide = 4 * size, codes = state_bits == 8 ? 4 : 16;
+  const unsigned wide = state_bits == 8 ? 16 : 4 * size, codes = state_bits == 8 ? 8 : 16;
   for (int i = 0; i < count; ++i) {
     const zmoe_adamw_tensor& t = tensors[i];
     const int64_t all = cdiv(t.n, kChunk);
