@@ -9,8 +9,6 @@
 //
 // Where p + b decides, one f32 rounding of p can decide: p comes from double, whose error (some 2^-52) moves an f32
 // rounding for one value in 2^28. Without a bias the experts' order is their logits' order.
-#include <type_traits>
-
 #include "zmoe_route.h"
 
 namespace zmoe {
@@ -30,30 +28,6 @@ struct RouteArgs {
   float* p;  // or null
 };
 
-// Over the LPR (8, 16 or 64) lanes of a row; every lane gets the result.
-template <int LPR>
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-  if constexpr (LPR == 64) return wave_max_u32(v);
-  else return row_max_u32<LPR>(v);
-}
-template <int LPR>
-__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
-  if constexpr (LPR == 64) return ~wave_max_u32(~v);
-  else return row_min_u32<LPR>(v);
-}
-template <int LPR, typename F>
-__device__ __forceinline__ F lanes_sum(F v) {
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-template <int LPR>
-__device__ __forceinline__ float lanes_fmax(float v) {
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
 // What a wave wrote to LDS is there for its other lanes (a wave's LDS accesses stay in order).
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -64,27 +38,6 @@ __device__ __forceinline__ void wave_sync() {
 // The float whose score_key is key (a NaN, +0 for both zeros).
 __device__ __forceinline__ float key_score(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-
-// Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: E and e0 are whole 16-byte chunks and rows lie on 16.
-template <int VPL, typename LT>
-__device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, int E, bool vec, bool live, float fill,
-                                          float (&v)[VPL]) {
-  constexpr int VC = 16 / sizeof(LT);
-  if (vec) {
-#pragma unroll
-    for (int c = 0; c < VPL / VC; ++c) {
-      if (live && e0 + c * VC < E) {
-        unpack_chunk(*reinterpret_cast<const uint4*>(row + e0 + c * VC), &v[c * VC], LT{});
-      } else {
-#pragma unroll
-        for (int u = 0; u < VC; ++u) v[c * VC + u] = fill;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < VPL; ++q) v[q] = live && e0 + q < E ? to_f32(row[e0 + q]) : fill;
-  }
 }
 
 // Rows of LPR lanes, VPL consecutive experts a lane, 64 / LPR tokens a wave at once; waves stride over the tokens.
@@ -225,7 +178,7 @@ struct RouteBackwardArgs {
 template <int LPR, int VPL, bool SOFT, typename LT>
 __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const RouteBackwardArgs a) {
 #pragma clang fp contract(off)  // (one expert's renormalised weight has a grad of rounding errors alone: 0, not fused ones)
-  constexpr int TPW = 64 / LPR, W = LPR * VPL, VC = 16 / sizeof(LT);
+  constexpr int TPW = 64 / LPR, W = LPR * VPL;
   __shared__ float ds[kWaves][TPW][W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = lane / LPR, r = lane % LPR, e0 = r * VPL;
@@ -293,53 +246,15 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
 #pragma unroll
       for (int q = 0; q < VPL; ++q) v[q] += add[q];
     }
-    if (live) {
-      LT* out = (LT*)a.dz + t * a.ld;
-      if (a.vec) {
-#pragma unroll
-        for (int c = 0; c < VPL / VC; ++c)
-          if (e0 + c * VC < E) *reinterpret_cast<uint4*>(out + e0 + c * VC) = pack_chunk(&v[c * VC], LT{});
-      } else {
-#pragma unroll
-        for (int q = 0; q < VPL; ++q)
-          if (e0 + q < E) out[e0 + q] = from_f32<LT>(v[q]);
-      }
-    }
+    if (live) store_lane<VPL>((LT*)a.dz + t * a.ld, e0, E, a.vec, v);
     wave_sync();
   }
-}
-
-using I8 = std::integral_constant<int, 8>;
-using I16 = std::integral_constant<int, 16>;
-using I64 = std::integral_constant<int, 64>;
-
-// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts.
-template <typename F>
-void by_layout(int E, bool soft, int dtype, F&& f) {
-  auto typed = [&](auto lpr, auto vpl) {
-    auto scored = [&](auto lt) {
-      if (soft) f(lpr, vpl, std::true_type{}, lt);
-      else f(lpr, vpl, std::false_type{}, lt);
-    };
-    if (dtype == ZMOE_DTYPE_BF16) scored(uint16_t{});
-    else scored(float{});
-  };
-  if (E <= 64) typed(I8{}, I8{});
-  else if (E <= 128) typed(I16{}, I8{});
-  else if (E <= 256) typed(I16{}, I16{});
-  else if (E <= 512) typed(I64{}, I8{});
-  else typed(I64{}, I16{});
 }
 
 // Workgroups that hold the tokens, at most eight a CU: their waves loop over the others.
 unsigned grid_of(int64_t T, int lpr) {
   const int64_t blocks = cdiv(T, (int64_t)kWaves * (64 / lpr));
   return (unsigned)(blocks < 2048 ? blocks : 2048);
-}
-
-bool rows_on_16(const void* base, int64_t ld, int E, int dtype) {
-  const int size = dtype_size(dtype);
-  return aligned16(base) && (ld * size) % 16 == 0 && (E * size) % 16 == 0;
 }
 
 }  // namespace
@@ -366,7 +281,7 @@ extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E
   ZMOE_REQUIRE(logits && topk_idx && topk_weight, ZMOE_ERR_NULL, "route: null pointer");
   const RouteArgs a{logits, expert_biases, T, E, k, groups, top_groups, group_scores, renormalize,
                     rows_on_16(logits, E, E, logits_dtype), scale, topk_idx, topk_weight, topk_prob};
-  by_layout(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
+  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
     hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
                        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
   });
@@ -391,7 +306,7 @@ extern "C" int zmoe_route_backward(const float* d_weight, const float* topk_prob
                    (!logits || rows_on_16(logits, E, E, d_logits_dtype));
   const RouteBackwardArgs a{d_weight, topk_prob, topk_idx, logits, add, ld_add, T, ld_d_logits, E, k, renormalize, vec,
                             scale, d_logits};
-  by_layout(E, score == ZMOE_SCORE_SOFTMAX, d_logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
+  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, d_logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
     hipLaunchKernelGGL(
         (route_backward_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
         dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);

@@ -6,9 +6,11 @@
 // The counts take no part in the gradient. A token whose logits are all -inf adds nothing and has no gradient; tokens
 // outside the sequences neither.
 //
-// The forward reads the logits once: a workgroup has a tile of kTile tokens, a wave a token, and the sums of the tile's
-// part of each sequence go to a slot of their own (tile i and sequence s meet in slot i + s: walking along the tokens
-// either number grows by one), which a second launch adds up in a fixed order. The gradient reads the logits again.
+// The forward reads the logits once: a workgroup has a tile of tokens, a row of LPR lanes a token (VPL consecutive experts a
+// lane), and the sums of the tile's part of each sequence go to a slot of their own (tile i and sequence s meet in slot
+// i + s: walking along the tokens either number grows by one), which a second launch adds up in a fixed order, a
+// workgroup for each sequence and 32 experts. The gradient reads the logits again. Both are short: what bounds them is
+// the latency of a few dependent reads in each of the launches.
 #include <type_traits>
 
 #include "zmoe_route.h"
@@ -29,28 +31,36 @@ struct Sequences {
     const int64_t v = wide ? ((const int64_t*)cu)[s] : ((const int32_t*)cu)[s];
     return v < 0 ? 0 : (v > T ? T : v);
   }
-  // The first sequence that ends after token t (S if none does).
+  // The first sequence that ends after token t (S if none does), for a t that is the same in the wave: all borders
+  // counted at once, many of them halved first.
   __device__ __forceinline__ int after(int64_t t) const {
+    if (!cu) return t < T ? 0 : 1;
     int lo = 0, hi = S;
-    while (lo < hi) {
+    while (hi - lo > 512) {
       const int mid = (lo + hi) >> 1;
       if (at(mid + 1) > t) hi = mid;
       else lo = mid + 1;
     }
-    return lo;
+    int n = 0;
+    for (int i = lo + (int)(threadIdx.x & 63); i - (int)(threadIdx.x & 63) < hi; i += 64)
+      n += __popcll(__ballot(i < hi && at(i + 1) <= t));
+    return lo + n;
   }
 };
 
-// Scratch: a slot's sums of ph [E], choices [E] and lse^2, then each sequence's part of the two losses.
+// Scratch: a slot's sums of ph [E], choices [E] and lse^2, then the parts of the two losses, S' and N, a counter.
 struct Scratch {
   float* mass;      // [slots, E]
   int32_t* count;   // [slots, E]
   float* zsum;      // [slots]
-  double* part;     // [S, 2]
+  double* part;     // [S, column blocks, 2]
+  int64_t* total;   // S', N
   int32_t* done;    // workgroups of the second launch that have ended
 };
 
 __host__ __device__ inline int64_t slots_of(int64_t T, int S) { return (T + kTile - 1) / kTile + S; }
+constexpr int kColumns = 32;  // experts of a workgroup of the second launch
+inline int column_blocks(int E) { return (E + kColumns - 1) / kColumns; }
 
 inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -66,36 +76,27 @@ size_t lay_out(int64_t T, int E, int S, char* base, Scratch* out) {
   s.mass = (float*)take(n * E * 4);
   s.count = (int32_t*)take(n * E * 4);
   s.zsum = (float*)take(n * 4);
-  s.part = (double*)take((size_t)S * 16);
+  s.part = (double*)take((size_t)S * column_blocks(E) * 16);
+  s.total = (int64_t*)take(16);
   s.done = (int32_t*)take(4);
   if (out) *out = s;
   return o;
 }
 
-__device__ __forceinline__ float wave_fmax(float v) {
+// A token's values in a row of lanes from its logits z (-inf past E): ph, the softmax's shares and (sigmoid form) the
+// sigmoids, all 0 where every logit is -inf; its lse.
+template <int LPR, int VPL, bool SOFT>
+__device__ __forceinline__ float token_row(const float (&z)[VPL], float (&ph)[VPL], float (&soft)[VPL],
+                                           float (&sig)[VPL]) {
+  float m = z[0];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
-// A token's row, expert lane + 64 q: ph, the softmax's shares (soft) and sigmoids (sig, sigmoid form), its lse; all 0
-// where every logit is -inf.
-template <int PL, bool SOFT, typename LT>
-__device__ __forceinline__ float token_row(const LT* __restrict__ row, int E, int lane, float (&ph)[PL],
-                                           float (&soft)[PL], float (&sig)[PL]) {
-  float z[PL], m = -INFINITY;
-#pragma unroll
-  for (int q = 0; q < PL; ++q) {
-    const int e = lane + 64 * q;
-    z[q] = e < E ? to_f32(row[e]) : -INFINITY;
-    m = fmaxf(m, z[q]);
-  }
-  m = wave_fmax(m);
+  for (int q = 1; q < VPL; ++q) m = fmaxf(m, z[q]);
+  m = lanes_fmax<LPR>(m);
   const bool none = m == -INFINITY;
   m = none ? 0.f : m;
   float sum = 0.f, total = 0.f;
 #pragma unroll
-  for (int q = 0; q < PL; ++q) {
+  for (int q = 0; q < VPL; ++q) {
     soft[q] = expf(z[q] - m);
     sum += soft[q];
     if constexpr (!SOFT) {
@@ -103,59 +104,95 @@ __device__ __forceinline__ float token_row(const LT* __restrict__ row, int E, in
       total += sig[q];
     }
   }
-  sum = wave_sum(sum);
+  sum = lanes_sum<LPR>(sum);
   const float inv = none && sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int q = 0; q < PL; ++q) soft[q] *= inv;
+  for (int q = 0; q < VPL; ++q) soft[q] *= inv;
   if constexpr (SOFT) {
 #pragma unroll
-    for (int q = 0; q < PL; ++q) ph[q] = soft[q];
+    for (int q = 0; q < VPL; ++q) ph[q] = soft[q];
   } else {
-    total = wave_sum(total);
+    total = lanes_sum<LPR>(total);
     const float inv_total = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int q = 0; q < PL; ++q) ph[q] = sig[q] * inv_total;
+    for (int q = 0; q < VPL; ++q) ph[q] = sig[q] * inv_total;
   }
   return none && sum == 0.f ? 0.f : m + logf(sum);
 }
 
-template <int PL, bool SOFT, typename LT>
+template <int LPR, int VPL, bool SOFT, typename LT>
 __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __restrict__ logits,
-                                                                  const int64_t* __restrict__ idx, int E, int k,
+                                                                  const int64_t* __restrict__ idx, int E, int k, bool vec,
                                                                   Sequences seq, Scratch w) {
-  __shared__ float mass[kWaves][64 * PL];
-  __shared__ int32_t count[64 * PL];
+  constexpr int TPW = 64 / LPR, ROWS = kWaves * TPW, W = LPR * VPL;
+  __shared__ float mass[kWaves][W];
+  __shared__ int32_t count[W];
   __shared__ float zs[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane / LPR, e0 = (lane % LPR) * VPL;
   const int64_t tile = blockIdx.x, t0 = tile * kTile, t1 = t0 + kTile < seq.T ? t0 + kTile : seq.T;
-  if (tile == 0 && threadIdx.x == 0) *w.done = 0;
+  if (tile == gridDim.x - 1) {  // a workgroup of its own: S' and N
+    int64_t live = 0, tokens = 0;
+    for (int i = threadIdx.x; i < seq.S; i += 64 * kWaves) {
+      const int64_t n = seq.at(i + 1) - seq.at(i);
+      live += n > 0;
+      tokens += n > 0 ? n : 0;
+    }
+    __shared__ int64_t part[kWaves][2];
+    live = lanes_sum<64>(live);
+    tokens = lanes_sum<64>(tokens);
+    if (lane == 0) {
+      part[wave][0] = live;
+      part[wave][1] = tokens;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      *w.done = 0;
+      w.total[0] = part[0][0] + part[1][0] + part[2][0] + part[3][0];
+      w.total[1] = part[0][1] + part[1][1] + part[2][1] + part[3][1];
+    }
+    return;
+  }
   for (int s = seq.after(t0); s < seq.S; ++s) {
     int64_t lo = seq.at(s), hi = seq.at(s + 1);
     if (lo >= t1) break;
     lo = lo < t0 ? t0 : lo;
     hi = hi > t1 ? t1 : hi;
     if (lo >= hi) continue;
-    float acc[PL], z2 = 0.f;
+    const int64_t slot = tile + s;
+    float acc[VPL], z2 = 0.f, nxt[VPL];
+    int64_t t = lo + wave * TPW + row;
+    load_lane<VPL>(logits + t * E, e0, E, vec, t < hi, -INFINITY, nxt);
 #pragma unroll
-    for (int q = 0; q < PL; ++q) acc[q] = 0.f;
+    for (int q = 0; q < VPL; ++q) acc[q] = 0.f;
     for (int e = threadIdx.x; e < E; e += 64 * kWaves) count[e] = 0;
     __syncthreads();
-    for (int64_t t = lo + wave; t < hi; t += kWaves) {
-      float ph[PL], soft[PL], sig[PL];
-      const float lse = token_row<PL, SOFT>(logits + t * E, E, lane, ph, soft, sig);
-      z2 += lse * lse;
-#pragma unroll
-      for (int q = 0; q < PL; ++q) acc[q] += ph[q];
-    }
     for (int64_t i = lo * k + threadIdx.x; i < hi * k; i += 64 * kWaves) {
       const int64_t e = idx[i];
       if (e >= 0 && e < E) atomicAdd(&count[e], 1);  // whole numbers: any order
     }
+    for (int64_t b = lo; b < hi; b += ROWS, t += ROWS) {  // the next rows are on their way while these are added
+      float z[VPL], ph[VPL], soft[VPL], sig[VPL];
 #pragma unroll
-    for (int q = 0; q < PL; ++q) mass[wave][lane + 64 * q] = acc[q];
+      for (int q = 0; q < VPL; ++q) z[q] = nxt[q];
+      load_lane<VPL>(logits + (t + ROWS) * E, e0, E, vec, t + ROWS < hi, -INFINITY, nxt);
+      const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, sig);  // (past the end: a row of -inf)
+      z2 += lse * lse;
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) acc[q] += ph[q];
+    }
+    // over the wave's rows
+#pragma unroll
+    for (int o = LPR; o < 64; o <<= 1) {
+      z2 += __shfl_xor(z2, o, 64);
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) acc[q] += __shfl_xor(acc[q], o, 64);
+    }
+    if (row == 0) {
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) mass[wave][e0 + q] = acc[q];
+    }
     if (lane == 0) zs[wave] = z2;
     __syncthreads();
-    const int64_t slot = tile + s;
     for (int e = threadIdx.x; e < E; e += 64 * kWaves) {
       w.mass[slot * E + e] = mass[0][e] + mass[1][e] + mass[2][e] + mass[3][e];
       w.count[slot * E + e] = count[e];
@@ -165,155 +202,126 @@ __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __re
   }
 }
 
-constexpr int kSumThreads = 1024;
+constexpr int kSumThreads = 512;
 
-// One workgroup a sequence: its slots added up, a_se and the sequence's parts of the losses; the workgroup that ends
-// last adds those (their order is the sequences').
+// A workgroup for each sequence and 32 experts: its slots added up, a_se and its parts of the losses; the workgroup that
+// ends last adds those, in the sequences' order.
 __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, Sequences seq, Scratch w,
                                                                  float* __restrict__ a, float* __restrict__ out,
                                                                  float* __restrict__ inv_tokens) {
-  __shared__ double red[kSumThreads / 64][2];
-  __shared__ int64_t tot[kSumThreads / 64][2];
+  constexpr int GROUPS = kSumThreads / kColumns;  // threads of one expert
+  __shared__ double red[GROUPS][kColumns];
+  __shared__ int32_t redc[GROUPS][kColumns];
+  __shared__ double wave_sums[kSumThreads / 64][2];
   __shared__ int last;
-  const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // S' and N
-  int64_t live = 0, tokens = 0;
-  for (int i = threadIdx.x; i < seq.S; i += kSumThreads) {
-    const int64_t n = seq.at(i + 1) - seq.at(i);
-    live += n > 0;
-    tokens += n > 0 ? n : 0;
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    live += __shfl_xor(live, o, 64);
-    tokens += __shfl_xor(tokens, o, 64);
-  }
-  if (lane == 0) {
-    tot[wave][0] = live;
-    tot[wave][1] = tokens;
-  }
-  __syncthreads();
-  live = tokens = 0;
-#pragma unroll
-  for (int i = 0; i < kSumThreads / 64; ++i) {
-    live += tot[i][0];
-    tokens += tot[i][1];
-  }
+  const int s = blockIdx.x, cb = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t lo = seq.at(s), hi = seq.at(s + 1), n = hi > lo ? hi - lo : 0;
   const int64_t first = lo / kTile + s, end = n > 0 ? (hi - 1) / kTile + s + 1 : first;  // its slots
-  const double f = n > 0 ? (double)E / ((double)k * (double)n * (double)n * (double)live) : 0.0;
-  double balance = 0.0, z2 = 0.0;
-  for (int e = threadIdx.x; e < E; e += kSumThreads) {
-    double mass = 0.0;
-    int64_t count = 0;
-    for (int64_t i = first; i < end; ++i) {
+  const int col = threadIdx.x % kColumns, group = threadIdx.x / kColumns, e = cb * kColumns + col;
+  double mass = 0.0;
+  int32_t count = 0;
+  if (e < E) {
+#pragma unroll 4
+    for (int64_t i = first + group; i < end; i += GROUPS) {
       mass += (double)w.mass[i * E + e];
       count += w.count[i * E + e];
     }
-    const double ae = f * (double)count;
-    a[(int64_t)s * E + e] = (float)ae;
-    balance += ae * mass;
   }
-  for (int64_t i = first + threadIdx.x; i < end; i += kSumThreads) z2 += (double)w.zsum[i];
-  auto block_sum = [&](double u, double v, double* to) {
-    u = [&] { double x = u; for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64); return x; }();
-    v = [&] { double x = v; for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64); return x; }();
+  double z2 = 0.0;
+  if (cb == 0)
+    for (int64_t i = first + threadIdx.x; i < end; i += kSumThreads) z2 += (double)w.zsum[i];
+  red[group][col] = mass;
+  redc[group][col] = count;
+  __syncthreads();
+  double balance = 0.0;
+  if (group == 0) {
+    for (int g = 1; g < GROUPS; ++g) {
+      mass += red[g][col];
+      count += redc[g][col];
+    }
+    if (e < E) {
+      const double ae =
+          n > 0 ? (double)E * (double)count / ((double)k * (double)n * (double)n * (double)w.total[0]) : 0.0;
+      a[(int64_t)s * E + e] = (float)ae;
+      balance = ae * mass;
+    }
+  }
+  auto block_sum = [&](double& u, double& v) {  // in thread 0
+    u = lanes_sum<64>(u);
+    v = lanes_sum<64>(v);
     if (lane == 0) {
-      red[wave][0] = u;
-      red[wave][1] = v;
+      wave_sums[wave][0] = u;
+      wave_sums[wave][1] = v;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      to[0] = to[1] = 0.0;
-      for (int i = 0; i < kSumThreads / 64; ++i) {
-        to[0] += red[i][0];
-        to[1] += red[i][1];
+      for (int i = 1; i < kSumThreads / 64; ++i) {
+        u += wave_sums[i][0];
+        v += wave_sums[i][1];
       }
     }
     __syncthreads();
   };
-  double sums[2] = {0.0, 0.0};
-  block_sum(balance, z2, sums);
+  block_sum(balance, z2);
+  const int parts = gridDim.x * gridDim.y;
   if (threadIdx.x == 0) {
-    w.part[2 * s] = sums[0];
-    w.part[2 * s + 1] = sums[1];
+    double* p = w.part + 2 * ((int64_t)s * gridDim.y + cb);
+    __hip_atomic_store(p, balance, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(p + 1, z2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __threadfence();
-    last = atomicAdd(w.done, 1) == seq.S - 1;
+    last = atomicAdd(w.done, 1) == parts - 1;
   }
   __syncthreads();
   if (!last) return;
   __threadfence();
   balance = z2 = 0.0;
-  for (int i = threadIdx.x; i < seq.S; i += kSumThreads) {
-    balance += __hip_atomic_load(&w.part[2 * i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    z2 += __hip_atomic_load(&w.part[2 * i + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = threadIdx.x; i < parts; i += kSumThreads) {
+    balance += __hip_atomic_load(&w.part[2 * (int64_t)i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    z2 += __hip_atomic_load(&w.part[2 * (int64_t)i + 1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  block_sum(balance, z2, sums);
+  block_sum(balance, z2);
   if (threadIdx.x == 0) {
-    const double inv = tokens > 0 ? 1.0 / (double)tokens : 0.0;
-    out[0] = (float)sums[0];
-    out[1] = (float)(sums[1] * inv);
+    const double inv = w.total[1] > 0 ? 1.0 / (double)w.total[1] : 0.0;
+    out[0] = (float)balance;
+    out[1] = (float)(z2 * inv);
     *inv_tokens = (float)inv;
   }
 }
 
-template <int PL, bool SOFT, typename LT>
-__global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* __restrict__ logits, int E,
+// A workgroup has ROWS tokens at a time, a quarter of a tile or so: as many workgroups as keep every CU's loads going.
+template <int LPR, int VPL, bool SOFT, typename LT>
+__global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* __restrict__ logits, int E, bool vec,
                                                                       Sequences seq, const float* __restrict__ a,
                                                                       const float* __restrict__ inv_tokens,
                                                                       const float* __restrict__ g_balance,
                                                                       const float* __restrict__ g_z,
                                                                       LT* __restrict__ dz) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t tile = blockIdx.x, t0 = tile * kTile, t1 = t0 + kTile < seq.T ? t0 + kTile : seq.T;
+  constexpr int TPW = 64 / LPR;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane / LPR, e0 = (lane % LPR) * VPL;
+  const int64_t tw = ((int64_t)blockIdx.x * kWaves + wave) * TPW, t = tw + row;
+  if (tw >= seq.T) return;
+  const bool there = t < seq.T;
+  float z[VPL];
+  load_lane<VPL>(logits + t * E, e0, E, vec, there, -INFINITY, z);
   const float gb = g_balance ? *g_balance : 0.f, gz = g_z ? 2.f * *g_z * *inv_tokens : 0.f;
-  int s = seq.after(t0 + wave);
-  for (int64_t t = t0 + wave; t < t1; t += kWaves) {
-    while (s < seq.S && seq.at(s + 1) <= t) ++s;
-    const bool in = s < seq.S && seq.at(s) <= t;
-    float v[PL];
+  int s = seq.after(tw);
+  while (s < seq.S && seq.at(s + 1) <= t) ++s;
+  const bool in = there && s < seq.S && seq.at(s) <= t;
+  float as[VPL];
+  load_lane<VPL>(a + (int64_t)s * E, e0, E, E % 4 == 0, in, 0.f, as);
+  float ph[VPL], soft[VPL], sig[VPL], dot = 0.f;
+  const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, sig);
 #pragma unroll
-    for (int q = 0; q < PL; ++q) v[q] = 0.f;
-    if (in) {
-      float ph[PL], soft[PL], sig[PL], as[PL], dot = 0.f;
-      const float lse = token_row<PL, SOFT>(logits + t * E, E, lane, ph, soft, sig);
+  for (int q = 0; q < VPL; ++q) dot += ph[q] * as[q];
+  dot = lanes_sum<LPR>(dot);
 #pragma unroll
-      for (int q = 0; q < PL; ++q) {
-        const int e = lane + 64 * q;
-        as[q] = e < E ? a[(int64_t)s * E + e] : 0.f;
-        dot += ph[q] * as[q];
-      }
-      dot = wave_sum(dot);
-#pragma unroll
-      for (int q = 0; q < PL; ++q) {
-        float d = gb * (ph[q] * (as[q] - dot));
-        if constexpr (!SOFT) d *= 1.f - sig[q];
-        v[q] = d + gz * lse * soft[q];
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < PL; ++q) {
-      const int e = lane + 64 * q;
-      if (e < E) dz[t * E + e] = from_f32<LT>(v[q]);
-    }
+  for (int q = 0; q < VPL; ++q) {
+    float d = gb * (ph[q] * (as[q] - dot));
+    if constexpr (!SOFT) d *= 1.f - sig[q];
+    z[q] = in ? d + gz * lse * soft[q] : 0.f;
   }
-}
-
-template <typename F>
-void by_width(int E, bool soft, int dtype, F&& f) {
-  auto typed = [&](auto pl) {
-    auto scored = [&](auto lt) {
-      if (soft) f(pl, std::true_type{}, lt);
-      else f(pl, std::false_type{}, lt);
-    };
-    if (dtype == ZMOE_DTYPE_BF16) scored(uint16_t{});
-    else scored(float{});
-  };
-  if (E <= 64) typed(std::integral_constant<int, 1>{});
-  else if (E <= 128) typed(std::integral_constant<int, 2>{});
-  else if (E <= 256) typed(std::integral_constant<int, 4>{});
-  else if (E <= 512) typed(std::integral_constant<int, 8>{});
-  else typed(std::integral_constant<int, 16>{});
+  if (there) store_lane<VPL>(dz + t * E, e0, E, vec, z);
 }
 
 int check_sizes(const char* what, int dtype, int64_t T, int E, int score, const void* cu, int64_t S) {
@@ -323,7 +331,8 @@ int check_sizes(const char* what, int dtype, int64_t T, int E, int score, const 
   ZMOE_REQUIRE(S >= 1 && S <= ZMOE_ROUTER_LOSSES_MAX_SEQUENCES, ZMOE_ERR_SHAPE, "%s: need 1 to %d sequences (%lld)", what,
                ZMOE_ROUTER_LOSSES_MAX_SEQUENCES, (long long)S);
   ZMOE_REQUIRE(cu || S == 1, ZMOE_ERR_NULL, "%s: null pointer", what);
-  ZMOE_REQUIRE(launch_fits(cdiv(T, kTile), 64 * kWaves), ZMOE_ERR_SHAPE, "%s: too many tokens for one launch", what);
+  // the backward has four tokens a workgroup where E > 256
+  ZMOE_REQUIRE(launch_fits(cdiv(T, kWaves) + 1, 64 * kWaves), ZMOE_ERR_SHAPE, "%s: too many tokens for one launch", what);
   return ZMOE_OK;
 }
 
@@ -352,15 +361,16 @@ extern "C" int zmoe_router_losses(const void* logits, int logits_dtype, int64_t 
   ZMOE_REQUIRE(workspace_bytes >= need, ZMOE_ERR_WORKSPACE, "router_losses: workspace %zu < %zu bytes", workspace_bytes,
                need);
   const Sequences seq{cu_seqlens, cu_int64 != 0, (int)S, T};
-  const unsigned tiles = (unsigned)(T > 0 ? cdiv(T, kTile) : 1);
-  by_width(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto pl, auto soft, auto lt) {
+  const bool vec = rows_on_16(logits, E, E, logits_dtype);
+  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
     using LT = decltype(lt);
-    hipLaunchKernelGGL((losses_tile_kernel<decltype(pl)::value, decltype(soft)::value, LT>), dim3(tiles),
-                       dim3(64 * kWaves), 0, as_stream(stream), (const LT*)logits, topk_idx, E, k, seq, w);
+    hipLaunchKernelGGL((losses_tile_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, LT>),
+                       dim3((unsigned)(cdiv(T, kTile) + 1)), dim3(64 * kWaves), 0, as_stream(stream), (const LT*)logits,
+                       topk_idx, E, k, vec, seq, w);
   });
   if (const int rc = check_launch("router_losses")) return rc;
-  hipLaunchKernelGGL(losses_sum_kernel, dim3((unsigned)S), dim3(kSumThreads), 0, as_stream(stream), E, k, seq, w,
-                     seq_grad, losses, inv_tokens);
+  hipLaunchKernelGGL(losses_sum_kernel, dim3((unsigned)S, (unsigned)column_blocks(E)), dim3(kSumThreads), 0,
+                     as_stream(stream), E, k, seq, w, seq_grad, losses, inv_tokens);
   return check_launch("router_losses");
 }
 
@@ -372,12 +382,15 @@ extern "C" int zmoe_router_losses_backward(const void* logits, int logits_dtype,
   if (T == 0) return ZMOE_OK;
   ZMOE_REQUIRE(logits && seq_grad && inv_tokens && d_logits, ZMOE_ERR_NULL,
                "router_losses_backward: null pointer");
+  ZMOE_REQUIRE(E % 4 != 0 || aligned16(seq_grad), ZMOE_ERR_ALIGN, "router_losses_backward: seq_grad must be 16-byte aligned");
   const Sequences seq{cu_seqlens, cu_int64 != 0, (int)S, T};
-  by_width(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto pl, auto soft, auto lt) {
+  const bool vec = rows_on_16(logits, E, E, logits_dtype) && rows_on_16(d_logits, E, E, logits_dtype);
+  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
     using LT = decltype(lt);
-    hipLaunchKernelGGL((losses_backward_kernel<decltype(pl)::value, decltype(soft)::value, LT>),
-                       dim3((unsigned)cdiv(T, kTile)), dim3(64 * kWaves), 0, as_stream(stream), (const LT*)logits, E, seq,
-                       seq_grad, inv_tokens, d_balance, d_z, (LT*)d_logits);
+    constexpr int rows = kWaves * (64 / decltype(lpr)::value);
+    hipLaunchKernelGGL((losses_backward_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, LT>),
+                       dim3((unsigned)cdiv(T, rows)), dim3(64 * kWaves), 0, as_stream(stream), (const LT*)logits, E, vec,
+                       seq, seq_grad, inv_tokens, d_balance, d_z, (LT*)d_logits);
   });
   return check_launch("router_losses_backward");
 }

@@ -1,5 +1,8 @@
-// What the routing kernels share: sort keys of scores, the sigmoid rounded once, reductions over rows of lanes.
+// What the routing kernels share: sort keys of scores, the sigmoid rounded once, tokens in rows of lanes, reductions over
+// them.
 #pragma once
+
+#include <type_traits>
 
 #include "zmoe_internal.h"
 
@@ -87,6 +90,91 @@ __device__ __forceinline__ float row_sum_f32(float v) {
   v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));
   if (LPR == 16) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));
   return v;
+}
+
+// Over the LPR (8, 16 or 64) lanes of a row; every lane gets the result.
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (LPR == 64) return wave_max_u32(v);
+  else return row_max_u32<LPR>(v);
+}
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
+  if constexpr (LPR == 64) return ~wave_max_u32(~v);
+  else return row_min_u32<LPR>(v);
+}
+template <int LPR, typename F>
+__device__ __forceinline__ F lanes_sum(F v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ float lanes_fmax(float v) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: E and e0 are whole 16-byte chunks and rows lie on 16.
+template <int VPL, typename LT>
+__device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, int E, bool vec, bool live, float fill,
+                                          float (&v)[VPL]) {
+  constexpr int VC = 16 / sizeof(LT);
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < VPL / VC; ++c) {
+      if (live && e0 + c * VC < E) {
+        unpack_chunk(*reinterpret_cast<const uint4*>(row + e0 + c * VC), &v[c * VC], LT{});
+      } else {
+#pragma unroll
+        for (int u = 0; u < VC; ++u) v[c * VC + u] = fill;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < VPL; ++q) v[q] = live && e0 + q < E ? to_f32(row[e0 + q]) : fill;
+  }
+}
+template <int VPL, typename LT>
+__device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, bool vec, const float (&v)[VPL]) {
+  constexpr int VC = 16 / sizeof(LT);
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < VPL / VC; ++c)
+      if (e0 + c * VC < E) *reinterpret_cast<uint4*>(row + e0 + c * VC) = pack_chunk(&v[c * VC], LT{});
+  } else {
+#pragma unroll
+    for (int q = 0; q < VPL; ++q)
+      if (e0 + q < E) row[e0 + q] = from_f32<LT>(v[q]);
+  }
+}
+
+// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts.
+template <typename F>
+void by_lanes(int E, bool soft, int dtype, F&& f) {
+  auto typed = [&](auto lpr, auto vpl) {
+    auto scored = [&](auto lt) {
+      if (soft) f(lpr, vpl, std::true_type{}, lt);
+      else f(lpr, vpl, std::false_type{}, lt);
+    };
+    if (dtype == ZMOE_DTYPE_BF16) scored(uint16_t{});
+    else scored(float{});
+  };
+  using I8 = std::integral_constant<int, 8>;
+  using I16 = std::integral_constant<int, 16>;
+  using I64 = std::integral_constant<int, 64>;
+  if (E <= 64) typed(I8{}, I8{});
+  else if (E <= 128) typed(I16{}, I8{});
+  else if (E <= 256) typed(I16{}, I16{});
+  else if (E <= 512) typed(I64{}, I8{});
+  else typed(I64{}, I16{});
+}
+
+// Whether a matrix of rows of E, ld apart, may be accessed in 16-byte chunks.
+inline bool rows_on_16(const void* base, int64_t ld, int E, int dtype) {
+  const int size = dtype_size(dtype);
+  return aligned16(base) && (ld * size) % 16 == 0 && (E * size) % 16 == 0;
 }
 
 }  // namespace zmoe
