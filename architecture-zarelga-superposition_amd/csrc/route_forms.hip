@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
         m = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int q = 0; q < VPL; ++q) {
-          z[q] = expf(z[q] - m);
+          z[q] = exp_fast(z[q] - m);
           sum += z[q];
         }
         sum = lanes_sum<LPR>(sum);

@@ -97,10 +97,10 @@ __device__ __forceinline__ float token_row(const float (&z)[VPL], float (&ph)[VP
   float sum = 0.f, total = 0.f;
 #pragma unroll
   for (int q = 0; q < VPL; ++q) {
-    soft[q] = expf(z[q] - m);
+    soft[q] = exp_fast(z[q] - m);
     sum += soft[q];
     if constexpr (!SOFT) {
-      sig[q] = 1.f / (1.f + expf(-z[q]));
+      sig[q] = sigmoid_hw(z[q]);
       total += sig[q];
     }
   }

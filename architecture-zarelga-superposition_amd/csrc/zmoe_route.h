@@ -92,6 +92,11 @@ __device__ __forceinline__ float row_sum_f32(float v) {
   return v;
 }
 
+// e^x and the sigmoid in f32 by the hardware's exp2 and reciprocal: off by |x| + 2 roundings (the product with log2 e, and the
+// two instructions); -inf gives 0, +inf inf (1), NaN stays. Where no selection hangs on them.
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
+__device__ __forceinline__ float sigmoid_hw(float x) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-x)); }
+
 // Over the LPR (8, 16 or 64) lanes of a row; every lane gets the result.
 template <int LPR>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
@@ -103,16 +108,58 @@ __device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
   if constexpr (LPR == 64) return ~wave_max_u32(~v);
   else return row_min_u32<LPR>(v);
 }
-template <int LPR, typename F>
-__device__ __forceinline__ F lanes_sum(F v) {
+// (xor 1, xor 2, mirrors within 8 and 16 lanes as above; between rows of 16 by shuffles)
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  const int64_t b = __double_as_longlong(v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, 0xF, 0xF, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, true);
+  return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo));
+}
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp_f32<0xB1>(v);
+  v += dpp_f32<0x4E>(v);
+  v += dpp_f32<0x141>(v);
+  if (LPR >= 16) v += dpp_f32<0x140>(v);
+  if (LPR == 64) {
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+  }
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ double lanes_sum(double v) {
+  v += dpp_f64<0xB1>(v);
+  v += dpp_f64<0x4E>(v);
+  v += dpp_f64<0x141>(v);
+  if (LPR >= 16) v += dpp_f64<0x140>(v);
+  if (LPR == 64) {
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+  }
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ int64_t lanes_sum(int64_t v) {
 #pragma unroll
   for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
 template <int LPR>
 __device__ __forceinline__ float lanes_fmax(float v) {
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  v = fmaxf(v, dpp_f32<0xB1>(v));
+  v = fmaxf(v, dpp_f32<0x4E>(v));
+  v = fmaxf(v, dpp_f32<0x141>(v));
+  if (LPR >= 16) v = fmaxf(v, dpp_f32<0x140>(v));
+  if (LPR == 64) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    v = fmaxf(v, __shfl_xor(v, 32, 64));
+  }
   return v;
 }
 

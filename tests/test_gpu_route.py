@@ -4,8 +4,8 @@ bounds counted from the roundings.
 Tolerances. A probability is rounded once, a weight is a sum of k of them, a quotient and a product: (k + 4) 2^-24 of the
 value. The grad of a sigmoid's or a renormalised softmax's logit goes through two such sums, a quotient and some six
 products of f32 numbers: (2 k + 12) 2^-24 of the magnitudes that it is added up from. Where a softmax is formed again in f32
-(not renormalised) its p is off by |z - max| + 2 roundings in the exponential and its argument, and as much
-again in their sum, which adds at most 16 in a lane and 6 over lanes: 2 (range + 2) + 22 more. Rounding to the grad's type adds
+(not renormalised) its p is off by 2 |z - max| + 2 roundings (the difference, its product with log2 e, the instruction), and as
+much again in their sum, which adds at most 16 in a lane and 6 over lanes: 2 (2 range + 2) + 22 more. Rounding to the grad's type adds
 half a step.
 """
 
@@ -52,7 +52,7 @@ def check(z, k, bias=None, score="sigmoid", groups=1, top_groups=1, group_scores
     val, mag = O.weights_backward(z, idx, dw, score, renormalize, scale)
     zf = z.float()
     span = (zf.amax(-1) - zf.masked_fill(zf == -math.inf, math.inf).amin(-1)).nan_to_num(0, 0, 0).clamp(0, 200).max() if z.numel() else 0
-    again = 0 if score == "sigmoid" or renormalize else 2 * (float(span) + 2) + 22
+    again = 0 if score == "sigmoid" or renormalize else 2 * (2 * float(span) + 2) + 22
     assert leaf.grad.dtype == z.dtype
     close("d logits", leaf.grad, val, mag, 2 * k + 12 + again)
     with torch.no_grad():

@@ -1,7 +1,8 @@
 """zmoe.functional.router_losses on the GPU against float64 (oracle.router_oracle).
 
-Tolerances. A share ph = p / sum p is off by |z| + 2 roundings in the exponential and its argument and as many in the sum,
-which adds at most 16 in a lane and 6 over lanes, and 3 in quotients: 2 (range + 2) + 25 =: u units of 2^-24, range the largest
+Tolerances. An exponential is off by 2 |z| + 2 roundings: the difference z - max and its product with log2 e, each rounded to
+2^-24 of it, and the instruction itself (and one more for a reciprocal). A share ph = p / sum p has those, as many in the sum,
+which adds at most 16 in a lane and 6 over lanes, and 3 in quotients: 2 (2 range + 2) + 25 =: u units of 2^-24, range the largest
 |z - max| (or |z| for a sigmoid) of the inputs. The losses add up shares of up to 16 tokens in f32 and the rest in double, and
 are rounded once: u + 16 + 2 (twice u for the square of the logsumexp, which is a logarithm of such a sum: off by u / |lse|
 units at most, and lse^2 is its own magnitude where |lse| >= 1; below, u 2^-24 absolute). A grad has two shares, a sum over a row of
@@ -30,7 +31,7 @@ def units(z, score):
     f = z.float()
     f = f[torch.isfinite(f) & (f > torch.finfo(z.dtype).min)]
     span = 0.0 if f.numel() == 0 else float(f.abs().max()) * (2 if score == "softmax" else 1)
-    return 2 * (span + 2) + 25
+    return 2 * (2 * span + 2) + 25
 
 
 def check(z, idx, score, cu=None, gb=0.3, gz=0.05):
