@@ -22,6 +22,7 @@ struct RouteArgs {
   const float* bias;  // or null
   int64_t T;
   int E, k, groups, top_groups, group_scores, renorm, vec;
+  int lanes_of_group;  // where a group is whole lanes, a power of two of them; else 0
   float scale;
   int64_t* idx;
   float* w;
@@ -71,16 +72,16 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
       double e[VPL], sum = 0.0;
 #pragma unroll
       for (int q = 0; q < VPL; ++q) {
-        e[q] = exp((double)z[q] - (double)m);
+        e[q] = exp_f64((double)z[q] - (double)m);
         sum += e[q];
       }
       sum = lanes_sum<LPR>(sum);
-      const double inv = sum == 0.0 ? 0.0 : 1.0 / sum;
+      const double inv = sum == 0.0 ? 0.0 : rcp_f64(sum);
 #pragma unroll
       for (int q = 0; q < VPL; ++q) p[q] = (float)(e[q] * inv);
     } else {
 #pragma unroll
-      for (int q = 0; q < VPL; ++q) p[q] = sigmoid_f64(z[q]);
+      for (int q = 0; q < VPL; ++q) p[q] = sigmoid_rounded(z[q]);
     }
     uint32_t key[VPL];
 #pragma unroll
@@ -89,46 +90,75 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
       ps[wave][row][e0 + q] = p[q];
     }
     if (G > 1) {
+      constexpr int PER = (64 + LPR - 1) / LPR;  // groups of a lane
+      uint32_t mine[PER];
+      if (a.lanes_of_group) {  // a group is whole lanes, a power of two of them: its first lane speaks for it
+        uint32_t k1 = 0, k2 = 0;
 #pragma unroll
-      for (int q = 0; q < VPL; ++q) gk[wave][row][e0 + q] = two && !by_p ? score_key(p[q]) : key[q];
-      wave_sync();
-      // lane r scores groups r, r + LPR, ...; the best top_groups of them in rounds
-      uint32_t mine[(64 + LPR - 1) / LPR];
+        for (int q = 0; q < VPL; ++q) {
+          const uint32_t v = two && !by_p ? (live && e0 + q < E ? score_key(p[q]) : 0u) : key[q];
+          k2 = max(k2, min(k1, v));
+          k1 = max(k1, v);
+        }
+        for (int o = 1; o < a.lanes_of_group; o <<= 1) {
+          const uint32_t o1 = __shfl_xor(k1, o, 64), o2 = __shfl_xor(k2, o, 64);
+          k2 = max(max(k2, o2), min(k1, o1));
+          k1 = max(k1, o1);
+        }
+        mine[0] = live && e0 < E && r % a.lanes_of_group == 0 ? (two ? score_key(key_score(k1) + key_score(k2)) : k1) : 0u;
 #pragma unroll
-      for (int i = 0; i < (64 + LPR - 1) / LPR; ++i) {
-        const int g = r + i * LPR;
-        mine[i] = 0;
-        if (g < G && live) {
-          uint32_t k1 = 0, k2 = 0;
-          for (int u = 0; u < gsz; ++u) {
-            const uint32_t v = gk[wave][row][g * gsz + u];
-            k2 = max(k2, min(k1, v));
-            k1 = max(k1, v);
+        for (int i = 1; i < PER; ++i) mine[i] = 0;
+      } else {
+#pragma unroll
+        for (int q = 0; q < VPL; ++q) gk[wave][row][e0 + q] = two && !by_p ? score_key(p[q]) : key[q];
+        wave_sync();
+        // lane r scores groups r, r + LPR, ..., each lane from a place of its own (banks)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int g = r + i * LPR;
+          mine[i] = 0;
+          if (g < G && live) {
+            uint32_t k1 = 0, k2 = 0;
+            int at = r % gsz;
+#pragma unroll 4
+            for (int u = 0; u < gsz; ++u) {
+              const uint32_t v = gk[wave][row][g * gsz + at];
+              at = at + 1 == gsz ? 0 : at + 1;
+              k2 = max(k2, min(k1, v));
+              k1 = max(k1, v);
+            }
+            mine[i] = two ? score_key(key_score(k1) + key_score(k2)) : k1;
           }
-          mine[i] = two ? score_key(key_score(k1) + key_score(k2)) : k1;
         }
       }
-      uint64_t keep = 0;  // the same in a row's lanes
+      const int scale_g = a.lanes_of_group ? a.lanes_of_group : 1;  // lane r speaks for group r / scale_g
+      uint64_t keep = 0;  // by speakers, the same in a row's lanes
       for (int j = 0; j < a.top_groups; ++j) {
         uint32_t m = mine[0];
 #pragma unroll
-        for (int i = 1; i < (64 + LPR - 1) / LPR; ++i) m = max(m, mine[i]);
+        for (int i = 1; i < PER; ++i) m = max(m, mine[i]);
         m = lanes_max<LPR>(m);
         uint32_t g = 0xffffffffu;
 #pragma unroll
-        for (int i = (64 + LPR - 1) / LPR - 1; i >= 0; --i) g = mine[i] == m ? (uint32_t)(r + i * LPR) : g;
+        for (int i = PER - 1; i >= 0; --i) g = mine[i] == m ? (uint32_t)(r + i * LPR) : g;
         g = lanes_min<LPR>(g);
         keep |= 1ull << (g & 63);
 #pragma unroll
-        for (int i = 0; i < (64 + LPR - 1) / LPR; ++i) mine[i] = (uint32_t)(r + i * LPR) == g ? 0u : mine[i];
+        for (int i = 0; i < PER; ++i) mine[i] = (uint32_t)(r + i * LPR) == g ? 0u : mine[i];
       }
-      int g = e0 / gsz, left = gsz - (e0 - g * gsz);
+      if (a.lanes_of_group) {
+        const bool stays = (keep >> ((r / scale_g * scale_g) & 63)) & 1;
 #pragma unroll
-      for (int q = 0; q < VPL; ++q) {
-        key[q] = (keep >> (g & 63)) & 1 ? key[q] : 0u;
-        if (--left == 0) {
-          left = gsz;
-          ++g;
+        for (int q = 0; q < VPL; ++q) key[q] = stays ? key[q] : 0u;
+      } else {
+        int g = e0 / gsz, left = gsz - (e0 - g * gsz);
+#pragma unroll
+        for (int q = 0; q < VPL; ++q) {
+          key[q] = (keep >> (g & 63)) & 1 ? key[q] : 0u;
+          if (--left == 0) {
+            left = gsz;
+            ++g;
+          }
         }
       }
     }
@@ -137,13 +167,23 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
 #pragma unroll
       for (int q = 1; q < VPL; ++q) m = max(m, key[q]);
       m = lanes_max<LPR>(m);
-      uint32_t e = 0xffffffffu;  // this lane's lowest expert holding m, then the row's
+      // this lane's lowest expert holding m, then the row's; that one is taken (the lane's first hit, by wave masks)
+      uint64_t hit[VPL];
 #pragma unroll
-      for (int q = VPL - 1; q >= 0; --q) e = key[q] == m ? (uint32_t)(e0 + q) : e;
-      e = lanes_min<LPR>(e);
+      for (int q = 0; q < VPL; ++q) hit[q] = __builtin_amdgcn_ballot_w64(key[q] == m);
+      uint32_t e = 0xffffffffu;
 #pragma unroll
-      for (int q = 0; q < VPL; ++q) key[q] = (uint32_t)(e0 + q) == e ? 0u : key[q];
-      if (r == 0) slots[wave][row][j] = (uint16_t)e;
+      for (int q = VPL - 1; q >= 0; --q) e = __builtin_amdgcn_inverse_ballot_w64(hit[q]) ? (uint32_t)(e0 + q) : e;
+      const uint32_t best = lanes_min<LPR>(e);
+      const uint64_t owner = __builtin_amdgcn_ballot_w64(e == best);
+      uint64_t seen = 0;
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) {
+        const uint64_t first = hit[q] & owner & ~seen;
+        seen |= hit[q];
+        key[q] = __builtin_amdgcn_inverse_ballot_w64(first) ? 0u : key[q];
+      }
+      if (r == 0) slots[wave][row][j] = (uint16_t)best;
     }
     wave_sync();
     float sum = 0.f;
@@ -279,12 +319,15 @@ extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E
                "route: need 1 <= k <= %d and experts to choose from (k=%d, %d)", kMaxSlots, k, top_groups * (E / groups));
   if (T == 0) return ZMOE_OK;
   ZMOE_REQUIRE(logits && topk_idx && topk_weight, ZMOE_ERR_NULL, "route: null pointer");
-  const RouteArgs a{logits, expert_biases, T, E, k, groups, top_groups, group_scores, renormalize,
-                    rows_on_16(logits, E, E, logits_dtype), scale, topk_idx, topk_weight, topk_prob};
-  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, [&](auto lpr, auto vpl, auto soft, auto lt) {
+  RouteArgs a{logits, expert_biases, T, E, k, groups, top_groups, group_scores, renormalize,
+              rows_on_16(logits, E, E, logits_dtype), 0, scale, topk_idx, topk_weight, topk_prob};
+  auto go = [&](auto lpr, auto vpl, auto soft, auto lt) {
+    const int lanes = E / groups / decltype(vpl)::value;
+    a.lanes_of_group = lanes * decltype(vpl)::value == E / groups && (lanes & (lanes - 1)) == 0 ? lanes : 0;
     hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
                        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
-  });
+  };
+  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, go);
   return check_launch("route");
 }
 

@@ -92,6 +92,42 @@ __device__ __forceinline__ float row_sum_f32(float v) {
   return v;
 }
 
+// e^x in double, x below 709 (e^-745 and less are 0; NaN stays): x = n ln 2 + r with |r| <= ln 2 / 2, ln 2 as a sum of two numbers
+// of which the first has so few bits that n times it is exact, and Taylor's polynomial of degree 12, whose first missing
+// term is below 2^-52.
+__device__ __forceinline__ double exp_f64(double x) {
+  x = x < -760.0 ? -760.0 : x;
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, -0x1.62e42fee00000p-1, x);
+  r = fma(n, -0x1.a39ef35793c76p-33, r);
+  double p = 1.0 / 479001600.0;
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, (int)n);
+}
+// 1 / x in double for a normal x with a normal reciprocal, to a rounding or two: two steps of Newton's from v_rcp_f64.
+__device__ __forceinline__ double rcp_f64(double x) {
+  double y = __builtin_amdgcn_rcp(x);
+  y = fma(fma(-x, y, 1.0), y, y);
+  return fma(fma(-x, y, 1.0), y, y);
+}
+// sigmoid_f64 of a logit by these two.
+__device__ __forceinline__ float sigmoid_rounded(float z) {
+  if (fabsf(z) < kSigmoidSeriesBelow) return sigmoid_f64(z);  // (exact ties)
+  const float p = (float)rcp_f64(1.0 + exp_f64(-(double)z));
+  return z <= kSigmoidZeroBelow ? 0.f : p;
+}
+
 // e^x and the sigmoid in f32 by the hardware's exp2 and reciprocal: off by |x| + 2 roundings (the product with log2 e, and the
 // two instructions); -inf gives 0, +inf inf (1), NaN stays. Where no selection hangs on them.
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
@@ -168,7 +204,7 @@ template <int VPL, typename LT>
 __device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, int E, bool vec, bool live, float fill,
                                           float (&v)[VPL]) {
   constexpr int VC = 16 / sizeof(LT);
-  if (vec) {
+  if (VPL >= VC && vec) {
 #pragma unroll
     for (int c = 0; c < VPL / VC; ++c) {
       if (live && e0 + c * VC < E) {
