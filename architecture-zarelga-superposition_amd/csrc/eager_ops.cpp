@@ -13,6 +13,7 @@
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -1013,6 +1014,82 @@ Tensors norm_residual_backward(const Opt& dR_out, const Opt& dX, const Tensor& R
   return op.call(dR_out, dX, R, Y, w1, w2, gate, kind, scale, scale_value, rho1, rho2);
 }
 
+// ------------------------------------------------------------------ autograd functions
+// route and router_losses with their gradients as C++ nodes, for calls with gradients on (zmoe/functional.py): a pass of a
+// few hundred tokens is bound by its host time, half of it the Python function's (ctx, apply, backward: 86 -> 45 us a
+// training pass of route). Under create_graph the backward calls the general form, which refuses a second derivative.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+Opt given(const at::Tensor& t) { return t.defined() ? Opt(t) : std::nullopt; }
+
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Opt& bias, int64_t k, int64_t score,
+                               int64_t groups, int64_t top_groups, int64_t group_scores, bool renorm, double scale) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensors out = route(logits, bias, k, score, groups, top_groups, group_scores, renorm, scale);
+    ctx->save_for_backward({out[2], out[0], logits});
+    ctx->saved_data["score"] = score;
+    ctx->saved_data["renorm"] = renorm;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({out[0]});
+    ctx->set_materialize_grads(false);
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list none(9);
+    if (!grads[1].defined()) return none;
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t score = ctx->saved_data["score"].toInt();
+    const bool renorm = ctx->saved_data["renorm"].toBool();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    if (at::GradMode::is_enabled()) {
+      static const auto op = general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, c10::SymInt, bool,
+                                            double)>("zmoe::route_backward");
+      none[0] = op.call(grads[1], saved[0], saved[1], saved[2], score, renorm, scale);
+    } else {
+      none[0] = route_backward(grads[1], saved[0], saved[1], saved[2], score, renorm, scale);
+    }
+    return none;
+  }
+};
+
+Tensors route_grad(const Tensor& logits, const Opt& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups,
+                   int64_t group_scores, bool renorm, double scale) {
+  return RouteFunction::apply(logits, bias, k, score, groups, top_groups, group_scores, renorm, scale);
+}
+
+struct RouterLossesFunction : torch::autograd::Function<RouterLossesFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& idx, const Opt& cu,
+                               int64_t score) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensors out = router_losses(logits, idx, cu, score);
+    ctx->save_for_backward({logits, cu ? *cu : Tensor(), out[1], out[2]});
+    ctx->saved_data["score"] = score;
+    ctx->set_materialize_grads(false);
+    return {out[0].select(0, 0), out[0].select(0, 1)};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list none(4);
+    if (!grads[0].defined() && !grads[1].defined()) return none;
+    const variable_list saved = ctx->get_saved_variables();
+    const int64_t score = ctx->saved_data["score"].toInt();
+    const Opt gb = given(grads[0]), gz = given(grads[1]), cu = given(saved[1]);
+    if (at::GradMode::is_enabled()) {
+      static const auto op = general<Tensor(const Opt&, const Opt&, const Tensor&, const Opt&, c10::SymInt, const Tensor&,
+                                            const Tensor&)>("zmoe::router_losses_backward");
+      none[0] = op.call(gb, gz, saved[0], cu, score, saved[2], saved[3]);
+    } else {
+      none[0] = router_losses_backward(gb, gz, saved[0], cu, score, saved[2], saved[3]);
+    }
+    return none;
+  }
+};
+
+Tensors router_losses_grad(const Tensor& logits, const Tensor& idx, const Opt& cu, int64_t score) {
+  return RouterLossesFunction::apply(logits, idx, cu, score);
+}
+
 // ------------------------------------------------------------------ mutating building blocks
 void rowwise_sum_product(const Tensor& out, const Tensor& A, const Tensor& B) {
   if (A.is_cuda() && known(A) && A.dim() == 3 && A.is_contiguous() && on(B, A) && known(B) && B.dim() == 2 &&
@@ -1076,6 +1153,10 @@ void groupXtY(int64_t E, const Tensor& DW, const Opt& Db, const Tensor& DY, cons
   m.impl(#name, c10::DispatchKey::CompositeExplicitAutograd, TORCH_FN(name))
 
 TORCH_LIBRARY(zmoe_eager, m) {
+  m.def("route_grad(Tensor logits, Tensor? expert_biases, int k, int score, int groups, int top_groups, int group_scores, "
+        "bool renormalize, float scale) -> Tensor[]", TORCH_FN(route_grad));
+  m.def("router_losses_grad(Tensor logits, Tensor topk_idx, Tensor? cu_seqlens, int score) -> Tensor[]",
+        TORCH_FN(router_losses_grad));
   ZMOE_EAGER(route_topk, "(Tensor logits, Tensor expert_biases, int k, bool round_probs_bf16) -> Tensor[]");
   ZMOE_EAGER(swiglu_route_backward,
              "(Tensor dAs, Tensor Hs, Tensor d_gates, Tensor topk_prob, Tensor topk_idx, int num_experts) -> Tensor");

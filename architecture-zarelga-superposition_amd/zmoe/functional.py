@@ -314,7 +314,8 @@ def route(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, sco
     flat = logits if logits.dim() == 2 else logits.reshape(-1, E)
     args = (flat, bias, int(k), code, int(groups), int(top_groups), int(group_scores), bool(renormalize), scale)
     if _needs_graph(logits):
-        idx, w = _Route.apply(*args)
+        node = zl.native_node("route_grad", args)
+        idx, w = _Route.apply(*args) if node is None else node(*args)
     else:
         with torch.no_grad():
             idx, w, _ = zl.route(*args)
@@ -352,4 +353,11 @@ def router_losses(logits: torch.Tensor, topk_idx: torch.Tensor, score: str = "si
     E, code = logits.shape[-1], _score(score)
     flat = logits.reshape(-1, E)
     idx = topk_idx.reshape(-1, topk_idx.shape[-1])
-    return _RouterLosses.apply(flat, idx, cu_seqlens, code)
+    args = (flat, idx, cu_seqlens, code)
+    if not _needs_graph(logits):
+        with torch.no_grad():
+            losses = zl.router_losses(*args)[0]
+        return losses[0], losses[1]
+    node = zl.native_node("router_losses_grad", args)
+    balance, z = _RouterLosses.apply(*args) if node is None else node(*args)
+    return balance, z

@@ -60,6 +60,27 @@ def _watched_by_function_mode() -> bool:
     return any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(_function_modes()))
 
 
+def _watched() -> bool:
+    """Whether what is active knows the ops by their zmoe:: names or has rules registered on them: a compiler or tracer, a
+    dispatch or function mode, a functorch transform, forward-mode AD, zmoe.profiling."""
+    return bool(_compiling() or _dispatch_modes() or _transforms() or _forward_ad._current_level >= 0 or _tracing()
+                or profiling.active() or (_function_modes() and _watched_by_function_mode()))
+
+
+_nodes: dict = {}
+
+
+def native_node(name: str, args: tuple):
+    """The C++ autograd function ``zmoe_eager::<name>`` for these arguments, or None where the Python one has to run."""
+    if _watched() or not _plain(map(type, args)):
+        return None
+    op = _nodes.get(name)
+    if op is None:
+        _load_eager()
+        op = _nodes[name] = getattr(torch.ops.zmoe_eager, name).default._op
+    return op
+
+
 class LayerOp(torch.library.CustomOpDef):
     """The custom op ``zmoe::<name>``, whose eager calls with gradients off run the native
     ``zmoe_eager::<name>`` of csrc/eager_ops.cpp.
