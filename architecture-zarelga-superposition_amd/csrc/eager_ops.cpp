@@ -1090,6 +1090,79 @@ Tensors router_losses_grad(const Tensor& logits, const Tensor& idx, const Opt& c
   return RouterLossesFunction::apply(logits, idx, cu, score);
 }
 
+// ------------------------------------------------------------------ the optimizer's step
+// AdamW's step over lists of tensors (zmoe/adamw.py): false where the general form (zmoe.ops) has to run or raise. Its host
+// time is this: 16 tensors 50 us with their descriptions written from Python, 8 here.
+bool dense_like(const Tensor& t, const Tensor& p) {
+  return t.is_cuda() && t.device() == p.device() && t.layout() == at::kStrided && t.sizes() == p.sizes() &&
+         t.strides() == p.strides();
+}
+
+bool adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avgs, const Tensors& exp_avg_sqs,
+                const Tensors& avg_scales, const Tensors& sq_scales, const Tensors& steps, int64_t state_bits,
+                const Opt& lr_t, double lr, double beta1, double beta2, double eps, double weight_decay,
+                const Opt& clip) {
+  const size_t n = params.size();
+  const bool eight = state_bits == 8;
+  if (n == 0 || !fits_int((int64_t)n) || grads.size() != n || exp_avgs.size() != n || exp_avg_sqs.size() != n ||
+      steps.size() != n || (eight && (avg_scales.size() != n || sq_scales.size() != n)) || !fits_int(state_bits))
+    return false;
+  const Tensor& first = params[0];
+  if (!first.is_cuda() || !known(first)) return false;
+  auto number = [&](const Opt& t) { return !t || (flat(*t, first, at::kFloat) && t->numel() == 1); };
+  if (!number(lr_t) || !number(clip)) return false;
+  std::vector<zmoe_adamw_tensor> table(n);
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor &p = params[i], &g = grads[i], &m = exp_avgs[i], &v = exp_avg_sqs[i], &t = steps[i];
+    const int64_t blocks = (p.numel() + 255) / 256;
+    if (!on(p, first) || p.scalar_type() != first.scalar_type() || g.scalar_type() != p.scalar_type() ||
+        !dense_like(g, p) || !dense_like(m, p) || !dense_like(v, p) || !p.is_non_overlapping_and_dense() ||
+        m.scalar_type() != (eight ? at::kChar : at::kFloat) || v.scalar_type() != (eight ? at::kByte : at::kFloat) ||
+        !flat(t, first, at::kFloat) || t.numel() != 1)
+      return false;
+    if (eight && !(flat(avg_scales[i], first, at::kFloat) && avg_scales[i].numel() == blocks &&
+                   flat(sq_scales[i], first, at::kFloat) && sq_scales[i].numel() == blocks))
+      return false;
+    table[i] = {raw(p), raw(g), raw(m), raw(v), eight ? ptr<float>(avg_scales[i]) : nullptr,
+                eight ? ptr<float>(sq_scales[i]) : nullptr, ptr<float>(t), p.numel()};
+  }
+  const c10::DeviceGuard guard(first.device());
+  Tensor ws = workspace(16 * n, first);
+  if (zmoe_adamw(table.data(), (int)n, code(first), (int)state_bits, lr_t ? ptr<const float>(*lr_t) : nullptr, lr, beta1,
+                 beta2, eps, weight_decay, clip ? ptr<const float>(*clip) : nullptr, ptr<float>(ws), 16 * n,
+                 stream_of(first)) != ZMOE_OK)
+    return false;
+  for (const Tensors* list : {&params, &exp_avgs, &exp_avg_sqs, &avg_scales, &sq_scales, &steps})
+    for (const Tensor& t : *list) t.unsafeGetTensorImpl()->bump_version();
+  return true;
+}
+
+// [norm, factor] of tensors of one type; undefined where the general form has to run.
+Opt grad_norm(const Tensors& grads, double max_norm) {
+  if (grads.empty() || !fits_int((int64_t)grads.size())) return std::nullopt;
+  const Tensor& first = grads[0];
+  if (!first.is_cuda() || !known(first)) return std::nullopt;
+  std::vector<const void*> at(grads.size());
+  std::vector<int64_t> n(grads.size());
+  size_t bytes = 0;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& g = grads[i];
+    if (!on(g, first) || g.layout() != at::kStrided || g.scalar_type() != first.scalar_type() ||
+        !g.is_non_overlapping_and_dense())
+      return std::nullopt;
+    at[i] = raw(g);
+    n[i] = g.numel();
+    bytes += zmoe_sum_squares_workspace_bytes(n[i]);
+  }
+  const c10::DeviceGuard guard(first.device());
+  Tensor parts = workspace(bytes, first), out = empty({2}, first, at::kFloat);
+  if (zmoe_sum_squares(at.data(), n.data(), (int)at.size(), code(first), ptr<double>(parts), stream_of(first)) != ZMOE_OK ||
+      zmoe_clip_factor(ptr<double>(parts), (int64_t)bytes / 8, (float)max_norm, ptr<float>(out), stream_of(first)) !=
+          ZMOE_OK)
+    return std::nullopt;
+  return out;
+}
+
 // ------------------------------------------------------------------ mutating building blocks
 void rowwise_sum_product(const Tensor& out, const Tensor& A, const Tensor& B) {
   if (A.is_cuda() && known(A) && A.dim() == 3 && A.is_contiguous() && on(B, A) && known(B) && B.dim() == 2 &&
@@ -1235,6 +1308,11 @@ TORCH_LIBRARY(zmoe_eager, m) {
   ZMOE_EAGER(norm_residual_backward,
              "(Tensor? dR_out, Tensor? dX, Tensor R, Tensor Y, Tensor? w_post, Tensor? w_next, Tensor? gate, "
              "int gate_kind, Tensor? scale, float scale_value, Tensor? rstd_post, Tensor? rstd_next) -> Tensor[]");
+  ZMOE_EAGER(adamw_step,
+             "(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
+             "Tensor(d!)[] avg_scales, Tensor(e!)[] sq_scales, Tensor(f!)[] steps, int state_bits, Tensor? lr_t, float lr, "
+             "float beta1, float beta2, float eps, float weight_decay, Tensor? clip) -> bool");
+  ZMOE_EAGER(grad_norm, "(Tensor[] grads, float max_norm) -> Tensor?");
   ZMOE_EAGER(rowwise_sum_product, "(Tensor(a!) output, Tensor A, Tensor B) -> ()");
   ZMOE_EAGER(group,
              "(Tensor A, int K, int N, Tensor(a!) Y, Tensor? coeff, bool has_coeff, int fan_out, "

@@ -13,7 +13,7 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from . import library, ops, profiling
 
 _STATE_DTYPES = {32: (torch.float32, torch.float32), 8: (torch.int8, torch.uint8)}
 
@@ -104,46 +104,66 @@ class AdamW(torch.optim.Optimizer):
         work, all_grads = [], []
         for group in self.param_groups:
             bits = group["state_bits"]
-            lists: dict = {}  # by device and dtype: (params, grads, m, v, m scales, v scales, steps)
+            lists = [], [], [], [], [], [], []  # params, grads, m, v, m scales, v scales, steps
+            ps, gs, ms, vs, sms, svs, ts = lists
             for p in group["params"]:
                 g = p.grad
                 if g is None:
                     continue
-                if g.is_sparse:
-                    raise RuntimeError("AdamW: sparse grads are not supported")
-                if g.dtype != p.dtype:
-                    raise RuntimeError(f"AdamW: a grad of {g.dtype} for a parameter of {p.dtype}")
-                if g.stride() != p.stride():  # the parameter's order in memory
-                    g = torch.empty_like(p).copy_(g)
-                st = self._state_of(p, bits)
-                key = (p.device, p.dtype)
-                to = lists.get(key)
-                if to is None:
-                    to = lists[key] = ([], [], [], [], [], [], [])
-                to[0].append(p)
-                to[1].append(g)
-                to[2].append(st["exp_avg"])
-                to[3].append(st["exp_avg_sq"])
+                st = self.state.get(p) or self._state_of(p, bits)
+                ps.append(p)
+                gs.append(g)
+                ms.append(st["exp_avg"])
+                vs.append(st["exp_avg_sq"])
+                ts.append(st["step"])
                 if bits == 8:
-                    to[4].append(st["exp_avg_scale"])
-                    to[5].append(st["exp_avg_sq_scale"])
-                to[6].append(st["step"])
-                all_grads.append(g)
-            if lists:
+                    sms.append(st["exp_avg_scale"])
+                    svs.append(st["exp_avg_sq_scale"])
+            if ps:
                 work.append((group, lists))
+                all_grads += gs
+        if not work:
+            return loss
+        native = None if profiling.active() else library.native_node("adamw_step", ())
         clip = None
-        if self.max_grad_norm is not None and all_grads:
-            norm = ops.grad_norm(all_grads, self.max_grad_norm)
+        if self.max_grad_norm is not None:
+            norm = None if native is None else library.native_node("grad_norm", ())(all_grads, self.max_grad_norm)
+            if norm is None:
+                for _, lists in work:
+                    self._in_order(lists)
+                norm = ops.grad_norm([g for _, lists in work for g in lists[1]], self.max_grad_norm)
             self.grad_norm, clip = norm[0], norm[1]
         for group, lists in work:
             lr = group["lr"]
             if isinstance(lr, torch.Tensor) and not lr.is_cuda:
                 lr = float(lr)
+            lr_t, lr = (lr, 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
             b1, b2 = group["betas"]
-            for to in lists.values():
-                ops.adamw_(*to, group["state_bits"], lr, b1, b2, group["eps"], group["weight_decay"], clip)
-                torch.autograd.graph.increment_version(to[0])
+            if native is not None and native(*lists, group["state_bits"], lr_t, lr, b1, b2, group["eps"],
+                                             group["weight_decay"], clip):
+                continue
+            self._in_order(lists)
+            by: dict = {}  # one call for each device and type
+            for i, p in enumerate(lists[0]):
+                for to, of in zip(by.setdefault((p.device, p.dtype), ([], [], [], [], [], [], [])), lists):
+                    if of:
+                        to.append(of[i])
+            for to in by.values():
+                ops.adamw_(*to, group["state_bits"], lr if lr_t is None else lr_t, b1, b2, group["eps"],
+                           group["weight_decay"], clip)
+                torch.autograd.graph.increment_version([t for some in (to[0], *to[2:]) for t in some])
         return loss
+
+    @staticmethod
+    def _in_order(lists) -> None:
+        """The grads as the kernels take them: dense, of the parameter's type and order in memory."""
+        for i, (p, g) in enumerate(zip(lists[0], lists[1])):
+            if g.layout != torch.strided:
+                raise RuntimeError("AdamW: sparse grads are not supported")
+            if g.dtype != p.dtype:
+                raise RuntimeError(f"AdamW: a grad of {g.dtype} for a parameter of {p.dtype}")
+            if g.stride() != p.stride():
+                lists[1][i] = torch.empty_like(p).copy_(g)
 
     @torch.no_grad()
     def moments(self) -> list:
