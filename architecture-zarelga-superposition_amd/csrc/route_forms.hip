@@ -22,7 +22,9 @@ struct RouteArgs {
   const float* bias;  // or null
   int64_t T;
   int E, k, groups, top_groups, group_scores, renorm, vec;
-  int lanes_of_group;  // where a group is whole lanes, a power of two of them; else 0
+  int lanes_of_group;  // where a group is whole lanes, a power of two of them; else 0, and
+  int lanes_together;  // so many lanes score a group
+  int inv_group;       // 2^20 / experts of a group, rounded up
   float scale;
   int64_t* idx;
   float* w;
@@ -34,6 +36,19 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// x as a value that the compiler knows nothing of (so nothing computed from it leaves the loop).
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// score_key in fewer instructions: -0 goes with +0 by an addition.
+__device__ __forceinline__ uint32_t order_key(float s) {
+  const uint32_t b = __float_as_uint(s + 0.f);
+  const uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return s != s ? 0xffffffffu : key;
 }
 
 // The float whose score_key is key (a NaN, +0 for both zeros).
@@ -80,23 +95,24 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
 #pragma unroll
       for (int q = 0; q < VPL; ++q) p[q] = (float)(e[q] * inv);
     } else {
-#pragma unroll
-      for (int q = 0; q < VPL; ++q) p[q] = sigmoid_rounded(z[q]);
+      sigmoids_rounded(z, p);
     }
+    const int have = live ? opaque(E - e0) : 0;  // of this lane's experts (not kept in masks over the loop: registers)
     uint32_t key[VPL];
 #pragma unroll
     for (int q = 0; q < VPL; ++q) {
-      key[q] = live && e0 + q < E ? score_key(by_p ? p[q] + b[q] : z[q]) : 0u;
+      key[q] = q < have ? order_key(by_p ? p[q] + b[q] : z[q]) : 0u;
       ps[wave][row][e0 + q] = p[q];
     }
     if (G > 1) {
       constexpr int PER = (64 + LPR - 1) / LPR;  // groups of a lane
+      const int share = a.lanes_together;
       uint32_t mine[PER];
       if (a.lanes_of_group) {  // a group is whole lanes, a power of two of them: its first lane speaks for it
         uint32_t k1 = 0, k2 = 0;
 #pragma unroll
         for (int q = 0; q < VPL; ++q) {
-          const uint32_t v = two && !by_p ? (live && e0 + q < E ? score_key(p[q]) : 0u) : key[q];
+          const uint32_t v = two && !by_p ? (q < have ? order_key(p[q]) : 0u) : key[q];
           k2 = max(k2, min(k1, v));
           k1 = max(k1, v);
         }
@@ -105,34 +121,38 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
           k2 = max(max(k2, o2), min(k1, o1));
           k1 = max(k1, o1);
         }
-        mine[0] = live && e0 < E && r % a.lanes_of_group == 0 ? (two ? score_key(key_score(k1) + key_score(k2)) : k1) : 0u;
+        mine[0] = live && e0 < E && r % a.lanes_of_group == 0 ? (two ? order_key(key_score(k1) + key_score(k2)) : k1) : 0u;
 #pragma unroll
         for (int i = 1; i < PER; ++i) mine[i] = 0;
       } else {
 #pragma unroll
-        for (int q = 0; q < VPL; ++q) gk[wave][row][e0 + q] = two && !by_p ? score_key(p[q]) : key[q];
+        for (int q = 0; q < VPL; ++q) gk[wave][row][e0 + q] = two && !by_p ? order_key(p[q]) : key[q];
         wave_sync();
-        // lane r scores groups r, r + LPR, ..., each lane from a place of its own (banks)
+        // share lanes score a group together (a power of two, one where there are more groups than half the lanes): lane r
+        // entries r % share, ... of group r / share, then of the next groups
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int g = r + i * LPR;
+          const int g = r / share + i * LPR;
           mine[i] = 0;
+          uint32_t k1 = 0, k2 = 0;
           if (g < G && live) {
-            uint32_t k1 = 0, k2 = 0;
-            int at = r % gsz;
+            const uint32_t* at = &gk[wave][row][g * gsz];
 #pragma unroll 4
-            for (int u = 0; u < gsz; ++u) {
-              const uint32_t v = gk[wave][row][g * gsz + at];
-              at = at + 1 == gsz ? 0 : at + 1;
+            for (int u = r % share; u < gsz; u += share) {
+              const uint32_t v = at[u];
               k2 = max(k2, min(k1, v));
               k1 = max(k1, v);
             }
-            mine[i] = two ? score_key(key_score(k1) + key_score(k2)) : k1;
           }
+          for (int o = 1; o < share; o <<= 1) {
+            const uint32_t o1 = __shfl_xor(k1, o, 64), o2 = __shfl_xor(k2, o, 64);
+            k2 = max(max(k2, o2), min(k1, o1));
+            k1 = max(k1, o1);
+          }
+          if (g < G && live && r % share == 0) mine[i] = two ? order_key(key_score(k1) + key_score(k2)) : k1;
         }
       }
-      const int scale_g = a.lanes_of_group ? a.lanes_of_group : 1;  // lane r speaks for group r / scale_g
-      uint64_t keep = 0;  // by speakers, the same in a row's lanes
+      uint64_t keep = 0;  // by the number of the lane that speaks for a group, the same in a row's lanes
       for (int j = 0; j < a.top_groups; ++j) {
         uint32_t m = mine[0];
 #pragma unroll
@@ -147,18 +167,16 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
         for (int i = 0; i < PER; ++i) mine[i] = (uint32_t)(r + i * LPR) == g ? 0u : mine[i];
       }
       if (a.lanes_of_group) {
-        const bool stays = (keep >> ((r / scale_g * scale_g) & 63)) & 1;
+        const bool stays = (keep >> (r / a.lanes_of_group * a.lanes_of_group)) & 1;
 #pragma unroll
         for (int q = 0; q < VPL; ++q) key[q] = stays ? key[q] : 0u;
       } else {
-        int g = e0 / gsz, left = gsz - (e0 - g * gsz);
+        const uint32_t lo = (uint32_t)keep, hi = (uint32_t)(keep >> 32);
+        uint32_t e = (uint32_t)opaque(e0);
 #pragma unroll
-        for (int q = 0; q < VPL; ++q) {
-          key[q] = (keep >> (g & 63)) & 1 ? key[q] : 0u;
-          if (--left == 0) {
-            left = gsz;
-            ++g;
-          }
+        for (int q = 0; q < VPL; ++q, ++e) {
+          const uint32_t bit = (e * (uint32_t)a.inv_group >> 20) * share;  // e / gsz, exact below 1024
+          key[q] = ((bit < 32 ? lo : hi) >> (bit & 31)) & 1 ? key[q] : 0u;
         }
       }
     }
@@ -291,6 +309,11 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
   }
 }
 
+// Up to so many tokens of 129 to 256 experts have a wave each, four experts a lane: the time is one wave's latency then
+// (3 tokens of 256 experts 5.6 us, by 16 lanes of 16 experts 9.2; 2048 7.1 and 10.2, 4096 10.1 and 10.6, 8192 16.7 and
+// 14.1; 160 experts 5.4 and 7.6, 6.7 and 8.5, 9.3 and 8.8, 15.6 and 10.7).
+constexpr int64_t kFewTokens = 2048;
+
 // Workgroups that hold the tokens, at most eight a CU: their waves loop over the others.
 unsigned grid_of(int64_t T, int lpr) {
   const int64_t blocks = cdiv(T, (int64_t)kWaves * (64 / lpr));
@@ -320,14 +343,26 @@ extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E
   if (T == 0) return ZMOE_OK;
   ZMOE_REQUIRE(logits && topk_idx && topk_weight, ZMOE_ERR_NULL, "route: null pointer");
   RouteArgs a{logits, expert_biases, T, E, k, groups, top_groups, group_scores, renormalize,
-              rows_on_16(logits, E, E, logits_dtype), 0, scale, topk_idx, topk_weight, topk_prob};
+              rows_on_16(logits, E, E, logits_dtype), 0, 1, (1 << 20) / (E / groups) + 1, scale, topk_idx, topk_weight, topk_prob};
   auto go = [&](auto lpr, auto vpl, auto soft, auto lt) {
     const int lanes = E / groups / decltype(vpl)::value;
     a.lanes_of_group = lanes * decltype(vpl)::value == E / groups && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    for (a.lanes_together = 1; 2 * a.lanes_together * groups <= decltype(lpr)::value;) a.lanes_together *= 2;
     hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
                        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
   };
-  by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, go);
+  if (E > 128 && E <= 256 && T <= kFewTokens) {
+    const auto few = [&](auto soft) {
+      const std::integral_constant<int, 64> lpr;
+      const std::integral_constant<int, 4> vpl;
+      if (logits_dtype == ZMOE_DTYPE_BF16) go(lpr, vpl, soft, uint16_t{});
+      else go(lpr, vpl, soft, float{});
+    };
+    if (score == ZMOE_SCORE_SOFTMAX) few(std::true_type{});
+    else few(std::false_type{});
+  } else {
+    by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, go);
+  }
   return check_launch("route");
 }
 

@@ -121,11 +121,21 @@ __device__ __forceinline__ double rcp_f64(double x) {
   y = fma(fma(-x, y, 1.0), y, y);
   return fma(fma(-x, y, 1.0), y, y);
 }
-// sigmoid_f64 of a logit by these two.
-__device__ __forceinline__ float sigmoid_rounded(float z) {
-  if (fabsf(z) < kSigmoidSeriesBelow) return sigmoid_f64(z);  // (exact ties)
-  const float p = (float)rcp_f64(1.0 + exp_f64(-(double)z));
-  return z <= kSigmoidZeroBelow ? 0.f : p;
+// sigmoid_f64 of a lane's logits by these two, all at once (their chains overlap); exact ties near 0 apart.
+template <int N>
+__device__ __forceinline__ void sigmoids_rounded(const float (&z)[N], float (&p)[N]) {
+  bool small = false;
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    const float v = (float)rcp_f64(1.0 + exp_f64(-(double)z[q]));
+    p[q] = z[q] <= kSigmoidZeroBelow ? 0.f : v;
+    small |= fabsf(z[q]) < kSigmoidSeriesBelow;
+  }
+  if (small) {
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (fabsf(z[q]) < kSigmoidSeriesBelow) p[q] = sigmoid_f64(z[q]);
+  }
 }
 
 // e^x and the sigmoid in f32 by the hardware's exp2 and reciprocal: off by |x| + 2 roundings (the product with log2 e, and the
@@ -199,19 +209,37 @@ __device__ __forceinline__ float lanes_fmax(float v) {
   return v;
 }
 
-// Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: E and e0 are whole 16-byte chunks and rows lie on 16.
+// Chunks of a lane's VPL elements: 16 bytes, or 8 where a lane's elements are no whole 16.
+template <int VPL, typename LT>
+struct LaneChunk {
+  static constexpr int N = VPL * sizeof(LT) % 16 == 0 ? 16 / sizeof(LT) : 8 / sizeof(LT);
+  static_assert(VPL % N == 0, "lanes of whole chunks");
+};
+
+// Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: rows are whole 16-byte chunks and lie on 16 (e0 is a
+// multiple of VPL, so a lane's chunks are wholly in the row or out of it).
 template <int VPL, typename LT>
 __device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, int E, bool vec, bool live, float fill,
                                           float (&v)[VPL]) {
-  constexpr int VC = 16 / sizeof(LT);
-  if (VPL >= VC && vec) {
+  constexpr int N = LaneChunk<VPL, LT>::N;
+  if (vec) {
 #pragma unroll
-    for (int c = 0; c < VPL / VC; ++c) {
-      if (live && e0 + c * VC < E) {
-        unpack_chunk(*reinterpret_cast<const uint4*>(row + e0 + c * VC), &v[c * VC], LT{});
+    for (int c = 0; c < VPL / N; ++c) {
+      if (live && e0 + c * N < E) {
+        if constexpr (N * sizeof(LT) == 16) {
+          unpack_chunk(*reinterpret_cast<const uint4*>(row + e0 + c * N), &v[c * N], LT{});
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(row + e0 + c * N);
+          if constexpr (sizeof(LT) == 2) {
+            v[c * N] = __uint_as_float(x.x << 16), v[c * N + 1] = __uint_as_float(x.x & 0xffff0000u);
+            v[c * N + 2] = __uint_as_float(x.y << 16), v[c * N + 3] = __uint_as_float(x.y & 0xffff0000u);
+          } else {
+            v[c * N] = __uint_as_float(x.x), v[c * N + 1] = __uint_as_float(x.y);
+          }
+        }
       } else {
 #pragma unroll
-        for (int u = 0; u < VC; ++u) v[c * VC + u] = fill;
+        for (int u = 0; u < N; ++u) v[c * N + u] = fill;
       }
     }
   } else {
@@ -221,11 +249,20 @@ __device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, in
 }
 template <int VPL, typename LT>
 __device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, bool vec, const float (&v)[VPL]) {
-  constexpr int VC = 16 / sizeof(LT);
+  constexpr int N = LaneChunk<VPL, LT>::N;
   if (vec) {
 #pragma unroll
-    for (int c = 0; c < VPL / VC; ++c)
-      if (e0 + c * VC < E) *reinterpret_cast<uint4*>(row + e0 + c * VC) = pack_chunk(&v[c * VC], LT{});
+    for (int c = 0; c < VPL / N; ++c) {
+      if (e0 + c * N >= E) continue;
+      if constexpr (N * sizeof(LT) == 16) {
+        *reinterpret_cast<uint4*>(row + e0 + c * N) = pack_chunk(&v[c * N], LT{});
+      } else if constexpr (sizeof(LT) == 2) {
+        *reinterpret_cast<uint2*>(row + e0 + c * N) =
+            make_uint2(pack_bf16x2(v[c * N], v[c * N + 1]), pack_bf16x2(v[c * N + 2], v[c * N + 3]));
+      } else {
+        *reinterpret_cast<float2*>(row + e0 + c * N) = make_float2(v[c * N], v[c * N + 1]);
+      }
+    }
   } else {
 #pragma unroll
     for (int q = 0; q < VPL; ++q)
@@ -233,7 +270,9 @@ __device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, 
   }
 }
 
-// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts.
+// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts: rows of 8 or 16 lanes, whose
+// sums stay within DPP rows, of at most 16 experts a lane (128 experts: 16 lanes of 8 route 32768 tokens in 17.6-19.2 us, 8
+// of 16 in 18.3-20.4, and 3 tokens in 5 and 7.6).
 template <typename F>
 void by_lanes(int E, bool soft, int dtype, F&& f) {
   auto typed = [&](auto lpr, auto vpl) {
@@ -245,10 +284,13 @@ void by_lanes(int E, bool soft, int dtype, F&& f) {
     else scored(float{});
   };
   using I8 = std::integral_constant<int, 8>;
+  using I12 = std::integral_constant<int, 12>;
   using I16 = std::integral_constant<int, 16>;
   using I64 = std::integral_constant<int, 64>;
   if (E <= 64) typed(I8{}, I8{});
+  else if (E <= 96) typed(I8{}, I12{});
   else if (E <= 128) typed(I16{}, I8{});
+  else if (E <= 192) typed(I16{}, I12{});
   else if (E <= 256) typed(I16{}, I16{});
   else if (E <= 512) typed(I64{}, I8{});
   else typed(I64{}, I16{});
