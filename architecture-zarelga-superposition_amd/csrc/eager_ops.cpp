@@ -147,11 +147,16 @@ Tensor swiglu_route_backward(const Tensor& dAs, const Tensor& Hs, const Tensor& 
   return op.call(dAs, Hs, dg, p, idx, E);
 }
 
+bool route_takes(const Tensor& logits, const Opt& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups,
+                 int64_t group_scores) {
+  return logits.is_cuda() && known(logits) && logits.dim() == 2 && logits.is_contiguous() && k >= 0 && fits_int(k) &&
+         fits_int(logits.size(1)) && fits_int(score) && fits_int(groups) && fits_int(top_groups) &&
+         fits_int(group_scores) && (!bias || (flat(*bias, logits, at::kFloat) && bias->numel() == logits.size(1)));
+}
+
 Tensors route(const Tensor& logits, const Opt& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups,
               int64_t group_scores, bool renorm, double scale) {
-  if (logits.is_cuda() && known(logits) && logits.dim() == 2 && logits.is_contiguous() && k >= 0 && fits_int(k) &&
-      fits_int(logits.size(1)) && fits_int(score) && fits_int(groups) && fits_int(top_groups) &&
-      fits_int(group_scores) && (!bias || (flat(*bias, logits, at::kFloat) && bias->numel() == logits.size(1)))) {
+  if (route_takes(logits, bias, k, score, groups, top_groups, group_scores)) {
     const c10::DeviceGuard guard(logits.device());
     const int64_t T = logits.size(0);
     Tensor idx = empty({T, k}, logits, at::kLong), w = empty({T, k}, logits, at::kFloat),
@@ -1059,6 +1064,22 @@ Tensors route_grad(const Tensor& logits, const Opt& bias, int64_t k, int64_t sco
   return RouteFunction::apply(logits, bias, k, score, groups, top_groups, group_scores, renorm, scale);
 }
 
+// route for calls that record no graph: without the probabilities that its backward reads.
+Tensors route_served(const Tensor& logits, const Opt& bias, int64_t k, int64_t score, int64_t groups, int64_t top_groups,
+                     int64_t group_scores, bool renorm, double scale) {
+  if (route_takes(logits, bias, k, score, groups, top_groups, group_scores)) {
+    const c10::DeviceGuard guard(logits.device());
+    const int64_t T = logits.size(0);
+    Tensor idx = empty({T, k}, logits, at::kLong), w = empty({T, k}, logits, at::kFloat);
+    if (zmoe_route(raw(logits), code(logits), T, (int)logits.size(1), (int)k, (int)score,
+                   bias ? ptr<const float>(*bias) : nullptr, (int)groups, (int)top_groups, (int)group_scores, renorm,
+                   (float)scale, ptr<int64_t>(idx), ptr<float>(w), nullptr, stream_of(logits)) == ZMOE_OK)
+      return {idx, w};
+  }
+  const Tensors out = route(logits, bias, k, score, groups, top_groups, group_scores, renorm, scale);
+  return {out[0], out[1]};
+}
+
 struct RouterLossesFunction : torch::autograd::Function<RouterLossesFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& idx, const Opt& cu,
                                int64_t score) {
@@ -1228,6 +1249,9 @@ void groupXtY(int64_t E, const Tensor& DW, const Opt& Db, const Tensor& DY, cons
 TORCH_LIBRARY(zmoe_eager, m) {
   m.def("route_grad(Tensor logits, Tensor? expert_biases, int k, int score, int groups, int top_groups, int group_scores, "
         "bool renormalize, float scale) -> Tensor[]", TORCH_FN(route_grad));
+  m.def("route_served(Tensor logits, Tensor? expert_biases, int k, int score, int groups, int top_groups, "
+        "int group_scores, bool renormalize, float scale) -> Tensor[]");
+  m.impl("route_served", c10::DispatchKey::CompositeExplicitAutograd, TORCH_FN(route_served));
   m.def("router_losses_grad(Tensor logits, Tensor topk_idx, Tensor? cu_seqlens, int score) -> Tensor[]",
         TORCH_FN(router_losses_grad));
   ZMOE_EAGER(route_topk, "(Tensor logits, Tensor expert_biases, int k, bool round_probs_bf16) -> Tensor[]");

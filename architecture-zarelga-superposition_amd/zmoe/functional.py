@@ -317,8 +317,12 @@ def route(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, sco
         node = zl.native_node("route_grad", args)
         idx, w = _Route.apply(*args) if node is None else node(*args)
     else:
-        with torch.no_grad():
-            idx, w, _ = zl.route(*args)
+        node = zl.native_node("route_served", args)
+        if node is not None:
+            idx, w = node(*args)
+        else:
+            with torch.no_grad():
+                idx, w, _ = zl.route(*args)
     if logits.dim() == 2:
         return idx, w
     return idx.view(*logits.shape[:-1], k), w.view(*logits.shape[:-1], k)
