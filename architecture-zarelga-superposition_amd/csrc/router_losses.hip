@@ -211,7 +211,7 @@ __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, S
                                                                  float* __restrict__ inv_tokens) {
   constexpr int GROUPS = kSumThreads / kColumns;  // threads of one expert
   __shared__ double red[GROUPS][kColumns];
-  __shared__ int32_t redc[GROUPS][kColumns];
+  __shared__ int64_t redc[GROUPS][kColumns];
   __shared__ double wave_sums[kSumThreads / 64][2];
   __shared__ int last;
   const int s = blockIdx.x, cb = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, S
   const int64_t first = lo / kTile + s, end = n > 0 ? (hi - 1) / kTile + s + 1 : first;  // its slots
   const int col = threadIdx.x % kColumns, group = threadIdx.x / kColumns, e = cb * kColumns + col;
   double mass = 0.0;
-  int32_t count = 0;
+  int64_t count = 0;
   if (e < E) {
 #pragma unroll 4
     for (int64_t i = first + group; i < end; i += GROUPS) {
