@@ -309,9 +309,10 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
   }
 }
 
-// Up to so many tokens of 129 to 256 experts have a wave each, four experts a lane: the time is one wave's latency then
-// (3 tokens of 256 experts 5.6 us, by 16 lanes of 16 experts 9.2; 2048 7.1 and 10.2, 4096 10.1 and 10.6, 8192 16.7 and
-// 14.1; 160 experts 5.4 and 7.6, 6.7 and 8.5, 9.3 and 8.8, 15.6 and 10.7).
+// Up to so many tokens of 129 to 512 experts have a wave each, four or eight experts a lane: the time is one wave's latency
+// then (3 tokens of 256 experts 5.6 us, by 16 lanes of 16 experts 8.3; 2048 7.1 and 9.1, 4096 10.1 and 9.4, 8192 16.7 and
+// 13.3; 160 experts 5.4 and 7.5, 6.7 and 8.3, 9.3 and 8.4; 512 experts 6.5 and, by 32 lanes of 16, 8.6, 9.2 and 9.4, 13.8 and
+// 13.1).
 constexpr int64_t kFewTokens = 2048;
 
 // Workgroups that hold the tokens, at most eight a CU: their waves loop over the others.
@@ -351,15 +352,18 @@ extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E
     hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
                        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
   };
-  if (E > 128 && E <= 256 && T <= kFewTokens) {
-    const auto few = [&](auto soft) {
+  if (E > 128 && E <= 512 && T <= kFewTokens) {
+    const auto few = [&](auto vpl, auto soft) {
       const std::integral_constant<int, 64> lpr;
-      const std::integral_constant<int, 4> vpl;
       if (logits_dtype == ZMOE_DTYPE_BF16) go(lpr, vpl, soft, uint16_t{});
       else go(lpr, vpl, soft, float{});
     };
-    if (score == ZMOE_SCORE_SOFTMAX) few(std::true_type{});
-    else few(std::false_type{});
+    const auto scored = [&](auto vpl) {
+      if (score == ZMOE_SCORE_SOFTMAX) few(vpl, std::true_type{});
+      else few(vpl, std::false_type{});
+    };
+    if (E <= 256) scored(std::integral_constant<int, 4>{});
+    else scored(std::integral_constant<int, 8>{});
   } else {
     by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, go);
   }

@@ -143,16 +143,31 @@ __device__ __forceinline__ void sigmoids_rounded(const float (&z)[N], float (&p)
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
 __device__ __forceinline__ float sigmoid_hw(float x) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-x)); }
 
-// Over the LPR (8, 16 or 64) lanes of a row; every lane gets the result.
+// A row of 16 lanes and its neighbour's value: two rows' results together, in 32 lanes.
+struct Two {
+  uint32_t a, b;
+};
+__device__ __forceinline__ Two rows_swapped(uint32_t v) {
+  const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return {(uint32_t)both[0], (uint32_t)both[1]};
+}
+
+// Over the LPR (8, 16, 32 or 64) lanes of a row; every lane gets the result.
 template <int LPR>
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
   if constexpr (LPR == 64) return wave_max_u32(v);
-  else return row_max_u32<LPR>(v);
+  else if constexpr (LPR == 32) {
+    const Two t = rows_swapped(row_max_u32<16>(v));
+    return max(t.a, t.b);
+  } else return row_max_u32<LPR>(v);
 }
 template <int LPR>
 __device__ __forceinline__ uint32_t lanes_min(uint32_t v) {
   if constexpr (LPR == 64) return ~wave_max_u32(~v);
-  else return row_min_u32<LPR>(v);
+  else if constexpr (LPR == 32) {
+    const Two t = rows_swapped(row_min_u32<16>(v));
+    return min(t.a, t.b);
+  } else return row_min_u32<LPR>(v);
 }
 // (xor 1, xor 2, mirrors within 8 and 16 lanes as above; between rows of 16 by shuffles)
 template <int CTRL>
@@ -172,10 +187,11 @@ __device__ __forceinline__ float lanes_sum(float v) {
   v += dpp_f32<0x4E>(v);
   v += dpp_f32<0x141>(v);
   if (LPR >= 16) v += dpp_f32<0x140>(v);
-  if (LPR == 64) {
-    v += __shfl_xor(v, 16, 64);
-    v += __shfl_xor(v, 32, 64);
+  if (LPR >= 32) {
+    const Two t = rows_swapped(__float_as_uint(v));
+    v = __uint_as_float(t.a) + __uint_as_float(t.b);
   }
+  if (LPR == 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 template <int LPR>
@@ -184,10 +200,8 @@ __device__ __forceinline__ double lanes_sum(double v) {
   v += dpp_f64<0x4E>(v);
   v += dpp_f64<0x141>(v);
   if (LPR >= 16) v += dpp_f64<0x140>(v);
-  if (LPR == 64) {
-    v += __shfl_xor(v, 16, 64);
-    v += __shfl_xor(v, 32, 64);
-  }
+  if (LPR >= 32) v += __shfl_xor(v, 16, 64);
+  if (LPR == 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 template <int LPR>
@@ -202,10 +216,11 @@ __device__ __forceinline__ float lanes_fmax(float v) {
   v = fmaxf(v, dpp_f32<0x4E>(v));
   v = fmaxf(v, dpp_f32<0x141>(v));
   if (LPR >= 16) v = fmaxf(v, dpp_f32<0x140>(v));
-  if (LPR == 64) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    v = fmaxf(v, __shfl_xor(v, 32, 64));
+  if (LPR >= 32) {
+    const Two t = rows_swapped(__float_as_uint(v));
+    v = fmaxf(__uint_as_float(t.a), __uint_as_float(t.b));
   }
+  if (LPR == 64) v = fmaxf(v, __shfl_xor(v, 32, 64));
   return v;
 }
 
@@ -270,9 +285,9 @@ __device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, 
   }
 }
 
-// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts: rows of 8 or 16 lanes, whose
-// sums stay within DPP rows, of at most 16 experts a lane (128 experts: 16 lanes of 8 route 32768 tokens in 17.6-19.2 us, 8
-// of 16 in 18.3-20.4, and 3 tokens in 5 and 7.6).
+// f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts: the fewest lanes that
+// hold them at 16 a lane (up to 128 at 8: 32768 tokens are routed in 17.6-19.2 us by 16 lanes of 8, 18.3-20.4 by 8 of 16, 3
+// tokens in 5 and 7.6; 32768 of 512 experts in 55-63 by 32 lanes of 16, 68-71 by 64 of 8).
 template <typename F>
 void by_lanes(int E, bool soft, int dtype, F&& f) {
   auto typed = [&](auto lpr, auto vpl) {
@@ -286,13 +301,14 @@ void by_lanes(int E, bool soft, int dtype, F&& f) {
   using I8 = std::integral_constant<int, 8>;
   using I12 = std::integral_constant<int, 12>;
   using I16 = std::integral_constant<int, 16>;
+  using I32 = std::integral_constant<int, 32>;
   using I64 = std::integral_constant<int, 64>;
   if (E <= 64) typed(I8{}, I8{});
   else if (E <= 96) typed(I8{}, I12{});
   else if (E <= 128) typed(I16{}, I8{});
   else if (E <= 192) typed(I16{}, I12{});
   else if (E <= 256) typed(I16{}, I16{});
-  else if (E <= 512) typed(I64{}, I8{});
+  else if (E <= 512) typed(I32{}, I16{});
   else typed(I64{}, I16{});
 }
 
