@@ -313,6 +313,38 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const 
   }
 }
 
+// What a lane reads of two whole blocks, as it lies in memory: on its way while the two before are worked on.
+template <typename T>
+struct Raw8 {
+  uint4 p[8 * sizeof(T) / 16], g[8 * sizeof(T) / 16];
+  uint2 m, v;
+  float am, av;
+  __device__ __forceinline__ void load(const zmoe_adamw_tensor& t, int64_t block, int lane) {
+    const int64_t at = block * kBlock + lane * 8;
+#pragma unroll
+    for (int c = 0; c < (int)(8 * sizeof(T) / 16); ++c) {
+      g[c] = reinterpret_cast<const uint4*>((const T*)t.grad + at)[c];
+      p[c] = reinterpret_cast<const uint4*>((const T*)t.param + at)[c];
+    }
+    m = *reinterpret_cast<const uint2*>((const uint8_t*)t.exp_avg + at);
+    v = *reinterpret_cast<const uint2*>((const uint8_t*)t.exp_avg_sq + at);
+    am = t.scale_avg[block + (lane >> 5)];
+    av = t.scale_sq[block + (lane >> 5)];
+  }
+  __device__ __forceinline__ void unpack(float (&w)[8], float (&gr)[8], uint32_t (&qm)[2], uint32_t (&qv)[2], float& a,
+                                         float& b) const {
+    constexpr int VC = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < 8 / VC; ++c) {
+      unpack_chunk(p[c], &w[c * VC], T{});
+      unpack_chunk(g[c], &gr[c * VC], T{});
+    }
+    qm[0] = m.x, qm[1] = m.y, qv[0] = v.x, qv[1] = v.y;
+    a = am;
+    b = av;
+  }
+};
+
 // Moments in 8 bits: a wave has two blocks at once, eight consecutive elements a lane, so that what is done once for a block
 // (the largest magnitudes over its lanes, the scales' quotients) is shared by twice as many. The arithmetic is the bound
 // as much as memory: some 70 instructions an element, 20 of them in double (which runs at f32's rate here).
@@ -327,6 +359,8 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Table tab, const
   const int64_t n = t.n;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
+  Raw8<T> nxt;
+  if (wide && n - first * kBlock >= 2 * kBlock) nxt.load(t, first, lane);
   for (int u = 0; u < kBlocks / 4; u += 2) {
     const int64_t at = (first + u) * kBlock, left = n - at;
     if (left <= 0) break;
@@ -336,13 +370,19 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Table tab, const
     T* p = (T*)t.param + at;
     uint8_t *pm = (uint8_t*)t.exp_avg + at, *pv = (uint8_t*)t.exp_avg_sq + at;
     float *sm = t.scale_avg + (first + u), *sv = t.scale_sq + (first + u);
-    float w[8], m[8], v[8];
+    float w[8], m[8], v[8], am, av;
     uint32_t qm[2], qv[2];
-    load_codes8(pm, i, left, vec, qm);
-    load_codes8(pv, i, left, vec, qv);
-    load8((const T*)t.grad + at, i, left, vec, v);
-    const float am = there ? sm[half] : 0.f, av = there ? sv[half] : 0.f;
-    load8(p, i, left, vec, w);
+    if (vec) {
+      nxt.unpack(w, v, qm, qv, am, av);
+      if (u + 2 < kBlocks / 4 && left >= 4 * kBlock) nxt.load(t, first + u + 2, lane);
+    } else {
+      load_codes8(pm, i, left, false, qm);
+      load_codes8(pv, i, left, false, qv);
+      load8((const T*)t.grad + at, i, left, false, v);
+      load8(p, i, left, false, w);
+      am = there ? sm[half] : 0.f;
+      av = there ? sv[half] : 0.f;
+    }
     const double um = unit2(am), uv = unit4(av);
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll

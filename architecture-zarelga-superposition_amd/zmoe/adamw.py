@@ -32,7 +32,7 @@ def _dense(t: torch.Tensor) -> bool:
 
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay, p <- p - lr wd p - lr mhat / (sqrt(vhat) + eps), for float32 and bfloat16
-    parameters on the GPU (float32 arithmetic, one rounding of a bfloat16 parameter).
+    parameters on the GPU (float32 arithmetic, one rounding of a bfloat16 parameter; parameters must not share memory).
 
     ``state_bits`` (also a group's): 32, moments in float32; 8, a byte for each element and a float32 scale for each 256 of
     them (``zmoe.h``, zmoe_adamw). ``max_grad_norm``: the grads of all groups are multiplied by
@@ -63,6 +63,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: eps and weight_decay must not be negative, got {g['eps']} and {g['weight_decay']}")
             if g["state_bits"] not in _STATE_DTYPES:
                 raise ValueError(f"AdamW: state_bits must be 32 or 8, got {g['state_bits']}")
+            if len({id(p) for p in g["params"]}) != len(g["params"]):
+                raise ValueError("AdamW: a parameter is given twice")  # (one launch would write it from two places)
             for p in g["params"]:
                 if p.dtype not in (torch.float32, torch.bfloat16):
                     raise ValueError(f"AdamW: parameters must be float32 or bfloat16, got {p.dtype}")

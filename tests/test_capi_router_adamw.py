@@ -146,6 +146,8 @@ def test_python_entry_points_refuse_host_tensors():
                dict(max_grad_norm=0.0), dict(max_grad_norm=float("nan"))):
         with pytest.raises(ValueError):
             AdamW([w], **kw)
+    with pytest.raises(ValueError), pytest.warns(UserWarning):
+        AdamW([w, w])
     opt = AdamW([w])
     with pytest.raises(ValueError):
         opt.add_param_group({"params": [torch.zeros(3, dtype=torch.float64, requires_grad=True)]})
