@@ -30,6 +30,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _alike(t: torch.Tensor, p: torch.Tensor) -> bool:
+    """Whether t's elements lie in memory as p's do."""
+    return t.shape == p.shape and all(a == b for a, b, n in zip(t.stride(), p.stride(), p.shape) if n != 1)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay, p <- p - lr wd p - lr mhat / (sqrt(vhat) + eps), for float32 and bfloat16
     parameters on the GPU (float32 arithmetic, one rounding of a bfloat16 parameter; parameters must not share memory).
@@ -75,6 +80,9 @@ class AdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
+    def __getstate__(self) -> dict:  # (copies and pickles keep the clipping; a state_dict leaves it to the constructor)
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "grad_norm": None}
+
     def __setstate__(self, state) -> None:
         super().__setstate__(state)
         for g in self.param_groups:
@@ -97,8 +105,11 @@ class AdamW(torch.optim.Optimizer):
                 st["exp_avg_sq_scale"] = torch.zeros(n, dtype=torch.float32, device=p.device)
         return st
 
-    @torch.no_grad()
     def step(self, closure=None):
+        return (self._uncompiled if torch.compiler.is_compiling() else self._step)(closure)
+
+    @torch.no_grad()
+    def _step(self, closure):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -113,6 +124,8 @@ class AdamW(torch.optim.Optimizer):
                 if g is None:
                     continue
                 st = self.state.get(p) or self._state_of(p, bits)
+                if bits == 8 and "exp_avg_scale" not in st:
+                    raise ValueError("AdamW: moments in 32 bits in a group of state_bits 8")
                 ps.append(p)
                 gs.append(g)
                 ms.append(st["exp_avg"])
@@ -145,6 +158,9 @@ class AdamW(torch.optim.Optimizer):
                                              group["weight_decay"], clip):
                 continue
             self._in_order(lists)
+            for p, m, v in zip(lists[0], lists[2], lists[3]):
+                if not _alike(m, p) or not _alike(v, p):
+                    raise RuntimeError("AdamW: a parameter's shape or order in memory is not its moments'")
             by: dict = {}  # one call for each device and type
             for i, p in enumerate(lists[0]):
                 for to, of in zip(by.setdefault((p.device, p.dtype), ([], [], [], [], [], [], [])), lists):
@@ -156,6 +172,8 @@ class AdamW(torch.optim.Optimizer):
                 torch.autograd.graph.increment_version([t for some in (to[0], *to[2:]) for t in some])
         return loss
 
+    _uncompiled = torch._disable_dynamo(_step)  # a compiled function calls the step as it is
+
     @staticmethod
     def _in_order(lists) -> None:
         """The grads as the kernels take them: dense, of the parameter's type and order in memory."""
@@ -164,7 +182,7 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError("AdamW: sparse grads are not supported")
             if g.dtype != p.dtype:
                 raise RuntimeError(f"AdamW: a grad of {g.dtype} for a parameter of {p.dtype}")
-            if g.stride() != p.stride():
+            if not _alike(g, p):
                 lists[1][i] = torch.empty_like(p).copy_(g)
 
     @torch.no_grad()
@@ -192,7 +210,10 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, with the state's own types kept (torch casts a state to its parameter's); a torch AdamW's state
-        loads too, its moments in float32."""
+        loads too, its moments in float32, but for forms of the step that this one does not have."""
+        for name in ("amsgrad", "maximize"):
+            if any(g.get(name) for g in state_dict["param_groups"]):
+                raise ValueError(f"AdamW: the state of a step with {name}")
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

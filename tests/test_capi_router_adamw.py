@@ -172,3 +172,18 @@ def test_router_config():
         hidden_size, n_experts_per_token, n_routed_experts, initializer_range = 64, 4, 16, 0.1
 
     assert MoEGate(Bare()).form is None
+
+
+def test_adamw_copies_and_states_of_other_forms():
+    import copy
+    import pickle
+
+    from zmoe.adamw import AdamW
+
+    w = torch.zeros(3, requires_grad=True)
+    opt = AdamW([w], max_grad_norm=0.5, state_bits=8)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.max_grad_norm == 0.5 and other.grad_norm is None and other.param_groups[0]["state_bits"] == 8
+    for name in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError, match=name):
+            opt.load_state_dict(torch.optim.AdamW([w], **{name: True}).state_dict())

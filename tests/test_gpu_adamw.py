@@ -398,3 +398,60 @@ def test_refusals(hip_device):
     cpu.grad = torch.zeros(3)
     with pytest.raises(ValueError):
         AdamW([cpu]).step()
+
+
+def test_parameters_and_groups_that_changed(hip_device):
+    """What no longer fits the state is refused; a copy goes on as its original."""
+    import copy
+
+    from zmoe.adamw import AdamW
+
+    def made(bits):
+        p = torch.randn(40, 30, generator=gen(11)).to(hip_device).requires_grad_(True)
+        opt = AdamW([p], state_bits=bits, max_grad_norm=0.5)
+        p.grad = torch.randn(40, 30, generator=gen(12)).to(hip_device)
+        opt.step()
+        return p, opt
+
+    p, opt = made(8)
+    q, twin = made(8)
+    other = copy.deepcopy(twin)
+    opt.step()
+    other.param_groups[0]["params"][0].grad = p.grad
+    other.step()
+    assert torch.equal(p, other.param_groups[0]["params"][0])
+    p.data = p.data.t().contiguous().t()
+    with pytest.raises(RuntimeError, match="order in memory"):
+        opt.step()
+    for bits in (8, 32):
+        p, opt = made(bits)
+        before = p.detach().clone()
+        opt.param_groups[0]["state_bits"] = 40 - bits
+        with pytest.raises(ValueError):
+            opt.step()
+        assert torch.equal(p, before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_called_from_a_compiled_function(bits, hip_device):
+    from zmoe.adamw import AdamW
+
+    x = torch.randn(8, 32, generator=gen(21)).to(hip_device)
+    grads = [torch.randn(16, 32, generator=gen(22 + i)).to(hip_device) for i in range(3)]
+    ps = [torch.randn(16, 32, generator=gen(20)).to(hip_device).requires_grad_(True) for _ in range(2)]
+    opts = [AdamW([p], state_bits=bits, max_grad_norm=1.0) for p in ps]
+
+    def step(p, opt, g):
+        y = (x @ g.t()).relu()  # something to compile around it
+        p.grad = g * 2.0
+        opt.step()
+        return y.sum()
+
+    compiled = torch.compile(step)
+    for g in grads:
+        step(ps[0], opts[0], g)
+        compiled(ps[1], opts[1], g)
+        assert torch.equal(ps[0], ps[1])
+    torch.compile(opts[1].step)()
+    opts[0].step()
+    assert torch.equal(ps[0], ps[1])
