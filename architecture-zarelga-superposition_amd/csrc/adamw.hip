@@ -16,7 +16,8 @@
 // finite makes its block's scale so, and all of the block's moments NaN.
 //
 // Everything is one pass over memory: 28 bytes an element (f32, 32 bits), 16 (f32, 8 bits), 22 and 10 (bf16). Tensors'
-// pointers travel in the launches' arguments, so nothing is copied to the device and a graph keeps them.
+// pointers travel in the launches' arguments, so nothing is copied to the device and a graph keeps them. The norm is a
+// pass of its own (302 M f32 elements 240 us, 5.0 TB/s), for the clip has to be known before the first element moves.
 #include <type_traits>
 
 #include "zmoe_route.h"  // row_max_u32
@@ -26,8 +27,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBlock = 256;   // elements with one scale
-constexpr int kBlocks = 16;   // of them in a workgroup's chunk: four a wave (two pairs in 8 bits)
+constexpr int kBlocks = 8;    // of them in a workgroup's chunk: two a wave
 constexpr int kChunk = kBlock * kBlocks;
+constexpr int kMomentBlocks = 16;  // the same where moments are decoded: four (302 M elements 541 us, with two 582)
+constexpr int kMomentChunk = kBlock * kMomentBlocks;
 constexpr int kTensors = 48;  // in a launch's arguments (under 4 KB)
 constexpr int kNormChunk = 16384;
 constexpr int kNormTensors = 128;
@@ -103,14 +106,15 @@ __device__ __forceinline__ float value4(uint32_t q, double unit) {
 }
 
 // A code's place in the root's domain: the code is the whole number next to it, unless half-way between two lies within
-// kNear2 or kNear4. The estimate has a reciprocal, a product, one or two roots and a product of f32, 2.4 roundings of 2^-23
-// at most in the root: 127 (255) of those are 3.7e-5 (7.3e-5).
+// kNear2 or kNear4. What the hardware's reciprocals and roots (one unit in the last place, 2^-23) and the products make
+// of it: 127 times 2.4 2^-23 = 3.7e-5 at most, and 255 times 2.8 2^-23 = 8.4e-5 from the step's own root of v
+// (root: 1, the other's reciprocal root: 1, their product: 1/2; halved by the second root: 1.25, its own 1, the product 1/2).
 constexpr float kNear2 = 0x1p-14f, kNear4 = 0x1p-13f;
 __device__ __forceinline__ float place2(float mag, float inv) {
   return __builtin_amdgcn_sqrtf(mag * inv) * (float)kTop2;
 }
-__device__ __forceinline__ float place4(float mag, float inv) {
-  return __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(mag * inv)) * (float)kTop4;
+__device__ __forceinline__ float place4(float root, float inv_root) {
+  return __builtin_amdgcn_sqrtf(root * inv_root) * (float)kTop4;
 }
 
 // The code itself, from one that is off by one at most: set right by the borders on its two sides.
@@ -125,50 +129,53 @@ __device__ __forceinline__ int settle4(int q, float mag, double A) {
   return q + (int)(q < kTop4 && at > 0.0 && h * h * A <= at) - (int)(q > 0 && l * l * A > at);
 }
 
-// The codes of a lane's N elements of each moment (v > 0 at least 1), the bytes of dwords. A block whose largest magnitude
-// has no f32 reciprocal takes its estimates from double; one that is not finite has any codes (its scale says it all).
+// The codes of a lane's N elements of each moment (v > 0 at least 1), the bytes of dwords; r = root(v). A block whose
+// largest magnitude has no f32 reciprocal, or so small a second moment that a root taken for 0 could have a code, takes its
+// estimates from double; one that is not finite has any codes (its scale says it all).
 template <int N>
-__device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], float Am, float Av, uint32_t (&qm)[N / 4],
-                                       uint32_t (&qv)[N / 4]) {
-  const bool odd = (Am > 0.f && Am < 0x1p-100f) || Am > 0x1p100f || (Av > 0.f && Av < 0x1p-100f) || Av > 0x1p100f;
-  const float im = Am > 0.f ? __builtin_amdgcn_rcpf(Am) : 0.f, iv = Av > 0.f ? __builtin_amdgcn_rcpf(Av) : 0.f;
+__device__ __forceinline__ void encode(const float (&m)[N], const float (&v)[N], const float (&r)[N], float Am, float Av,
+                                       uint32_t (&qm)[N / 4], uint32_t (&qv)[N / 4]) {
+  const bool odd = (Am > 0.f && Am < 0x1p-100f) || Am > 0x1p100f || (Av > 0.f && Av < 0x1p-88f) || Av > 0x1p100f;
+  const float im = Am > 0.f ? __builtin_amdgcn_rcpf(Am) : 0.f, iv = Av > 0.f ? __builtin_amdgcn_rsqf(Av) : 0.f;
   float far_m = 0.f, far_v = 0.f;  // from the nearest whole number, at most
-  int cm[N], cv[N];                // magnitudes
+  float cm[N], cv[N];              // magnitudes
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const float y = place2(fabsf(m[e]), im), z = place4(v[e], iv);
-    const float ry = rintf(y), rz = rintf(z);
-    far_m = fmaxf(far_m, fabsf(y - ry));
-    far_v = fmaxf(far_v, fabsf(z - rz));
-    cm[e] = (int)ry;
-    cv[e] = (int)rz;
+    const float y = place2(fabsf(m[e]), im), z = place4(r[e], iv);
+    cm[e] = rintf(y);
+    cv[e] = rintf(z);
+    far_m = fmaxf(far_m, fabsf(y - cm[e]));
+    far_v = fmaxf(far_v, fabsf(z - cv[e]));
   }
   if (odd) {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      cm[e] = Am > 0.f ? (int)rintf(sqrtf((float)(fabs((double)m[e]) / (double)Am)) * (float)kTop2) : 0;
-      cv[e] = Av > 0.f ? (int)rintf(sqrtf(sqrtf((float)((double)v[e] / (double)Av))) * (float)kTop4) : 0;
+      cm[e] = Am > 0.f ? rintf(sqrtf((float)(fabs((double)m[e]) / (double)Am)) * (float)kTop2) : 0.f;
+      cv[e] = Av > 0.f ? rintf(sqrtf(sqrtf((float)((double)v[e] / (double)Av))) * (float)kTop4) : 0.f;
     }
     far_m = far_v = 0.5f;
   }
   if (far_m > 0.5f - kNear2) {  // one lane in a thousand
 #pragma unroll
-    for (int e = 0; e < N; ++e) cm[e] = settle2(cm[e], fabsf(m[e]), (double)Am);
+    for (int e = 0; e < N; ++e) cm[e] = (float)settle2((int)cm[e], fabsf(m[e]), (double)Am);
   }
   if (far_v > 0.5f - kNear4) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) cv[e] = settle4(cv[e], v[e], (double)Av);
+    for (int e = 0; e < N; ++e) cv[e] = (float)settle4((int)cv[e], v[e], (double)Av);
   }
 #pragma unroll
   for (int d = 0; d < N / 4; ++d) {
-    qm[d] = qv[d] = 0;
+    int c[4];
+    qv[d] = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = 4 * d + e;
-      const int sign = (int)__float_as_uint(m[i]) >> 31;  // two's complement of a negative moment's code
-      qm[d] |= (uint32_t)(((cm[i] ^ sign) - sign) & 0xff) << (8 * e);
-      qv[d] |= max((uint32_t)cv[i], min(__float_as_uint(v[i]), 1u)) << (8 * e);
+      c[e] = (int)copysignf(cm[i], m[i]);
+      const float some = __builtin_amdgcn_fmed3f(__builtin_ldexpf(v[i], 200), 0.f, 1.f);  // 1 where v > 0, else 0
+      qv[d] = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(cv[i], some), e, qv[d]);
     }
+    const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+    qm[d] = __builtin_amdgcn_perm(hi, lo, 0x05040100u);  // their low bytes
   }
 }
 
@@ -189,10 +196,9 @@ __device__ __forceinline__ float root(float v) {
   return small ? r * 0x1p-16f : r;
 }
 
-// The parameter after the step: the quotient by v_rcp_f32, whose argument is a normal number.
-template <bool SCALED>
-__device__ __forceinline__ float stepped(float w, float m, float v, const float4& c, float eps) {
-  return fmaf(-(c.x * m), __builtin_amdgcn_rcpf(fmaf(root<SCALED>(v), c.y, eps)), fmaf(-c.z, w, w));
+// The parameter after the step (r: the root of v): the quotient by v_rcp_f32, whose argument is a normal number.
+__device__ __forceinline__ float stepped(float w, float m, float r, const float4& c, float eps) {
+  return fmaf(-(c.x * m), __builtin_amdgcn_rcpf(fmaf(r, c.y, eps)), fmaf(-c.z, w, w));
 }
 
 // ------------------------------------------------------------------ elements
@@ -224,16 +230,11 @@ __device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, con
       if (i + u < n) p[i + u] = from_f32<T>(v[u]);
   }
 }
+// Eight of a block's last elements or of arrays that do not lie on whole vectors.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int i, int64_t n, bool vec, float (&v)[8]) {
-  if (vec) {
-    constexpr int VC = 16 / sizeof(T);
+__device__ __forceinline__ void load8(const T* p, int i, int64_t n, float (&v)[8]) {
 #pragma unroll
-    for (int c = 0; c < 8 / VC; ++c) unpack_chunk(*reinterpret_cast<const uint4*>(p + i + c * VC), &v[c * VC], T{});
-  } else {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = i + u < n ? to_f32(p[i + u]) : 0.f;
-  }
+  for (int u = 0; u < 8; ++u) v[u] = i + u < n ? to_f32(p[i + u]) : 0.f;
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int i, int64_t n, bool vec, const float (&v)[8]) {
@@ -248,16 +249,11 @@ __device__ __forceinline__ void store8(T* p, int i, int64_t n, bool vec, const f
   }
 }
 // Eight codes as the bytes of two dwords.
-__device__ __forceinline__ void load_codes8(const uint8_t* p, int i, int64_t n, bool vec, uint32_t (&c)[2]) {
-  if (vec) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p + i);
-    c[0] = x.x, c[1] = x.y;
-  } else {
-    c[0] = c[1] = 0;
+__device__ __forceinline__ void load_codes8(const uint8_t* p, int i, int64_t n, uint32_t (&c)[2]) {
+  c[0] = c[1] = 0;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (i + u < n) c[u >> 2] |= (uint32_t)p[i + u] << (8 * (u & 3));
-  }
+  for (int u = 0; u < 8; ++u)
+    if (i + u < n) c[u >> 2] |= (uint32_t)p[i + u] << (8 * (u & 3));
 }
 __device__ __forceinline__ void store_codes8(uint8_t* p, int i, int64_t n, bool vec, const uint32_t (&c)[2]) {
   if (vec) {
@@ -277,6 +273,9 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int6
     if (i + u < n) c |= (uint32_t)p[i + u] << (8 * u);
   return c;
 }
+
+// Moments in 32 bits: memory alone (302 M f32 elements 1544-1557 us, 5.4 TB/s); four consecutive elements a lane, a wave's
+// two blocks read before the first is written.
 template <typename T, bool SCALED>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const Hyper h,
                                                          const float4* __restrict__ coef) {
@@ -305,7 +304,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const 
       const float gs = gr[e] * c.w;
       m[e] = fmaf(h.b1f, m[e], h.c1f * gs);
       v[e] = fmaf(h.b2f, v[e], h.c2f * (gs * gs));
-      w[e] = stepped<SCALED>(w[e], m[e], v[e], c, h.eps);
+      w[e] = stepped(w[e], m[e], root<SCALED>(v[e]), c, h.eps);
     }
     store4(pm, i, left, vec, m);
     store4(pv, i, left, vec, v);
@@ -313,7 +312,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const 
   }
 }
 
-// What a lane reads of two whole blocks, as it lies in memory: on its way while the two before are worked on.
+// What a lane reads of two whole blocks, as it lies in memory: all on its way at once (with a branch for whole vectors at
+// each of the reads they come one after the other: 24.5 M bf16 elements 72 us against 61).
 template <typename T>
 struct Raw8 {
   uint4 p[8 * sizeof(T) / 16], g[8 * sizeof(T) / 16];
@@ -345,66 +345,66 @@ struct Raw8 {
   }
 };
 
-// Moments in 8 bits: a wave has two blocks at once, eight consecutive elements a lane, so that what is done once for a block
-// (the largest magnitudes over its lanes, the scales' quotients) is shared by twice as many. The arithmetic is the bound
-// as much as memory: some 70 instructions an element, 20 of them in double (which runs at f32's rate here).
+// Moments in 8 bits: a wave has two blocks at once, eight consecutive elements a lane, so that what is done once for a
+// block (the largest magnitudes over its lanes, the scales' quotients) is shared by twice as many. The arithmetic is the
+// bound as much as memory: 520 vector instructions a lane, 42 of them roots and reciprocals at a quarter of the rate
+// (doubles run at f32's), 50 us of 61 for 24.5 M bf16 elements (4.0 TB/s); 302 M f32 elements 900 us, 5.4 TB/s. One pair a
+// wave: with two, the second's reads under way while the first is worked on, 28 more registers cost more than that
+// hides (repeated on the same tensors, 24.5 M bf16 elements 51 and 56 us, 100 M f32 295 and 299).
 template <typename T, bool SCALED>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Table tab, const Hyper h,
                                                           const float4* __restrict__ coef) {
+  static_assert(kBlocks == 2 * kThreads / 64);
   const int which = owner_of(tab.start, tab.count, blockIdx.x);
   const zmoe_adamw_tensor& t = tab.t[which];
-  const bool wide = (tab.vec >> which) & 1;
   const float4 c = coef[which];
   const double clip = (double)c.w;
-  const int64_t n = t.n;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
-  Raw8<T> nxt;
-  if (wide && n - first * kBlock >= 2 * kBlock) nxt.load(t, first, lane);
-  for (int u = 0; u < kBlocks / 4; u += 2) {
-    const int64_t at = (first + u) * kBlock, left = n - at;
-    if (left <= 0) break;
-    const bool vec = wide && left >= 2 * kBlock;
-    const int i = lane * 8, half = lane >> 5;
-    const bool there = left > half * kBlock;  // this half's block has elements
-    T* p = (T*)t.param + at;
-    uint8_t *pm = (uint8_t*)t.exp_avg + at, *pv = (uint8_t*)t.exp_avg_sq + at;
-    float *sm = t.scale_avg + (first + u), *sv = t.scale_sq + (first + u);
-    float w[8], m[8], v[8], am, av;
-    uint32_t qm[2], qv[2];
-    if (vec) {
-      nxt.unpack(w, v, qm, qv, am, av);
-      if (u + 2 < kBlocks / 4 && left >= 4 * kBlock) nxt.load(t, first + u + 2, lane);
-    } else {
-      load_codes8(pm, i, left, false, qm);
-      load_codes8(pv, i, left, false, qv);
-      load8((const T*)t.grad + at, i, left, false, v);
-      load8(p, i, left, false, w);
-      am = there ? sm[half] : 0.f;
-      av = there ? sv[half] : 0.f;
-    }
-    const double um = unit2(am), uv = unit4(av);
-    uint32_t top_m = 0, top_v = 0;
+  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * 2;
+  const int64_t at = first * kBlock, left = t.n - at;
+  if (left <= 0) return;
+  const bool vec = ((tab.vec >> which) & 1) && left >= 2 * kBlock;
+  const int i = lane * 8, half = lane >> 5;
+  const bool there = left > half * kBlock;  // this half's block has elements
+  T* p = (T*)t.param + at;
+  uint8_t *pm = (uint8_t*)t.exp_avg + at, *pv = (uint8_t*)t.exp_avg_sq + at;
+  float *sm = t.scale_avg + first, *sv = t.scale_sq + first;
+  float w[8], m[8], v[8], r[8], am, av;
+  uint32_t qm[2], qv[2];
+  if (vec) {
+    Raw8<T> raw;
+    raw.load(t, first, lane);
+    raw.unpack(w, v, qm, qv, am, av);
+  } else {
+    load_codes8(pm, i, left, qm);
+    load_codes8(pv, i, left, qv);
+    load8((const T*)t.grad + at, i, left, v);
+    load8(p, i, left, w);
+    am = there ? sm[half] : 0.f;
+    av = there ? sv[half] : 0.f;
+  }
+  const double um = unit2(am), uv = unit4(av);
+  uint32_t top_m = 0, top_v = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double gd = (double)v[e] * clip;
-      const uint32_t byte = 8 * (e & 3);
-      m[e] = blend(h.b1, (double)value2((int)(int8_t)(qm[e >> 2] >> byte), um), h.c1, gd);
-      v[e] = blend(h.b2, (double)value4((qv[e >> 2] >> byte) & 0xffu, uv), h.c2, gd * gd);
-      // magnitudes order as their bits, NaN above all (past the end everything is 0)
-      top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
-      top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
-      w[e] = stepped<SCALED>(w[e], m[e], v[e], c, h.eps);
-    }
-    store8(p, i, left, vec, w);
-    const float Am = __uint_as_float(half_max_u32(top_m)), Av = __uint_as_float(half_max_u32(top_v));
-    encode<8>(m, v, Am, Av, qm, qv);
-    store_codes8(pm, i, left, vec, qm);
-    store_codes8(pv, i, left, vec, qv);
-    if ((lane & 31) == 0 && there) {
-      sm[half] = Am;
-      sv[half] = Av;
-    }
+  for (int e = 0; e < 8; ++e) {
+    const double gd = (double)v[e] * clip;
+    const uint32_t byte = 8 * (e & 3);
+    m[e] = blend(h.b1, (double)value2((int)(int8_t)(qm[e >> 2] >> byte), um), h.c1, gd);
+    v[e] = blend(h.b2, (double)value4((qv[e >> 2] >> byte) & 0xffu, uv), h.c2, gd * gd);
+    // magnitudes order as their bits, NaN above all (past the end everything is 0; v has no sign but a NaN's)
+    top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
+    top_v = max(top_v, __float_as_uint(v[e]));
+    r[e] = root<SCALED>(v[e]);
+    w[e] = stepped(w[e], m[e], r[e], c, h.eps);
+  }
+  store8(p, i, left, vec, w);
+  const float Am = __uint_as_float(half_max_u32(top_m)), Av = __uint_as_float(half_max_u32(top_v));
+  encode<8>(m, v, r, Am, Av, qm, qv);
+  store_codes8(pm, i, left, vec, qm);
+  store_codes8(pv, i, left, vec, qv);
+  if ((lane & 31) == 0 && there) {
+    sm[half] = Am;
+    sv[half] = Av;
   }
 }
 
@@ -421,9 +421,9 @@ __global__ __launch_bounds__(kThreads) void moments_kernel(const MomentTable tab
   const zmoe_moment& t = tab.t[which];
   const bool wide = (tab.vec >> which) & 1;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kBlocks + wave * (kBlocks / 4);
+  const int64_t first = (int64_t)(blockIdx.x - tab.start[which]) * kMomentBlocks + wave * (kMomentBlocks / 4);
 #pragma unroll
-  for (int u = 0; u < kBlocks / 4; ++u) {
+  for (int u = 0; u < kMomentBlocks / 4; ++u) {
     const int64_t b = first + u, i = b * kBlock + lane * 4;
     if (b * kBlock >= t.n) break;
     const bool vec = wide && (b + 1) * kBlock <= t.n;
@@ -592,7 +592,8 @@ extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype
                        beta2, weight_decay, clip, coef + i);
     if (const int rc = check_launch("adamw")) return rc;
   }
-  const Hyper h{beta1, beta2, 1.0 - beta1, 1.0 - beta2, (float)beta1, (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)eps};
+  const Hyper h{beta1,        beta2,        1.0 - beta1,          1.0 - beta2,         (float)beta1,
+                (float)beta2, (float)(1.0 - beta1), (float)(1.0 - beta2), (float)eps};
   Table tab;
   tab.count = 0;
   tab.start[0] = 0;
@@ -682,19 +683,19 @@ extern "C" int zmoe_adamw_moments(const zmoe_moment* moments, int count, void* s
   constexpr int64_t kMost = kMaxLaunchThreads / kThreads / 2;
   for (int i = 0; i < count; ++i) {
     const zmoe_moment& t = moments[i];
-    for (int64_t first = 0, all = cdiv(t.n, kChunk); first < all;) {
+    for (int64_t first = 0, all = cdiv(t.n, kMomentChunk); first < all;) {
       const int64_t room = kMost - tab.start[tab.count];
       if (room <= 0 || tab.count == kTensors) {
         if (const int rc = launch()) return rc;
         continue;
       }
-      const int64_t take = all - first < room ? all - first : room, at = first * kChunk;
+      const int64_t take = all - first < room ? all - first : room, at = first * kMomentChunk;
       zmoe_moment& u = tab.t[tab.count];
       u = t;
       u.codes = (const char*)t.codes + at;
-      u.scale = t.scale + first * kBlocks;
+      u.scale = t.scale + first * kMomentBlocks;
       u.out = t.out + at;
-      u.n = t.n - at < take * kChunk ? t.n - at : take * kChunk;
+      u.n = t.n - at < take * kMomentChunk ? t.n - at : take * kMomentChunk;
       if (on(t.codes, 4) && on(t.out, 16)) tab.vec |= 1ull << tab.count;
       tab.start[tab.count + 1] = tab.start[tab.count] + (int32_t)take;
       ++tab.count;
