@@ -21,9 +21,9 @@ struct RouteArgs {
   const void* logits;
   const float* bias;  // or null
   int64_t T;
-  int E, k, groups, top_groups, group_scores, renorm, vec;
+  int E, k, groups, group_size, top_groups, group_scores, renorm, vec, bias_vec;
   int lanes_of_group;  // where a group is whole lanes, a power of two of them; else 0, and
-  int lanes_together;  // so many lanes score a group
+  int log_together;    // 2^that many lanes score a group
   int inv_group;       // 2^20 / experts of a group, rounded up
   float scale;
   int64_t* idx;
@@ -36,12 +36,6 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// x as a value that the compiler knows nothing of (so nothing computed from it leaves the loop).
-__device__ __forceinline__ int opaque(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
 }
 
 // score_key in fewer instructions: -0 goes with +0 by an addition.
@@ -65,12 +59,11 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
   __shared__ uint16_t slots[kWaves][TPW][kMaxSlots];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int row = lane / LPR, r = lane % LPR, e0 = r * VPL;
-  const int E = a.E, k = a.k, G = a.groups, gsz = E / G;
+  const int E = a.E, k = a.k, G = a.groups, gsz = a.group_size;
   const bool two = a.group_scores == 2 && G > 1;
   const bool by_p = a.bias != nullptr;
-  float b[VPL];
-#pragma unroll
-  for (int q = 0; q < VPL; ++q) b[q] = by_p && e0 + q < E ? a.bias[e0 + q] : 0.f;
+  float b[VPL];  // past E -inf, as the logits: behind every expert
+  if (by_p) load_lane<VPL>(a.bias, e0, E, a.bias_vec, true, -INFINITY, b);
 
   const int64_t step = (int64_t)gridDim.x * kWaves * TPW;
   for (int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * TPW; t0 < a.T; t0 += step) {
@@ -97,22 +90,25 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
     } else {
       sigmoids_rounded(z, p);
     }
-    const int have = live ? opaque(E - e0) : 0;  // of this lane's experts (not kept in masks over the loop: registers)
+    if (by_p) {
+#pragma unroll
+      for (int q = 0; q < VPL; ++q) z[q] = p[q] + b[q];
+    }
     uint32_t key[VPL];
 #pragma unroll
     for (int q = 0; q < VPL; ++q) {
-      key[q] = q < have ? order_key(by_p ? p[q] + b[q] : z[q]) : 0u;
+      key[q] = order_key(z[q]);
       ps[wave][row][e0 + q] = p[q];
     }
     if (G > 1) {
       constexpr int PER = (64 + LPR - 1) / LPR;  // groups of a lane
-      const int share = a.lanes_together;
+      const int share = 1 << a.log_together;
       uint32_t mine[PER];
       if (a.lanes_of_group) {  // a group is whole lanes, a power of two of them: its first lane speaks for it
         uint32_t k1 = 0, k2 = 0;
 #pragma unroll
         for (int q = 0; q < VPL; ++q) {
-          const uint32_t v = two && !by_p ? (q < have ? order_key(p[q]) : 0u) : key[q];
+          const uint32_t v = two && !by_p ? order_key(p[q]) : key[q];
           k2 = max(k2, min(k1, v));
           k1 = max(k1, v);
         }
@@ -121,7 +117,8 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
           k2 = max(max(k2, o2), min(k1, o1));
           k1 = max(k1, o1);
         }
-        mine[0] = live && e0 < E && r % a.lanes_of_group == 0 ? (two ? order_key(key_score(k1) + key_score(k2)) : k1) : 0u;
+        const uint32_t best = two ? order_key(key_score(k1) + key_score(k2)) : k1;
+        mine[0] = live && e0 < E && (r & (a.lanes_of_group - 1)) == 0 ? best : 0u;
 #pragma unroll
         for (int i = 1; i < PER; ++i) mine[i] = 0;
       } else {
@@ -130,15 +127,16 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
         wave_sync();
         // share lanes score a group together (a power of two, one where there are more groups than half the lanes): lane r
         // entries r % share, ... of group r / share, then of the next groups
+        const int ro = opaque(r);  // (nothing of this path is kept over the loop)
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int g = r / share + i * LPR;
+          const int g = (ro >> a.log_together) + i * LPR;
           mine[i] = 0;
           uint32_t k1 = 0, k2 = 0;
           if (g < G && live) {
             const uint32_t* at = &gk[wave][row][g * gsz];
 #pragma unroll 4
-            for (int u = r % share; u < gsz; u += share) {
+            for (int u = ro & (share - 1); u < gsz; u += share) {
               const uint32_t v = at[u];
               k2 = max(k2, min(k1, v));
               k1 = max(k1, v);
@@ -149,7 +147,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
             k2 = max(max(k2, o2), min(k1, o1));
             k1 = max(k1, o1);
           }
-          if (g < G && live && r % share == 0) mine[i] = two ? order_key(key_score(k1) + key_score(k2)) : k1;
+          if (g < G && live && (ro & (share - 1)) == 0) mine[i] = two ? order_key(key_score(k1) + key_score(k2)) : k1;
         }
       }
       uint64_t keep = 0;  // by the number of the lane that speaks for a group, the same in a row's lanes
@@ -167,7 +165,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
         for (int i = 0; i < PER; ++i) mine[i] = (uint32_t)(r + i * LPR) == g ? 0u : mine[i];
       }
       if (a.lanes_of_group) {
-        const bool stays = (keep >> (r / a.lanes_of_group * a.lanes_of_group)) & 1;
+        const bool stays = (keep >> (r & -a.lanes_of_group)) & 1;
 #pragma unroll
         for (int q = 0; q < VPL; ++q) key[q] = stays ? key[q] : 0u;
       } else {
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_kernel(const RouteArgs a) {
         uint32_t e = (uint32_t)opaque(e0);
 #pragma unroll
         for (int q = 0; q < VPL; ++q, ++e) {
-          const uint32_t bit = (e * (uint32_t)a.inv_group >> 20) * share;  // e / gsz, exact below 1024
+          const uint32_t bit = (e * (uint32_t)a.inv_group >> 20) << a.log_together;  // e / gsz, exact below 1024
           key[q] = ((bit < 32 ? lo : hi) >> (bit & 31)) & 1 ? key[q] : 0u;
         }
       }
@@ -343,12 +341,13 @@ extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E
                "route: need 1 <= k <= %d and experts to choose from (k=%d, %d)", kMaxSlots, k, top_groups * (E / groups));
   if (T == 0) return ZMOE_OK;
   ZMOE_REQUIRE(logits && topk_idx && topk_weight, ZMOE_ERR_NULL, "route: null pointer");
-  RouteArgs a{logits, expert_biases, T, E, k, groups, top_groups, group_scores, renormalize,
-              rows_on_16(logits, E, E, logits_dtype), 0, 1, (1 << 20) / (E / groups) + 1, scale, topk_idx, topk_weight, topk_prob};
+  RouteArgs a{logits, expert_biases, T, E, k, groups, E / groups, top_groups, group_scores, renormalize,
+              rows_on_16(logits, E, E, logits_dtype), rows_on_16(expert_biases, E, E, ZMOE_DTYPE_F32), 0, 1,
+              (1 << 20) / (E / groups) + 1, scale, topk_idx, topk_weight, topk_prob};
   auto go = [&](auto lpr, auto vpl, auto soft, auto lt) {
     const int lanes = E / groups / decltype(vpl)::value;
     a.lanes_of_group = lanes * decltype(vpl)::value == E / groups && (lanes & (lanes - 1)) == 0 ? lanes : 0;
-    for (a.lanes_together = 1; 2 * a.lanes_together * groups <= decltype(lpr)::value;) a.lanes_together *= 2;
+    for (a.log_together = 0; (2 << a.log_together) * groups <= decltype(lpr)::value;) ++a.log_together;
     hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
                        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
   };

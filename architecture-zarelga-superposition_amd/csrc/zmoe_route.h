@@ -231,6 +231,12 @@ struct LaneChunk {
   static_assert(VPL % N == 0, "lanes of whole chunks");
 };
 
+// x as a value that the compiler knows nothing of (so nothing computed from it leaves the loop).
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: rows are whole 16-byte chunks and lie on 16 (e0 is a
 // multiple of VPL, so a lane's chunks are wholly in the row or out of it).
 template <int VPL, typename LT>
@@ -258,8 +264,9 @@ __device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, in
       }
     }
   } else {
+    const int have = live ? opaque(E - e0) : 0;  // (not kept as VPL masks over a caller's loop: registers)
 #pragma unroll
-    for (int q = 0; q < VPL; ++q) v[q] = live && e0 + q < E ? to_f32(row[e0 + q]) : fill;
+    for (int q = 0; q < VPL; ++q) v[q] = q < have ? to_f32(row[e0 + q]) : fill;
   }
 }
 template <int VPL, typename LT>
@@ -279,9 +286,10 @@ __device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, 
       }
     }
   } else {
+    const int have = opaque(E - e0);
 #pragma unroll
     for (int q = 0; q < VPL; ++q)
-      if (e0 + q < E) row[e0 + q] = from_f32<LT>(v[q]);
+      if (q < have) row[e0 + q] = from_f32<LT>(v[q]);
   }
 }
 
