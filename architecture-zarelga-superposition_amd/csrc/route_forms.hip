@@ -307,11 +307,15 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
   }
 }
 
-// Up to so many tokens of 129 to 512 experts have a wave each, four or eight experts a lane: the time is one wave's latency
-// then (3 tokens of 256 experts 5.6 us, by 16 lanes of 16 experts 8.3; 2048 7.1 and 9.1, 4096 10.1 and 9.4, 8192 16.7 and
-// 13.3; 160 experts 5.4 and 7.5, 6.7 and 8.3, 9.3 and 8.4; 512 experts 6.5 and, by 32 lanes of 16, 8.6, 9.2 and 9.4, 13.8 and
-// 13.1).
-constexpr int64_t kFewTokens = 2048;
+// Few tokens are a wave's latency, which fewer experts a lane shorten (us in a graph's replays, sigmoids and groups):
+//   tokens of 256 experts      3    512   2048   4096   8192  32768
+//   64 lanes of 4            5.2    5.5    6.3    8.6   13.5   48.4
+//   32 lanes of 8            5.3    5.6    5.7    6.8    9.9   29.9
+//   16 lanes of 16           6.8    7.3    7.5    7.6    9.6   27.2
+//   512 experts, 64 of 8     5.9    6.3    7.5   10.8   17.9   65.1
+//   32 of 16                 7.3    7.6    7.8    9.7   16.0   52.4
+// (160 experts: 64 of 4 4.8, 5.3, 6.0, 8.2, 12.5; 16 of 12 6.4, 6.9, 6.9, 7.0, 8.6; 128: 16 of 8 4.1 to 4.7, 8 of 16 5.7 to 6.3.)
+constexpr int64_t kFewTokens = 512, kSomeTokens = 4096, kFewOfMany = 2048;
 
 // Workgroups that hold the tokens, at most eight a CU: their waves loop over the others.
 unsigned grid_of(int64_t T, int lpr) {
@@ -351,18 +355,18 @@ extern "C" int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E
     hipLaunchKernelGGL((route_kernel<decltype(lpr)::value, decltype(vpl)::value, decltype(soft)::value, decltype(lt)>),
                        dim3(grid_of(T, decltype(lpr)::value)), dim3(64 * kWaves), 0, as_stream(stream), a);
   };
-  if (E > 128 && E <= 512 && T <= kFewTokens) {
-    const auto few = [&](auto vpl, auto soft) {
-      const std::integral_constant<int, 64> lpr;
+  if (E > 128 && T <= (E <= 256 ? kSomeTokens : E <= 512 ? kFewOfMany : 0)) {
+    const auto typed = [&](auto lpr, auto vpl, auto soft) {
       if (logits_dtype == ZMOE_DTYPE_BF16) go(lpr, vpl, soft, uint16_t{});
       else go(lpr, vpl, soft, float{});
     };
-    const auto scored = [&](auto vpl) {
-      if (score == ZMOE_SCORE_SOFTMAX) few(vpl, std::true_type{});
-      else few(vpl, std::false_type{});
+    const auto scored = [&](auto lpr, auto vpl) {
+      if (score == ZMOE_SCORE_SOFTMAX) typed(lpr, vpl, std::true_type{});
+      else typed(lpr, vpl, std::false_type{});
     };
-    if (E <= 256) scored(std::integral_constant<int, 4>{});
-    else scored(std::integral_constant<int, 8>{});
+    if (E > 256) scored(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    else if (T <= kFewTokens) scored(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    else scored(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
   } else {
     by_lanes(E, score == ZMOE_SCORE_SOFTMAX, logits_dtype, go);
   }

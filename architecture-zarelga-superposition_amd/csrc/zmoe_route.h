@@ -294,8 +294,8 @@ __device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, 
 }
 
 // f(lanes of a row, experts a lane, softmax?, logits' type), the layout by the number of experts: the fewest lanes that
-// hold them at 16 a lane (up to 128 at 8: 32768 tokens are routed in 17.6-19.2 us by 16 lanes of 8, 18.3-20.4 by 8 of 16, 3
-// tokens in 5 and 7.6; 32768 of 512 experts in 55-63 by 32 lanes of 16, 68-71 by 64 of 8).
+// hold them at 16 a lane (up to 128 at 8: 32768 tokens are routed in 12.9-13.4 us by 16 lanes of 8, 11.7-13.4 by 8 of 16, 3
+// tokens in 4 and 5.7; 32768 of 512 experts in 46-52 by 32 lanes of 16, 62-65 by 64 of 8).
 template <typename F>
 void by_lanes(int E, bool soft, int dtype, F&& f) {
   auto typed = [&](auto lpr, auto vpl) {

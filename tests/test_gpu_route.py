@@ -254,3 +254,22 @@ def test_compiled(hip_device):
     lb.backward()
     assert torch.equal(ia, ib) and torch.equal(a.grad, b.grad)
     torch.testing.assert_close(la, lb)
+
+
+@pytest.mark.parametrize("E,G,g,k", [(130, 10, 3, 8), (160, 8, 3, 6), (200, 4, 2, 9), (250, 5, 2, 8), (256, 8, 4, 8), (256, 64, 9, 17),
+                                     (192, 64, 64, 12), (300, 6, 2, 8), (384, 16, 3, 8), (512, 8, 4, 8), (510, 2, 1, 5)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("T", [600, 4097])
+def test_groups_of_many_tokens(E, G, g, k, score, T, hip_device):
+    """A token's experts over fewer or more lanes, by the number of tokens: groups and biases in each of them, experts
+    that a bias rules out among those that have to be taken, rows without any."""
+    bias = (torch.randn(E, generator=gen(E)) * 0.05).to(hip_device)
+    out = bias.clone()
+    out[torch.randperm(E, generator=gen(E + 1))[: E - 3].to(hip_device)] = -math.inf  # three are left, fewer than k
+    for dt, with_bias, two in (("bf16", bias, 2), ("f32", None, 1), ("f32", out, 2), ("bf16", out, 1)):
+        z = logits_of(T, E, dt, hip_device, seed=7)
+        z[T // 2], z[-1, 3:] = -math.inf, -math.inf
+        two = min(two, E // G)
+        check(z, k, with_bias, score, G, g, two, dt == "bf16", 1.5)
+        if G < 64:
+            check(z, min(k, E // G), with_bias, score, renormalize=False)
