@@ -1021,7 +1021,7 @@ Tensors norm_residual_backward(const Opt& dR_out, const Opt& dX, const Tensor& R
 
 // ------------------------------------------------------------------ autograd functions
 // route and router_losses with their gradients as C++ nodes, for calls with gradients on (zmoe/functional.py): a pass of a
-// few hundred tokens is bound by its host time, half of it the Python function's (ctx, apply, backward: 86 -> 45 us a
+// few hundred tokens is bound by its host time, half of it the Python function's (ctx, apply, backward: 86 -> 52 us a
 // training pass of route). Under create_graph the backward calls the general form, which refuses a second derivative.
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -1112,8 +1112,8 @@ Tensors router_losses_grad(const Tensor& logits, const Tensor& idx, const Opt& c
 }
 
 // ------------------------------------------------------------------ the optimizer's step
-// AdamW's step over lists of tensors (zmoe/adamw.py): false where the general form (zmoe.ops) has to run or raise. Its host
-// time is this: 16 tensors 50 us with their descriptions written from Python, 8 here.
+// AdamW's step over lists of tensors (zmoe/adamw.py): false where the general form (zmoe.ops) has to run or raise. A step
+// of small tensors is its host time: 16 of them with the clip 104 us with their descriptions written from Python, 49 so.
 bool dense_like(const Tensor& t, const Tensor& p) {
   return t.is_cuda() && t.device() == p.device() && t.layout() == at::kStrided && t.sizes() == p.sizes() &&
          t.strides() == p.strides();

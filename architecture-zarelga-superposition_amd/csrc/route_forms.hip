@@ -9,6 +9,12 @@
 //
 // Where p + b decides, one f32 rounding of p can decide: p comes from double, whose error (some 2^-52) moves an f32
 // rounding for one value in 2^28. Without a bias the experts' order is their logits' order.
+//
+// Few bytes (8192 tokens of 256 experts 5 MB, 1 us at the copy's rate) and many instructions: a token's experts lie over a
+// row of lanes, so that a wave has several tokens; of its 2100 instructions for four of them 570 are the sigmoids in
+// double, 1030 the k = 8 rounds of maximum, first holder and mark, 200 the groups. 8192 tokens of 256 experts in 8 groups
+// 9.6 us in a graph's replays (11.1 traced; two waves a SIMD), 32768 of 128 by softmax 12.9 (14.8), 32749 of 160 in f32 23
+// traced; their backwards, a pass over the [T, E] grad, 5.4 and 13.6 (2.3 and 3.3 TB/s).
 #include "zmoe_route.h"
 
 namespace zmoe {

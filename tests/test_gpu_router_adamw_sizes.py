@@ -94,6 +94,32 @@ def test_many_sequences(hip_device):
     assert ((leaf.grad.double() - val).abs() <= 1e-5 * mag + 1e-38).all()
 
 
+def test_most_sequences(hip_device):
+    """As many sequences as a call takes, of one token each and a few of none: a's formula is then a token's own counts
+    (tolerances as above)."""
+    from zmoe.functional import router_losses
+
+    S, E, k = 1 << 20, 40, 2
+    T = S - 3
+    z = torch.randn(T, E, generator=gen(3)).to(hip_device)
+    idx = torch.topk(z, k).indices
+    cu = torch.arange(S + 1, device=hip_device).clamp(max=T)
+    leaf = z.clone().requires_grad_(True)
+    b, q = router_losses(leaf, idx, "softmax", cu)
+    (0.5 * b + 0.25 * q).backward()
+    z = z.double()
+    ph, lse = torch.softmax(z, -1), torch.logsumexp(z, -1)
+    a = torch.zeros_like(z).scatter_(1, idx, E / (k * T))
+    vb, vz = float((a * ph).sum()), float(lse.square().mean())
+    assert abs(float(b) - vb) <= 1e-5 * vb and abs(float(q) - vz) <= 1e-5 * vz
+    dot = (a * ph).sum(-1, keepdim=True)
+    zpart = 0.5 * lse[:, None] / T * ph
+    val, mag = 0.5 * ph * (a - dot) + zpart, 0.5 * ph * (a + dot) + zpart.abs()
+    assert ((leaf.grad.double() - val).abs() <= 1e-5 * mag + 1e-38).all()
+    with pytest.raises(ValueError):
+        router_losses(leaf, idx, "softmax", torch.arange(S + 2, device=hip_device).clamp(max=T))
+
+
 def test_most_tensors(hip_device):
     """Some thousand tensors: many launches, each with its own table."""
     from zmoe.adamw import AdamW
