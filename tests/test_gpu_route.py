@@ -273,3 +273,16 @@ def test_groups_of_many_tokens(E, G, g, k, score, T, hip_device):
         check(z, k, with_bias, score, G, g, two, dt == "bf16", 1.5)
         if G < 64:
             check(z, min(k, E // G), with_bias, score, renormalize=False)
+
+
+def test_no_tokens(hip_device):
+    from zmoe.functional import route
+
+    for shape in ((0, 16), (3, 0, 200)):
+        z = torch.zeros(*shape, device=hip_device, dtype=torch.bfloat16, requires_grad=True)
+        idx, w = route(z, 4, torch.zeros(shape[-1], device=hip_device), "softmax")
+        assert idx.shape == w.shape == (*shape[:-1], 4) and idx.dtype == torch.int64
+        w.sum().backward()
+        assert z.grad.shape == z.shape and z.grad.dtype == z.dtype
+        with torch.no_grad():
+            assert route(z, 4)[1].shape == (*shape[:-1], 4)
