@@ -14,7 +14,7 @@
 // row of lanes, so that a wave has several tokens; of its 2100 instructions for four of them 570 are the sigmoids in
 // double, 1030 the k = 8 rounds of maximum, first holder and mark, 200 the groups. 8192 tokens of 256 experts in 8 groups
 // 9.6 us in a graph's replays (11.1 traced; two waves a SIMD), 32768 of 128 by softmax 12.9 (14.8), 32749 of 160 in f32 23
-// traced; their backwards, a pass over the [T, E] grad, 5.4 and 13.6 (2.3 and 3.3 TB/s).
+// traced; their backwards, a pass over the [T, E] grad, 5.4 and 11.6 (2.3 and 3.9 TB/s).
 #include "zmoe_route.h"
 
 namespace zmoe {
@@ -240,10 +240,10 @@ struct RouteBackwardArgs {
 template <int LPR, int VPL, bool SOFT, typename LT>
 __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const RouteBackwardArgs a) {
 #pragma clang fp contract(off)  // (one expert's renormalised weight has a grad of rounding errors alone: 0, not fused ones)
-  constexpr int TPW = 64 / LPR, W = LPR * VPL;
+  constexpr int TPW = 64 / LPR, W = LPR * VPL, STEP = kSpread<LPR, VPL, LT>;
   __shared__ float ds[kWaves][TPW][W];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int row = lane / LPR, r = lane % LPR, e0 = r * VPL;
+  const int row = lane / LPR, r = lane % LPR, e0 = spread_first<VPL, LT>(r);
   const int E = a.E, k = a.k;
   const int64_t step = (int64_t)gridDim.x * kWaves * TPW;
   for (int64_t t0 = ((int64_t)blockIdx.x * kWaves + wave) * TPW; t0 < a.T; t0 += step) {
@@ -251,9 +251,9 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
     const bool live = t < a.T;
     float* mine = &ds[wave][row][0];
 #pragma unroll
-    for (int q = 0; q < VPL; ++q) mine[e0 + q] = 0.f;
+    for (int q = 0; q < VPL; ++q) mine[e0 + lane_element<VPL, STEP, LT>(q)] = 0.f;
     float add[VPL];
-    if (a.add) load_lane<VPL>((const LT*)a.add + t * a.ld_add, e0, E, a.vec, live, 0.f, add);
+    if (a.add) load_lane<VPL, STEP>((const LT*)a.add + t * a.ld_add, e0, E, a.vec, live, 0.f, add);
     float S = 0.f, dot = 0.f;  // sum p, sum c dw p
     if (live)
       for (int j = r; j < k; j += LPR) {
@@ -277,11 +277,11 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
     wave_sync();
     float v[VPL];
 #pragma unroll
-    for (int q = 0; q < VPL; ++q) v[q] = mine[e0 + q];
+    for (int q = 0; q < VPL; ++q) v[q] = mine[e0 + lane_element<VPL, STEP, LT>(q)];
     if constexpr (SOFT) {
       if (!scaled) {  // every logit has a grad: -p_e sum dp p where it is not selected
         float z[VPL];
-        load_lane<VPL>((const LT*)a.logits + t * E, e0, E, a.vec, live, -INFINITY, z);
+        load_lane<VPL, STEP>((const LT*)a.logits + t * E, e0, E, a.vec, live, -INFINITY, z);
         float m = z[0], sum = 0.f;
 #pragma unroll
         for (int q = 1; q < VPL; ++q) m = fmaxf(m, z[q]);
@@ -297,8 +297,9 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
         uint32_t sel = 0;
         if (live)
           for (int j = 0; j < k; ++j) {
-            const int64_t q = a.idx[t * k + j] - e0;
-            if (q >= 0 && q < VPL) sel |= 1u << (int)q;
+            const int64_t d = a.idx[t * k + j] - e0;  // the lane's chunk d / STEP, and its place in it
+            constexpr int N = LaneChunk<VPL, LT>::N;
+            if (d >= 0 && d < W && d % STEP < N) sel |= 1u << (int)(d / STEP * N + d % STEP);
           }
 #pragma unroll
         for (int q = 0; q < VPL; ++q) v[q] = (sel >> q) & 1 ? v[q] : -(z[q] * inv) * inner;
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
 #pragma unroll
       for (int q = 0; q < VPL; ++q) v[q] += add[q];
     }
-    if (live) store_lane<VPL>((LT*)a.dz + t * a.ld, e0, E, a.vec, v);
+    if (live) store_lane<VPL, STEP>((LT*)a.dz + t * a.ld, e0, E, a.vec, v);
     wave_sync();
   }
 }

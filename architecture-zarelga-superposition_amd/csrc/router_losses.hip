@@ -6,13 +6,13 @@
 // The counts take no part in the gradient. A token whose logits are all -inf adds nothing and has no gradient; tokens
 // outside the sequences neither.
 //
-// The forward reads the logits once: a workgroup has a tile of tokens, a row of LPR lanes a token (VPL consecutive experts a
+// The forward reads the logits once: a workgroup has a tile of tokens, a row of LPR lanes a token (VPL experts a
 // lane), and the sums of the tile's part of each sequence go to a slot of their own (tile i and sequence s meet in slot
 // i + s: walking along the tokens either number grows by one), which a second launch adds up in a fixed order, a
 // workgroup for each sequence and 32 experts. The gradient reads the logits again. Both are short: what bounds them is
 // the latency of a few dependent reads in each of the launches, and the exponentials (32749 tokens of 256 experts in 37
-// sequences, f32: 15.4 us, 2.3 TB/s, then 10.6 for the sums and 20.6 for the gradient, 3.3 TB/s; 32768 of 128, bf16, one
-// sequence: 6.9, 8.6 and 7.4; 517 of 32: 5.9, 6.6 and 4.2).
+// sequences, f32: 14.8 us, 2.4 TB/s, then 10.4 for the sums and 18.2 for the gradient, 3.7 TB/s; 32768 of 128, bf16, one
+// sequence: 6.7, 7.4 and 7.6; 517 of 32: 6.2, 6.8 and 4.1).
 #include <type_traits>
 
 #include "zmoe_route.h"
@@ -130,7 +130,9 @@ __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __re
   __shared__ float mass[kWaves][W];
   __shared__ int32_t count[W];
   __shared__ float zs[kWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane / LPR, e0 = (lane % LPR) * VPL;
+  constexpr int STEP = kSpread<LPR, VPL, LT>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane / LPR;
+  const int e0 = spread_first<VPL, LT>(lane % LPR);
   const int64_t tile = blockIdx.x, t0 = tile * kTile, t1 = t0 + kTile < seq.T ? t0 + kTile : seq.T;
   if (tile == gridDim.x - 1) {  // a workgroup of its own: S' and N
     int64_t live = 0, tokens = 0;
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __re
     const int64_t slot = tile + s;
     float acc[VPL], z2 = 0.f, nxt[VPL];
     int64_t t = lo + wave * TPW + row;
-    load_lane<VPL>(logits + t * E, e0, E, vec, t < hi, -INFINITY, nxt);
+    load_lane<VPL, STEP>(logits + t * E, e0, E, vec, t < hi, -INFINITY, nxt);
 #pragma unroll
     for (int q = 0; q < VPL; ++q) acc[q] = 0.f;
     for (int e = threadIdx.x; e < E; e += 64 * kWaves) count[e] = 0;
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __re
       float z[VPL], ph[VPL], soft[VPL], sig[VPL];
 #pragma unroll
       for (int q = 0; q < VPL; ++q) z[q] = nxt[q];
-      load_lane<VPL>(logits + (t + ROWS) * E, e0, E, vec, t + ROWS < hi, -INFINITY, nxt);
+      load_lane<VPL, STEP>(logits + (t + ROWS) * E, e0, E, vec, t + ROWS < hi, -INFINITY, nxt);
       const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, sig);  // (past the end: a row of -inf)
       z2 += lse * lse;
 #pragma unroll
@@ -191,7 +193,7 @@ __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __re
     }
     if (row == 0) {
 #pragma unroll
-      for (int q = 0; q < VPL; ++q) mass[wave][e0 + q] = acc[q];
+      for (int q = 0; q < VPL; ++q) mass[wave][e0 + lane_element<VPL, STEP, LT>(q)] = acc[q];
     }
     if (lane == 0) zs[wave] = z2;
     __syncthreads();
@@ -212,8 +214,9 @@ __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, S
                                                                  float* __restrict__ a, float* __restrict__ out,
                                                                  float* __restrict__ inv_tokens) {
   constexpr int GROUPS = kSumThreads / kColumns;  // threads of one expert
-  __shared__ double red[GROUPS][kColumns];
-  __shared__ int64_t redc[GROUPS][kColumns];
+  constexpr int WAVES = kSumThreads / 64;
+  __shared__ double red[WAVES][kColumns];
+  __shared__ int64_t redc[WAVES][kColumns];
   __shared__ double wave_sums[kSumThreads / 64][2];
   __shared__ int last;
   const int s = blockIdx.x, cb = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, S
   double mass = 0.0;
   int64_t count = 0;
   if (e < E) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = first + group; i < end; i += GROUPS) {
       mass += (double)w.mass[i * E + e];
       count += w.count[i * E + e];
@@ -232,14 +235,19 @@ __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, S
   double z2 = 0.0;
   if (cb == 0)
     for (int64_t i = first + threadIdx.x; i < end; i += kSumThreads) z2 += (double)w.zsum[i];
-  red[group][col] = mass;
-  redc[group][col] = count;
+  mass += __shfl_xor(mass, kColumns, 64);  // a wave has two threads of an expert
+  count += __shfl_xor(count, kColumns, 64);
+  if (lane < kColumns) {
+    red[wave][col] = mass;
+    redc[wave][col] = count;
+  }
   __syncthreads();
   double balance = 0.0;
   if (group == 0) {
-    for (int g = 1; g < GROUPS; ++g) {
-      mass += red[g][col];
-      count += redc[g][col];
+#pragma unroll
+    for (int w2 = 1; w2 < WAVES; ++w2) {
+      mass += red[w2][col];
+      count += redc[w2][col];
     }
     if (e < E) {
       const double ae =
@@ -290,6 +298,24 @@ __global__ __launch_bounds__(kSumThreads) void losses_sum_kernel(int E, int k, S
   }
 }
 
+// A lane's numbers of a row of E in f32, at the places of its logits (of type LT), 0 past it; rows of whole 16 bytes in
+// fours.
+template <int VPL, int STEP, typename LT>
+__device__ __forceinline__ void load_of(const float* __restrict__ row, int e0, int E, bool live, float (&v)[VPL]) {
+  const bool vec = E % 4 == 0;
+#pragma unroll
+  for (int q = 0; q < VPL; q += 4) {
+    const int e = e0 + lane_element<VPL, STEP, LT>(q);
+    if (vec && live && e < E) {
+      const float4 x = *reinterpret_cast<const float4*>(row + e);
+      v[q] = x.x, v[q + 1] = x.y, v[q + 2] = x.z, v[q + 3] = x.w;
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[q + u] = !vec && live && e + u < E ? row[e + u] : 0.f;
+    }
+  }
+}
+
 // A workgroup has ROWS tokens at a time, a quarter of a tile or so: as many workgroups as keep every CU's loads going.
 template <int LPR, int VPL, bool SOFT, typename LT>
 __global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* __restrict__ logits, int E, bool vec,
@@ -298,20 +324,20 @@ __global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* 
                                                                       const float* __restrict__ g_balance,
                                                                       const float* __restrict__ g_z,
                                                                       LT* __restrict__ dz) {
-  constexpr int TPW = 64 / LPR;
+  constexpr int TPW = 64 / LPR, STEP = kSpread<LPR, VPL, LT>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = lane / LPR, e0 = (lane % LPR) * VPL;
+  const int row = lane / LPR, e0 = spread_first<VPL, LT>(lane % LPR);
   const int64_t tw = ((int64_t)blockIdx.x * kWaves + wave) * TPW, t = tw + row;
   if (tw >= seq.T) return;
   const bool there = t < seq.T;
   float z[VPL];
-  load_lane<VPL>(logits + t * E, e0, E, vec, there, -INFINITY, z);
+  load_lane<VPL, STEP>(logits + t * E, e0, E, vec, there, -INFINITY, z);
   const float gb = g_balance ? *g_balance : 0.f, gz = g_z ? 2.f * *g_z * *inv_tokens : 0.f;
   int s = seq.after(tw);
   while (s < seq.S && seq.at(s + 1) <= t) ++s;
   const bool in = there && s < seq.S && seq.at(s) <= t;
   float as[VPL];
-  load_lane<VPL>(a + (int64_t)s * E, e0, E, E % 4 == 0, in, 0.f, as);
+  load_of<VPL, STEP, LT>(a + (int64_t)s * E, e0, E, in, as);
   float ph[VPL], soft[VPL], sig[VPL], dot = 0.f;
   const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, sig);
 #pragma unroll
@@ -323,7 +349,7 @@ __global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* 
     if constexpr (!SOFT) d *= 1.f - sig[q];
     z[q] = in ? d + gz * lse * soft[q] : 0.f;
   }
-  if (there) store_lane<VPL>(dz + t * E, e0, E, vec, z);
+  if (there) store_lane<VPL, STEP>(dz + t * E, e0, E, vec, z);
 }
 
 int check_sizes(const char* what, int dtype, int64_t T, int E, int score, const void* cu, int64_t S) {

@@ -224,11 +224,11 @@ __device__ __forceinline__ float lanes_fmax(float v) {
   return v;
 }
 
-// Chunks of a lane's VPL elements: 16 bytes, or 8 where a lane's elements are no whole 16.
+// Chunks of a lane's VPL elements: 16 bytes, or four bf16 where a lane's elements are no whole 16.
 template <int VPL, typename LT>
 struct LaneChunk {
-  static constexpr int N = VPL * sizeof(LT) % 16 == 0 ? 16 / sizeof(LT) : 8 / sizeof(LT);
-  static_assert(VPL % N == 0, "lanes of whole chunks");
+  static constexpr int N = VPL * sizeof(LT) % 16 == 0 ? 16 / sizeof(LT) : 4;
+  static_assert(VPL % N == 0 && N % 4 == 0, "lanes of whole chunks");
 };
 
 // x as a value that the compiler knows nothing of (so nothing computed from it leaves the loop).
@@ -237,26 +237,38 @@ __device__ __forceinline__ int opaque(int x) {
   return x;
 }
 
-// Elements e0 .. e0 + VPL - 1 of a row of E, `fill` past it. vec: rows are whole 16-byte chunks and lie on 16 (e0 is a
-// multiple of VPL, so a lane's chunks are wholly in the row or out of it).
+// Where a lane's element q lies: VPL consecutive ones (STEP 0), or chunks STEP elements apart, so that a row's lanes
+// read and write consecutive chunks (from the lane's first, `spread_first`): f32 grads of 32749 x 256 logits 18.2 us against
+// 21.8 with 64 bytes from lane to lane.
+template <int VPL, int STEP, typename LT>
+__device__ __forceinline__ constexpr int lane_element(int q) {
+  constexpr int N = LaneChunk<VPL, LT>::N;
+  return STEP ? q / N * STEP + q % N : q;
+}
+template <int LPR, int VPL, typename LT>
+constexpr int kSpread = LPR * LaneChunk<VPL, LT>::N;
 template <int VPL, typename LT>
+__device__ __forceinline__ int spread_first(int lane_of_row) {
+  return lane_of_row * LaneChunk<VPL, LT>::N;
+}
+
+// A lane's elements of a row of E from e0 on, `fill` past it. vec: rows are whole 16-byte chunks and lie on 16 (so a
+// lane's chunks are wholly in the row or out of it).
+template <int VPL, int STEP = 0, typename LT>
 __device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, int E, bool vec, bool live, float fill,
                                           float (&v)[VPL]) {
   constexpr int N = LaneChunk<VPL, LT>::N;
   if (vec) {
 #pragma unroll
     for (int c = 0; c < VPL / N; ++c) {
-      if (live && e0 + c * N < E) {
+      const int e = e0 + lane_element<VPL, STEP, LT>(c * N);
+      if (live && e < E) {
         if constexpr (N * sizeof(LT) == 16) {
-          unpack_chunk(*reinterpret_cast<const uint4*>(row + e0 + c * N), &v[c * N], LT{});
+          unpack_chunk(*reinterpret_cast<const uint4*>(row + e), &v[c * N], LT{});
         } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(row + e0 + c * N);
-          if constexpr (sizeof(LT) == 2) {
-            v[c * N] = __uint_as_float(x.x << 16), v[c * N + 1] = __uint_as_float(x.x & 0xffff0000u);
-            v[c * N + 2] = __uint_as_float(x.y << 16), v[c * N + 3] = __uint_as_float(x.y & 0xffff0000u);
-          } else {
-            v[c * N] = __uint_as_float(x.x), v[c * N + 1] = __uint_as_float(x.y);
-          }
+          const uint2 x = *reinterpret_cast<const uint2*>(row + e);
+          v[c * N] = __uint_as_float(x.x << 16), v[c * N + 1] = __uint_as_float(x.x & 0xffff0000u);
+          v[c * N + 2] = __uint_as_float(x.y << 16), v[c * N + 3] = __uint_as_float(x.y & 0xffff0000u);
         }
       } else {
 #pragma unroll
@@ -266,30 +278,34 @@ __device__ __forceinline__ void load_lane(const LT* __restrict__ row, int e0, in
   } else {
     const int have = live ? opaque(E - e0) : 0;  // (not kept as VPL masks over a caller's loop: registers)
 #pragma unroll
-    for (int q = 0; q < VPL; ++q) v[q] = q < have ? to_f32(row[e0 + q]) : fill;
+    for (int q = 0; q < VPL; ++q) {
+      const int at = lane_element<VPL, STEP, LT>(q);
+      v[q] = at < have ? to_f32(row[e0 + at]) : fill;
+    }
   }
 }
-template <int VPL, typename LT>
+template <int VPL, int STEP = 0, typename LT>
 __device__ __forceinline__ void store_lane(LT* __restrict__ row, int e0, int E, bool vec, const float (&v)[VPL]) {
   constexpr int N = LaneChunk<VPL, LT>::N;
   if (vec) {
 #pragma unroll
     for (int c = 0; c < VPL / N; ++c) {
-      if (e0 + c * N >= E) continue;
+      const int e = e0 + lane_element<VPL, STEP, LT>(c * N);
+      if (e >= E) continue;
       if constexpr (N * sizeof(LT) == 16) {
-        *reinterpret_cast<uint4*>(row + e0 + c * N) = pack_chunk(&v[c * N], LT{});
-      } else if constexpr (sizeof(LT) == 2) {
-        *reinterpret_cast<uint2*>(row + e0 + c * N) =
-            make_uint2(pack_bf16x2(v[c * N], v[c * N + 1]), pack_bf16x2(v[c * N + 2], v[c * N + 3]));
+        *reinterpret_cast<uint4*>(row + e) = pack_chunk(&v[c * N], LT{});
       } else {
-        *reinterpret_cast<float2*>(row + e0 + c * N) = make_float2(v[c * N], v[c * N + 1]);
+        *reinterpret_cast<uint2*>(row + e) =
+            make_uint2(pack_bf16x2(v[c * N], v[c * N + 1]), pack_bf16x2(v[c * N + 2], v[c * N + 3]));
       }
     }
   } else {
     const int have = opaque(E - e0);
 #pragma unroll
-    for (int q = 0; q < VPL; ++q)
-      if (q < have) row[e0 + q] = from_f32<LT>(v[q]);
+    for (int q = 0; q < VPL; ++q) {
+      const int at = lane_element<VPL, STEP, LT>(q);
+      if (at < have) row[e0 + at] = from_f32<LT>(v[q]);
+    }
   }
 }
 
