@@ -52,22 +52,27 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: Optional[torch.Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
+    @staticmethod
+    def _check_group(g) -> None:
+        """Whether a group's numbers are a step's."""
+        lr, betas = g["lr"], tuple(g["betas"])
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
+                raise ValueError("AdamW: lr must be a number or a float32 tensor of one element")
+        elif not lr >= 0.0:
+            raise ValueError(f"AdamW: lr must not be negative, got {lr}")
+        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
+        if not g["eps"] >= 0.0 or not g["weight_decay"] >= 0.0:
+            raise ValueError(f"AdamW: eps and weight_decay must not be negative, got {g['eps']} and {g['weight_decay']}")
+        if g["state_bits"] not in _STATE_DTYPES:
+            raise ValueError(f"AdamW: state_bits must be 32 or 8, got {g['state_bits']}")
+
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         g = self.param_groups[-1]
         try:
-            lr, betas = g["lr"], tuple(g["betas"])
-            if isinstance(lr, torch.Tensor):
-                if lr.numel() != 1 or (lr.is_cuda and lr.dtype != torch.float32):
-                    raise ValueError("AdamW: lr must be a number or a float32 tensor of one element")
-            elif not lr >= 0.0:
-                raise ValueError(f"AdamW: lr must not be negative, got {lr}")
-            if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
-                raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
-            if not g["eps"] >= 0.0 or not g["weight_decay"] >= 0.0:
-                raise ValueError(f"AdamW: eps and weight_decay must not be negative, got {g['eps']} and {g['weight_decay']}")
-            if g["state_bits"] not in _STATE_DTYPES:
-                raise ValueError(f"AdamW: state_bits must be 32 or 8, got {g['state_bits']}")
+            self._check_group(g)
             if len({id(p) for p in g["params"]}) != len(g["params"]):
                 raise ValueError("AdamW: a parameter is given twice")  # (one launch would write it from two places)
             for p in g["params"]:
@@ -210,32 +215,61 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, with the state's own types kept (torch casts a state to its parameter's); a torch AdamW's state
-        loads too, its moments in float32, but for forms of the step that this one does not have."""
-        for name in ("amsgrad", "maximize"):
-            if any(g.get(name) for g in state_dict["param_groups"]):
-                raise ValueError(f"AdamW: the state of a step with {name}")
-        super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        groups = [(g, p) for g in self.param_groups for p in g["params"]]
-        for i, (g, p) in zip(ids, groups):
-            if i not in saved:
-                continue
-            m, v = _STATE_DTYPES[g["state_bits"]]
-            src, st = saved[i], {}
-            st["step"] = torch.as_tensor(src["step"]).to(dtype=torch.float32, device=p.device, copy=True).reshape(())
-            for name, dtype in (("exp_avg", m), ("exp_avg_sq", v)):
-                t = src[name]
-                if t.shape != p.shape or t.is_floating_point() != (dtype == torch.float32) \
-                        or (dtype != torch.float32 and t.dtype != dtype):
-                    raise ValueError(f"AdamW: {name} of {t.dtype} and shape {tuple(t.shape)} does not fit a parameter of "
-                                     f"shape {tuple(p.shape)} with moments in {g['state_bits']} bits")
-                st[name] = torch.empty_like(p, dtype=dtype)
-                if g["state_bits"] == 8 and not (t.is_contiguous() and p.is_contiguous()) \
-                        and t.stride() != st[name].stride():  # blocks are of elements next to each other in memory
-                    raise ValueError(f"AdamW: 8-bit {name} of strides {t.stride()} for a parameter of strides {p.stride()}")
-                st[name].copy_(t)
-            if g["state_bits"] == 8:
-                for name in ("exp_avg_scale", "exp_avg_sq_scale"):
-                    st[name] = src[name].to(dtype=torch.float32, device=p.device, copy=True)
-            self.state[p] = st
+        loads too, its moments in float32, but for forms of the step that this one does not have. A state that is refused
+        leaves the optimizer as it was: the new state is made, and checked, before torch takes the groups over."""
+        made: dict = {}
+        before = self.register_load_state_dict_pre_hook(lambda opt, d: made.update(opt._state_made_of(d)))
+        after = self.register_load_state_dict_post_hook(lambda opt: opt.state.update(made), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()
+
+    def _state_made_of(self, state_dict) -> dict:
+        """Each parameter's state from a state dict, or ValueError."""
+        saved, new = state_dict["param_groups"], {}
+        if [len(g["params"]) for g in saved] != [len(g["params"]) for g in self.param_groups]:
+            return new  # (which torch refuses)
+        for g, group in zip(saved, self.param_groups):
+            for name in ("amsgrad", "maximize"):
+                if g.get(name):
+                    raise ValueError(f"AdamW: the state of a step with {name}")
+            missing = {"lr", "betas", "eps", "weight_decay"} - g.keys()
+            if missing:
+                raise ValueError(f"AdamW: a group without {', '.join(sorted(missing))}")
+            g = {"state_bits": 32, **g}
+            self._check_group(g)
+            for i, p in zip(g["params"], group["params"]):
+                if i in state_dict["state"]:
+                    new[p] = self._one_state_made_of(state_dict["state"][i], p, g["state_bits"])
+        return new
+
+    @staticmethod
+    def _one_state_made_of(src, p: torch.Tensor, bits: int) -> dict:
+        moments = dict(zip(("exp_avg", "exp_avg_sq"), _STATE_DTYPES[bits]))
+        scales = ("exp_avg_scale", "exp_avg_sq_scale") if bits == 8 else ()
+        for name in (*moments, *scales):
+            if not isinstance(src.get(name), torch.Tensor):
+                raise ValueError(f"AdamW: a state without {name}")
+        if "step" not in src or torch.as_tensor(src["step"]).numel() != 1:
+            raise ValueError("AdamW: a state without its step count")
+        st = {"step": torch.as_tensor(src["step"]).to(dtype=torch.float32, device=p.device, copy=True).reshape(())}
+        for name, dtype in moments.items():
+            t = src[name]
+            if t.shape != p.shape or t.is_floating_point() != (dtype == torch.float32) \
+                    or (dtype != torch.float32 and t.dtype != dtype):
+                raise ValueError(f"AdamW: {name} of {t.dtype} and shape {tuple(t.shape)} does not fit a parameter of "
+                                 f"shape {tuple(p.shape)} with moments in {bits} bits")
+            st[name] = torch.empty_like(p, dtype=dtype, requires_grad=False)
+            if bits == 8 and not (t.is_contiguous() and p.is_contiguous()) \
+                    and t.stride() != st[name].stride():  # blocks are of elements next to each other in memory
+                raise ValueError(f"AdamW: 8-bit {name} of strides {t.stride()} for a parameter of strides {p.stride()}")
+            st[name].copy_(t)
+        blocks = -(-p.numel() // ops.ADAMW_BLOCK)
+        for name in scales:
+            if src[name].shape != (blocks,) or not src[name].is_floating_point():
+                raise ValueError(f"AdamW: {name} of {src[name].dtype} and shape {tuple(src[name].shape)}, not a scale for each "
+                                 f"of {blocks} blocks")
+            st[name] = src[name].to(dtype=torch.float32, device=p.device, copy=True)
+        return st
