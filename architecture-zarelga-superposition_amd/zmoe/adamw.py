@@ -241,7 +241,7 @@ class AdamW(torch.optim.Optimizer):
             g = {"state_bits": 32, **g}
             self._check_group(g)
             for i, p in zip(g["params"], group["params"]):
-                if i in state_dict["state"]:
+                if state_dict["state"].get(i):  # (reading opt.state of a parameter before its first step leaves an empty one)
                     new[p] = self._one_state_made_of(state_dict["state"][i], p, g["state_bits"])
         return new
 

@@ -110,6 +110,17 @@ def test_groups_that_do_not_match():
         assert same(opt.state_dict(), before)
 
 
+def test_parameters_without_a_state():
+    """Those that had no step yet: no entry, or an empty one (which reading opt.state leaves)."""
+    params, opt = made()
+    some = states(32)
+    some[1] = {}
+    del some[2]
+    opt.load_state_dict(dict_of(opt, some))
+    assert same(dict(opt.state[params[0]]), some[0]) and not opt.state[params[1]] and not opt.state[params[2]]
+    assert len(opt.moments()) == 3
+
+
 def test_hooks():
     """A caller's hooks in front of a load change what is loaded, those behind it see the state as it stays."""
     params, opt = made(8)
