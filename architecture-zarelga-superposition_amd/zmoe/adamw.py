@@ -240,6 +240,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: a group without {', '.join(sorted(missing))}")
             g = {"state_bits": 32, **g}
             self._check_group(g)
+            if g.get("decoupled_weight_decay") is False and g["weight_decay"] != 0.0:
+                raise ValueError("AdamW: the state of a step whose decay goes through its moments")
             for i, p in zip(g["params"], group["params"]):
                 if state_dict["state"].get(i):  # (reading opt.state of a parameter before its first step leaves an empty one)
                     new[p] = self._one_state_made_of(state_dict["state"][i], p, g["state_bits"])

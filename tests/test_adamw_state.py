@@ -74,7 +74,7 @@ REFUSED = {
          change(2, exp_avg_sq=torch.zeros(300, dtype=torch.int64)), change(1, exp_avg=None), change(1, step=None),
          change(2, step=torch.zeros(2)), change(2, exp_avg_sq=0.5), groups(state_bits=16), groups(state_bits=8),
          groups(lr=-1.0), groups(betas=(0.9, 1.0)), groups(eps=-1e-8), groups(weight_decay=-0.1), groups(amsgrad=True),
-         groups(maximize=True)],
+         groups(maximize=True), groups(decoupled_weight_decay=False, weight_decay=0.1)],
     8: [lambda d: d.update(state=states(32)), change(1, **states(32)[1]), change(1, exp_avg_scale=torch.zeros(2)),
         change(2, exp_avg_sq_scale=torch.zeros(3)), change(1, exp_avg_scale=None),
         change(1, exp_avg_scale=torch.zeros(3, dtype=torch.int64)), change(2, exp_avg=torch.zeros(300, dtype=torch.uint8)),
@@ -140,3 +140,16 @@ def test_torchs_states():
     state = theirs.state_dict()["state"]
     opt.load_state_dict(dict_of(opt, state))
     assert same(opt.state_dict()["state"], {i: {k: v.float() for k, v in s.items()} for i, s in state.items()})
+    # Adam's decay goes through its moments, which this step does not do; without decay the two steps are one
+    for decay, ok in ((0.0, True), (0.1, False)):
+        adam = torch.optim.Adam(params, lr=0.1, weight_decay=decay)
+        adam.step()
+        from zmoe.adamw import AdamW
+
+        ours = AdamW(params)
+        if ok:
+            ours.load_state_dict(adam.state_dict())
+        else:
+            with pytest.raises(ValueError, match="decay"):
+                ours.load_state_dict(adam.state_dict())
+            assert not ours.state
