@@ -172,18 +172,19 @@ Tensors route(const Tensor& logits, const Opt& bias, int64_t k, int64_t score, i
 }
 
 // route's gradient into out [T, E] (rows `ld` elements apart); false where the general form has to run.
-bool route_form_backward_into(const Tensor& dw, const Tensor& p, const Tensor& idx, const Tensor& logits, int64_t score,
+bool route_form_backward_into(const Tensor& dw, const Tensor& p, const Tensor& idx, const Opt& logits, int64_t score,
                               bool renorm, double scale, const Opt& add, void* out, int64_t ld) {
-  if (!logits.is_cuda() || !known(logits) || logits.dim() != 2 || !logits.is_contiguous() || idx.dim() != 2 ||
-      idx.size(0) != logits.size(0) || !flat(idx, logits, at::kLong) || !flat(dw, logits, at::kFloat) ||
-      !flat(p, logits, at::kFloat) || dw.sizes() != idx.sizes() || p.sizes() != idx.sizes() ||
-      !fits_int(logits.size(1)) || !fits_int(idx.size(1)) || !fits_int(score) ||
-      (add && !(apart(*add) && rows2(*add, logits) && add->sizes() == logits.sizes())))
+  const Tensor& like = logits ? *logits : *add;  // [T, E]
+  if (!like.is_cuda() || !known(like) || like.dim() != 2 || (logits && !logits->is_contiguous()) || idx.dim() != 2 ||
+      idx.size(0) != like.size(0) || !flat(idx, like, at::kLong) || !flat(dw, like, at::kFloat) ||
+      !flat(p, like, at::kFloat) || dw.sizes() != idx.sizes() || p.sizes() != idx.sizes() ||
+      !fits_int(like.size(1)) || !fits_int(idx.size(1)) || !fits_int(score) ||
+      (add && !(apart(*add) && rows2(*add, like) && add->sizes() == like.sizes())))
     return false;
-  const int64_t E = logits.size(1);
+  const int64_t E = like.size(1);
   return zmoe_route_backward(ptr<const float>(dw), ptr<const float>(p), ids(idx), idx.size(0), (int)E, (int)idx.size(1),
-                             (int)score, raw(logits), renorm, (float)scale, add ? raw(*add) : nullptr,
-                             add ? std::max(add->stride(0), E) : 0, out, ld, code(logits), stream_of(logits)) == ZMOE_OK;
+                             (int)score, logits ? raw(*logits) : nullptr, renorm, (float)scale, add ? raw(*add) : nullptr,
+                             add ? std::max(add->stride(0), E) : 0, out, ld, code(like), stream_of(like)) == ZMOE_OK;
 }
 
 Tensor route_backward(const Tensor& dw, const Tensor& p, const Tensor& idx, const Tensor& logits, int64_t score,
@@ -200,13 +201,15 @@ Tensor route_backward(const Tensor& dw, const Tensor& p, const Tensor& idx, cons
 }
 
 Tensor swiglu_route_form_backward(const Tensor& dAs, const Tensor& Hs, const Tensor& dg, const Tensor& p,
-                                  const Tensor& idx, const Tensor& logits, int64_t score, bool renorm, double scale,
+                                  const Tensor& idx, const Opt& logits, int64_t score, bool renorm, double scale,
                                   const Opt& add) {
+  auto rows = [&](const Tensor& t) {
+    return on(t, Hs) && t.scalar_type() == Hs.scalar_type() && t.dim() == 2 && t.size(0) == Hs.size(0);
+  };
   if (Hs.is_cuda() && known(Hs) && Hs.dim() == 2 && Hs.is_contiguous() && flat(dAs, Hs, Hs.scalar_type()) &&
-      dAs.numel() * 2 == Hs.numel() && on(logits, Hs) && logits.scalar_type() == Hs.scalar_type() && logits.dim() == 2 &&
-      logits.size(0) == Hs.size(0)) {
+      dAs.numel() * 2 == Hs.numel() && (logits || add) && rows(logits ? *logits : *add)) {
     const c10::DeviceGuard guard(Hs.device());
-    const int64_t T = Hs.size(0), two_f = Hs.size(1), ld = two_f + logits.size(1);
+    const int64_t T = Hs.size(0), two_f = Hs.size(1), ld = two_f + (logits ? *logits : *add).size(1);
     Tensor G = empty({T, ld}, Hs);
     char* tail = static_cast<char*>(raw(G)) + two_f * G.element_size();
     if (zmoe_swiglu_backward(raw(dAs), raw(Hs), T, two_f / 2, code(Hs), raw(G), ld, stream_of(Hs)) == ZMOE_OK &&
@@ -214,7 +217,7 @@ Tensor swiglu_route_form_backward(const Tensor& dAs, const Tensor& Hs, const Ten
       return G;
   }
   static const auto op =
-      general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+      general<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Opt&,
                      c10::SymInt, bool, double, const Opt&)>("zmoe::swiglu_route_form_backward");
   return op.call(dAs, Hs, dg, p, idx, logits, score, renorm, scale, add);
 }
@@ -1266,7 +1269,7 @@ TORCH_LIBRARY(zmoe_eager, m) {
              "(Tensor d_weight, Tensor topk_prob, Tensor topk_idx, Tensor logits, int score, bool renormalize, "
              "float scale) -> Tensor");
   ZMOE_EAGER(swiglu_route_form_backward,
-             "(Tensor dAs, Tensor Hs, Tensor d_gates, Tensor topk_prob, Tensor topk_idx, Tensor logits, int score, "
+             "(Tensor dAs, Tensor Hs, Tensor d_gates, Tensor topk_prob, Tensor topk_idx, Tensor? logits, int score, "
              "bool renormalize, float scale, Tensor? add) -> Tensor");
   ZMOE_EAGER(router_losses, "(Tensor logits, Tensor topk_idx, Tensor? cu_seqlens, int score) -> Tensor[]");
   ZMOE_EAGER(router_losses_backward,

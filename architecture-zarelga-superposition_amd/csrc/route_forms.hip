@@ -4,8 +4,9 @@
 //   a group's score: its highest s, or the sum of its two highest; the top_groups best groups stay
 //   idx = the k best s in them (s desc, expert asc, NaN first);  w = c p_idx / max(sum p_idx, 1e-12), or c p_idx
 // Backward: dp_j = c (dw_j - sum_i dw_i p_i / S) / S (S the clamped sum; clamped or not renormalised: without the
-// sum's part), dz = dp p (1 - p) for a sigmoid, dz_e = p_e (dp_e - sum_j dp_j p_j) for a softmax, where the sum is 0 if
-// the weights are renormalised: then only selected experts have a grad and the logits are not read.
+// sum's part). Sigmoid: dz = dp p (1 - p), 1 - p from the logit again, for a rounded p has lost it (at z = 12 it is off by 0.5%, from
+// 17.4 on 0). Softmax: dz_e = p_e (dp_e - sum_j dp_j p_j), where the sum is 0 if the weights are renormalised: then
+// only selected experts have a grad and the logits are not read.
 //
 // Where p + b decides, one f32 rounding of p can decide: p comes from double, whose error (some 2^-52) moves an f32
 // rounding for one value in 2^28. Without a bias the experts' order is their logits' order.
@@ -229,7 +230,7 @@ struct RouteBackwardArgs {
   const float* dw;
   const float* p;
   const int64_t* idx;
-  const void* logits;  // softmax only
+  const void* logits;  // null: sigmoids of which p is all there is
   const void* add;     // or null: [T, E] of the grad's type, rows ld_add apart
   int64_t ld_add, T, ld;
   int E, k, renorm, vec;
@@ -272,7 +273,9 @@ __global__ __launch_bounds__(64 * kWaves) void route_backward_kernel(const Route
       for (int j = r; j < k; j += LPR) {
         const int64_t e = a.idx[t * k + j];
         const float pj = a.p[t * k + j], dp = (a.scale * a.dw[t * k + j] - mean) / total;
-        if (e >= 0 && e < E) mine[e] = SOFT ? pj * (dp - inner) : dp * pj * (1.f - pj);
+        if (e < 0 || e >= E) continue;
+        if constexpr (SOFT) mine[e] = pj * (dp - inner);
+        else mine[e] = dp * pj * (a.logits ? sigmoid_complement(to_f32(((const LT*)a.logits)[t * E + e])) : 1.f - pj);
       }
     wave_sync();
     float v[VPL];

@@ -121,6 +121,10 @@ __device__ __forceinline__ double rcp_f64(double x) {
   y = fma(fma(-x, y, 1.0), y, y);
   return fma(fma(-x, y, 1.0), y, y);
 }
+// 1 - sigmoid(z) rounded once, with all its digits where the sigmoid is near 1 (past 100 below every f32).
+__device__ __forceinline__ float sigmoid_complement(float z) {
+  return (float)rcp_f64(1.0 + exp_f64((double)(z > 100.f ? 100.f : z)));
+}
 // sigmoid_f64 of a lane's logits by these two, all at once (their chains overlap); exact ties near 0 apart.
 template <int N>
 __device__ __forceinline__ void sigmoids_rounded(const float (&z)[N], float (&p)[N]) {

@@ -125,7 +125,7 @@ class _FusedMoELayer(torch.autograd.Function):
                                  "scatter2scatter")                                  # = w * Y
         out = _zl.combine(Y_s, None, k, S, pad_rows, pad_total)                      # moe_layer.py:48-56
         ctx.save_for_backward(x, W1, W2, W3, Ws_down, Hs, As, p, idx, w_sorted, se, ss, off, H, A_s, pad_rows,
-                              None if form is None and not with_logits else logits)
+                              None if form is None else logits)  # (the reference's form has its slope from p, in bf16)
         ctx.k, ctx.E, ctx.fs, ctx.form, ctx.out_rows = k, E, fs, form, out.shape[0]
         ctx.mark_non_differentiable(idx, off)
         ctx.set_materialize_grads(False)  # no zero-filled grads for idx and off (two fill launches)

@@ -302,7 +302,7 @@ def route(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, sco
     of which the ``top_groups`` with the highest score stay, a group's score being the sum of its two best experts'
     (``group_scores`` 2) or the best one's (1). Slots come best first, equal experts by their number, NaN first. Weights are
     ``scale`` p / max(sum p, 1e-12) over a token's k, without ``renormalize`` ``scale`` p. Gradients reach the logits through
-    the weights. A row of -inf alone has p = 0."""
+    the weights; the logits are kept for that. A row of -inf alone has p = 0."""
     if logits.dim() < 1:
         raise ValueError("route: logits must be [..., E]")
     if bias is not None:

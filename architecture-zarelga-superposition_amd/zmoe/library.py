@@ -201,10 +201,11 @@ def _(d_weight, topk_prob, topk_idx, logits, score, renormalize, scale):
 
 @layer_op("swiglu_route_form_backward")
 def swiglu_route_form_backward(dAs: torch.Tensor, Hs: torch.Tensor, d_gates: torch.Tensor, topk_prob: torch.Tensor,
-                               topk_idx: torch.Tensor, logits: torch.Tensor, score: int, renormalize: bool, scale: float,
-                               add: Optional[torch.Tensor]) -> torch.Tensor:
-    """``swiglu_route_backward`` for ``route``'s forms; ``add``: what the router's losses give the logits."""
-    (T, two_f), E = Hs.shape, logits.shape[1]
+                               topk_idx: torch.Tensor, logits: Optional[torch.Tensor], score: int, renormalize: bool,
+                               scale: float, add: Optional[torch.Tensor]) -> torch.Tensor:
+    """``swiglu_route_backward`` for ``route``'s forms; ``add``: what the router's losses give the logits. ``logits`` None
+    (``add`` is given then): the reference's form, whose slope is that of its rounded probabilities."""
+    (T, two_f), E = Hs.shape, (add if logits is None else logits).shape[1]
     G = torch.empty((T, two_f + E), dtype=Hs.dtype, device=Hs.device)
     _z.swiglu_backward(dAs, Hs, out=G[:, :two_f])
     _z.route_backward(d_gates, topk_prob, topk_idx, E, logits, score, renormalize, scale, Hs.dtype, add, out=G[:, two_f:])
@@ -213,7 +214,7 @@ def swiglu_route_form_backward(dAs: torch.Tensor, Hs: torch.Tensor, d_gates: tor
 
 @swiglu_route_form_backward.register_fake
 def _(dAs, Hs, d_gates, topk_prob, topk_idx, logits, score, renormalize, scale, add):
-    return _empty((Hs.shape[0], Hs.shape[1] + logits.shape[1]), Hs)
+    return _empty((Hs.shape[0], Hs.shape[1] + (add if logits is None else logits).shape[1]), Hs)
 
 
 @layer_op("router_losses")

@@ -203,7 +203,8 @@ def route_backward(d_weight: torch.Tensor, topk_prob: torch.Tensor, topk_idx: to
                    logits: Optional[torch.Tensor], score: int, renormalize: bool, scale: float, dtype: torch.dtype,
                    add: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """d_logits [T, E] of ``dtype`` (``add``, of the same, added before its rounding); ``out`` may be a column slice of a
-    wider row-major buffer. ``logits`` (of ``dtype``): softmax scores need them."""
+    wider row-major buffer. ``logits`` (of ``dtype``): softmax scores need them; None: a sigmoid's slope is p (1 - p) of the
+    given probabilities."""
     dev = _require_cuda(d_weight, topk_prob, topk_idx, logits, add, out)
     T, k = topk_idx.shape
     E = num_experts

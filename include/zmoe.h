@@ -541,7 +541,9 @@ int zmoe_route(const void* logits, int logits_dtype, int64_t T, int E, int k, in
 
 /* Its gradient by the logits, from d_weight [T, k] f32: d_logits [T, E], rows ld_d_logits >= E apart; `add` (or NULL), of
  * the same type with rows ld_add apart, is added before the one rounding (the losses' gradient). `logits` (type of
- * d_logits, packed) are needed for softmax scores. Selection and biases have no gradient. */
+ * d_logits, packed) are needed for softmax scores; for sigmoids the slope's 1 - p comes from them, or, where they are NULL, from
+ * topk_prob (all that a gate which rounds its probabilities has; no slope is left of a p that is rounded to 1). Selection and
+ * biases have no gradient. */
 int zmoe_route_backward(const float* d_weight, const float* topk_prob, const int64_t* topk_idx, int64_t T, int E, int k,
                         int score, const void* logits, int renormalize, float scale, const void* add, int64_t ld_add,
                         void* d_logits, int64_t ld_d_logits, int d_logits_dtype, void* stream);

@@ -22,6 +22,11 @@ def probabilities(z, score):
     return torch.where(none, torch.zeros_like(e), e / e.sum(-1, keepdim=True))
 
 
+def complement(z):
+    """1 - sigmoid(z) in float64, with all its digits where the sigmoid is near 1."""
+    return 1 / (1 + torch.exp(z.detach().to(F64)))
+
+
 def rounded(z, score):
     """The probabilities rounded once to float32 (those that the selection sees)."""
     if score == "sigmoid":
@@ -72,9 +77,8 @@ def weights_backward(z, idx, dw, score, renormalize, scale):
         dp = (dp - torch.where(free, (dp * p).sum(1, keepdim=True) / S, 0.0)) / S
         mp = (mp + torch.where(free, (mp * p).sum(1, keepdim=True) / S, 0.0)) / S
     if score == "sigmoid":
-        at = torch.zeros_like(full)
-        # (1 - p of a p that is rounded to f32 is off by that rounding: 2^-24 p, not 2^-24 (1 - p))
-        return at.scatter(1, idx, dp * p * (1 - p)), at.scatter(1, idx, mp * p * (1 + p))
+        at, slope = torch.zeros_like(full), p * complement(z).gather(1, idx)
+        return at.scatter(1, idx, dp * slope), at.scatter(1, idx, mp * slope)
     at = torch.zeros_like(full)
     inner, minner = (dp * p).sum(1, keepdim=True), (mp * p).sum(1, keepdim=True)
     if renormalize:
