@@ -85,11 +85,11 @@ size_t lay_out(int64_t T, int E, int S, char* base, Scratch* out) {
   return o;
 }
 
-// A token's values in a row of lanes from its logits z (-inf past E): ph, the softmax's shares and (sigmoid form) the
-// sigmoids, all 0 where every logit is -inf; its lse.
+// A token's values in a row of lanes from its logits z (-inf past E): ph and the softmax's shares, all 0 where every logit
+// is -inf, and (sigmoid form) 1 - sigmoid, for z > 0 from e^-z, as the difference would lose it; its lse.
 template <int LPR, int VPL, bool SOFT>
 __device__ __forceinline__ float token_row(const float (&z)[VPL], float (&ph)[VPL], float (&soft)[VPL],
-                                           float (&sig)[VPL]) {
+                                           float (&rest)[VPL]) {
   float m = z[0];
 #pragma unroll
   for (int q = 1; q < VPL; ++q) m = fmaxf(m, z[q]);
@@ -102,8 +102,10 @@ __device__ __forceinline__ float token_row(const float (&z)[VPL], float (&ph)[VP
     soft[q] = exp_fast(z[q] - m);
     sum += soft[q];
     if constexpr (!SOFT) {
-      sig[q] = sigmoid_hw(z[q]);
-      total += sig[q];
+      const float u = exp_fast(-z[q]);
+      ph[q] = __builtin_amdgcn_rcpf(1.f + u);
+      rest[q] = z[q] > 0.f ? u * ph[q] : 1.f - ph[q];
+      total += ph[q];
     }
   }
   sum = lanes_sum<LPR>(sum);
@@ -117,7 +119,7 @@ __device__ __forceinline__ float token_row(const float (&z)[VPL], float (&ph)[VP
     total = lanes_sum<LPR>(total);
     const float inv_total = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
-    for (int q = 0; q < VPL; ++q) ph[q] = sig[q] * inv_total;
+    for (int q = 0; q < VPL; ++q) ph[q] *= inv_total;
   }
   return none && sum == 0.f ? 0.f : m + logf(sum);
 }
@@ -175,11 +177,11 @@ __global__ __launch_bounds__(64 * kWaves) void losses_tile_kernel(const LT* __re
       if (e >= 0 && e < E) atomicAdd(&count[e], 1);  // whole numbers: any order
     }
     for (int64_t b = lo; b < hi; b += ROWS, t += ROWS) {  // the next rows are on their way while these are added
-      float z[VPL], ph[VPL], soft[VPL], sig[VPL];
+      float z[VPL], ph[VPL], soft[VPL], rest[VPL];
 #pragma unroll
       for (int q = 0; q < VPL; ++q) z[q] = nxt[q];
       load_lane<VPL, STEP>(logits + (t + ROWS) * E, e0, E, vec, t + ROWS < hi, -INFINITY, nxt);
-      const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, sig);  // (past the end: a row of -inf)
+      const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, rest);  // (past the end: a row of -inf)
       z2 += lse * lse;
 #pragma unroll
       for (int q = 0; q < VPL; ++q) acc[q] += ph[q];
@@ -338,15 +340,15 @@ __global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* 
   const bool in = there && s < seq.S && seq.at(s) <= t;
   float as[VPL];
   load_of<VPL, STEP, LT>(a + (int64_t)s * E, e0, E, in, as);
-  float ph[VPL], soft[VPL], sig[VPL], dot = 0.f;
-  const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, sig);
+  float ph[VPL], soft[VPL], rest[VPL], dot = 0.f;
+  const float lse = token_row<LPR, VPL, SOFT>(z, ph, soft, rest);
 #pragma unroll
   for (int q = 0; q < VPL; ++q) dot += ph[q] * as[q];
   dot = lanes_sum<LPR>(dot);
 #pragma unroll
   for (int q = 0; q < VPL; ++q) {
     float d = gb * (ph[q] * (as[q] - dot));
-    if constexpr (!SOFT) d *= 1.f - sig[q];
+    if constexpr (!SOFT) d *= rest[q];
     z[q] = in ? d + gz * lse * soft[q] : 0.f;
   }
   if (there) store_lane<VPL, STEP>(dz + t * E, e0, E, vec, z);

@@ -142,10 +142,9 @@ __device__ __forceinline__ void sigmoids_rounded(const float (&z)[N], float (&p)
   }
 }
 
-// e^x and the sigmoid in f32 by the hardware's exp2 and reciprocal: off by |x| + 2 roundings (the product with log2 e, and the
-// two instructions); -inf gives 0, +inf inf (1), NaN stays. Where no selection hangs on them.
+// e^x in f32 by the hardware's exp2: off by |x| + 1 roundings (the product with log2 e, and the instruction); -inf gives 0,
+// +inf inf, NaN stays. Where no selection hangs on it.
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f); }
-__device__ __forceinline__ float sigmoid_hw(float x) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-x)); }
 
 // A row of 16 lanes and its neighbour's value: two rows' results together, in 32 lanes.
 struct Two {

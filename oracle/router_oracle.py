@@ -125,16 +125,15 @@ def losses_backward(z, idx, score, cu, g_balance, g_z):
     T, E = z.shape
     _, _, a, n_all = losses(z, idx, score, cu)
     cu = [0, T] if cu is None else cu.tolist()
-    ph, soft, sig, lse = _shares(z, score)
+    ph, soft, _, lse = _shares(z, score)
     val, mag = torch.zeros(T, E, dtype=F64, device=z.device), torch.zeros(T, E, dtype=F64, device=z.device)
     for s, (lo, hi) in enumerate(zip(cu[:-1], cu[1:])):
         if hi <= lo:
             continue
         r = slice(lo, hi)
         dot = (ph[r] * a[s]).sum(-1, keepdim=True)
-        f = ph[r] * (1 - sig[r]) if score == "sigmoid" else ph[r]
+        f = ph[r] * complement(z[r]) if score == "sigmoid" else ph[r]
         zpart = 2 * g_z / n_all * lse[r].unsqueeze(1) * soft[r]
         val[r] = g_balance * f * (a[s] - dot) + zpart
-        fm = ph[r] * (1 + sig[r]) if score == "sigmoid" else ph[r]
-        mag[r] = abs(g_balance) * fm * (a[s] + dot) + zpart.abs()
+        mag[r] = abs(g_balance) * f * (a[s] + dot) + zpart.abs()
     return val, mag

@@ -10,6 +10,7 @@ import torch
 from helpers import gen
 from oracle import router_oracle as O
 from test_gpu_route import check as check_route
+from test_gpu_router_losses import check as check_losses
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +103,19 @@ def test_default_form_keeps_its_probabilities(hip_device):
     out, idx, (balance, z) = layer(xg, router_losses=True)
     torch.autograd.backward([out, balance, z], [dout, torch.zeros_like(balance), torch.zeros_like(z)])
     assert torch.equal(layer.gate.weight.grad, without["gate.weight"]) and torch.equal(xg.grad, without["x"])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("T,E,k", [(1, 2, 2), (7, 8, 3), (33, 64, 8), (20, 72, 5), (130, 128, 8), (40, 160, 6), (65, 256, 8),
+                                   (9, 300, 7), (33, 1024, 16)])
+def test_losses(T, E, k, dt, hip_device):
+    """Both losses, and the balance alone: the z loss would cover what the balance loses."""
+    z = saturated(T, E, dt, hip_device)
+    z[1 % T] = z[1 % T].clamp(-80, 80)  # (far logits apart: a z loss of 1e60)
+    idx = torch.topk(z.float(), k).indices
+    cu = torch.tensor([0, T // 3, T], device=hip_device)
+    for gb, gz in ((0.3, 0.05), (0.3, 0.0)):
+        grad = check_losses(z, idx, "sigmoid", cu, gb, gz)[2]
+    far = (z.float() > 20) & (z.float() < 40)
+    if T > 20:  # (two experts and more in a row: their shares pull against each other)
+        assert far.any() and (grad[far] != 0).float().mean() > 0.99
