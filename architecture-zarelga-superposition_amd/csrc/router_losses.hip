@@ -95,7 +95,7 @@ __device__ __forceinline__ float token_row(const float (&z)[VPL], float (&ph)[VP
   for (int q = 1; q < VPL; ++q) m = fmaxf(m, z[q]);
   m = lanes_fmax<LPR>(m);
   const bool none = m == -INFINITY;
-  m = none ? 0.f : m;
+  m = fabsf(m) == INFINITY ? 0.f : m;  // (+inf: an lse of inf, unless a NaN is there too)
   float sum = 0.f, total = 0.f;
 #pragma unroll
   for (int q = 0; q < VPL; ++q) {
@@ -349,7 +349,8 @@ __global__ __launch_bounds__(64 * kWaves) void losses_backward_kernel(const LT* 
   for (int q = 0; q < VPL; ++q) {
     float d = gb * (ph[q] * (as[q] - dot));
     if constexpr (!SOFT) d *= rest[q];
-    z[q] = in ? d + gz * lse * soft[q] : 0.f;
+    if (g_z) d += gz * lse * soft[q];  // (not 0 times an lse of inf)
+    z[q] = in ? d : 0.f;
   }
   if (there) store_lane<VPL, STEP>(dz + t * E, e0, E, vec, z);
 }

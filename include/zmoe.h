@@ -554,7 +554,8 @@ int zmoe_route_backward(const float* d_weight, const float* topk_prob, const int
  *   ph = p / sum_e p with p = sigmoid(z) or softmax(z);  n_s tokens, c_se choices of e in s, S' sequences with tokens
  *   losses[0] = 1/S' sum_s sum_e (E c_se / (k n_s)) (sum_t ph_te / n_s)       balance of each sequence
  *   losses[1] = 1/N sum_t logsumexp(z_t)^2                                      over all N tokens
- * (0 without tokens; a token whose p are all 0 adds nothing to the balance, one of -inf alone nothing to either).
+ * (0 without tokens; a token whose p are all 0 adds nothing to the balance, one of -inf alone nothing to either; a logit of
+ * +inf makes losses[1] inf and a softmax's balance NaN, a sigmoid's p is 1 there).
  * topk_idx [T, k]; ids outside [0, E) are not counted. seq_grad [S, E] f32 and inv_tokens [1] f32 are what the backward
  * takes. Sums in a fixed order.
  * ------------------------------------------------------------------------- */
