@@ -196,9 +196,14 @@ __device__ __forceinline__ float root(float v) {
   return small ? r * 0x1p-16f : r;
 }
 
-// The parameter after the step (r: the root of v): the quotient by v_rcp_f32, whose argument is a normal number.
+// The parameter after the step (r: the root of v): the quotient by v_rcp_f32, whose argument has to be a normal number. Without
+// an eps, or with one that is none (SCALED), it may not be: then a division, and no change where there is no moment.
+template <bool SCALED>
 __device__ __forceinline__ float stepped(float w, float m, float r, const float4& c, float eps) {
-  return fmaf(-(c.x * m), __builtin_amdgcn_rcpf(fmaf(r, c.y, eps)), fmaf(-c.z, w, w));
+  const float kept = fmaf(-c.z, w, w), d = fmaf(r, c.y, eps);
+  if constexpr (SCALED)
+    if (d < 0x1p-126f) return m == 0.f ? kept : kept - c.x * m / d;
+  return fmaf(-(c.x * m), __builtin_amdgcn_rcpf(d), kept);
 }
 
 // ------------------------------------------------------------------ elements
@@ -304,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const 
       const float gs = gr[e] * c.w;
       m[e] = fmaf(h.b1f, m[e], h.c1f * gs);
       v[e] = fmaf(h.b2f, v[e], h.c2f * (gs * gs));
-      w[e] = stepped(w[e], m[e], root<SCALED>(v[e]), c, h.eps);
+      w[e] = stepped<SCALED>(w[e], m[e], root<SCALED>(v[e]), c, h.eps);
     }
     store4(pm, i, left, vec, m);
     store4(pv, i, left, vec, v);
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(const Table tab, const
     top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
     top_v = max(top_v, __float_as_uint(v[e]));
     r[e] = root<SCALED>(v[e]);
-    w[e] = stepped(w[e], m[e], r[e], c, h.eps);
+    w[e] = stepped<SCALED>(w[e], m[e], r[e], c, h.eps);
   }
   store8(p, i, left, vec, w);
   const float Am = __uint_as_float(half_max_u32(top_m)), Av = __uint_as_float(half_max_u32(top_v));
@@ -566,6 +571,7 @@ extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype
   ZMOE_REQUIRE(count >= 0, ZMOE_ERR_SHAPE, "adamw: %d tensors", count);
   ZMOE_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, ZMOE_ERR_SHAPE, "adamw: betas %g, %g", beta1,
                beta2);
+  ZMOE_REQUIRE(eps >= 0.0, ZMOE_ERR_SHAPE, "adamw: eps %g", eps);
   if (count == 0) return ZMOE_OK;
   ZMOE_REQUIRE(tensors && workspace, ZMOE_ERR_NULL, "adamw: null pointer");
   ZMOE_REQUIRE(aligned16(workspace), ZMOE_ERR_ALIGN, "adamw: the workspace must be 16-byte aligned");

@@ -576,6 +576,7 @@ int zmoe_router_losses_backward(const void* logits, int logits_dtype, int64_t T,
  * leaves), in f32 with one rounding of the parameter:
  *   g' = clip g;  m' = b1 m + (1 - b1) g';  v' = b2 v + (1 - b2) g'^2
  *   p' = p - lr wd p - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps),   t = *step + 1, written back
+ * (eps >= 0; the last term is 0 where m' is 0 and the denominator is 0 too)
  * Arrays of n elements each, param and grad of `dtype`. state_bits 32: exp_avg and exp_avg_sq f32. 8: a byte an element
  * and a scale (f32, a block's largest magnitude A) for each 256 of them, [ceil(n / 256)]:
  *   m = sign(q) q^2 A / 127^2 (int8), v = q^4 A / 255^4 (uint8), rounded to f32; nearest codes, half-way ones up, v > 0

@@ -153,3 +153,13 @@ def test_torchs_states():
             with pytest.raises(ValueError, match="decay"):
                 ours.load_state_dict(adam.state_dict())
             assert not ours.state
+
+
+def test_what_the_step_refuses_of_eps():
+    """Without tensors, so that nothing could be launched."""
+    from zmoe import _lib
+
+    lib = _lib.load()
+    call = lambda eps: lib.zmoe_adamw(None, 0, 0, 32, None, 1e-3, 0.9, 0.999, eps, 0.0, None, None, 0, None)  # noqa: E731
+    assert call(0.0) == call(1e-40) == call(1e-8) == 0
+    assert call(-1e-8) == call(float("nan")) == 2
