@@ -18,6 +18,7 @@
 // Everything is one pass over memory: 28 bytes an element (f32, 32 bits), 16 (f32, 8 bits), 22 and 10 (bf16). Tensors'
 // pointers travel in the launches' arguments, so nothing is copied to the device and a graph keeps them. The norm is a
 // pass of its own (302 M f32 elements 240 us, 5.0 TB/s), for the clip has to be known before the first element moves.
+#include <cmath>
 #include <type_traits>
 
 #include "zmoe_route.h"  // row_max_u32
@@ -186,8 +187,8 @@ __device__ __forceinline__ uint32_t half_max_u32(uint32_t v) {
   return max((uint32_t)both[0], (uint32_t)both[1]);
 }
 
-// A square root to one rounding of f32. v_sqrt_f32 takes subnormals for 0, which does not count under an eps that is
-// some 2^-40 or more (SCALED false).
+// A square root to one rounding of f32. v_sqrt_f32 takes subnormals for 0 (SCALED false): their roots, below 2^-63, stand in
+// the denominator as at most 2^-63 / sqrt(1 - b2), 2^-25 of an eps of 2^-38 / sqrt(1 - b2) or more.
 template <bool SCALED>
 __device__ __forceinline__ float root(float v) {
   if constexpr (!SCALED) return __builtin_amdgcn_sqrtf(v);
@@ -618,7 +619,7 @@ extern "C" int zmoe_adamw(const zmoe_adamw_tensor* tensors, int count, int dtype
           hipLaunchKernelGGL((adamw_kernel<T, S>), grid, block, 0, as_stream(stream), tab, h, coef + first_of_launch);
       };
       auto typed = [&](auto type) {
-        if (eps >= 0x1p-40) go(type, std::false_type{});
+        if (eps * std::sqrt(1.0 - beta2) >= 0x1p-38) go(type, std::false_type{});  // (root)
         else go(type, std::true_type{});
       };
       if (dtype == ZMOE_DTYPE_BF16) typed(uint16_t{});

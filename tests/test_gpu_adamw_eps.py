@@ -1,5 +1,5 @@
 """zmoe.adamw.AdamW where the step's denominator is small: no eps, one that is no normal f32 number, elements without a
-grad.
+grad, second moments that are no normal numbers.
 
 Tolerances: tests/test_gpu_adamw.py's after one or two steps: 12 units of 2^-24 of the change for each step, 2 of the parameter,
 and half a step of its type each time it is kept."""
@@ -61,6 +61,23 @@ def test_squares_below_every_f32(eps, bits, hip_device):
     m = 0.1 * g.double()
     change = 0.1 * m / float(torch.tensor(eps))  # (eps is an f32 number in the step)
     # m is off by what an f32 near 2^-90 is, the quotient by two roundings and the product's
+    assert ((p.detach().double() + change).abs() <= 12 * 2.0 ** -24 * change.abs()).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("beta2", [0.95, 0.999, 1 - 1e-6])
+@pytest.mark.parametrize("eps", [2.0 ** -41, 2.0 ** -39, 2.0 ** -36, 2.0 ** -33, 1e-8])
+def test_second_moments_below_the_normal_numbers(eps, beta2, bits, hip_device):
+    """Roots of v' below 2^-126 count where eps does not drown them."""
+    p = torch.zeros(512, device=hip_device, requires_grad=True)
+    opt = made(p, eps=eps, betas=(0.9, beta2), state_bits=bits)
+    top = math.sqrt(2.0 ** -126 / (1 - beta2))
+    g = torch.linspace(0.9, 0.99, 512).to(hip_device) * top
+    p.grad = g
+    opt.step()
+    v = ((1 - beta2) * g.double().square())
+    assert (v < 2.0 ** -126).all()
+    change = 0.1 * (0.1 * g.double()) / (v.sqrt() / math.sqrt(1 - beta2) + eps)
     assert ((p.detach().double() + change).abs() <= 12 * 2.0 ** -24 * change.abs()).all()
 
 
