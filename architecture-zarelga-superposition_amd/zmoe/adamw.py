@@ -76,6 +76,9 @@ class AdamW(torch.optim.Optimizer):
             if len({id(p) for p in g["params"]}) != len(g["params"]):
                 raise ValueError("AdamW: a parameter is given twice")  # (one launch would write it from two places)
             for p in g["params"]:
+                if type(p).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
+                    raise ValueError(f"AdamW: a parameter of {type(p).__name__}, whose memory is not its own (sharded and other "
+                                     "wrapped tensors: give what they hold)")
                 if p.dtype not in (torch.float32, torch.bfloat16):
                     raise ValueError(f"AdamW: parameters must be float32 or bfloat16, got {p.dtype}")
                 if not _dense(p):

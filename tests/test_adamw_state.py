@@ -163,3 +163,37 @@ def test_what_the_step_refuses_of_eps():
     call = lambda eps: lib.zmoe_adamw(None, 0, 0, 32, None, 1e-3, 0.9, 0.999, eps, 0.0, None, None, 0, None)  # noqa: E731
     assert call(0.0) == call(1e-40) == call(1e-8) == 0
     assert call(-1e-8) == call(float("nan")) == 2
+
+
+class Wrapped(torch.Tensor):
+    """A tensor that holds another and has a dispatch of its own, as sharded and quantised ones do."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device,
+                                                   requires_grad=inner.requires_grad)
+
+    def __init__(self, inner):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        plain = lambda t: t.inner if isinstance(t, Wrapped) else t  # noqa: E731
+        return func(*map(plain, args), **{k: plain(v) for k, v in (kwargs or {}).items()})
+
+
+class Marked(torch.nn.Parameter):
+    """A parameter by another name, whose memory is its own."""
+
+
+def test_tensors_with_a_dispatch_of_their_own():
+    from zmoe.adamw import AdamW
+
+    p = torch.zeros(4, requires_grad=True)
+    w = Wrapped(torch.zeros(4)).requires_grad_(True)
+    with pytest.raises(ValueError, match="Wrapped"):
+        AdamW([p, w])
+    opt = AdamW([p, Marked(torch.zeros(3))])
+    with pytest.raises(ValueError, match="Wrapped"):
+        opt.add_param_group({"params": [w]})
+    assert len(opt.param_groups) == 1
