@@ -1150,14 +1150,15 @@ bool adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     table[i] = {raw(p), raw(g), raw(m), raw(v), eight ? ptr<float>(avg_scales[i]) : nullptr,
                 eight ? ptr<float>(sq_scales[i]) : nullptr, ptr<float>(t), p.numel()};
   }
+  // before the launch: refused (it throws) where tensors of inference mode would be changed outside of it
+  for (const Tensors* list : {&params, &exp_avgs, &exp_avg_sqs, &avg_scales, &sq_scales, &steps})
+    for (const Tensor& t : *list) t.unsafeGetTensorImpl()->bump_version();
   const c10::DeviceGuard guard(first.device());
   Tensor ws = workspace(16 * n, first);
   if (zmoe_adamw(table.data(), (int)n, code(first), (int)state_bits, lr_t ? ptr<const float>(*lr_t) : nullptr, lr, beta1,
                  beta2, eps, weight_decay, clip ? ptr<const float>(*clip) : nullptr, ptr<float>(ws), 16 * n,
                  stream_of(first)) != ZMOE_OK)
     return false;
-  for (const Tensors* list : {&params, &exp_avgs, &exp_avg_sqs, &avg_scales, &sq_scales, &steps})
-    for (const Tensor& t : *list) t.unsafeGetTensorImpl()->bump_version();
   return true;
 }
 

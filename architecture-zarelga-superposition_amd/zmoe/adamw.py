@@ -96,6 +96,7 @@ class AdamW(torch.optim.Optimizer):
         for g in self.param_groups:
             g.setdefault("state_bits", 32)
 
+    @torch.inference_mode(False)  # (a state made under inference mode could not be changed after it)
     def _state_of(self, p: torch.Tensor, bits: int) -> dict:
         st = self.state[p]
         if not st:
@@ -166,6 +167,8 @@ class AdamW(torch.optim.Optimizer):
                                              group["weight_decay"], clip):
                 continue
             self._in_order(lists)
+            if not torch.is_inference_mode_enabled() and any(t.is_inference() for some in (lists[0], *lists[2:]) for t in some):
+                raise RuntimeError("AdamW: a parameter or state made under inference mode is changed under it only")
             for p, m, v in zip(lists[0], lists[2], lists[3]):
                 if not _alike(m, p) or not _alike(v, p):
                     raise RuntimeError("AdamW: a parameter's shape or order in memory is not its moments'")
@@ -229,6 +232,7 @@ class AdamW(torch.optim.Optimizer):
             before.remove()
             after.remove()
 
+    @torch.inference_mode(False)
     def _state_made_of(self, state_dict) -> dict:
         """Each parameter's state from a state dict, or ValueError."""
         saved, new = state_dict["param_groups"], {}
