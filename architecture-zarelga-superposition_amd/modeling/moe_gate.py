@@ -66,6 +66,8 @@ class RouteForm(NamedTuple):
 
 
 class MoEGate(nn.Module):
+    form = None  # the reference's (also of gates pickled before there were others)
+
     def __init__(self, config):
         super().__init__()
         self.config = config
@@ -73,7 +75,7 @@ class MoEGate(nn.Module):
         self.n_routed_experts = config.n_routed_experts
         self.gating_dim = config.hidden_size
         form = RouteForm.of(config)
-        self.form = None if form == RouteForm() else form  # None: the reference's
+        self.form = None if form == RouteForm() else form
         self.weight = nn.Parameter(torch.empty((self.n_routed_experts, self.gating_dim)))
         self.register_buffer("expert_biases", torch.zeros(self.n_routed_experts))
         self.reset_parameters()
