@@ -235,7 +235,8 @@ class MoELayer(nn.Module):
 
         ``router_losses``: (out, topk_idx, (balance, z)) with the losses of ``zmoe.functional.router_losses`` on this call's
         router, over the sequences ``cu_seqlens`` of the tokens that the layer routes (the unpadded ones where
-        ``unpad_indices`` are given); None: each row of the batch is one, with ``unpad_indices`` all tokens.
+        ``unpad_indices`` are given); None: each row of the batch is one, with ``unpad_indices`` all tokens. (``cu_seqlens`` is
+        read for the losses alone: without them it changes nothing.)
 
         ``norm`` (a ZeroCenteredRMSNorm, optional): the layer's input is
         ``norm(hidden_states)``, as the transformer block computes it before calling the
@@ -302,8 +303,8 @@ class MoELayer(nn.Module):
 
 class Fp8MoELayer(Fp8Module):
     """``MoELayer`` for serving: the routed and the shared experts' weights in e4m3 with a power-of-two scale for each
-    128 x 128 block (``Fp8GLUMLP``, ``Fp8ExpertMLP``); the gate, routing and combine as in the layer. Same
-    arguments and results as ``MoELayer.forward``; no gradients."""
+    128 x 128 block (``Fp8GLUMLP``, ``Fp8ExpertMLP``); the gate, routing and combine as in the layer. Arguments and
+    results as ``MoELayer.forward``'s, but for the router's losses, which serving has no use for; no gradients."""
 
     def __init__(self, layer: MoELayer):
         super().__init__()
