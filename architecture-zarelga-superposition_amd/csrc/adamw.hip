@@ -280,7 +280,7 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t i, int6
   return c;
 }
 
-// Moments in 32 bits: memory alone (302 M f32 elements 1544-1557 us, 5.4 TB/s); four consecutive elements a lane, a wave's
+// Moments in 32 bits: memory alone (302 M f32 elements 1544-1564 us, 5.4 TB/s, as many of bf16 1247, 5.3 TB/s); four consecutive elements a lane, a wave's
 // two blocks read before the first is written.
 template <typename T, bool SCALED>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab, const Hyper h,
@@ -353,7 +353,7 @@ struct Raw8 {
 
 // Moments in 8 bits: a wave has two blocks at once, eight consecutive elements a lane, so that what is done once for a
 // block (the largest magnitudes over its lanes, the scales' quotients) is shared by twice as many. The arithmetic is the
-// bound as much as memory: 520 vector instructions a lane, 42 of them roots and reciprocals at a quarter of the rate
+// bound as much as memory: 503 vector instructions a wave (counted), 42 of them roots and reciprocals at a quarter of the rate
 // (doubles run at f32's), 50 us of 61 for 24.5 M bf16 elements (4.0 TB/s); 302 M f32 elements 900 us, 5.4 TB/s. One pair a
 // wave: with two, the second's reads under way while the first is worked on, 28 more registers cost more than that
 // hides (repeated on the same tensors, 24.5 M bf16 elements 51 and 56 us, 100 M f32 295 and 299).

@@ -12,10 +12,11 @@
 // rounding for one value in 2^28. Without a bias the experts' order is their logits' order.
 //
 // Few bytes (8192 tokens of 256 experts 5 MB, 1 us at the copy's rate) and many instructions: a token's experts lie over a
-// row of lanes, so that a wave has several tokens; of its 2100 instructions for four of them 570 are the sigmoids in
-// double, 1030 the k = 8 rounds of maximum, first holder and mark, 200 the groups. 8192 tokens of 256 experts in 8 groups
-// 9.6 us in a graph's replays (11.1 traced; two waves a SIMD), 32768 of 128 by softmax 12.9 (14.8), 32749 of 160 in f32 23
-// traced; their backwards, a pass over the [T, E] grad, 5.4 and 11.6 (2.3 and 3.9 TB/s).
+// row of lanes, so that a wave has several tokens; of its 1650 vector and 600 scalar instructions (counted) for four of them 570
+// are the sigmoids in double, 1030 the k = 8 rounds of maximum, first holder and mark, 200 the groups (by the listing). 8192
+// tokens of 256 experts in 8 groups 9.6 us in a graph's replays (11.5 traced; two waves a SIMD), 32768 of 128 by softmax 12.9
+// (14.6), 32749 of 160 in f32 23 traced; the softmaxes' backwards, a pass over the [T, E] grad, 5.4 and 12 traced (4.2 and 11.5 in
+// replays, 3.0 and 3.9 TB/s). A sigmoid's, with the logits of those taken, 5.3 and 7.6 in replays (4.8 and 6.4 from p alone).
 #include "zmoe_route.h"
 
 namespace zmoe {

@@ -11,8 +11,16 @@
 // i + s: walking along the tokens either number grows by one), which a second launch adds up in a fixed order, a
 // workgroup for each sequence and 32 experts. The gradient reads the logits again. Both are short: what bounds them is
 // the latency of a few dependent reads in each of the launches, and the exponentials (32749 tokens of 256 experts in 37
-// sequences, f32: 14.8 us, 2.4 TB/s, then 10.4 for the sums and 18.2 for the gradient, 3.7 TB/s; 32768 of 128, bf16, one
-// sequence: 6.7, 7.4 and 7.6; 517 of 32: 6.2, 6.8 and 4.1).
+// sequences, f32: 15.3 us, 2.4 TB/s, then 10.8 for the sums and 18.8 for the gradient, 3.6 TB/s; 32768 of 128, bf16, one
+// sequence: 6.8, 7.3 and 7.7; 517 of 32: 6.2, 6.7 and 4.3).
+//
+// A workgroup takes the sequences of its tile one after the other, empty ones among them (two dependent reads, 0.4 us, each), and
+// the second launch has a workgroup for each sequence, empty or not, and 32 experts. So the forward grows with short, empty or very long
+// sequences (in a graph's replays, 128 experts, bf16): 32768 tokens in 37 sequences 15.6 us; with the last border repeated up to
+// S = 4096 286 where it is a tile's border or T, 1755 inside a tile; in 4096 sequences of 8 tokens 313, in 32768 of one 2460; 2^20
+// tokens in one sequence 137 (of 32 experts 112). The backward skips empty sequences 64 at a time from its wave's first
+// token on (5.6 to 12 us for those of 32768 tokens), and walks one by one from there: 605 us where a wave has rows past T and
+// T's border is repeated up to S = 4096.
 #include <type_traits>
 
 #include "zmoe_route.h"

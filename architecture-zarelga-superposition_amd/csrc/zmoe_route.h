@@ -92,9 +92,9 @@ __device__ __forceinline__ float row_sum_f32(float v) {
   return v;
 }
 
-// e^x in double, x below 709 (e^-745 and less are 0; NaN stays): x = n ln 2 + r with |r| <= ln 2 / 2, ln 2 as a sum of two numbers
-// of which the first has so few bits that n times it is exact, and Taylor's polynomial of degree 12, whose first missing
-// term is below 2^-52.
+// e^x in double, x below 709 (e^-745 and less are 0; NaN stays): x = n ln 2 + r with |r| <= ln 2 / 2 by the reduction of Cody and
+// Waite (ln 2 as a sum of two numbers, of which the first has so few bits that n times it is exact), and Taylor's polynomial
+// of degree 12, whose first missing term is below 2^-52.
 __device__ __forceinline__ double exp_f64(double x) {
   x = x < -760.0 ? -760.0 : x;
   const double n = rint(x * 1.4426950408889634);
